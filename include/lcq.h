@@ -461,6 +461,66 @@ int lcq_group_dots(const void* x, const void* w, int dtype, int64_t R, int64_t K
 int lcq_clamp_groups(const void* w, int dtype, int64_t R, int64_t K, int group_size, const void* lo, const void* hi,
                      void* out, void* stream);
 
+/* ---- running a w8a8 model ------------------------------------------------- */
+
+/* Int8 codes of tokens (rows), in fp32 arithmetic whatever the row type: IntegerQuantizer's per_token quantization
+ * (quant.py:544-558, 698-716) of fp32 rows, codes stored as int8 (the unsigned codes of an asymmetric quantizer less 128).
+ *  x       [T, K] of `dtype`, rows `ldx` elements apart;  K <= 65536
+ *  scale   NULL: s = max(max|x|, 1e-5) / 127 per row, or with `asym` s = max(max x - min x, 1e-5) / 255 and
+ *          z = clamp(-128 - rint(min x / s), -128, 127); else one fp32 scale for all rows (static activations; not `asym`)
+ *  codes   [T, K] int8: clamp(rint(x / s) + z, -128, 127);  scales [T] fp32, zeros [T] int32 (`asym`): output
+ * A row with an infinity or a NaN gets a scale that is not finite, and with it every product of that row. */
+int lcq_quant_tokens(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, int asym, const float* scale, int8_t* codes,
+                     float* scales, int32_t* zeros, void* stream);
+
+/* y[m, n] = as[m] * ws[n] * (sum_k a[m, k] w[n, k] - az[m] * sum_k w[n, k]) + bias[n]: the product of int8 codes with a scale for
+ * each token and each channel.  The sums are exact integers; the factors and the bias are applied in fp32, y is rounded once.
+ *  a       [M, K] int8, as [M] fp32 (or [1] with a_scalar), az [M] int32 within +-128 or NULL
+ *  w       [N, K] int8, ws [N] of ws_dtype (or [1] with w_scalar), bias [N] of bias_dtype or NULL;  K <= 65536
+ *  y       [M, N] of `dtype`
+ *  workspace of lcq_int8_matmul_workspace_bytes(M, N, K) (0: none), 16-byte aligned. */
+int64_t lcq_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int lcq_int8_matmul(const int8_t* a, const float* as, int a_scalar, const int32_t* az, const int8_t* w, const void* ws, int ws_dtype,
+                    int w_scalar, const void* bias, int bias_dtype, int64_t M, int64_t N, int64_t K, void* y, int dtype,
+                    void* workspace, void* stream);
+
+/* The end of one block and the start of the next, in fp32 between loads and stores:
+ *    b = x or norm(x; post_weight, post_bias);   h = residual + scale * gate * b;   out = norm(h; weight, bias)
+ *    norm(v; w, b) = v / sqrt(mean v^2 + eps) * (w + weight_offset) + b   (LCQ_NORM_LAYER: of v - mean v)
+ *  x        [T, K] of `dtype`, rows ldx elements apart;  K <= 65536
+ *  residual [T, K] of `dtype` (LCQ_NORM_RESIDUAL_F32: fp32), rows ldr apart, or NULL (0)
+ *  gate     [T, K] of `dtype`, rows ldg apart (0: one row for all tokens), or NULL (1)
+ *  post_weight, post_bias, weight, bias  [K] of `dtype` (fp32 with their flag) or NULL; no post_weight: no norm of x
+ *  h        [T, K] of the residual's type: output (may be `residual`)
+ *  out      [T, K] of `dtype` (LCQ_NORM_OUT_F32: fp32) or NULL;  codes [T, K] int8 with scales [T] (and zeros [T] with LCQ_NORM_ASYM)
+ *           or NULL: lcq_quant_tokens of the unrounded norm.  At least one of the two. */
+#define LCQ_NORM_LAYER 1
+#define LCQ_NORM_POST_WEIGHT_F32 2
+#define LCQ_NORM_POST_BIAS_F32 4
+#define LCQ_NORM_WEIGHT_F32 8
+#define LCQ_NORM_BIAS_F32 16
+#define LCQ_NORM_RESIDUAL_F32 32
+#define LCQ_NORM_OUT_F32 64
+#define LCQ_NORM_ASYM 128
+int lcq_residual_norm(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, const void* residual, int64_t ldr, const void* gate,
+                      int64_t ldg, const void* post_weight, const void* post_bias, const void* weight, const void* bias, float scale,
+                      float eps, float weight_offset, int flags, void* h, void* out, int8_t* codes, float* scales, int32_t* zeros,
+                      void* stream);
+
+/* Log probabilities of given tokens, entropy and best alternatives, from logits:
+ *    l = log sum_v exp(x_v);   logprobs = x_token - l;   entropy = l - sum_v p_v x_v;   top: the k largest x_v, as x_v - l
+ *  logits   [T, V] of `dtype`, rows ldx elements apart;  V < 2^31
+ *  tokens   [T, m] int64 or NULL; logprobs [T, m] fp32.  A token equal to `ignore` gives 0, another one outside [0, V) NaN
+ *  entropy  [T] fp32 or NULL
+ *  top_logprobs [T, k] fp32, top_tokens [T, k] int64, 0 <= k <= min(64, V): largest first, equal logits by the lowest index, a NaN
+ *           above everything
+ * Masked logits (-inf) have probability 0; a row of nothing else, or one with a NaN or +inf, gives NaN as log_softmax does.
+ *  workspace of lcq_token_logprobs_workspace_bytes(T, V, k) (0: none), 16-byte aligned. */
+int64_t lcq_token_logprobs_workspace_bytes(int64_t T, int64_t V, int k);
+int lcq_token_logprobs(const void* logits, int dtype, int64_t T, int64_t V, int64_t ldx, const int64_t* tokens, int64_t m,
+                       int64_t ignore, float* logprobs, float* entropy, int k, float* top_logprobs, int64_t* top_tokens,
+                       void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,31 +11,12 @@
 // do); LCQ_FLAG_TIE_AWAY nudges exact ties one ulp outwards first (the add-half-then-truncate model of
 // float_quantize).
 #include "rowquant.h"
+#include "divisor.h"
 
 namespace {
 using namespace lcq;
 
 constexpr int BS = 128;
-
-// x / s for a divisor that many elements share, correctly rounded without the division sequence: with y = RN(1/s) the product
-// q0 = x y is within 2 ulp, one residual step makes it faithful and a second one exact (Markstein, IBM J. R&D 34(1), 1990;
-// the residuals are exact).  Five full-rate instructions; a guarded product needs as many to find out whether it may stay, and
-// values below the minimum normal, where the grid's midpoints are not a bit pattern, went through the division sequence.
-// Scales outside 2^-60 .. 2^60 (an infinite or NaN block, a block of subnormals) divide.
-struct Divisor {
-  float s, y;
-  bool fast;
-  __device__ __forceinline__ explicit Divisor(float s_) : s(s_), fast(s_ > 8.6736174e-19f && s_ < 1.1529215e18f) {
-    const float y0 = __builtin_amdgcn_rcpf(s);
-    y = __builtin_fmaf(__builtin_fmaf(-s, y0, 1.0f), y0, y0);
-  }
-  __device__ __forceinline__ float quotient(float x) const {
-    if (__builtin_expect(!fast, 0)) return x / s;
-    float q = x * y;                                         // (s q - x taken off, not x - s q added: that way -0 / s stays -0)
-    q = __builtin_fmaf(-__builtin_fmaf(s, q, -x), y, q);
-    return __builtin_fmaf(-__builtin_fmaf(s, q, -x), y, q);
-  }
-};
 
 // value handed to the float8 convert.  model = false: x / s itself (Triton / torch cast: one rounding, to
 // nearest even, done by the convert).  model = true: the FloatQuantizer route, "x / s + 0" rounded by the

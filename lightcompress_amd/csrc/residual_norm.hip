@@ -1,0 +1,289 @@
+// The end of one block and the start of the next, one pass over a token's row:
+//
+//   b = x                 or  norm(x; post_weight, post_bias)
+//   h = residual + scale * (gate * b)                              -> the residual stream
+//   y = norm(h; weight, bias)                                      -> the next block's input, as values or as int8 codes
+//   rms:   norm(v) = v / sqrt(mean v^2 + eps) * (w + offset) + bias
+//   layer: norm(v) = (v - mean) / sqrt(mean (v - mean)^2 + eps) * (w + offset) + bias
+//
+// and the int8 codes of a token by themselves (lcq_quant_tokens: the same rows without norm and residual):
+//
+//   symmetric   s = max(max |y|, 1e-5) / 127         q = clamp(rint(y / s), -128, 127)
+//   asymmetric  s = max(max y - min y, 1e-5) / 255   z = clamp(-128 - rint(min y / s), -128, 127)
+//               q = clamp(rint(y / s) + z, -128, 127)
+//   given scale q = clamp(rint(y / s), -128, 127)
+//
+// Everything between the loads and the stores is in 32 bits: y is taken from h before h is rounded to the stream's type, codes
+// from y before any rounding.  The quantizer arithmetic is IntegerQuantizer's (quant.py:544-558, 698-716) on fp32 rows with
+// granularity per_token, codes moved to int8 (its unsigned codes less 128).
+#include "rowquant.h"
+#include "divisor.h"
+
+namespace {
+using namespace lcq;
+
+struct NormArgs {
+  const void *x, *residual, *gate, *post_weight, *post_bias, *weight, *bias;
+  const float* scale_in;
+  void *h, *out;
+  int8_t* codes;
+  float* scales;
+  int32_t* zeros;
+  int64_t T, ldx, ldr, ldg;
+  int K, flags;
+  float scale, eps, offset;
+};
+
+constexpr int NORM = 1 << 20;                       // (internal: y is a norm of h; without it y = h)
+
+// V consecutive elements at index i of a row of type BF, or of fp32 where f32 says so
+template <int BF, int V>
+__device__ __forceinline__ void load_v(const void* p, int64_t i, bool f32, float* v) {
+  if constexpr (V == 1) {
+    v[0] = f32 ? ((const float*)p)[i] : load_scalar<BF>(p, i);
+  } else {
+    if (BF == ROW_F32 || f32) {
+      unpack<ROW_F32>(*(const u32x4*)((const float*)p + i), v);
+      unpack<ROW_F32>(*(const u32x4*)((const float*)p + i + 4), v + 4);
+    } else {
+      unpack<BF>(*(const u32x4*)((const uint16_t*)p + i), v);
+    }
+  }
+}
+template <int BF, int V>
+__device__ __forceinline__ void store_v(void* p, int64_t i, bool f32, const float* v) {
+  if constexpr (V == 1) {
+    if (f32) ((float*)p)[i] = v[0];
+    else store_scalar<BF>(p, i, rnd<BF>(v[0]));
+  } else {
+    if (BF == ROW_F32 || f32) {
+      *(u32x4*)((float*)p + i) = pack<ROW_F32>(v);
+      *(u32x4*)((float*)p + i + 4) = pack<ROW_F32>(v + 4);
+    } else {
+      *(u32x4*)((uint16_t*)p + i) = pack_rne<BF>(v);
+    }
+  }
+}
+
+// TEAM lanes share a row: 64 (a wave, four rows per workgroup) or the whole workgroup.  A sum or a maximum over the row in a fixed order.
+template <int TEAM>
+struct Row {
+  float* sm;                                        // one float per wave
+  template <int OP>                                 // 0 sum, 1 maximum, 2 minimum (both NaN where an element is)
+  __device__ __forceinline__ float reduce(float v) const {
+    if constexpr (OP == 0) v = team_sum<64>(v);
+    else v = team_reduce<64, OP == 1>(v);
+    if constexpr (TEAM > 64) {
+      __syncthreads();
+      if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = v;
+      __syncthreads();
+      v = sm[0];
+      #pragma unroll
+      for (int w = 1; w < TEAM / 64; ++w) v = OP == 0 ? v + sm[w] : OP == 1 ? nan_max(v, sm[w]) : nan_min(v, sm[w]);
+    }
+    return v;
+  }
+};
+
+// One row per TEAM lanes, CH pieces of V elements per lane in registers; V = 8 where every row starts on 16 bytes, 1 else.
+template <int BF, int V, int TEAM, int CH>
+__global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void residual_norm_kernel(NormArgs a) {
+  __shared__ float sm[TEAM / 64];
+  const Row<TEAM> row_{sm};
+  const int t = threadIdx.x % TEAM;
+  const int64_t r = TEAM == 64 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x;
+  if (r >= a.T) return;                             // (whole waves, and no barriers where TEAM is a wave)
+  const int K = a.K, flags = a.flags;
+  const float rK = 1.0f / (float)K;
+  float v[CH][V];
+  #pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int i = (t + c * TEAM) * V;
+    #pragma unroll
+    for (int j = 0; j < V; ++j) v[c][j] = 0.0f;
+    if (i < K) load_v<BF, V>(a.x, r * a.ldx + i, false, v[c]);
+  }
+  const auto each = [&](auto&& f) {
+    #pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int i = (t + c * TEAM) * V;
+      if (i < K) f(i, v[c]);
+    }
+  };
+  const auto norm = [&](const void* w, bool w32, const void* b, bool b32) {
+    float sum = 0.0f, mean = 0.0f;
+    if (flags & LCQ_NORM_LAYER) {
+      each([&](int, float* e) {
+        #pragma unroll
+        for (int j = 0; j < V; ++j) sum += e[j];
+      });
+      mean = row_.template reduce<0>(sum) * rK;
+      sum = 0.0f;
+    }
+    each([&](int, float* e) {
+      #pragma unroll
+      for (int j = 0; j < V; ++j) { e[j] -= mean; sum = __builtin_fmaf(e[j], e[j], sum); }
+    });
+    const float inv = 1.0f / sqrtf(row_.template reduce<0>(sum) * rK + a.eps);
+    each([&](int i, float* e) {
+      float f[V];
+      if (w) {
+        load_v<BF, V>(w, i, w32, f);
+        #pragma unroll
+        for (int j = 0; j < V; ++j) e[j] = e[j] * inv * (f[j] + a.offset);
+      } else {
+        #pragma unroll
+        for (int j = 0; j < V; ++j) e[j] *= inv;
+      }
+      if (b) {
+        load_v<BF, V>(b, i, b32, f);
+        #pragma unroll
+        for (int j = 0; j < V; ++j) e[j] += f[j];
+      }
+    });
+  };
+
+  if (a.post_weight) norm(a.post_weight, flags & LCQ_NORM_POST_WEIGHT_F32, a.post_bias, flags & LCQ_NORM_POST_BIAS_F32);
+  if (a.gate) {
+    each([&](int i, float* e) {
+      float f[V];
+      load_v<BF, V>(a.gate, r * a.ldg + i, false, f);
+      #pragma unroll
+      for (int j = 0; j < V; ++j) e[j] *= f[j];
+    });
+  }
+  if (a.residual) {
+    each([&](int i, float* e) {
+      float f[V];
+      load_v<BF, V>(a.residual, r * a.ldr + i, flags & LCQ_NORM_RESIDUAL_F32, f);
+      #pragma unroll
+      for (int j = 0; j < V; ++j) e[j] = __builtin_fmaf(a.scale, e[j], f[j]);
+    });
+  } else if (flags & NORM) {
+    each([&](int, float* e) {
+      #pragma unroll
+      for (int j = 0; j < V; ++j) e[j] *= a.scale;
+    });
+  }
+  if (a.h) each([&](int i, float* e) { store_v<BF, V>(a.h, r * K + i, flags & LCQ_NORM_RESIDUAL_F32, e); });
+  if (flags & NORM) norm(a.weight, flags & LCQ_NORM_WEIGHT_F32, a.bias, flags & LCQ_NORM_BIAS_F32);
+  if (a.out) each([&](int i, float* e) { store_v<BF, V>(a.out, r * K + i, flags & LCQ_NORM_OUT_F32, e); });
+  if (!a.codes) return;
+
+  float s, z = 0.0f;
+  bool bounded = true;                              // |y / s| stays far from the largest fp32 number
+  if (a.scale_in) {
+    bounded = false;
+    s = a.scale_in[0];
+  } else if (flags & LCQ_NORM_ASYM) {
+    const float inf = __builtin_inff();
+    float hi = -inf, lo = inf;
+    each([&](int, float* e) {
+      #pragma unroll
+      for (int j = 0; j < V; ++j) { hi = nan_max(hi, e[j]); lo = nan_min(lo, e[j]); }
+    });
+    hi = row_.template reduce<1>(hi);
+    lo = row_.template reduce<2>(lo);
+    s = nan_max(hi - lo, 1e-5f) / 255.0f;
+    z = fminf(fmaxf(-128.0f - rintf(lo / s), -128.0f), 127.0f);
+    bounded = fmaxf(fabsf(hi), fabsf(lo)) < 1e30f;  // (s >= 1e-5 / 255: a narrow range far from zero)
+  } else {
+    float m = 0.0f;
+    each([&](int, float* e) {
+      #pragma unroll
+      for (int j = 0; j < V; ++j) m = nan_max(m, fabsf(e[j]));
+    });
+    m = row_.template reduce<1>(m);
+    s = nan_max(m, 1e-5f) / 127.0f;
+  }
+  Divisor d(s);
+  d.fast = d.fast && bounded;
+  each([&](int i, float* e) {
+    int q[V];
+    #pragma unroll
+    for (int j = 0; j < V; ++j) q[j] = (int)fminf(fmaxf(rintf(d.quotient(e[j])) + z, -128.0f), 127.0f);
+    if constexpr (V == 1) {
+      a.codes[r * K + i] = (int8_t)q[0];
+    } else {
+      u32x2 w;
+      #pragma unroll
+      for (int p = 0; p < 2; ++p)
+        w[p] = (uint32_t)(q[4 * p] & 255) | (uint32_t)(q[4 * p + 1] & 255) << 8 | (uint32_t)(q[4 * p + 2] & 255) << 16 | (uint32_t)q[4 * p + 3] << 24;
+      *(u32x2*)(a.codes + r * K + i) = w;
+    }
+  });
+  if (t == 0 && a.scales) a.scales[r] = s;
+  if (t == 0 && a.zeros) a.zeros[r] = (int)z;
+}
+
+template <int BF, int V, int TEAM, int CH>
+void launch(const NormArgs& a, hipStream_t st) {
+  constexpr int rows = TEAM == 64 ? 4 : 1;
+  residual_norm_kernel<BF, V, TEAM, V == 1 ? CH * 8 : CH><<<dim3((unsigned)((a.T + rows - 1) / rows)), dim3(TEAM == 64 ? 256 : TEAM), 0, st>>>(a);
+}
+template <int BF, int V>
+void launch_rows(const NormArgs& a, hipStream_t st) {
+  if (a.K <= 512) launch<BF, V, 64, 1>(a, st);
+  else if (a.K <= 1024) launch<BF, V, 64, 2>(a, st);
+  else if (a.K <= 2048) launch<BF, V, 256, 1>(a, st);
+  else if (a.K <= 4096) launch<BF, V, 256, 2>(a, st);
+  else if (a.K <= 8192) launch<BF, V, 256, 4>(a, st);
+  else if (a.K <= 16384) launch<BF, V, 1024, 2>(a, st);
+  else if (a.K <= 32768) launch<BF, V, 1024, 4>(a, st);
+  else launch<BF, V, 1024, 8>(a, st);
+}
+
+constexpr int64_t MOST_COLS = 65536;                // a row stays in the registers of 1024 lanes
+
+bool aligned(const void* p) { return (uintptr_t)p % 16 == 0; }
+
+int run(const NormArgs& a, int dtype, hipStream_t st) {
+  const int f = a.flags;
+  const auto stride = [&](int64_t ld, bool f32) { return ld * (f32 || dtype == LCQ_F32 ? 4 : 2) % 16 == 0; };
+  const bool wide = a.K % 8 == 0 && aligned(a.x) && stride(a.ldx, false) && aligned(a.residual) && stride(a.ldr, f & LCQ_NORM_RESIDUAL_F32) &&
+                    aligned(a.gate) && stride(a.ldg, false) && aligned(a.post_weight) && aligned(a.post_bias) && aligned(a.weight) &&
+                    aligned(a.bias) && aligned(a.h) && aligned(a.out) && (uintptr_t)a.codes % 8 == 0;
+  if (dtype == LCQ_BF16) { if (wide) launch_rows<ROW_BF16, 8>(a, st); else launch_rows<ROW_BF16, 1>(a, st); }
+  else if (dtype == LCQ_F16) { if (wide) launch_rows<ROW_F16, 8>(a, st); else launch_rows<ROW_F16, 1>(a, st); }
+  else { if (wide) launch_rows<ROW_F32, 8>(a, st); else launch_rows<ROW_F32, 1>(a, st); }
+  LCQ_CHECK_LAUNCH();
+  return LCQ_OK;
+}
+
+bool known_dtype(int dtype) { return dtype == LCQ_F32 || dtype == LCQ_BF16 || dtype == LCQ_F16; }
+
+}  // namespace
+
+extern "C" {
+
+int lcq_residual_norm(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, const void* residual, int64_t ldr, const void* gate,
+                      int64_t ldg, const void* post_weight, const void* post_bias, const void* weight, const void* bias, float scale,
+                      float eps, float weight_offset, int flags, void* h, void* out, int8_t* codes, float* scales, int32_t* zeros,
+                      void* stream) {
+  if (!x || !h || T <= 0 || K <= 0 || T > 0x7fffffff || (!out && !codes) || (codes && !scales)) return LCQ_EINVAL;
+  if ((post_bias && !post_weight) || ldx < 0 || ldr < 0 || ldg < 0) return LCQ_EINVAL;
+  if ((flags & LCQ_NORM_ASYM) && codes && !zeros) return LCQ_EINVAL;
+  if (flags & ~255) return LCQ_EINVAL;
+  if (!known_dtype(dtype)) return LCQ_EDTYPE;
+  if (K > MOST_COLS) return LCQ_ESIZE;
+  NormArgs a = {};
+  a.x = x; a.residual = residual; a.gate = gate; a.post_weight = post_weight; a.post_bias = post_bias; a.weight = weight; a.bias = bias;
+  a.h = h; a.out = out; a.codes = codes; a.scales = scales; a.zeros = zeros;
+  a.T = T; a.ldx = ldx; a.ldr = ldr; a.ldg = ldg; a.K = (int)K; a.flags = flags | NORM;
+  a.scale = scale; a.eps = eps; a.offset = weight_offset;
+  return run(a, dtype, (hipStream_t)stream);
+}
+
+int lcq_quant_tokens(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, int asym, const float* scale, int8_t* codes,
+                     float* scales, int32_t* zeros, void* stream) {
+  if (!x || !codes || T <= 0 || K <= 0 || T > 0x7fffffff || ldx < 0 || (!scale && !scales)) return LCQ_EINVAL;
+  if (asym && (scale || !zeros)) return LCQ_EINVAL;
+  if (!known_dtype(dtype)) return LCQ_EDTYPE;
+  if (K > MOST_COLS) return LCQ_ESIZE;
+  NormArgs a = {};
+  a.x = x; a.scale_in = scale; a.codes = codes; a.scales = scale ? nullptr : scales; a.zeros = asym ? zeros : nullptr;
+  a.T = T; a.ldx = ldx; a.K = (int)K; a.flags = asym ? LCQ_NORM_ASYM : 0; a.scale = 1.0f;
+  return run(a, dtype, (hipStream_t)stream);
+}
+
+}  // extern "C"

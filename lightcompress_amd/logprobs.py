@@ -1,0 +1,62 @@
+"""Log probabilities of given tokens, with entropy and best alternatives, from a model's logits in one pass: what the
+reference's perplexity (llmc/eval/eval_ppl.py) and token-consistency (llmc/eval/eval_token_consist.py) evaluations
+take from a whole log-softmax and an argmax.  Forward only: nothing here records a gradient."""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib as L
+from .w8a8 import _on, _rows
+
+MOST_TOP = 64
+
+
+class TokenLogprobs(NamedTuple):
+    logprobs: Optional[torch.Tensor]          # fp32, like tokens
+    entropy: torch.Tensor                     # fp32 [...], in nats
+    top_logprobs: torch.Tensor                # fp32 [..., top], largest first
+    top_tokens: torch.Tensor                  # int64 [..., top]
+
+
+@torch.no_grad()
+def token_logprobs(logits, tokens=None, top=0, ignore_index=-100):
+    """logits [..., V] (fp32, bf16, fp16); tokens int64 [...] or [..., m], the ids whose log probability is asked for.
+
+    A token equal to `ignore_index` gives 0, any other id outside the vocabulary NaN.  Masked logits (-inf) have
+    probability 0 and log probability -inf; a row that is masked everywhere, or holds a NaN or +inf, gives NaN, as
+    log_softmax does.  The `top` (at most 64) alternatives come largest first, equal logits by the lowest id, a NaN first."""
+    if logits.dim() == 0 or logits.shape[-1] == 0:
+        raise ValueError(f'logits need a vocabulary, got shape {tuple(logits.shape)}')
+    V, lead = logits.shape[-1], logits.shape[:-1]
+    code = L.dtype_code(logits.dtype)
+    if not 0 <= top <= min(MOST_TOP, V):
+        raise ValueError(f'top {top}: between 0 and {min(MOST_TOP, V)}')
+    m = 0
+    if tokens is not None:
+        if tokens.dtype != torch.int64:
+            raise L.LcqError(f'tokens are int64, got {tokens.dtype}')
+        if tokens.shape == lead:
+            m = 1
+        elif tokens.dim() == logits.dim() and tokens.shape[:-1] == lead:
+            m = tokens.shape[-1]
+        else:
+            raise ValueError(f'tokens {tuple(tokens.shape)} next to logits {tuple(logits.shape)}')
+    with _on(logits, tokens=tokens):
+        dev = logits.device
+        rows, T, ld = _rows(logits, V)
+        ids = None if tokens is None else tokens.contiguous()
+        logprobs = None if tokens is None else torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+        entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+        top_logprobs = torch.empty((*lead, top), dtype=torch.float32, device=dev)
+        top_tokens = torch.empty((*lead, top), dtype=torch.int64, device=dev)
+        if T:
+            lib = L.lib()
+            size = lib.lcq_token_logprobs_workspace_bytes(T, V, top)
+            ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+            L.check(lib.lcq_token_logprobs(rows.data_ptr(), code, T, V, ld, ids.data_ptr() if m else None, m, ignore_index,
+                                           logprobs.data_ptr() if m else None, entropy.data_ptr(), top,
+                                           top_logprobs.data_ptr() if top else None, top_tokens.data_ptr() if top else None,
+                                           L.ptr(ws), L.stream()), 'lcq_token_logprobs')
+    return TokenLogprobs(logprobs, entropy, top_logprobs, top_tokens)

@@ -19,6 +19,7 @@ import torch.nn.modules.module as _module
 from . import _lib as L
 from .quant import IntegerQuantizer, weight_cast_to_bf16
 from .rtn import RTN
+from .w8a8 import QuantizedTokens, int8_linear, int8_matmul
 
 _CODE = {torch.int32: L.CODE_I32, torch.int8: L.CODE_I8, torch.uint8: L.CODE_U8}
 # torch's register_buffer itself (None where it was already replaced by another when this module was imported)
@@ -193,7 +194,30 @@ class _RealQuantLinear(torch.nn.Module):
         return f'{type(self).__name__}(' + ', '.join(parts) + ')'
 
 
+def _act_form(quant_config):
+    """How a w8a8 container's activations are quantized: 'symmetric' / 'asymmetric' (a scale per token) or 'static' (one given
+    scale); None where the configuration is not int8 codes on both sides with scales per token and channel."""
+    w, a = quant_config['weight'], quant_config.get('act')
+    if a is None or w.get('need_pack', False):
+        return None
+    for cfg in (w, a):
+        if cfg.get('quant_type', 'int-quant') != 'int-quant' or cfg['bit'] != 8:
+            return None
+    if not w['symmetric'] or w['granularity'] not in ('per_channel', 'per_tensor') or a.get('int_range') is not None:
+        return None
+    if a.get('static', False):
+        return 'static' if a['symmetric'] and a['granularity'] == 'per_tensor' else None
+    if a['granularity'] != 'per_token' or a.get('calib_algo', 'minmax') != 'minmax' or not a.get('round_zp', True):
+        return None
+    return 'symmetric' if a['symmetric'] else 'asymmetric'
+
+
 class VllmRealQuantLinear(_RealQuantLinear):
+    """The container, and for w8a8 (int8 weight with a scale per channel or one for all, symmetric; int8 activations per token,
+    or static per tensor and symmetric) its forward pass."""
+
+    act_form = None
+
     def __init__(self, weight, bias, scales, input_scale, need_pack, scales_name):
         super().__init__()
         self._buffer('weight_packed' if need_pack else 'weight', weight)
@@ -215,7 +239,19 @@ class VllmRealQuantLinear(_RealQuantLinear):
         scales_name = 'weight_scale_inv' if quant_config['weight']['granularity'] == 'per_block' else 'weight_scale'
         new_module = cls(weight, bias, scales, input_scale, need_pack, scales_name)
         new_module._describe(module, weight, scales, None)
+        new_module.__dict__['act_form'] = _act_form(quant_config)
         return new_module
+
+    @torch.no_grad()
+    def forward(self, x, out_dtype=None):
+        """x [..., in_features] as values, or as codes that a norm before it made (QuantizedTokens; their output has the type of
+        the weight's scales)."""
+        if self.act_form is None:
+            raise NotImplementedError('only w8a8 containers (int8 weight per channel or tensor, int8 activations per token or static) run')
+        if isinstance(x, QuantizedTokens):
+            return int8_matmul(x, self.weight, self.weight_scale, self.bias, out_dtype or self.weight_scale.dtype)
+        return int8_linear(x, self.weight, self.weight_scale, self.bias, symmetric=self.act_form != 'asymmetric',
+                           scale=self.input_scale if self.act_form == 'static' else None, out_dtype=out_dtype)
 
     @classmethod
     @torch.no_grad()

@@ -1,0 +1,219 @@
+"""Running a w8a8 model: int8 codes of tokens, the int8 product with a scale for each token and channel, and the norm
+between two blocks that can hand its result on as codes.
+
+``VllmRealQuantLinear`` (module_utils.py:855-955) holds such a Linear's int8 weight and its scale per channel; the
+reference leaves running it to the serving engine, here its ``forward`` is ``int8_linear``.  The codes of activations
+are those of ``IntegerQuantizer`` with granularity per_token (quant.py:544-558, 698-716) on fp32 rows.
+All of this is forward only: nothing here records a gradient.
+"""
+from __future__ import annotations
+
+from contextlib import nullcontext
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib as L
+
+NORM_LAYER, NORM_POST_WEIGHT_F32, NORM_POST_BIAS_F32, NORM_WEIGHT_F32, NORM_BIAS_F32, NORM_RESIDUAL_F32 = 1, 2, 4, 8, 16, 32
+NORM_OUT_F32, NORM_ASYM = 64, 128
+MOST_COLS = 65536
+
+
+class QuantizedTokens(NamedTuple):
+    """(codes - zeros) * scales stands for the tokens."""
+    codes: torch.Tensor                       # int8 [..., K]
+    scales: torch.Tensor                      # fp32 [..., 1], or one for all tokens
+    zeros: Optional[torch.Tensor] = None      # int32 [..., 1]; None: 0
+
+
+class ResidualNorm(NamedTuple):
+    out: object                               # a tensor, or QuantizedTokens
+    residual: torch.Tensor
+
+
+_HERE = nullcontext()
+
+
+def _on(x, **others):
+    """Checks that all tensors are on x's GPU; a context in which that GPU is the current one."""
+    if not x.is_cuda:
+        raise L.LcqError('liblcq operates on GPU tensors only (no CPU fallback)')
+    index = x.get_device()
+    for name, t in others.items():
+        if t is not None and t.get_device() != index:
+            raise L.LcqError(f'{name} is on {t.device}, the tokens are on {x.device}')
+    return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+
+
+def _rows(t, K):
+    """-> (t or a contiguous copy, number of rows of K elements, distance between rows)."""
+    if t.dim() == 2 and t.stride(1) == 1:
+        return t, t.shape[0], t.stride(0)
+    t = t.contiguous()
+    return t, t.numel() // K, K
+
+
+def _cols(x):
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f'tokens need a last dimension of at least one column, got shape {tuple(x.shape)}')
+    if x.shape[-1] > MOST_COLS:
+        raise ValueError(f'at most {MOST_COLS} columns, got {x.shape[-1]}')
+    return x.shape[-1]
+
+
+@torch.no_grad()
+def quantize_tokens(x, symmetric=True, scale=None):
+    """Int8 codes of the tokens x [..., K] (fp32, bf16, fp16), one fp32 scale per token (and, not symmetric, one zero
+    point): QuantizedTokens.  `scale`: one given fp32 scale for all tokens (static activations, symmetric)."""
+    K = _cols(x)
+    code = L.dtype_code(x.dtype)
+    if scale is not None:
+        if not symmetric:
+            raise ValueError('a given scale is a symmetric one')
+        if scale.numel() != 1:
+            raise ValueError(f'one scale for all tokens, got {tuple(scale.shape)}')
+        scale = scale.reshape(1).float()
+    with _on(x, scale=scale):
+        rows, T, ld = _rows(x, K)
+        lead = x.shape[:-1]
+        codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+        scales = scale if scale is not None else torch.empty((*lead, 1), dtype=torch.float32, device=x.device)
+        zeros = None if symmetric else torch.empty((*lead, 1), dtype=torch.int32, device=x.device)
+        if T:
+            L.check(L.lib().lcq_quant_tokens(rows.data_ptr(), code, T, K, ld, not symmetric, L.ptr(scale), codes.data_ptr(),
+                                             None if scale is not None else scales.data_ptr(), L.ptr(zeros), L.stream()), 'lcq_quant_tokens')
+    return QuantizedTokens(codes, scales, zeros)
+
+
+def _check_weight(weight, weight_scales, bias, K):
+    if weight.dtype != torch.int8:
+        raise L.LcqError(f'an int8 weight is needed, got {weight.dtype}')
+    if weight.dim() != 2 or weight.shape[1] != K:
+        raise ValueError(f'weight {tuple(weight.shape)} does not take tokens of {K} columns')
+    N = weight.shape[0]
+    if weight_scales.numel() not in (1, N):
+        raise ValueError(f'{N} weight scales (or one) are needed, got {tuple(weight_scales.shape)}')
+    if bias is not None and tuple(bias.shape) != (N,):
+        raise ValueError(f'the bias of {N} channels has shape {tuple(bias.shape)}')
+    return N
+
+
+@torch.no_grad()
+def int8_matmul(tokens, weight, weight_scales, bias=None, out_dtype=torch.bfloat16):
+    """Tokens as codes (QuantizedTokens, codes [..., K]) times an int8 weight [N, K] with a scale per channel ([N], [N, 1], or
+    one for all; fp32, bf16, fp16), plus a bias [N]: [..., N] of `out_dtype`.  The sums are exact integers, scales and bias
+    are applied in fp32, the result is rounded once."""
+    codes, scales, zeros = tokens
+    K = _cols(codes)
+    if codes.dtype != torch.int8 or scales.dtype != torch.float32 or (zeros is not None and zeros.dtype != torch.int32):
+        raise L.LcqError('tokens are int8 codes with fp32 scales and int32 zero points')
+    N = _check_weight(weight, weight_scales, bias, K)
+    M = codes.numel() // K
+    if scales.numel() not in (1, M) or (zeros is not None and zeros.numel() != M):
+        raise ValueError(f'{M} token scales and zero points are needed, got {tuple(scales.shape)}'
+                         + ('' if zeros is None else f' and {tuple(zeros.shape)}'))
+    with _on(codes, scales=scales, zeros=zeros, weight=weight, weight_scales=weight_scales, bias=bias):
+        y = torch.empty((*codes.shape[:-1], N), dtype=out_dtype, device=codes.device)
+        code = L.dtype_code(out_dtype)
+        if M and N:
+            lib = L.lib()
+            size = lib.lcq_int8_matmul_workspace_bytes(M, N, K)
+            ws = torch.empty(size, dtype=torch.uint8, device=codes.device) if size else None
+            L.check(lib.lcq_int8_matmul(L.ptr(codes), L.ptr(scales), scales.numel() == 1, L.ptr(zeros), L.ptr(weight),
+                                        L.ptr(weight_scales), L.dtype_code(weight_scales.dtype), weight_scales.numel() == 1,
+                                        L.ptr(bias), 0 if bias is None else L.dtype_code(bias.dtype), M, N, K, y.data_ptr(),
+                                        code, L.ptr(ws), L.stream()), 'lcq_int8_matmul')
+    return y
+
+
+@torch.no_grad()
+def int8_linear(x, weight, weight_scales, bias=None, symmetric=True, scale=None, out_dtype=None):
+    """A w8a8 Linear on x [..., K]: quantize_tokens(x, symmetric, scale), then int8_matmul to x's type (or `out_dtype`)."""
+    return int8_matmul(quantize_tokens(x, symmetric, scale), weight, weight_scales, bias, out_dtype or x.dtype)
+
+
+def _affine(name, t, K, x, flag):
+    """The flag of a [K] parameter of a norm: of the tokens' type, or fp32."""
+    if t is None:
+        return 0
+    if tuple(t.shape) != (K,):
+        raise ValueError(f'{name} of {K} columns has shape {tuple(t.shape)}')
+    if t.dtype == x.dtype:
+        return 0
+    if t.dtype != torch.float32:
+        raise L.LcqError(f'{name} is {t.dtype}: the tokens\' {x.dtype} or float32 is needed')
+    return flag
+
+
+@torch.no_grad()
+def residual_norm(x, residual=None, weight=None, bias=None, *, gate=None, post_weight=None, post_bias=None, scale=1.0,
+                  eps=1e-6, kind='rms', weight_offset=0.0, quantize=None, out_dtype=None, inplace=False):
+    """The end of one block and the start of the next, for the block's output x [..., K], in one pass:
+
+        b = x, or norm(x) with post_weight / post_bias where post_weight is given
+        h = residual + scale * (gate * b)                       the residual stream
+        out = norm(h) with weight / bias                        the next block's input
+
+    kind 'rms': norm(v) = v / sqrt(mean v^2 + eps) * (w + weight_offset) + b;  'layer': the same of v - mean v.
+    residual: like x, in x's type or fp32 (the stream keeps it); None: 0.  gate: like x, or [K]; None: 1.  A missing
+    weight is 1 without an offset.  quantize 'symmetric' / 'asymmetric': out is quantize_tokens of the unrounded norm.
+    out_dtype: x's type (default) or fp32.  inplace: h is written over residual.  -> ResidualNorm(out, residual = h)"""
+    K = _cols(x)
+    code = L.dtype_code(x.dtype)
+    if kind not in ('rms', 'layer') or quantize not in (None, 'symmetric', 'asymmetric'):
+        raise ValueError(f'kind {kind!r}, quantize {quantize!r}')
+    if post_bias is not None and post_weight is None:
+        raise ValueError('post_bias goes with post_weight')
+    flags = (NORM_LAYER if kind == 'layer' else 0) | _affine('post_weight', post_weight, K, x, NORM_POST_WEIGHT_F32) \
+        | _affine('post_bias', post_bias, K, x, NORM_POST_BIAS_F32) | _affine('weight', weight, K, x, NORM_WEIGHT_F32) \
+        | _affine('bias', bias, K, x, NORM_BIAS_F32)
+    stream_dtype = x.dtype
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise ValueError(f'residual {tuple(residual.shape)} next to x {tuple(x.shape)}')
+        if residual.dtype not in (x.dtype, torch.float32):
+            raise L.LcqError(f'residual is {residual.dtype}: x\'s {x.dtype} or float32 is needed')
+        stream_dtype = residual.dtype
+        if stream_dtype != x.dtype:
+            flags |= NORM_RESIDUAL_F32
+    if inplace and (residual is None or not residual.is_contiguous()):
+        raise ValueError('inplace needs a contiguous residual')
+    if gate is not None:
+        if gate.dtype != x.dtype:
+            raise L.LcqError(f'gate is {gate.dtype}, x is {x.dtype}')
+        if tuple(gate.shape) != (K,) and gate.shape != x.shape:
+            raise ValueError(f'gate {tuple(gate.shape)} next to x {tuple(x.shape)}')
+    if out_dtype is None or out_dtype == x.dtype:
+        out_dtype = x.dtype
+    elif out_dtype == torch.float32:
+        flags |= NORM_OUT_F32
+    else:
+        raise L.LcqError(f'out_dtype {out_dtype}: x\'s {x.dtype} or float32 is needed')
+    with _on(x, residual=residual, weight=weight, bias=bias, gate=gate, post_weight=post_weight, post_bias=post_bias):
+        rows, T, ldx = _rows(x, K)
+        res, ldr, g, ldg = residual, 0, gate, 0
+        if residual is not None:
+            res, _, ldr = _rows(residual, K)
+        if gate is not None and gate.dim() == 1:
+            g = gate.contiguous()
+            ldg = 0
+        elif gate is not None:
+            g, _, ldg = _rows(gate, K)
+        h = residual if inplace else torch.empty(x.shape, dtype=stream_dtype, device=x.device)
+        out = codes = scales = zeros = None
+        if quantize is None:
+            out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+        else:
+            codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+            scales = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=x.device)
+            if quantize == 'asymmetric':
+                flags |= NORM_ASYM
+                zeros = torch.empty((*x.shape[:-1], 1), dtype=torch.int32, device=x.device)
+        if T:
+            at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+            L.check(L.lib().lcq_residual_norm(rows.data_ptr(), code, T, K, ldx, at(res), ldr, at(g), ldg, L.ptr(post_weight),
+                                              L.ptr(post_bias), L.ptr(weight), L.ptr(bias), scale, eps, weight_offset, flags,
+                                              h.data_ptr(), at(out), at(codes), at(scales), at(zeros), L.stream()),
+                    'lcq_residual_norm')
+    return ResidualNorm(out if quantize is None else QuantizedTokens(codes, scales, zeros), h)
