@@ -1,18 +1,36 @@
-// Log probabilities of given tokens, entropy and best alternatives of logits x [T, V]:
-//   m = max x,  S = sum exp(x - m),  U = sum exp(x - m) (x - m)
-//   log sum exp x = m + log S;   logprob of a token t = (x_t - m) - log S;   entropy = log S - U / S
+// Log probabilities of given tokens, entropy and best alternatives of logits x [T, V], in one pass over them:
+//   S = sum exp(x - c),  U = sum exp(x - c) (x - c)   for any reference c
+//   log sum exp x = c + log S;   logprob of a token t = (x_t - c) - log S;   entropy = log S - U / S
+//
+//  * A lane keeps its own c, S and U.  c is a logit that the lane has seen; it moves only where a later one is more than 8 above
+//    it, so that almost no piece pays for a change of reference, S stays below V e^8 and log S and U / S do not cancel to more than a few
+//    times their last bits.  References meet once, when lanes, waves and parts are joined.
+//  * The best alternatives: each wave keeps 64 keys, one per lane in descending order.  A key is a whole number that orders by value
+//    and then by the lowest index.  A 16-byte piece whose maximum lies below the k-th best so far costs one comparison; what passes is
+//    collected in LDS and taken over 64 at a time (a bitonic sort, then a merge).  Where many lanes pass at once (the first piece,
+//    ascending logits) the k-th best of the lanes' maxima is a bound first.
+//  * A row is one workgroup's where there are enough rows, else it is cut into parts of whole 256-lane passes for about four workgroups
+//    per CU, which leave (c, S, U) and k keys each for a second, small kernel.
 #include "rowquant.h"
+#include <type_traits>
 
 namespace {
 using namespace lcq;
+
+constexpr float LOWEST = -3.4028234663852886e38f, MOVE = 8.0f;
+constexpr int THREADS = 256, WAVES = THREADS / 64;
+constexpr int FLIGHT = 4;                           // 16-byte pieces that a lane has in flight
 
 struct LogprobArgs {
   const void* x;
   const int64_t* tokens;
   float *logprobs, *entropy, *top_logprobs;
   int64_t* top_tokens;
-  int64_t T, V, ldx, m, ignore;
-  int k;
+  int64_t V, ldx, m, ignore;
+  int k, parts;
+  int64_t per;                                      // 16-byte pieces of a part
+  f32x4* sums;                                      // [T, parts]: c, S, U
+  uint64_t* keys;                                   // [T, parts, k]
 };
 
 // A whole number that orders logits by value and, among equal ones, by the lowest index; a NaN is above everything, -0 equals +0.
@@ -28,82 +46,268 @@ __device__ __forceinline__ float logit_of(uint64_t key) {
 }
 __device__ __forceinline__ uint32_t index_of(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
 
-// One workgroup per row: a pass for the maximum, one for the sums, one for each alternative.
+__device__ __forceinline__ uint64_t other_lane(uint64_t v, int lane) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(lane * 4, (int)(uint32_t)v), hi = (uint32_t)__builtin_amdgcn_ds_bpermute(lane * 4, (int)(v >> 32));
+  return (uint64_t)hi << 32 | lo;
+}
+// lane i and lane i ^ d: the larger key to the lower lane where `down`, else the other way
+__device__ __forceinline__ uint64_t exchange(uint64_t v, int lane, int d, bool down) {
+  const uint64_t o = other_lane(v, lane ^ d);
+  return (((lane & d) == 0) == down) == (v > o) ? v : o;
+}
+// the wave's 64 keys in descending order
+__device__ __forceinline__ uint64_t sorted(uint64_t v, int lane) {
+  #pragma unroll
+  for (int n = 2; n <= 64; n *= 2)
+    #pragma unroll
+    for (int d = n / 2; d; d /= 2) v = exchange(v, lane, d, (lane & n) == 0);
+  return v;
+}
+// the 64 largest of two descending lists, `turned` with its lanes in ascending order
+__device__ __forceinline__ uint64_t merged(uint64_t v, uint64_t turned, int lane) {
+  v = v > turned ? v : turned;
+  #pragma unroll
+  for (int d = 32; d; d /= 2) v = exchange(v, lane, d, true);
+  return v;
+}
+
+// The best 64 of a wave.  `count` and `bound` are the same in all lanes.
+struct Best {
+  uint64_t mine = 0, bound = 0;                     // lane i: the i-th best; the k-th best, 0 while there are fewer
+  float limit = -__builtin_inff();                  // bound's logit: a logit below it is not among the best k
+  int lane, k;
+  __device__ __forceinline__ Best(int lane_, int k_) : lane(lane_), k(k_) {}
+  __device__ __forceinline__ void raise(uint64_t key) {
+    if (key > bound) { bound = key; limit = logit_of(key); }
+    limit = limit == limit ? limit : __builtin_inff();       // (k NaNs: whatever is not one stays out; a NaN passes every limit)
+  }
+  __device__ __forceinline__ uint64_t kth(uint64_t v) const {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, k - 1), hi = (uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), k - 1);
+    return (uint64_t)hi << 32 | lo;
+  }
+  // one key per lane (0: none)
+  __device__ __forceinline__ void take(uint64_t key) {
+    if (__builtin_amdgcn_ballot_w64(key > bound) == 0) return;
+    mine = merged(mine, other_lane(sorted(key, lane), 63 - lane), lane);
+    raise(kth(mine));
+  }
+};
+
+struct Sums {
+  float c = LOWEST, S = 0.0f, U = 0.0f;
+  // to the reference `to` >= c
+  __device__ __forceinline__ void refer(float to) {
+    const float d = c - to, f = __builtin_amdgcn_exp2f(d * 1.44269504088896340736f);
+    U = f * (U + S * nan_max(d, -150.0f));          // (f is 0 below that)
+    S *= f;
+    c = to;
+  }
+  __device__ __forceinline__ void add(const Sums& o) { S += o.S; U += o.U; }
+  __device__ __forceinline__ void join_wave() {
+    refer(team_reduce<64, true>(c));
+    S = team_sum<64>(S);
+    U = team_sum<64>(U);
+  }
+};
+
+// What a workgroup's waves found, joined in wave 0 -> true there
+template <bool TOP>
+__device__ __forceinline__ bool join_waves(Sums& s, Best& best) {
+  __shared__ float part[WAVES][3];
+  __shared__ uint64_t keys[TOP ? WAVES : 1][64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  s.join_wave();
+  if (lane == 0) { part[wave][0] = s.c; part[wave][1] = s.S; part[wave][2] = s.U; }
+  if (TOP) keys[wave][lane] = best.mine;
+  __syncthreads();
+  if (wave) return false;
+  float c = s.c;
+  #pragma unroll
+  for (int w = 1; w < WAVES; ++w) c = nan_max(c, part[w][0]);
+  s.refer(c);
+  #pragma unroll
+  for (int w = 1; w < WAVES; ++w) {
+    Sums o;
+    o.c = part[w][0]; o.S = part[w][1]; o.U = part[w][2];
+    o.refer(c);
+    s.add(o);
+    if (TOP) best.mine = merged(best.mine, keys[w][63 - lane], lane);
+  }
+  return true;
+}
+
 template <int BF>
-__global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
-  __shared__ float sf[256];
-  __shared__ uint64_t sk[256];
-  const int tid = threadIdx.x;
-  const int64_t row = blockIdx.x, base = row * a.ldx;
-  const auto fold = [&](float v, auto&& f) {
-    __syncthreads();
-    sf[tid] = v;
-    __syncthreads();
-    for (int d = 128; d; d >>= 1) {
-      if (tid < d) sf[tid] = f(sf[tid], sf[tid + d]);
-      __syncthreads();
-    }
-    return sf[0];
-  };
-  float m = -3.4028234663852886e38f;
-  for (int64_t v = tid; v < a.V; v += 256) m = nan_max(m, load_scalar<BF>(a.x, base + v));
-  m = fold(m, [](float p, float q) { return nan_max(p, q); });
-  float S = 0.0f, U = 0.0f;
-  for (int64_t v = tid; v < a.V; v += 256) {
-    const float d = load_scalar<BF>(a.x, base + v) - m, e = expf(d);
-    S += e;
-    U += e * nan_max(d, -150.0f);
-  }
-  S = fold(S, [](float p, float q) { return p + q; });
-  U = fold(U, [](float p, float q) { return p + q; });
-  const float l = logf(S);
-  if (tid == 0 && a.entropy) a.entropy[row] = l - U / S;
-  for (int64_t j = tid; j < a.m; j += 256) {
+__device__ __forceinline__ void answer(const LogprobArgs& a, int64_t row, const Sums& s, uint64_t mine, int lane) {
+  const float l = logf(s.S);
+  if (lane == 0 && a.entropy) a.entropy[row] = l - s.U / s.S;
+  for (int64_t j = lane; j < a.m; j += 64) {
     const int64_t t = a.tokens[row * a.m + j];
-    a.logprobs[row * a.m + j] = t == a.ignore ? 0.0f : t < 0 || t >= a.V ? __builtin_nanf("") : (load_scalar<BF>(a.x, base + t) - m) - l;
+    a.logprobs[row * a.m + j] = t == a.ignore ? 0.0f : t < 0 || t >= a.V ? __builtin_nanf("") : (load_scalar<BF>(a.x, row * a.ldx + t) - s.c) - l;
   }
-  uint64_t last = ~0ull;
-  for (int j = 0; j < a.k; ++j) {
-    uint64_t best = 0;
-    for (int64_t v = tid; v < a.V; v += 256) {
-      const uint64_t key = key_of(load_scalar<BF>(a.x, base + v), (uint32_t)v);
-      if (key < last && key > best) best = key;
+  if (lane < a.k) {
+    a.top_logprobs[row * a.k + lane] = (logit_of(mine) - s.c) - l;
+    a.top_tokens[row * a.k + lane] = index_of(mine);
+  }
+}
+
+template <int BF, bool TOP>
+__global__ __launch_bounds__(THREADS) void logprobs_kernel(LogprobArgs a) {
+  constexpr int N = Vec<BF>::N;
+  __shared__ uint64_t found[TOP ? WAVES : 1][TOP ? 64 * N + 64 : 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = (int64_t)blockIdx.x / a.parts;
+  const int part = (int)((int64_t)blockIdx.x - row * a.parts);
+  const char* const first = (const char*)a.x + row * a.ldx * (16 / N);
+  // pieces of 16 aligned bytes: piece j holds logits N j - before ...; only the first and the last may reach out of the row
+  const int before = (int)((uintptr_t)first % 16) / (16 / N);
+  const char* const base = first - before * (16 / N);
+  const int64_t pieces = (a.V + before + N - 1) / N;
+  const int64_t from = part * a.per, to = from + a.per < pieces ? from + a.per : pieces;
+
+  Sums s;
+  Best best(lane, TOP ? a.k : 1);
+  int count = 0;
+  const auto drain = [&] {                          // takes over what was collected
+    for (int at = 0; at < count; at += 64) best.take(at + lane < count ? found[wave][at + lane] : 0);
+    count = 0;
+  };
+  const auto piece = [&](const u32x4& raw, int64_t j) {
+    float v[N];
+    unpack<BF>(raw, v);
+    float top = v[0];
+    #pragma unroll
+    for (int i = 1; i < N; ++i) top = nan_max(top, v[i]);
+    if (top > s.c + MOVE) s.refer(top);
+    if constexpr (TOP) {
+      const uint64_t pass = __builtin_amdgcn_ballot_w64(!(top < best.limit));
+      if (__builtin_expect(pass != 0, 0)) {
+        const int64_t v0 = j * N - before;
+        uint64_t key[N];
+        #pragma unroll
+        for (int i = 0; i < N; ++i) key[i] = v0 + i >= 0 && v0 + i < a.V ? key_of(v[i], (uint32_t)(v0 + i)) : 0;
+        if (__builtin_popcountll(pass) > 16) {
+          uint64_t m = key[0];
+          #pragma unroll
+          for (int i = 1; i < N; ++i) m = key[i] > m ? key[i] : m;
+          m = best.kth(sorted(m, lane));
+          if (m) best.raise(m - 1);                          // (less one: the k-th itself has still to be collected)
+        }
+        #pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const bool in = key[i] > best.bound;
+          const uint64_t lanes = __builtin_amdgcn_ballot_w64(in);
+          if (lanes == 0) continue;
+          if (in) found[wave][count + __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0))] = key[i];
+          count += __builtin_popcountll(lanes);
+        }
+        if (count >= 64) drain();
+      }
     }
-    __syncthreads();
-    sk[tid] = best;
-    __syncthreads();
-    for (int d = 128; d; d >>= 1) {
-      if (tid < d && sk[tid + d] > sk[tid]) sk[tid] = sk[tid + d];
-      __syncthreads();
+    #pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float d = v[i] - s.c, e = __builtin_amdgcn_exp2f(d * 1.44269504088896340736f);
+      s.S += e;
+      s.U = __builtin_fmaf(e, nan_max(d, -150.0f), s.U);     // (-inf: e is 0)
     }
-    last = sk[0];
-    if (tid == 0) {
-      a.top_logprobs[row * a.k + j] = (logit_of(last) - m) - l;
-      a.top_tokens[row * a.k + j] = index_of(last);
+  };
+  const auto load = [&](int64_t j) -> u32x4 {
+    const int64_t v0 = j * N - before;
+    if (v0 >= 0 && v0 + N <= a.V) return *(const u32x4*)(base + j * 16);
+    float v[N];
+    #pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = v0 + i >= 0 && v0 + i < a.V ? load_scalar<BF>(first, v0 + i) : -__builtin_inff();
+    return pack<BF>(v);
+  };
+  const u32x4 nothing = N == 4 ? u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u}      // -inf
+                               : u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u} & (BF == ROW_F16 ? 0xfc00fc00u : ~0u);
+  for (int64_t j0 = from; j0 < to; j0 += THREADS * FLIGHT) {
+    u32x4 raw[FLIGHT];
+    #pragma unroll
+    for (int f = 0; f < FLIGHT; ++f) {
+      const int64_t j = j0 + f * THREADS + threadIdx.x;
+      raw[f] = j < to ? load(j) : nothing;
+    }
+    #pragma unroll
+    for (int f = 0; f < FLIGHT; ++f) {
+      const int64_t j = j0 + f * THREADS + threadIdx.x;
+      piece(raw[f], j < to ? j : pieces + 1);       // (past the end of the row: nothing of it can be among the best)
     }
   }
+  if constexpr (TOP) drain();
+  if (!join_waves<TOP>(s, best)) return;
+  if (a.parts == 1) {
+    answer<BF>(a, row, s, best.mine, lane);
+    return;
+  }
+  if (lane == 0) a.sums[blockIdx.x] = f32x4{s.c, s.S, s.U, 0.0f};
+  if (lane < a.k) a.keys[(int64_t)blockIdx.x * a.k + lane] = best.mine;
+}
+
+// The parts of a row joined: one workgroup per row.
+template <int BF>
+__global__ __launch_bounds__(THREADS) void join_kernel(LogprobArgs a) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = blockIdx.x;
+  Sums s;
+  for (int p = threadIdx.x; p < a.parts; p += THREADS) {
+    const f32x4 v = a.sums[row * a.parts + p];
+    Sums o;
+    o.c = v[0]; o.S = v[1]; o.U = v[2];
+    const float c = nan_max(s.c, o.c);
+    s.refer(c);
+    o.refer(c);
+    s.add(o);
+  }
+  Best best(lane, a.k > 0 ? a.k : 1);
+  const int all = a.parts * a.k;
+  for (int i = wave * 64; i < all; i += THREADS) best.take(i + lane < all ? a.keys[row * all + i + lane] : 0);
+  if (join_waves<true>(s, best)) answer<BF>(a, row, s, best.mine, lane);
+}
+
+int parts_of(int64_t T, int64_t V, int dtype) {
+  const int64_t passes = (V * (dtype == LCQ_F32 ? 4 : 2) + 16 * THREADS - 1) / (16 * THREADS);
+  const int64_t want = 1024 / T;
+  return (int)(want < 1 ? 1 : want < passes ? want : passes);
 }
 
 }  // namespace
 
 extern "C" {
 
-int64_t lcq_token_logprobs_workspace_bytes(int64_t T, int64_t V, int k) { (void)T; (void)V; (void)k; return 0; }
+int64_t lcq_token_logprobs_workspace_bytes(int64_t T, int64_t V, int k) {
+  if (T <= 0 || V <= 0 || k < 0) return 0;
+  const int parts = parts_of(T, V, LCQ_F32);        // (the most there are)
+  return parts == 1 ? 0 : T * parts * (16 + 8 * (int64_t)k);
+}
 
 int lcq_token_logprobs(const void* logits, int dtype, int64_t T, int64_t V, int64_t ldx, const int64_t* tokens, int64_t m,
                        int64_t ignore, float* logprobs, float* entropy, int k, float* top_logprobs, int64_t* top_tokens,
                        void* workspace, void* stream) {
-  (void)workspace;
   if (!logits || T <= 0 || V <= 0 || ldx < 0 || m < 0 || k < 0 || k > 64 || k > V) return LCQ_EINVAL;
   if ((m > 0 && (!tokens || !logprobs)) || (k > 0 && (!top_logprobs || !top_tokens))) return LCQ_EINVAL;
   if (dtype != LCQ_F32 && dtype != LCQ_BF16 && dtype != LCQ_F16) return LCQ_EDTYPE;
   if (T > 0x7fffffff || V > 0x7fffffff) return LCQ_ESIZE;
-  const LogprobArgs a = {logits, tokens, logprobs, entropy, top_logprobs, top_tokens, T, V, ldx, m, ignore, k};
-  const dim3 grid((unsigned)T);
+  if ((uintptr_t)logits % (dtype == LCQ_F32 ? 4 : 2)) return LCQ_EALIGN;
+  LogprobArgs a = {logits, tokens, logprobs, entropy, top_logprobs, top_tokens, V, ldx, m, ignore, k, parts_of(T, V, dtype), 0, nullptr, nullptr};
+  if (a.parts > 1) {
+    if (!workspace) return LCQ_EWORKSPACE;
+    if ((uintptr_t)workspace % 16) return LCQ_EALIGN;
+    a.sums = (f32x4*)workspace;
+    a.keys = (uint64_t*)(a.sums + T * a.parts);
+  }
+  const int n = dtype == LCQ_F32 ? 4 : 8;
+  a.per = ((V + n - 1) / n + 1 + a.parts - 1) / a.parts;       // (one more piece where a row does not start on 16 bytes)
+  const dim3 grid((unsigned)(T * a.parts)), block(THREADS);
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == LCQ_BF16) logprobs_kernel<ROW_BF16><<<grid, dim3(256), 0, st>>>(a);
-  else if (dtype == LCQ_F16) logprobs_kernel<ROW_F16><<<grid, dim3(256), 0, st>>>(a);
-  else logprobs_kernel<ROW_F32><<<grid, dim3(256), 0, st>>>(a);
+  const auto run = [&](auto bf) {
+    constexpr int BF = decltype(bf)::value;
+    if (k) logprobs_kernel<BF, true><<<grid, block, 0, st>>>(a);
+    else logprobs_kernel<BF, false><<<grid, block, 0, st>>>(a);
+    if (a.parts > 1) join_kernel<BF><<<dim3((unsigned)T), block, 0, st>>>(a);
+  };
+  if (dtype == LCQ_BF16) run(std::integral_constant<int, ROW_BF16>{});
+  else if (dtype == LCQ_F16) run(std::integral_constant<int, ROW_F16>{});
+  else run(std::integral_constant<int, ROW_F32>{});
   LCQ_CHECK_LAUNCH();
   return LCQ_OK;
 }

@@ -1,5 +1,5 @@
 """Log probabilities of given tokens, with entropy and best alternatives, from a model's logits in one pass: what the
-reference's perplexity (llmc/eval/eval_ppl.py) and token-consistency (llmc/eval/eval_token_consist.py) evaluations
+reference's perplexity (llmc/eval/eval_ppl.py) and token-consistency evaluations
 take from a whole log-softmax and an argmax.  Forward only: nothing here records a gradient."""
 from __future__ import annotations
 
