@@ -86,6 +86,10 @@ def quantize_tokens(x, symmetric=True, scale=None):
     return QuantizedTokens(codes, scales, zeros)
 
 
+def _on16(t):
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _check_weight(weight, weight_scales, bias, K):
     if weight.dtype != torch.int8:
         raise L.LcqError(f'an int8 weight is needed, got {weight.dtype}')
@@ -114,6 +118,8 @@ def int8_matmul(tokens, weight, weight_scales, bias=None, out_dtype=torch.bfloat
         raise ValueError(f'{M} token scales and zero points are needed, got {tuple(scales.shape)}'
                          + ('' if zeros is None else f' and {tuple(zeros.shape)}'))
     with _on(codes, scales=scales, zeros=zeros, weight=weight, weight_scales=weight_scales, bias=bias):
+        if K % 16 == 0:                       # (other widths are copied to padded rows by the call itself)
+            codes, weight = _on16(codes), _on16(weight)
         y = torch.empty((*codes.shape[:-1], N), dtype=out_dtype, device=codes.device)
         code = L.dtype_code(out_dtype)
         if M and N:
