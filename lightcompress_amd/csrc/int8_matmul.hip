@@ -6,6 +6,8 @@
 // Both operands are read along K, as the matrix pipe takes them: a lane of v_mfma_i32_32x32x32_i8 holds 16 codes of one row.
 // The weight is the first operand, so an accumulator's four neighbouring registers are four neighbouring channels of one token.
 #include "rowquant.h"
+#include "token_codes.h"
+#include <type_traits>
 
 namespace {
 using namespace lcq;
@@ -236,6 +238,158 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MatmulArgs g, int tiles_m,
   }
 }
 
+// ---- few tokens ---------------------------------------------------------------------------------------------------
+// The weight is read once, straight into the matrix pipe's operands: a lane of v_mfma_i32_16x16x64_i8 takes 16 codes of one of 16
+// channels, so a load of the wave is 16 rows x 64 bytes in a row.  A workgroup owns 16 channels, its eight waves take pieces of 256
+// codes of K in turn and meet in LDS; two pieces (8 KiB of weight per wave) are in flight.  The tokens' codes come from the cache, every
+// wave other ones.
+// x: the tokens as values (at most MOST_FUSED of them): every workgroup makes their codes itself, in LDS, while its first weights are on
+// their way - cheaper for one token than another kernel in front.
+constexpr int STREAM_THREADS = 512, STREAM_WAVES = STREAM_THREADS / 64, PIECE = 256;
+constexpr int MOST_FUSED = 4;
+constexpr int64_t MOST_FUSED_CODES = 40960;         // in LDS
+
+struct TokenArgs {
+  const void* x;
+  const float* scale;
+  int64_t ldx;
+  int asym;
+};
+
+// One row of x to int8 codes in LDS, by the whole workgroup; K % 16 == 0.
+template <int XT>
+__device__ __forceinline__ void codes_to_lds(const TokenArgs& t, int64_t row, int K, int8_t* out, float* red, float* scale, int* zero) {
+  const int tid = threadIdx.x;
+  const char* const x = (const char*)t.x + row * t.ldx * (XT == ROW_F32 ? 4 : 2);
+  const bool wide = (uintptr_t)x % 16 == 0;
+  const auto load = [&](int i, float* v) {
+    if (wide) {
+      if constexpr (XT == ROW_F32) { unpack<XT>(*(const u32x4*)(x + i * 4), v); unpack<XT>(*(const u32x4*)(x + i * 4 + 16), v + 4); }
+      else unpack<XT>(*(const u32x4*)(x + i * 2), v);
+    } else {
+      #pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = load_scalar<XT>(x, i + e);
+    }
+  };
+  constexpr int KEEP = 4;                           // pieces of eight that stay in registers: K up to 16384
+  float v[KEEP][8];
+  float hi = t.asym ? -__builtin_inff() : 0.0f, lo = __builtin_inff();
+  const auto range = [&](const float* e) {
+    #pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      hi = nan_max(hi, t.asym ? e[j] : fabsf(e[j]));
+      lo = nan_min(lo, e[j]);
+    }
+  };
+  #pragma unroll
+  for (int c = 0; c < KEEP; ++c) {
+    const int i = (tid + c * STREAM_THREADS) * 8;
+    if (i < K) { load(i, v[c]); range(v[c]); }
+  }
+  for (int i = (tid + KEEP * STREAM_THREADS) * 8; i < K; i += STREAM_THREADS * 8) {
+    float e[8];
+    load(i, e);
+    range(e);
+  }
+  hi = team_reduce<64, true>(hi);
+  lo = team_reduce<64, false>(lo);
+  if ((tid & 63) == 0) { red[tid >> 6] = hi; red[STREAM_WAVES + (tid >> 6)] = lo; }
+  __syncthreads();
+  #pragma unroll
+  for (int w = 0; w < STREAM_WAVES; ++w) { hi = nan_max(hi, red[w]); lo = nan_min(lo, red[STREAM_WAVES + w]); }
+  const TokenCodes q = t.scale ? TokenCodes::given(t.scale[0]) : t.asym ? TokenCodes::asymmetric(lo, hi) : TokenCodes::symmetric(hi);
+  #pragma unroll
+  for (int c = 0; c < KEEP; ++c) {
+    const int i = (tid + c * STREAM_THREADS) * 8;
+    if (i < K) *(u32x2*)(out + i) = u32x2{q.codes(v[c]), q.codes(v[c] + 4)};
+  }
+  for (int i = (tid + KEEP * STREAM_THREADS) * 8; i < K; i += STREAM_THREADS * 8) {
+    float e[8];
+    load(i, e);
+    *(u32x2*)(out + i) = u32x2{q.codes(e), q.codes(e + 4)};
+  }
+  if (tid == 0) {
+    *scale = q.d.s;
+    *zero = (int)q.z;
+  }
+  __syncthreads();
+}
+
+// XT: the type of the tokens' values, or -1 for codes
+template <int TB, int BF, int XT>
+__global__ __launch_bounds__(STREAM_THREADS) void stream_kernel(MatmulArgs g, TokenArgs t) {
+  __shared__ __attribute__((aligned(16))) int red[STREAM_WAVES][TB + 1][64][4];
+  __shared__ float token_scale[XT < 0 ? 1 : MOST_FUSED];
+  __shared__ int token_zero[XT < 0 ? 1 : MOST_FUSED];
+  extern __shared__ __attribute__((aligned(16))) int8_t codes[];             // [M, K], XT >= 0 only
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int64_t n = n0 + (lane & 15) < g.N ? n0 + (lane & 15) : g.N - 1;
+  const int at = (lane >> 4) * 16;
+  const int8_t* const w = g.w + n * g.ldw + at;
+  const bool asym = XT < 0 ? g.az != nullptr : t.asym;
+
+  struct Piece { i32x4 v[4]; };
+  const auto weights = [&](int k, Piece& p) {       // codes k .. k + 255 of this lane's channel
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) p.v[i] = k + i * 64 + at < g.K ? *(const i32x4*)(w + k + i * 64) : i32x4{0, 0, 0, 0};
+  };
+  Piece cur, nxt;
+  const int step = STREAM_WAVES * PIECE;
+  int k = wave * PIECE;
+  weights(k, cur);
+  weights(k + step, nxt);
+  if constexpr (XT >= 0) {
+    for (int m = 0; m < (int)g.M; ++m)
+      codes_to_lds<XT>(t, m, g.K, codes + m * g.K, (float*)red, token_scale + m, token_zero + m);
+  }
+  const int8_t* a[TB];
+  #pragma unroll
+  for (int b = 0; b < TB; ++b) {
+    const int64_t m = b * 16 + (lane & 15) < g.M ? b * 16 + (lane & 15) : g.M - 1;           // (a token twice: not stored)
+    a[b] = XT < 0 ? g.a + m * g.lda + at : codes + m * g.K + at;
+  }
+  i32x4 acc[TB] = {};
+  int wsum = 0;
+  while (k < g.K) {
+    Piece tok[TB];
+    #pragma unroll
+    for (int b = 0; b < TB; ++b)
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) tok[b].v[i] = k + i * 64 + at < g.K ? *(const i32x4*)(a[b] + k + i * 64) : i32x4{0, 0, 0, 0};
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      #pragma unroll
+      for (int b = 0; b < TB; ++b) acc[b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cur.v[i], tok[b].v[i], acc[b], 0, 0, 0);
+      if (asym) wsum = add_bytes(cur.v[i], wsum);
+    }
+    k += step;
+    cur = nxt;
+    weights(k + step, nxt);
+  }
+  #pragma unroll
+  for (int b = 0; b < TB; ++b) *(i32x4*)red[wave][b][lane] = acc[b];
+  red[wave][TB][lane][0] = wsum;
+  __syncthreads();
+  // accumulator register r of lane l: channel 4 (l / 16) + r of token l % 16
+  for (int o = tid; o < TB * 256; o += STREAM_THREADS) {
+    const int c = o & 15, tok = (o >> 4) & 15, b = o >> 8;
+    const int64_t m = b * 16 + tok, nn = n0 + c;
+    if (m >= g.M || nn >= g.N) continue;
+    int s = 0, sum = 0;
+    #pragma unroll
+    for (int v = 0; v < STREAM_WAVES; ++v) {
+      s += red[v][b][(c >> 2) * 16 + tok][c & 3];
+      if (asym) sum += (red[v][TB][c][0] + red[v][TB][c + 16][0]) + (red[v][TB][c + 32][0] + red[v][TB][c + 48][0]);
+    }
+    if (asym) s -= (XT < 0 ? g.az[m] : token_zero[m]) * sum;
+    const float as = XT < 0 ? g.as[g.a_scalar ? 0 : m] : token_scale[m];
+    const float y = (float)s * (as * load_any(g.ws, g.ws_dtype, g.w_scalar ? 0 : nn)) + (g.bias ? load_any(g.bias, g.bias_dtype, nn) : 0.0f);
+    if constexpr (BF == ROW_F32) ((float*)g.y)[m * g.N + nn] = y;
+    else store_scalar<BF>(g.y, m * g.N + nn, rnd<BF>(y));
+  }
+}
+
 // Rows of K codes to rows of Kp, the next multiple of 16, with zeros behind them: operands whose rows do not start on 16 bytes.
 __global__ __launch_bounds__(256) void pad_kernel(const int8_t* __restrict__ x, int64_t rows, int K, int Kp, int8_t* __restrict__ out) {
   const int per = Kp / 16;
@@ -266,6 +420,44 @@ void launch_tiles(const MatmulArgs& g, hipStream_t st) {
   else tile_kernel<FM, FN, BF, false><<<grid, dim3(256), 0, st>>>(g, (int)tm, (int)tn);
 }
 
+#ifndef STREAM_MOST
+#define STREAM_MOST 32
+#endif
+constexpr int64_t MOST_STREAMED = STREAM_MOST;      // tokens
+
+template <int BF, int XT>
+void launch_stream(const MatmulArgs& g, const TokenArgs& t, hipStream_t st) {
+  const dim3 grid((unsigned)((g.N + 15) / 16));
+  if constexpr (XT >= 0) {
+    stream_kernel<1, BF, XT><<<grid, dim3(STREAM_THREADS), (unsigned)(g.M * g.K), st>>>(g, t);
+  } else {
+    if (g.M <= 16) stream_kernel<1, BF, -1><<<grid, dim3(STREAM_THREADS), 0, st>>>(g, t);
+    else if (g.M <= 32) stream_kernel<2, BF, -1><<<grid, dim3(STREAM_THREADS), 0, st>>>(g, t);
+    else stream_kernel<4, BF, -1><<<grid, dim3(STREAM_THREADS), 0, st>>>(g, t);
+  }
+}
+
+template <int BF>
+void launch_codes(const MatmulArgs& g, hipStream_t st) {
+  if (g.M <= MOST_STREAMED) launch_stream<BF, -1>(g, TokenArgs{}, st);
+  else if ((g.M + 255) / 256 * ((g.N + 255) / 256) >= 160) launch_tiles<4, 4, BF>(g, st);
+  else launch_tiles<2, 2, BF>(g, st);
+}
+
+bool known(int dtype) { return dtype == LCQ_F32 || dtype == LCQ_BF16 || dtype == LCQ_F16; }
+
+int check(const int8_t* w, const void* ws, int ws_dtype, const void* bias, int bias_dtype, int64_t M, int64_t N, int64_t K, const void* y, int dtype) {
+  if (!w || !ws || !y || M <= 0 || N <= 0 || K <= 0) return LCQ_EINVAL;
+  if (!known(dtype) || !known(ws_dtype) || (bias && !known(bias_dtype))) return LCQ_EDTYPE;
+  if (K > 65536 || (M + 127) / 128 * ((N + 127) / 128) > 0x7ffffff0) return LCQ_ESIZE;
+  if (K % 16 == 0 && (uintptr_t)w % 16) return LCQ_EALIGN;
+  return LCQ_OK;
+}
+
+// tokens whose codes the product makes itself
+bool fused(int64_t M, int64_t K) { return M <= MOST_FUSED && K % 16 == 0 && M * K <= MOST_FUSED_CODES; }
+int64_t on256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
 }  // namespace
 
 extern "C" {
@@ -278,10 +470,9 @@ int64_t lcq_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K) {
 int lcq_int8_matmul(const int8_t* a, const float* as, int a_scalar, const int32_t* az, const int8_t* w, const void* ws, int ws_dtype,
                     int w_scalar, const void* bias, int bias_dtype, int64_t M, int64_t N, int64_t K, void* y, int dtype,
                     void* workspace, void* stream) {
-  if (!a || !as || !w || !ws || !y || M <= 0 || N <= 0 || K <= 0) return LCQ_EINVAL;
-  const auto known = [](int d) { return d == LCQ_F32 || d == LCQ_BF16 || d == LCQ_F16; };
-  if (!known(dtype) || !known(ws_dtype) || (bias && !known(bias_dtype))) return LCQ_EDTYPE;
-  if (K > 65536 || (M + 127) / 128 * ((N + 127) / 128) > 0x7ffffff0) return LCQ_ESIZE;
+  if (!a || !as) return LCQ_EINVAL;
+  const int bad = check(w, ws, ws_dtype, bias, bias_dtype, M, N, K, y, dtype);
+  if (bad) return bad;
   hipStream_t st = (hipStream_t)stream;
   MatmulArgs g = {a, w, as, az, ws, bias, y, M, N, K, K, (int)K, ws_dtype, bias_dtype, a_scalar, w_scalar};
   if (K % 16) {
@@ -294,20 +485,53 @@ int lcq_int8_matmul(const int8_t* a, const float* as, int a_scalar, const int32_
     pad_kernel<<<grid(M), dim3(256), 0, st>>>(a, M, (int)K, Kp, pa);
     pad_kernel<<<grid(N), dim3(256), 0, st>>>(w, N, (int)K, Kp, pw);
     g.a = pa; g.w = pw; g.lda = g.ldw = g.K = Kp;
-  } else if ((uintptr_t)a % 16 || (uintptr_t)w % 16) {
+  } else if ((uintptr_t)a % 16) {
     return LCQ_EALIGN;
   }
-  const auto run = [&](auto big) {
-    constexpr bool BIG = decltype(big)::value;
-    constexpr int F = BIG ? 4 : 2;
-    if (dtype == LCQ_BF16) launch_tiles<F, F, ROW_BF16>(g, st);
-    else if (dtype == LCQ_F16) launch_tiles<F, F, ROW_F16>(g, st);
-    else launch_tiles<F, F, ROW_F32>(g, st);
-  };
-  if ((M + 255) / 256 * ((N + 255) / 256) >= 160) run(std::true_type{});
-  else run(std::false_type{});
+  if (dtype == LCQ_BF16) launch_codes<ROW_BF16>(g, st);
+  else if (dtype == LCQ_F16) launch_codes<ROW_F16>(g, st);
+  else launch_codes<ROW_F32>(g, st);
   LCQ_CHECK_LAUNCH();
   return LCQ_OK;
+}
+
+int64_t lcq_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0 || K > 65536 || fused(M, K)) return 0;
+  return on256(M * K) + on256(8 * M) + lcq_int8_matmul_workspace_bytes(M, N, K);
+}
+
+int lcq_int8_linear(const void* x, int x_dtype, int64_t ldx, int asym, const float* scale, const int8_t* w, const void* ws, int ws_dtype,
+                    int w_scalar, const void* bias, int bias_dtype, int64_t M, int64_t N, int64_t K, void* y, int dtype,
+                    void* workspace, void* stream) {
+  if (!x || ldx < 0 || (asym && scale)) return LCQ_EINVAL;
+  const int bad = check(w, ws, ws_dtype, bias, bias_dtype, M, N, K, y, dtype);
+  if (bad) return bad;
+  if (!known(x_dtype)) return LCQ_EDTYPE;
+  if (fused(M, K)) {
+    hipStream_t st = (hipStream_t)stream;
+    const MatmulArgs g = {nullptr, w, nullptr, nullptr, ws, bias, y, M, N, K, K, (int)K, ws_dtype, bias_dtype, 0, w_scalar};
+    const TokenArgs t = {x, scale, ldx, asym};
+    const auto run = [&](auto xt) {
+      constexpr int XT = decltype(xt)::value;
+      if (dtype == LCQ_BF16) launch_stream<ROW_BF16, XT>(g, t, st);
+      else if (dtype == LCQ_F16) launch_stream<ROW_F16, XT>(g, t, st);
+      else launch_stream<ROW_F32, XT>(g, t, st);
+    };
+    if (x_dtype == LCQ_BF16) run(std::integral_constant<int, ROW_BF16>{});
+    else if (x_dtype == LCQ_F16) run(std::integral_constant<int, ROW_F16>{});
+    else run(std::integral_constant<int, ROW_F32>{});
+    LCQ_CHECK_LAUNCH();
+    return LCQ_OK;
+  }
+  if (!workspace) return LCQ_EWORKSPACE;
+  if ((uintptr_t)workspace % 16) return LCQ_EALIGN;
+  int8_t* const codes = (int8_t*)workspace;
+  float* const scales = (float*)(codes + on256(M * K));
+  int32_t* const zeros = asym ? (int32_t*)(scales + M) : nullptr;
+  const int rc = lcq_quant_tokens(x, x_dtype, M, K, ldx, asym, scale, codes, scales, zeros, stream);
+  if (rc) return rc;
+  return lcq_int8_matmul(codes, scale ? scale : scales, scale != nullptr, zeros, w, ws, ws_dtype, w_scalar, bias, bias_dtype, M, N, K, y, dtype,
+                         (char*)scales + on256(8 * M), stream);
 }
 
 }  // extern "C"

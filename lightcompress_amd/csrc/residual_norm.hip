@@ -6,18 +6,13 @@
 //   rms:   norm(v) = v / sqrt(mean v^2 + eps) * (w + offset) + bias
 //   layer: norm(v) = (v - mean) / sqrt(mean (v - mean)^2 + eps) * (w + offset) + bias
 //
-// and the int8 codes of a token by themselves (lcq_quant_tokens: the same rows without norm and residual):
-//
-//   symmetric   s = max(max |y|, 1e-5) / 127         q = clamp(rint(y / s), -128, 127)
-//   asymmetric  s = max(max y - min y, 1e-5) / 255   z = clamp(-128 - rint(min y / s), -128, 127)
-//               q = clamp(rint(y / s) + z, -128, 127)
-//   given scale q = clamp(rint(y / s), -128, 127)
+// and the int8 codes of a token by themselves (lcq_quant_tokens: the same rows without norm and residual; token_codes.h).
 //
 // Everything between the loads and the stores is in 32 bits: y is taken from h before h is rounded to the stream's type, codes
 // from y before any rounding.  The quantizer arithmetic is IntegerQuantizer's (quant.py:544-558, 698-716) on fp32 rows with
 // granularity per_token, codes moved to int8 (its unsigned codes less 128).
 #include "rowquant.h"
-#include "divisor.h"
+#include "token_codes.h"
 
 namespace {
 using namespace lcq;
@@ -170,50 +165,31 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void residual_norm_kernel(
   if (a.out) each([&](int i, float* e) { store_v<BF, V>(a.out, r * K + i, flags & LCQ_NORM_OUT_F32, e); });
   if (!a.codes) return;
 
-  float s, z = 0.0f;
-  bool bounded = true;                              // |y / s| stays far from the largest fp32 number
-  if (a.scale_in) {
-    bounded = false;
-    s = a.scale_in[0];
-  } else if (flags & LCQ_NORM_ASYM) {
-    const float inf = __builtin_inff();
-    float hi = -inf, lo = inf;
-    each([&](int, float* e) {
-      #pragma unroll
-      for (int j = 0; j < V; ++j) { hi = nan_max(hi, e[j]); lo = nan_min(lo, e[j]); }
-    });
-    hi = row_.template reduce<1>(hi);
-    lo = row_.template reduce<2>(lo);
-    s = nan_max(hi - lo, 1e-5f) / 255.0f;
-    z = fminf(fmaxf(-128.0f - rintf(lo / s), -128.0f), 127.0f);
-    bounded = fmaxf(fabsf(hi), fabsf(lo)) < 1e30f;  // (s >= 1e-5 / 255: a narrow range far from zero)
-  } else {
+  const auto make = [&]() -> TokenCodes {
+    if (a.scale_in) return TokenCodes::given(a.scale_in[0]);
+    if (flags & LCQ_NORM_ASYM) {
+      float hi = -__builtin_inff(), lo = __builtin_inff();
+      each([&](int, float* e) {
+        #pragma unroll
+        for (int j = 0; j < V; ++j) { hi = nan_max(hi, e[j]); lo = nan_min(lo, e[j]); }
+      });
+      hi = row_.template reduce<1>(hi);
+      return TokenCodes::asymmetric(row_.template reduce<2>(lo), hi);
+    }
     float m = 0.0f;
     each([&](int, float* e) {
       #pragma unroll
       for (int j = 0; j < V; ++j) m = nan_max(m, fabsf(e[j]));
     });
-    m = row_.template reduce<1>(m);
-    s = nan_max(m, 1e-5f) / 127.0f;
-  }
-  Divisor d(s);
-  d.fast = d.fast && bounded;
+    return TokenCodes::symmetric(row_.template reduce<1>(m));
+  };
+  const TokenCodes q = make();
   each([&](int i, float* e) {
-    int q[V];
-    #pragma unroll
-    for (int j = 0; j < V; ++j) q[j] = (int)fminf(fmaxf(rintf(d.quotient(e[j])) + z, -128.0f), 127.0f);
-    if constexpr (V == 1) {
-      a.codes[r * K + i] = (int8_t)q[0];
-    } else {
-      u32x2 w;
-      #pragma unroll
-      for (int p = 0; p < 2; ++p)
-        w[p] = (uint32_t)(q[4 * p] & 255) | (uint32_t)(q[4 * p + 1] & 255) << 8 | (uint32_t)(q[4 * p + 2] & 255) << 16 | (uint32_t)q[4 * p + 3] << 24;
-      *(u32x2*)(a.codes + r * K + i) = w;
-    }
+    if constexpr (V == 1) a.codes[r * K + i] = (int8_t)q.code(e[0]);
+    else *(u32x2*)(a.codes + r * K + i) = u32x2{q.codes(e), q.codes(e + 4)};
   });
-  if (t == 0 && a.scales) a.scales[r] = s;
-  if (t == 0 && a.zeros) a.zeros[r] = (int)z;
+  if (t == 0 && a.scales) a.scales[r] = q.d.s;
+  if (t == 0 && a.zeros) a.zeros[r] = (int)q.z;
 }
 
 template <int BF, int V, int TEAM, int CH>

@@ -62,18 +62,23 @@ def _cols(x):
     return x.shape[-1]
 
 
+def _given(scale, symmetric):
+    if scale is None:
+        return None
+    if not symmetric:
+        raise ValueError('a given scale is a symmetric one')
+    if scale.numel() != 1:
+        raise ValueError(f'one scale for all tokens, got {tuple(scale.shape)}')
+    return scale.reshape(1).float()
+
+
 @torch.no_grad()
 def quantize_tokens(x, symmetric=True, scale=None):
     """Int8 codes of the tokens x [..., K] (fp32, bf16, fp16), one fp32 scale per token (and, not symmetric, one zero
     point): QuantizedTokens.  `scale`: one given fp32 scale for all tokens (static activations, symmetric)."""
     K = _cols(x)
     code = L.dtype_code(x.dtype)
-    if scale is not None:
-        if not symmetric:
-            raise ValueError('a given scale is a symmetric one')
-        if scale.numel() != 1:
-            raise ValueError(f'one scale for all tokens, got {tuple(scale.shape)}')
-        scale = scale.reshape(1).float()
+    scale = _given(scale, symmetric)
     with _on(x, scale=scale):
         rows, T, ld = _rows(x, K)
         lead = x.shape[:-1]
@@ -136,7 +141,26 @@ def int8_matmul(tokens, weight, weight_scales, bias=None, out_dtype=torch.bfloat
 @torch.no_grad()
 def int8_linear(x, weight, weight_scales, bias=None, symmetric=True, scale=None, out_dtype=None):
     """A w8a8 Linear on x [..., K]: quantize_tokens(x, symmetric, scale), then int8_matmul to x's type (or `out_dtype`)."""
-    return int8_matmul(quantize_tokens(x, symmetric, scale), weight, weight_scales, bias, out_dtype or x.dtype)
+    K = _cols(x)
+    x_code = L.dtype_code(x.dtype)
+    out_dtype = out_dtype or x.dtype
+    code = L.dtype_code(out_dtype)
+    scale = _given(scale, symmetric)
+    N = _check_weight(weight, weight_scales, bias, K)
+    with _on(x, scale=scale, weight=weight, weight_scales=weight_scales, bias=bias):
+        rows, M, ld = _rows(x, K)
+        if K % 16 == 0:                       # (other widths are copied to padded rows by the call itself)
+            weight = _on16(weight)
+        y = torch.empty((*x.shape[:-1], N), dtype=out_dtype, device=x.device)
+        if M and N:
+            lib = L.lib()
+            size = lib.lcq_int8_linear_workspace_bytes(M, N, K)
+            ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+            L.check(lib.lcq_int8_linear(rows.data_ptr(), x_code, ld, not symmetric, L.ptr(scale), L.ptr(weight), L.ptr(weight_scales),
+                                        L.dtype_code(weight_scales.dtype), weight_scales.numel() == 1, L.ptr(bias),
+                                        0 if bias is None else L.dtype_code(bias.dtype), M, N, K, y.data_ptr(), code, L.ptr(ws),
+                                        L.stream()), 'lcq_int8_linear')
+    return y
 
 
 def _affine(name, t, K, x, flag):

@@ -175,6 +175,22 @@ def test_product_off_alignment(dev, M, N, K):
         check_product(got, q, s, z, w, ws, None, F32)
 
 
+@pytest.mark.parametrize('dtype', [BF, HF, F32])
+@pytest.mark.parametrize('M,K', [(1, 1), (1, 16), (1, 4096), (1, 16400), (1, 40960), (1, 40976), (1, 65536), (2, 1040), (3, 4096), (4, 10240), (4, 10256), (4, 1000),
+                                 (5, 512), (16, 4096), (33, 1024), (300, 528)])
+def test_linear_is_codes_and_product(dev, M, K, dtype):
+    """However few the tokens, however they lie: the same bits as by the codes."""
+    g = gen(M + K)
+    w = torch.randint(-128, 128, (72, K), generator=g, dtype=torch.int8).to(dev)
+    ws, b = (0.01 * torch.rand(72, 1, generator=g)).to(dev), torch.randn(72, generator=g).to(dev)
+    wide = acts(M, K + 24, dtype, seed=K, shift=0.2).to(dev)
+    for x in (wide[:, :K], wide[:, 3:K + 3], wide[:, :K].contiguous()):
+        for kw in (dict(symmetric=True), dict(symmetric=False), dict(scale=torch.tensor([0.03], device=dev))):
+            want = int8_matmul(quantize_tokens(x, **kw), w, ws, b, out_dtype=F32)
+            assert_bit_equal(int8_linear(x, w, ws, b, out_dtype=F32, **kw), want, f'{kw}')
+        assert int8_linear(x, w, ws).dtype == dtype
+
+
 def test_product_shapes_and_nothing(dev):
     q, s, _, w, ws, _ = product_inputs(6, 40, 128, False, False, dev=dev)
     flat = int8_matmul(QuantizedTokens(q, s), w, ws)
