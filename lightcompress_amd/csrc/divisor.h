@@ -16,11 +16,14 @@ struct Divisor {
     const float y0 = __builtin_amdgcn_rcpf(s);
     y = __builtin_fmaf(__builtin_fmaf(-s, y0, 1.0f), y0, y0);
   }
-  __device__ __forceinline__ float quotient(float x) const {
-    if (__builtin_expect(!fast, 0)) return x / s;
+  __device__ __forceinline__ float fast_quotient(float x) const {            // where `fast`
     float q = x * y;                                         // (s q - x taken off, not x - s q added: that way -0 / s stays -0)
     q = __builtin_fmaf(-__builtin_fmaf(s, q, -x), y, q);
     return __builtin_fmaf(-__builtin_fmaf(s, q, -x), y, q);
+  }
+  __device__ __forceinline__ float quotient(float x) const {
+    if (__builtin_expect(!fast, 0)) return x / s;
+    return fast_quotient(x);
   }
 };
 

@@ -7,6 +7,7 @@
 // The weight is the first operand, so an accumulator's four neighbouring registers are four neighbouring channels of one token.
 #include "rowquant.h"
 #include "token_codes.h"
+#include "launch_rules.h"
 #include <type_traits>
 
 namespace {
@@ -16,6 +17,8 @@ typedef __attribute__((ext_vector_type(4))) int i32x4;
 typedef __attribute__((ext_vector_type(16))) int i32x16;
 typedef __attribute__((address_space(3))) char* lds_ptr;
 typedef __attribute__((address_space(3))) i32x4* lds_frag;
+
+template <int I> using Int = std::integral_constant<int, I>;
 
 struct MatmulArgs {
   const int8_t *a, *w;
@@ -30,6 +33,11 @@ struct MatmulArgs {
 __device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
   return dtype == LCQ_F32 ? load_scalar<ROW_F32>(p, i) : dtype == LCQ_BF16 ? load_scalar<ROW_BF16>(p, i) : load_scalar<ROW_F16>(p, i);
 }
+// the same in two steps, so that nothing waits for the load before the value is used
+__device__ __forceinline__ uint32_t load_raw(const void* p, int dtype, int64_t i) { return dtype == LCQ_F32 ? ((const uint32_t*)p)[i] : (uint32_t)((const uint16_t*)p)[i]; }
+__device__ __forceinline__ float from_raw(uint32_t u, int dtype) {
+  return dtype == LCQ_F32 ? u2f(u) : dtype == LCQ_BF16 ? u2f(u << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)u);
+}
 // the four byte sums of a register added to `sum`
 __device__ __forceinline__ int add_bytes(const i32x4& v, int sum) {
   #pragma unroll
@@ -39,24 +47,27 @@ __device__ __forceinline__ int add_bytes(const i32x4& v, int sum) {
 
 // ---- tiles --------------------------------------------------------------------------------------------------------
 // A workgroup of four waves (2 x 2) owns 64 FM tokens x 64 FN channels, a wave FM x FN accumulators of 32 x 32.
-//  * K streams through four LDS stages of 64 codes per row by direct loads; rows past the end of a matrix and codes past K lie outside the
-//    buffer that the loads are told and read as zero;
-//  * a row of a stage is 64 bytes, 16 bytes per lane of a load; piece p of row r lies at p ^ (r / 4 % 4), so that the 16 lanes of an
-//    operand read touch all 64 banks once;
-//  * operands are double-buffered in registers: while the products of one 32-code step run, the reads of the next are issued between
-//    them, and the direct loads of the stage three ahead are spread over them; one barrier per stage, at its middle, where every wave holds
-//    the rest of it in registers.
-constexpr int STAGES = 4, SLAB = 64;
+//  * K streams through LDS stages of 64 or 128 codes per row by direct loads; rows past the end of a matrix and codes past K lie outside
+//    the buffer that the loads are told and read as zero;
+//  * piece p of 16 bytes of row r lies at p ^ (r / 4 % 4) or p ^ (r / 2 % 8), so that 16 lanes of an operand read touch all 64 banks once;
+//  * operands are buffered in registers: while the products of one 32-code step run, the reads of a later one are issued between them;
+//    one barrier per stage, where every wave holds the rest of it in registers: its place is loaded again from there.
+constexpr int ROW_I32 = 3;                          // an output type: the sums of a part of K as they are
 
-template <int FM, int FN>
+template <int FM_, int FN_, int SLAB_, int STAGES_, int SETS_>
 struct Tile {
-  static constexpr int TM = 64 * FM, TN = 64 * FN;
+  static constexpr int FM = FM_, FN = FN_, SLAB = SLAB_, STAGES = STAGES_, SETS = SETS_;     // codes of a row per stage; sets of operands
+  static constexpr int TM = 64 * FM, TN = 64 * FN, STEPS = SLAB / 32;
   static constexpr int STAGE = (TM + TN) * SLAB;
 };
 
-template <int FM, int FN, int BF, bool ASYM>
-__global__ __launch_bounds__(256, 1) void tile_kernel(MatmulArgs g, int tiles_m, int tiles_n) {
-  typedef Tile<FM, FN> T;
+// 16-byte piece p of row r of a stage lies at p ^ swizzle(r)
+template <int SLAB>
+__device__ __forceinline__ int swizzle(int r) { return SLAB == 64 ? (r >> 2) & 3 : (r >> 1) & 7; }
+
+template <class T, int BF, bool ASYM>
+__global__ __launch_bounds__(256, 1) void tile_kernel(MatmulArgs g, int tiles_m, int tiles_n, int parts) {
+  constexpr int FM = T::FM, FN = T::FN, SLAB = T::SLAB, STAGES = T::STAGES, SETS = T::SETS, STEPS = T::STEPS;
   __shared__ __attribute__((aligned(1024))) char lds[STAGES * T::STAGE];
   __shared__ __attribute__((aligned(16))) float channel[2][T::TN];           // scales, biases
   __shared__ __attribute__((aligned(16))) int sums[ASYM ? T::TN : 4];        // sums of the weight's rows
@@ -66,11 +77,13 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MatmulArgs g, int tiles_m,
 
   // Workgroup b runs on XCD b % 8: every XCD takes a contiguous range of an order in which 32 consecutive tiles are 4 x 8, so the
   // tiles that share an L2 at one time share a handful of stripes.
-  int ti, tj;
+  int ti, tj, part;
   {
-    const int total = tiles_m * tiles_n, each = (total + 7) >> 3;
-    const int v = ((int)blockIdx.x & 7) * each + ((int)blockIdx.x >> 3);
+    const int total = tiles_m * tiles_n * parts, each = (total + 7) >> 3;
+    int v = ((int)blockIdx.x & 7) * each + ((int)blockIdx.x >> 3);
     if (((int)blockIdx.x >> 3) >= each || v >= total) return;
+    part = v / (tiles_m * tiles_n);
+    v -= part * tiles_m * tiles_n;
     const int group = v / (4 * tiles_n), first = group * 4, rows = tiles_m - first < 4 ? tiles_m - first : 4;
     const int in = v - group * 4 * tiles_n;
     tj = in / rows;
@@ -78,35 +91,46 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MatmulArgs g, int tiles_m,
   }
   const int64_t m0 = (int64_t)ti * T::TM, n0 = (int64_t)tj * T::TN;
   const int rows_a = (int)(g.M - m0 < T::TM ? g.M - m0 : T::TM), rows_w = (int)(g.N - n0 < T::TN ? g.N - n0 : T::TN);
-  const int steps = (g.K + SLAB - 1) / SLAB;
+  const int slabs = (g.K + SLAB - 1) / SLAB;
+  const int begin = (int)((int64_t)slabs * part / parts), steps = (int)((int64_t)slabs * (part + 1) / parts) - begin;
 
   const auto buffer = [&](const int8_t* p, int64_t ld, int rows) {
     const uint64_t at = (uint64_t)(uintptr_t)p;
-    return i32x4{(int)(uint32_t)at, (int)(uint32_t)(at >> 32) & 0xffff, (int)((rows - 1) * ld + g.K), 0x00020000};
+    const auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    return i32x4{one((int)(uint32_t)at), one((int)(uint32_t)(at >> 32) & 0xffff), one((int)((rows - 1) * ld + g.K)), 0x00020000};
   };
   const i32x4 bufA = buffer(g.a + m0 * g.lda, g.lda, rows_a), bufW = buffer(g.w + n0 * g.ldw, g.ldw, rows_w);
   constexpr uint32_t OUTSIDE = 0x80000000u;
-  constexpr int LA = T::TM / 64, LW = T::TN / 64;   // a wave's loads of tokens and of weights per stage
-  const int piece16 = ((lane & 3) ^ ((lane >> 4) & 3)) * 16;                 // this lane's 16 bytes of a row of 64
+  constexpr int ROWS = 1024 / SLAB, LANES = 64 / ROWS;                       // of a load
+  constexpr int LA = T::TM / (4 * ROWS), LW = T::TN / (4 * ROWS);            // a wave's loads of tokens and of weights per stage
+  static_assert(SLAB == 64 || (LA % 2 == 0 && LW % 2 == 0), "a wave's loads start with an even one");
+  // this lane's 16 bytes of a row: of an even load, and of an odd one (the same for 64 codes)
+  int piece16[2];
+  #pragma unroll
+  for (int e = 0; e < 2; ++e) piece16[e] = ((lane % LANES) ^ swizzle<SLAB>(e * ROWS + lane / LANES)) * 16;
   uint32_t gof[LA + LW];
   #pragma unroll
   for (int p = 0; p < LA + LW; ++p) {
-    const int r = (wave * (p < LA ? LA : LW) + (p < LA ? p : p - LA)) * 16 + (lane >> 2);
-    gof[p] = r < (p < LA ? rows_a : rows_w) ? (uint32_t)(r * (p < LA ? g.lda : g.ldw) + piece16) : OUTSIDE;
+    const int r = (wave * (p < LA ? LA : LW) + (p < LA ? p : p - LA)) * ROWS + lane / LANES;
+    gof[p] = r < (p < LA ? rows_a : rows_w) ? (uint32_t)(r * (p < LA ? g.lda : g.ldw) + piece16[p & 1]) : OUTSIDE;
   }
   const uint32_t lds0 = (uint32_t)(size_t)(lds_ptr)lds;
-  // load p of the stage at LDS address dst, codes [at, at + 64) of K
-  const auto gload = [&](uint32_t dst, int at, uint32_t outside, int p) {
+  struct Outside { uint32_t of[2]; };
+  // load p of the stage at LDS address dst, codes [at, at + SLAB) of K
+  const auto gload = [&](uint32_t dst, int at, const Outside& outside, int p) {
     const uint32_t to = dst + (p < LA ? (wave * LA + p) * 1024 : T::TM * SLAB + (wave * LW + p - LA) * 1024);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                 ::"s"(to), "v"(gof[p] | outside), "s"(p < LA ? bufA : bufW), "s"(at) : "memory");
+                 ::"s"(to), "v"(gof[p] | outside.of[p & 1]), "s"(p < LA ? bufA : bufW), "s"(at) : "memory");
   };
-  const auto outside_at = [&](int at) { return piece16 < g.K - at ? 0u : OUTSIDE; };
+  const auto outside_at = [&](int at) { return Outside{{piece16[0] < g.K - at ? 0u : OUTSIDE, piece16[1] < g.K - at ? 0u : OUTSIDE}}; };
 
-  const int slot = (lane >> 5) ^ ((lane >> 2) & 3);
+  // step ks reads pieces 2 ks (lanes 0 .. 31) and 2 ks + 1 of a row
+  const int slot = (lane >> 5) ^ swizzle<SLAB>(lane & 31);
   const lds_ptr readA = (lds_ptr)lds + (wr * FM * 32 + (lane & 31)) * SLAB + slot * 16;
   const lds_ptr readW = (lds_ptr)lds + T::TM * SLAB + (wc * FN * 32 + (lane & 31)) * SLAB + slot * 16;
-  const int second = ((slot ^ 2) - slot) * 16;      // from the first 32 codes of a stage to the others
+  int step_at[STEPS];                               // from the first 32 codes of a stage to the others
+  #pragma unroll
+  for (int ks = 0; ks < STEPS; ++ks) step_at[ks] = ((slot ^ (2 * ks)) - slot) * 16;
   i32x16 acc[FN][FM];
   #pragma unroll
   for (int j = 0; j < FN; ++j)
@@ -115,67 +139,88 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MatmulArgs g, int tiles_m,
       #pragma unroll
       for (int r = 0; r < 16; ++r) acc[j][i][r] = 0;
   int wsum[FN] = {};
-  i32x4 fr[2][FN + FM];                             // two sets of operands: weights, tokens
-  const auto rd = [&](int set, int f, uint32_t stage, int ks) {
-    fr[set][f] = *(lds_frag)((f < FN ? readW + f * 32 * SLAB : readA + (f - FN) * 32 * SLAB) + stage + (ks ? second : 0));
+  i32x4 fr[SETS][FN + FM];                          // operands of 32 codes: weights, tokens
+  const auto rd = [&](int set, int ks, int f, uint32_t stage) {
+    fr[set][f] = *(lds_frag)((f < FN ? readW + f * 32 * SLAB : readA + (f - FN) * 32 * SLAB) + stage + step_at[ks]);
   };
-  constexpr int PRODUCTS = FM * FN, HALF = (LA + LW) / 2;
-  const auto products = [&](int set, auto&& read, auto&& load) {
-    #pragma unroll
-    for (int m = 0; m < PRODUCTS; ++m) {
-      const int i = m % FM, j = m / FM;
-      acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fr[set][j], fr[set][FN + i], acc[j][i], 0, 0, 0);
-      if (ASYM && i == 0) wsum[j] = add_bytes(fr[set][j], wsum[j]);
-      // the operand reads in the first three quarters of the products, the loads spread over all of them
-      #pragma unroll
-      for (int f = 0; f < FN + FM; ++f)             // in the order in which the products need them
-        if (f * PRODUCTS * 3 / 4 / (FN + FM) == m) read(f == 0 ? 0 : f <= FM ? FN + f - 1 : f - FM);
-      #pragma unroll
-      for (int p = 0; p < HALF; ++p)
-        if ((p + 1) * PRODUCTS / HALF - 1 == m) load(p);
-      __builtin_amdgcn_sched_barrier(0);
+  // What the outputs need besides the sums, on its way during the products (used behind them, so no wait counts it).
+  float as[FM];
+  uint32_t chan[2] = {};
+  int az[FM] = {};
+  if constexpr (BF != ROW_I32) {
+    if (tid < rows_w) {
+      chan[0] = load_raw(g.ws, g.ws_dtype, g.w_scalar ? 0 : n0 + tid);
+      if (g.bias) chan[1] = load_raw(g.bias, g.bias_dtype, n0 + tid);
     }
-  };
-
-  constexpr int LOADS = LA + LW;
-  #pragma unroll
-  for (int s = 0; s < STAGES; ++s) {
-    const uint32_t outside = outside_at(s * SLAB);
-    #pragma unroll
-    for (int p = 0; p < (s == STAGES - 1 ? HALF : LOADS); ++p) gload(lds0 + s * T::STAGE, s * SLAB, outside, p);
   }
-  constexpr int FIRST = (STAGES - 1) * LOADS - LOADS + HALF, LATER = (STAGES - 2) * LOADS;
-  __builtin_amdgcn_s_waitcnt(0x0F70 | (FIRST & 15) | ((FIRST >> 4) << 14));
-  __syncthreads();
   #pragma unroll
-  for (int f = 0; f < FN + FM; ++f) rd(0, f, 0, 0);
-  uint32_t cur = 0, dst = lds0 + (STAGES - 1) * T::STAGE;
-  int at = (STAGES - 1) * SLAB;
-  uint32_t outside = outside_at(at);
+  for (int i = 0; i < FM; ++i) {
+    const int m = wr * FM * 32 + i * 32 + (lane & 31), at = m < rows_a ? m : rows_a - 1;       // (a token past the last one is not stored)
+    as[i] = BF != ROW_I32 ? g.as[g.a_scalar ? 0 : m0 + at] : 0.0f;
+    if (ASYM) az[i] = g.az[m0 + at];
+  }
   __builtin_amdgcn_sched_barrier(0);
-  for (int s = 0; s < steps; ++s) {
-    // the first 32 codes of the stage; meanwhile the reads of the others, and the second half of the loads three stages ahead
-    products(0, [&](int f) { rd(1, f, cur, 1); }, [&](int p) { gload(dst, at, outside, HALF + p); });
-    // The next stage has landed (the loads of the two behind it may be in flight) and this one is in registers, in every wave: its place
-    // takes the stage four ahead.
-    __builtin_amdgcn_s_waitcnt(0x0070 | (LATER & 15) | ((LATER >> 4) << 14));
+
+  constexpr int LOADS = LA + LW, PRODUCTS = FM * FN, READS = FN + FM;
+  // The reads run SETS - 1 steps ahead of the products, so in front of step SWITCH of a stage the rest of it is in registers.  There is its
+  // barrier: its place is free, and the stage STAGES ahead is loaded there during the next STEPS steps.
+  constexpr int SWITCH = STEPS - (SETS - 1);
+  static_assert(SWITCH >= 1 && STEPS % SETS == 0, "operand sets");
+  const auto wait = [&](auto in_flight_) {          // for all loads but the youngest, and for the operands; then for the other waves
+    constexpr int in_flight = decltype(in_flight_)::value;
+    static_assert(in_flight < 64, "loads in flight");
+    __builtin_amdgcn_s_waitcnt(0x0070 | (in_flight & 15) | ((in_flight >> 4) << 14));
     asm volatile("s_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    const uint32_t nxt = cur == (STAGES - 1) * T::STAGE ? 0 : cur + T::STAGE;
-    dst = lds0 + cur;
-    at += SLAB;
-    outside = outside_at(at);
-    products(1, [&](int f) { rd(0, f, nxt, 0); }, [&](int p) { gload(dst, at, outside, p); });
-    cur = nxt;
+  };
+  constexpr int AHEAD = (STAGES - 1) * LOADS + LOADS * (STEPS - SWITCH) / STEPS;             // loads in front of the first product
+  #pragma unroll
+  for (int l = 0; l < AHEAD; ++l) {
+    const int k = (begin + l / LOADS) * SLAB;
+    gload(lds0 + l / LOADS * T::STAGE, k, outside_at(k), l % LOADS);
   }
+  wait(Int<AHEAD - LOADS>{});
+  #pragma unroll
+  for (int st = 0; st < SETS - 1; ++st)
+    #pragma unroll
+    for (int f = 0; f < READS; ++f) rd(st, st, f, 0);
+  __builtin_amdgcn_sched_barrier(0);
+  uint32_t cur = 0, dst = lds0 + (STAGES - 1) * T::STAGE;
+  int at = (begin + STAGES - 1) * SLAB, s = 0;
+  Outside outside = outside_at(at);
+  do {                                              // (a part has at least one stage)
+    const uint32_t nxt = cur == (STAGES - 1) * T::STAGE ? 0 : cur + T::STAGE;
+    #pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      if (st == SWITCH) {
+        wait(Int<(STAGES - 2) * LOADS>{});          // the next stage has landed; the loads of those behind it may be in flight
+        dst = lds0 + cur;
+        at += SLAB;
+        outside = outside_at(at);
+      }
+      const int set = st % SETS, after = (st + STEPS - SWITCH) % STEPS, l0 = LOADS * after / STEPS, l1 = LOADS * (after + 1) / STEPS;
+      #pragma unroll
+      for (int m = 0; m < PRODUCTS; ++m) {
+        const int j = m / FM, i = m % FM;
+        acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fr[set][j], fr[set][FN + i], acc[j][i], 0, 0, 0);
+        if (ASYM && i == 0) wsum[j] = add_bytes(fr[set][j], wsum[j]);
+        // the reads in the first three quarters of the products and in their order, the loads spread over all of them
+        #pragma unroll
+        for (int f = 0; f < READS; ++f)
+          if (f * PRODUCTS * 3 / 4 / READS == m)
+            rd((st + SETS - 1) % SETS, (st + SETS - 1) % STEPS, f == 0 ? 0 : f <= FM ? FN + f - 1 : f - FM, st < SWITCH ? cur : nxt);
+        #pragma unroll
+        for (int p = 0; p < LOADS; ++p)
+          if (p >= l0 && p < l1 && (p - l0 + 1) * PRODUCTS / (l1 - l0) - 1 == m) gload(dst, at, outside, p);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    cur = nxt;
+  } while (++s < steps);
   __builtin_amdgcn_s_waitcnt(0x0070);               // nothing may still be on its way to LDS when it is used again
 
   // ---- outputs: register r of lane l is channel 8 (r / 4) + 4 (l / 32) + r % 4 of token l % 32 ----
-  for (int c = tid; c < T::TN; c += 256) {
-    const int64_t n = n0 + c;
-    channel[0][c] = c < rows_w ? load_any(g.ws, g.ws_dtype, g.w_scalar ? 0 : n) : 0.0f;
-    channel[1][c] = c < rows_w && g.bias ? load_any(g.bias, g.bias_dtype, n) : 0.0f;
-  }
+  if (BF != ROW_I32 && tid < T::TN) { channel[0][tid] = from_raw(chan[0], g.ws_dtype); channel[1][tid] = from_raw(chan[1], g.bias_dtype); }
   if (ASYM && wr == 0) {
     #pragma unroll
     for (int j = 0; j < FN; ++j) {
@@ -184,45 +229,54 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MatmulArgs g, int tiles_m,
     }
   }
   __syncthreads();
-  // A wave's outputs leave through its own part of LDS, 16 bytes per lane along a token: 32 or (fp32) 64 bytes of a token's row per
-  // accumulator; chunk c of 16 bytes of token t lies at c ^ t.
-  constexpr int E = BF == ROW_F32 ? 4 : 2, CH = 16 / E;                      // bytes of an output, outputs of a chunk
+  // A wave's outputs leave through its own part of LDS, 16 bytes per lane along a token; chunk c of 16 bytes of token t lies at c ^ t.
+  constexpr int E = BF == ROW_F32 || BF == ROW_I32 ? 4 : 2, CH = 16 / E;     // bytes of an output, outputs of a chunk
   constexpr int ROW = FN * 32 * E, CHUNKS = ROW / 16;
-  char* const mine = lds + wave * 32 * ROW;
+  constexpr int STEP = E == 4 && FM > 1 ? FM / 2 : FM;                       // blocks of 32 tokens that leave together
+  static_assert(4 * STEP * 32 * ROW <= STAGES * T::STAGE, "outputs on their way out");
+  char* const mine = lds + wave * STEP * 32 * ROW;
   const int t = lane & 31, h = lane >> 5;
   const bool wide = (uintptr_t)g.y % 16 == 0 && (g.N * E) % 16 == 0;
   #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int m = wr * FM * 32 + i * 32;            // token 0 of these 32, in the tile
-    const bool in = m + t < rows_a;
-    const float as = in ? g.as[g.a_scalar ? 0 : m0 + m + t] : 0.0f;
-    const int az = ASYM && in ? g.az[m0 + m + t] : 0;
+  for (int i0 = 0; i0 < FM; i0 += STEP) {
     #pragma unroll
-    for (int j = 0; j < FN; ++j)
+    for (int j = 0; j < FN; ++j) {
+      // (the accumulators stay where they are until their turn: copied out together they would not fit the other registers)
+      if constexpr (FM * FN > 8) {
+        #pragma unroll
+        for (int i = i0; i < i0 + STEP; ++i) asm volatile("" : "+a"(acc[j][i]));
+      }
       #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int c = j * 32 + 8 * q + 4 * h;       // first of four channels, in the wave
-        const f32x4 ws = *(const f32x4*)&channel[0][wc * FN * 32 + c], b = *(const f32x4*)&channel[1][wc * FN * 32 + c];
-        float v[4];
+        f32x4 ws, b;
+        i32x4 sum;
+        if constexpr (BF != ROW_I32) { ws = *(const f32x4*)&channel[0][wc * FN * 32 + c]; b = *(const f32x4*)&channel[1][wc * FN * 32 + c]; }
+        if constexpr (ASYM) sum = *(const i32x4*)&sums[wc * FN * 32 + c];
         #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          int s = acc[j][i][4 * q + r];
-          if (ASYM) s -= az * sums[wc * FN * 32 + c + r];
-          v[r] = (float)s * (as * ws[r]) + b[r];
+        for (int i = i0; i < i0 + STEP; ++i) {
+          float v[4];
+          #pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            int s = acc[j][i][4 * q + r];
+            if constexpr (ASYM) s -= az[i] * sum[r];
+            v[r] = BF == ROW_I32 ? __builtin_bit_cast(float, s) : __builtin_fmaf((float)s, as[i] * ws[r], b[r]);
+          }
+          char* const to = mine + ((i - i0) * 32 + t) * ROW + (((c / CH) ^ t) % CHUNKS) * 16 + (c % CH) * E;
+          if constexpr (E == 4) *(f32x4*)to = f32x4{v[0], v[1], v[2], v[3]};
+          else if constexpr (BF == ROW_BF16) *(u32x2*)to = u32x2{bf16_pack_rne(v[0], v[1]), bf16_pack_rne(v[2], v[3])};
+          else *(u32x2*)to = u32x2{f16_pack_rne(v[0], v[1]), f16_pack_rne(v[2], v[3])};
         }
-        char* const to = mine + t * ROW + (((c / CH) ^ t) % CHUNKS) * 16 + (c % CH) * E;
-        if constexpr (BF == ROW_F32) *(f32x4*)to = f32x4{v[0], v[1], v[2], v[3]};
-        else if constexpr (BF == ROW_BF16) *(u32x2*)to = u32x2{bf16_pack_rne(v[0], v[1]), bf16_pack_rne(v[2], v[3])};
-        else *(u32x2*)to = u32x2{f16_pack_rne(v[0], v[1]), f16_pack_rne(v[2], v[3])};
       }
-    asm volatile("" ::: "memory");                // (LDS serves a wave in order)
+    }
+    asm volatile("" ::: "memory");                  // (LDS serves a wave in order)
     #pragma unroll
-    for (int o = 0; o < 32 * CHUNKS / 64; ++o) {
+    for (int o = 0; o < STEP * 32 * CHUNKS / 64; ++o) {
       const int idx = o * 64 + lane, tt = idx / CHUNKS, ch = idx % CHUNKS;
       const u32x4 v = *(const u32x4*)(mine + tt * ROW + ((ch ^ tt) % CHUNKS) * 16);
-      const int n = wc * FN * 32 + ch * CH;
-      if (m + tt >= rows_a || n >= rows_w) continue;
-      const int64_t cell = (m0 + m + tt) * g.N + n0 + n;
+      const int m = wr * FM * 32 + i0 * 32 + tt, n = wc * FN * 32 + ch * CH;
+      if (m >= rows_a || n >= rows_w) continue;
+      const int64_t cell = (m0 + m) * g.N + n0 + n + (BF == ROW_I32 ? part * g.M * g.N : 0);
       if (wide && n + CH <= rows_w) {
         *(u32x4*)((char*)g.y + cell * E) = v;
       } else {
@@ -238,16 +292,46 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MatmulArgs g, int tiles_m,
   }
 }
 
+// The parts of K added up, scaled and rounded: sums [parts, M, N], V channels of a token per lane.
+template <int BF, int V>
+__global__ __launch_bounds__(256) void join_kernel(MatmulArgs g, const int* __restrict__ sums, int parts) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V, all = g.M * g.N;
+  if (i >= all) return;
+  const int64_t m = i / g.N, n = i - m * g.N;
+  int s[V] = {};
+  for (int p = 0; p < parts; ++p) {
+    if constexpr (V == 4) {
+      const i32x4 v = *(const i32x4*)(sums + p * all + i);
+      #pragma unroll
+      for (int e = 0; e < V; ++e) s[e] += v[e];
+    } else {
+      s[0] += sums[p * all + i];
+    }
+  }
+  const float as = g.as[g.a_scalar ? 0 : m];
+  float v[V];
+  #pragma unroll
+  for (int e = 0; e < V; ++e)
+    v[e] = __builtin_fmaf((float)s[e], as * load_any(g.ws, g.ws_dtype, g.w_scalar ? 0 : n + e), g.bias ? load_any(g.bias, g.bias_dtype, n + e) : 0.0f);
+  if constexpr (V == 4) {
+    if constexpr (BF == ROW_F32) *(f32x4*)((float*)g.y + i) = f32x4{v[0], v[1], v[2], v[3]};
+    else if constexpr (BF == ROW_BF16) *(u32x2*)((uint16_t*)g.y + i) = u32x2{bf16_pack_rne(v[0], v[1]), bf16_pack_rne(v[2], v[3])};
+    else *(u32x2*)((uint16_t*)g.y + i) = u32x2{f16_pack_rne(v[0], v[1]), f16_pack_rne(v[2], v[3])};
+  } else {
+    if constexpr (BF == ROW_F32) ((float*)g.y)[i] = v[0];
+    else store_scalar<BF>(g.y, i, rnd<BF>(v[0]));
+  }
+}
+
 // ---- few tokens ---------------------------------------------------------------------------------------------------
 // The weight is read once, straight into the matrix pipe's operands: a lane of v_mfma_i32_16x16x64_i8 takes 16 codes of one of 16
 // channels, so a load of the wave is 16 rows x 64 bytes in a row.  A workgroup owns 16 channels, its eight waves take pieces of 256
-// codes of K in turn and meet in LDS; two pieces (8 KiB of weight per wave) are in flight.  The tokens' codes come from the cache, every
+// codes of K in turn and meet in LDS; three pieces (12 KiB of weight per wave) are in flight.  The tokens' codes come from the cache, every
 // wave other ones.
-// x: the tokens as values (at most MOST_FUSED of them): every workgroup makes their codes itself, in LDS, while its first weights are on
-// their way - cheaper for one token than another kernel in front.
-constexpr int STREAM_THREADS = 512, STREAM_WAVES = STREAM_THREADS / 64, PIECE = 256;
-constexpr int MOST_FUSED = 4;
-constexpr int64_t MOST_FUSED_CODES = 40960;         // in LDS
+// A single token may come as values: every workgroup makes its codes itself, in LDS, while its first weights are on their way - cheaper
+// than another kernel in front.
+constexpr int PIECE = 256;
+constexpr int64_t MOST_FUSED = 32768;               // codes of a token that is quantized in LDS
 
 struct TokenArgs {
   const void* x;
@@ -256,137 +340,178 @@ struct TokenArgs {
   int asym;
 };
 
-// One row of x to int8 codes in LDS, by the whole workgroup; K % 16 == 0.
-template <int XT>
-__device__ __forceinline__ void codes_to_lds(const TokenArgs& t, int64_t row, int K, int8_t* out, float* red, float* scale, int* zero) {
-  const int tid = threadIdx.x;
-  const char* const x = (const char*)t.x + row * t.ldx * (XT == ROW_F32 ? 4 : 2);
-  const bool wide = (uintptr_t)x % 16 == 0;
-  const auto load = [&](int i, float* v) {
-    if (wide) {
-      if constexpr (XT == ROW_F32) { unpack<XT>(*(const u32x4*)(x + i * 4), v); unpack<XT>(*(const u32x4*)(x + i * 4 + 16), v + 4); }
-      else unpack<XT>(*(const u32x4*)(x + i * 2), v);
+// A row of x in registers, pieces of eight values per lane (K up to 16384), and its int8 codes to LDS, by the whole workgroup;
+// K % 16 == 0.  The loads are apart from the rest, so that the weight's can be issued behind them.
+template <int XT, int WAVES>
+struct TokenRow {
+  static constexpr int KEEP = 4, RAW = XT == ROW_F32 ? 2 : 1;
+  u32x4 raw[KEEP][RAW];
+  const char* x;
+  int K;
+  __device__ __forceinline__ void load8(int i, u32x4* r) const {
+    if ((uintptr_t)x % 16 == 0) {
+      #pragma unroll
+      for (int p = 0; p < RAW; ++p) r[p] = *(const u32x4*)(x + i * (2 * RAW) + 16 * p);
     } else {
       #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = load_scalar<XT>(x, i + e);
+      for (int p = 0; p < RAW; ++p) {
+        float v[8];
+        #pragma unroll
+        for (int e = 0; e < 8 / RAW; ++e) v[e] = load_scalar<XT>(x, i + p * 4 + e);
+        r[p] = pack<XT>(v);
+      }
     }
-  };
-  constexpr int KEEP = 4;                           // pieces of eight that stay in registers: K up to 16384
-  float v[KEEP][8];
-  float hi = t.asym ? -__builtin_inff() : 0.0f, lo = __builtin_inff();
-  const auto range = [&](const float* e) {
+  }
+  __device__ __forceinline__ void load(const TokenArgs& t, int64_t row, int K_) {
+    K = K_;
+    x = (const char*)t.x + row * t.ldx * (2 * RAW);
     #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      hi = nan_max(hi, t.asym ? e[j] : fabsf(e[j]));
-      lo = nan_min(lo, e[j]);
+    for (int c = 0; c < KEEP; ++c) {
+      const int i = (threadIdx.x + c * WAVES * 64) * 8;
+      if (i < K) load8(i, raw[c]);
     }
-  };
-  #pragma unroll
-  for (int c = 0; c < KEEP; ++c) {
-    const int i = (tid + c * STREAM_THREADS) * 8;
-    if (i < K) { load(i, v[c]); range(v[c]); }
   }
-  for (int i = (tid + KEEP * STREAM_THREADS) * 8; i < K; i += STREAM_THREADS * 8) {
-    float e[8];
-    load(i, e);
-    range(e);
-  }
-  hi = team_reduce<64, true>(hi);
-  lo = team_reduce<64, false>(lo);
-  if ((tid & 63) == 0) { red[tid >> 6] = hi; red[STREAM_WAVES + (tid >> 6)] = lo; }
-  __syncthreads();
-  #pragma unroll
-  for (int w = 0; w < STREAM_WAVES; ++w) { hi = nan_max(hi, red[w]); lo = nan_min(lo, red[STREAM_WAVES + w]); }
-  const TokenCodes q = t.scale ? TokenCodes::given(t.scale[0]) : t.asym ? TokenCodes::asymmetric(lo, hi) : TokenCodes::symmetric(hi);
-  #pragma unroll
-  for (int c = 0; c < KEEP; ++c) {
-    const int i = (tid + c * STREAM_THREADS) * 8;
-    if (i < K) *(u32x2*)(out + i) = u32x2{q.codes(v[c]), q.codes(v[c] + 4)};
-  }
-  for (int i = (tid + KEEP * STREAM_THREADS) * 8; i < K; i += STREAM_THREADS * 8) {
-    float e[8];
-    load(i, e);
-    *(u32x2*)(out + i) = u32x2{q.codes(e), q.codes(e + 4)};
-  }
-  if (tid == 0) {
-    *scale = q.d.s;
-    *zero = (int)q.z;
-  }
-  __syncthreads();
-}
-
-// XT: the type of the tokens' values, or -1 for codes
-template <int TB, int BF, int XT>
-__global__ __launch_bounds__(STREAM_THREADS) void stream_kernel(MatmulArgs g, TokenArgs t) {
-  __shared__ __attribute__((aligned(16))) int red[STREAM_WAVES][TB + 1][64][4];
-  __shared__ float token_scale[XT < 0 ? 1 : MOST_FUSED];
-  __shared__ int token_zero[XT < 0 ? 1 : MOST_FUSED];
-  extern __shared__ __attribute__((aligned(16))) int8_t codes[];             // [M, K], XT >= 0 only
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t n0 = (int64_t)blockIdx.x * 16;
-  const int64_t n = n0 + (lane & 15) < g.N ? n0 + (lane & 15) : g.N - 1;
-  const int at = (lane >> 4) * 16;
-  const int8_t* const w = g.w + n * g.ldw + at;
-  const bool asym = XT < 0 ? g.az != nullptr : t.asym;
-
-  struct Piece { i32x4 v[4]; };
-  const auto weights = [&](int k, Piece& p) {       // codes k .. k + 255 of this lane's channel
+  template <class F>
+  __device__ __forceinline__ void each(F&& f) const {
     #pragma unroll
-    for (int i = 0; i < 4; ++i) p.v[i] = k + i * 64 + at < g.K ? *(const i32x4*)(w + k + i * 64) : i32x4{0, 0, 0, 0};
-  };
-  Piece cur, nxt;
-  const int step = STREAM_WAVES * PIECE;
-  int k = wave * PIECE;
-  weights(k, cur);
-  weights(k + step, nxt);
-  if constexpr (XT >= 0) {
-    for (int m = 0; m < (int)g.M; ++m)
-      codes_to_lds<XT>(t, m, g.K, codes + m * g.K, (float*)red, token_scale + m, token_zero + m);
-  }
-  const int8_t* a[TB];
-  #pragma unroll
-  for (int b = 0; b < TB; ++b) {
-    const int64_t m = b * 16 + (lane & 15) < g.M ? b * 16 + (lane & 15) : g.M - 1;           // (a token twice: not stored)
-    a[b] = XT < 0 ? g.a + m * g.lda + at : codes + m * g.K + at;
-  }
-  i32x4 acc[TB] = {};
-  int wsum = 0;
-  while (k < g.K) {
-    Piece tok[TB];
-    #pragma unroll
-    for (int b = 0; b < TB; ++b)
+    for (int c = 0; c < KEEP; ++c) {
+      const int i = (threadIdx.x + c * WAVES * 64) * 8;
+      float v[8];
+      if (i < K) {
+        #pragma unroll
+        for (int p = 0; p < RAW; ++p) unpack<XT>(raw[c][p], v + 4 * p);
+        f(i, v);
+      }
+    }
+    for (int i = (threadIdx.x + KEEP * WAVES * 64) * 8; i < K; i += WAVES * 64 * 8) {
+      u32x4 r[RAW];
+      float v[8];
+      load8(i, r);
       #pragma unroll
-      for (int i = 0; i < 4; ++i) tok[b].v[i] = k + i * 64 + at < g.K ? *(const i32x4*)(a[b] + k + i * 64) : i32x4{0, 0, 0, 0};
+      for (int p = 0; p < RAW; ++p) unpack<XT>(r[p], v + 4 * p);
+      f(i, v);
+    }
+  }
+  // red: 2 WAVES floats
+  __device__ __forceinline__ void to_codes(const TokenArgs& t, int8_t* out, float* red, float* scale, int* zero) const {
+    const int wave = threadIdx.x >> 6;
+    float hi = t.asym ? -__builtin_inff() : 0.0f, lo = __builtin_inff();
+    each([&](int, const float* e) {
+      #pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        hi = nan_max(hi, t.asym ? e[j] : fabsf(e[j]));
+        lo = nan_min(lo, e[j]);
+      }
+    });
+    hi = team_reduce<64, true>(hi);
+    if (t.asym) lo = team_reduce<64, false>(lo);
+    if ((threadIdx.x & 63) == 0) { red[wave] = hi; red[WAVES + wave] = lo; }
+    __syncthreads();
+    #pragma unroll
+    for (int w = 0; w < WAVES; ++w) { hi = nan_max(hi, red[w]); lo = nan_min(lo, red[WAVES + w]); }
+    const TokenCodes q = t.scale ? TokenCodes::given(t.scale[0]) : t.asym ? TokenCodes::asymmetric(lo, hi) : TokenCodes::symmetric(hi);
+    each([&](int i, const float* e) { *(u32x2*)(out + i) = q.codes(e); });
+    if (threadIdx.x == 0) {
+      *scale = q.d.s;
+      *zero = (int)q.z;
+    }
+    __syncthreads();
+  }
+};
+template <int WAVES> struct TokenRow<-1, WAVES> {};
+
+// TB blocks of 16 tokens, NB blocks of 16 channels.  XT: the type of one token's values (TB = 1), or -1 for codes.
+template <int TB, int NB, int BF, int XT, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void stream_kernel(MatmulArgs g, TokenArgs t) {
+  __shared__ __attribute__((aligned(16))) int red[WAVES][NB][TB + 1][64][4];
+  __shared__ float token_scale;
+  __shared__ int token_zero;
+  extern __shared__ __attribute__((aligned(16))) int8_t codes[];             // [K], XT >= 0 only
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t n0 = (int64_t)blockIdx.x * (16 * NB);
+  const int rows_w = (int)(g.N - n0 < 16 * NB ? g.N - n0 : 16 * NB);
+  const int at = (lane >> 4) * 16;                  // this lane's 16 codes of 64
+  const bool asym = XT < 0 ? g.az != nullptr : t.asym;
+  TokenRow<XT, WAVES> row;
+  if constexpr (XT >= 0) row.load(t, 0, g.K);
+
+  // Loads are told where their matrix ends: codes past K and rows past the last one read as zero, without a branch.
+  const __amdgpu_buffer_rsrc_t bufW = __builtin_amdgcn_make_buffer_rsrc((void*)(g.w + n0 * g.ldw), 0, (int)((rows_w - 1) * g.ldw + g.K), 0x00020000);
+  const __amdgpu_buffer_rsrc_t bufA = __builtin_amdgcn_make_buffer_rsrc((void*)g.a, 0, XT < 0 ? (int)((g.M - 1) * g.lda + g.K) : 0, 0x00020000);
+  constexpr uint32_t OUTSIDE = 0x80000000u;
+  uint32_t ofW[NB], ofA[TB];
+  #pragma unroll
+  for (int c = 0; c < NB; ++c) ofW[c] = c * 16 + (lane & 15) < rows_w ? (uint32_t)((c * 16 + (lane & 15)) * g.ldw) + at : OUTSIDE;
+  #pragma unroll
+  for (int b = 0; b < TB; ++b) ofA[b] = b * 16 + (lane & 15) < g.M ? (uint32_t)((b * 16 + (lane & 15)) * g.lda) + at : OUTSIDE;
+  // DEPTH pieces of 256 codes in flight, each with its tokens': waiting for the oldest leaves the others on their way
+  constexpr int DEPTH = TB + NB <= 3 ? 3 : 2, STEP = WAVES * PIECE;
+  struct Piece { i32x4 w[NB][4], a[TB][4]; } ring[DEPTH];
+  const auto load = [&](int k, Piece& p) {          // codes k .. k + 255
     #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      const uint32_t outside = k + i * 64 + at < g.K ? 0u : OUTSIDE;
       #pragma unroll
-      for (int b = 0; b < TB; ++b) acc[b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cur.v[i], tok[b].v[i], acc[b], 0, 0, 0);
-      if (asym) wsum = add_bytes(cur.v[i], wsum);
+      for (int c = 0; c < NB; ++c)
+        p.w[c][i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(bufW, ofW[c] | outside, k + i * 64, 0));
+      if constexpr (XT < 0) {
+        #pragma unroll
+        for (int b = 0; b < TB; ++b)
+          p.a[b][i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(bufA, ofA[b] | outside, k + i * 64, 0));
+      }
     }
-    k += step;
-    cur = nxt;
-    weights(k + step, nxt);
+  };
+  int k = wave * PIECE;
+  #pragma unroll
+  for (int d = 0; d < DEPTH; ++d) {
+    load(k + d * STEP, ring[d]);
+    __builtin_amdgcn_sched_barrier(0);              // (in this order: a wait counts the loads behind it)
+  }
+  if constexpr (XT >= 0) row.to_codes(t, codes, (float*)red, &token_scale, &token_zero);
+  i32x4 acc[NB][TB] = {};
+  int wsum[NB] = {};
+  while (k < g.K) {
+    #pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      Piece& p = ring[d];
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (XT >= 0) p.a[0][i] = *(const i32x4*)(codes + (k + i * 64 + at < g.K ? k + i * 64 + at : 0));   // (every column the token; past K the weight is 0)
+        #pragma unroll
+        for (int c = 0; c < NB; ++c) {
+          #pragma unroll
+          for (int b = 0; b < TB; ++b) acc[c][b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(p.w[c][i], p.a[b][i], acc[c][b], 0, 0, 0);
+          if (asym) wsum[c] = add_bytes(p.w[c][i], wsum[c]);
+        }
+      }
+      load(k + DEPTH * STEP, p);
+      k += STEP;
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
   #pragma unroll
-  for (int b = 0; b < TB; ++b) *(i32x4*)red[wave][b][lane] = acc[b];
-  red[wave][TB][lane][0] = wsum;
+  for (int c = 0; c < NB; ++c) {
+    #pragma unroll
+    for (int b = 0; b < TB; ++b) *(i32x4*)red[wave][c][b][lane] = acc[c][b];
+    red[wave][c][TB][lane][0] = wsum[c];
+  }
   __syncthreads();
   // accumulator register r of lane l: channel 4 (l / 16) + r of token l % 16
-  for (int o = tid; o < TB * 256; o += STREAM_THREADS) {
-    const int c = o & 15, tok = (o >> 4) & 15, b = o >> 8;
-    const int64_t m = b * 16 + tok, nn = n0 + c;
-    if (m >= g.M || nn >= g.N) continue;
+  for (int o = tid; o < TB * NB * 256; o += WAVES * 64) {
+    const int c = o % (16 * NB), cb = c >> 4, cc = c & 15, token = o / (16 * NB), b = token >> 4, tok = token & 15;
+    const int64_t nn = n0 + c;
+    if (token >= g.M || nn >= g.N) continue;
     int s = 0, sum = 0;
     #pragma unroll
-    for (int v = 0; v < STREAM_WAVES; ++v) {
-      s += red[v][b][(c >> 2) * 16 + tok][c & 3];
-      if (asym) sum += (red[v][TB][c][0] + red[v][TB][c + 16][0]) + (red[v][TB][c + 32][0] + red[v][TB][c + 48][0]);
+    for (int v = 0; v < WAVES; ++v) {
+      s += red[v][cb][b][(cc >> 2) * 16 + tok][cc & 3];
+      if (asym) sum += (red[v][cb][TB][cc][0] + red[v][cb][TB][cc + 16][0]) + (red[v][cb][TB][cc + 32][0] + red[v][cb][TB][cc + 48][0]);
     }
-    if (asym) s -= (XT < 0 ? g.az[m] : token_zero[m]) * sum;
-    const float as = XT < 0 ? g.as[g.a_scalar ? 0 : m] : token_scale[m];
-    const float y = (float)s * (as * load_any(g.ws, g.ws_dtype, g.w_scalar ? 0 : nn)) + (g.bias ? load_any(g.bias, g.bias_dtype, nn) : 0.0f);
-    if constexpr (BF == ROW_F32) ((float*)g.y)[m * g.N + nn] = y;
-    else store_scalar<BF>(g.y, m * g.N + nn, rnd<BF>(y));
+    if (asym) s -= (XT < 0 ? g.az[token] : token_zero) * sum;
+    const float as = XT < 0 ? g.as[g.a_scalar ? 0 : token] : token_scale;
+    const float y = __builtin_fmaf((float)s, as * load_any(g.ws, g.ws_dtype, g.w_scalar ? 0 : nn), g.bias ? load_any(g.bias, g.bias_dtype, nn) : 0.0f);
+    if constexpr (BF == ROW_F32) ((float*)g.y)[token * g.N + nn] = y;
+    else store_scalar<BF>(g.y, token * g.N + nn, rnd<BF>(y));
   }
 }
 
@@ -411,37 +536,62 @@ __global__ __launch_bounds__(256) void pad_kernel(const int8_t* __restrict__ x, 
 }
 
 int64_t padded(int64_t K) { return (K + 15) / 16 * 16; }
+int64_t on256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
-template <int FM, int FN, int BF>
-void launch_tiles(const MatmulArgs& g, hipStream_t st) {
-  const int64_t tm = (g.M + Tile<FM, FN>::TM - 1) / Tile<FM, FN>::TM, tn = (g.N + Tile<FM, FN>::TN - 1) / Tile<FM, FN>::TN;
-  const dim3 grid((unsigned)((tm * tn + 7) / 8 * 8));
-  if (g.az) tile_kernel<FM, FN, BF, true><<<grid, dim3(256), 0, st>>>(g, (int)tm, (int)tn);
-  else tile_kernel<FM, FN, BF, false><<<grid, dim3(256), 0, st>>>(g, (int)tm, (int)tn);
+// The large tiles run at the rate at which half lines reach LDS (64 codes of a row; 27 bytes per clock and CU), but two stages of 128 codes,
+// all that fits next to each other, are too few for the latency of the cache: 256 x 256 took 0.59 us per 64 codes with them, 0.50 so.
+// 128 x 128 has room for four stages of whole lines (41 bytes per clock): 0.167 us per 64 codes, with half lines 0.25, with two stages 0.37
+// (and 0.20 as two workgroups per CU).
+typedef Tile<4, 4, 64, 4, 2> Tile256;
+typedef Tile<4, 3, 64, 4, 2> Tile192;
+typedef Tile<2, 2, 128, 4, 2> Tile128;
+
+template <class T, int BF>
+void launch_tiles(const MatmulArgs& g, int parts, hipStream_t st) {
+  const int64_t tm = (g.M + T::TM - 1) / T::TM, tn = (g.N + T::TN - 1) / T::TN;
+  const dim3 grid((unsigned)((tm * tn * parts + 7) / 8 * 8));
+  if (g.az) tile_kernel<T, BF, true><<<grid, dim3(256), 0, st>>>(g, (int)tm, (int)tn, parts);
+  else tile_kernel<T, BF, false><<<grid, dim3(256), 0, st>>>(g, (int)tm, (int)tn, parts);
+}
+template <int BF>
+void launch_join(const MatmulArgs& g, const int* sums, int parts, hipStream_t st) {
+  const bool wide = g.N % 4 == 0 && (uintptr_t)g.y % 16 == 0;
+  const int64_t all = g.M * g.N;
+  if (wide) join_kernel<BF, 4><<<dim3((unsigned)((all / 4 + 255) / 256)), dim3(256), 0, st>>>(g, sums, parts);
+  else join_kernel<BF, 1><<<dim3((unsigned)((all + 255) / 256)), dim3(256), 0, st>>>(g, sums, parts);
 }
 
-#ifndef STREAM_MOST
-#define STREAM_MOST 32
-#endif
-constexpr int64_t MOST_STREAMED = STREAM_MOST;      // tokens
-
-template <int BF, int XT>
+template <int TB, int NB, int BF, int XT, int WAVES>
 void launch_stream(const MatmulArgs& g, const TokenArgs& t, hipStream_t st) {
-  const dim3 grid((unsigned)((g.N + 15) / 16));
-  if constexpr (XT >= 0) {
-    stream_kernel<1, BF, XT><<<grid, dim3(STREAM_THREADS), (unsigned)(g.M * g.K), st>>>(g, t);
-  } else {
-    if (g.M <= 16) stream_kernel<1, BF, -1><<<grid, dim3(STREAM_THREADS), 0, st>>>(g, t);
-    else if (g.M <= 32) stream_kernel<2, BF, -1><<<grid, dim3(STREAM_THREADS), 0, st>>>(g, t);
-    else stream_kernel<4, BF, -1><<<grid, dim3(STREAM_THREADS), 0, st>>>(g, t);
-  }
+  stream_kernel<TB, NB, BF, XT, WAVES><<<dim3((unsigned)((g.N + 16 * NB - 1) / (16 * NB))), dim3(WAVES * 64), XT < 0 ? 0 : (unsigned)g.K, st>>>(g, t);
 }
 
 template <int BF>
-void launch_codes(const MatmulArgs& g, hipStream_t st) {
-  if (g.M <= MOST_STREAMED) launch_stream<BF, -1>(g, TokenArgs{}, st);
-  else if ((g.M + 255) / 256 * ((g.N + 255) / 256) >= 160) launch_tiles<4, 4, BF>(g, st);
-  else launch_tiles<2, 2, BF>(g, st);
+void launch_codes(const MatmulArgs& g, int* sums, hipStream_t st) {
+  if (g.M <= INT8_STREAMED) {
+    if (g.M <= 16) launch_stream<1, 1, BF, -1, 2>(g, TokenArgs{}, st);
+    else if (g.N <= 4096) launch_stream<2, 1, BF, -1, 2>(g, TokenArgs{}, st);
+    else launch_stream<2, 2, BF, -1, 2>(g, TokenArgs{}, st);
+  }
+  else {
+    const Int8Cut c = int8_cut(g.M, g.N, g.K);
+    if (c.parts > 1) {
+      MatmulArgs p = g;
+      p.y = sums;
+      launch_tiles<Tile128, ROW_I32>(p, c.parts, st);
+      launch_join<BF>(g, sums, c.parts, st);
+    }
+    else if (c.tile == 0) launch_tiles<Tile256, BF>(g, 1, st);
+    else if (c.tile == 1) launch_tiles<Tile192, BF>(g, 1, st);
+    else launch_tiles<Tile128, BF>(g, 1, st);
+  }
+}
+
+template <int BF, int XT>
+void launch_token(const MatmulArgs& g, const TokenArgs& t, hipStream_t st) {
+  if (g.N > 8192) launch_stream<1, 1, BF, XT, 2>(g, t, st);
+  else if (g.K <= 8192) launch_stream<1, 1, BF, XT, 4>(g, t, st);
+  else launch_stream<1, 1, BF, XT, 8>(g, t, st);
 }
 
 bool known(int dtype) { return dtype == LCQ_F32 || dtype == LCQ_BF16 || dtype == LCQ_F16; }
@@ -454,9 +604,8 @@ int check(const int8_t* w, const void* ws, int ws_dtype, const void* bias, int b
   return LCQ_OK;
 }
 
-// tokens whose codes the product makes itself
-bool fused(int64_t M, int64_t K) { return M <= MOST_FUSED && K % 16 == 0 && M * K <= MOST_FUSED_CODES; }
-int64_t on256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+// one token, whose codes the product makes itself
+bool fused(int64_t M, int64_t K) { return M == 1 && K % 16 == 0 && K <= MOST_FUSED; }
 
 }  // namespace
 
@@ -464,7 +613,8 @@ extern "C" {
 
 int64_t lcq_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0 || K > 65536) return 0;
-  return K % 16 ? (M + N) * padded(K) : 0;
+  const int parts = M <= INT8_STREAMED ? 1 : int8_cut(M, N, padded(K)).parts;
+  return (parts > 1 ? on256(4 * M * N * parts) : 0) + (K % 16 ? (M + N) * padded(K) : 0);
 }
 
 int lcq_int8_matmul(const int8_t* a, const float* as, int a_scalar, const int32_t* az, const int8_t* w, const void* ws, int ws_dtype,
@@ -475,22 +625,24 @@ int lcq_int8_matmul(const int8_t* a, const float* as, int a_scalar, const int32_
   if (bad) return bad;
   hipStream_t st = (hipStream_t)stream;
   MatmulArgs g = {a, w, as, az, ws, bias, y, M, N, K, K, (int)K, ws_dtype, bias_dtype, a_scalar, w_scalar};
-  if (K % 16) {
+  if (K % 16 == 0 && (uintptr_t)a % 16) return LCQ_EALIGN;
+  const int parts = M <= INT8_STREAMED ? 1 : int8_cut(M, N, padded(K)).parts;
+  if (K % 16 || parts > 1) {
     if (!workspace) return LCQ_EWORKSPACE;
     if ((uintptr_t)workspace % 16) return LCQ_EALIGN;
+  }
+  if (K % 16) {
     const int Kp = (int)padded(K);
-    int8_t* const pa = (int8_t*)workspace;
+    int8_t* const pa = (int8_t*)workspace + (parts > 1 ? on256(4 * M * N * parts) : 0);
     int8_t* const pw = pa + M * Kp;
     const auto grid = [&](int64_t rows) { const int64_t b = (rows * (Kp / 16) + 255) / 256; return dim3((unsigned)(b < 4096 ? b : 4096)); };
     pad_kernel<<<grid(M), dim3(256), 0, st>>>(a, M, (int)K, Kp, pa);
     pad_kernel<<<grid(N), dim3(256), 0, st>>>(w, N, (int)K, Kp, pw);
     g.a = pa; g.w = pw; g.lda = g.ldw = g.K = Kp;
-  } else if ((uintptr_t)a % 16) {
-    return LCQ_EALIGN;
   }
-  if (dtype == LCQ_BF16) launch_codes<ROW_BF16>(g, st);
-  else if (dtype == LCQ_F16) launch_codes<ROW_F16>(g, st);
-  else launch_codes<ROW_F32>(g, st);
+  if (dtype == LCQ_BF16) launch_codes<ROW_BF16>(g, (int*)workspace, st);
+  else if (dtype == LCQ_F16) launch_codes<ROW_F16>(g, (int*)workspace, st);
+  else launch_codes<ROW_F32>(g, (int*)workspace, st);
   LCQ_CHECK_LAUNCH();
   return LCQ_OK;
 }
@@ -513,13 +665,13 @@ int lcq_int8_linear(const void* x, int x_dtype, int64_t ldx, int asym, const flo
     const TokenArgs t = {x, scale, ldx, asym};
     const auto run = [&](auto xt) {
       constexpr int XT = decltype(xt)::value;
-      if (dtype == LCQ_BF16) launch_stream<ROW_BF16, XT>(g, t, st);
-      else if (dtype == LCQ_F16) launch_stream<ROW_F16, XT>(g, t, st);
-      else launch_stream<ROW_F32, XT>(g, t, st);
+      if (dtype == LCQ_BF16) launch_token<ROW_BF16, XT>(g, t, st);
+      else if (dtype == LCQ_F16) launch_token<ROW_F16, XT>(g, t, st);
+      else launch_token<ROW_F32, XT>(g, t, st);
     };
-    if (x_dtype == LCQ_BF16) run(std::integral_constant<int, ROW_BF16>{});
-    else if (x_dtype == LCQ_F16) run(std::integral_constant<int, ROW_F16>{});
-    else run(std::integral_constant<int, ROW_F32>{});
+    if (x_dtype == LCQ_BF16) run(Int<ROW_BF16>{});
+    else if (x_dtype == LCQ_F16) run(Int<ROW_F16>{});
+    else run(Int<ROW_F32>{});
     LCQ_CHECK_LAUNCH();
     return LCQ_OK;
   }

@@ -39,4 +39,36 @@ inline bool gptq_by_panels(bool is_static, bool has_gidx, bool rounded, int grou
   return is_static || divides || codes * group < 65536.0f || codes * R <= 32768.0f || R > 4096;
 }
 
+// Int8 product of more than INT8_STREAMED tokens (int8_matmul.hip): which tile, and into how many parts K is cut.  A tile takes
+//   start + slabs (busy + crowd share) us     slabs of 128 codes of K, share of the chip's 256 CUs at work
+// and the tiles of a workgroup slot follow one another; parts leave their sums (written and read once, 4 bytes per us and MB / 4) for
+// another kernel (3 us).  Constants fitted to one round at K = 4096 and 14336 (us): 256 x 256 alone 42 and 125, on all CUs 60;
+// 256 x 192 35 and 98, 53; 128 x 128 15.5 and 42, 20.  Measured choices, us at K = 4096 as 256 x 256 / 256 x 192 / 128 x 128:
+//   N = 4096    1024 tokens 44.3 / 37.6 / 19.8    2048 tokens  45.5 / 41.6 / 38.3
+//   N = 6144    1024 tokens 44.7 / 37.7 / 34.0    2048 tokens  52.6 / 52.9 / 56.8
+//   N = 14336    512 tokens 45.1 / 39.5 / 35.6    1024 tokens  57.8 / 85.0 / 68.5    2048 tokens 112 / 134 / 129
+constexpr int INT8_STREAMED = 32;
+struct Int8Cut { int tile, parts; };                // tile 0: 256 x 256, 1: 256 x 192, 2: 128 x 128
+inline Int8Cut int8_cut(long long M, long long N, long long K) {
+  struct Shape { int tm, tn; double start, busy, crowd; };
+  const Shape shapes[3] = {{256, 256, 9.0, 1.03, 0.56}, {256, 192, 8.0, 0.81, 0.60}, {128, 128, 5.0, 0.333, 0.14}};
+  const long long slabs = (K + 127) / 128;
+  Int8Cut best = {0, 1};
+  double least = 0.0;
+  for (int i = 0; i < 3; ++i) {
+    const Shape& s = shapes[i];
+    const long long tiles = (M + s.tm - 1) / s.tm * ((N + s.tn - 1) / s.tn);
+    for (int parts = 1; parts <= (i == 2 ? 16 : 1); ++parts) {
+      if (parts > 1 && (tiles * parts > 256 || slabs / parts < 2)) break;
+      const long long rounds = tiles * parts / 256, rest = tiles * parts % 256;
+      const double each = (double)((slabs + parts - 1) / parts);
+      double t = rounds * (s.start + each * (s.busy + s.crowd));
+      if (rest) t += s.start + each * (s.busy + s.crowd * (double)rest / 256.0);
+      if (parts > 1) t += 3.0 + 8.0 * parts * (double)M * (double)N / 4e6;
+      if (least == 0.0 || t < least) { least = t; best = {i, parts}; }
+    }
+  }
+  return best;
+}
+
 }  // namespace lcq

@@ -186,7 +186,7 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void residual_norm_kernel(
   const TokenCodes q = make();
   each([&](int i, float* e) {
     if constexpr (V == 1) a.codes[r * K + i] = (int8_t)q.code(e[0]);
-    else *(u32x2*)(a.codes + r * K + i) = u32x2{q.codes(e), q.codes(e + 4)};
+    else *(u32x2*)(a.codes + r * K + i) = q.codes(e);
   });
   if (t == 0 && a.scales) a.scales[r] = q.d.s;
   if (t == 0 && a.zeros) a.zeros[r] = (int)q.z;

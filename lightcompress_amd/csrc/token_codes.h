@@ -19,9 +19,23 @@ struct TokenCodes {
     // (s >= 1e-5 / 255: x / s overflows only for a narrow range far from zero)
     return TokenCodes(s, fminf(fmaxf(-128.0f - rintf(lo / s), -128.0f), 127.0f), fmaxf(fabsf(hi), fabsf(lo)) < 1e30f);
   }
-  __device__ __forceinline__ int code(float x) const { return (int)fminf(fmaxf(rintf(d.quotient(x)) + z, -128.0f), 127.0f); }
-  __device__ __forceinline__ uint32_t codes(const float* x) const {          // four of them, the first in the lowest byte
-    return (uint32_t)(code(x[0]) & 255) | (uint32_t)(code(x[1]) & 255) << 8 | (uint32_t)(code(x[2]) & 255) << 16 | (uint32_t)code(x[3]) << 24;
+  __device__ __forceinline__ int clamped(float quotient) const { return (int)fminf(fmaxf(rintf(quotient) + z, -128.0f), 127.0f); }
+  __device__ __forceinline__ int code(float x) const { return clamped(d.quotient(x)); }
+  // eight of them, the first in the lowest byte; the wave holds one token (one branch, not one per value)
+  __device__ __forceinline__ u32x2 codes(const float* x) const {
+    int q[8];
+    if (__builtin_amdgcn_readfirstlane((int)d.fast)) {
+      #pragma unroll
+      for (int j = 0; j < 8; ++j) q[j] = clamped(d.fast_quotient(x[j]));
+    } else {
+      #pragma unroll
+      for (int j = 0; j < 8; ++j) q[j] = clamped(x[j] / d.s);
+    }
+    u32x2 w;
+    #pragma unroll
+    for (int p = 0; p < 2; ++p)
+      w[p] = (uint32_t)(q[4 * p] & 255) | (uint32_t)(q[4 * p + 1] & 255) << 8 | (uint32_t)(q[4 * p + 2] & 255) << 16 | (uint32_t)q[4 * p + 3] << 24;
+    return w;
   }
 };
 
