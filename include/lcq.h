@@ -517,7 +517,7 @@ int lcq_residual_norm(const void* x, int dtype, int64_t T, int64_t K, int64_t ld
 
 /* Log probabilities of given tokens, entropy and best alternatives, from logits:
  *    l = log sum_v exp(x_v);   logprobs = x_token - l;   entropy = l - sum_v p_v x_v;   top: the k largest x_v, as x_v - l
- *  logits   [T, V] of `dtype`, rows ldx elements apart;  V < 2^31
+ *  logits   [T, V] of `dtype`, rows ldx elements apart;  V <= 2^28
  *  tokens   [T, m] int64 or NULL; logprobs [T, m] fp32.  A token equal to `ignore` gives 0, another one outside [0, V) NaN
  *  entropy  [T] fp32 or NULL
  *  top_logprobs [T, k] fp32, top_tokens [T, k] int64, 0 <= k <= min(64, V): largest first, equal logits by the lowest index, a NaN

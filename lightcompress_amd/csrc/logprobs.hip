@@ -19,7 +19,7 @@ using namespace lcq;
 
 constexpr float LOWEST = -3.4028234663852886e38f, MOVE = 8.0f;
 constexpr int THREADS = 256, WAVES = THREADS / 64;
-constexpr int FLIGHT = 4;                           // 16-byte pieces that a lane has in flight
+constexpr int FLIGHT = 2;                           // 16-byte pieces that a lane has on their way while it works on as many
 
 struct LogprobArgs {
   const void* x;
@@ -28,7 +28,7 @@ struct LogprobArgs {
   int64_t* top_tokens;
   int64_t V, ldx, m, ignore;
   int k, parts;
-  int64_t per;                                      // 16-byte pieces of a part
+  int per;                                          // 16-byte pieces of a part
   f32x4* sums;                                      // [T, parts]: c, S, U
   uint64_t* keys;                                   // [T, parts, k]
 };
@@ -50,26 +50,47 @@ __device__ __forceinline__ uint64_t other_lane(uint64_t v, int lane) {
   const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(lane * 4, (int)(uint32_t)v), hi = (uint32_t)__builtin_amdgcn_ds_bpermute(lane * 4, (int)(v >> 32));
   return (uint64_t)hi << 32 | lo;
 }
-// lane i and lane i ^ d: the larger key to the lower lane where `down`, else the other way
-__device__ __forceinline__ uint64_t exchange(uint64_t v, int lane, int d, bool down) {
-  const uint64_t o = other_lane(v, lane ^ d);
-  return (((lane & d) == 0) == down) == (v > o) ? v : o;
+// the value that lane i ^ D holds, without LDS: mirrors of a row's 16 lanes, their halves and quads, and swaps of rows
+template <int D>
+__device__ __forceinline__ uint32_t across(uint32_t v) {
+  const auto dpp = [](uint32_t u, auto ctrl) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, decltype(ctrl)::value, 0xf, 0xf, true); };
+  constexpr std::integral_constant<int, 0xB1> xor1; constexpr std::integral_constant<int, 0x4E> xor2; constexpr std::integral_constant<int, 0x1B> xor3;
+  constexpr std::integral_constant<int, 0x141> xor7; constexpr std::integral_constant<int, 0x140> xor15;
+  if constexpr (D == 1) return dpp(v, xor1);
+  else if constexpr (D == 2) return dpp(v, xor2);
+  else if constexpr (D == 4) return dpp(dpp(v, xor7), xor3);
+  else if constexpr (D == 8) return dpp(dpp(v, xor15), xor7);
+  else if constexpr (D == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);     // rows 0, 0, 2, 2 and 1, 1, 3, 3
+    return threadIdx.x & 16 ? r[0] : r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);     // the lower half twice, and the upper
+    return threadIdx.x & 32 ? r[0] : r[1];
+  }
+}
+// lane i and lane i ^ D: the larger key to the lower lane where `down`, else the other way
+template <int D>
+__device__ __forceinline__ uint64_t exchange(uint64_t v, int lane, bool down) {
+  const uint64_t o = (uint64_t)across<D>((uint32_t)(v >> 32)) << 32 | across<D>((uint32_t)v);
+  return (((lane & D) == 0) == down) == (v > o) ? v : o;
+}
+// a bitonic sequence of N lanes into order
+template <int N>
+__device__ __forceinline__ uint64_t ordered(uint64_t v, int lane, bool down) {
+  if constexpr (N > 1) return ordered<N / 2>(exchange<N / 2>(v, lane, down), lane, down);
+  return v;
 }
 // the wave's 64 keys in descending order
 __device__ __forceinline__ uint64_t sorted(uint64_t v, int lane) {
-  #pragma unroll
-  for (int n = 2; n <= 64; n *= 2)
-    #pragma unroll
-    for (int d = n / 2; d; d /= 2) v = exchange(v, lane, d, (lane & n) == 0);
-  return v;
+  v = ordered<2>(v, lane, (lane & 2) == 0);
+  v = ordered<4>(v, lane, (lane & 4) == 0);
+  v = ordered<8>(v, lane, (lane & 8) == 0);
+  v = ordered<16>(v, lane, (lane & 16) == 0);
+  v = ordered<32>(v, lane, (lane & 32) == 0);
+  return ordered<64>(v, lane, true);
 }
 // the 64 largest of two descending lists, `turned` with its lanes in ascending order
-__device__ __forceinline__ uint64_t merged(uint64_t v, uint64_t turned, int lane) {
-  v = v > turned ? v : turned;
-  #pragma unroll
-  for (int d = 32; d; d /= 2) v = exchange(v, lane, d, true);
-  return v;
-}
+__device__ __forceinline__ uint64_t merged(uint64_t v, uint64_t turned, int lane) { return ordered<64>(v > turned ? v : turned, lane, true); }
 
 // The best 64 of a wave.  `count` and `bound` are the same in all lanes.
 struct Best {
@@ -152,86 +173,135 @@ __device__ __forceinline__ void answer(const LogprobArgs& a, int64_t row, const 
 
 template <int BF, bool TOP>
 __global__ __launch_bounds__(THREADS) void logprobs_kernel(LogprobArgs a) {
-  constexpr int N = Vec<BF>::N;
+  constexpr int N = Vec<BF>::N, PASS = THREADS * FLIGHT;
   __shared__ uint64_t found[TOP ? WAVES : 1][TOP ? 64 * N + 64 : 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ uint32_t shared;                       // the upper half of a key: the largest k-th best that a wave has
+  if (threadIdx.x == 0) shared = 0;
+  if constexpr (TOP) __syncthreads();
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row = (int64_t)blockIdx.x / a.parts;
   const int part = (int)((int64_t)blockIdx.x - row * a.parts);
-  const char* const first = (const char*)a.x + row * a.ldx * (16 / N);
-  // pieces of 16 aligned bytes: piece j holds logits N j - before ...; only the first and the last may reach out of the row
-  const int before = (int)((uintptr_t)first % 16) / (16 / N);
-  const char* const base = first - before * (16 / N);
-  const int64_t pieces = (a.V + before + N - 1) / N;
-  const int64_t from = part * a.per, to = from + a.per < pieces ? from + a.per : pieces;
+  const char* const x = (const char*)a.x + row * a.ldx * (16 / N);
+  const int V = (int)a.V, pieces = (V + N - 1) / N;
+  const int from = part * a.per, to = from + a.per < pieces ? from + a.per : pieces;
 
   Sums s;
   Best best(lane, TOP ? a.k : 1);
   int count = 0;
-  const auto drain = [&] {                          // takes over what was collected
+  const auto drain = [&]() __attribute__((always_inline)) {                          // takes over what was collected
     for (int at = 0; at < count; at += 64) best.take(at + lane < count ? found[wave][at + lane] : 0);
     count = 0;
   };
-  const auto piece = [&](const u32x4& raw, int64_t j) {
+  // The waves share the best of their bounds: what lies below one wave's k-th best is not among the row's.
+  const auto share = [&]() __attribute__((always_inline)) {
+    if (lane == 0 && best.bound) __hip_atomic_fetch_max(&shared, (uint32_t)(best.bound >> 32), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  };
+  // piece j of the row, its largest logit `top` (one that lies past the row's end holds nothing): what of it may be among the best
+  const auto consider = [&](const u32x4& raw, float top, int j) __attribute__((always_inline)) {
     float v[N];
     unpack<BF>(raw, v);
-    float top = v[0];
-    #pragma unroll
-    for (int i = 1; i < N; ++i) top = nan_max(top, v[i]);
-    if (top > s.c + MOVE) s.refer(top);
-    if constexpr (TOP) {
-      const uint64_t pass = __builtin_amdgcn_ballot_w64(!(top < best.limit));
-      if (__builtin_expect(pass != 0, 0)) {
-        const int64_t v0 = j * N - before;
-        uint64_t key[N];
-        #pragma unroll
-        for (int i = 0; i < N; ++i) key[i] = v0 + i >= 0 && v0 + i < a.V ? key_of(v[i], (uint32_t)(v0 + i)) : 0;
-        if (__builtin_popcountll(pass) > 16) {
-          uint64_t m = key[0];
-          #pragma unroll
-          for (int i = 1; i < N; ++i) m = key[i] > m ? key[i] : m;
-          m = best.kth(sorted(m, lane));
-          if (m) best.raise(m - 1);                          // (less one: the k-th itself has still to be collected)
-        }
-        #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const bool in = key[i] > best.bound;
-          const uint64_t lanes = __builtin_amdgcn_ballot_w64(in);
-          if (lanes == 0) continue;
-          if (in) found[wave][count + __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0))] = key[i];
-          count += __builtin_popcountll(lanes);
-        }
-        if (count >= 64) drain();
+    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(!(top < best.limit))) > 16) {
+      uint64_t m = 0;
+      #pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint64_t key = (int64_t)j * N + i < V ? key_of(v[i], (uint32_t)(j * N + i)) : 0;
+        m = key > m ? key : m;
       }
+      m = best.kth(sorted(m, lane));
+      if (m) best.raise(m - 1);                     // (less one: the k-th itself has still to be collected)
+      share();
     }
     #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float d = v[i] - s.c, e = __builtin_amdgcn_exp2f(d * 1.44269504088896340736f);
-      s.S += e;
-      s.U = __builtin_fmaf(e, nan_max(d, -150.0f), s.U);     // (-inf: e is 0)
+      if (__builtin_amdgcn_ballot_w64(!(v[i] < best.limit)) == 0) continue;
+      const uint64_t key = (int64_t)j * N + i < V ? key_of(v[i], (uint32_t)(j * N + i)) : 0;
+      const bool in = key > best.bound && !(v[i] < best.limit);
+      const uint64_t lanes = __builtin_amdgcn_ballot_w64(in);
+      if (in) found[wave][count + __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0))] = key;
+      count += __builtin_popcountll(lanes);
+    }
+    if (count >= 64) {
+      drain();
+      share();
     }
   };
-  const auto load = [&](int64_t j) -> u32x4 {
-    const int64_t v0 = j * N - before;
-    if (v0 >= 0 && v0 + N <= a.V) return *(const u32x4*)(base + j * 16);
-    float v[N];
-    #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = v0 + i >= 0 && v0 + i < a.V ? load_scalar<BF>(first, v0 + i) : -__builtin_inff();
-    return pack<BF>(v);
-  };
-  const u32x4 nothing = N == 4 ? u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u}      // -inf
-                               : u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u} & (BF == ROW_F16 ? 0xfc00fc00u : ~0u);
-  for (int64_t j0 = from; j0 < to; j0 += THREADS * FLIGHT) {
-    u32x4 raw[FLIGHT];
-    #pragma unroll
-    for (int f = 0; f < FLIGHT; ++f) {
-      const int64_t j = j0 + f * THREADS + threadIdx.x;
-      raw[f] = j < to ? load(j) : nothing;
+  // the pieces j0 + f THREADS of this lane
+  const auto take = [&](const u32x4 (&raw)[FLIGHT], int j0) __attribute__((always_inline)) {
+    float top[FLIGHT];
+    uint64_t pass[FLIGHT], any = 0;
+    if constexpr (TOP) {
+      const float theirs = logit_of((uint64_t)__hip_atomic_load(&shared, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) << 32);
+      best.limit = theirs > best.limit ? theirs : best.limit;
     }
     #pragma unroll
     for (int f = 0; f < FLIGHT; ++f) {
-      const int64_t j = j0 + f * THREADS + threadIdx.x;
-      piece(raw[f], j < to ? j : pieces + 1);       // (past the end of the row: nothing of it can be among the best)
+      float v[N];
+      unpack<BF>(raw[f], v);
+      top[f] = v[0];
+      #pragma unroll
+      for (int i = 1; i < N; ++i) top[f] = nan_max(top[f], v[i]);
+      if constexpr (TOP) any |= pass[f] = __builtin_amdgcn_ballot_w64(!(top[f] < best.limit));
+      if (top[f] > s.c + MOVE) s.refer(top[f]);
+      #pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float d = v[i] - s.c, e = __builtin_amdgcn_exp2f(d * 1.44269504088896340736f);
+        s.S += e;
+        s.U = __builtin_fmaf(e, nan_max(d, -150.0f), s.U);   // (-inf: e is 0)
+      }
     }
+    if constexpr (TOP) {
+      if (__builtin_expect(any != 0, 0)) {
+        #pragma unroll 1
+        for (int f = 0; f < FLIGHT; ++f) {          // (one copy of the code for all of them)
+          u32x4 r = raw[0];
+          float t = top[0];
+          uint64_t p = pass[0];
+          #pragma unroll
+          for (int g = 1; g < FLIGHT; ++g) { r = f == g ? raw[g] : r; t = f == g ? top[g] : t; p = f == g ? pass[g] : p; }
+          if (p) consider(r, t, j0 + f * THREADS + (int)threadIdx.x);
+        }
+      }
+    }
+  };
+  const auto fetch = [&](u32x4 (&raw)[FLIGHT], int j0) {    // whole pieces
+    #pragma unroll
+    for (int f = 0; f < FLIGHT; ++f) __builtin_memcpy(&raw[f], x + (uint32_t)(j0 + f * THREADS + (int)threadIdx.x) * 16u, 16);      // (rows may start anywhere)
+  };
+
+  // whole passes, one of them on its way while another is worked on
+  const int last = to < V / N ? to : V / N;         // (all pieces of the row but its last hold N logits)
+  int j0 = from;
+  u32x4 one[FLIGHT], two[FLIGHT];
+  if (j0 + PASS <= last) fetch(one, j0);
+  while (j0 + 2 * PASS <= last) {
+    fetch(two, j0 + PASS);
+    __builtin_amdgcn_sched_barrier(0);
+    take(one, j0);
+    j0 += PASS;
+    #pragma unroll
+    for (int f = 0; f < FLIGHT; ++f) one[f] = two[f];
+  }
+  if (j0 + PASS <= last) {
+    take(one, j0);
+    j0 += PASS;
+  }
+  // what is left, less than a pass and the row's last piece
+  for (; j0 < to; j0 += PASS) {
+    #pragma unroll
+    for (int f = 0; f < FLIGHT; ++f) {
+      const int j = j0 + f * THREADS + (int)threadIdx.x;
+      one[f] = N == 4 ? u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u}            // -inf
+                      : u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u} & (BF == ROW_F16 ? 0xfc00fc00u : ~0u);
+      if (j < last) {
+        __builtin_memcpy(&one[f], x + (uint32_t)j * 16u, 16);
+      } else if (j < to) {
+        float v[N];
+        #pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = j * N + i < V ? load_scalar<BF>(x, j * N + i) : -__builtin_inff();
+        one[f] = pack<BF>(v);
+      }
+    }
+    take(one, j0);
   }
   if constexpr (TOP) drain();
   if (!join_waves<TOP>(s, best)) return;
@@ -286,7 +356,7 @@ int lcq_token_logprobs(const void* logits, int dtype, int64_t T, int64_t V, int6
   if (!logits || T <= 0 || V <= 0 || ldx < 0 || m < 0 || k < 0 || k > 64 || k > V) return LCQ_EINVAL;
   if ((m > 0 && (!tokens || !logprobs)) || (k > 0 && (!top_logprobs || !top_tokens))) return LCQ_EINVAL;
   if (dtype != LCQ_F32 && dtype != LCQ_BF16 && dtype != LCQ_F16) return LCQ_EDTYPE;
-  if (T > 0x7fffffff || V > 0x7fffffff) return LCQ_ESIZE;
+  if (T > 0x7fffffff || V > (1 << 28)) return LCQ_ESIZE;
   if ((uintptr_t)logits % (dtype == LCQ_F32 ? 4 : 2)) return LCQ_EALIGN;
   LogprobArgs a = {logits, tokens, logprobs, entropy, top_logprobs, top_tokens, V, ldx, m, ignore, k, parts_of(T, V, dtype), 0, nullptr, nullptr};
   if (a.parts > 1) {
@@ -296,7 +366,7 @@ int lcq_token_logprobs(const void* logits, int dtype, int64_t T, int64_t V, int6
     a.keys = (uint64_t*)(a.sums + T * a.parts);
   }
   const int n = dtype == LCQ_F32 ? 4 : 8;
-  a.per = ((V + n - 1) / n + 1 + a.parts - 1) / a.parts;       // (one more piece where a row does not start on 16 bytes)
+  a.per = (int)(((V + n - 1) / n + a.parts - 1) / a.parts);
   const dim3 grid((unsigned)(T * a.parts)), block(THREADS);
   hipStream_t st = (hipStream_t)stream;
   const auto run = [&](auto bf) {

@@ -8,7 +8,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib as L
-from .w8a8 import _on, _rows
+from .w8a8 import _code, _here, _rows, _workspace
 
 MOST_TOP = 64
 
@@ -20,7 +20,6 @@ class TokenLogprobs(NamedTuple):
     top_tokens: torch.Tensor                  # int64 [..., top]
 
 
-@torch.no_grad()
 def token_logprobs(logits, tokens=None, top=0, ignore_index=-100):
     """logits [..., V] (fp32, bf16, fp16); tokens int64 [...] or [..., m], the ids whose log probability is asked for.
 
@@ -30,7 +29,7 @@ def token_logprobs(logits, tokens=None, top=0, ignore_index=-100):
     if logits.dim() == 0 or logits.shape[-1] == 0:
         raise ValueError(f'logits need a vocabulary, got shape {tuple(logits.shape)}')
     V, lead = logits.shape[-1], logits.shape[:-1]
-    code = L.dtype_code(logits.dtype)
+    code = _code(logits.dtype)
     if not 0 <= top <= min(MOST_TOP, V):
         raise ValueError(f'top {top}: between 0 and {min(MOST_TOP, V)}')
     m = 0
@@ -43,19 +42,19 @@ def token_logprobs(logits, tokens=None, top=0, ignore_index=-100):
             m = tokens.shape[-1]
         else:
             raise ValueError(f'tokens {tuple(tokens.shape)} next to logits {tuple(logits.shape)}')
-    with _on(logits, tokens=tokens):
-        dev = logits.device
-        rows, T, ld = _rows(logits, V)
-        ids = None if tokens is None else tokens.contiguous()
-        logprobs = None if tokens is None else torch.empty(tokens.shape, dtype=torch.float32, device=dev)
-        entropy = torch.empty(lead, dtype=torch.float32, device=dev)
-        top_logprobs = torch.empty((*lead, top), dtype=torch.float32, device=dev)
-        top_tokens = torch.empty((*lead, top), dtype=torch.int64, device=dev)
-        if T:
-            lib = L.lib()
-            size = lib.lcq_token_logprobs_workspace_bytes(T, V, top)
-            ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-            L.check(lib.lcq_token_logprobs(rows.data_ptr(), code, T, V, ld, ids.data_ptr() if m else None, m, ignore_index,
+    if not _here(logits, tokens):
+        with torch.cuda.device(logits.device):
+            return token_logprobs(logits, tokens, top, ignore_index)
+    dev = logits.device
+    rows, T, ld = _rows(logits, V)
+    ids = None if tokens is None else tokens.contiguous()
+    logprobs = None if tokens is None else torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+    top_logprobs = torch.empty((*lead, top), dtype=torch.float32, device=dev)
+    top_tokens = torch.empty((*lead, top), dtype=torch.int64, device=dev)
+    if T:
+        ws = _workspace(logits, 'lcq_token_logprobs_workspace_bytes', T, V, top)
+        L.check(L.lib().lcq_token_logprobs(rows.data_ptr(), code, T, V, ld, ids.data_ptr() if m else None, m, ignore_index,
                                            logprobs.data_ptr() if m else None, entropy.data_ptr(), top,
                                            top_logprobs.data_ptr() if top else None, top_tokens.data_ptr() if top else None,
                                            L.ptr(ws), L.stream()), 'lcq_token_logprobs')

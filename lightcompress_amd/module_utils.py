@@ -242,7 +242,6 @@ class VllmRealQuantLinear(_RealQuantLinear):
         new_module.__dict__['act_form'] = _act_form(quant_config)
         return new_module
 
-    @torch.no_grad()
     def forward(self, x, out_dtype=None):
         """x [..., in_features] as values, or as codes that a norm before it made (QuantizedTokens; their output has the type of
         the weight's scales)."""

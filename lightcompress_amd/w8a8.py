@@ -8,7 +8,7 @@ All of this is forward only: nothing here records a gradient.
 """
 from __future__ import annotations
 
-from contextlib import nullcontext
+from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
@@ -32,18 +32,36 @@ class ResidualNorm(NamedTuple):
     residual: torch.Tensor
 
 
-_HERE = nullcontext()
+_CODES = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
+_current = torch._C._cuda_getDevice
 
 
-def _on(x, **others):
-    """Checks that all tensors are on x's GPU; a context in which that GPU is the current one."""
-    if not x.is_cuda:
-        raise L.LcqError('liblcq operates on GPU tensors only (no CPU fallback)')
+def _code(dtype):
+    code = _CODES.get(dtype)
+    return L.dtype_code(dtype) if code is None else code
+
+
+def _here(x, *others):
+    """Checks that all tensors are on x's GPU.  -> is that the current one?  (If not, the caller runs again with it made current:
+    kernels go to the current device's current stream.)"""
     index = x.get_device()
-    for name, t in others.items():
+    if index < 0:
+        raise L.LcqError('liblcq operates on GPU tensors only (no CPU fallback)')
+    for t in others:
         if t is not None and t.get_device() != index:
-            raise L.LcqError(f'{name} is on {t.device}, the tokens are on {x.device}')
-    return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+            raise L.LcqError(f'a tensor of the call is on {t.device}, the tokens are on {x.device}')
+    return index == _current()
+
+
+@lru_cache(maxsize=1024)
+def _bytes(entry, *sizes):
+    """What a workspace entry of the library answers for these sizes (its answer depends on nothing else)."""
+    return getattr(L.lib(), entry)(*sizes)
+
+
+def _workspace(x, entry, *sizes):
+    size = _bytes(entry, *sizes)
+    return torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
 
 
 def _rows(t, K):
@@ -72,22 +90,23 @@ def _given(scale, symmetric):
     return scale.reshape(1).float()
 
 
-@torch.no_grad()
 def quantize_tokens(x, symmetric=True, scale=None):
     """Int8 codes of the tokens x [..., K] (fp32, bf16, fp16), one fp32 scale per token (and, not symmetric, one zero
     point): QuantizedTokens.  `scale`: one given fp32 scale for all tokens (static activations, symmetric)."""
     K = _cols(x)
-    code = L.dtype_code(x.dtype)
-    scale = _given(scale, symmetric)
-    with _on(x, scale=scale):
-        rows, T, ld = _rows(x, K)
-        lead = x.shape[:-1]
-        codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-        scales = scale if scale is not None else torch.empty((*lead, 1), dtype=torch.float32, device=x.device)
-        zeros = None if symmetric else torch.empty((*lead, 1), dtype=torch.int32, device=x.device)
-        if T:
-            L.check(L.lib().lcq_quant_tokens(rows.data_ptr(), code, T, K, ld, not symmetric, L.ptr(scale), codes.data_ptr(),
-                                             None if scale is not None else scales.data_ptr(), L.ptr(zeros), L.stream()), 'lcq_quant_tokens')
+    code = _code(x.dtype)
+    given = _given(scale, symmetric)
+    if not _here(x, given):
+        with torch.cuda.device(x.device):
+            return quantize_tokens(x, symmetric, scale)
+    rows, T, ld = _rows(x, K)
+    one = (*x.shape[:-1], 1)
+    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scales = torch.empty(one, dtype=torch.float32, device=x.device) if given is None else given
+    zeros = None if symmetric else torch.empty(one, dtype=torch.int32, device=x.device)
+    if T:
+        L.check(L.lib().lcq_quant_tokens(rows.data_ptr(), code, T, K, ld, not symmetric, L.ptr(given), codes.data_ptr(),
+                                         scales.data_ptr(), L.ptr(zeros), L.stream()), 'lcq_quant_tokens')
     return QuantizedTokens(codes, scales, zeros)
 
 
@@ -108,7 +127,6 @@ def _check_weight(weight, weight_scales, bias, K):
     return N
 
 
-@torch.no_grad()
 def int8_matmul(tokens, weight, weight_scales, bias=None, out_dtype=torch.bfloat16):
     """Tokens as codes (QuantizedTokens, codes [..., K]) times an int8 weight [N, K] with a scale per channel ([N], [N, 1], or
     one for all; fp32, bf16, fp16), plus a bias [N]: [..., N] of `out_dtype`.  The sums are exact integers, scales and bias
@@ -122,43 +140,43 @@ def int8_matmul(tokens, weight, weight_scales, bias=None, out_dtype=torch.bfloat
     if scales.numel() not in (1, M) or (zeros is not None and zeros.numel() != M):
         raise ValueError(f'{M} token scales and zero points are needed, got {tuple(scales.shape)}'
                          + ('' if zeros is None else f' and {tuple(zeros.shape)}'))
-    with _on(codes, scales=scales, zeros=zeros, weight=weight, weight_scales=weight_scales, bias=bias):
-        if K % 16 == 0:                       # (other widths are copied to padded rows by the call itself)
-            codes, weight = _on16(codes), _on16(weight)
-        y = torch.empty((*codes.shape[:-1], N), dtype=out_dtype, device=codes.device)
-        code = L.dtype_code(out_dtype)
-        if M and N:
-            lib = L.lib()
-            size = lib.lcq_int8_matmul_workspace_bytes(M, N, K)
-            ws = torch.empty(size, dtype=torch.uint8, device=codes.device) if size else None
-            L.check(lib.lcq_int8_matmul(L.ptr(codes), L.ptr(scales), scales.numel() == 1, L.ptr(zeros), L.ptr(weight),
-                                        L.ptr(weight_scales), L.dtype_code(weight_scales.dtype), weight_scales.numel() == 1,
-                                        L.ptr(bias), 0 if bias is None else L.dtype_code(bias.dtype), M, N, K, y.data_ptr(),
-                                        code, L.ptr(ws), L.stream()), 'lcq_int8_matmul')
+    code = _code(out_dtype)
+    if not _here(codes, scales, zeros, weight, weight_scales, bias):
+        with torch.cuda.device(codes.device):
+            return int8_matmul(tokens, weight, weight_scales, bias, out_dtype)
+    if K % 16 == 0:                           # (other widths are copied to padded rows by the call itself)
+        codes, weight = _on16(codes), _on16(weight)
+    y = torch.empty((*codes.shape[:-1], N), dtype=out_dtype, device=codes.device)
+    if M and N:
+        ws = _workspace(codes, 'lcq_int8_matmul_workspace_bytes', M, N, K)
+        L.check(L.lib().lcq_int8_matmul(L.ptr(codes), L.ptr(scales), scales.numel() == 1, L.ptr(zeros), L.ptr(weight),
+                                        L.ptr(weight_scales), _code(weight_scales.dtype), weight_scales.numel() == 1, L.ptr(bias),
+                                        0 if bias is None else _code(bias.dtype), M, N, K, y.data_ptr(), code, L.ptr(ws),
+                                        L.stream()), 'lcq_int8_matmul')
     return y
 
 
-@torch.no_grad()
 def int8_linear(x, weight, weight_scales, bias=None, symmetric=True, scale=None, out_dtype=None):
     """A w8a8 Linear on x [..., K]: quantize_tokens(x, symmetric, scale), then int8_matmul to x's type (or `out_dtype`)."""
     K = _cols(x)
-    x_code = L.dtype_code(x.dtype)
-    out_dtype = out_dtype or x.dtype
-    code = L.dtype_code(out_dtype)
-    scale = _given(scale, symmetric)
+    x_code = _code(x.dtype)
+    if out_dtype is None:
+        out_dtype = x.dtype
+    code = _code(out_dtype)
+    given = _given(scale, symmetric)
     N = _check_weight(weight, weight_scales, bias, K)
-    with _on(x, scale=scale, weight=weight, weight_scales=weight_scales, bias=bias):
-        rows, M, ld = _rows(x, K)
-        if K % 16 == 0:                       # (other widths are copied to padded rows by the call itself)
-            weight = _on16(weight)
-        y = torch.empty((*x.shape[:-1], N), dtype=out_dtype, device=x.device)
-        if M and N:
-            lib = L.lib()
-            size = lib.lcq_int8_linear_workspace_bytes(M, N, K)
-            ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-            L.check(lib.lcq_int8_linear(rows.data_ptr(), x_code, ld, not symmetric, L.ptr(scale), L.ptr(weight), L.ptr(weight_scales),
-                                        L.dtype_code(weight_scales.dtype), weight_scales.numel() == 1, L.ptr(bias),
-                                        0 if bias is None else L.dtype_code(bias.dtype), M, N, K, y.data_ptr(), code, L.ptr(ws),
+    if not _here(x, given, weight, weight_scales, bias):
+        with torch.cuda.device(x.device):
+            return int8_linear(x, weight, weight_scales, bias, symmetric, scale, out_dtype)
+    rows, M, ld = _rows(x, K)
+    if K % 16 == 0:                           # (other widths are copied to padded rows by the call itself)
+        weight = _on16(weight)
+    y = torch.empty((*x.shape[:-1], N), dtype=out_dtype, device=x.device)
+    if M and N:
+        ws = _workspace(x, 'lcq_int8_linear_workspace_bytes', M, N, K)
+        L.check(L.lib().lcq_int8_linear(rows.data_ptr(), x_code, ld, not symmetric, L.ptr(given), L.ptr(weight), L.ptr(weight_scales),
+                                        _code(weight_scales.dtype), weight_scales.numel() == 1, L.ptr(bias),
+                                        0 if bias is None else _code(bias.dtype), M, N, K, y.data_ptr(), code, L.ptr(ws),
                                         L.stream()), 'lcq_int8_linear')
     return y
 
@@ -176,7 +194,6 @@ def _affine(name, t, K, x, flag):
     return flag
 
 
-@torch.no_grad()
 def residual_norm(x, residual=None, weight=None, bias=None, *, gate=None, post_weight=None, post_bias=None, scale=1.0,
                   eps=1e-6, kind='rms', weight_offset=0.0, quantize=None, out_dtype=None, inplace=False):
     """The end of one block and the start of the next, for the block's output x [..., K], in one pass:
@@ -190,7 +207,7 @@ def residual_norm(x, residual=None, weight=None, bias=None, *, gate=None, post_w
     weight is 1 without an offset.  quantize 'symmetric' / 'asymmetric': out is quantize_tokens of the unrounded norm.
     out_dtype: x's type (default) or fp32.  inplace: h is written over residual.  -> ResidualNorm(out, residual = h)"""
     K = _cols(x)
-    code = L.dtype_code(x.dtype)
+    code = _code(x.dtype)
     if kind not in ('rms', 'layer') or quantize not in (None, 'symmetric', 'asymmetric'):
         raise ValueError(f'kind {kind!r}, quantize {quantize!r}')
     if post_bias is not None and post_weight is None:
@@ -220,30 +237,29 @@ def residual_norm(x, residual=None, weight=None, bias=None, *, gate=None, post_w
         flags |= NORM_OUT_F32
     else:
         raise L.LcqError(f'out_dtype {out_dtype}: x\'s {x.dtype} or float32 is needed')
-    with _on(x, residual=residual, weight=weight, bias=bias, gate=gate, post_weight=post_weight, post_bias=post_bias):
-        rows, T, ldx = _rows(x, K)
-        res, ldr, g, ldg = residual, 0, gate, 0
-        if residual is not None:
-            res, _, ldr = _rows(residual, K)
-        if gate is not None and gate.dim() == 1:
-            g = gate.contiguous()
-            ldg = 0
-        elif gate is not None:
-            g, _, ldg = _rows(gate, K)
-        h = residual if inplace else torch.empty(x.shape, dtype=stream_dtype, device=x.device)
-        out = codes = scales = zeros = None
-        if quantize is None:
-            out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-        else:
-            codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-            scales = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=x.device)
-            if quantize == 'asymmetric':
-                flags |= NORM_ASYM
-                zeros = torch.empty((*x.shape[:-1], 1), dtype=torch.int32, device=x.device)
-        if T:
-            at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-            L.check(L.lib().lcq_residual_norm(rows.data_ptr(), code, T, K, ldx, at(res), ldr, at(g), ldg, L.ptr(post_weight),
-                                              L.ptr(post_bias), L.ptr(weight), L.ptr(bias), scale, eps, weight_offset, flags,
-                                              h.data_ptr(), at(out), at(codes), at(scales), at(zeros), L.stream()),
-                    'lcq_residual_norm')
+    if not _here(x, residual, weight, bias, gate, post_weight, post_bias):
+        with torch.cuda.device(x.device):
+            return residual_norm(x, residual, weight, bias, gate=gate, post_weight=post_weight, post_bias=post_bias, scale=scale,
+                                 eps=eps, kind=kind, weight_offset=weight_offset, quantize=quantize, out_dtype=out_dtype, inplace=inplace)
+    rows, T, ldx = _rows(x, K)
+    res, ldr, g, ldg = residual, 0, gate, 0
+    if residual is not None:
+        res, _, ldr = _rows(residual, K)
+    if gate is not None:
+        g, _, ldg = (gate.contiguous(), 1, 0) if gate.dim() == 1 else _rows(gate, K)
+    h = residual if inplace else torch.empty(x.shape, dtype=stream_dtype, device=x.device)
+    out = codes = scales = zeros = None
+    if quantize is None:
+        out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    else:
+        codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+        scales = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=x.device)
+        if quantize == 'asymmetric':
+            flags |= NORM_ASYM
+            zeros = torch.empty((*x.shape[:-1], 1), dtype=torch.int32, device=x.device)
+    if T:
+        at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        L.check(L.lib().lcq_residual_norm(rows.data_ptr(), code, T, K, ldx, at(res), ldr, at(g), ldg, L.ptr(post_weight),
+                                          L.ptr(post_bias), L.ptr(weight), L.ptr(bias), scale, eps, weight_offset, flags,
+                                          h.data_ptr(), at(out), at(codes), at(scales), at(zeros), L.stream()), 'lcq_residual_norm')
     return ResidualNorm(out if quantize is None else QuantizedTokens(codes, scales, zeros), h)
