@@ -35,11 +35,11 @@ struct LogprobArgs {
 
 // A whole number that orders logits by value and, among equal ones, by the lowest index; a NaN is above everything, -0 equals +0.
 // 0 is below every logit's.
-__device__ __forceinline__ uint64_t key_of(float x, uint32_t index) {
-  uint32_t u = x == x ? f2u(x + 0.0f) : 0x7fc00000u;
-  u = (u & 0x80000000u) ? ~u : u | 0x80000000u;
-  return (uint64_t)u << 32 | (0xffffffffu - index);
+__device__ __forceinline__ uint32_t rank_of(float x) {      // the upper half: equal logits, equal ranks
+  const uint32_t u = x == x ? f2u(x + 0.0f) : 0x7fc00000u;
+  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ uint64_t key_of(float x, uint32_t index) { return (uint64_t)rank_of(x) << 32 | (0xffffffffu - index); }
 __device__ __forceinline__ float logit_of(uint64_t key) {
   const uint32_t u = (uint32_t)(key >> 32);
   return u2f((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
@@ -68,49 +68,64 @@ __device__ __forceinline__ uint32_t across(uint32_t v) {
     return threadIdx.x & 32 ? r[0] : r[1];
   }
 }
-// lane i and lane i ^ D: the larger key to the lower lane where `down`, else the other way
-template <int D>
-__device__ __forceinline__ uint64_t exchange(uint64_t v, int lane, bool down) {
-  const uint64_t o = (uint64_t)across<D>((uint32_t)(v >> 32)) << 32 | across<D>((uint32_t)v);
-  return (((lane & D) == 0) == down) == (v > o) ? v : o;
+template <int D> __device__ __forceinline__ uint64_t across(uint64_t v) { return (uint64_t)across<D>((uint32_t)(v >> 32)) << 32 | across<D>((uint32_t)v); }
+// lane i and lane i ^ D, in blocks of N lanes whose order turns from block to block (down first): the larger value to the lane it belongs to
+template <int D, int N, class K>
+__device__ __forceinline__ K exchange(K v) {
+  constexpr uint64_t larger = [] {
+    uint64_t m = 0;
+    for (int l = 0; l < 64; ++l) m |= (uint64_t)(((l & D) == 0) == ((l & N) == 0)) << l;
+    return m;
+  }();
+  const K o = across<D>(v);
+  if constexpr (sizeof(K) == 4) return __builtin_amdgcn_inverse_ballot_w64(larger) ? (v > o ? v : o) : (v > o ? o : v);
+  else return __builtin_amdgcn_inverse_ballot_w64(~(larger ^ __builtin_amdgcn_ballot_w64(v > o))) ? v : o;
 }
-// a bitonic sequence of N lanes into order
-template <int N>
-__device__ __forceinline__ uint64_t ordered(uint64_t v, int lane, bool down) {
-  if constexpr (N > 1) return ordered<N / 2>(exchange<N / 2>(v, lane, down), lane, down);
+// bitonic sequences of N lanes into order, step by step
+template <int D, int N, class K>
+__device__ __forceinline__ K ordered(K v) {
+  if constexpr (D > 0) return ordered<D / 2, N>(exchange<D, N>(v));
   return v;
 }
-// the wave's 64 keys in descending order
-__device__ __forceinline__ uint64_t sorted(uint64_t v, int lane) {
-  v = ordered<2>(v, lane, (lane & 2) == 0);
-  v = ordered<4>(v, lane, (lane & 4) == 0);
-  v = ordered<8>(v, lane, (lane & 8) == 0);
-  v = ordered<16>(v, lane, (lane & 16) == 0);
-  v = ordered<32>(v, lane, (lane & 32) == 0);
-  return ordered<64>(v, lane, true);
+// the wave's 64 values in descending order
+template <class K>
+__device__ __forceinline__ K sorted(K v) {
+  v = ordered<1, 2>(v);
+  v = ordered<2, 4>(v);
+  v = ordered<4, 8>(v);
+  v = ordered<8, 16>(v);
+  v = ordered<16, 32>(v);
+  return ordered<32, 64>(v);
 }
 // the 64 largest of two descending lists, `turned` with its lanes in ascending order
-__device__ __forceinline__ uint64_t merged(uint64_t v, uint64_t turned, int lane) { return ordered<64>(v > turned ? v : turned, lane, true); }
+__device__ __forceinline__ uint64_t merged(uint64_t v, uint64_t turned) { return ordered<32, 64>(v > turned ? v : turned); }
 
-// The best 64 of a wave.  `count` and `bound` are the same in all lanes.
+// The best 64 of a wave.  `bound`, `limit` and `some` are the same in all lanes.
 struct Best {
-  uint64_t mine = 0, bound = 0;                     // lane i: the i-th best; the k-th best, 0 while there are fewer
-  float limit = -__builtin_inff();                  // bound's logit: a logit below it is not among the best k
+  uint64_t mine = 0, bound = 0;                   
+  float limit = -__builtin_inff();                  // a logit below it is not among the best k
+  bool some = false;                                // `mine` holds something
   int lane, k;
   __device__ __forceinline__ Best(int lane_, int k_) : lane(lane_), k(k_) {}
-  __device__ __forceinline__ void raise(uint64_t key) {
-    if (key > bound) { bound = key; limit = logit_of(key); }
-    limit = limit == limit ? limit : __builtin_inff();       // (k NaNs: whatever is not one stays out; a NaN passes every limit)
+  // at least k keys lie above `key`; the k-th best logit is that of `rank` or larger
+  __device__ __forceinline__ void raise(uint64_t key, uint32_t rank) {
+    if (key <= bound) return;
+    bound = key;
+    const float x = logit_of((uint64_t)rank << 32);
+    limit = x == x ? x : __builtin_inff();          // (k NaNs: whatever is not one stays out; a NaN passes every limit)
   }
-  __device__ __forceinline__ uint64_t kth(uint64_t v) const {
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, k - 1), hi = (uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), k - 1);
-    return (uint64_t)hi << 32 | lo;
-  }
+  // at least k logits reach `rank`; keys of that rank are still to be collected
+  __device__ __forceinline__ void raise_to(uint32_t rank) { if (rank) raise(((uint64_t)rank << 32) - 1, rank); }
+  // the k-th largest of 64 ranks
+  __device__ __forceinline__ uint32_t kth(uint32_t rank) const { return (uint32_t)__builtin_amdgcn_readlane((int)sorted(rank), k - 1); }
   // one key per lane (0: none)
   __device__ __forceinline__ void take(uint64_t key) {
     if (__builtin_amdgcn_ballot_w64(key > bound) == 0) return;
-    mine = merged(mine, other_lane(sorted(key, lane), 63 - lane), lane);
-    raise(kth(mine));
+    const uint64_t s = sorted(key);
+    mine = some ? merged(mine, other_lane(s, 63 - lane)) : s;
+    some = true;
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)mine, k - 1), hi = (uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), k - 1);
+    if (hi) raise((uint64_t)hi << 32 | lo, hi);
   }
 };
 
@@ -131,15 +146,12 @@ struct Sums {
   }
 };
 
-// What a workgroup's waves found, joined in wave 0 -> true there
-template <bool TOP>
-__device__ __forceinline__ bool join_waves(Sums& s, Best& best) {
+// The waves' sums joined in wave 0 -> true there.  Its barrier is also what the waves' lists in LDS wait for.
+__device__ __forceinline__ bool join_sums(Sums& s) {
   __shared__ float part[WAVES][3];
-  __shared__ uint64_t keys[TOP ? WAVES : 1][64];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   s.join_wave();
   if (lane == 0) { part[wave][0] = s.c; part[wave][1] = s.S; part[wave][2] = s.U; }
-  if (TOP) keys[wave][lane] = best.mine;
   __syncthreads();
   if (wave) return false;
   float c = s.c;
@@ -152,18 +164,84 @@ __device__ __forceinline__ bool join_waves(Sums& s, Best& best) {
     o.c = part[w][0]; o.S = part[w][1]; o.U = part[w][2];
     o.refer(c);
     s.add(o);
-    if (TOP) best.mine = merged(best.mine, keys[w][63 - lane], lane);
   }
   return true;
 }
+// What the waves of a workgroup collect: keys that may be among the best k, in LDS until there are 64 of them.
+template <int ROOM>
+struct Lists {
+  uint64_t found[WAVES][ROOM], best[WAVES][64];
+  int count[WAVES], some[WAVES];
+  uint32_t rank;                                    // at least k logits of the row reach it: the best of the waves' bounds
+};
+template <int ROOM>
+struct Collector {
+  Lists<ROOM>& l;
+  Best best;
+  int count = 0, wave;
+  __device__ __forceinline__ Collector(Lists<ROOM>& l_, int wave_, int lane, int k) : l(l_), best(lane, k), wave(wave_) {}
+  __device__ __forceinline__ void collect(bool in, uint64_t key) {
+    const uint64_t lanes = __builtin_amdgcn_ballot_w64(in);
+    if (in) l.found[wave][count + __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0))] = key;
+    count += __builtin_popcountll(lanes);
+  }
+  __device__ __forceinline__ void drain() {
+    #pragma unroll 1
+    for (int at = 0; at < count; at += 64) best.take(at + best.lane < count ? l.found[wave][at + best.lane] : 0);
+    count = 0;
+  }
+  __device__ __forceinline__ void share() {
+    if (best.lane == 0 && best.bound) __hip_atomic_fetch_max(&l.rank, (uint32_t)((best.bound + 1) >> 32), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  }
+  __device__ __forceinline__ uint32_t shared() const { return __hip_atomic_load(&l.rank, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
+  __device__ __forceinline__ void leave() {         // for the wave that joins them, behind a barrier
+    if (best.some) l.best[wave][best.lane] = best.mine;
+    if (best.lane == 0) { l.count[wave] = count; l.some[wave] = best.some; }
+  }
+  // wave 0: everything that the waves have collected and not sorted, 64 at a time, then their lists
+  __device__ __forceinline__ void join() {
+    int end[WAVES], total = 0;
+    #pragma unroll
+    for (int w = 0; w < WAVES; ++w) end[w] = total += l.count[w];
+    #pragma unroll 1
+    for (int at = 0; at < total; at += 64) {
+      const int i = at + best.lane;
+      int w = 0, begin = 0;
+      #pragma unroll
+      for (int v = 0; v < WAVES - 1; ++v)
+        if (i >= end[v]) { w = v + 1; begin = end[v]; }
+      best.take(i < total ? l.found[w][i - begin] : 0);
+    }
+    #pragma unroll 1
+    for (int w = 1; w < WAVES; ++w)
+      if (l.some[w]) {
+        best.mine = best.some ? merged(best.mine, l.best[w][63 - best.lane]) : l.best[w][best.lane];
+        best.some = true;
+      }
+  }
+};
+
+// The row's first 64 given tokens, one per lane, read early: their logits are on their way while the lists are joined.
+template <int BF>
+struct Given {
+  int64_t token = 0;
+  float x = 0.0f;
+  __device__ __forceinline__ void tokens(const LogprobArgs& a, int64_t row, int lane) { if (lane < a.m) token = a.tokens[row * a.m + lane]; }
+  __device__ __forceinline__ void logits(const LogprobArgs& a, int64_t row, int lane) {
+    if (lane < a.m && token >= 0 && token < a.V) x = load_scalar<BF>(a.x, row * a.ldx + token);
+  }
+};
 
 template <int BF>
-__device__ __forceinline__ void answer(const LogprobArgs& a, int64_t row, const Sums& s, uint64_t mine, int lane) {
+__device__ __forceinline__ void answer(const LogprobArgs& a, int64_t row, const Sums& s, Given<BF> g, uint64_t mine, int lane) {
   const float l = logf(s.S);
   if (lane == 0 && a.entropy) a.entropy[row] = l - s.U / s.S;
   for (int64_t j = lane; j < a.m; j += 64) {
-    const int64_t t = a.tokens[row * a.m + j];
-    a.logprobs[row * a.m + j] = t == a.ignore ? 0.0f : t < 0 || t >= a.V ? __builtin_nanf("") : (load_scalar<BF>(a.x, row * a.ldx + t) - s.c) - l;
+    if (j >= 64) {
+      g.token = a.tokens[row * a.m + j];
+      if (g.token >= 0 && g.token < a.V) g.x = load_scalar<BF>(a.x, row * a.ldx + g.token);
+    }
+    a.logprobs[row * a.m + j] = g.token == a.ignore ? 0.0f : g.token < 0 || g.token >= a.V ? __builtin_nanf("") : (g.x - s.c) - l;
   }
   if (lane < a.k) {
     a.top_logprobs[row * a.k + lane] = (logit_of(mine) - s.c) - l;
@@ -174,64 +252,29 @@ __device__ __forceinline__ void answer(const LogprobArgs& a, int64_t row, const 
 template <int BF, bool TOP>
 __global__ __launch_bounds__(THREADS) void logprobs_kernel(LogprobArgs a) {
   constexpr int N = Vec<BF>::N, PASS = THREADS * FLIGHT;
-  __shared__ uint64_t found[TOP ? WAVES : 1][TOP ? 64 * N + 64 : 1];
-  __shared__ uint32_t shared;                       // the upper half of a key: the largest k-th best that a wave has
-  if (threadIdx.x == 0) shared = 0;
-  if constexpr (TOP) __syncthreads();
+  __shared__ Lists<TOP ? 64 * N + 64 : 1> lists;
+  if constexpr (TOP) {
+    if (threadIdx.x == 0) lists.rank = 0;
+    __syncthreads();
+  }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row = (int64_t)blockIdx.x / a.parts;
-  const int part = (int)((int64_t)blockIdx.x - row * a.parts);
+  const int64_t row = blockIdx.x;
+  const int part = blockIdx.y;
   const char* const x = (const char*)a.x + row * a.ldx * (16 / N);
   const int V = (int)a.V, pieces = (V + N - 1) / N;
   const int from = part * a.per, to = from + a.per < pieces ? from + a.per : pieces;
 
+  Given<BF> given;
+  if (a.parts == 1 && wave == 0) given.tokens(a, row, lane);
   Sums s;
-  Best best(lane, TOP ? a.k : 1);
-  int count = 0;
-  const auto drain = [&]() __attribute__((always_inline)) {                          // takes over what was collected
-    for (int at = 0; at < count; at += 64) best.take(at + lane < count ? found[wave][at + lane] : 0);
-    count = 0;
-  };
-  // The waves share the best of their bounds: what lies below one wave's k-th best is not among the row's.
-  const auto share = [&]() __attribute__((always_inline)) {
-    if (lane == 0 && best.bound) __hip_atomic_fetch_max(&shared, (uint32_t)(best.bound >> 32), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-  };
-  // piece j of the row, its largest logit `top` (one that lies past the row's end holds nothing): what of it may be among the best
-  const auto consider = [&](const u32x4& raw, float top, int j) __attribute__((always_inline)) {
-    float v[N];
-    unpack<BF>(raw, v);
-    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(!(top < best.limit))) > 16) {
-      uint64_t m = 0;
-      #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const uint64_t key = (int64_t)j * N + i < V ? key_of(v[i], (uint32_t)(j * N + i)) : 0;
-        m = key > m ? key : m;
-      }
-      m = best.kth(sorted(m, lane));
-      if (m) best.raise(m - 1);                     // (less one: the k-th itself has still to be collected)
-      share();
-    }
-    #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (__builtin_amdgcn_ballot_w64(!(v[i] < best.limit)) == 0) continue;
-      const uint64_t key = (int64_t)j * N + i < V ? key_of(v[i], (uint32_t)(j * N + i)) : 0;
-      const bool in = key > best.bound && !(v[i] < best.limit);
-      const uint64_t lanes = __builtin_amdgcn_ballot_w64(in);
-      if (in) found[wave][count + __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0))] = key;
-      count += __builtin_popcountll(lanes);
-    }
-    if (count >= 64) {
-      drain();
-      share();
-    }
-  };
+  Collector<TOP ? 64 * N + 64 : 1> c(lists, wave, lane, TOP ? a.k : 1);
   // the pieces j0 + f THREADS of this lane
   const auto take = [&](const u32x4 (&raw)[FLIGHT], int j0) __attribute__((always_inline)) {
     float top[FLIGHT];
-    uint64_t pass[FLIGHT], any = 0;
+    float limit = c.best.limit;
     if constexpr (TOP) {
-      const float theirs = logit_of((uint64_t)__hip_atomic_load(&shared, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) << 32);
-      best.limit = theirs > best.limit ? theirs : best.limit;
+      const float theirs = logit_of((uint64_t)c.shared() << 32);
+      limit = theirs > limit ? theirs : limit;
     }
     #pragma unroll
     for (int f = 0; f < FLIGHT; ++f) {
@@ -240,7 +283,6 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(LogprobArgs a) {
       top[f] = v[0];
       #pragma unroll
       for (int i = 1; i < N; ++i) top[f] = nan_max(top[f], v[i]);
-      if constexpr (TOP) any |= pass[f] = __builtin_amdgcn_ballot_w64(!(top[f] < best.limit));
       if (top[f] > s.c + MOVE) s.refer(top[f]);
       #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -250,88 +292,134 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(LogprobArgs a) {
       }
     }
     if constexpr (TOP) {
-      if (__builtin_expect(any != 0, 0)) {
+      float most = top[0];
+      #pragma unroll
+      for (int f = 1; f < FLIGHT; ++f) most = nan_max(most, top[f]);
+      const uint64_t pass = __builtin_amdgcn_ballot_w64(!(most < limit));
+      if (__builtin_expect(pass != 0, 0)) {
+        c.best.raise_to(c.shared());
+        if (__builtin_popcountll(pass) > 16) {
+          c.best.raise_to(c.best.kth(rank_of(most)));
+          c.share();
+        }
         #pragma unroll 1
         for (int f = 0; f < FLIGHT; ++f) {          // (one copy of the code for all of them)
           u32x4 r = raw[0];
           float t = top[0];
-          uint64_t p = pass[0];
           #pragma unroll
-          for (int g = 1; g < FLIGHT; ++g) { r = f == g ? raw[g] : r; t = f == g ? top[g] : t; p = f == g ? pass[g] : p; }
-          if (p) consider(r, t, j0 + f * THREADS + (int)threadIdx.x);
+          for (int g = 1; g < FLIGHT; ++g) { r = f == g ? raw[g] : r; t = f == g ? top[g] : t; }
+          if (__builtin_amdgcn_ballot_w64(!(t < c.best.limit)) == 0) continue;
+          const int64_t v0 = (int64_t)(j0 + f * THREADS + (int)threadIdx.x) * N;             // (past the row's end: holds nothing)
+          float v[N];
+          unpack<BF>(r, v);
+          #pragma unroll
+          for (int i = 0; i < N; ++i) {
+            if (__builtin_amdgcn_ballot_w64(!(v[i] < c.best.limit)) == 0) continue;
+            const uint64_t key = v0 + i < V ? key_of(v[i], (uint32_t)(v0 + i)) : 0;
+            c.collect(key > c.best.bound, key);
+          }
+          if (c.count >= 64) {
+            c.drain();
+            c.share();
+          }
         }
       }
     }
   };
-  const auto fetch = [&](u32x4 (&raw)[FLIGHT], int j0) {    // whole pieces
-    #pragma unroll
-    for (int f = 0; f < FLIGHT; ++f) __builtin_memcpy(&raw[f], x + (uint32_t)(j0 + f * THREADS + (int)threadIdx.x) * 16u, 16);      // (rows may start anywhere)
-  };
 
-  // whole passes, one of them on its way while another is worked on
+  // A pass is on its way while the one in front of it is worked on.  Rows may start anywhere.
   const int last = to < V / N ? to : V / N;         // (all pieces of the row but its last hold N logits)
-  int j0 = from;
   u32x4 one[FLIGHT], two[FLIGHT];
-  if (j0 + PASS <= last) fetch(one, j0);
-  while (j0 + 2 * PASS <= last) {
-    fetch(two, j0 + PASS);
+  for (int j0 = from - PASS; j0 < to; j0 += PASS) {
+    const int next = j0 + PASS;
+    if (next + PASS <= last) {
+      #pragma unroll
+      for (int f = 0; f < FLIGHT; ++f) __builtin_memcpy(&two[f], x + (uint32_t)(next + f * THREADS + (int)threadIdx.x) * 16u, 16);
+    } else if (next < to) {
+      #pragma unroll
+      for (int f = 0; f < FLIGHT; ++f) {
+        const int j = next + f * THREADS + (int)threadIdx.x;
+        two[f] = N == 4 ? u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u}          // -inf
+                        : u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u} & (BF == ROW_F16 ? 0xfc00fc00u : ~0u);
+        if (j < last) {
+          __builtin_memcpy(&two[f], x + (uint32_t)j * 16u, 16);
+        } else if (j < to) {
+          float v[N];
+          #pragma unroll
+          for (int i = 0; i < N; ++i) v[i] = j * N + i < V ? load_scalar<BF>(x, j * N + i) : -__builtin_inff();
+          two[f] = pack<BF>(v);
+        }
+      }
+    }
     __builtin_amdgcn_sched_barrier(0);
-    take(one, j0);
-    j0 += PASS;
+    if (j0 >= from) take(one, j0);
     #pragma unroll
     for (int f = 0; f < FLIGHT; ++f) one[f] = two[f];
   }
-  if (j0 + PASS <= last) {
-    take(one, j0);
-    j0 += PASS;
-  }
-  // what is left, less than a pass and the row's last piece
-  for (; j0 < to; j0 += PASS) {
-    #pragma unroll
-    for (int f = 0; f < FLIGHT; ++f) {
-      const int j = j0 + f * THREADS + (int)threadIdx.x;
-      one[f] = N == 4 ? u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u}            // -inf
-                      : u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u} & (BF == ROW_F16 ? 0xfc00fc00u : ~0u);
-      if (j < last) {
-        __builtin_memcpy(&one[f], x + (uint32_t)j * 16u, 16);
-      } else if (j < to) {
-        float v[N];
-        #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = j * N + i < V ? load_scalar<BF>(x, j * N + i) : -__builtin_inff();
-        one[f] = pack<BF>(v);
-      }
-    }
-    take(one, j0);
-  }
-  if constexpr (TOP) drain();
-  if (!join_waves<TOP>(s, best)) return;
+  if (a.parts == 1 && wave == 0) given.logits(a, row, lane);
+  if constexpr (TOP) c.leave();
+  if (!join_sums(s)) return;
+  if constexpr (TOP) c.join();
   if (a.parts == 1) {
-    answer<BF>(a, row, s, best.mine, lane);
+    answer<BF>(a, row, s, given, c.best.mine, lane);
     return;
   }
-  if (lane == 0) a.sums[blockIdx.x] = f32x4{s.c, s.S, s.U, 0.0f};
-  if (lane < a.k) a.keys[(int64_t)blockIdx.x * a.k + lane] = best.mine;
+  const int64_t at = row * a.parts + part;
+  if (lane == 0) a.sums[at] = f32x4{s.c, s.S, s.U, 0.0f};
+  if (lane < a.k) a.keys[at * a.k + lane] = c.best.mine;
 }
 
 // The parts of a row joined: one workgroup per row.
 template <int BF>
 __global__ __launch_bounds__(THREADS) void join_kernel(LogprobArgs a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ Lists<128> lists;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row = blockIdx.x;
+  Given<BF> given;
+  if (wave == 0) given.tokens(a, row, lane);
+  const f32x4* const sums = a.sums + row * a.parts;
+  const int all = a.parts * a.k;
+  const uint64_t* const keys = a.keys + row * all;
+  constexpr int KEEP = 8;                           // loads that a lane has in flight
+  uint64_t key[KEEP];
+  const auto fetch = [&](int at) __attribute__((always_inline)) {
+    #pragma unroll
+    for (int i = 0; i < KEEP; ++i) key[i] = at + i * THREADS + (int)threadIdx.x < all ? keys[at + i * THREADS + threadIdx.x] : 0;
+  };
+  f32x4 v = {LOWEST, 0.0f, 0.0f, 0.0f};
+  if ((int)threadIdx.x < a.parts) v = sums[threadIdx.x];
+  fetch(0);
   Sums s;
-  for (int p = threadIdx.x; p < a.parts; p += THREADS) {
-    const f32x4 v = a.sums[row * a.parts + p];
+  for (int p = threadIdx.x;;) {
     Sums o;
     o.c = v[0]; o.S = v[1]; o.U = v[2];
     const float c = nan_max(s.c, o.c);
     s.refer(c);
     o.refer(c);
     s.add(o);
+    if ((p += THREADS) >= a.parts) break;
+    v = sums[p];
   }
-  Best best(lane, a.k > 0 ? a.k : 1);
-  const int all = a.parts * a.k;
-  for (int i = wave * 64; i < all; i += THREADS) best.take(i + lane < all ? a.keys[row * all + i + lane] : 0);
-  if (join_waves<true>(s, best)) answer<BF>(a, row, s, best.mine, lane);
+  if (wave == 0) given.logits(a, row, lane);
+  Collector<128> c(lists, wave, lane, a.k > 0 ? a.k : 1);
+  #pragma unroll 1
+  for (int at = 0; at < all; at += KEEP * THREADS) {
+    if (at) fetch(at);
+    uint32_t most = 0;
+    #pragma unroll
+    for (int i = 0; i < KEEP; ++i) most = (uint32_t)(key[i] >> 32) > most ? (uint32_t)(key[i] >> 32) : most;
+    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(most > (uint32_t)(c.best.bound >> 32))) > 16) c.best.raise_to(c.best.kth(most));
+    #pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+      if (__builtin_amdgcn_ballot_w64(key[i] > c.best.bound) == 0) continue;
+      c.collect(key[i] > c.best.bound, key[i]);
+      if (c.count >= 64) c.drain();
+    }
+  }
+  c.leave();
+  if (!join_sums(s)) return;
+  if (all) c.join();
+  answer<BF>(a, row, s, given, c.best.mine, lane);
 }
 
 int parts_of(int64_t T, int64_t V, int dtype) {
@@ -367,7 +455,7 @@ int lcq_token_logprobs(const void* logits, int dtype, int64_t T, int64_t V, int6
   }
   const int n = dtype == LCQ_F32 ? 4 : 8;
   a.per = (int)(((V + n - 1) / n + a.parts - 1) / a.parts);
-  const dim3 grid((unsigned)(T * a.parts)), block(THREADS);
+  const dim3 grid((unsigned)T, (unsigned)a.parts), block(THREADS);
   hipStream_t st = (hipStream_t)stream;
   const auto run = [&](auto bf) {
     constexpr int BF = decltype(bf)::value;
