@@ -410,10 +410,14 @@ struct TokenRow {
     #pragma unroll
     for (int w = 0; w < WAVES; ++w) { hi = nan_max(hi, red[w]); lo = nan_min(lo, red[WAVES + w]); }
     const TokenCodes q = t.scale ? TokenCodes::given(t.scale[0]) : t.asym ? TokenCodes::asymmetric(lo, hi) : TokenCodes::symmetric(hi);
-    each([&](int i, const float* e) { *(u32x2*)(out + i) = q.codes(e); });
+    each([&](int i, const float* e) {
+      uint32_t w[2];
+      q.codes<8>(e, w);
+      *(u32x2*)(out + i) = u32x2{w[0], w[1]};
+    });
     if (threadIdx.x == 0) {
       *scale = q.d.s;
-      *zero = (int)q.z;
+      *zero = q.z;
     }
     __syncthreads();
   }

@@ -31,32 +31,47 @@ struct NormArgs {
 
 constexpr int NORM = 1 << 20;                       // (internal: y is a norm of h; without it y = h)
 
-// V consecutive elements at index i of a row of type BF, or of fp32 where f32 says so
+// n <= V consecutive elements at index i of a row of type BF, or of fp32 where f32 says so; rows may start anywhere.  Those past n are 0.
 template <int BF, int V>
-__device__ __forceinline__ void load_v(const void* p, int64_t i, bool f32, float* v) {
-  if constexpr (V == 1) {
-    v[0] = f32 ? ((const float*)p)[i] : load_scalar<BF>(p, i);
-  } else {
+__device__ __forceinline__ void load_v(const void* p, int64_t i, bool f32, float* v, int n) {
+  if (n == V) {
     if (BF == ROW_F32 || f32) {
-      unpack<ROW_F32>(*(const u32x4*)((const float*)p + i), v);
-      unpack<ROW_F32>(*(const u32x4*)((const float*)p + i + 4), v + 4);
+      #pragma unroll
+      for (int q = 0; q < V / 4; ++q) {
+        u32x4 r;
+        __builtin_memcpy(&r, (const float*)p + i + 4 * q, 16);
+        unpack<ROW_F32>(r, v + 4 * q);
+      }
     } else {
-      unpack<BF>(*(const u32x4*)((const uint16_t*)p + i), v);
+      u32x4 r;
+      __builtin_memcpy(&r, (const uint16_t*)p + i, 16);
+      unpack<BF>(r, v);
     }
+  } else {
+    #pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = j < n ? f32 ? ((const float*)p)[i + j] : load_scalar<BF>(p, i + j) : 0.0f;
   }
 }
 template <int BF, int V>
-__device__ __forceinline__ void store_v(void* p, int64_t i, bool f32, const float* v) {
-  if constexpr (V == 1) {
-    if (f32) ((float*)p)[i] = v[0];
-    else store_scalar<BF>(p, i, rnd<BF>(v[0]));
-  } else {
+__device__ __forceinline__ void store_v(void* p, int64_t i, bool f32, const float* v, int n) {
+  if (n == V) {
     if (BF == ROW_F32 || f32) {
-      *(u32x4*)((float*)p + i) = pack<ROW_F32>(v);
-      *(u32x4*)((float*)p + i + 4) = pack<ROW_F32>(v + 4);
+      #pragma unroll
+      for (int q = 0; q < V / 4; ++q) {
+        const u32x4 r = pack<ROW_F32>(v + 4 * q);
+        __builtin_memcpy((float*)p + i + 4 * q, &r, 16);
+      }
     } else {
-      *(u32x4*)((uint16_t*)p + i) = pack_rne<BF>(v);
+      const u32x4 r = pack_rne<BF>(v);
+      __builtin_memcpy((uint16_t*)p + i, &r, 16);
     }
+  } else {
+    #pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (j < n) {
+        if (f32) ((float*)p)[i + j] = v[j];
+        else store_scalar<BF>(p, i + j, rnd<BF>(v[j]));
+      }
   }
 }
 
@@ -80,9 +95,10 @@ struct Row {
   }
 };
 
-// One row per TEAM lanes, CH pieces of V elements per lane in registers; V = 8 where every row starts on 16 bytes, 1 else.
-template <int BF, int V, int TEAM, int CH>
+// One row per TEAM lanes, CH pieces of V elements (16 bytes) per lane in registers.
+template <int BF, int TEAM, int CH>
 __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void residual_norm_kernel(NormArgs a) {
+  constexpr int V = Vec<BF>::N;
   __shared__ float sm[TEAM / 64];
   const Row<TEAM> row_{sm};
   const int t = threadIdx.x % TEAM;
@@ -91,39 +107,37 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void residual_norm_kernel(
   const int K = a.K, flags = a.flags;
   const float rK = 1.0f / (float)K;
   float v[CH][V];
-  #pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    const int i = (t + c * TEAM) * V;
-    #pragma unroll
-    for (int j = 0; j < V; ++j) v[c][j] = 0.0f;
-    if (i < K) load_v<BF, V>(a.x, r * a.ldx + i, false, v[c]);
-  }
-  const auto each = [&](auto&& f) {
+  const auto each = [&](auto&& f) {                 // f(index, elements, how many of them are in the row)
     #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int i = (t + c * TEAM) * V;
-      if (i < K) f(i, v[c]);
+      if (i < K) f(i, v[c], K - i < V ? K - i : V);
     }
   };
+  each([&](int i, float* e, int n) { load_v<BF, V>(a.x, r * a.ldx + i, false, e, n); });
   const auto norm = [&](const void* w, bool w32, const void* b, bool b32) {
     float sum = 0.0f, mean = 0.0f;
     if (flags & LCQ_NORM_LAYER) {
-      each([&](int, float* e) {
+      each([&](int, float* e, int) {
         #pragma unroll
         for (int j = 0; j < V; ++j) sum += e[j];
       });
       mean = row_.template reduce<0>(sum) * rK;
       sum = 0.0f;
+      each([&](int, float* e, int n) {
+        #pragma unroll
+        for (int j = 0; j < V; ++j) e[j] = j < n ? e[j] - mean : 0.0f;
+      });
     }
-    each([&](int, float* e) {
+    each([&](int, float* e, int) {
       #pragma unroll
-      for (int j = 0; j < V; ++j) { e[j] -= mean; sum = __builtin_fmaf(e[j], e[j], sum); }
+      for (int j = 0; j < V; ++j) sum = __builtin_fmaf(e[j], e[j], sum);
     });
     const float inv = 1.0f / sqrtf(row_.template reduce<0>(sum) * rK + a.eps);
-    each([&](int i, float* e) {
+    each([&](int i, float* e, int n) {
       float f[V];
       if (w) {
-        load_v<BF, V>(w, i, w32, f);
+        load_v<BF, V>(w, i, w32, f, n);
         #pragma unroll
         for (int j = 0; j < V; ++j) e[j] = e[j] * inv * (f[j] + a.offset);
       } else {
@@ -131,7 +145,7 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void residual_norm_kernel(
         for (int j = 0; j < V; ++j) e[j] *= inv;
       }
       if (b) {
-        load_v<BF, V>(b, i, b32, f);
+        load_v<BF, V>(b, i, b32, f, n);
         #pragma unroll
         for (int j = 0; j < V; ++j) e[j] += f[j];
       }
@@ -140,88 +154,94 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void residual_norm_kernel(
 
   if (a.post_weight) norm(a.post_weight, flags & LCQ_NORM_POST_WEIGHT_F32, a.post_bias, flags & LCQ_NORM_POST_BIAS_F32);
   if (a.gate) {
-    each([&](int i, float* e) {
+    each([&](int i, float* e, int n) {
       float f[V];
-      load_v<BF, V>(a.gate, r * a.ldg + i, false, f);
+      load_v<BF, V>(a.gate, r * a.ldg + i, false, f, n);
       #pragma unroll
       for (int j = 0; j < V; ++j) e[j] *= f[j];
     });
   }
   if (a.residual) {
-    each([&](int i, float* e) {
+    each([&](int i, float* e, int n) {
       float f[V];
-      load_v<BF, V>(a.residual, r * a.ldr + i, flags & LCQ_NORM_RESIDUAL_F32, f);
+      load_v<BF, V>(a.residual, r * a.ldr + i, flags & LCQ_NORM_RESIDUAL_F32, f, n);
       #pragma unroll
       for (int j = 0; j < V; ++j) e[j] = __builtin_fmaf(a.scale, e[j], f[j]);
     });
   } else if (flags & NORM) {
-    each([&](int, float* e) {
+    each([&](int, float* e, int) {
       #pragma unroll
       for (int j = 0; j < V; ++j) e[j] *= a.scale;
     });
   }
-  if (a.h) each([&](int i, float* e) { store_v<BF, V>(a.h, r * K + i, flags & LCQ_NORM_RESIDUAL_F32, e); });
+  if (a.h) each([&](int i, float* e, int n) { store_v<BF, V>(a.h, r * K + i, flags & LCQ_NORM_RESIDUAL_F32, e, n); });
   if (flags & NORM) norm(a.weight, flags & LCQ_NORM_WEIGHT_F32, a.bias, flags & LCQ_NORM_BIAS_F32);
-  if (a.out) each([&](int i, float* e) { store_v<BF, V>(a.out, r * K + i, flags & LCQ_NORM_OUT_F32, e); });
+  if (a.out) each([&](int i, float* e, int n) { store_v<BF, V>(a.out, r * K + i, flags & LCQ_NORM_OUT_F32, e, n); });
   if (!a.codes) return;
 
   const auto make = [&]() -> TokenCodes {
     if (a.scale_in) return TokenCodes::given(a.scale_in[0]);
     if (flags & LCQ_NORM_ASYM) {
       float hi = -__builtin_inff(), lo = __builtin_inff();
-      each([&](int, float* e) {
+      each([&](int, float* e, int n) {
         #pragma unroll
-        for (int j = 0; j < V; ++j) { hi = nan_max(hi, e[j]); lo = nan_min(lo, e[j]); }
+        for (int j = 0; j < V; ++j) {
+          const float x = j < n ? e[j] : e[0];
+          hi = nan_max(hi, x);
+          lo = nan_min(lo, x);
+        }
       });
       hi = row_.template reduce<1>(hi);
       return TokenCodes::asymmetric(row_.template reduce<2>(lo), hi);
     }
     float m = 0.0f;
-    each([&](int, float* e) {
+    each([&](int, float* e, int n) {
       #pragma unroll
-      for (int j = 0; j < V; ++j) m = nan_max(m, fabsf(e[j]));
+      for (int j = 0; j < V; ++j) m = nan_max(m, j < n ? fabsf(e[j]) : 0.0f);
     });
     return TokenCodes::symmetric(row_.template reduce<1>(m));
   };
   const TokenCodes q = make();
-  each([&](int i, float* e) {
-    if constexpr (V == 1) a.codes[r * K + i] = (int8_t)q.code(e[0]);
-    else *(u32x2*)(a.codes + r * K + i) = q.codes(e);
+  each([&](int i, float* e, int n) {
+    uint32_t w[V / 4];
+    q.template codes<V>(e, w);
+    int8_t* const to = a.codes + r * K + i;
+    if (n == V) {
+      __builtin_memcpy(to, w, V);
+    } else {
+      #pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j < n) to[j] = (int8_t)(w[j / 4] >> 8 * (j % 4));
+    }
   });
   if (t == 0 && a.scales) a.scales[r] = q.d.s;
-  if (t == 0 && a.zeros) a.zeros[r] = (int)q.z;
+  if (t == 0 && a.zeros) a.zeros[r] = q.z;
 }
 
-template <int BF, int V, int TEAM, int CH>
+// E elements per lane
+template <int BF, int TEAM, int E>
 void launch(const NormArgs& a, hipStream_t st) {
   constexpr int rows = TEAM == 64 ? 4 : 1;
-  residual_norm_kernel<BF, V, TEAM, V == 1 ? CH * 8 : CH><<<dim3((unsigned)((a.T + rows - 1) / rows)), dim3(TEAM == 64 ? 256 : TEAM), 0, st>>>(a);
+  residual_norm_kernel<BF, TEAM, E / Vec<BF>::N><<<dim3((unsigned)((a.T + rows - 1) / rows)), dim3(TEAM == 64 ? 256 : TEAM), 0, st>>>(a);
 }
-template <int BF, int V>
+template <int BF>
 void launch_rows(const NormArgs& a, hipStream_t st) {
-  if (a.K <= 512) launch<BF, V, 64, 1>(a, st);
-  else if (a.K <= 1024) launch<BF, V, 64, 2>(a, st);
-  else if (a.K <= 2048) launch<BF, V, 256, 1>(a, st);
-  else if (a.K <= 4096) launch<BF, V, 256, 2>(a, st);
-  else if (a.K <= 8192) launch<BF, V, 256, 4>(a, st);
-  else if (a.K <= 16384) launch<BF, V, 1024, 2>(a, st);
-  else if (a.K <= 32768) launch<BF, V, 1024, 4>(a, st);
-  else launch<BF, V, 1024, 8>(a, st);
+  if (a.K <= 512) launch<BF, 64, 8>(a, st);
+  else if (a.K <= 1024) launch<BF, 64, 16>(a, st);
+  else if (a.K <= 2048) launch<BF, 256, 8>(a, st);
+  else if (a.K <= 4096) launch<BF, 256, 16>(a, st);
+  else if (a.K <= 8192) launch<BF, 512, 16>(a, st);
+  else if (a.K <= 16384) launch<BF, 1024, 16>(a, st);
+  else if (a.K <= 32768) launch<BF, 1024, 32>(a, st);
+  else launch<BF, 1024, 64>(a, st);
 }
 
 constexpr int64_t MOST_COLS = 65536;                // a row stays in the registers of 1024 lanes
 
-bool aligned(const void* p) { return (uintptr_t)p % 16 == 0; }
-
 int run(const NormArgs& a, int dtype, hipStream_t st) {
-  const int f = a.flags;
-  const auto stride = [&](int64_t ld, bool f32) { return ld * (f32 || dtype == LCQ_F32 ? 4 : 2) % 16 == 0; };
-  const bool wide = a.K % 8 == 0 && aligned(a.x) && stride(a.ldx, false) && aligned(a.residual) && stride(a.ldr, f & LCQ_NORM_RESIDUAL_F32) &&
-                    aligned(a.gate) && stride(a.ldg, false) && aligned(a.post_weight) && aligned(a.post_bias) && aligned(a.weight) &&
-                    aligned(a.bias) && aligned(a.h) && aligned(a.out) && (uintptr_t)a.codes % 8 == 0;
-  if (dtype == LCQ_BF16) { if (wide) launch_rows<ROW_BF16, 8>(a, st); else launch_rows<ROW_BF16, 1>(a, st); }
-  else if (dtype == LCQ_F16) { if (wide) launch_rows<ROW_F16, 8>(a, st); else launch_rows<ROW_F16, 1>(a, st); }
-  else { if (wide) launch_rows<ROW_F32, 8>(a, st); else launch_rows<ROW_F32, 1>(a, st); }
+  if (dtype == LCQ_BF16) launch_rows<ROW_BF16>(a, st);
+  else if (dtype == LCQ_F16) launch_rows<ROW_F16>(a, st);
+  else launch_rows<ROW_F32>(a, st);
   LCQ_CHECK_LAUNCH();
   return LCQ_OK;
 }
