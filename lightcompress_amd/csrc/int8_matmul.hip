@@ -236,7 +236,6 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MatmulArgs g, int tiles_m,
   static_assert(4 * STEP * 32 * ROW <= STAGES * T::STAGE, "outputs on their way out");
   char* const mine = lds + wave * STEP * 32 * ROW;
   const int t = lane & 31, h = lane >> 5;
-  const bool wide = (uintptr_t)g.y % 16 == 0 && (g.N * E) % 16 == 0;
   #pragma unroll
   for (int i0 = 0; i0 < FM; i0 += STEP) {
     #pragma unroll
@@ -277,8 +276,8 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MatmulArgs g, int tiles_m,
       const int m = wr * FM * 32 + i0 * 32 + tt, n = wc * FN * 32 + ch * CH;
       if (m >= rows_a || n >= rows_w) continue;
       const int64_t cell = (m0 + m) * g.N + n0 + n + (BF == ROW_I32 ? part * g.M * g.N : 0);
-      if (wide && n + CH <= rows_w) {
-        *(u32x4*)((char*)g.y + cell * E) = v;
+      if (n + CH <= rows_w) {
+        __builtin_memcpy((char*)g.y + cell * E, &v, 16);     // (rows may start anywhere)
       } else {
         #pragma unroll
         for (int e = 0; e < CH; ++e)
@@ -519,23 +518,25 @@ __global__ __launch_bounds__(WAVES * 64) void stream_kernel(MatmulArgs g, TokenA
   }
 }
 
-// Rows of K codes to rows of Kp, the next multiple of 16, with zeros behind them: operands whose rows do not start on 16 bytes.
-__global__ __launch_bounds__(256) void pad_kernel(const int8_t* __restrict__ x, int64_t rows, int K, int Kp, int8_t* __restrict__ out) {
-  const int per = Kp / 16;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / per;
-    const int k = (int)(i - r * per) * 16;
-    const int8_t* const p = x + r * K + k;
-    union { u32x4 v; int8_t b[16]; } u;
-    if (k + 16 <= K) {
-      __builtin_memcpy(&u, p, 16);
-    } else {
-      u.v = u32x4{0, 0, 0, 0};
-      #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (k + e < K) u.b[e] = p[e];
+// Rows of K codes to rows of Kp, the next multiple of 16, with zeros behind them: operands whose rows do not start on 16 bytes.  The
+// rows of a, then those of w; `out` has them one behind the other.
+__global__ __launch_bounds__(256) void pad_kernel(const int8_t* __restrict__ a, int64_t rows_a, const int8_t* __restrict__ w, int64_t rows, int K, int Kp,
+                                                  int8_t* __restrict__ out) {
+  // a wave takes a row (grid-stride): no division by the row's length
+  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)gridDim.x * 4) {
+    const int8_t* const x = r < rows_a ? a + r * K : w + (r - rows_a) * K;
+    for (int k = (threadIdx.x & 63) * 16; k < Kp; k += 1024) {
+      union { u32x4 v; int8_t b[16]; } u;
+      if (k + 16 <= K) {
+        __builtin_memcpy(&u, x + k, 16);
+      } else {
+        u.v = u32x4{0, 0, 0, 0};
+        #pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (k + e < K) u.b[e] = x[k + e];
+      }
+      *(u32x4*)(out + r * Kp + k) = u.v;
     }
-    *(u32x4*)(out + i * 16) = u.v;
   }
 }
 
@@ -559,7 +560,7 @@ void launch_tiles(const MatmulArgs& g, int parts, hipStream_t st) {
 }
 template <int BF>
 void launch_join(const MatmulArgs& g, const int* sums, int parts, hipStream_t st) {
-  const bool wide = g.N % 4 == 0 && (uintptr_t)g.y % 16 == 0;
+  const bool wide = g.N % 4 == 0 && (uintptr_t)g.y % 16 == 0;      // (four channels of one token)
   const int64_t all = g.M * g.N;
   if (wide) join_kernel<BF, 4><<<dim3((unsigned)((all / 4 + 255) / 256)), dim3(256), 0, st>>>(g, sums, parts);
   else join_kernel<BF, 1><<<dim3((unsigned)((all + 255) / 256)), dim3(256), 0, st>>>(g, sums, parts);
@@ -638,11 +639,9 @@ int lcq_int8_matmul(const int8_t* a, const float* as, int a_scalar, const int32_
   if (K % 16) {
     const int Kp = (int)padded(K);
     int8_t* const pa = (int8_t*)workspace + (parts > 1 ? on256(4 * M * N * parts) : 0);
-    int8_t* const pw = pa + M * Kp;
-    const auto grid = [&](int64_t rows) { const int64_t b = (rows * (Kp / 16) + 255) / 256; return dim3((unsigned)(b < 4096 ? b : 4096)); };
-    pad_kernel<<<grid(M), dim3(256), 0, st>>>(a, M, (int)K, Kp, pa);
-    pad_kernel<<<grid(N), dim3(256), 0, st>>>(w, N, (int)K, Kp, pw);
-    g.a = pa; g.w = pw; g.lda = g.ldw = g.K = Kp;
+    const int64_t blocks = (M + N + 3) / 4;
+    pad_kernel<<<dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st>>>(a, M, w, M + N, (int)K, Kp, pa);
+    g.a = pa; g.w = pa + M * Kp; g.lda = g.ldw = g.K = Kp;
   }
   if (dtype == LCQ_BF16) launch_codes<ROW_BF16>(g, (int*)workspace, st);
   else if (dtype == LCQ_F16) launch_codes<ROW_F16>(g, (int*)workspace, st);
