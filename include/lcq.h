@@ -522,12 +522,10 @@ int lcq_residual_norm(const void* x, int dtype, int64_t T, int64_t K, int64_t ld
  *  entropy  [T] fp32 or NULL
  *  top_logprobs [T, k] fp32, top_tokens [T, k] int64, 0 <= k <= min(64, V): largest first, equal logits by the lowest index, a NaN
  *           above everything
- * Masked logits (-inf) have probability 0; a row of nothing else, or one with a NaN or +inf, gives NaN as log_softmax does.
- *  workspace of lcq_token_logprobs_workspace_bytes(T, V, k) (0: none), 16-byte aligned. */
-int64_t lcq_token_logprobs_workspace_bytes(int64_t T, int64_t V, int k);
+ * Masked logits (-inf) have probability 0; a row of nothing else, or one with a NaN or +inf, gives NaN as log_softmax does. */
 int lcq_token_logprobs(const void* logits, int dtype, int64_t T, int64_t V, int64_t ldx, const int64_t* tokens, int64_t m,
                        int64_t ignore, float* logprobs, float* entropy, int k, float* top_logprobs, int64_t* top_tokens,
-                       void* workspace, void* stream);
+                       void* stream);
 
 #ifdef __cplusplus
 }

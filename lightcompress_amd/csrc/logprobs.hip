@@ -5,12 +5,12 @@
 //  * A lane keeps its own c, S and U.  c is a logit that the lane has seen; it moves only where a later one is more than 8 above
 //    it, so that almost no piece pays for a change of reference, S stays below V e^8 and log S and U / S do not cancel to more than a few
 //    times their last bits.  References meet once, when lanes, waves and parts are joined.
-//  * The best alternatives: each wave keeps 64 keys, one per lane in descending order.  A key is a whole number that orders by value
-//    and then by the lowest index.  A 16-byte piece whose maximum lies below the k-th best so far costs one comparison; what passes is
-//    collected in LDS and taken over 64 at a time (a bitonic sort, then a merge).  Where many lanes pass at once (the first piece,
-//    ascending logits) the k-th best of the lanes' maxima is a bound first.
-//  * A row is one workgroup's where there are enough rows, else it is cut into parts of whole 256-lane passes for about four workgroups
-//    per CU, which leave (c, S, U) and k keys each for a second, small kernel.
+//  * The best alternatives cost the pass one comparison per piece: a lane keeps the largest logit of each 8th (12th) of the pass.  Behind it, the k-th
+//    largest of all lanes' maxima is a bound that k logits reach, few more do, and only those parts of a lane's logits that reach it are read
+//    again for the keys of those logits, which one wave sorts.  A key is a whole number that orders by value and then by the lowest index.  Where
+//    more keys reach the bound than there is room for (ties: constant rows, rows masked but for fewer than k), every wave finds its best
+//    by itself.
+//  * A row is one workgroup's: of 1024 lanes where there are at most as many rows as CUs, of 512 or 256 where there are more.
 #include "rowquant.h"
 #include <type_traits>
 
@@ -18,7 +18,6 @@ namespace {
 using namespace lcq;
 
 constexpr float LOWEST = -3.4028234663852886e38f, MOVE = 8.0f;
-constexpr int THREADS = 256, WAVES = THREADS / 64;
 constexpr int FLIGHT = 2;                           // 16-byte pieces that a lane has on their way while it works on as many
 
 struct LogprobArgs {
@@ -27,10 +26,7 @@ struct LogprobArgs {
   float *logprobs, *entropy, *top_logprobs;
   int64_t* top_tokens;
   int64_t V, ldx, m, ignore;
-  int k, parts;
-  int per;                                          // 16-byte pieces of a part
-  f32x4* sums;                                      // [T, parts]: c, S, U
-  uint64_t* keys;                                   // [T, parts, k]
+  int k;
 };
 
 // A whole number that orders logits by value and, among equal ones, by the lowest index; a NaN is above everything, -0 equals +0.
@@ -100,24 +96,12 @@ __device__ __forceinline__ K sorted(K v) {
 // the 64 largest of two descending lists, `turned` with its lanes in ascending order
 __device__ __forceinline__ uint64_t merged(uint64_t v, uint64_t turned) { return ordered<32, 64>(v > turned ? v : turned); }
 
-// The best 64 of a wave.  `bound`, `limit` and `some` are the same in all lanes.
+// The best 64 keys of a wave, one per lane in descending order; of them `k` are wanted.
 struct Best {
-  uint64_t mine = 0, bound = 0;                   
-  float limit = -__builtin_inff();                  // a logit below it is not among the best k
+  uint64_t mine = 0, bound = 0;                     // a key that is not above bound is not among the best k
   bool some = false;                                // `mine` holds something
   int lane, k;
   __device__ __forceinline__ Best(int lane_, int k_) : lane(lane_), k(k_) {}
-  // at least k keys lie above `key`; the k-th best logit is that of `rank` or larger
-  __device__ __forceinline__ void raise(uint64_t key, uint32_t rank) {
-    if (key <= bound) return;
-    bound = key;
-    const float x = logit_of((uint64_t)rank << 32);
-    limit = x == x ? x : __builtin_inff();          // (k NaNs: whatever is not one stays out; a NaN passes every limit)
-  }
-  // at least k logits reach `rank`; keys of that rank are still to be collected
-  __device__ __forceinline__ void raise_to(uint32_t rank) { if (rank) raise(((uint64_t)rank << 32) - 1, rank); }
-  // the k-th largest of 64 ranks
-  __device__ __forceinline__ uint32_t kth(uint32_t rank) const { return (uint32_t)__builtin_amdgcn_readlane((int)sorted(rank), k - 1); }
   // one key per lane (0: none)
   __device__ __forceinline__ void take(uint64_t key) {
     if (__builtin_amdgcn_ballot_w64(key > bound) == 0) return;
@@ -125,7 +109,7 @@ struct Best {
     mine = some ? merged(mine, other_lane(s, 63 - lane)) : s;
     some = true;
     const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)mine, k - 1), hi = (uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), k - 1);
-    if (hi) raise((uint64_t)hi << 32 | lo, hi);
+    bound = (uint64_t)hi << 32 | lo;
   }
 };
 
@@ -143,81 +127,6 @@ struct Sums {
     refer(team_reduce<64, true>(c));
     S = team_sum<64>(S);
     U = team_sum<64>(U);
-  }
-};
-
-// The waves' sums joined in wave 0 -> true there.  Its barrier is also what the waves' lists in LDS wait for.
-__device__ __forceinline__ bool join_sums(Sums& s) {
-  __shared__ float part[WAVES][3];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  s.join_wave();
-  if (lane == 0) { part[wave][0] = s.c; part[wave][1] = s.S; part[wave][2] = s.U; }
-  __syncthreads();
-  if (wave) return false;
-  float c = s.c;
-  #pragma unroll
-  for (int w = 1; w < WAVES; ++w) c = nan_max(c, part[w][0]);
-  s.refer(c);
-  #pragma unroll
-  for (int w = 1; w < WAVES; ++w) {
-    Sums o;
-    o.c = part[w][0]; o.S = part[w][1]; o.U = part[w][2];
-    o.refer(c);
-    s.add(o);
-  }
-  return true;
-}
-// What the waves of a workgroup collect: keys that may be among the best k, in LDS until there are 64 of them.
-template <int ROOM>
-struct Lists {
-  uint64_t found[WAVES][ROOM], best[WAVES][64];
-  int count[WAVES], some[WAVES];
-  uint32_t rank;                                    // at least k logits of the row reach it: the best of the waves' bounds
-};
-template <int ROOM>
-struct Collector {
-  Lists<ROOM>& l;
-  Best best;
-  int count = 0, wave;
-  __device__ __forceinline__ Collector(Lists<ROOM>& l_, int wave_, int lane, int k) : l(l_), best(lane, k), wave(wave_) {}
-  __device__ __forceinline__ void collect(bool in, uint64_t key) {
-    const uint64_t lanes = __builtin_amdgcn_ballot_w64(in);
-    if (in) l.found[wave][count + __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0))] = key;
-    count += __builtin_popcountll(lanes);
-  }
-  __device__ __forceinline__ void drain() {
-    #pragma unroll 1
-    for (int at = 0; at < count; at += 64) best.take(at + best.lane < count ? l.found[wave][at + best.lane] : 0);
-    count = 0;
-  }
-  __device__ __forceinline__ void share() {
-    if (best.lane == 0 && best.bound) __hip_atomic_fetch_max(&l.rank, (uint32_t)((best.bound + 1) >> 32), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-  }
-  __device__ __forceinline__ uint32_t shared() const { return __hip_atomic_load(&l.rank, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
-  __device__ __forceinline__ void leave() {         // for the wave that joins them, behind a barrier
-    if (best.some) l.best[wave][best.lane] = best.mine;
-    if (best.lane == 0) { l.count[wave] = count; l.some[wave] = best.some; }
-  }
-  // wave 0: everything that the waves have collected and not sorted, 64 at a time, then their lists
-  __device__ __forceinline__ void join() {
-    int end[WAVES], total = 0;
-    #pragma unroll
-    for (int w = 0; w < WAVES; ++w) end[w] = total += l.count[w];
-    #pragma unroll 1
-    for (int at = 0; at < total; at += 64) {
-      const int i = at + best.lane;
-      int w = 0, begin = 0;
-      #pragma unroll
-      for (int v = 0; v < WAVES - 1; ++v)
-        if (i >= end[v]) { w = v + 1; begin = end[v]; }
-      best.take(i < total ? l.found[w][i - begin] : 0);
-    }
-    #pragma unroll 1
-    for (int w = 1; w < WAVES; ++w)
-      if (l.some[w]) {
-        best.mine = best.some ? merged(best.mine, l.best[w][63 - best.lane]) : l.best[w][best.lane];
-        best.some = true;
-      }
   }
 };
 
@@ -249,219 +158,209 @@ __device__ __forceinline__ void answer(const LogprobArgs& a, int64_t row, const 
   }
 }
 
-template <int BF, bool TOP>
+constexpr int ROOM = 512;                           // keys that find room
+
+template <int BF, bool TOP, int THREADS>
 __global__ __launch_bounds__(THREADS) void logprobs_kernel(LogprobArgs a) {
-  constexpr int N = Vec<BF>::N, PASS = THREADS * FLIGHT;
-  __shared__ Lists<TOP ? 64 * N + 64 : 1> lists;
-  if constexpr (TOP) {
-    if (threadIdx.x == 0) lists.rank = 0;
-    __syncthreads();
-  }
+  constexpr int N = Vec<BF>::N, PASS = THREADS * FLIGHT, WAVES = THREADS / 64, PARTS = THREADS == 1024 ? 8 : 12;
+  __shared__ float most[TOP ? PARTS : 1][TOP ? THREADS : 1];                 // largest logit of a lane in each part of the row
+  __shared__ uint64_t keys[TOP ? ROOM : 1], lists[TOP ? WAVES : 1][64];
+  __shared__ uint32_t ranks[TOP ? WAVES : 1][64];
+  __shared__ float sums[WAVES][3];
+  __shared__ uint32_t reach;
+  __shared__ int count;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row = blockIdx.x;
-  const int part = blockIdx.y;
   const char* const x = (const char*)a.x + row * a.ldx * (16 / N);
   const int V = (int)a.V, pieces = (V + N - 1) / N;
-  const int from = part * a.per, to = from + a.per < pieces ? from + a.per : pieces;
+  const int last = V / N;                           // (all pieces of the row but its last hold N logits)
+  const int passes = (pieces + PASS - 1) / PASS, per = (passes + PARTS - 1) / PARTS;
 
   Given<BF> given;
-  if (a.parts == 1 && wave == 0) given.tokens(a, row, lane);
+  if (wave == 0) given.tokens(a, row, lane);
   Sums s;
-  Collector<TOP ? 64 * N + 64 : 1> c(lists, wave, lane, TOP ? a.k : 1);
-  // the pieces j0 + f THREADS of this lane
-  const auto take = [&](const u32x4 (&raw)[FLIGHT], int j0) __attribute__((always_inline)) {
-    float top[FLIGHT];
-    float limit = c.best.limit;
-    if constexpr (TOP) {
-      const float theirs = logit_of((uint64_t)c.shared() << 32);
-      limit = theirs > limit ? theirs : limit;
-    }
-    #pragma unroll
-    for (int f = 0; f < FLIGHT; ++f) {
-      float v[N];
-      unpack<BF>(raw[f], v);
-      top[f] = v[0];
+  float top = -__builtin_inff();
+  // the pieces j0 + f THREADS of this lane; -inf past the row's end
+  const auto fetch = [&](u32x4 (&raw)[FLIGHT], int j0) __attribute__((always_inline)) {
+    if (j0 + PASS <= last) {
       #pragma unroll
-      for (int i = 1; i < N; ++i) top[f] = nan_max(top[f], v[i]);
-      if (top[f] > s.c + MOVE) s.refer(top[f]);
-      #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float d = v[i] - s.c, e = __builtin_amdgcn_exp2f(d * 1.44269504088896340736f);
-        s.S += e;
-        s.U = __builtin_fmaf(e, nan_max(d, -150.0f), s.U);   // (-inf: e is 0)
-      }
-    }
-    if constexpr (TOP) {
-      float most = top[0];
-      #pragma unroll
-      for (int f = 1; f < FLIGHT; ++f) most = nan_max(most, top[f]);
-      const uint64_t pass = __builtin_amdgcn_ballot_w64(!(most < limit));
-      if (__builtin_expect(pass != 0, 0)) {
-        c.best.raise_to(c.shared());
-        if (__builtin_popcountll(pass) > 16) {
-          c.best.raise_to(c.best.kth(rank_of(most)));
-          c.share();
-        }
-        #pragma unroll 1
-        for (int f = 0; f < FLIGHT; ++f) {          // (one copy of the code for all of them)
-          u32x4 r = raw[0];
-          float t = top[0];
-          #pragma unroll
-          for (int g = 1; g < FLIGHT; ++g) { r = f == g ? raw[g] : r; t = f == g ? top[g] : t; }
-          if (__builtin_amdgcn_ballot_w64(!(t < c.best.limit)) == 0) continue;
-          const int64_t v0 = (int64_t)(j0 + f * THREADS + (int)threadIdx.x) * N;             // (past the row's end: holds nothing)
-          float v[N];
-          unpack<BF>(r, v);
-          #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            if (__builtin_amdgcn_ballot_w64(!(v[i] < c.best.limit)) == 0) continue;
-            const uint64_t key = v0 + i < V ? key_of(v[i], (uint32_t)(v0 + i)) : 0;
-            c.collect(key > c.best.bound, key);
-          }
-          if (c.count >= 64) {
-            c.drain();
-            c.share();
-          }
-        }
-      }
-    }
-  };
-
-  // A pass is on its way while the one in front of it is worked on.  Rows may start anywhere.
-  const int last = to < V / N ? to : V / N;         // (all pieces of the row but its last hold N logits)
-  u32x4 one[FLIGHT], two[FLIGHT];
-  for (int j0 = from - PASS; j0 < to; j0 += PASS) {
-    const int next = j0 + PASS;
-    if (next + PASS <= last) {
-      #pragma unroll
-      for (int f = 0; f < FLIGHT; ++f) __builtin_memcpy(&two[f], x + (uint32_t)(next + f * THREADS + (int)threadIdx.x) * 16u, 16);
-    } else if (next < to) {
+      for (int f = 0; f < FLIGHT; ++f) __builtin_memcpy(&raw[f], x + (uint32_t)(j0 + f * THREADS + (int)threadIdx.x) * 16u, 16);      // (rows may start anywhere)
+    } else if (j0 < pieces) {
       #pragma unroll
       for (int f = 0; f < FLIGHT; ++f) {
-        const int j = next + f * THREADS + (int)threadIdx.x;
-        two[f] = N == 4 ? u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u}          // -inf
+        const int j = j0 + f * THREADS + (int)threadIdx.x;
+        raw[f] = N == 4 ? u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u}
                         : u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u} & (BF == ROW_F16 ? 0xfc00fc00u : ~0u);
         if (j < last) {
-          __builtin_memcpy(&two[f], x + (uint32_t)j * 16u, 16);
-        } else if (j < to) {
+          __builtin_memcpy(&raw[f], x + (uint32_t)j * 16u, 16);
+        } else if (j < pieces) {
           float v[N];
           #pragma unroll
           for (int i = 0; i < N; ++i) v[i] = j * N + i < V ? load_scalar<BF>(x, j * N + i) : -__builtin_inff();
-          two[f] = pack<BF>(v);
+          raw[f] = pack<BF>(v);
         }
       }
     }
+  };
+
+  // A pass is on its way while the one in front of it is worked on.
+  u32x4 one[FLIGHT], two[FLIGHT];
+  int part = 0, left = per;
+  for (int p = -1; p < passes; ++p) {
+    fetch(two, (p + 1) * PASS);
     __builtin_amdgcn_sched_barrier(0);
-    if (j0 >= from) take(one, j0);
+    if (p >= 0) {
+      #pragma unroll
+      for (int f = 0; f < FLIGHT; ++f) {
+        float v[N];
+        unpack<BF>(one[f], v);
+        float t = v[0];
+        #pragma unroll
+        for (int i = 1; i < N; ++i) t = nan_max(t, v[i]);
+        if (t > s.c + MOVE) s.refer(t);
+        top = nan_max(top, t);
+        #pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float d = v[i] - s.c, e = __builtin_amdgcn_exp2f(d * 1.44269504088896340736f);
+          s.S += e;
+          s.U = __builtin_fmaf(e, nan_max(d, -150.0f), s.U); // (-inf: e is 0)
+        }
+      }
+      if (TOP && --left == 0) {
+        most[part++][threadIdx.x] = top;
+        top = -__builtin_inff();
+        left = per;
+      }
+    }
     #pragma unroll
     for (int f = 0; f < FLIGHT; ++f) one[f] = two[f];
   }
-  if (a.parts == 1 && wave == 0) given.logits(a, row, lane);
-  if constexpr (TOP) c.leave();
-  if (!join_sums(s)) return;
-  if constexpr (TOP) c.join();
-  if (a.parts == 1) {
-    answer<BF>(a, row, s, given, c.best.mine, lane);
-    return;
-  }
-  const int64_t at = row * a.parts + part;
-  if (lane == 0) a.sums[at] = f32x4{s.c, s.S, s.U, 0.0f};
-  if (lane < a.k) a.keys[at * a.k + lane] = c.best.mine;
-}
-
-// The parts of a row joined: one workgroup per row.
-template <int BF>
-__global__ __launch_bounds__(THREADS) void join_kernel(LogprobArgs a) {
-  __shared__ Lists<128> lists;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row = blockIdx.x;
-  Given<BF> given;
-  if (wave == 0) given.tokens(a, row, lane);
-  const f32x4* const sums = a.sums + row * a.parts;
-  const int all = a.parts * a.k;
-  const uint64_t* const keys = a.keys + row * all;
-  constexpr int KEEP = 8;                           // loads that a lane has in flight
-  uint64_t key[KEEP];
-  const auto fetch = [&](int at) __attribute__((always_inline)) {
-    #pragma unroll
-    for (int i = 0; i < KEEP; ++i) key[i] = at + i * THREADS + (int)threadIdx.x < all ? keys[at + i * THREADS + threadIdx.x] : 0;
-  };
-  f32x4 v = {LOWEST, 0.0f, 0.0f, 0.0f};
-  if ((int)threadIdx.x < a.parts) v = sums[threadIdx.x];
-  fetch(0);
-  Sums s;
-  for (int p = threadIdx.x;;) {
-    Sums o;
-    o.c = v[0]; o.S = v[1]; o.U = v[2];
-    const float c = nan_max(s.c, o.c);
-    s.refer(c);
-    o.refer(c);
-    s.add(o);
-    if ((p += THREADS) >= a.parts) break;
-    v = sums[p];
-  }
   if (wave == 0) given.logits(a, row, lane);
-  Collector<128> c(lists, wave, lane, a.k > 0 ? a.k : 1);
-  #pragma unroll 1
-  for (int at = 0; at < all; at += KEEP * THREADS) {
-    if (at) fetch(at);
-    uint32_t most = 0;
+  s.join_wave();
+  if (lane == 0) { sums[wave][0] = s.c; sums[wave][1] = s.S; sums[wave][2] = s.U; }
+  Best best(lane, TOP ? a.k : 1);
+  if constexpr (TOP) {
+    if (left != per) most[part++][threadIdx.x] = top;        // (the last part, cut short)
+    for (int p = 0; p < part; ++p) top = nan_max(top, most[p][threadIdx.x]);
+    // the k-th largest of the lanes' maxima: sorted by waves, joined by pairs
+    uint32_t r = sorted(rank_of(top));
+    ranks[wave][lane] = r;
+    if (threadIdx.x == 0) count = 0;
     #pragma unroll
-    for (int i = 0; i < KEEP; ++i) most = (uint32_t)(key[i] >> 32) > most ? (uint32_t)(key[i] >> 32) : most;
-    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(most > (uint32_t)(c.best.bound >> 32))) > 16) c.best.raise_to(c.best.kth(most));
-    #pragma unroll
-    for (int i = 0; i < KEEP; ++i) {
-      if (__builtin_amdgcn_ballot_w64(key[i] > c.best.bound) == 0) continue;
-      c.collect(key[i] > c.best.bound, key[i]);
-      if (c.count >= 64) c.drain();
+    for (int w = 1; w < WAVES; w *= 2) {
+      __syncthreads();
+      if (wave % (2 * w) == 0) {
+        const uint32_t o = ranks[wave + w][63 - lane];
+        r = ordered<32, 64>(r > o ? r : o);
+        ranks[wave][lane] = r;
+      }
+    }
+    if (wave == 0 && lane == a.k - 1) reach = r;
+    __syncthreads();
+    const uint32_t bound = reach;
+    const auto keep = [&](float v, int at) {
+      const int c = __hip_atomic_fetch_add(&count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      if (c < ROOM) keys[c] = key_of(v, (uint32_t)at);
+    };
+    // every logit that reaches it: each lane goes through those of its parts that do, so that the few that have any go side by side
+    uint32_t todo = 0;
+    for (int q = 0; q < part; ++q) todo |= (uint32_t)(rank_of(most[q][threadIdx.x]) >= bound) << q;
+    while (todo) {
+      const int q = __builtin_ctz(todo);
+      todo &= todo - 1;
+      const int end = (q + 1) * per < passes ? (q + 1) * per : passes;
+      constexpr int SOME = 6;                       // pieces on their way at once
+      for (int p = q * per * FLIGHT; p < end * FLIGHT; p += SOME) {
+        u32x4 raw[SOME];
+        const auto piece = [&](int i) { return (p + i) * THREADS + (int)threadIdx.x; };
+        #pragma unroll
+        for (int i = 0; i < SOME; ++i)
+          if (p + i < end * FLIGHT && piece(i) < last) __builtin_memcpy(&raw[i], x + (uint32_t)piece(i) * 16u, 16);
+        #pragma unroll
+        for (int i = 0; i < SOME; ++i) {
+          if (p + i >= end * FLIGHT || piece(i) >= last) continue;
+          float v[N];
+          unpack<BF>(raw[i], v);
+          #pragma unroll
+          for (int e = 0; e < N; ++e)
+            if (rank_of(v[e]) >= bound) keep(v[e], piece(i) * N + e);
+        }
+        #pragma unroll 1
+        for (int at = last * N; at < V; ++at) {     // (the row's last piece, if it is among these)
+          const int i = (last / THREADS) - p;
+          if (i < 0 || i >= SOME || p + i >= end * FLIGHT || last % THREADS != (int)threadIdx.x) break;
+          const float v = load_scalar<BF>(x, at);
+          if (rank_of(v) >= bound) keep(v, at);
+        }
+      }
+    }
+    __syncthreads();
+    if (count > ROOM) {                             // (the same in all waves)
+      #pragma unroll 1
+      for (int v0 = wave * 64 + lane; v0 - lane < V; v0 += THREADS * 8) {
+        float v[8];
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = v0 + i * THREADS < V ? load_scalar<BF>(x, v0 + i * THREADS) : 0.0f;
+        #pragma unroll 1
+        for (int i = 0; i < 8; ++i) {               // (one copy of the sort)
+          float e = v[0];
+          #pragma unroll
+          for (int j = 1; j < 8; ++j) e = i == j ? v[j] : e;
+          const int at = v0 + i * THREADS;
+          best.take(at < V ? key_of(e, (uint32_t)at) : 0);
+        }
+      }
+      lists[wave][lane] = best.mine;
     }
   }
-  c.leave();
-  if (!join_sums(s)) return;
-  if (all) c.join();
-  answer<BF>(a, row, s, given, c.best.mine, lane);
-}
-
-int parts_of(int64_t T, int64_t V, int dtype) {
-  const int64_t passes = (V * (dtype == LCQ_F32 ? 4 : 2) + 16 * THREADS - 1) / (16 * THREADS);
-  const int64_t want = 1024 / T;
-  return (int)(want < 1 ? 1 : want < passes ? want : passes);
+  __syncthreads();
+  if (wave) return;
+  float c = s.c;
+  #pragma unroll
+  for (int w = 1; w < WAVES; ++w) c = nan_max(c, sums[w][0]);
+  s.refer(c);
+  #pragma unroll
+  for (int w = 1; w < WAVES; ++w) {
+    Sums o;
+    o.c = sums[w][0]; o.S = sums[w][1]; o.U = sums[w][2];
+    o.refer(c);
+    s.add(o);
+  }
+  if constexpr (TOP) {
+    if (count > ROOM) {
+      #pragma unroll 1
+      for (int w = 1; w < WAVES; ++w) best.mine = merged(best.mine, lists[w][63 - lane]);
+    } else {
+      #pragma unroll 1
+      for (int i = 0; i < count; i += 64) best.take(i + lane < count ? keys[i + lane] : 0);
+    }
+  }
+  answer<BF>(a, row, s, given, best.mine, lane);
 }
 
 }  // namespace
 
 extern "C" {
 
-int64_t lcq_token_logprobs_workspace_bytes(int64_t T, int64_t V, int k) {
-  if (T <= 0 || V <= 0 || k < 0) return 0;
-  const int parts = parts_of(T, V, LCQ_F32);        // (the most there are)
-  return parts == 1 ? 0 : T * parts * (16 + 8 * (int64_t)k);
-}
-
 int lcq_token_logprobs(const void* logits, int dtype, int64_t T, int64_t V, int64_t ldx, const int64_t* tokens, int64_t m,
                        int64_t ignore, float* logprobs, float* entropy, int k, float* top_logprobs, int64_t* top_tokens,
-                       void* workspace, void* stream) {
+                       void* stream) {
   if (!logits || T <= 0 || V <= 0 || ldx < 0 || m < 0 || k < 0 || k > 64 || k > V) return LCQ_EINVAL;
   if ((m > 0 && (!tokens || !logprobs)) || (k > 0 && (!top_logprobs || !top_tokens))) return LCQ_EINVAL;
   if (dtype != LCQ_F32 && dtype != LCQ_BF16 && dtype != LCQ_F16) return LCQ_EDTYPE;
   if (T > 0x7fffffff || V > (1 << 28)) return LCQ_ESIZE;
   if ((uintptr_t)logits % (dtype == LCQ_F32 ? 4 : 2)) return LCQ_EALIGN;
-  LogprobArgs a = {logits, tokens, logprobs, entropy, top_logprobs, top_tokens, V, ldx, m, ignore, k, parts_of(T, V, dtype), 0, nullptr, nullptr};
-  if (a.parts > 1) {
-    if (!workspace) return LCQ_EWORKSPACE;
-    if ((uintptr_t)workspace % 16) return LCQ_EALIGN;
-    a.sums = (f32x4*)workspace;
-    a.keys = (uint64_t*)(a.sums + T * a.parts);
-  }
-  const int n = dtype == LCQ_F32 ? 4 : 8;
-  a.per = (int)(((V + n - 1) / n + a.parts - 1) / a.parts);
-  const dim3 grid((unsigned)T, (unsigned)a.parts), block(THREADS);
-  hipStream_t st = (hipStream_t)stream;
+  const LogprobArgs a = {logits, tokens, logprobs, entropy, top_logprobs, top_tokens, V, ldx, m, ignore, k};
+  const auto launch = [&](auto bf, auto threads) {
+    constexpr int BF = decltype(bf)::value, THREADS = decltype(threads)::value;
+    const dim3 grid((unsigned)T), block(THREADS);
+    if (k) logprobs_kernel<BF, true, THREADS><<<grid, block, 0, (hipStream_t)stream>>>(a);
+    else logprobs_kernel<BF, false, THREADS><<<grid, block, 0, (hipStream_t)stream>>>(a);
+  };
   const auto run = [&](auto bf) {
-    constexpr int BF = decltype(bf)::value;
-    if (k) logprobs_kernel<BF, true><<<grid, block, 0, st>>>(a);
-    else logprobs_kernel<BF, false><<<grid, block, 0, st>>>(a);
-    if (a.parts > 1) join_kernel<BF><<<dim3((unsigned)T), block, 0, st>>>(a);
+    if (T <= 256) launch(bf, std::integral_constant<int, 1024>{});
+    else if (T <= 1024) launch(bf, std::integral_constant<int, 512>{});
+    else launch(bf, std::integral_constant<int, 256>{});
   };
   if (dtype == LCQ_BF16) run(std::integral_constant<int, ROW_BF16>{});
   else if (dtype == LCQ_F16) run(std::integral_constant<int, ROW_F16>{});

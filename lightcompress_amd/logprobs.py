@@ -8,7 +8,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib as L
-from .w8a8 import _code, _here, _rows, _workspace
+from .w8a8 import _code, _here, _rows
 
 MOST_TOP = 64
 
@@ -53,9 +53,8 @@ def token_logprobs(logits, tokens=None, top=0, ignore_index=-100):
     top_logprobs = torch.empty((*lead, top), dtype=torch.float32, device=dev)
     top_tokens = torch.empty((*lead, top), dtype=torch.int64, device=dev)
     if T:
-        ws = _workspace(logits, 'lcq_token_logprobs_workspace_bytes', T, V, top)
         L.check(L.lib().lcq_token_logprobs(rows.data_ptr(), code, T, V, ld, ids.data_ptr() if m else None, m, ignore_index,
                                            logprobs.data_ptr() if m else None, entropy.data_ptr(), top,
                                            top_logprobs.data_ptr() if top else None, top_tokens.data_ptr() if top else None,
-                                           L.ptr(ws), L.stream()), 'lcq_token_logprobs')
+                                           L.stream()), 'lcq_token_logprobs')
     return TokenLogprobs(logprobs, entropy, top_logprobs, top_tokens)

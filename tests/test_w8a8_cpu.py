@@ -87,7 +87,7 @@ def test_the_c_entries_refuse_before_a_launch():
     assert norm(x=None) == norm(h=None) == norm(o=None) == norm(c=P) == norm(T=0) == norm(pb=P) == norm(f=256) == -1
     assert norm(f=128, c=P, s=P) == -1 and norm(d=7) == -3 and norm(K=65537) == -6
     lp = lambda x=P, d=0, T=2, V=100, ld=100, t=None, m=0, o=None, k=0, tv=None, ti=None: lib.lcq_token_logprobs(  # noqa: E731
-        x, d, T, V, ld, t, m, -100, o, None, k, tv, ti, None, None)
+        x, d, T, V, ld, t, m, -100, o, None, k, tv, ti, None)
     assert lp(x=None) == lp(T=0) == lp(V=0) == lp(m=1) == lp(k=1) == lp(k=65, tv=P, ti=P) == lp(V=3, k=4, tv=P, ti=P) == lp(m=-1) == -1
     assert lp(d=4) == -3 and lp(V=1 << 31) == -6
 
