@@ -46,15 +46,26 @@ def token_logprobs(logits, tokens=None, top=0, ignore_index=-100):
         with torch.cuda.device(logits.device):
             return token_logprobs(logits, tokens, top, ignore_index)
     dev = logits.device
-    rows, T, ld = _rows(logits, V)
     ids = None if tokens is None else tokens.contiguous()
     logprobs = None if tokens is None else torch.empty(tokens.shape, dtype=torch.float32, device=dev)
     entropy = torch.empty(lead, dtype=torch.float32, device=dev)
     top_logprobs = torch.empty((*lead, top), dtype=torch.float32, device=dev)
     top_tokens = torch.empty((*lead, top), dtype=torch.int64, device=dev)
-    if T:
-        L.check(L.lib().lcq_token_logprobs(rows.data_ptr(), code, T, V, ld, ids.data_ptr() if m else None, m, ignore_index,
-                                           logprobs.data_ptr() if m else None, entropy.data_ptr(), top,
-                                           top_logprobs.data_ptr() if top else None, top_tokens.data_ptr() if top else None,
-                                           L.stream()), 'lcq_token_logprobs')
+
+    def run(x, at):
+        """The logits x, whose rows are the rows from `at` on of all of them."""
+        if x.dim() > 2 and x.stride(-1) == 1 and not x.is_contiguous():      # logits[:, :-1]: a call per sequence, and no copy
+            rows = x[0].numel() // V
+            for i in range(x.shape[0]):
+                run(x[i], at + i * rows)
+            return
+        rows, T, ld = _rows(x, V)
+        if T:
+            L.check(L.lib().lcq_token_logprobs(rows.data_ptr(), code, T, V, ld, ids.data_ptr() + 8 * m * at if m else None, m, ignore_index,
+                                               logprobs.data_ptr() + 4 * m * at if m else None, entropy.data_ptr() + 4 * at, top,
+                                               top_logprobs.data_ptr() + 4 * top * at if top else None,
+                                               top_tokens.data_ptr() + 8 * top * at if top else None, L.stream()), 'lcq_token_logprobs')
+
+    if logits.numel():
+        run(logits, 0)
     return TokenLogprobs(logprobs, entropy, top_logprobs, top_tokens)

@@ -64,8 +64,17 @@ def _workspace(x, entry, *sizes):
     return torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
 
 
+def _like(x, dtype):
+    """A new contiguous tensor of x's shape.  (empty_like keeps strides, so only where they are those; it costs a third less.)"""
+    if x.is_contiguous():
+        return torch.empty_like(x, dtype=dtype)
+    return torch.empty(x.shape, dtype=dtype, device=x.device)
+
+
 def _rows(t, K):
     """-> (t or a contiguous copy, number of rows of K elements, distance between rows)."""
+    if t.is_contiguous():
+        return t, t.numel() // K, K
     if t.dim() == 2 and t.stride(1) == 1:
         return t, t.shape[0], t.stride(0)
     t = t.contiguous()
@@ -101,7 +110,7 @@ def quantize_tokens(x, symmetric=True, scale=None):
             return quantize_tokens(x, symmetric, scale)
     rows, T, ld = _rows(x, K)
     one = (*x.shape[:-1], 1)
-    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    codes = _like(x, torch.int8)
     scales = torch.empty(one, dtype=torch.float32, device=x.device) if given is None else given
     zeros = None if symmetric else torch.empty(one, dtype=torch.int32, device=x.device)
     if T:
@@ -183,9 +192,7 @@ def int8_linear(x, weight, weight_scales, bias=None, symmetric=True, scale=None,
 
 def _affine(name, t, K, x, flag):
     """The flag of a [K] parameter of a norm: of the tokens' type, or fp32."""
-    if t is None:
-        return 0
-    if tuple(t.shape) != (K,):
+    if t.dim() != 1 or t.shape[0] != K:
         raise ValueError(f'{name} of {K} columns has shape {tuple(t.shape)}')
     if t.dtype == x.dtype:
         return 0
@@ -212,9 +219,15 @@ def residual_norm(x, residual=None, weight=None, bias=None, *, gate=None, post_w
         raise ValueError(f'kind {kind!r}, quantize {quantize!r}')
     if post_bias is not None and post_weight is None:
         raise ValueError('post_bias goes with post_weight')
-    flags = (NORM_LAYER if kind == 'layer' else 0) | _affine('post_weight', post_weight, K, x, NORM_POST_WEIGHT_F32) \
-        | _affine('post_bias', post_bias, K, x, NORM_POST_BIAS_F32) | _affine('weight', weight, K, x, NORM_WEIGHT_F32) \
-        | _affine('bias', bias, K, x, NORM_BIAS_F32)
+    flags = NORM_LAYER if kind == 'layer' else 0
+    if weight is not None:
+        flags |= _affine('weight', weight, K, x, NORM_WEIGHT_F32)
+    if bias is not None:
+        flags |= _affine('bias', bias, K, x, NORM_BIAS_F32)
+    if post_weight is not None:
+        flags |= _affine('post_weight', post_weight, K, x, NORM_POST_WEIGHT_F32)
+    if post_bias is not None:
+        flags |= _affine('post_bias', post_bias, K, x, NORM_POST_BIAS_F32)
     stream_dtype = x.dtype
     if residual is not None:
         if residual.shape != x.shape:
@@ -226,6 +239,8 @@ def residual_norm(x, residual=None, weight=None, bias=None, *, gate=None, post_w
             flags |= NORM_RESIDUAL_F32
     if inplace and (residual is None or not residual.is_contiguous()):
         raise ValueError('inplace needs a contiguous residual')
+    if inplace and residual.requires_grad and torch.is_grad_enabled():
+        raise ValueError('inplace would change a residual that autograd keeps')
     if gate is not None:
         if gate.dtype != x.dtype:
             raise L.LcqError(f'gate is {gate.dtype}, x is {x.dtype}')
@@ -247,12 +262,12 @@ def residual_norm(x, residual=None, weight=None, bias=None, *, gate=None, post_w
         res, _, ldr = _rows(residual, K)
     if gate is not None:
         g, _, ldg = (gate.contiguous(), 1, 0) if gate.dim() == 1 else _rows(gate, K)
-    h = residual if inplace else torch.empty(x.shape, dtype=stream_dtype, device=x.device)
+    h = residual if inplace else _like(x, stream_dtype)
     out = codes = scales = zeros = None
     if quantize is None:
-        out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+        out = _like(x, out_dtype)
     else:
-        codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+        codes = _like(x, torch.int8)
         scales = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=x.device)
         if quantize == 'asymmetric':
             flags |= NORM_ASYM

@@ -1,0 +1,50 @@
+"""The rule by which the int8 product is cut (csrc/launch_rules.h), over sizes: compiled with the host compiler, no GPU needed."""
+import ctypes
+import itertools
+import shutil
+import subprocess
+
+import pytest
+
+from lightcompress_amd import _lib as L
+from lightcompress_amd.build import CSRC
+
+WRAPPERS = '''
+#include "launch_rules.h"
+extern "C" int cut(long long M, long long N, long long K) { const lcq::Int8Cut c = lcq::int8_cut(M, N, K); return c.tile * 256 + c.parts; }
+'''
+
+
+@pytest.fixture(scope='module')
+def cut(tmp_path_factory):
+    if not shutil.which('g++'):
+        pytest.skip('no host compiler')
+    d = tmp_path_factory.mktemp('cut')
+    (d / 'w.cpp').write_text(WRAPPERS)
+    subprocess.run(['g++', '-std=c++17', '-shared', '-fPIC', f'-I{CSRC}', str(d / 'w.cpp'), '-o', str(d / 'w.so')], check=True)
+    f = ctypes.CDLL(str(d / 'w.so')).cut
+    f.argtypes = [ctypes.c_longlong] * 3
+    return lambda *s: divmod(f(*s), 256)
+
+
+def test_parts_are_whole_fit_the_chip_and_the_workspace(cut):
+    for M, N, K in itertools.product((33, 64, 129, 300, 1000, 5000, 100000), (1, 16, 100, 4096, 6144, 14336, 140000), (16, 128, 2048, 4096, 14336, 65536)):
+        tile, parts = cut(M, N, K)
+        tiles = -(-M // 128) * -(-N // 128)
+        assert tile in (0, 1, 2) and 1 <= parts <= 16
+        if parts > 1:                              # parts of 128 x 128 tiles only, at least two stages each, one per CU, sums in the workspace
+            assert tile == 2 and parts * tiles <= 256 and -(-K // 128) // parts >= 2
+            assert L.lib().lcq_int8_matmul_workspace_bytes(M, N, K) >= 4 * M * N * parts
+        else:
+            assert L.lib().lcq_int8_matmul_workspace_bytes(M, N, K) == 0
+    for M, N, K in ((1, 4096, 4096), (32, 4096, 4096)):
+        assert L.lib().lcq_int8_matmul_workspace_bytes(M, N, K) == 0           # (streamed)
+        assert L.lib().lcq_int8_matmul_workspace_bytes(M, N, K + 1) >= (M + N) * (K + 16)
+
+
+def test_measured_choices(cut):
+    """The sizes at which the tiles were timed against each other: the fastest, or one within a few percent of it."""
+    for (M, N), tile in {(1024, 4096): 2, (2048, 4096): 2, (1024, 6144): 2, (2048, 6144): 1, (512, 14336): 2, (1024, 14336): 0,
+                         (2048, 14336): 0, (8192, 14336): 0}.items():
+        assert cut(M, N, 4096)[0] == tile, (M, N)
+    assert cut(64, 4096, 4096)[1] > 1 and cut(2048, 4096, 4096)[1] == 1

@@ -134,6 +134,34 @@ def test_shapes_strides_and_alignment(dev):
     assert token_logprobs(wide[:0].to(dev), top=3).top_tokens.shape == (0, 3)
 
 
+def test_sequences_without_their_last_logits(dev):
+    """logits[:, :-1] next to tokens[:, 1:], as perplexity takes them: the same bits as from a copy."""
+    x = (torch.randn(3, 9, 1001, generator=gen(12)) * 3).to(BF).to(dev)
+    t = torch.randint(0, 1001, (3, 9), generator=gen(13)).to(dev)
+    views = [(x[:, :-1], t[:, 1:]), (x[1:, 2:7], t[1:, :5]), (x[:1, :-1], t[:1, 1:]), (x.transpose(0, 1), t.t()), (x[:, :0], t[:, :0]),
+             (x[..., 3:900], t.clamp(max=800)), (x.view(3, 3, 3, 1001)[:, :2, 1:], t.view(3, 3, 3)[:, :2, 1:])]
+    for v, ids in views:
+        a, b = token_logprobs(v, ids, top=3), token_logprobs(v.clone(memory_format=torch.contiguous_format), ids.clone(), top=3)
+        assert all(torch.equal(p, q) and p.shape == q.shape for p, q in zip(a, b))
+    a = token_logprobs(x[:, :-1], torch.stack([t[:, 1:], t[:, :-1]], -1))
+    want = torch.log_softmax(x[:, :-1].double(), -1).gather(-1, torch.stack([t[:, 1:], t[:, :-1]], -1))
+    assert float((a.logprobs - want).abs().max()) < 1e-5
+
+
+@pytest.mark.parametrize('T,V', [(2, 30000), (700, 30000), (1500, 5000)])
+@pytest.mark.parametrize('dtype', [BF, F32])
+def test_rows_with_more_ties_than_room(dev, T, V, dtype):
+    """Alternatives out of hundreds of equal logits, and of fewer logits than alternatives."""
+    x = torch.randn(T, V, generator=gen(T + V))
+    x[0] = torch.randint(0, 3, (V,), generator=gen(20)).float()
+    x[1] = -INF
+    x[1, torch.randint(0, V, (7,), generator=gen(21))] = 1.0
+    x[T - 1, ::2] = 9.0
+    x[T // 2, V // 3:V // 3 + 513] = 8.0
+    for top in (1, 7, 20, 64):
+        check(x.to(dtype).to(dev), torch.zeros(T, dtype=torch.int64, device=dev), top)
+
+
 def test_behind_two_to_the_31(dev):
     T, V = 17000, 128256
     x = torch.zeros(T, V, dtype=BF, device=dev)

@@ -54,6 +54,7 @@ def test_cpu_tensors_are_refused():
     (lambda: residual_norm(torch.zeros(2, 64), out_dtype=torch.bfloat16), L.LcqError),
     (lambda: residual_norm(torch.zeros(2, 64), inplace=True), ValueError),
     (lambda: residual_norm(torch.zeros(2, 64), torch.zeros(64, 2).t(), inplace=True), ValueError),
+    (lambda: residual_norm(torch.zeros(2, 64), torch.zeros(2, 64, requires_grad=True), inplace=True), ValueError),
     (lambda: token_logprobs(torch.zeros(2, 0)), ValueError),
     (lambda: token_logprobs(torch.zeros(2, 8), top=9), ValueError),
     (lambda: token_logprobs(torch.zeros(2, 80), top=65), ValueError),
