@@ -229,12 +229,13 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MatmulArgs g, int tiles_m,
     }
   }
   __syncthreads();
-  // A wave's outputs leave through its own part of LDS, 16 bytes per lane along a token; chunk c of 16 bytes of token t lies at c ^ t.
+  // A wave's outputs leave through its own part of LDS, 16 bytes per lane along a token; the chunks of 16 bytes of token t are turned by t.
   constexpr int E = BF == ROW_F32 || BF == ROW_I32 ? 4 : 2, CH = 16 / E;     // bytes of an output, outputs of a chunk
   constexpr int ROW = FN * 32 * E, CHUNKS = ROW / 16;
   constexpr int STEP = E == 4 && FM > 1 ? FM / 2 : FM;                       // blocks of 32 tokens that leave together
   static_assert(4 * STEP * 32 * ROW <= STAGES * T::STAGE, "outputs on their way out");
   char* const mine = lds + wave * STEP * 32 * ROW;
+  const auto turned = [](int chunk, int token) { return (chunk + token) % CHUNKS; };
   const int t = lane & 31, h = lane >> 5;
   #pragma unroll
   for (int i0 = 0; i0 < FM; i0 += STEP) {
@@ -261,7 +262,7 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MatmulArgs g, int tiles_m,
             if constexpr (ASYM) s -= az[i] * sum[r];
             v[r] = BF == ROW_I32 ? __builtin_bit_cast(float, s) : __builtin_fmaf((float)s, as[i] * ws[r], b[r]);
           }
-          char* const to = mine + ((i - i0) * 32 + t) * ROW + (((c / CH) ^ t) % CHUNKS) * 16 + (c % CH) * E;
+          char* const to = mine + ((i - i0) * 32 + t) * ROW + turned(c / CH, t) * 16 + (c % CH) * E;
           if constexpr (E == 4) *(f32x4*)to = f32x4{v[0], v[1], v[2], v[3]};
           else if constexpr (BF == ROW_BF16) *(u32x2*)to = u32x2{bf16_pack_rne(v[0], v[1]), bf16_pack_rne(v[2], v[3])};
           else *(u32x2*)to = u32x2{f16_pack_rne(v[0], v[1]), f16_pack_rne(v[2], v[3])};
@@ -272,7 +273,7 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MatmulArgs g, int tiles_m,
     #pragma unroll
     for (int o = 0; o < STEP * 32 * CHUNKS / 64; ++o) {
       const int idx = o * 64 + lane, tt = idx / CHUNKS, ch = idx % CHUNKS;
-      const u32x4 v = *(const u32x4*)(mine + tt * ROW + ((ch ^ tt) % CHUNKS) * 16);
+      const u32x4 v = *(const u32x4*)(mine + tt * ROW + turned(ch, tt % 32) * 16);
       const int m = wr * FM * 32 + i0 * 32 + tt, n = wc * FN * 32 + ch * CH;
       if (m >= rows_a || n >= rows_w) continue;
       const int64_t cell = (m0 + m) * g.N + n0 + n + (BF == ROW_I32 ? part * g.M * g.N : 0);

@@ -48,3 +48,9 @@ def test_measured_choices(cut):
                          (2048, 14336): 0, (8192, 14336): 0}.items():
         assert cut(M, N, 4096)[0] == tile, (M, N)
     assert cut(64, 4096, 4096)[1] > 1 and cut(2048, 4096, 4096)[1] == 1
+
+
+def test_sizes_of_the_gpu_tests_reach_every_tile(cut):
+    from tests.test_w8a8_gpu import SIZES, TILED
+    assert {cut(*s)[0] for s in TILED} == {0, 1, 2} and {cut(M, N, -(-K // 16) * 16)[0] for M, N, K in SIZES if M > 32} >= {2}
+    assert sum(cut(*s)[1] > 1 for s in TILED) >= 2 and [cut(*s)[0] for s in TILED[:5]] == [0, 0, 1, 1, 1]

@@ -59,7 +59,7 @@ def check(x, tokens=None, top=0, ignore=-100, got=None):
 @pytest.mark.parametrize('dtype', [BF, HF, F32])
 @pytest.mark.parametrize('T,V,top', [(1, 1, 1), (1, 2, 2), (3, 7, 3), (2, 63, 20), (5, 64, 64), (4, 100, 1), (2, 511, 5), (3, 512, 64), (700, 513, 5),
                                      (1, 2047, 10), (2, 2048, 0), (1, 32000, 20), (9, 32001, 64), (1, 128256, 20), (33, 50257, 5), (600, 8191, 2),
-                                     (1, 160001, 64), (2048, 1000, 3), (4097, 130, 1)])
+                                     (1, 160001, 64), (2048, 1000, 3), (4097, 130, 1), (1100, 70001, 7), (300, 70001, 20), (2, 262144, 64)])
 def test_logprobs(dev, T, V, top, dtype):
     x = (torch.randn(T, V, generator=gen(T + V)) * 3).to(dtype).to(dev)
     tokens = torch.randint(0, V, (T,), generator=gen(V)).to(dev)

@@ -132,7 +132,8 @@ def product_inputs(M, N, K, asym, bias, ws_dtype=F32, seed=0, dev=None):
 SIZES = [(1, 1, 1), (1, 64, 64), (1, 1000, 4096), (2, 17, 63), (3, 4096, 128), (7, 100, 2050), (8, 256, 1024), (15, 33, 80), (16, 4096, 4096),
          (17, 130, 272), (31, 64, 4112), (32, 512, 512), (33, 257, 1040), (48, 1024, 2048), (64, 64, 64), (65, 1001, 2047), (100, 300, 4096),
          (127, 129, 144), (128, 128, 16), (129, 2048, 512), (200, 96, 14336), (255, 511, 1008), (256, 256, 4096), (257, 4096, 1024),
-         (300, 5000, 48), (513, 513, 513), (1000, 777, 2064), (2048, 1024, 4096), (4097, 300, 256), (20, 24, 65536), (300, 264, 65536)]
+         (300, 5000, 48), (513, 513, 513), (1000, 777, 2064), (2048, 1024, 4096), (4097, 300, 256), (20, 24, 65536), (300, 264, 65536),
+         (17, 4112, 528), (32, 5001, 272), (25, 9000, 4112), (5, 9001, 2064)]
 
 
 @pytest.mark.parametrize('asym,bias,dtype', [(False, False, BF), (True, True, F32), (True, False, HF), (False, True, F32)])
@@ -141,6 +142,19 @@ def test_product(dev, M, N, K, asym, bias, dtype):
     q, s, z, w, ws, b = product_inputs(M, N, K, asym, bias, dev=dev)
     if dtype == HF:
         ws = ws / K                                # (sums of K products of 128 by 128 stay within fp16)
+    check_product(int8_matmul(QuantizedTokens(q, s, z), w, ws, b, out_dtype=dtype), q, s, z, w, ws, b, dtype)
+
+
+# sizes of each tile (test_int8_cut_cpu.py holds the rule to them): 256 x 256, 256 x 192, 128 x 128 in parts of K
+TILED = [(1000, 14300, 1040), (4090, 4090, 528), (1500, 6100, 640), (2048, 6144, 4096), (700, 14300, 1040), (70, 4100, 4112), (300, 1000, 14336)]
+
+
+@pytest.mark.parametrize('asym,dtype', [(False, BF), (True, F32), (True, HF)])
+@pytest.mark.parametrize('M,N,K', TILED)
+def test_product_in_every_tile(dev, M, N, K, asym, dtype):
+    q, s, z, w, ws, b = product_inputs(M, N, K, asym, True, dev=dev)
+    if dtype == HF:
+        ws = ws / K
     check_product(int8_matmul(QuantizedTokens(q, s, z), w, ws, b, out_dtype=dtype), q, s, z, w, ws, b, dtype)
 
 
@@ -189,6 +203,18 @@ def test_linear_is_codes_and_product(dev, M, K, dtype):
             want = int8_matmul(quantize_tokens(x, **kw), w, ws, b, out_dtype=F32)
             assert_bit_equal(int8_linear(x, w, ws, b, out_dtype=F32, **kw), want, f'{kw}')
         assert int8_linear(x, w, ws).dtype == dtype
+
+
+@pytest.mark.parametrize('N,K', [(8200, 512), (8193, 4096), (9000, 16400), (4096, 8208), (1, 8192), (17, 16)])
+@pytest.mark.parametrize('symmetric', [True, False])
+def test_one_token(dev, N, K, symmetric):
+    g = torch.Generator(device=dev)
+    g.manual_seed(N)
+    w = torch.randint(-128, 128, (N, K), generator=g, dtype=torch.int8, device=dev)
+    ws = 0.01 * torch.rand(N, 1, generator=g, device=dev)
+    x = acts(1, K, BF, seed=N, shift=0.2).to(dev)
+    q = quantize_tokens(x, symmetric)
+    check_product(int8_linear(x, w, ws, symmetric=symmetric, out_dtype=F32), q.codes, q.scales, q.zeros, w, ws, None, F32)
 
 
 def test_product_shapes_and_nothing(dev):
