@@ -325,11 +325,12 @@ __global__ __launch_bounds__(256) void join_kernel(MatmulArgs g, const int* __re
 
 // ---- few tokens ---------------------------------------------------------------------------------------------------
 // The weight is read once, straight into the matrix pipe's operands: a lane of v_mfma_i32_16x16x64_i8 takes 16 codes of one of 16
-// channels, so a load of the wave is 16 rows x 64 bytes in a row.  A workgroup owns 16 channels, its eight waves take pieces of 256
-// codes of K in turn and meet in LDS; three pieces (12 KiB of weight per wave) are in flight.  The tokens' codes come from the cache, every
-// wave other ones.
+// channels, so a load of the wave is 16 rows x 64 bytes in a row.  A workgroup owns 16 or 32 channels, its waves take pieces of 256
+// codes of K in turn and meet in LDS; four (two) pieces, 16 KiB of weight per wave, are in flight, with the codes of the tokens beside them,
+// which come from the cache.  What bounds it is the ramp of the first loads and then HBM, 3 us + the weight at 5.5 TB/s: 2 tokens take 6.1 us
+// at N = K = 4096, 43 us (5.4 TB/s) at 8192 x 28672; the tokens' codes pass the L2 once per workgroup, which tells from 16 tokens on.
 // A single token may come as values: every workgroup makes its codes itself, in LDS, while its first weights are on their way - cheaper
-// than another kernel in front.
+// than another kernel in front (6.4 us at N = K = 4096, the quantizer alone 3.4).
 constexpr int PIECE = 256;
 constexpr int64_t MOST_FUSED = 32768;               // codes of a token that is quantized in LDS
 
@@ -449,7 +450,7 @@ __global__ __launch_bounds__(WAVES * 64) void stream_kernel(MatmulArgs g, TokenA
   #pragma unroll
   for (int b = 0; b < TB; ++b) ofA[b] = b * 16 + (lane & 15) < g.M ? (uint32_t)((b * 16 + (lane & 15)) * g.lda) + at : OUTSIDE;
   // DEPTH pieces of 256 codes in flight, each with its tokens': waiting for the oldest leaves the others on their way
-  constexpr int DEPTH = TB + NB <= 3 ? 3 : 2, STEP = WAVES * PIECE;
+  constexpr int DEPTH = TB + NB <= 3 ? 4 : 2, STEP = WAVES * PIECE;
   struct Piece { i32x4 w[NB][4], a[TB][4]; } ring[DEPTH];
   const auto load = [&](int k, Piece& p) {          // codes k .. k + 255
     #pragma unroll
@@ -572,12 +573,25 @@ void launch_stream(const MatmulArgs& g, const TokenArgs& t, hipStream_t st) {
   stream_kernel<TB, NB, BF, XT, WAVES><<<dim3((unsigned)((g.N + 16 * NB - 1) / (16 * NB))), dim3(WAVES * 64), XT < 0 ? 0 : (unsigned)g.K, st>>>(g, t);
 }
 
+// Two blocks of channels per workgroup halve the passes of the tokens' codes through the L2, one block spreads better over 256 CUs: it is
+// taken where the busiest CU then has at most 3/4 (beyond 16 tokens half) of the channels.  us for one / two blocks:
+//   N = 4096, K = 4096    16 tokens  7.0 / 9.5   32 tokens  9.5 / 12.8      N = 10240, K = 8192   16 tokens 26.4 / 27.9   32 tokens 39.5 / 35.8
+//   N = 6144, K = 4096    16 tokens 11.3 / 10.9  32 tokens 16.2 / 13.0      N = 14336, K = 4096   16 tokens 19.5 / 17.1   32 tokens 28.6 / 22.4
+// Two waves share K (four: 7.5 us for 7.1 in the first of these), one where there are two blocks and more workgroups than CUs (the last of
+// these takes 23.7 with two waves; 8192 x 28672 at 32 tokens 65.5 with one for 64.5).
+template <int TB, int BF>
+void launch_few(const MatmulArgs& g, hipStream_t st) {
+  const int64_t one = (g.N + 4095) / 4096, two = (g.N + 8191) / 8192 * 2;    // blocks of 16 channels on the busiest CU
+  if (4 * one <= (TB == 1 ? 3 : 2) * two) launch_stream<TB, 1, BF, -1, 2>(g, TokenArgs{}, st);
+  else if (two == 2) launch_stream<TB, 2, BF, -1, 2>(g, TokenArgs{}, st);
+  else launch_stream<TB, 2, BF, -1, 1>(g, TokenArgs{}, st);
+}
+
 template <int BF>
 void launch_codes(const MatmulArgs& g, int* sums, hipStream_t st) {
   if (g.M <= INT8_STREAMED) {
-    if (g.M <= 16) launch_stream<1, 1, BF, -1, 2>(g, TokenArgs{}, st);
-    else if (g.N <= 4096) launch_stream<2, 1, BF, -1, 2>(g, TokenArgs{}, st);
-    else launch_stream<2, 2, BF, -1, 2>(g, TokenArgs{}, st);
+    if (g.M <= 16) launch_few<1, BF>(g, st);
+    else launch_few<2, BF>(g, st);
   }
   else {
     const Int8Cut c = int8_cut(g.M, g.N, g.K);
@@ -593,10 +607,11 @@ void launch_codes(const MatmulArgs& g, int* sums, hipStream_t st) {
   }
 }
 
+// Few waves share the quantization of a short token (N = K = 4096: four waves 6.4 us, two 6.9, eight 7.6; N = 28672: 25.4, 26.7, 34),
+// eight keep enough of a long weight row on its way (4096 x 14336: 14.7 us, four 16.9; 8192 x 28672: 45.4, four 50.6).
 template <int BF, int XT>
 void launch_token(const MatmulArgs& g, const TokenArgs& t, hipStream_t st) {
-  if (g.N > 8192) launch_stream<1, 1, BF, XT, 2>(g, t, st);
-  else if (g.K <= 8192) launch_stream<1, 1, BF, XT, 4>(g, t, st);
+  if (g.K <= 8192) launch_stream<1, 1, BF, XT, 4>(g, t, st);
   else launch_stream<1, 1, BF, XT, 8>(g, t, st);
 }
 

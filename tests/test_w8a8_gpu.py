@@ -158,6 +158,20 @@ def test_product_in_every_tile(dev, M, N, K, asym, dtype):
     check_product(int8_matmul(QuantizedTokens(q, s, z), w, ws, b, out_dtype=dtype), q, s, z, w, ws, b, dtype)
 
 
+# at most 32 tokens: one or two blocks of 16 of them by one or two of 16 channels
+FEW = [(16, 4096, 1040), (2, 4100, 528), (16, 8192, 4112), (7, 8200, 272), (1, 14339, 528), (17, 4096, 528), (24, 4097, 1040), (32, 8192, 4112),
+       (31, 8200, 272), (32, 14339, 16), (9, 14336, 1040), (3, 28673, 48)]
+
+
+@pytest.mark.parametrize('asym,dtype', [(False, BF), (True, F32), (True, HF)])
+@pytest.mark.parametrize('M,N,K', FEW)
+def test_product_of_few_tokens(dev, M, N, K, asym, dtype):
+    q, s, z, w, ws, b = product_inputs(M, N, K, asym, True, dev=dev)
+    if dtype == HF:
+        ws = ws / K
+    check_product(int8_matmul(QuantizedTokens(q, s, z), w, ws, b, out_dtype=dtype), q, s, z, w, ws, b, dtype)
+
+
 @pytest.mark.parametrize('M', [1, 16, 40, 300])
 def test_product_at_the_ends_of_the_range(dev, M):
     """All codes -128 at K = 65536, zero points 127: the largest sums there are."""
