@@ -425,8 +425,21 @@ struct TokenRow {
 };
 template <int WAVES> struct TokenRow<-1, WAVES> {};
 
+// 16 codes that were read `codes` too early: the first ones leave, zeros follow
+__device__ __forceinline__ i32x4 later(i32x4 v, int codes) {
+  struct Halves { uint64_t lo, hi; } h = __builtin_bit_cast(Halves, v);
+  const int s = (codes & 7) * 8;
+  if (codes >= 8) { h.lo = h.hi; h.hi = 0; }
+  if (codes >= 16) h.lo = 0;
+  h.lo = h.lo >> s | (h.hi << 1) << (63 - s);
+  h.hi >>= s;
+  return __builtin_bit_cast(i32x4, h);
+}
+
 // TB blocks of 16 tokens, NB blocks of 16 channels.  XT: the type of one token's values (TB = 1), or -1 for codes.
-template <int TB, int NB, int BF, int XT, int WAVES>
+// ODD: rows start on any byte (K >= 16).  16 codes are cut from the five words that hold them, which costs far less than loads off word
+// alignment (K = 4097, N = 14336, 16 tokens: 25.5 us for 66; 38 by padded copies); a row's last codes are read from K - 16 and moved.
+template <int TB, int NB, int BF, int XT, int WAVES, bool ODD>
 __global__ __launch_bounds__(WAVES * 64) void stream_kernel(MatmulArgs g, TokenArgs t) {
   __shared__ __attribute__((aligned(16))) int red[WAVES][NB][TB + 1][64][4];
   __shared__ float token_scale;
@@ -449,12 +462,40 @@ __global__ __launch_bounds__(WAVES * 64) void stream_kernel(MatmulArgs g, TokenA
   for (int c = 0; c < NB; ++c) ofW[c] = c * 16 + (lane & 15) < rows_w ? (uint32_t)((c * 16 + (lane & 15)) * g.ldw) + at : OUTSIDE;
   #pragma unroll
   for (int b = 0; b < TB; ++b) ofA[b] = b * 16 + (lane & 15) < g.M ? (uint32_t)((b * 16 + (lane & 15)) * g.lda) + at : OUTSIDE;
+  // words around the first codes of the matrices and, from there, this lane's rows (what a channel or token past the last one gives is not stored)
+  const int8_t *wordsW = nullptr, *wordsA = nullptr;
+  if constexpr (ODD) {
+    const int8_t *const w = g.w + n0 * g.ldw, *const a = g.a;
+    const uint32_t inW = (uint32_t)(uintptr_t)w & 3, inA = (uint32_t)(uintptr_t)a & 3;
+    wordsW = w - inW;
+    wordsA = a - inA;
+    #pragma unroll
+    for (int c = 0; c < NB; ++c) ofW[c] = inW + (uint32_t)((c * 16 + (lane & 15) < rows_w ? c * 16 + (lane & 15) : rows_w - 1) * g.ldw);
+    #pragma unroll
+    for (int b = 0; b < TB; ++b) ofA[b] = inA + (uint32_t)((b * 16 + (lane & 15) < g.M ? b * 16 + (lane & 15) : g.M - 1) * g.lda);
+  }
+  const auto words = [](const int8_t* p, uint32_t of, i32x4& v, int& fifth) {          // (every word holds one of the codes at least)
+    __builtin_memcpy(&v, __builtin_assume_aligned(p + (of & ~3u), 4), 16);
+    fifth = *(const int*)(p + (of & ~3u) + (of & 3 ? 16 : 12));
+  };
+  const auto cut = [](i32x4 v, int fifth, uint32_t of) {
+    return i32x4{(int)__builtin_amdgcn_alignbyte(v[1], v[0], of), (int)__builtin_amdgcn_alignbyte(v[2], v[1], of),
+                 (int)__builtin_amdgcn_alignbyte(v[3], v[2], of), (int)__builtin_amdgcn_alignbyte(fifth, v[3], of)};
+  };
   // DEPTH pieces of 256 codes in flight, each with its tokens': waiting for the oldest leaves the others on their way
-  constexpr int DEPTH = TB + NB <= 3 ? 4 : 2, STEP = WAVES * PIECE;
-  struct Piece { i32x4 w[NB][4], a[TB][4]; } ring[DEPTH];
+  constexpr int DEPTH = ODD ? (TB + NB == 2 ? 3 : 2) : TB + NB <= 3 ? 4 : 2, STEP = WAVES * PIECE;
+  struct Piece { i32x4 w[NB][4], a[TB][4]; int w5[ODD ? NB : 1][4], a5[ODD ? TB : 1][4]; } ring[DEPTH];
   const auto load = [&](int k, Piece& p) {          // codes k .. k + 255
     #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      if constexpr (ODD) {
+        const uint32_t from = k + i * 64 + at < g.K - 16 ? k + i * 64 + at : g.K - 16;
+        #pragma unroll
+        for (int c = 0; c < NB; ++c) words(wordsW, ofW[c] + from, p.w[c][i], p.w5[c][i]);
+        #pragma unroll
+        for (int b = 0; b < TB; ++b) words(wordsA, ofA[b] + from, p.a[b][i], p.a5[b][i]);
+        continue;
+      }
       const uint32_t outside = k + i * 64 + at < g.K ? 0u : OUTSIDE;
       #pragma unroll
       for (int c = 0; c < NB; ++c)
@@ -479,6 +520,23 @@ __global__ __launch_bounds__(WAVES * 64) void stream_kernel(MatmulArgs g, TokenA
     #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
       Piece& p = ring[d];
+      if constexpr (ODD) {
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int early = k + i * 64 + at - (g.K - 16);
+          const uint32_t from = early < 0 ? 0 : g.K - 16;                    // (k + i 64 + at is whole words)
+          #pragma unroll
+          for (int c = 0; c < NB; ++c) p.w[c][i] = cut(p.w[c][i], p.w5[c][i], ofW[c] + from);
+          #pragma unroll
+          for (int b = 0; b < TB; ++b) p.a[b][i] = cut(p.a[b][i], p.a5[b][i], ofA[b] + from);
+          if (k + PIECE > g.K) {
+            #pragma unroll
+            for (int c = 0; c < NB; ++c) p.w[c][i] = later(p.w[c][i], early > 0 ? early : 0);
+            #pragma unroll
+            for (int b = 0; b < TB; ++b) p.a[b][i] = later(p.a[b][i], early > 0 ? early : 0);
+          }
+        }
+      }
       #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if constexpr (XT >= 0) p.a[0][i] = *(const i32x4*)(codes + (k + i * 64 + at < g.K ? k + i * 64 + at : 0));   // (every column the token; past K the weight is 0)
@@ -568,9 +626,9 @@ void launch_join(const MatmulArgs& g, const int* sums, int parts, hipStream_t st
   else join_kernel<BF, 1><<<dim3((unsigned)((all + 255) / 256)), dim3(256), 0, st>>>(g, sums, parts);
 }
 
-template <int TB, int NB, int BF, int XT, int WAVES>
+template <int TB, int NB, int BF, int XT, int WAVES, bool ODD = false>
 void launch_stream(const MatmulArgs& g, const TokenArgs& t, hipStream_t st) {
-  stream_kernel<TB, NB, BF, XT, WAVES><<<dim3((unsigned)((g.N + 16 * NB - 1) / (16 * NB))), dim3(WAVES * 64), XT < 0 ? 0 : (unsigned)g.K, st>>>(g, t);
+  stream_kernel<TB, NB, BF, XT, WAVES, ODD><<<dim3((unsigned)((g.N + 16 * NB - 1) / (16 * NB))), dim3(WAVES * 64), XT < 0 ? 0 : (unsigned)g.K, st>>>(g, t);
 }
 
 // Two blocks of channels per workgroup halve the passes of the tokens' codes through the L2, one block spreads better over 256 CUs: it is
@@ -579,19 +637,20 @@ void launch_stream(const MatmulArgs& g, const TokenArgs& t, hipStream_t st) {
 //   N = 6144, K = 4096    16 tokens 11.3 / 10.9  32 tokens 16.2 / 13.0      N = 14336, K = 4096   16 tokens 19.5 / 17.1   32 tokens 28.6 / 22.4
 // Two waves share K (four: 7.5 us for 7.1 in the first of these), one where there are two blocks and more workgroups than CUs (the last of
 // these takes 23.7 with two waves; 8192 x 28672 at 32 tokens 65.5 with one for 64.5).
-template <int TB, int BF>
+template <int TB, int BF, bool ODD>
 void launch_few(const MatmulArgs& g, hipStream_t st) {
   const int64_t one = (g.N + 4095) / 4096, two = (g.N + 8191) / 8192 * 2;    // blocks of 16 channels on the busiest CU
-  if (4 * one <= (TB == 1 ? 3 : 2) * two) launch_stream<TB, 1, BF, -1, 2>(g, TokenArgs{}, st);
-  else if (two == 2) launch_stream<TB, 2, BF, -1, 2>(g, TokenArgs{}, st);
-  else launch_stream<TB, 2, BF, -1, 1>(g, TokenArgs{}, st);
+  if (4 * one <= (TB == 1 ? 3 : 2) * two) launch_stream<TB, 1, BF, -1, 2, ODD>(g, TokenArgs{}, st);
+  else if (two == 2) launch_stream<TB, 2, BF, -1, 2, ODD>(g, TokenArgs{}, st);
+  else launch_stream<TB, 2, BF, -1, 1, ODD>(g, TokenArgs{}, st);
 }
 
 template <int BF>
 void launch_codes(const MatmulArgs& g, int* sums, hipStream_t st) {
   if (g.M <= INT8_STREAMED) {
-    if (g.M <= 16) launch_few<1, BF>(g, st);
-    else launch_few<2, BF>(g, st);
+    const bool odd = g.K % 16 != 0;
+    if (g.M <= 16) odd ? launch_few<1, BF, true>(g, st) : launch_few<1, BF, false>(g, st);
+    else odd ? launch_few<2, BF, true>(g, st) : launch_few<2, BF, false>(g, st);
   }
   else {
     const Int8Cut c = int8_cut(g.M, g.N, g.K);
@@ -625,6 +684,9 @@ int check(const int8_t* w, const void* ws, int ws_dtype, const void* bias, int b
   return LCQ_OK;
 }
 
+// rows that only the padding kernel brings to where they can be read
+bool pads(int64_t M, int64_t K) { return K % 16 != 0 && (M > INT8_STREAMED || K < 16); }
+
 // one token, whose codes the product makes itself
 bool fused(int64_t M, int64_t K) { return M == 1 && K % 16 == 0 && K <= MOST_FUSED; }
 
@@ -635,7 +697,7 @@ extern "C" {
 int64_t lcq_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0 || K > 65536) return 0;
   const int parts = M <= INT8_STREAMED ? 1 : int8_cut(M, N, padded(K)).parts;
-  return (parts > 1 ? on256(4 * M * N * parts) : 0) + (K % 16 ? (M + N) * padded(K) : 0);
+  return (parts > 1 ? on256(4 * M * N * parts) : 0) + (pads(M, K) ? (M + N) * padded(K) : 0);
 }
 
 int lcq_int8_matmul(const int8_t* a, const float* as, int a_scalar, const int32_t* az, const int8_t* w, const void* ws, int ws_dtype,
@@ -648,11 +710,11 @@ int lcq_int8_matmul(const int8_t* a, const float* as, int a_scalar, const int32_
   MatmulArgs g = {a, w, as, az, ws, bias, y, M, N, K, K, (int)K, ws_dtype, bias_dtype, a_scalar, w_scalar};
   if (K % 16 == 0 && (uintptr_t)a % 16) return LCQ_EALIGN;
   const int parts = M <= INT8_STREAMED ? 1 : int8_cut(M, N, padded(K)).parts;
-  if (K % 16 || parts > 1) {
+  if (pads(M, K) || parts > 1) {
     if (!workspace) return LCQ_EWORKSPACE;
     if ((uintptr_t)workspace % 16) return LCQ_EALIGN;
   }
-  if (K % 16) {
+  if (pads(M, K)) {
     const int Kp = (int)padded(K);
     int8_t* const pa = (int8_t*)workspace + (parts > 1 ? on256(4 * M * N * parts) : 0);
     const int64_t blocks = (M + N + 3) / 4;

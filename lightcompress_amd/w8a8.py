@@ -153,7 +153,7 @@ def int8_matmul(tokens, weight, weight_scales, bias=None, out_dtype=torch.bfloat
     if not _here(codes, scales, zeros, weight, weight_scales, bias):
         with torch.cuda.device(codes.device):
             return int8_matmul(tokens, weight, weight_scales, bias, out_dtype)
-    if K % 16 == 0:                           # (other widths are copied to padded rows by the call itself)
+    if K % 16 == 0:                           # (rows of other widths may start anywhere)
         codes, weight = _on16(codes), _on16(weight)
     y = torch.empty((*codes.shape[:-1], N), dtype=out_dtype, device=codes.device)
     if M and N:
@@ -178,7 +178,7 @@ def int8_linear(x, weight, weight_scales, bias=None, symmetric=True, scale=None,
         with torch.cuda.device(x.device):
             return int8_linear(x, weight, weight_scales, bias, symmetric, scale, out_dtype)
     rows, M, ld = _rows(x, K)
-    if K % 16 == 0:                           # (other widths are copied to padded rows by the call itself)
+    if K % 16 == 0:                           # (rows of other widths may start anywhere)
         weight = _on16(weight)
     y = torch.empty((*x.shape[:-1], N), dtype=out_dtype, device=x.device)
     if M and N:
