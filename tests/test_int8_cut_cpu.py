@@ -40,8 +40,8 @@ def test_parts_are_whole_fit_the_chip_and_the_workspace(cut):
     for M, N, K in ((1, 4096, 4096), (32, 4096, 4096)):
         assert L.lib().lcq_int8_matmul_workspace_bytes(M, N, K) == 0           # (streamed)
         assert L.lib().lcq_int8_matmul_workspace_bytes(M, N, K + 1) == 0       # (whatever the width)
-    for M, N, K in ((33, 4096, 4096), (1, 4096, 0), (32, 100, 14)):            # padded rows: many tokens, fewer than 16 codes
-        assert L.lib().lcq_int8_matmul_workspace_bytes(M, N, K + 1) >= (M + N) * (K + 16)
+    for M, N, K in ((33, 4096, 4097), (1, 4096, 1), (32, 100, 15)):            # padded rows: many tokens, fewer than 16 codes
+        assert L.lib().lcq_int8_matmul_workspace_bytes(M, N, K) >= (M + N) * -(-K // 16) * 16
 
 
 def test_measured_choices(cut):
