@@ -477,8 +477,8 @@ int lcq_quant_tokens(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx
  * each token and each channel.  The sums are exact integers; the factors and the bias are applied in fp32, y is rounded once.
  *  a       [M, K] int8, as [M] fp32 (or [1] with a_scalar), az [M] int32 within +-128 or NULL
  *  w       [N, K] int8, ws [N] of ws_dtype (or [1] with w_scalar), bias [N] of bias_dtype or NULL;  K <= 65536
- *          (a and w on 16 bytes where K is a multiple of 16; rows of other widths may start anywhere: beyond 32 tokens they are copied
- *          to padded rows in the workspace)
+ *          (a and w on 16 bytes where K is a multiple of 16; rows of other widths may start anywhere: for many tokens they are
+ *          copied to padded rows in the workspace)
  *  y       [M, N] of `dtype`
  *  workspace of lcq_int8_matmul_workspace_bytes(M, N, K) (0: none), 16-byte aligned. */
 int64_t lcq_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);

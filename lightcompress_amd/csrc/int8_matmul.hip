@@ -645,12 +645,19 @@ void launch_few(const MatmulArgs& g, hipStream_t st) {
   else launch_stream<TB, 2, BF, -1, 1, ODD>(g, TokenArgs{}, st);
 }
 
+template <int BF, bool ODD>
+void launch_blocks(const MatmulArgs& g, hipStream_t st) {
+  if (g.M <= 16) launch_few<1, BF, ODD>(g, st);
+  else if (g.M <= 32) launch_few<2, BF, ODD>(g, st);
+  else if (g.M <= 48) launch_stream<3, 1, BF, -1, 2, ODD>(g, TokenArgs{}, st);
+  else launch_stream<4, 1, BF, -1, 2, ODD>(g, TokenArgs{}, st);
+}
+
 template <int BF>
-void launch_codes(const MatmulArgs& g, int* sums, hipStream_t st) {
-  if (g.M <= INT8_STREAMED) {
-    const bool odd = g.K % 16 != 0;
-    if (g.M <= 16) odd ? launch_few<1, BF, true>(g, st) : launch_few<1, BF, false>(g, st);
-    else odd ? launch_few<2, BF, true>(g, st) : launch_few<2, BF, false>(g, st);
+void launch_codes(const MatmulArgs& g, bool streams, int* sums, hipStream_t st) {
+  if (streams) {
+    if (g.K % 16) launch_blocks<BF, true>(g, st);
+    else launch_blocks<BF, false>(g, st);
   }
   else {
     const Int8Cut c = int8_cut(g.M, g.N, g.K);
@@ -685,7 +692,7 @@ int check(const int8_t* w, const void* ws, int ws_dtype, const void* bias, int b
 }
 
 // rows that only the padding kernel brings to where they can be read
-bool pads(int64_t M, int64_t K) { return K % 16 != 0 && (M > INT8_STREAMED || K < 16); }
+bool pads(int64_t K, bool streams) { return K % 16 != 0 && (!streams || K < 16); }
 
 // one token, whose codes the product makes itself
 bool fused(int64_t M, int64_t K) { return M == 1 && K % 16 == 0 && K <= MOST_FUSED; }
@@ -696,8 +703,9 @@ extern "C" {
 
 int64_t lcq_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0 || K > 65536) return 0;
-  const int parts = M <= INT8_STREAMED ? 1 : int8_cut(M, N, padded(K)).parts;
-  return (parts > 1 ? on256(4 * M * N * parts) : 0) + (pads(M, K) ? (M + N) * padded(K) : 0);
+  const bool streams = int8_streams(M, N, K);
+  const int parts = streams ? 1 : int8_cut(M, N, padded(K)).parts;
+  return (parts > 1 ? on256(4 * M * N * parts) : 0) + (pads(K, streams) ? (M + N) * padded(K) : 0);
 }
 
 int lcq_int8_matmul(const int8_t* a, const float* as, int a_scalar, const int32_t* az, const int8_t* w, const void* ws, int ws_dtype,
@@ -709,21 +717,22 @@ int lcq_int8_matmul(const int8_t* a, const float* as, int a_scalar, const int32_
   hipStream_t st = (hipStream_t)stream;
   MatmulArgs g = {a, w, as, az, ws, bias, y, M, N, K, K, (int)K, ws_dtype, bias_dtype, a_scalar, w_scalar};
   if (K % 16 == 0 && (uintptr_t)a % 16) return LCQ_EALIGN;
-  const int parts = M <= INT8_STREAMED ? 1 : int8_cut(M, N, padded(K)).parts;
-  if (pads(M, K) || parts > 1) {
+  const bool streams = int8_streams(M, N, K);
+  const int parts = streams ? 1 : int8_cut(M, N, padded(K)).parts;
+  if (pads(K, streams) || parts > 1) {
     if (!workspace) return LCQ_EWORKSPACE;
     if ((uintptr_t)workspace % 16) return LCQ_EALIGN;
   }
-  if (pads(M, K)) {
+  if (pads(K, streams)) {
     const int Kp = (int)padded(K);
     int8_t* const pa = (int8_t*)workspace + (parts > 1 ? on256(4 * M * N * parts) : 0);
     const int64_t blocks = (M + N + 3) / 4;
     pad_kernel<<<dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st>>>(a, M, w, M + N, (int)K, Kp, pa);
     g.a = pa; g.w = pa + M * Kp; g.lda = g.ldw = g.K = Kp;
   }
-  if (dtype == LCQ_BF16) launch_codes<ROW_BF16>(g, (int*)workspace, st);
-  else if (dtype == LCQ_F16) launch_codes<ROW_F16>(g, (int*)workspace, st);
-  else launch_codes<ROW_F32>(g, (int*)workspace, st);
+  if (dtype == LCQ_BF16) launch_codes<ROW_BF16>(g, streams, (int*)workspace, st);
+  else if (dtype == LCQ_F16) launch_codes<ROW_F16>(g, streams, (int*)workspace, st);
+  else launch_codes<ROW_F32>(g, streams, (int*)workspace, st);
   LCQ_CHECK_LAUNCH();
   return LCQ_OK;
 }

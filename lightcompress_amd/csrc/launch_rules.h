@@ -39,7 +39,7 @@ inline bool gptq_by_panels(bool is_static, bool has_gidx, bool rounded, int grou
   return is_static || divides || codes * group < 65536.0f || codes * R <= 32768.0f || R > 4096;
 }
 
-// Int8 product of more than INT8_STREAMED tokens (int8_matmul.hip): which tile, and into how many parts K is cut.  A tile takes
+// Int8 product in tiles (int8_matmul.hip): which tile, and into how many parts K is cut.  A tile takes
 //   start + slabs (busy + crowd share) us     slabs of 128 codes of K, share of the chip's 256 CUs at work
 // and the tiles of a workgroup slot follow one another; parts leave their sums (written and read once, 4 bytes per us and MB / 4) for
 // another kernel (3 us).  Constants fitted to one round at K = 4096 and 14336 (us): 256 x 256 alone 42 and 125, on all CUs 60;
@@ -47,14 +47,12 @@ inline bool gptq_by_panels(bool is_static, bool has_gidx, bool rounded, int grou
 //   N = 4096    1024 tokens 44.3 / 37.6 / 19.8    2048 tokens  45.5 / 41.6 / 38.3
 //   N = 6144    1024 tokens 44.7 / 37.7 / 34.0    2048 tokens  52.6 / 52.9 / 56.8
 //   N = 14336    512 tokens 45.1 / 39.5 / 35.6    1024 tokens  57.8 / 85.0 / 68.5    2048 tokens 112 / 134 / 129
-constexpr int INT8_STREAMED = 32;
-struct Int8Cut { int tile, parts; };                // tile 0: 256 x 256, 1: 256 x 192, 2: 128 x 128
+struct Int8Cut { int tile, parts; double us; };     // tile 0: 256 x 256, 1: 256 x 192, 2: 128 x 128
 inline Int8Cut int8_cut(long long M, long long N, long long K) {
   struct Shape { int tm, tn; double start, busy, crowd; };
   const Shape shapes[3] = {{256, 256, 9.0, 1.03, 0.56}, {256, 192, 8.0, 0.81, 0.60}, {128, 128, 5.0, 0.333, 0.14}};
   const long long slabs = (K + 127) / 128;
-  Int8Cut best = {0, 1};
-  double least = 0.0;
+  Int8Cut best = {0, 1, 0.0};
   for (int i = 0; i < 3; ++i) {
     const Shape& s = shapes[i];
     const long long tiles = (M + s.tm - 1) / s.tm * ((N + s.tn - 1) / s.tn);
@@ -65,10 +63,28 @@ inline Int8Cut int8_cut(long long M, long long N, long long K) {
       double t = rounds * (s.start + each * (s.busy + s.crowd));
       if (rest) t += s.start + each * (s.busy + s.crowd * (double)rest / 256.0);
       if (parts > 1) t += 3.0 + 8.0 * parts * (double)M * (double)N / 4e6;
-      if (least == 0.0 || t < least) { least = t; best = {i, parts}; }
+      if (best.us == 0.0 || t < best.us) best = {i, parts, t};
     }
   }
   return best;
+}
+
+// Whether the weight is streamed past the tokens instead: always for up to 16 of them, up to 64 where that is the faster.  A stream takes
+//   3.2 + M K (0.15 + 0.85 blocks) / 25000 us     blocks of 16 channels on the busiest of 256 CUs
+// and 1.6 (beyond 32 tokens 2.4) times the second term where rows do not start on 16 bytes, which tiles need copied first.  Measured as
+// stream / tiles, us:
+//   512 x 512     64 tokens  5.6 / 6.1     2048 x 2048   33 tokens  6.5 / 10.2    64 tokens  8.9 / 10.2
+//   4096 x 4096   33 tokens 10.0 / 13.4    64 tokens 15.2 / 14.1    14336 x 4096  32 tokens 22.3 / 18.2    4096 x 14336  32 tokens 24.0 / 19.9
+//   4096 x 4097   48 tokens 21.5 / 23.4    64 tokens 26.8 / 23.5    14336 x 4097  32 tokens 35.9 / 42     33 tokens 57 / 42
+constexpr int INT8_STREAMED = 64;
+inline bool int8_streams(long long M, long long N, long long K) {
+  if (M > INT8_STREAMED) return false;
+  if (M <= 16) return true;
+  const bool odd = K % 16 != 0;
+  const double blocks = (double)((N + 4095) / 4096);
+  const double stream = 3.2 + (odd ? M <= 32 ? 1.6 : 2.4 : 1.0) * (double)M * (double)K * (0.15 + 0.85 * blocks) / 25000.0;
+  const double tiles = int8_cut(M, N, (K + 15) / 16 * 16).us + (odd ? 3.0 + 2.0 * (double)(M + N) * (double)K / 4.9e6 : 0.0);
+  return stream < tiles;
 }
 
 }  // namespace lcq

@@ -12,19 +12,26 @@ from lightcompress_amd.build import CSRC
 WRAPPERS = '''
 #include "launch_rules.h"
 extern "C" int cut(long long M, long long N, long long K) { const lcq::Int8Cut c = lcq::int8_cut(M, N, K); return c.tile * 256 + c.parts; }
+extern "C" int streams(long long M, long long N, long long K) { return lcq::int8_streams(M, N, K); }
 '''
 
 
 @pytest.fixture(scope='module')
-def cut(tmp_path_factory):
+def rules(tmp_path_factory):
     if not shutil.which('g++'):
         pytest.skip('no host compiler')
     d = tmp_path_factory.mktemp('cut')
     (d / 'w.cpp').write_text(WRAPPERS)
     subprocess.run(['g++', '-std=c++17', '-shared', '-fPIC', f'-I{CSRC}', str(d / 'w.cpp'), '-o', str(d / 'w.so')], check=True)
-    f = ctypes.CDLL(str(d / 'w.so')).cut
-    f.argtypes = [ctypes.c_longlong] * 3
-    return lambda *s: divmod(f(*s), 256)
+    so = ctypes.CDLL(str(d / 'w.so'))
+    for f in (so.cut, so.streams):
+        f.argtypes = [ctypes.c_longlong] * 3
+    return so
+
+
+@pytest.fixture(scope='module')
+def cut(rules):
+    return lambda *s: divmod(rules.cut(*s), 256)
 
 
 def test_parts_are_whole_fit_the_chip_and_the_workspace(cut):
@@ -34,14 +41,25 @@ def test_parts_are_whole_fit_the_chip_and_the_workspace(cut):
         assert tile in (0, 1, 2) and 1 <= parts <= 16
         if parts > 1:                              # parts of 128 x 128 tiles only, at least two stages each, one per CU, sums in the workspace
             assert tile == 2 and parts * tiles <= 256 and -(-K // 128) // parts >= 2
-            assert L.lib().lcq_int8_matmul_workspace_bytes(M, N, K) >= 4 * M * N * parts
-        else:
-            assert L.lib().lcq_int8_matmul_workspace_bytes(M, N, K) == 0
-    for M, N, K in ((1, 4096, 4096), (32, 4096, 4096)):
-        assert L.lib().lcq_int8_matmul_workspace_bytes(M, N, K) == 0           # (streamed)
-        assert L.lib().lcq_int8_matmul_workspace_bytes(M, N, K + 1) == 0       # (whatever the width)
-    for M, N, K in ((33, 4096, 4097), (1, 4096, 1), (32, 100, 15)):            # padded rows: many tokens, fewer than 16 codes
-        assert L.lib().lcq_int8_matmul_workspace_bytes(M, N, K) >= (M + N) * -(-K // 16) * 16
+
+
+def test_the_workspace_follows_the_rules(cut, rules):
+    need = L.lib().lcq_int8_matmul_workspace_bytes
+    for M, N, K in itertools.product((1, 16, 17, 33, 64, 65, 300, 5000), (1, 100, 4096, 14336), (1, 15, 16, 17, 1024, 4097, 14336, 65536)):
+        streams = rules.streams(M, N, K)
+        parts = 1 if streams else cut(M, N, -(-K // 16) * 16)[1]
+        padded = K % 16 and (not streams or K < 16)
+        assert streams == 1 if M <= 16 else True
+        assert not streams or M <= 64
+        assert (need(M, N, K) == 0) == (parts == 1 and not padded)
+        assert need(M, N, K) >= (4 * M * N * parts if parts > 1 else 0) + ((M + N) * -(-K // 16) * 16 if padded else 0)
+
+
+def test_measured_streams(rules):
+    """The sizes at which streams and tiles were timed against each other."""
+    for (M, N, K), streams in {(64, 512, 512): 1, (33, 2048, 2048): 1, (64, 2048, 2048): 1, (33, 4096, 4096): 1, (64, 4096, 4096): 0,
+                               (32, 14336, 4096): 0, (32, 4096, 14336): 0, (16, 14336, 4096): 1, (65, 512, 512): 0}.items():
+        assert rules.streams(M, N, K) == streams, (M, N, K)
 
 
 def test_measured_choices(cut):

@@ -81,7 +81,7 @@ def test_the_c_entries_refuse_before_a_launch():
     lin = lambda x=P, xd=0, asym=0, sc=None, w=P, ld=64, M=8, K=64, ws=None: lib.lcq_int8_linear(  # noqa: E731
         x, xd, ld, asym, sc, w, P, 0, 0, None, 0, M, 8, K, P, 0, ws, None)
     assert lin(x=None) == lin(w=None) == lin(ld=-1) == lin(asym=1, sc=P) == lin(M=0) == -1 and lin(xd=5) == -3 and lin(K=65537) == -6
-    assert lin(w=P + 8) == -2 and lin() == -5 and lin(ws=P + 8) == -2 and mm(w=P + 1) == mm(a=P + 4) == -2 and mm(M=33, K=63) == mm(K=15) == -5
+    assert lin(w=P + 8) == -2 and lin() == -5 and lin(ws=P + 8) == -2 and mm(w=P + 1) == mm(a=P + 4) == -2 and mm(M=65, K=63) == mm(K=15) == -5
     assert lib.lcq_int8_linear_workspace_bytes(1, 8, 64) == 0 < lib.lcq_int8_linear_workspace_bytes(8, 8, 64)
     norm = lambda x=P, d=0, T=2, K=64, pw=None, pb=None, f=0, h=P, o=P, c=None, s=None, z=None: lib.lcq_residual_norm(  # noqa: E731
         x, d, T, K, 64, None, 0, None, 0, pw, pb, None, None, 1.0, 1e-6, 0.0, f, h, o, c, s, z, None)

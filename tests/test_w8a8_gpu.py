@@ -158,10 +158,11 @@ def test_product_in_every_tile(dev, M, N, K, asym, dtype):
     check_product(int8_matmul(QuantizedTokens(q, s, z), w, ws, b, out_dtype=dtype), q, s, z, w, ws, b, dtype)
 
 
-# at most 32 tokens: one or two blocks of 16 of them by one or two of 16 channels, rows that start on 16 bytes and such that do not
+# few tokens: one to four blocks of 16 of them by one or two of 16 channels, rows that start on 16 bytes and such that do not
 FEW = [(16, 4096, 1040), (2, 4100, 528), (16, 8192, 4112), (7, 8200, 272), (1, 14339, 528), (17, 4096, 528), (24, 4097, 1040), (32, 8192, 4112),
        (31, 8200, 272), (32, 14339, 16), (9, 14336, 1040), (3, 28673, 48),
-       (16, 4096, 1041), (1, 300, 17), (5, 4100, 4111), (2, 70, 15), (9, 14339, 300), (32, 300, 31), (20, 4096, 1023), (31, 8193, 2047), (25, 6200, 513)]
+       (16, 4096, 1041), (1, 300, 17), (5, 4100, 4111), (2, 70, 15), (9, 14339, 300), (32, 300, 31), (20, 4096, 1023), (31, 8193, 2047), (25, 6200, 513),
+       (33, 1000, 1024), (48, 4096, 2064), (64, 600, 512), (50, 2048, 2048), (40, 300, 1041), (64, 1001, 2047), (64, 100, 15), (49, 4095, 300)]
 
 
 @pytest.mark.parametrize('asym,dtype', [(False, BF), (True, F32), (True, HF)])
