@@ -579,23 +579,26 @@ __global__ __launch_bounds__(WAVES * 64) void stream_kernel(MatmulArgs g, TokenA
 }
 
 // Rows of K codes to rows of Kp, the next multiple of 16, with zeros behind them: operands whose rows do not start on 16 bytes.  The
-// rows of a, then those of w; `out` has them one behind the other.
+// rows of a, then those of w; `out` has them one behind the other.  A wave takes a row at a time, 4096 codes with all loads on their way at
+// once; the last 16 codes are read from K - 16 and moved.
 __global__ __launch_bounds__(256) void pad_kernel(const int8_t* __restrict__ a, int64_t rows_a, const int8_t* __restrict__ w, int64_t rows, int K, int Kp,
                                                   int8_t* __restrict__ out) {
-  // a wave takes a row (grid-stride): no division by the row's length
+  const int lane = threadIdx.x & 63;
   for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)gridDim.x * 4) {
     const int8_t* const x = r < rows_a ? a + r * K : w + (r - rows_a) * K;
-    for (int k = (threadIdx.x & 63) * 16; k < Kp; k += 1024) {
-      union { u32x4 v; int8_t b[16]; } u;
-      if (k + 16 <= K) {
-        __builtin_memcpy(&u, x + k, 16);
-      } else {
-        u.v = u32x4{0, 0, 0, 0};
-        #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (k + e < K) u.b[e] = x[k + e];
+    if (K < 16) {
+      if (lane < 16) out[r * 16 + lane] = lane < K ? x[lane] : (int8_t)0;
+      continue;
+    }
+    for (int k0 = lane * 16; k0 < Kp; k0 += 4096) {
+      i32x4 v[4];
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) __builtin_memcpy(&v[i], x + (k0 + i * 1024 < K - 16 ? k0 + i * 1024 : K - 16), 16);
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = k0 + i * 1024;
+        if (k < Kp) *(i32x4*)(out + r * Kp + k) = k > K - 16 ? later(v[i], k - (K - 16)) : v[i];
       }
-      *(u32x4*)(out + r * Kp + k) = u.v;
     }
   }
 }
@@ -686,7 +689,7 @@ bool known(int dtype) { return dtype == LCQ_F32 || dtype == LCQ_BF16 || dtype ==
 int check(const int8_t* w, const void* ws, int ws_dtype, const void* bias, int bias_dtype, int64_t M, int64_t N, int64_t K, const void* y, int dtype) {
   if (!w || !ws || !y || M <= 0 || N <= 0 || K <= 0) return LCQ_EINVAL;
   if (!known(dtype) || !known(ws_dtype) || (bias && !known(bias_dtype))) return LCQ_EDTYPE;
-  if (K > 65536 || (M + 127) / 128 * ((N + 127) / 128) > 0x7ffffff0) return LCQ_ESIZE;
+  if (K > 65536 || M > 1 << 28 || N > 1 << 28 || (M + 127) / 128 * ((N + 127) / 128) >= 1 << 24) return LCQ_ESIZE;   // (a launch has fewer than 2^32 lanes)
   if (K % 16 == 0 && (uintptr_t)w % 16) return LCQ_EALIGN;
   return LCQ_OK;
 }
@@ -727,7 +730,7 @@ int lcq_int8_matmul(const int8_t* a, const float* as, int a_scalar, const int32_
     const int Kp = (int)padded(K);
     int8_t* const pa = (int8_t*)workspace + (parts > 1 ? on256(4 * M * N * parts) : 0);
     const int64_t blocks = (M + N + 3) / 4;
-    pad_kernel<<<dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st>>>(a, M, w, M + N, (int)K, Kp, pa);
+    pad_kernel<<<dim3((unsigned)(blocks < 1 << 16 ? blocks : 1 << 16)), dim3(256), 0, st>>>(a, M, w, M + N, (int)K, Kp, pa);
     g.a = pa; g.w = pa + M * Kp; g.lda = g.ldw = g.K = Kp;
   }
   if (dtype == LCQ_BF16) launch_codes<ROW_BF16>(g, streams, (int*)workspace, st);

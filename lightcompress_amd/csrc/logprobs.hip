@@ -27,6 +27,7 @@ struct LogprobArgs {
   int64_t* top_tokens;
   int64_t V, ldx, m, ignore;
   int k;
+  int64_t first;                                    // row of a launch
 };
 
 // A whole number that orders logits by value and, among equal ones, by the lowest index; a NaN is above everything, -0 equals +0.
@@ -170,7 +171,7 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(LogprobArgs a) {
   __shared__ uint32_t reach;
   __shared__ int count;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row = blockIdx.x;
+  const int64_t row = a.first + blockIdx.x;
   const char* const x = (const char*)a.x + row * a.ldx * (16 / N);
   const int V = (int)a.V, pieces = (V + N - 1) / N;
   const int last = V / N;                           // (all pieces of the row but its last hold N logits)
@@ -350,12 +351,16 @@ int lcq_token_logprobs(const void* logits, int dtype, int64_t T, int64_t V, int6
   if (dtype != LCQ_F32 && dtype != LCQ_BF16 && dtype != LCQ_F16) return LCQ_EDTYPE;
   if (T > 0x7fffffff || V > (1 << 28)) return LCQ_ESIZE;
   if ((uintptr_t)logits % (dtype == LCQ_F32 ? 4 : 2)) return LCQ_EALIGN;
-  const LogprobArgs a = {logits, tokens, logprobs, entropy, top_logprobs, top_tokens, V, ldx, m, ignore, k};
+  const LogprobArgs a = {logits, tokens, logprobs, entropy, top_logprobs, top_tokens, V, ldx, m, ignore, k, 0};
   const auto launch = [&](auto bf, auto threads) {
     constexpr int BF = decltype(bf)::value, THREADS = decltype(threads)::value;
-    const dim3 grid((unsigned)T), block(THREADS);
-    if (k) logprobs_kernel<BF, true, THREADS><<<grid, block, 0, (hipStream_t)stream>>>(a);
-    else logprobs_kernel<BF, false, THREADS><<<grid, block, 0, (hipStream_t)stream>>>(a);
+    constexpr int64_t rows = 1 << 21;               // (a launch has fewer than 2^32 lanes)
+    LogprobArgs part = a;
+    for (; part.first < T; part.first += rows) {
+      const dim3 grid((unsigned)(T - part.first < rows ? T - part.first : rows)), block(THREADS);
+      if (k) logprobs_kernel<BF, true, THREADS><<<grid, block, 0, (hipStream_t)stream>>>(part);
+      else logprobs_kernel<BF, false, THREADS><<<grid, block, 0, (hipStream_t)stream>>>(part);
+    }
   };
   const auto run = [&](auto bf) {
     if (T <= 256) launch(bf, std::integral_constant<int, 1024>{});

@@ -24,7 +24,7 @@ struct NormArgs {
   int8_t* codes;
   float* scales;
   int32_t* zeros;
-  int64_t T, ldx, ldr, ldg;
+  int64_t T, ldx, ldr, ldg, first;                  // (first: the first row of a launch)
   int K, flags;
   float scale, eps, offset;
 };
@@ -102,7 +102,7 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void residual_norm_kernel(
   __shared__ float sm[TEAM / 64];
   const Row<TEAM> row_{sm};
   const int t = threadIdx.x % TEAM;
-  const int64_t r = TEAM == 64 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x;
+  const int64_t r = a.first + (TEAM == 64 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x);
   if (r >= a.T) return;                             // (whole waves, and no barriers where TEAM is a wave)
   const int K = a.K, flags = a.flags;
   const float rK = 1.0f / (float)K;
@@ -218,11 +218,17 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void residual_norm_kernel(
   if (t == 0 && a.zeros) a.zeros[r] = q.z;
 }
 
+constexpr int64_t ROWS_OF_A_LAUNCH = 1 << 21;       // (a launch has fewer than 2^32 lanes)
+
 // E elements per lane
 template <int BF, int TEAM, int E>
 void launch(const NormArgs& a, hipStream_t st) {
   constexpr int rows = TEAM == 64 ? 4 : 1;
-  residual_norm_kernel<BF, TEAM, E / Vec<BF>::N><<<dim3((unsigned)((a.T + rows - 1) / rows)), dim3(TEAM == 64 ? 256 : TEAM), 0, st>>>(a);
+  NormArgs part = a;
+  for (part.first = 0; part.first < a.T; part.first += ROWS_OF_A_LAUNCH) {
+    const int64_t left = a.T - part.first, n = left < ROWS_OF_A_LAUNCH ? left : ROWS_OF_A_LAUNCH;
+    residual_norm_kernel<BF, TEAM, E / Vec<BF>::N><<<dim3((unsigned)((n + rows - 1) / rows)), dim3(TEAM == 64 ? 256 : TEAM), 0, st>>>(part);
+  }
 }
 template <int BF>
 void launch_rows(const NormArgs& a, hipStream_t st) {

@@ -172,6 +172,15 @@ def test_behind_two_to_the_31(dev):
     assert bool((got.top_tokens[:-3] == torch.arange(3, device=dev)).all())
 
 
+def test_more_rows_than_a_launch(dev):
+    T, V = 2 ** 21 + 300, 40
+    x = torch.randn(T, V, device=dev)
+    t = torch.randint(0, V, (T,), device=dev)
+    rows = torch.cat([torch.arange(300), 2 ** 21 + torch.arange(-200, 300)]).to(dev)
+    got = token_logprobs(x, t, 3)
+    check(x[rows], t[rows], 3, got=type(got)(*(v[rows] for v in got)))
+
+
 def test_captured_and_again(dev):
     """One row (several parts and a join) and many, captured; the same bits on every replay and on every call."""
     xs = [(torch.randn(T, V, generator=gen(T)) * 3).to(BF).to(dev) for T, V in ((1, 50001), (3, 128256), (600, 4000))]

@@ -390,6 +390,23 @@ def test_norm_behind_two_to_the_31(dev):
 
 
 # -- the container, and all of it together ------------------------------------------------------------------------------
+def test_more_rows_than_a_launch(dev):
+    """2^21 rows and more: those around the seam and the last ones."""
+    T, K = 2 ** 22 + 70, 16
+    x, r = torch.randn(T, K, device=dev), torch.randn(T, K, device=dev)
+    rows = torch.cat([torch.arange(300), 2 ** 21 + torch.arange(-200, 200), T - 1 - torch.arange(200)]).to(dev)
+    got, want = quantize_tokens(x, False), quantize_tokens(x[rows], False)
+    assert torch.equal(got.codes[rows], want.codes) and torch.equal(got.scales[rows], want.scales) and torch.equal(got.zeros[rows], want.zeros)
+    codes, s, z = codes_of(x[rows].cpu(), False)
+    assert torch.equal(want.codes.cpu(), codes)
+    got = residual_norm(x, r)
+    part = residual_norm(x[rows], r[rows])
+    assert_bit_equal(got.out[rows], part.out, 'out')
+    assert_bit_equal(got.residual[rows], part.residual, 'residual')
+    q, s, z, w, ws, b = product_inputs(2 ** 21 + 300, 3, 17, True, True, dev=dev)
+    check_product(int8_matmul(QuantizedTokens(q, s, z), w, ws, b, out_dtype=F32), q, s, z, w, ws, b, F32)
+
+
 def linear(N, K, dtype, seed, bias=True):
     m = torch.nn.Linear(K, N, bias=bias, dtype=dtype)
     m.weight.data = (torch.randn(N, K, generator=gen(seed)) * 0.02).to(dtype)
