@@ -54,7 +54,7 @@ def token_logprobs(logits, tokens=None, top=0, ignore_index=-100):
 
     def run(x, at):
         """The logits x, whose rows are the rows from `at` on of all of them."""
-        if x.dim() > 2 and x.stride(-1) == 1 and not x.is_contiguous():      # logits[:, :-1]: a call per sequence, and no copy
+        if apart and x.dim() > 2:                   # logits[:, :-1]: a call per sequence, and no copy
             rows = x[0].numel() // V
             for i in range(x.shape[0]):
                 run(x[i], at + i * rows)
@@ -67,5 +67,9 @@ def token_logprobs(logits, tokens=None, top=0, ignore_index=-100):
                                                top_tokens.data_ptr() + 8 * top * at if top else None, L.stream()), 'lcq_token_logprobs')
 
     if logits.numel():
+        apart = logits.dim() > 2 and logits.stride(-1) == 1 and not logits.is_contiguous()
+        if apart:                                   # many short sequences (a transposed batch): one copy is faster than their calls
+            each = V * lead[-1]
+            apart = logits.numel() // each <= 64 or each * logits.element_size() >= 1 << 25
         run(logits, 0)
     return TokenLogprobs(logprobs, entropy, top_logprobs, top_tokens)

@@ -201,6 +201,14 @@ def _affine(name, t, K, x, flag):
     return flag
 
 
+def _meets(t, out):
+    """Does t lie where the contiguous `out` is written, other than element on element?"""
+    if not t.numel() or (t.data_ptr() == out.data_ptr() and t.dtype == out.dtype and t.shape == out.shape and t.is_contiguous()):
+        return False
+    span = (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    return t.data_ptr() < out.data_ptr() + out.numel() * out.element_size() and out.data_ptr() < t.data_ptr() + span
+
+
 def residual_norm(x, residual=None, weight=None, bias=None, *, gate=None, post_weight=None, post_bias=None, scale=1.0,
                   eps=1e-6, kind='rms', weight_offset=0.0, quantize=None, out_dtype=None, inplace=False):
     """The end of one block and the start of the next, for the block's output x [..., K], in one pass:
@@ -212,7 +220,7 @@ def residual_norm(x, residual=None, weight=None, bias=None, *, gate=None, post_w
     kind 'rms': norm(v) = v / sqrt(mean v^2 + eps) * (w + weight_offset) + b;  'layer': the same of v - mean v.
     residual: like x, in x's type or fp32 (the stream keeps it); None: 0.  gate: like x, or [K]; None: 1.  A missing
     weight is 1 without an offset.  quantize 'symmetric' / 'asymmetric': out is quantize_tokens of the unrounded norm.
-    out_dtype: x's type (default) or fp32.  inplace: h is written over residual.  -> ResidualNorm(out, residual = h)"""
+    out_dtype: x's type (default) or fp32.  inplace: h is written over residual, which may be x itself.  -> ResidualNorm(out, residual = h)"""
     K = _cols(x)
     code = _code(x.dtype)
     if kind not in ('rms', 'layer') or quantize not in (None, 'symmetric', 'asymmetric'):
@@ -241,6 +249,10 @@ def residual_norm(x, residual=None, weight=None, bias=None, *, gate=None, post_w
         raise ValueError('inplace needs a contiguous residual')
     if inplace and residual.requires_grad and torch.is_grad_enabled():
         raise ValueError('inplace would change a residual that autograd keeps')
+    if inplace:
+        for t in (x, weight, bias, gate, post_weight, post_bias):
+            if t is not None and _meets(t, residual):
+                raise ValueError('inplace would write over a part of another operand that is still read')
     if gate is not None:
         if gate.dtype != x.dtype:
             raise L.LcqError(f'gate is {gate.dtype}, x is {x.dtype}')

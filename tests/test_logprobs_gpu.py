@@ -143,6 +143,9 @@ def test_sequences_without_their_last_logits(dev):
     for v, ids in views:
         a, b = token_logprobs(v, ids, top=3), token_logprobs(v.clone(memory_format=torch.contiguous_format), ids.clone(), top=3)
         assert all(torch.equal(p, q) and p.shape == q.shape for p, q in zip(a, b))
+    x2 = torch.randn(5, 100, 70, generator=gen(14)).to(dev).transpose(0, 1)     # more sequences than are worth a call each
+    a, b = token_logprobs(x2, top=2), token_logprobs(x2.contiguous(), top=2)
+    assert all(torch.equal(p, q) and p.shape == q.shape for p, q in zip(a[1:], b[1:]))
     a = token_logprobs(x[:, :-1], torch.stack([t[:, 1:], t[:, :-1]], -1))
     want = torch.log_softmax(x[:, :-1].double(), -1).gather(-1, torch.stack([t[:, 1:], t[:, :-1]], -1))
     assert float((a.logprobs - want).abs().max()) < 1e-5

@@ -13,6 +13,9 @@ BUF = ctypes.create_string_buffer(256)
 P = ctypes.addressof(BUF) & ~15                  # stands for a device pointer: every call below returns before it is used
 
 
+ROWS = torch.zeros(3, 64)
+
+
 def tokens(M=2, K=64):
     return QuantizedTokens(torch.zeros(M, K, dtype=torch.int8), torch.ones(M, 1))
 
@@ -53,6 +56,10 @@ def test_cpu_tensors_are_refused():
     (lambda: residual_norm(torch.zeros(2, 64), quantize='int4'), ValueError),
     (lambda: residual_norm(torch.zeros(2, 64), out_dtype=torch.bfloat16), L.LcqError),
     (lambda: residual_norm(torch.zeros(2, 64), inplace=True), ValueError),
+    (lambda: residual_norm(ROWS[1:], ROWS[:2], inplace=True), ValueError),
+    (lambda: residual_norm(ROWS[:2].clone(), ROWS[:2], ROWS[1], inplace=True), ValueError),
+    (lambda: residual_norm(ROWS.view(torch.bfloat16)[:1, :64], ROWS[:1], inplace=True), ValueError),
+    (lambda: residual_norm(ROWS[:2].clone(), ROWS[:2], gate=ROWS[1:], inplace=True), ValueError),
     (lambda: residual_norm(torch.zeros(2, 64), torch.zeros(64, 2).t(), inplace=True), ValueError),
     (lambda: residual_norm(torch.zeros(2, 64), torch.zeros(2, 64, requires_grad=True), inplace=True), ValueError),
     (lambda: token_logprobs(torch.zeros(2, 0)), ValueError),

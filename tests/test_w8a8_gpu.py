@@ -221,7 +221,7 @@ def test_linear_is_codes_and_product(dev, M, K, dtype):
         assert int8_linear(x, w, ws).dtype == dtype
 
 
-@pytest.mark.parametrize('N,K', [(8200, 512), (8193, 4096), (9000, 16400), (4096, 8208), (1, 8192), (17, 16)])
+@pytest.mark.parametrize('N,K', [(8200, 512), (8193, 4096), (9000, 16400), (4096, 8208), (1, 8192), (17, 16), (9000, 8192), (300, 32768)])
 @pytest.mark.parametrize('symmetric', [True, False])
 def test_one_token(dev, N, K, symmetric):
     g = torch.Generator(device=dev)
