@@ -67,7 +67,7 @@ def _workspace(x, entry, *sizes):
 def _like(x, dtype):
     """A new contiguous tensor of x's shape.  (empty_like keeps strides, so only where they are those; it costs a third less.)"""
     if x.is_contiguous():
-        return torch.empty_like(x, dtype=dtype)
+        return torch.empty_like(x) if dtype is x.dtype else torch.empty_like(x, dtype=dtype)
     return torch.empty(x.shape, dtype=dtype, device=x.device)
 
 
@@ -81,17 +81,17 @@ def _rows(t, K):
     return t, t.numel() // K, K
 
 
-def _cols(x):
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError(f'tokens need a last dimension of at least one column, got shape {tuple(x.shape)}')
-    if x.shape[-1] > MOST_COLS:
-        raise ValueError(f'at most {MOST_COLS} columns, got {x.shape[-1]}')
-    return x.shape[-1]
+def _cols(shape):
+    """-> the last of a shape's sizes, the columns of the tokens."""
+    if not shape or shape[-1] == 0:
+        raise ValueError(f'tokens need a last dimension of at least one column, got shape {tuple(shape)}')
+    K = shape[-1]
+    if K > MOST_COLS:
+        raise ValueError(f'at most {MOST_COLS} columns, got {K}')
+    return K
 
 
 def _given(scale, symmetric):
-    if scale is None:
-        return None
     if not symmetric:
         raise ValueError('a given scale is a symmetric one')
     if scale.numel() != 1:
@@ -102,20 +102,22 @@ def _given(scale, symmetric):
 def quantize_tokens(x, symmetric=True, scale=None):
     """Int8 codes of the tokens x [..., K] (fp32, bf16, fp16), one fp32 scale per token (and, not symmetric, one zero
     point): QuantizedTokens.  `scale`: one given fp32 scale for all tokens (static activations, symmetric)."""
-    K = _cols(x)
+    shape = x.shape
+    K = _cols(shape)
     code = _code(x.dtype)
-    given = _given(scale, symmetric)
+    given = None if scale is None else _given(scale, symmetric)
     if not _here(x, given):
         with torch.cuda.device(x.device):
             return quantize_tokens(x, symmetric, scale)
     rows, T, ld = _rows(x, K)
-    one = (*x.shape[:-1], 1)
+    one = shape[:-1] + (1,)
     codes = _like(x, torch.int8)
     scales = torch.empty(one, dtype=torch.float32, device=x.device) if given is None else given
     zeros = None if symmetric else torch.empty(one, dtype=torch.int32, device=x.device)
     if T:
-        L.check(L.lib().lcq_quant_tokens(rows.data_ptr(), code, T, K, ld, not symmetric, L.ptr(given), codes.data_ptr(),
-                                         scales.data_ptr(), L.ptr(zeros), L.stream()), 'lcq_quant_tokens')
+        L.check(L.lib().lcq_quant_tokens(rows.data_ptr(), code, T, K, ld, not symmetric, None if given is None else given.data_ptr(),
+                                         codes.data_ptr(), scales.data_ptr(), None if symmetric else zeros.data_ptr(), L.stream()),
+                'lcq_quant_tokens')
     return QuantizedTokens(codes, scales, zeros)
 
 
@@ -126,12 +128,13 @@ def _on16(t):
 def _check_weight(weight, weight_scales, bias, K):
     if weight.dtype != torch.int8:
         raise L.LcqError(f'an int8 weight is needed, got {weight.dtype}')
-    if weight.dim() != 2 or weight.shape[1] != K:
-        raise ValueError(f'weight {tuple(weight.shape)} does not take tokens of {K} columns')
-    N = weight.shape[0]
+    shape = weight.shape
+    if len(shape) != 2 or shape[1] != K:
+        raise ValueError(f'weight {tuple(shape)} does not take tokens of {K} columns')
+    N = shape[0]
     if weight_scales.numel() not in (1, N):
         raise ValueError(f'{N} weight scales (or one) are needed, got {tuple(weight_scales.shape)}')
-    if bias is not None and tuple(bias.shape) != (N,):
+    if bias is not None and bias.shape != (N,):
         raise ValueError(f'the bias of {N} channels has shape {tuple(bias.shape)}')
     return N
 
@@ -141,7 +144,8 @@ def int8_matmul(tokens, weight, weight_scales, bias=None, out_dtype=torch.bfloat
     one for all; fp32, bf16, fp16), plus a bias [N]: [..., N] of `out_dtype`.  The sums are exact integers, scales and bias
     are applied in fp32, the result is rounded once."""
     codes, scales, zeros = tokens
-    K = _cols(codes)
+    shape = codes.shape
+    K = _cols(shape)
     if codes.dtype != torch.int8 or scales.dtype != torch.float32 or (zeros is not None and zeros.dtype != torch.int32):
         raise L.LcqError('tokens are int8 codes with fp32 scales and int32 zero points')
     N = _check_weight(weight, weight_scales, bias, K)
@@ -155,7 +159,7 @@ def int8_matmul(tokens, weight, weight_scales, bias=None, out_dtype=torch.bfloat
             return int8_matmul(tokens, weight, weight_scales, bias, out_dtype)
     if K % 16 == 0:                           # (rows of other widths may start anywhere)
         codes, weight = _on16(codes), _on16(weight)
-    y = torch.empty((*codes.shape[:-1], N), dtype=out_dtype, device=codes.device)
+    y = torch.empty(shape[:-1] + (N,), dtype=out_dtype, device=codes.device)
     if M and N:
         ws = _workspace(codes, 'lcq_int8_matmul_workspace_bytes', M, N, K)
         L.check(L.lib().lcq_int8_matmul(L.ptr(codes), L.ptr(scales), scales.numel() == 1, L.ptr(zeros), L.ptr(weight),
@@ -167,12 +171,14 @@ def int8_matmul(tokens, weight, weight_scales, bias=None, out_dtype=torch.bfloat
 
 def int8_linear(x, weight, weight_scales, bias=None, symmetric=True, scale=None, out_dtype=None):
     """A w8a8 Linear on x [..., K]: quantize_tokens(x, symmetric, scale), then int8_matmul to x's type (or `out_dtype`)."""
-    K = _cols(x)
-    x_code = _code(x.dtype)
+    shape = x.shape
+    K = _cols(shape)
+    x_code = code = _code(x.dtype)
     if out_dtype is None:
         out_dtype = x.dtype
-    code = _code(out_dtype)
-    given = _given(scale, symmetric)
+    else:
+        code = _code(out_dtype)
+    given = None if scale is None else _given(scale, symmetric)
     N = _check_weight(weight, weight_scales, bias, K)
     if not _here(x, given, weight, weight_scales, bias):
         with torch.cuda.device(x.device):
@@ -180,7 +186,7 @@ def int8_linear(x, weight, weight_scales, bias=None, symmetric=True, scale=None,
     rows, M, ld = _rows(x, K)
     if K % 16 == 0:                           # (rows of other widths may start anywhere)
         weight = _on16(weight)
-    y = torch.empty((*x.shape[:-1], N), dtype=out_dtype, device=x.device)
+    y = torch.empty(shape[:-1] + (N,), dtype=out_dtype, device=x.device)
     if M and N:
         ws = _workspace(x, 'lcq_int8_linear_workspace_bytes', M, N, K)
         L.check(L.lib().lcq_int8_linear(rows.data_ptr(), x_code, ld, not symmetric, L.ptr(given), L.ptr(weight), L.ptr(weight_scales),
@@ -190,14 +196,14 @@ def int8_linear(x, weight, weight_scales, bias=None, symmetric=True, scale=None,
     return y
 
 
-def _affine(name, t, K, x, flag):
+def _affine(name, t, K, dtype, flag):
     """The flag of a [K] parameter of a norm: of the tokens' type, or fp32."""
-    if t.dim() != 1 or t.shape[0] != K:
+    if t.shape != (K,):
         raise ValueError(f'{name} of {K} columns has shape {tuple(t.shape)}')
-    if t.dtype == x.dtype:
+    if t.dtype is dtype:
         return 0
     if t.dtype != torch.float32:
-        raise L.LcqError(f'{name} is {t.dtype}: the tokens\' {x.dtype} or float32 is needed')
+        raise L.LcqError(f'{name} is {t.dtype}: the tokens\' {dtype} or float32 is needed')
     return flag
 
 
@@ -221,49 +227,50 @@ def residual_norm(x, residual=None, weight=None, bias=None, *, gate=None, post_w
     residual: like x, in x's type or fp32 (the stream keeps it); None: 0.  gate: like x, or [K]; None: 1.  A missing
     weight is 1 without an offset.  quantize 'symmetric' / 'asymmetric': out is quantize_tokens of the unrounded norm.
     out_dtype: x's type (default) or fp32.  inplace: h is written over residual, which may be x itself.  -> ResidualNorm(out, residual = h)"""
-    K = _cols(x)
-    code = _code(x.dtype)
+    shape, dtype = x.shape, x.dtype
+    K = _cols(shape)
+    code = _code(dtype)
     if kind not in ('rms', 'layer') or quantize not in (None, 'symmetric', 'asymmetric'):
         raise ValueError(f'kind {kind!r}, quantize {quantize!r}')
     if post_bias is not None and post_weight is None:
         raise ValueError('post_bias goes with post_weight')
     flags = NORM_LAYER if kind == 'layer' else 0
     if weight is not None:
-        flags |= _affine('weight', weight, K, x, NORM_WEIGHT_F32)
+        flags |= _affine('weight', weight, K, dtype, NORM_WEIGHT_F32)
     if bias is not None:
-        flags |= _affine('bias', bias, K, x, NORM_BIAS_F32)
+        flags |= _affine('bias', bias, K, dtype, NORM_BIAS_F32)
     if post_weight is not None:
-        flags |= _affine('post_weight', post_weight, K, x, NORM_POST_WEIGHT_F32)
+        flags |= _affine('post_weight', post_weight, K, dtype, NORM_POST_WEIGHT_F32)
     if post_bias is not None:
-        flags |= _affine('post_bias', post_bias, K, x, NORM_POST_BIAS_F32)
-    stream_dtype = x.dtype
+        flags |= _affine('post_bias', post_bias, K, dtype, NORM_POST_BIAS_F32)
+    stream_dtype = dtype
     if residual is not None:
-        if residual.shape != x.shape:
-            raise ValueError(f'residual {tuple(residual.shape)} next to x {tuple(x.shape)}')
-        if residual.dtype not in (x.dtype, torch.float32):
-            raise L.LcqError(f'residual is {residual.dtype}: x\'s {x.dtype} or float32 is needed')
-        stream_dtype = residual.dtype
-        if stream_dtype != x.dtype:
+        if residual.shape != shape:
+            raise ValueError(f'residual {tuple(residual.shape)} next to x {tuple(shape)}')
+        if residual.dtype is not dtype:
+            if residual.dtype != torch.float32:
+                raise L.LcqError(f'residual is {residual.dtype}: x\'s {dtype} or float32 is needed')
+            stream_dtype = torch.float32
             flags |= NORM_RESIDUAL_F32
-    if inplace and (residual is None or not residual.is_contiguous()):
-        raise ValueError('inplace needs a contiguous residual')
-    if inplace and residual.requires_grad and torch.is_grad_enabled():
-        raise ValueError('inplace would change a residual that autograd keeps')
     if inplace:
+        if residual is None or not residual.is_contiguous():
+            raise ValueError('inplace needs a contiguous residual')
+        if residual.requires_grad and torch.is_grad_enabled():
+            raise ValueError('inplace would change a residual that autograd keeps')
         for t in (x, weight, bias, gate, post_weight, post_bias):
             if t is not None and _meets(t, residual):
                 raise ValueError('inplace would write over a part of another operand that is still read')
     if gate is not None:
-        if gate.dtype != x.dtype:
-            raise L.LcqError(f'gate is {gate.dtype}, x is {x.dtype}')
-        if tuple(gate.shape) != (K,) and gate.shape != x.shape:
-            raise ValueError(f'gate {tuple(gate.shape)} next to x {tuple(x.shape)}')
-    if out_dtype is None or out_dtype == x.dtype:
-        out_dtype = x.dtype
+        if gate.dtype is not dtype:
+            raise L.LcqError(f'gate is {gate.dtype}, x is {dtype}')
+        if gate.shape != shape and gate.shape != (K,):
+            raise ValueError(f'gate {tuple(gate.shape)} next to x {tuple(shape)}')
+    if out_dtype is None or out_dtype == dtype:
+        out_dtype = dtype
     elif out_dtype == torch.float32:
         flags |= NORM_OUT_F32
     else:
-        raise L.LcqError(f'out_dtype {out_dtype}: x\'s {x.dtype} or float32 is needed')
+        raise L.LcqError(f'out_dtype {out_dtype}: x\'s {dtype} or float32 is needed')
     if not _here(x, residual, weight, bias, gate, post_weight, post_bias):
         with torch.cuda.device(x.device):
             return residual_norm(x, residual, weight, bias, gate=gate, post_weight=post_weight, post_bias=post_bias, scale=scale,
@@ -280,13 +287,14 @@ def residual_norm(x, residual=None, weight=None, bias=None, *, gate=None, post_w
         out = _like(x, out_dtype)
     else:
         codes = _like(x, torch.int8)
-        scales = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=x.device)
+        scales = torch.empty(shape[:-1] + (1,), dtype=torch.float32, device=x.device)
         if quantize == 'asymmetric':
             flags |= NORM_ASYM
-            zeros = torch.empty((*x.shape[:-1], 1), dtype=torch.int32, device=x.device)
+            zeros = torch.empty(shape[:-1] + (1,), dtype=torch.int32, device=x.device)
     if T:
-        at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        L.check(L.lib().lcq_residual_norm(rows.data_ptr(), code, T, K, ldx, at(res), ldr, at(g), ldg, L.ptr(post_weight),
-                                          L.ptr(post_bias), L.ptr(weight), L.ptr(bias), scale, eps, weight_offset, flags,
-                                          h.data_ptr(), at(out), at(codes), at(scales), at(zeros), L.stream()), 'lcq_residual_norm')
+        L.check(L.lib().lcq_residual_norm(
+            rows.data_ptr(), code, T, K, ldx, None if res is None else res.data_ptr(), ldr, None if g is None else g.data_ptr(), ldg,
+            L.ptr(post_weight), L.ptr(post_bias), L.ptr(weight), L.ptr(bias), scale, eps, weight_offset, flags, h.data_ptr(),
+            None if out is None else out.data_ptr(), None if codes is None else codes.data_ptr(),
+            None if scales is None else scales.data_ptr(), None if zeros is None else zeros.data_ptr(), L.stream()), 'lcq_residual_norm')
     return ResidualNorm(out if quantize is None else QuantizedTokens(codes, scales, zeros), h)
