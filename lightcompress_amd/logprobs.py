@@ -28,7 +28,8 @@ def token_logprobs(logits, tokens=None, top=0, ignore_index=-100):
     log_softmax does.  The `top` (at most 64) alternatives come largest first, equal logits by the lowest id, a NaN first."""
     if logits.dim() == 0 or logits.shape[-1] == 0:
         raise ValueError(f'logits need a vocabulary, got shape {tuple(logits.shape)}')
-    V, lead = logits.shape[-1], logits.shape[:-1]
+    shape = logits.shape
+    V, lead = shape[-1], (shape[0],) if len(shape) == 2 else tuple(shape[:-1])
     code = _code(logits.dtype)
     if not 0 <= top <= min(MOST_TOP, V):
         raise ValueError(f'top {top}: between 0 and {min(MOST_TOP, V)}')
@@ -45,12 +46,11 @@ def token_logprobs(logits, tokens=None, top=0, ignore_index=-100):
     if not _here(logits, tokens):
         with torch.cuda.device(logits.device):
             return token_logprobs(logits, tokens, top, ignore_index)
-    dev = logits.device
     ids = None if tokens is None else tokens.contiguous()
-    logprobs = None if tokens is None else torch.empty(tokens.shape, dtype=torch.float32, device=dev)
-    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
-    top_logprobs = torch.empty((*lead, top), dtype=torch.float32, device=dev)
-    top_tokens = torch.empty((*lead, top), dtype=torch.int64, device=dev)
+    logprobs = None if ids is None else torch.empty_like(ids, dtype=torch.float32)
+    entropy = logits.new_empty(lead, dtype=torch.float32)
+    top_logprobs = logits.new_empty((*lead, top), dtype=torch.float32)
+    top_tokens = logits.new_empty((*lead, top), dtype=torch.int64)
 
     def run(x, at):
         """The logits x, whose rows are the rows from `at` on of all of them."""
