@@ -205,6 +205,18 @@ def test_product_off_alignment(dev, M, N, K):
         check_product(got, q, s, z, w, ws, None, F32)
 
 
+@pytest.mark.parametrize('M,N,K', [(1, 80, 513), (5, 4100, 17), (20, 300, 1023), (40, 70, 258), (60, 33, 1041), (90, 300, 515), (3, 5, 9)])
+def test_product_of_odd_rows_off_alignment(dev, M, N, K):
+    """Rows of odd widths in operands that start on any byte, next to other bytes on both sides."""
+    q, s, z, w, ws, b = product_inputs(M, N, K, True, False, dev=dev)
+    for off in (0, 1, 2, 3):
+        qb = torch.full((M * K + 32,), 77, dtype=torch.int8, device=dev)
+        wb = torch.full((N * K + 32,), -99, dtype=torch.int8, device=dev)
+        qb[16 + off:16 + off + M * K], wb[19 - off:19 - off + N * K] = q.view(-1), w.view(-1)
+        got = int8_matmul(QuantizedTokens(qb[16 + off:16 + off + M * K].view(M, K), s, z), wb[19 - off:19 - off + N * K].view(N, K), ws, out_dtype=F32)
+        check_product(got, q, s, z, w, ws, None, F32)
+
+
 @pytest.mark.parametrize('dtype', [BF, HF, F32])
 @pytest.mark.parametrize('M,K', [(1, 1), (1, 16), (1, 4096), (1, 16400), (1, 40960), (1, 40976), (1, 65536), (2, 1040), (3, 4096), (4, 10240), (4, 10256), (4, 1000),
                                  (5, 512), (16, 4096), (33, 1024), (300, 528)])
