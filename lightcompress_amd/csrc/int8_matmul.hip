@@ -329,7 +329,7 @@ __global__ __launch_bounds__(256) void join_kernel(MatmulArgs g, const int* __re
 // codes of K in turn and meet in LDS; four (two) pieces, 16 KiB of weight per wave, are in flight, with the codes of the tokens beside them,
 // which come from the cache.  What bounds it is the ramp of the first loads and then HBM, 3 us + the weight at 5.5 TB/s: 2 tokens take 6.1 us
 // at N = K = 4096, 43 us (5.4 TB/s) at 8192 x 28672; the tokens' codes pass the L2 once per workgroup, which tells from 16 tokens on.
-// A single token may come as values: every workgroup makes its codes itself, in LDS, while its first weights are on their way - cheaper
+// One token or a few may come as values: every workgroup makes their codes itself, in LDS, while its first weights are on their way - cheaper
 // than another kernel in front (6.4 us at N = K = 4096, the quantizer alone 3.4).
 constexpr int PIECE = 256;
 constexpr int64_t MOST_FUSED = 32768;               // codes of a token that is quantized in LDS
@@ -341,11 +341,11 @@ struct TokenArgs {
   int asym;
 };
 
-// A row of x in registers, pieces of eight values per lane (K up to 16384), and its int8 codes to LDS, by the whole workgroup;
-// K % 16 == 0.  The loads are apart from the rest, so that the weight's can be issued behind them.
-template <int XT, int WAVES>
+// A row of x, KEEP pieces of eight values per lane of it in registers, and its int8 codes to LDS, by the whole workgroup or, WAVES = 1, by any
+// wave of it; K % 16 == 0.  The loads are apart from the rest, so that the weight's can be issued behind them.
+template <int XT, int WAVES, int KEEP = 4>
 struct TokenRow {
-  static constexpr int KEEP = 4, RAW = XT == ROW_F32 ? 2 : 1;
+  static constexpr int RAW = XT == ROW_F32 ? 2 : 1;
   u32x4 raw[KEEP][RAW];
   const char* x;
   int K;
@@ -368,7 +368,7 @@ struct TokenRow {
     x = (const char*)t.x + row * t.ldx * (2 * RAW);
     #pragma unroll
     for (int c = 0; c < KEEP; ++c) {
-      const int i = (threadIdx.x + c * WAVES * 64) * 8;
+      const int i = (threadIdx.x % (WAVES * 64) + c * WAVES * 64) * 8;
       if (i < K) load8(i, raw[c]);
     }
   }
@@ -376,7 +376,7 @@ struct TokenRow {
   __device__ __forceinline__ void each(F&& f) const {
     #pragma unroll
     for (int c = 0; c < KEEP; ++c) {
-      const int i = (threadIdx.x + c * WAVES * 64) * 8;
+      const int i = (threadIdx.x % (WAVES * 64) + c * WAVES * 64) * 8;
       float v[8];
       if (i < K) {
         #pragma unroll
@@ -384,7 +384,7 @@ struct TokenRow {
         f(i, v);
       }
     }
-    for (int i = (threadIdx.x + KEEP * WAVES * 64) * 8; i < K; i += WAVES * 64 * 8) {
+    for (int i = (threadIdx.x % (WAVES * 64) + KEEP * WAVES * 64) * 8; i < K; i += WAVES * 64 * 8) {
       u32x4 r[RAW];
       float v[8];
       load8(i, r);
@@ -393,7 +393,7 @@ struct TokenRow {
       f(i, v);
     }
   }
-  // red: 2 WAVES floats
+  // red: 2 WAVES floats (WAVES = 1: none, and the caller waits for the other waves)
   __device__ __forceinline__ void to_codes(const TokenArgs& t, int8_t* out, float* red, float* scale, int* zero) const {
     const int wave = threadIdx.x >> 6;
     float hi = t.asym ? -__builtin_inff() : 0.0f, lo = __builtin_inff();
@@ -406,24 +406,27 @@ struct TokenRow {
     });
     hi = team_reduce<64, true>(hi);
     if (t.asym) lo = team_reduce<64, false>(lo);
-    if ((threadIdx.x & 63) == 0) { red[wave] = hi; red[WAVES + wave] = lo; }
-    __syncthreads();
-    #pragma unroll
-    for (int w = 0; w < WAVES; ++w) { hi = nan_max(hi, red[w]); lo = nan_min(lo, red[WAVES + w]); }
+    if constexpr (WAVES > 1) {
+      if ((threadIdx.x & 63) == 0) { red[wave] = hi; red[WAVES + wave] = lo; }
+      __syncthreads();
+      #pragma unroll
+      for (int w = 0; w < WAVES; ++w) { hi = nan_max(hi, red[w]); lo = nan_min(lo, red[WAVES + w]); }
+    }
     const TokenCodes q = t.scale ? TokenCodes::given(t.scale[0]) : t.asym ? TokenCodes::asymmetric(lo, hi) : TokenCodes::symmetric(hi);
     each([&](int i, const float* e) {
       uint32_t w[2];
       q.codes<8>(e, w);
       *(u32x2*)(out + i) = u32x2{w[0], w[1]};
     });
-    if (threadIdx.x == 0) {
+    if (threadIdx.x % (WAVES * 64) == 0) {
       *scale = q.d.s;
       *zero = q.z;
     }
-    __syncthreads();
+    if constexpr (WAVES > 1) __syncthreads();
   }
 };
-template <int WAVES> struct TokenRow<-1, WAVES> {};
+template <int WAVES, int KEEP> struct TokenRow<-1, WAVES, KEEP> {};
+
 
 // 16 codes that were read `codes` too early: the first ones leave, zeros follow
 __device__ __forceinline__ i32x4 later(i32x4 v, int codes) {
@@ -436,22 +439,24 @@ __device__ __forceinline__ i32x4 later(i32x4 v, int codes) {
   return __builtin_bit_cast(i32x4, h);
 }
 
-// TB blocks of 16 tokens, NB blocks of 16 channels.  XT: the type of one token's values (TB = 1), or -1 for codes.
+// TB blocks of 16 tokens, NB blocks of 16 channels.  XT: the type of the tokens' values (one token, or MANY of up to 16: a wave quantizes a
+// row at a time), or -1 for codes.
 // ODD: rows start on any byte (K >= 16).  16 codes are cut from the five words that hold them, which costs far less than loads off word
 // alignment (K = 4097, N = 14336, 16 tokens: 25.5 us for 66; 38 by padded copies); a row's last codes are read from K - 16 and moved.
-template <int TB, int NB, int BF, int XT, int WAVES, bool ODD>
+template <int TB, int NB, int BF, int XT, int WAVES, bool ODD, bool MANY>
 __global__ __launch_bounds__(WAVES * 64) void stream_kernel(MatmulArgs g, TokenArgs t) {
   __shared__ __attribute__((aligned(16))) int red[WAVES][NB][TB + 1][64][4];
-  __shared__ float token_scale;
-  __shared__ int token_zero;
-  extern __shared__ __attribute__((aligned(16))) int8_t codes[];             // [K], XT >= 0 only
+  __shared__ float token_scale[MANY ? 16 : 1];
+  __shared__ int token_zero[MANY ? 16 : 1];
+  extern __shared__ __attribute__((aligned(16))) int8_t codes[];             // XT >= 0: [M] rows, K + 16 apart (16 lanes' reads touch all banks once)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t n0 = (int64_t)blockIdx.x * (16 * NB);
   const int rows_w = (int)(g.N - n0 < 16 * NB ? g.N - n0 : 16 * NB);
   const int at = (lane >> 4) * 16;                  // this lane's 16 codes of 64
   const bool asym = XT < 0 ? g.az != nullptr : t.asym;
-  TokenRow<XT, WAVES> row;
-  if constexpr (XT >= 0) row.load(t, 0, g.K);
+  TokenRow<XT, MANY ? 1 : WAVES, MANY ? 8 : 4> row;
+  if constexpr (XT >= 0) row.load(t, MANY && wave < g.M ? wave : 0, g.K);
+  const int8_t* const mine = codes + (MANY && (lane & 15) < g.M ? (lane & 15) * (g.K + 16) : 0);       // (a token past the last one is not stored)
 
   // Loads are told where their matrix ends: codes past K and rows past the last one read as zero, without a branch.
   const __amdgpu_buffer_rsrc_t bufW = __builtin_amdgcn_make_buffer_rsrc((void*)(g.w + n0 * g.ldw), 0, (int)((rows_w - 1) * g.ldw + g.K), 0x00020000);
@@ -513,7 +518,15 @@ __global__ __launch_bounds__(WAVES * 64) void stream_kernel(MatmulArgs g, TokenA
     load(k + d * STEP, ring[d]);
     __builtin_amdgcn_sched_barrier(0);              // (in this order: a wait counts the loads behind it)
   }
-  if constexpr (XT >= 0) row.to_codes(t, codes, (float*)red, &token_scale, &token_zero);
+  if constexpr (MANY) {
+    for (int r = wave; r < g.M; r += WAVES) {
+      if (r != wave) row.load(t, r, g.K);
+      row.to_codes(t, codes + r * (g.K + 16), nullptr, &token_scale[r], &token_zero[r]);
+    }
+    __syncthreads();
+  } else if constexpr (XT >= 0) {
+    row.to_codes(t, codes, (float*)red, token_scale, token_zero);
+  }
   i32x4 acc[NB][TB] = {};
   int wsum[NB] = {};
   while (k < g.K) {
@@ -539,7 +552,7 @@ __global__ __launch_bounds__(WAVES * 64) void stream_kernel(MatmulArgs g, TokenA
       }
       #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if constexpr (XT >= 0) p.a[0][i] = *(const i32x4*)(codes + (k + i * 64 + at < g.K ? k + i * 64 + at : 0));   // (every column the token; past K the weight is 0)
+        if constexpr (XT >= 0) p.a[0][i] = *(const i32x4*)(mine + (k + i * 64 + at < g.K ? k + i * 64 + at : 0));   // (past K the weight is 0)
         #pragma unroll
         for (int c = 0; c < NB; ++c) {
           #pragma unroll
@@ -570,8 +583,8 @@ __global__ __launch_bounds__(WAVES * 64) void stream_kernel(MatmulArgs g, TokenA
       s += red[v][cb][b][(cc >> 2) * 16 + tok][cc & 3];
       if (asym) sum += (red[v][cb][TB][cc][0] + red[v][cb][TB][cc + 16][0]) + (red[v][cb][TB][cc + 32][0] + red[v][cb][TB][cc + 48][0]);
     }
-    if (asym) s -= (XT < 0 ? g.az[token] : token_zero) * sum;
-    const float as = XT < 0 ? g.as[g.a_scalar ? 0 : token] : token_scale;
+    if (asym) s -= (XT < 0 ? g.az[token] : token_zero[MANY ? token : 0]) * sum;
+    const float as = XT < 0 ? g.as[g.a_scalar ? 0 : token] : token_scale[MANY ? token : 0];
     const float y = __builtin_fmaf((float)s, as * load_any(g.ws, g.ws_dtype, g.w_scalar ? 0 : nn), g.bias ? load_any(g.bias, g.bias_dtype, nn) : 0.0f);
     if constexpr (BF == ROW_F32) ((float*)g.y)[token * g.N + nn] = y;
     else store_scalar<BF>(g.y, token * g.N + nn, rnd<BF>(y));
@@ -629,9 +642,10 @@ void launch_join(const MatmulArgs& g, const int* sums, int parts, hipStream_t st
   else join_kernel<BF, 1><<<dim3((unsigned)((all + 255) / 256)), dim3(256), 0, st>>>(g, sums, parts);
 }
 
-template <int TB, int NB, int BF, int XT, int WAVES, bool ODD = false>
+template <int TB, int NB, int BF, int XT, int WAVES, bool ODD = false, bool MANY = false>
 void launch_stream(const MatmulArgs& g, const TokenArgs& t, hipStream_t st) {
-  stream_kernel<TB, NB, BF, XT, WAVES, ODD><<<dim3((unsigned)((g.N + 16 * NB - 1) / (16 * NB))), dim3(WAVES * 64), XT < 0 ? 0 : (unsigned)g.K, st>>>(g, t);
+  stream_kernel<TB, NB, BF, XT, WAVES, ODD, MANY><<<dim3((unsigned)((g.N + 16 * NB - 1) / (16 * NB))), dim3(WAVES * 64),
+                                                    XT < 0 ? 0 : (unsigned)(g.M * (g.K + 16)), st>>>(g, t);
 }
 
 // Two blocks of channels per workgroup halve the passes of the tokens' codes through the L2, one block spreads better over 256 CUs: it is
@@ -680,7 +694,8 @@ void launch_codes(const MatmulArgs& g, bool streams, int* sums, hipStream_t st) 
 // eight keep enough of a long weight row on its way (4096 x 14336: 14.7 us, four 16.9; 8192 x 28672: 45.4, four 50.6).
 template <int BF, int XT>
 void launch_token(const MatmulArgs& g, const TokenArgs& t, hipStream_t st) {
-  if (g.K <= 8192) launch_stream<1, 1, BF, XT, 4>(g, t, st);
+  if (g.M > 1) launch_stream<1, 1, BF, XT, 4, false, true>(g, t, st);
+  else if (g.K <= 8192) launch_stream<1, 1, BF, XT, 4>(g, t, st);
   else launch_stream<1, 1, BF, XT, 8>(g, t, st);
 }
 
@@ -697,8 +712,15 @@ int check(const int8_t* w, const void* ws, int ws_dtype, const void* bias, int b
 // rows that only the padding kernel brings to where they can be read
 bool pads(int64_t K, bool streams) { return K % 16 != 0 && (!streams || K < 16); }
 
-// one token, whose codes the product makes itself
-bool fused(int64_t M, int64_t K) { return M == 1 && K % 16 == 0 && K <= MOST_FUSED; }
+// Tokens whose codes every workgroup of the product makes itself: one, and up to eight where a wave's rows are short and hardly more workgroups than
+// CUs make them.  One launch instead of two costs the host 4 us less; on the GPU it takes, with the quantizer's launch beside it, us:
+//   N = K = 4096, 4 tokens 9.6 / 9.7     K = 1024, 4 tokens 5.4 / 6.1, 8 tokens 6.9 / 6.6     K = 2048, 8 tokens 8.8 / 7.0 (by itself)
+//   N = 14336, K = 4096, 4 tokens 21.1 / 17.7 and N = 1024, K = 8192, 2 tokens 13.3 / 10.5 (by itself both)
+bool fused(int64_t M, int64_t N, int64_t K) {
+  if (K % 16) return false;
+  const int64_t rows = (M + 3) / 4;                 // of a wave
+  return M == 1 ? K <= MOST_FUSED : M <= 8 && N <= 4096 && rows * rows * K <= 4096;
+}
 
 }  // namespace
 
@@ -741,7 +763,7 @@ int lcq_int8_matmul(const int8_t* a, const float* as, int a_scalar, const int32_
 }
 
 int64_t lcq_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  if (M <= 0 || N <= 0 || K <= 0 || K > 65536 || fused(M, K)) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || K > 65536 || fused(M, N, K)) return 0;
   return on256(M * K) + on256(8 * M) + lcq_int8_matmul_workspace_bytes(M, N, K);
 }
 
@@ -752,7 +774,7 @@ int lcq_int8_linear(const void* x, int x_dtype, int64_t ldx, int asym, const flo
   const int bad = check(w, ws, ws_dtype, bias, bias_dtype, M, N, K, y, dtype);
   if (bad) return bad;
   if (!known(x_dtype)) return LCQ_EDTYPE;
-  if (fused(M, K)) {
+  if (fused(M, N, K)) {
     hipStream_t st = (hipStream_t)stream;
     const MatmulArgs g = {nullptr, w, nullptr, nullptr, ws, bias, y, M, N, K, K, (int)K, ws_dtype, bias_dtype, 0, w_scalar};
     const TokenArgs t = {x, scale, ldx, asym};

@@ -85,11 +85,11 @@ def test_the_c_entries_refuse_before_a_launch():
     assert mm(a=None) == mm(s=None) == mm(w=None) == mm(ws=None) == mm(y=None) == mm(M=0) == mm(N=0) == mm(K=0) == mm(M=-1) == -1
     assert mm(wd=5) == mm(d=-1) == mm(b=P, bd=9) == -3 and mm(K=65537) == -6
     assert lib.lcq_int8_matmul_workspace_bytes(0, 8, 64) == lib.lcq_int8_matmul_workspace_bytes(2, 8, 65537) == 0
-    lin = lambda x=P, xd=0, asym=0, sc=None, w=P, ld=64, M=8, K=64, ws=None: lib.lcq_int8_linear(  # noqa: E731
+    lin = lambda x=P, xd=0, asym=0, sc=None, w=P, ld=64, M=9, K=64, ws=None: lib.lcq_int8_linear(  # noqa: E731
         x, xd, ld, asym, sc, w, P, 0, 0, None, 0, M, 8, K, P, 0, ws, None)
     assert lin(x=None) == lin(w=None) == lin(ld=-1) == lin(asym=1, sc=P) == lin(M=0) == -1 and lin(xd=5) == -3 and lin(K=65537) == -6
     assert lin(w=P + 8) == -2 and lin() == -5 and lin(ws=P + 8) == -2 and mm(w=P + 1) == mm(a=P + 4) == -2 and mm(M=65, K=63) == mm(K=15) == -5
-    assert lib.lcq_int8_linear_workspace_bytes(1, 8, 64) == 0 < lib.lcq_int8_linear_workspace_bytes(8, 8, 64)
+    assert lib.lcq_int8_linear_workspace_bytes(1, 8, 64) == lib.lcq_int8_linear_workspace_bytes(8, 8, 64) == 0 < lib.lcq_int8_linear_workspace_bytes(9, 8, 64)
     norm = lambda x=P, d=0, T=2, K=64, pw=None, pb=None, f=0, h=P, o=P, c=None, s=None, z=None: lib.lcq_residual_norm(  # noqa: E731
         x, d, T, K, 64, None, 0, None, 0, pw, pb, None, None, 1.0, 1e-6, 0.0, f, h, o, c, s, z, None)
     assert norm(x=None) == norm(h=None) == norm(o=None) == norm(c=P) == norm(T=0) == norm(pb=P) == norm(f=256) == -1

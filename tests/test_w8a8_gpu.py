@@ -219,7 +219,7 @@ def test_product_of_odd_rows_off_alignment(dev, M, N, K):
 
 @pytest.mark.parametrize('dtype', [BF, HF, F32])
 @pytest.mark.parametrize('M,K', [(1, 1), (1, 16), (1, 4096), (1, 16400), (1, 40960), (1, 40976), (1, 65536), (2, 1040), (3, 4096), (4, 10240), (4, 10256), (4, 1000),
-                                 (5, 512), (16, 4096), (33, 1024), (300, 528)])
+                                 (5, 512), (16, 4096), (33, 1024), (300, 528), (2, 16), (8, 1024), (6, 1008), (4, 4112)])
 def test_linear_is_codes_and_product(dev, M, K, dtype):
     """However few the tokens, however they lie: the same bits as by the codes."""
     g = gen(M + K)
