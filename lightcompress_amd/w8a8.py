@@ -212,9 +212,9 @@ def _affine(name, t, K, dtype, flag):
     return flag
 
 
-def _meets(t, out):
-    """Does t lie where the contiguous `out` is written, other than element on element?"""
-    if not t.numel() or (t.data_ptr() == out.data_ptr() and t.dtype == out.dtype and t.shape == out.shape and t.is_contiguous()):
+def _meets(t, out, read_before):
+    """Does t lie where the contiguous `out` is written?  What is read before that (read_before) may lie there element on element."""
+    if not t.numel() or (read_before and t.data_ptr() == out.data_ptr() and t.dtype == out.dtype and t.shape == out.shape and t.is_contiguous()):
         return False
     span = (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
     return t.data_ptr() < out.data_ptr() + out.numel() * out.element_size() and out.data_ptr() < t.data_ptr() + span
@@ -262,8 +262,8 @@ def residual_norm(x, residual=None, weight=None, bias=None, *, gate=None, post_w
             raise ValueError('inplace needs a contiguous residual')
         if residual.requires_grad and torch.is_grad_enabled():
             raise ValueError('inplace would change a residual that autograd keeps')
-        for t in (x, weight, bias, gate, post_weight, post_bias):
-            if t is not None and _meets(t, residual):
+        for t in (x, gate, post_weight, post_bias, weight, bias):
+            if t is not None and _meets(t, residual, t is not weight and t is not bias):      # (the last norm reads its own behind h)
                 raise ValueError('inplace would write over a part of another operand that is still read')
     if gate is not None:
         if gate.dtype is not dtype:
