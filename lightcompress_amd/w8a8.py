@@ -302,4 +302,6 @@ def residual_norm(x, residual=None, weight=None, bias=None, *, gate=None, post_w
             L.ptr(post_weight), L.ptr(post_bias), L.ptr(weight), L.ptr(bias), scale, eps, weight_offset, flags, h.data_ptr(),
             None if out is None else out.data_ptr(), None if codes is None else codes.data_ptr(),
             None if scales is None else scales.data_ptr(), None if zeros is None else zeros.data_ptr(), L.stream()), 'lcq_residual_norm')
+        if inplace:                           # (so that a backward pass which kept the old values says so)
+            torch.autograd.graph.increment_version(residual)
     return ResidualNorm(out if quantize is None else QuantizedTokens(codes, scales, zeros), h)
