@@ -126,6 +126,15 @@ def quantize_tokens(x, symmetric=True, scale=None):
     return QuantizedTokens(codes, scales, zeros)
 
 
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def _whole(t):
+    """t (or None), or a contiguous copy."""
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
 def _on16(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
@@ -147,7 +156,8 @@ def _check_weight(weight, weight_scales, bias, K):
 def int8_matmul(tokens, weight, weight_scales, bias=None, out_dtype=torch.bfloat16):
     """Tokens as codes (QuantizedTokens, codes [..., K]) times an int8 weight [N, K] with a scale per channel ([N], [N, 1], or
     one for all; fp32, bf16, fp16), plus a bias [N]: [..., N] of `out_dtype`.  The sums are exact integers, scales and bias
-    are applied in fp32, the result is rounded once."""
+    are applied in fp32, the result is rounded once.  Operands with strides (the last token's codes of each sequence) are copied, a
+    weight too, and in every call."""
     codes, scales, zeros = tokens
     shape = codes.shape
     K = _cols(shape)
@@ -162,14 +172,16 @@ def int8_matmul(tokens, weight, weight_scales, bias=None, out_dtype=torch.bfloat
     if not _here(codes, scales, zeros, weight, weight_scales, bias):
         with torch.cuda.device(codes.device):
             return int8_matmul(tokens, weight, weight_scales, bias, out_dtype)
+    codes, scales, zeros = _whole(codes), _whole(scales), _whole(zeros)
+    weight, weight_scales, bias = _whole(weight), _whole(weight_scales), _whole(bias)
     if K % 16 == 0:                           # (rows of other widths may start anywhere)
         codes, weight = _on16(codes), _on16(weight)
     y = codes.new_empty(_with(shape, N), dtype=out_dtype)
     if M and N:
         ws = _workspace(codes, 'lcq_int8_matmul_workspace_bytes', M, N, K)
-        L.check(L.lib().lcq_int8_matmul(L.ptr(codes), L.ptr(scales), scales.numel() == 1, L.ptr(zeros), L.ptr(weight),
-                                        L.ptr(weight_scales), _code(weight_scales.dtype), weight_scales.numel() == 1, L.ptr(bias),
-                                        0 if bias is None else _code(bias.dtype), M, N, K, y.data_ptr(), code, L.ptr(ws),
+        L.check(L.lib().lcq_int8_matmul(codes.data_ptr(), scales.data_ptr(), scales.numel() == 1, _at(zeros), weight.data_ptr(),
+                                        weight_scales.data_ptr(), _code(weight_scales.dtype), weight_scales.numel() == 1, _at(bias),
+                                        0 if bias is None else _code(bias.dtype), M, N, K, y.data_ptr(), code, _at(ws),
                                         L.stream()), 'lcq_int8_matmul')
     return y
 
@@ -189,14 +201,15 @@ def int8_linear(x, weight, weight_scales, bias=None, symmetric=True, scale=None,
         with torch.cuda.device(x.device):
             return int8_linear(x, weight, weight_scales, bias, symmetric, scale, out_dtype)
     rows, M, ld = _rows(x, K)
+    weight, weight_scales, bias = _whole(weight), _whole(weight_scales), _whole(bias)
     if K % 16 == 0:                           # (rows of other widths may start anywhere)
         weight = _on16(weight)
     y = x.new_empty(_with(shape, N), dtype=out_dtype)
     if M and N:
         ws = _workspace(x, 'lcq_int8_linear_workspace_bytes', M, N, K)
-        L.check(L.lib().lcq_int8_linear(rows.data_ptr(), x_code, ld, not symmetric, L.ptr(given), L.ptr(weight), L.ptr(weight_scales),
-                                        _code(weight_scales.dtype), weight_scales.numel() == 1, L.ptr(bias),
-                                        0 if bias is None else _code(bias.dtype), M, N, K, y.data_ptr(), code, L.ptr(ws),
+        L.check(L.lib().lcq_int8_linear(rows.data_ptr(), x_code, ld, not symmetric, _at(given), weight.data_ptr(),
+                                        weight_scales.data_ptr(), _code(weight_scales.dtype), weight_scales.numel() == 1, _at(bias),
+                                        0 if bias is None else _code(bias.dtype), M, N, K, y.data_ptr(), code, _at(ws),
                                         L.stream()), 'lcq_int8_linear')
     return y
 
@@ -285,7 +298,8 @@ def residual_norm(x, residual=None, weight=None, bias=None, *, gate=None, post_w
     if residual is not None:
         res, _, ldr = _rows(residual, K)
     if gate is not None:
-        g, _, ldg = (gate.contiguous(), 1, 0) if gate.dim() == 1 else _rows(gate, K)
+        g, _, ldg = (_whole(gate), 1, 0) if gate.dim() == 1 else _rows(gate, K)
+    weight, bias, post_weight, post_bias = _whole(weight), _whole(bias), _whole(post_weight), _whole(post_bias)
     h = residual if inplace else _like(x, stream_dtype)
     out = codes = scales = zeros = None
     if quantize is None:
@@ -298,10 +312,8 @@ def residual_norm(x, residual=None, weight=None, bias=None, *, gate=None, post_w
             zeros = x.new_empty(_with(shape, 1), dtype=torch.int32)
     if T:
         L.check(L.lib().lcq_residual_norm(
-            rows.data_ptr(), code, T, K, ldx, None if res is None else res.data_ptr(), ldr, None if g is None else g.data_ptr(), ldg,
-            L.ptr(post_weight), L.ptr(post_bias), L.ptr(weight), L.ptr(bias), scale, eps, weight_offset, flags, h.data_ptr(),
-            None if out is None else out.data_ptr(), None if codes is None else codes.data_ptr(),
-            None if scales is None else scales.data_ptr(), None if zeros is None else zeros.data_ptr(), L.stream()), 'lcq_residual_norm')
+            rows.data_ptr(), code, T, K, ldx, _at(res), ldr, _at(g), ldg, _at(post_weight), _at(post_bias), _at(weight), _at(bias),
+            scale, eps, weight_offset, flags, h.data_ptr(), _at(out), _at(codes), _at(scales), _at(zeros), L.stream()), 'lcq_residual_norm')
         if inplace:                           # (so that a backward pass which kept the old values says so)
             torch.autograd.graph.increment_version(residual)
     return ResidualNorm(out if quantize is None else QuantizedTokens(codes, scales, zeros), h)

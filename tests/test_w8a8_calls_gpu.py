@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from lightcompress_amd.w8a8 import residual_norm
+from lightcompress_amd.w8a8 import QuantizedTokens, int8_linear, int8_matmul, quantize_tokens, residual_norm
 from tests.helpers import gen
 
 pytestmark = pytest.mark.gpu
@@ -34,3 +34,39 @@ def test_in_place_leaves_versions_alone_that_it_does_not_write(dev):
         t = torch.randn(4, 64, device=dev)
         want = t + x
         assert torch.equal(residual_norm(x, t, inplace=True).residual, want)
+
+
+# -- strides ----------------------------------------------------------------------------------------------------------------
+def same(got, want):
+    return all((a is None and b is None) or (torch.equal(a, b) and a.shape == b.shape) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize('symmetric', [True, False])
+@pytest.mark.parametrize('K', [64, 63])
+@pytest.mark.parametrize('B', [1, 3, 70])
+def test_codes_of_the_last_tokens(dev, B, K, symmetric):
+    """Codes, scales and zero points of [B, S, K] cut to one token of each sequence, as in front of a head; operands with strides."""
+    x = (torch.randn(B, 5, K, generator=gen(B + K)) + 0.5).to(BF).to(dev)
+    w = torch.randint(-127, 128, (40, K), generator=gen(7), dtype=torch.int8).to(dev)
+    ws, bias = torch.rand(40, generator=gen(8)).to(dev), torch.randn(40, generator=gen(9)).to(dev)
+    spread = lambda t: torch.stack([t, t], -1).flatten(-2)[..., ::2]  # noqa: E731  (t in twice the room)
+    q = quantize_tokens(x, symmetric)
+    for cut in ((slice(None), -1), (slice(None), slice(1, 3)), (slice(None, None, 2),)):
+        part = QuantizedTokens(*(None if t is None else t[cut] for t in q))
+        whole = QuantizedTokens(*(None if t is None else t[cut].contiguous() for t in q))
+        want = int8_matmul(whole, w, ws, bias)
+        assert torch.equal(int8_matmul(part, w, ws, bias), want)
+        assert torch.equal(int8_matmul(part, spread(w), spread(ws), spread(bias)), want)
+        assert torch.equal(int8_matmul(part, w.t().contiguous().t(), spread(ws)[:, None], spread(bias)), want)
+    want = int8_linear(x, w, ws, bias, symmetric)
+    assert torch.equal(int8_linear(x, spread(w), spread(ws), spread(bias), symmetric), want)
+    one = ws[:1]
+    assert torch.equal(int8_linear(x, w, one.expand(40), bias, symmetric), int8_linear(x, w, one, bias, symmetric))
+
+
+def test_norm_parameters_with_strides(dev):
+    x, r = torch.randn(3, 96, generator=gen(5)).to(dev), torch.randn(3, 96, generator=gen(6)).to(dev)
+    p = torch.randn(96, 5, generator=gen(7)).to(dev)
+    names = ('weight', 'bias', 'post_weight', 'post_bias', 'gate')
+    kw = {n: p[:, i] for i, n in enumerate(names)}
+    assert same(residual_norm(x, r, **kw), residual_norm(x, r, **{n: t.contiguous() for n, t in kw.items()}))
