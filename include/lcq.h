@@ -528,6 +528,12 @@ int lcq_token_logprobs(const void* logits, int dtype, int64_t T, int64_t V, int6
                        int64_t ignore, float* logprobs, float* entropy, int k, float* top_logprobs, int64_t* top_tokens,
                        void* stream);
 
+/* The same of B sequences of S rows each, in one launch: rows `ldx` elements apart, sequences `lds` (all but the last row of each sequence
+ * of [B, S + 1, V]: lds = (S + 1) V).  T = B S < 2^31; tokens and outputs are [B, S, ...] without gaps. */
+int lcq_token_logprobs_of(const void* logits, int dtype, int64_t B, int64_t S, int64_t V, int64_t lds, int64_t ldx, const int64_t* tokens,
+                          int64_t m, int64_t ignore, float* logprobs, float* entropy, int k, float* top_logprobs, int64_t* top_tokens,
+                          void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -27,9 +27,15 @@ struct LogprobArgs {
   const int64_t* tokens;
   float *logprobs, *entropy, *top_logprobs;
   int64_t* top_tokens;
-  int64_t V, ldx, m, ignore;
+  int64_t V, ldx, lds, m, ignore;
+  uint32_t rows;                                    // of a sequence: `ldx` elements apart, sequences `lds`
   int k;
   int64_t first;                                    // row of a launch
+
+  __device__ __forceinline__ int64_t start(int64_t row) const {              // of a row's logits
+    const uint32_t s = (uint32_t)row / rows;
+    return s * lds + ((uint32_t)row - s * rows) * ldx;
+  }
 };
 
 // A whole number that orders logits by value and, among equal ones, by the lowest index; a NaN is above everything, -0 equals +0.
@@ -139,19 +145,19 @@ struct Given {
   int64_t token = 0;
   float x = 0.0f;
   __device__ __forceinline__ void tokens(const LogprobArgs& a, int64_t row, int lane) { if (lane < a.m) token = a.tokens[row * a.m + lane]; }
-  __device__ __forceinline__ void logits(const LogprobArgs& a, int64_t row, int lane) {
-    if (lane < a.m && token >= 0 && token < a.V) x = load_scalar<BF>(a.x, row * a.ldx + token);
+  __device__ __forceinline__ void logits(const LogprobArgs& a, int64_t start, int lane) {
+    if (lane < a.m && token >= 0 && token < a.V) x = load_scalar<BF>(a.x, start + token);
   }
 };
 
 template <int BF>
-__device__ __forceinline__ void answer(const LogprobArgs& a, int64_t row, const Sums& s, Given<BF> g, uint64_t mine, int lane) {
+__device__ __forceinline__ void answer(const LogprobArgs& a, int64_t row, int64_t start, const Sums& s, Given<BF> g, uint64_t mine, int lane) {
   const float l = logf(s.S);
   if (lane == 0 && a.entropy) a.entropy[row] = l - s.U / s.S;
   for (int64_t j = lane; j < a.m; j += 64) {
     if (j >= 64) {
       g.token = a.tokens[row * a.m + j];
-      if (g.token >= 0 && g.token < a.V) g.x = load_scalar<BF>(a.x, row * a.ldx + g.token);
+      if (g.token >= 0 && g.token < a.V) g.x = load_scalar<BF>(a.x, start + g.token);
     }
     a.logprobs[row * a.m + j] = g.token == a.ignore ? 0.0f : g.token < 0 || g.token >= a.V ? __builtin_nanf("") : (g.x - s.c) - l;
   }
@@ -173,8 +179,8 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(LogprobArgs a) {
   __shared__ uint32_t reach;
   __shared__ int count;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row = a.first + blockIdx.x;
-  const char* const x = (const char*)a.x + row * a.ldx * (16 / N);
+  const int64_t row = a.first + blockIdx.x, start = a.start(row);
+  const char* const x = (const char*)a.x + start * (16 / N);
   const int V = (int)a.V, pieces = (V + N - 1) / N;
   const int last = V / N;                           // (all pieces of the row but its last hold N logits)
   const int passes = (pieces + PASS - 1) / PASS, per = (passes + PARTS - 1) / PARTS;
@@ -238,7 +244,7 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(LogprobArgs a) {
     #pragma unroll
     for (int f = 0; f < FLIGHT; ++f) one[f] = two[f];
   }
-  if (wave == 0) given.logits(a, row, lane);
+  if (wave == 0) given.logits(a, start, lane);
   s.join_wave();
   if (lane == 0) { sums[wave][0] = s.c; sums[wave][1] = s.S; sums[wave][2] = s.U; }
   Best best(lane, TOP ? a.k : 1);
@@ -338,22 +344,23 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(LogprobArgs a) {
       for (int i = 0; i < count; i += 64) best.take(i + lane < count ? keys[i + lane] : 0);
     }
   }
-  answer<BF>(a, row, s, given, best.mine, lane);
+  answer<BF>(a, row, start, s, given, best.mine, lane);
 }
 
 }  // namespace
 
 extern "C" {
 
-int lcq_token_logprobs(const void* logits, int dtype, int64_t T, int64_t V, int64_t ldx, const int64_t* tokens, int64_t m,
-                       int64_t ignore, float* logprobs, float* entropy, int k, float* top_logprobs, int64_t* top_tokens,
-                       void* stream) {
-  if (!logits || T <= 0 || V <= 0 || ldx < 0 || m < 0 || k < 0 || k > 64 || k > V) return LCQ_EINVAL;
+int lcq_token_logprobs_of(const void* logits, int dtype, int64_t B, int64_t S, int64_t V, int64_t lds, int64_t ldx, const int64_t* tokens,
+                          int64_t m, int64_t ignore, float* logprobs, float* entropy, int k, float* top_logprobs, int64_t* top_tokens,
+                          void* stream) {
+  if (!logits || B <= 0 || S <= 0 || V <= 0 || lds < 0 || ldx < 0 || m < 0 || k < 0 || k > 64 || k > V) return LCQ_EINVAL;
   if ((m > 0 && (!tokens || !logprobs)) || (k > 0 && (!top_logprobs || !top_tokens))) return LCQ_EINVAL;
   if (dtype != LCQ_F32 && dtype != LCQ_BF16 && dtype != LCQ_F16) return LCQ_EDTYPE;
-  if (T > 0x7fffffff || V > (1 << 28)) return LCQ_ESIZE;
+  if (S > 0x7fffffff || B > 0x7fffffff / S || V > (1 << 28)) return LCQ_ESIZE;
   if ((uintptr_t)logits % (dtype == LCQ_F32 ? 4 : 2)) return LCQ_EALIGN;
-  const LogprobArgs a = {logits, tokens, logprobs, entropy, top_logprobs, top_tokens, V, ldx, m, ignore, k, 0};
+  const int64_t T = B * S;
+  const LogprobArgs a = {logits, tokens, logprobs, entropy, top_logprobs, top_tokens, V, ldx, lds, m, ignore, (uint32_t)S, k, 0};
   const auto launch = [&](auto bf, auto threads) {
     constexpr int BF = decltype(bf)::value, THREADS = decltype(threads)::value;
     constexpr int64_t rows = 1 << 21;               // (a launch has fewer than 2^32 lanes)
@@ -374,6 +381,12 @@ int lcq_token_logprobs(const void* logits, int dtype, int64_t T, int64_t V, int6
   else run(std::integral_constant<int, ROW_F32>{});
   LCQ_CHECK_LAUNCH();
   return LCQ_OK;
+}
+
+int lcq_token_logprobs(const void* logits, int dtype, int64_t T, int64_t V, int64_t ldx, const int64_t* tokens, int64_t m,
+                       int64_t ignore, float* logprobs, float* entropy, int k, float* top_logprobs, int64_t* top_tokens,
+                       void* stream) {
+  return lcq_token_logprobs_of(logits, dtype, 1, T, V, 0, ldx, tokens, m, ignore, logprobs, entropy, k, top_logprobs, top_tokens, stream);
 }
 
 }  // extern "C"

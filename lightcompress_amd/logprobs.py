@@ -8,7 +8,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib as L
-from .w8a8 import _code, _here, _rows
+from .w8a8 import _code, _here
 
 MOST_TOP = 64
 
@@ -18,6 +18,25 @@ class TokenLogprobs(NamedTuple):
     entropy: torch.Tensor                     # fp32 [...], in nats
     top_logprobs: torch.Tensor                # fp32 [..., top], largest first
     top_tokens: torch.Tensor                  # int64 [..., top]
+
+
+def _sequences(x):
+    """Logits [..., V] as B sequences of S rows -> (x or a contiguous copy, B, S, distance between sequences, between rows).
+    Dimensions that one stride covers are one; a copy is made only where more than two are left, or a row is not in one piece."""
+    V = x.shape[-1]
+    if x.is_contiguous():
+        return x, 1, x.numel() // V, 0, V
+    dims = []
+    for n, stride in zip(x.shape[:-1], x.stride()[:-1]):
+        if n == 1:
+            continue
+        if dims and dims[-1][1] == n * stride:
+            n *= dims.pop()[0]
+        dims.append((n, stride))
+    if len(dims) > 2 or (x.stride(-1) != 1 and V > 1):
+        return _sequences(x.contiguous())
+    (B, lds), (S, ldx) = [(1, 0)] * (2 - len(dims)) + dims
+    return x, B, S, lds, ldx
 
 
 def token_logprobs(logits, tokens=None, top=0, ignore_index=-100):
@@ -51,25 +70,10 @@ def token_logprobs(logits, tokens=None, top=0, ignore_index=-100):
     entropy = logits.new_empty(lead, dtype=torch.float32)
     top_logprobs = logits.new_empty((*lead, top), dtype=torch.float32)
     top_tokens = logits.new_empty((*lead, top), dtype=torch.int64)
-
-    def run(x, at):
-        """The logits x, whose rows are the rows from `at` on of all of them."""
-        if apart and x.dim() > 2:                   # logits[:, :-1]: a call per sequence, and no copy
-            rows = x[0].numel() // V
-            for i in range(x.shape[0]):
-                run(x[i], at + i * rows)
-            return
-        rows, T, ld = _rows(x, V)
-        if T:
-            L.check(L.lib().lcq_token_logprobs(rows.data_ptr(), code, T, V, ld, ids.data_ptr() + 8 * m * at if m else None, m, ignore_index,
-                                               logprobs.data_ptr() + 4 * m * at if m else None, entropy.data_ptr() + 4 * at, top,
-                                               top_logprobs.data_ptr() + 4 * top * at if top else None,
-                                               top_tokens.data_ptr() + 8 * top * at if top else None, L.stream()), 'lcq_token_logprobs')
-
     if logits.numel():
-        apart = logits.dim() > 2 and logits.stride(-1) == 1 and not logits.is_contiguous()
-        if apart:                                   # many short sequences (a transposed batch): one copy is faster than their calls
-            each = V * lead[-1]
-            apart = logits.numel() // each <= 64 or each * logits.element_size() >= 1 << 25
-        run(logits, 0)
+        x, B, S, lds, ldx = _sequences(logits)
+        L.check(L.lib().lcq_token_logprobs_of(x.data_ptr(), code, B, S, V, lds, ldx, ids.data_ptr() if m else None, m, ignore_index,
+                                              logprobs.data_ptr() if m else None, entropy.data_ptr(), top,
+                                              top_logprobs.data_ptr() if top else None, top_tokens.data_ptr() if top else None,
+                                              L.stream()), 'lcq_token_logprobs_of')
     return TokenLogprobs(logprobs, entropy, top_logprobs, top_tokens)

@@ -1,9 +1,15 @@
 """Calls of the operators of a running w8a8 model that are refused before any launch: operands that meet, forms that are unknown."""
+import ctypes
+
 import pytest
 import torch
 
 from lightcompress_amd import _lib as L
+from lightcompress_amd.logprobs import _sequences
 from lightcompress_amd.w8a8 import residual_norm
+
+BUF = ctypes.create_string_buffer(256)
+P = ctypes.addressof(BUF) & ~15                  # stands for a device pointer: every call below returns before it is used
 
 
 @pytest.mark.parametrize('name', ['weight', 'bias'])
@@ -24,3 +30,32 @@ def test_in_place_over_what_is_read_before():
                  lambda: residual_norm(torch.zeros(64), v, post_weight=v, post_bias=v, inplace=True)):
         with pytest.raises(L.LcqError, match='GPU tensors only'):
             call()
+
+
+def test_strided_logits_are_one_call():
+    """Views of logits as sequences of rows, without a copy wherever two strides say where the rows are."""
+    x = torch.arange(4 * 6 * 5 * 7.0).view(4, 6, 5, 7)
+    flat = x.view(24, 5, 7)
+
+    def form(v, copied=False):
+        t, B, S, lds, ldx = _sequences(v)
+        assert B * S * v.shape[-1] == v.numel() and (t is v) != copied
+        at = torch.arange(B)[:, None, None] * lds + torch.arange(S)[:, None] * ldx + torch.arange(v.shape[-1])
+        got = torch.as_strided(t, (t.untyped_storage().size() // 4,), (1,), 0)[at + t.storage_offset()]
+        assert torch.equal(got.reshape(v.shape), v)
+        return B, S
+
+    assert form(x) == (1, 120) and form(flat[0, 2]) == (1, 1) and form(flat[:, 1]) == (1, 24) and form(flat[:, -1:]) == (1, 24)
+    assert form(flat[:, :-1]) == (24, 4) and form(flat[:1, :-1]) == (1, 4) and form(flat[3:, 1:3, 2:]) == (21, 2)
+    assert form(x[:, :, :-1]) == (24, 4) and form(x[:, :-1]) == (4, 25) and form(x[:, 2]) == (4, 5) and form(x[..., 3:]) == (1, 120)
+    assert form(flat.transpose(0, 1)) == (5, 24) and form(flat[:1].expand(3, 5, 7)) == (3, 5) and form(flat[0, :1].expand(9, 7)) == (1, 9)
+    assert form(x[..., :1]) == (1, 120) and form(x[:, :-1, :-1], copied=True) == (1, 80) and form(x.transpose(2, 3), copied=True) == (1, 168)
+    assert form(x[0, 0].t(), copied=True) == (1, 7)
+
+
+def test_the_entry_of_sequences_refuses_before_a_launch():
+    call = lambda x=P, d=0, B=2, S=3, V=100, lds=300, ld=100, t=None, m=0, o=None, k=0: L.lib().lcq_token_logprobs_of(  # noqa: E731
+        x, d, B, S, V, lds, ld, t, m, -100, o, None, k, None, None, None)
+    assert call(x=None) == call(B=0) == call(S=0) == call(V=0) == call(lds=-1) == call(ld=-1) == call(m=1) == call(k=1) == call(k=65) == -1
+    assert call(d=4) == -3 and call(B=1 << 16, S=1 << 15) == call(B=1 << 31, S=1) == call(S=1 << 31) == call(V=1 << 29) == -6
+    assert call(x=P + 1) == -2

@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+from lightcompress_amd import _lib as L
+from lightcompress_amd.logprobs import token_logprobs
 from lightcompress_amd.w8a8 import QuantizedTokens, int8_linear, int8_matmul, quantize_tokens, residual_norm
 from tests.helpers import gen
 
@@ -70,3 +72,56 @@ def test_norm_parameters_with_strides(dev):
     names = ('weight', 'bias', 'post_weight', 'post_bias', 'gate')
     kw = {n: p[:, i] for i, n in enumerate(names)}
     assert same(residual_norm(x, r, **kw), residual_norm(x, r, **{n: t.contiguous() for n, t in kw.items()}))
+
+
+# -- log probabilities of views -----------------------------------------------------------------------------------------------
+class Counted:
+    """The library with its calls of one entry counted."""
+
+    def __init__(self, lib):
+        self.lib, self.calls = lib, 0
+
+    def __getattr__(self, name):
+        if name.startswith('lcq_token_logprobs'):
+            self.calls += 1
+        return getattr(self.lib, name)
+
+
+@pytest.mark.parametrize('dtype', [BF, F32])
+@pytest.mark.parametrize('B,S,V', [(64, 2, 30000), (64, 3, 30001), (3, 400, 5000), (300, 2, 1001), (5, 7, 9), (1, 9, 50)])
+def test_sequences_are_one_call_without_a_copy(dev, B, S, V, dtype, monkeypatch):
+    """Short sequences and long ones, less their last row or cut to it: one launch, no copy, the bits of a contiguous copy."""
+    x = (torch.randn(B, S, V, generator=gen(B + V)) * 3).to(dtype).to(dev)
+    t = torch.randint(0, V, (B, S), generator=gen(S)).to(dev)
+    views = [(x[:, :-1], t[:, 1:]), (x[:, -1:], t[:, -1:]), (x[:, -1], t[:, -1]), (x[:, 1:, 2:], t[:, 1:].clamp(max=V - 3)),
+             (x.transpose(0, 1), t.t()), (x[::2, 1:], t[::2, :-1]), (x[:1].expand(B, S, V)[:, :-1], t[:, 1:])]
+    want = [token_logprobs(v.clone(memory_format=torch.contiguous_format), i.clone(), top=3) for v, i in views]
+    lib = Counted(L.lib())
+    monkeypatch.setattr(L, 'lib', lambda: lib)
+    for (v, i), w in zip(views, want):
+        lib.calls = 0
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        got = token_logprobs(v, i, top=3)
+        torch.cuda.synchronize()
+        assert lib.calls == 1
+        # the answers (48 bytes a row, the ids once more), five allocations of at most 512 bytes above that: no room for the logits
+        assert torch.cuda.max_memory_allocated() - before <= 64 * i.numel() + 5 * 512
+        assert same(got, w)
+
+
+def test_sequences_against_the_formula(dev):
+    x = (torch.randn(70, 3, 2000, generator=gen(31)) * 3).to(HF).to(dev)
+    t = torch.randint(0, 2000, (70, 3), generator=gen(32)).to(dev)
+    t[4, 1], t[5, 1] = -100, 2000
+    got = token_logprobs(x[:, 1:], t[:, 1:], top=2)
+    logp = torch.log_softmax(x[:, 1:].double(), -1)
+    want = logp.gather(-1, t[:, 1:, None].clamp(0, 1999))[..., 0]
+    want[4, 0] = 0.0
+    assert bool(torch.isnan(got.logprobs[5, 0]))
+    want[5, 0] = got.logprobs[5, 0].double()
+    # a sum of 2000 terms in 256 lanes and joins, exponentials within 2^-22: below 2^-17; numbers up to 32 in 24 bits, three roundings: 2^-17
+    assert torch.allclose(got.logprobs.double(), want, rtol=0, atol=2.0 ** -16, equal_nan=True)
+    assert torch.equal(got.top_tokens, torch.sort(x[:, 1:].double(), dim=-1, descending=True, stable=True).indices[..., :2])
+    assert torch.allclose(got.entropy.double(), -(logp.exp() * logp).sum(-1), rtol=0, atol=2.0 ** -14)
