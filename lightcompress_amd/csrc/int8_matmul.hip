@@ -704,7 +704,8 @@ bool known(int dtype) { return dtype == LCQ_F32 || dtype == LCQ_BF16 || dtype ==
 int check(const int8_t* w, const void* ws, int ws_dtype, const void* bias, int bias_dtype, int64_t M, int64_t N, int64_t K, const void* y, int dtype) {
   if (!w || !ws || !y || M <= 0 || N <= 0 || K <= 0) return LCQ_EINVAL;
   if (!known(dtype) || !known(ws_dtype) || (bias && !known(bias_dtype))) return LCQ_EDTYPE;
-  if (K > 65536 || M > 1 << 28 || N > 1 << 28 || (M + 127) / 128 * ((N + 127) / 128) >= 1 << 24) return LCQ_ESIZE;   // (a launch has fewer than 2^32 lanes)
+  // A launch has fewer than 2^32 lanes: tiles of 256, rounded up to eight; 16 channels of 256 lanes, of 512 where a token is long.
+  if (K > 65536 || M > 1 << 28 || N > (K <= 8192 ? 1 << 28 : 1 << 27) - 16 || (M + 127) / 128 * ((N + 127) / 128) > (1 << 24) - 8) return LCQ_ESIZE;
   if (K % 16 == 0 && (uintptr_t)w % 16) return LCQ_EALIGN;
   return LCQ_OK;
 }

@@ -59,3 +59,11 @@ def test_the_entry_of_sequences_refuses_before_a_launch():
     assert call(x=None) == call(B=0) == call(S=0) == call(V=0) == call(lds=-1) == call(ld=-1) == call(m=1) == call(k=1) == call(k=65) == -1
     assert call(d=4) == -3 and call(B=1 << 16, S=1 << 15) == call(B=1 << 31, S=1) == call(S=1 << 31) == call(V=1 << 29) == -6
     assert call(x=P + 1) == -2
+
+
+def test_products_of_more_lanes_than_a_launch_has_are_refused():
+    """2^24 workgroups of 256 lanes are 2^32: one block of channels, or one tile, too many."""
+    linear = lambda M, N, K: L.lib().lcq_int8_linear(P, 0, K, 0, None, P, P, 0, 0, None, 0, M, N, K, P, 0, P, None)  # noqa: E731
+    product = lambda M, N, K: L.lib().lcq_int8_matmul(P, P, 0, None, P, P, 0, 0, None, 0, M, N, K, P, 0, P, None)  # noqa: E731
+    assert linear(1, (1 << 28) - 15, 64) == linear(1, 1 << 28, 64) == linear(1, (1 << 27) - 15, 8208) == linear(1, 1 << 29, 64) == -6
+    assert product(4095 * 128, 4097 * 128, 64) == product(1, 1 << 28, 64) == product(1 << 29, 1, 64) == -6
