@@ -214,7 +214,10 @@ def _act_form(quant_config):
 
 class VllmRealQuantLinear(_RealQuantLinear):
     """The container, and for w8a8 (int8 weight with a scale per channel or one for all, symmetric; int8 activations per token,
-    or static per tensor and symmetric) its forward pass."""
+    or static per tensor and symmetric) its forward pass.
+
+    act_form: how the activations are quantized, 'symmetric', 'asymmetric' or 'static' (by input_scale); None: it does not run.  `new` sets it
+    from the configuration; a container that the constructor made around saved buffers is given it by whoever knows the configuration."""
 
     act_form = None
 
@@ -247,6 +250,8 @@ class VllmRealQuantLinear(_RealQuantLinear):
         the weight's scales)."""
         if self.act_form is None:
             raise NotImplementedError('only w8a8 containers (int8 weight per channel or tensor, int8 activations per token or static) run')
+        if self.act_form not in ('symmetric', 'asymmetric', 'static') or (self.act_form == 'static' and self.input_scale is None):
+            raise ValueError(f'act_form {self.act_form!r}, input_scale {self.input_scale}')
         if isinstance(x, QuantizedTokens):
             return int8_matmul(x, self.weight, self.weight_scale, self.bias, out_dtype or self.weight_scale.dtype)
         return int8_linear(x, self.weight, self.weight_scale, self.bias, symmetric=self.act_form != 'asymmetric',

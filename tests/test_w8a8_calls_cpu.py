@@ -6,6 +6,7 @@ import torch
 
 from lightcompress_amd import _lib as L
 from lightcompress_amd.logprobs import _sequences
+from lightcompress_amd.module_utils import VllmRealQuantLinear
 from lightcompress_amd.w8a8 import residual_norm
 
 BUF = ctypes.create_string_buffer(256)
@@ -67,3 +68,20 @@ def test_products_of_more_lanes_than_a_launch_has_are_refused():
     product = lambda M, N, K: L.lib().lcq_int8_matmul(P, P, 0, None, P, P, 0, 0, None, 0, M, N, K, P, 0, P, None)  # noqa: E731
     assert linear(1, (1 << 28) - 15, 64) == linear(1, 1 << 28, 64) == linear(1, (1 << 27) - 15, 8208) == linear(1, 1 << 29, 64) == -6
     assert product(4095 * 128, 4097 * 128, 64) == product(1, 1 << 28, 64) == product(1 << 29, 1, 64) == -6
+
+
+def test_containers_that_are_told_their_form():
+    """Made by the constructor around saved buffers: with a form they get as far as a GPU, one that is unknown or lacks its scale is refused."""
+    def made(form, scale=None):
+        c = VllmRealQuantLinear(torch.zeros(8, 64, dtype=torch.int8), None, torch.ones(8, 1), scale, False, 'weight_scale')
+        c.act_form = form
+        return c
+
+    for form, scale in (('symmetric', None), ('asymmetric', None), ('static', torch.ones(1))):
+        with pytest.raises(L.LcqError, match='GPU tensors only'):
+            made(form, scale)(torch.zeros(2, 64))
+    for form, scale in (('per_token', None), ('asym', None), ('static', None)):
+        with pytest.raises(ValueError, match='act_form'):
+            made(form, scale)(torch.zeros(2, 64))
+    with pytest.raises(NotImplementedError):
+        made(None)(torch.zeros(2, 64))

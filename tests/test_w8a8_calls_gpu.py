@@ -1,9 +1,12 @@
 """Calls of the operators of a running w8a8 model as a program makes them: beside autograd, on views, captured, of many shapes."""
+import copy
+
 import pytest
 import torch
 
 from lightcompress_amd import _lib as L
 from lightcompress_amd.logprobs import token_logprobs
+from lightcompress_amd.module_utils import VllmRealQuantLinear
 from lightcompress_amd.w8a8 import QuantizedTokens, int8_linear, int8_matmul, quantize_tokens, residual_norm
 from tests.helpers import gen
 
@@ -125,3 +128,15 @@ def test_sequences_against_the_formula(dev):
     assert torch.allclose(got.logprobs.double(), want, rtol=0, atol=2.0 ** -16, equal_nan=True)
     assert torch.equal(got.top_tokens, torch.sort(x[:, 1:].double(), dim=-1, descending=True, stable=True).indices[..., :2])
     assert torch.allclose(got.entropy.double(), -(logp.exp() * logp).sum(-1), rtol=0, atol=2.0 ** -14)
+
+
+@pytest.mark.parametrize('form', ['symmetric', 'asymmetric', 'static'])
+def test_a_container_around_saved_buffers(dev, form):
+    x = torch.randn(5, 64, generator=gen(41)).to(BF).to(dev)
+    w = torch.randint(-127, 128, (24, 64), generator=gen(42), dtype=torch.int8).to(dev)
+    ws, b = torch.rand(24, 1, generator=gen(43)).to(BF).to(dev), torch.randn(24, generator=gen(44)).to(BF).to(dev)
+    scale = torch.tensor([0.02], device=dev) if form == 'static' else None
+    c = VllmRealQuantLinear(w, b, ws, scale, False, 'weight_scale')
+    c.act_form = form
+    assert torch.equal(c(x), int8_linear(x, w, ws, b, form != 'asymmetric', scale))
+    assert torch.equal(copy.deepcopy(c)(x), c(x))
