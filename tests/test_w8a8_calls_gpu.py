@@ -140,3 +140,47 @@ def test_a_container_around_saved_buffers(dev, form):
     c.act_form = form
     assert torch.equal(c(x), int8_linear(x, w, ws, b, form != 'asymmetric', scale))
     assert torch.equal(copy.deepcopy(c)(x), c(x))
+
+
+# -- graphs -------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('symmetric', [True, False])
+def test_graphs_whose_products_have_workspaces(dev, symmetric):
+    """Products that cut K, that pad their rows and both, and a Linear with its codes: each needs a workspace (asserted), in graphs of their
+    own, replayed beside each other with eager calls of the same between the replays."""
+    N, cases = 200, ((40, 4096, 'cut'), (100, 4096, 'cut'), (70, 4097, 'pad'), (37, 9, 'pad'), (150, 512, 'linear'))
+    lib, inputs = L.lib(), []
+    for M, K, kind in cases:
+        g = gen(M)
+        x = (torch.randn(M, K, generator=g) + 0.3).to(BF).to(dev)
+        w = torch.randint(-127, 128, (N, K), generator=g, dtype=torch.int8).to(dev)
+        ws, b = torch.rand(N, generator=g).to(dev), torch.randn(N, generator=g).to(dev)
+        inputs.append((kind, x, quantize_tokens(x, symmetric), w, ws, b))
+        entry = lib.lcq_int8_linear_workspace_bytes if kind == 'linear' else lib.lcq_int8_matmul_workspace_bytes
+        assert entry(M, N, K) > 0
+        assert kind != 'pad' or entry(M, N, K) >= (M + N) * ((K + 15) // 16 * 16)
+
+    def call(kind, x, q, w, ws, b):
+        return int8_linear(x, w, ws, b, symmetric, out_dtype=F32) if kind == 'linear' else int8_matmul(q, w, ws, b, out_dtype=F32)
+
+    want = [call(*i) for i in inputs]
+    for (kind, x, q, w, ws, b), y in zip(inputs, want):                      # exact sums; their conversion, as ws and the fma round
+        z = torch.zeros_like(q.scales) if q.zeros is None else q.zeros
+        s = (q.codes.double() - z.double()) @ w.double().t() * q.scales.double() * ws.double()
+        assert bool(((y.double() - (s + b.double())).abs() <= 2.0 ** -22 * s.abs() + 2.0 ** -23 * b.double().abs()).all())
+    graphs, outs = [], []
+    for i in inputs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(call(*i))
+    streams = [torch.cuda.Stream() for _ in inputs]
+    for rep in range(5):
+        for o in outs:
+            o.zero_()
+        eager = [call(*i) for i in inputs]
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        eager += [call(*i) for i in inputs]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want + want, eager)) and all(torch.equal(a, b) for a, b in zip(want, outs)), rep
