@@ -475,7 +475,7 @@ int lcq_quant_tokens(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx
 
 /* y[m, n] = as[m] * ws[n] * (sum_k a[m, k] w[n, k] - az[m] * sum_k w[n, k]) + bias[n]: the product of int8 codes with a scale for
  * each token and each channel.  The sums are exact integers; the factors and the bias are applied in fp32, y is rounded once.
- *  a       [M, K] int8, as [M] fp32 (or [1] with a_scalar), az [M] int32 within +-128 or NULL
+ *  a       [M, K] int8, as [M] fp32 (or [1] with a_scalar), az [M] int32, -128 .. 127, or NULL (128 at K = 65536 could give 2^31)
  *  w       [N, K] int8, ws [N] of ws_dtype (or [1] with w_scalar), bias [N] of bias_dtype or NULL;  K <= 65536; M <= 2^28, N <= 2^28 - 16 (2^27 - 16 for K > 8192)
  *          (a and w on 16 bytes where K is a multiple of 16; rows of other widths may start anywhere: for many tokens they are
  *          copied to padded rows in the workspace)

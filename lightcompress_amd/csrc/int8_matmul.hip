@@ -1,6 +1,6 @@
 // Product of int8 codes with a scale for each token and each channel:
 //   y[m, n] = as[m] ws[n] (sum_k a[m, k] w[n, k] - az[m] sum_k w[n, k]) + bias[n]
-// The sums are exact in 32-bit integers for K <= 65536 (|a - az| <= 255, |w| <= 128: 255 * 128 * 65536 < 2^31), so results do not
+// The sums are exact in 32-bit integers for K <= 65536 (-128 <= az <= 127, so |a - az| <= 255; |w| <= 128: 255 * 128 * 65536 < 2^31), so results do not
 // depend on how the work is cut.
 //
 // Both operands are read along K, as the matrix pipe takes them: a lane of v_mfma_i32_32x32x32_i8 holds 16 codes of one row.

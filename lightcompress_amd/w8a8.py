@@ -21,7 +21,7 @@ MOST_COLS = 65536
 
 
 class QuantizedTokens(NamedTuple):
-    """(codes - zeros) * scales stands for the tokens."""
+    """(codes - zeros) * scales stands for the tokens; zero points are within -128 .. 127."""
     codes: torch.Tensor                       # int8 [..., K]
     scales: torch.Tensor                      # fp32 [..., 1], or one for all tokens
     zeros: Optional[torch.Tensor] = None      # int32 [..., 1]; None: 0

@@ -142,6 +142,17 @@ def test_a_container_around_saved_buffers(dev, form):
     assert torch.equal(copy.deepcopy(c)(x), c(x))
 
 
+@pytest.mark.parametrize('M', [1, 20, 70])
+@pytest.mark.parametrize('code,weight,zero', [(127, -128, -128), (-128, -128, 127), (-128, 127, 127), (127, 127, -128)])
+def test_both_ends_of_the_zero_points(dev, M, code, weight, zero):
+    """The largest and the smallest sums that zero points of -128 .. 127 allow, at the longest K: 255 * 128 * 65536 < 2^31."""
+    K, N = 65536, 24
+    q = QuantizedTokens(torch.full((M, K), code, dtype=torch.int8, device=dev), torch.ones(M, 1, device=dev),
+                        torch.full((M, 1), zero, dtype=torch.int32, device=dev))
+    y = int8_matmul(q, torch.full((N, K), weight, dtype=torch.int8, device=dev), torch.ones(1, device=dev), out_dtype=F32)
+    assert bool((y == float((code - zero) * weight * K)).all())              # (a multiple of 2^16 below 2^31: exact in fp32)
+
+
 # -- graphs -------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize('symmetric', [True, False])
 def test_graphs_whose_products_have_workspaces(dev, symmetric):
