@@ -333,6 +333,7 @@ __global__ __launch_bounds__(256) void join_kernel(MatmulArgs g, const int* __re
 // than another kernel in front (6.4 us at N = K = 4096, the quantizer alone 3.4).
 constexpr int PIECE = 256;
 constexpr int64_t MOST_FUSED = 32768;               // codes of a token that is quantized in LDS
+constexpr int MOST_TOKENS = 8;                      // that every workgroup quantizes itself
 
 struct TokenArgs {
   const void* x;
@@ -439,15 +440,15 @@ __device__ __forceinline__ i32x4 later(i32x4 v, int codes) {
   return __builtin_bit_cast(i32x4, h);
 }
 
-// TB blocks of 16 tokens, NB blocks of 16 channels.  XT: the type of the tokens' values (one token, or MANY of up to 16: a wave quantizes a
-// row at a time), or -1 for codes.
+// TB blocks of 16 tokens, NB blocks of 16 channels.  XT: the type of the tokens' values (one token, or MANY of up to MOST_TOKENS: a wave quantizes
+// a row at a time), or -1 for codes.
 // ODD: rows start on any byte (K >= 16).  16 codes are cut from the five words that hold them, which costs far less than loads off word
 // alignment (K = 4097, N = 14336, 16 tokens: 25.5 us for 66; 38 by padded copies); a row's last codes are read from K - 16 and moved.
 template <int TB, int NB, int BF, int XT, int WAVES, bool ODD, bool MANY>
 __global__ __launch_bounds__(WAVES * 64) void stream_kernel(MatmulArgs g, TokenArgs t) {
   __shared__ __attribute__((aligned(16))) int red[WAVES][NB][TB + 1][64][4];
-  __shared__ float token_scale[MANY ? 16 : 1];
-  __shared__ int token_zero[MANY ? 16 : 1];
+  __shared__ float token_scale[MANY ? MOST_TOKENS : 1];
+  __shared__ int token_zero[MANY ? MOST_TOKENS : 1];
   extern __shared__ __attribute__((aligned(16))) int8_t codes[];             // XT >= 0: [M] rows, K + 16 apart (16 lanes' reads touch all banks once)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t n0 = (int64_t)blockIdx.x * (16 * NB);
@@ -720,7 +721,7 @@ bool pads(int64_t K, bool streams) { return K % 16 != 0 && (!streams || K < 16);
 bool fused(int64_t M, int64_t N, int64_t K) {
   if (K % 16) return false;
   const int64_t rows = (M + 3) / 4;                 // of a wave
-  return M == 1 ? K <= MOST_FUSED : M <= 8 && N <= 4096 && rows * rows * K <= 4096;
+  return M == 1 ? K <= MOST_FUSED : M <= MOST_TOKENS && N <= 4096 && rows * rows * K <= 4096;
 }
 
 }  // namespace
