@@ -255,12 +255,16 @@ def residual_norm(x, residual=None, weight=None, bias=None, *, gate=None, post_w
     flags = NORM_LAYER if kind == 'layer' else 0
     if weight is not None:
         flags |= _affine('weight', weight, K, dtype, NORM_WEIGHT_F32)
+        weight = _whole(weight)
     if bias is not None:
         flags |= _affine('bias', bias, K, dtype, NORM_BIAS_F32)
+        bias = _whole(bias)
     if post_weight is not None:
         flags |= _affine('post_weight', post_weight, K, dtype, NORM_POST_WEIGHT_F32)
+        post_weight = _whole(post_weight)
     if post_bias is not None:
         flags |= _affine('post_bias', post_bias, K, dtype, NORM_POST_BIAS_F32)
+        post_bias = _whole(post_bias)
     stream_dtype = dtype
     if residual is not None:
         if residual.shape != shape:
@@ -299,7 +303,6 @@ def residual_norm(x, residual=None, weight=None, bias=None, *, gate=None, post_w
         res, _, ldr = _rows(residual, K)
     if gate is not None:
         g, _, ldg = (_whole(gate), 1, 0) if gate.dim() == 1 else _rows(gate, K)
-    weight, bias, post_weight, post_bias = _whole(weight), _whole(bias), _whole(post_weight), _whole(post_bias)
     h = residual if inplace else _like(x, stream_dtype)
     out = codes = scales = zeros = None
     if quantize is None:
