@@ -469,7 +469,8 @@ int lcq_clamp_groups(const void* w, int dtype, int64_t R, int64_t K, int group_s
  *  scale   NULL: s = max(max|x|, 1e-5) / 127 per row, or with `asym` s = max(max x - min x, 1e-5) / 255 and
  *          z = clamp(-128 - rint(min x / s), -128, 127); else one fp32 scale for all rows (static activations; not `asym`)
  *  codes   [T, K] int8: clamp(rint(x / s) + z, -128, 127);  scales [T] fp32, zeros [T] int32 (`asym`): output
- * A row with an infinity or a NaN gets a scale that is not finite, and with it every product of that row. */
+ * A row with an infinity or a NaN, or (`asym`) a range that overflows, gets a scale that is not finite, and with it every product of that row.  With a given
+ * scale nothing carries that: infinities saturate and a NaN becomes -128. */
 int lcq_quant_tokens(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, int asym, const float* scale, int8_t* codes,
                      float* scales, int32_t* zeros, void* stream);
 

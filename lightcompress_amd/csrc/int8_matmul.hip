@@ -718,6 +718,7 @@ bool pads(int64_t K, bool streams) { return K % 16 != 0 && (!streams || K < 16);
 // CUs make them.  One launch instead of two costs the host 4 us less; on the GPU it takes, with the quantizer's launch beside it, us:
 //   N = K = 4096, 4 tokens 9.6 / 9.7     K = 1024, 4 tokens 5.4 / 6.1, 8 tokens 6.9 / 6.6     K = 2048, 8 tokens 8.8 / 7.0 (by itself)
 //   N = 14336, K = 4096, 4 tokens 21.1 / 17.7 and N = 1024, K = 8192, 2 tokens 13.3 / 10.5 (by itself both)
+// The rule goes by a call from Python, whose host time is the longer at these sizes; in a captured graph 8 tokens at K = 1024 lose the 0.3 us of the table.
 bool fused(int64_t M, int64_t N, int64_t K) {
   if (K % 16) return false;
   const int64_t rows = (M + 3) / 4;                 // of a wave

@@ -4,15 +4,17 @@
 //
 //  * A lane keeps its own c, S and U.  c is a logit that the lane has seen; it moves only where a later one is more than 8 above
 //    it, so that almost no piece pays for a change of reference, S stays below V e^8 and log S and U / S do not cancel to more than a few
-//    times their last bits.  References meet once, when lanes, waves and parts are joined.
+//    times their last bits.  References meet once, when lanes and waves are joined.
 //  * The best alternatives cost the pass one comparison per piece: a lane keeps the largest logit of each 8th (12th) of the pass.  Behind it, the k-th
 //    largest of all lanes' maxima is a bound that k logits reach, few more do, and only those parts of a lane's logits that reach it are read
 //    again for the keys of those logits, which one wave sorts.  A key is a whole number that orders by value and then by the lowest index.  Where
-//    more keys reach the bound than there is room for (ties: constant rows, rows masked but for fewer than k), every wave finds its best
-//    by itself.
-//  * Bound by HBM where there are many rows: 2048 x 128256 bf16 with their best 5 in 112 us (4.7 TB/s); a row alone takes 15 us with its best 20, 6 of them
+//    more keys reach the bound than there is room for, every wave finds its best by itself from a third reading: ties (constant rows), and masks
+//    that leave finite logits to fewer than k lanes - fewer than k of them, or neighbours (30 in a row are 4 or 5 lanes' in bf16) -, whose bound is
+//    -inf.  Such a row of 128256 bf16 takes 74 us with its best 20, an ordinary one 16; 64 of either side by side 76 and 17.6.
+//  * Bound by HBM where there are many rows: 2048 x 128256 bf16 with their best 5 in 112 us (4.7 TB/s); a row alone takes 16 us with its best 20, 6 of them
 //    behind the pass.  333 x 50001 fp32, best 10: 18.4 us.
-//  * A row is one workgroup's: of 1024 lanes where there are at most as many rows as CUs, of 512 or 256 where there are more.
+//  * A row is one workgroup's: of 1024 lanes where there are at most as many rows as CUs, of 512 or 256 where there are more.  A row in parts and a
+//    second kernel that joins them took 11.6 us of the GPU and 19.1 a call from Python, whose host time is then the longer; one kernel takes 16 of both.
 #include "rowquant.h"
 #include <type_traits>
 

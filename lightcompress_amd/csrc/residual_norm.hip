@@ -13,7 +13,7 @@
 // granularity per_token, codes moved to int8 (its unsigned codes less 128).
 //
 // A row stays in the registers of 64 to 1024 lanes, 16 values per lane for most widths, so every operand is read once.  Bound by HBM: 8192 x 4096
-// bf16 with residual and weight 46 us (5.8 TB/s read and written; a copy runs at 5.1), with codes for values 45, the codes alone 20.5; 16384 x 4096 with
+// bf16 with residual and weight 46 us (5.8 TB/s read and written; a copy runs at 5.1), with codes for values 45, the codes alone 20 one after another (24 to 26 a launch by itself); 16384 x 4096 with
 // two norms and a gate 119 us (5.6 TB/s).  Rows of 4096 on one wave took 60 us for these 46, on two 51; nontemporal loads 51.
 #include "rowquant.h"
 #include "token_codes.h"
