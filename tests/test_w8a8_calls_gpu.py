@@ -130,6 +130,30 @@ def test_sequences_against_the_formula(dev):
     assert torch.allclose(got.entropy.double(), -(logp.exp() * logp).sum(-1), rtol=0, atol=2.0 ** -14)
 
 
+def test_sequences_behind_two_to_the_31_and_captured(dev):
+    """The last rows of the third of three sequences whose logits start behind 2^31 elements; the same bits from a graph."""
+    B, S, V = 3, 9001, 128256
+    x = torch.zeros(B, S, V, dtype=BF, device=dev)
+    x[2, -4:] = (torch.randn(4, V, generator=gen(51)) * 3).to(BF).to(dev)
+    t = torch.full((B, S - 1), 7, dtype=torch.int64, device=dev)
+    got = token_logprobs(x[:, :-1], t, top=3)
+    logp = torch.log_softmax(x[2, -4:-1].double(), -1)
+    # V terms in 256 lanes, 501 one after another, and joins: 2^-24 each on numbers of at most 32; exponentials 2^-22: below 2^-14
+    assert torch.allclose(got.logprobs[2, -3:].double(), logp[:, 7], rtol=0, atol=2.0 ** -14)
+    assert torch.equal(got.top_tokens[2, -3:], torch.sort(x[2, -4:-1].double(), dim=-1, descending=True, stable=True).indices[:, :3])
+    assert bool((got.top_tokens[:2] == torch.arange(3, device=dev)).all()) and bool((got.top_tokens[2, :-3] == torch.arange(3, device=dev)).all())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = token_logprobs(x[:, :-1], t, top=3)
+    for rep in range(3):
+        x[1, 5 + rep].normal_()
+        want = token_logprobs(x[:, :-1], t, top=3)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same(out, want), rep
+
+
 @pytest.mark.parametrize('form', ['symmetric', 'asymmetric', 'static'])
 def test_a_container_around_saved_buffers(dev, form):
     x = torch.randn(5, 64, generator=gen(41)).to(BF).to(dev)
