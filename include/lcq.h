@@ -535,6 +535,35 @@ int lcq_token_logprobs_of(const void* logits, int dtype, int64_t B, int64_t S, i
                           int64_t m, int64_t ignore, float* logprobs, float* entropy, int k, float* top_logprobs, int64_t* top_tokens,
                           void* stream);
 
+/* ---- microscaled 4-bit numbers (MXFP4) ------------------------------------
+ * Blocks of 32 values along a row: e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign), two to a byte, the lower half first, and one E8M0 scale
+ * byte s per block, for 2^(s - 127) (255: NaN).  A row of K values has B = ceil(K / 32) blocks: 16 B bytes of codes, zeros behind K, and
+ * B of scales. */
+
+/* The codes of rows of values.  A block's scale is 2^(floor(log2 max|x|) - 2), at least 2^-127; codes are the nearest, ties to the even one,
+ * saturated at 6.  A block with an infinity or a NaN gets scale 255 and codes 0.
+ *  x       [rows, K] of `dtype`, rows `ldx` elements apart
+ *  codes   [rows, 16 B], 4-byte aligned;  scales [rows, B], rows `lds` bytes apart: output */
+int lcq_mxfp4_quant(const void* x, int dtype, int64_t rows, int64_t K, int64_t ldx, uint8_t* codes, uint8_t* scales, int64_t lds, void* stream);
+
+/* What codes (rows ldc bytes apart, a multiple of 4) and scales (rows lds apart) stand for: y [rows, K] of `dtype`, rounded once (fp32 and bf16 hold every value). */
+int lcq_mxfp4_dequant(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, int64_t rows, int64_t K, void* y, int dtype, void* stream);
+
+/* y[m, n] = sum_k a[m, k] w[n, k] + bias[n] of such rows: products exact, sums in fp32, rounded once.
+ *  a, w    codes [M, 16 B] and [N, 16 B], rows lda / ldw bytes apart, all on 16 bytes;  sa, sw scales, rows ldsa / ldsw apart.  Distances up to 2^22
+ *  bias    [N] of bias_dtype or NULL;  y [M, N] of `dtype`;  K <= 65536, M <= 2^28, N <= 2^28 - 16
+ *  workspace of lcq_mxfp4_matmul_workspace_bytes(M, N, K) (0: none), 16-byte aligned. */
+int64_t lcq_mxfp4_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int lcq_mxfp4_matmul(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t ldsa, const uint8_t* w, int64_t ldw, const uint8_t* sw,
+                     int64_t ldsw, const void* bias, int bias_dtype, int64_t M, int64_t N, int64_t K, void* y, int dtype, void* workspace,
+                     void* stream);
+
+/* lcq_mxfp4_quant of x [M, K] (x_dtype, rows ldx elements apart), then lcq_mxfp4_matmul.
+ *  workspace of lcq_mxfp4_linear_workspace_bytes(M, N, K) (0: none), 16-byte aligned. */
+int64_t lcq_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int lcq_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w, int64_t ldw, const uint8_t* sw, int64_t ldsw, const void* bias,
+                     int bias_dtype, int64_t M, int64_t N, int64_t K, void* y, int dtype, void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
