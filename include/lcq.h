@@ -564,6 +564,40 @@ int64_t lcq_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int lcq_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w, int64_t ldw, const uint8_t* sw, int64_t ldsw, const void* bias,
                      int bias_dtype, int64_t M, int64_t N, int64_t K, void* y, int dtype, void* workspace, void* stream);
 
+/* ---- experts of microscaled 4-bit numbers ---------------------------------- */
+
+/* The experts of each token and their weights.
+ *    score = softmax(logits), LCQ_ROUTE_SIGMOID: 1 / (1 + e^-logit);   the `top` largest logits are chosen, with a correction the largest
+ *    fp32(score) + correction; equal ones by the lowest index, NaN first, -inf last (score 0)
+ *    weight = score, LCQ_ROUTE_RENORMALIZE: over the sum of the chosen (0 where that is 0);   times scale
+ *  logits  [T, E] of `dtype`, rows ldl elements apart;  E <= 1024, top <= min(E, 32), T <= 2^25
+ *  correction [E] fp32 or NULL;  experts [T, top] int32, weights [T, top] fp32: output, best first */
+#define LCQ_ROUTE_SIGMOID 1
+#define LCQ_ROUTE_RENORMALIZE 2
+int lcq_route(const void* logits, int dtype, int64_t T, int64_t E, int64_t ldl, int top, int flags, const float* correction, float scale, int* experts,
+              float* weights, void* stream);
+
+/* A mixture-of-experts layer for a few tokens, the experts in microscaled 4-bit numbers, sums in fp32:
+ *    y[t] = sum_s weight[t, s] (down_e (act(gate_e x[t] + b) * (up_e x[t] + b)) + b),  e = expert[t, s]
+ *  x       [T, K] of `dtype`, rows ldx elements apart.  Any T; 128 tokens share a pass over the experts' bytes
+ *  logits  [T, E] (logits_dtype, ldl) with flags, correction and scale of lcq_route, and experts, weights NULL; or
+ *  experts [T, top] int32, weights [T, top] fp32 (logits NULL): an index outside 0 .. E - 1 is no expert, several of the same of a token count
+ *          as one with the sum of their weights
+ *  gate_up [E, 2 I, 16 ceil(K / 32)]: the gates' rows, then the ups'; from an expert gate_up_lde, from a row gate_up_ld bytes to the next, all on 16
+ *          bytes; gate_up_scales with gate_up_ldse, gate_up_lds.  down [E, N, 16 ceil(I / 32)] the same.  Row distances up to 2^22
+ *  gate_up_bias [E, 2 I], down_bias [E, N] of bias_dtype, or NULL;  y [T, N] of out_dtype;  K, I, N <= 65536
+ *  workspace of lcq_mxfp4_moe_workspace_bytes(T, top, K, I), 16-byte aligned.
+ * An expert whose weight is 0 is not asked (its infinities and NaN do not reach y); a token without experts gives 0. */
+#define LCQ_ACT_SILU 0
+#define LCQ_ACT_GELU 1
+int64_t lcq_mxfp4_moe_workspace_bytes(int64_t T, int64_t top, int64_t K, int64_t I);
+int lcq_mxfp4_moe(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, const void* logits, int logits_dtype, int64_t ldl, int flags,
+                  const float* correction, float scale, const int* experts, const float* weights, int64_t E, int top, const uint8_t* gate_up,
+                  int64_t gate_up_lde, int64_t gate_up_ld, const uint8_t* gate_up_scales, int64_t gate_up_ldse, int64_t gate_up_lds,
+                  const void* gate_up_bias, const uint8_t* down, int64_t down_lde, int64_t down_ld, const uint8_t* down_scales, int64_t down_ldse,
+                  int64_t down_lds, const void* down_bias, int bias_dtype, int64_t I, int64_t N, int activation, void* y, int out_dtype,
+                  void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

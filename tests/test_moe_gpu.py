@@ -1,0 +1,312 @@
+"""The router, a mixture-of-experts layer on MXFP4 experts and their run together, against the definitions in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from lightcompress_amd._lib import LcqError
+from lightcompress_amd.moe import Router, Routing, mxfp4_moe, route_tokens
+from lightcompress_amd.mxfp4 import Mxfp4, mxfp4_linear, quantize_mxfp4
+from lightcompress_amd.w8a8 import residual_norm
+from tests.test_mxfp4_gpu import half_step, gpu_gen, random_mx, values
+
+pytestmark = pytest.mark.gpu
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+f64 = torch.float64
+U = 2.0 ** -24
+
+
+# -- the router -----------------------------------------------------------------------------------------------------
+def routed(logits, top, scoring, renormalize, correction, scale):
+    """The definition in 64 bits; with a correction scores are rounded to fp32 and summed there, as the definition says."""
+    x = logits.to(f64)
+    if scoring == 'softmax':
+        m = x.amax(-1, keepdim=True)
+        e = torch.where(torch.isneginf(x), 0.0, torch.exp(x - torch.where(torch.isneginf(m), 0.0, m)))
+        total = e.sum(-1, keepdim=True)
+        scores = torch.where(total == 0, 0.0, e / total)
+    else:
+        scores = torch.sigmoid(x)
+    by = x if correction is None else (scores.float() + correction).to(f64)
+    by = torch.where(torch.isneginf(x), -math.inf, by)
+    order = torch.sort(by, dim=-1, descending=True, stable=True).indices[..., :top]
+    w = torch.take_along_dim(scores, order, -1)
+    if renormalize:
+        total = w.sum(-1, keepdim=True)
+        w = torch.where(total == 0, 0.0, w / total)
+    return order, w * scale
+
+
+@pytest.mark.parametrize('scoring,renormalize,corrected,scale', [('softmax', True, False, 1.0), ('softmax', False, False, 1.0), ('softmax', True, True, 2.5),
+                                                                 ('sigmoid', True, True, 2.5), ('sigmoid', False, False, 0.5)])
+@pytest.mark.parametrize('dtype', [F32, BF, HF])
+@pytest.mark.parametrize('T,E,top', [(1, 1, 1), (1, 8, 2), (3, 63, 5), (5, 64, 64 // 2), (7, 65, 3), (2, 256, 8), (33, 257, 4), (4, 1000, 32), (2, 1024, 16),
+                                     (1000, 60, 6)])
+def test_route(dev, T, E, top, dtype, scoring, renormalize, corrected, scale):
+    """Scores: exp, sum and quotient in fp32, 1 / (1 + exp) alike, each step within a few U; sums of E numbers in a tree of 16 + 6 steps
+    at most.  16-bit logits have many ties."""
+    g = gpu_gen(T + E)
+    x = (2 * torch.randn(T, E, generator=g, device=dev)).to(dtype)
+    x[0, E // 2] = -math.inf
+    if T > 2:
+        x[1] = -math.inf
+        x[2] = x[2, 0]
+    c = 0.3 * torch.randn(E, generator=g, device=dev) if corrected else None
+    got = route_tokens(Router(x, top, scoring, renormalize, c, scale))
+    experts, weights = routed(x, top, scoring, renormalize, c, scale)
+    assert got.experts.dtype == torch.int32 and got.weights.dtype == F32
+    assert torch.equal(got.experts.long(), experts)
+    assert bool(((got.weights.to(f64) - weights).abs() <= 64 * U * weights + 1e-37).all())
+    if T > 2:
+        assert bool((got.weights[1] == 0).all()) and torch.equal(got.experts[1].long(), torch.arange(top, device=dev))
+
+
+def test_route_of_logits_apart(dev):
+    g = gpu_gen(5)
+    big = torch.randn(6, 4, 100, generator=g, device=dev)
+    for view in (big[..., :64], big[:, 1:3, 3:90], big[:, 0], big.transpose(0, 1), big[:1].expand(3, 4, 100)):
+        a, b = route_tokens(Router(view, 3)), route_tokens(Router(view.contiguous(), 3))
+        assert torch.equal(a.experts, b.experts) and torch.equal(a.weights, b.weights) and a.experts.shape == (*view.shape[:-1], 3)
+
+
+def test_nan_logits_come_first_and_spoil_their_token(dev):
+    x = torch.randn(3, 20, generator=gpu_gen(1), device=dev)
+    x[1, 7] = math.nan
+    got = route_tokens(Router(x, 2))
+    assert int(got.experts[1, 0]) == 7 and bool(torch.isnan(got.weights[1]).all()) and bool(torch.isfinite(got.weights[[0, 2]]).all())
+
+
+def test_route_refusals(dev):
+    x = torch.zeros(3, 20, device=dev)
+    for bad in (Router(x, 0), Router(x, 21), Router(x, 2, 'tanh'), Router(x, 2, correction=torch.zeros(19, device=dev)),
+                Router(torch.zeros(2, 1025, device=dev), 2), Router(torch.zeros(2, 64, device=dev), 33), Router(torch.zeros(2, 0, device=dev), 1)):
+        with pytest.raises(ValueError):
+            route_tokens(bad)
+    for bad in (Router(x.to(torch.int32), 2), Router(x, 2, correction=torch.zeros(20, device=dev, dtype=BF)), Router(x.cpu(), 2),
+                Router(x, 2, correction=torch.zeros(20))):
+        with pytest.raises(LcqError):
+            route_tokens(bad)
+    assert route_tokens(Router(x[:0], 2)).experts.shape == (0, 2)
+
+
+# -- the layer ------------------------------------------------------------------------------------------------------
+def experts_of(E, rows, K, g, dev):
+    """Random experts, their columns' values around 2^-5 / sqrt(K)-ish: scales 2^-9 .. 2^-5."""
+    q = random_mx(E * rows, K, g, dev, 118, 122)
+    return Mxfp4(q.codes.view(E, rows, -1), q.scales.view(E, rows, -1), K)
+
+
+def layer(x, experts, weights, gate_up, down, gb, db, activation):
+    """y in 64 bits, and bounds: |x| through the magnitudes of the weights, for errors that are relative to what was summed.
+
+    size of gate and up: sum |w| |x|.  An error d of gate moves act by at most 1.2 |d| (the slopes of silu and gelu are below 1.13), one of
+    up moves the product by |act| |d|, and down carries both on through its magnitudes."""
+    T = x.shape[0]
+    E, N, I = down.codes.shape[0], down.codes.shape[1], down.cols
+    y, size, moved = (torch.zeros(T, N, dtype=f64, device=x.device) for _ in range(3))
+    xs = x.to(f64)
+    for e in range(E):
+        t, s = (experts == e).nonzero(as_tuple=True)
+        if not len(t):
+            continue
+        wt = weights[t, s].to(f64)[:, None]
+        wg, wd = values(Mxfp4(gate_up.codes[e], gate_up.scales[e], gate_up.cols)), values(Mxfp4(down.codes[e], down.scales[e], down.cols))
+        v, sv = xs[t] @ wg.t(), xs[t].abs() @ wg.abs().t()
+        if gb is not None:
+            v, sv = v + gb[e].to(f64), sv + gb[e].to(f64).abs()
+        a = torch.nn.functional.silu(v[:, :I]) if activation == 'silu' else torch.nn.functional.gelu(v[:, :I])
+        h = a * v[:, I:]
+        o, so = h @ wd.t(), h.abs() @ wd.abs().t()
+        if db is not None:
+            o, so = o + db[e].to(f64), so + db[e].to(f64).abs()
+        d = 1.2 * sv[:, :I] * v[:, I:].abs() + a.abs() * sv[:, I:]                         # per unit of relative error of the first sums
+        y.index_add_(0, t, wt * o)
+        size.index_add_(0, t, wt.abs() * so)
+        moved.index_add_(0, t, wt.abs() * (d @ wd.abs().t()))
+    return y, size, moved
+
+
+def check_layer(got, dtype, x, experts, weights, gate_up, down, gb, db, activation, weight_error=0.0):
+    y, size, moved = layer(x, experts, weights, gate_up, down, gb, db, activation)
+    K, I, E = gate_up.cols, down.cols, down.codes.shape[0]
+    # sums in fp32: a step per 32 codes and plane, and those of the waves; the activation's few steps; planes of h: 2^-17 (fp32 tokens 2^-24);
+    # fp32 tokens in three planes: 2^-24; the weighted sums of the experts
+    planes = {BF: 1, HF: 2, F32: 3}[x.dtype]
+    first = (planes * K / 32 + 16) * 2.0 ** -23 + (2.0 ** -23 if x.dtype == F32 else 0)
+    second = (3 * I / 32 + 64) * 2.0 ** -23 + (2.0 ** -23 if x.dtype == F32 else 2.0 ** -17) + (E + 16) * 2.0 ** -23 + weight_error
+    err32 = first * moved + second * size
+    tol = err32 + half_step(dtype) * (y.abs() + err32) + (2.0 ** -25 if dtype == HF else 2.0 ** -140)
+    err = (got.to(f64) - y).abs()
+    assert bool((err <= tol).all()), f'{float((err / tol).max())} of the tolerance'
+    # and not by the slack of the bound alone: the typical error is a rounding of the output
+    assert float(err.norm()) <= 2.0 * float((half_step(dtype) + 4 * 2.0 ** -17 * (x.dtype != F32) + 2.0 ** -20) * y.norm()) + 1e-30
+
+
+@pytest.mark.parametrize('dtype', [BF, HF, F32])
+@pytest.mark.parametrize('T,E,top,K,I,N,bias,activation', [
+    (1, 8, 2, 256, 128, 256, False, 'silu'), (1, 256, 8, 1024, 256, 1024, False, 'silu'), (2, 4, 4, 64, 32, 64, True, 'gelu'), (3, 7, 3, 100, 70, 90, True, 'silu'),
+    (16, 64, 8, 512, 160, 512, False, 'silu'), (17, 5, 2, 4096, 96, 33, True, 'silu'), (33, 6, 6, 130, 50, 17, True, 'gelu'), (64, 32, 4, 264, 512, 264, False, 'silu'),
+    (50, 8, 2, 1000, 1408, 1000, True, 'silu'), (128, 3, 2, 96, 96, 96, False, 'silu'), (129, 5, 3, 160, 40, 100, True, 'silu'), (300, 4, 2, 64, 64, 64, False, 'gelu'),
+    (1, 1, 1, 1, 1, 1, True, 'silu'), (5, 1000, 32, 64, 33, 40, False, 'silu'), (4, 12, 3, 7168, 64, 96, False, 'silu'), (7, 12, 3, 64, 4096, 48, True, 'silu'),
+    (200, 1, 1, 33, 65, 31, True, 'silu')])
+def test_layer(dev, T, E, top, K, I, N, bias, activation, dtype):
+    g = gpu_gen(T + E + K)
+    x = torch.randn(T, K, generator=g, device=dev).to(dtype)
+    gate_up, down = experts_of(E, 2 * I, K, g, dev), experts_of(E, N, I, g, dev)
+    gb = (0.2 * torch.randn(E, 2 * I, generator=g, device=dev)).to(dtype) if bias else None
+    db = (0.2 * torch.randn(E, N, generator=g, device=dev)).to(dtype) if bias else None
+    router = Router(torch.randn(T, E, generator=g, device=dev), top)
+    r = route_tokens(router)
+    got = mxfp4_moe(x, r, gate_up, down, gate_up_bias=gb, down_bias=db, activation=activation)
+    assert got.dtype == dtype and got.shape == (T, N)
+    check_layer(got, dtype, x, r.experts, r.weights, gate_up, down, gb, db, activation)
+    assert torch.equal(mxfp4_moe(x, router, gate_up, down, gate_up_bias=gb, down_bias=db, activation=activation), got)      # the same choices, the same weights
+    wide = mxfp4_moe(x, r, gate_up, down, gate_up_bias=gb, down_bias=db, activation=activation, out_dtype=F32)
+    assert torch.equal(wide.to(dtype), got)
+
+
+@pytest.mark.parametrize('T,crowd', [(20, 20), (64, 60), (128, 128), (100, 33)])
+def test_tokens_that_crowd_one_expert(dev, T, crowd):
+    """More than 16 tokens of one expert, beside lonely ones."""
+    g = gpu_gen(T)
+    E, K, I, N = 9, 224, 80, 112
+    x = torch.randn(T, K, generator=g, device=dev).to(BF)
+    gate_up, down = experts_of(E, 2 * I, K, g, dev), experts_of(E, N, I, g, dev)
+    experts = torch.randint(0, E, (T, 2), generator=g, device=dev, dtype=torch.int32)
+    experts[:, 1] = (experts[:, 0] + 1) % E
+    experts[:crowd, 0], experts[:crowd, 1] = 4, 7
+    weights = torch.rand(T, 2, generator=g, device=dev)
+    check_layer(mxfp4_moe(x, Routing(experts, weights), gate_up, down), BF, x, experts, weights, gate_up, down, None, None, 'silu')
+
+
+def test_given_choices_none_twice_and_of_no_weight(dev):
+    """No expert, an expert out of range, one expert several times, weights of 0: a token of nothing gives zeros; an expert of weight 0 is not
+    asked, whatever it holds."""
+    g = gpu_gen(7)
+    E, K, I, N = 6, 96, 64, 80
+    x = torch.randn(5, K, generator=g, device=dev).to(BF)
+    gate_up, down = experts_of(E, 2 * I, K, g, dev), experts_of(E, N, I, g, dev)
+    down.scales[5] = 255                           # this expert is NaN
+    experts = torch.tensor([[-1, 2, 2], [-1, 6, 1000000], [3, 5, 3], [1, 1, 1], [0, -7, 4]], dtype=torch.int32, device=dev)
+    weights = torch.tensor([[0.5, 0.25, 0.5], [1.0, 1.0, 1.0], [0.5, 0.0, -0.25], [0.5, -0.25, -0.25], [1.0, 3.0, 0.125]], device=dev)
+    got = mxfp4_moe(x, Routing(experts, weights), gate_up, down)
+    simple = torch.tensor([[2, 0], [0, 0], [3, 0], [0, 0], [0, 4]], dtype=torch.int32, device=dev)
+    sw = torch.tensor([[0.75, 0.0], [0.0, 0.0], [0.25, 0.0], [0.0, 0.0], [1.0, 0.125]], device=dev)
+    check_layer(got, BF, x, simple, sw, gate_up, down, None, None, 'silu')
+    assert bool((got[[1, 3]] == 0).all())
+    away = torch.full((5, E), -math.inf, device=dev)
+    assert bool((mxfp4_moe(x, Router(away, 2), gate_up, down) == 0).all())
+    away[2, 1] = 0.0
+    y = mxfp4_moe(x, Router(away, 2), gate_up, down)
+    assert bool((y[[0, 1, 3, 4]] == 0).all()) and bool(torch.isfinite(y).all()) and bool((y[2] != 0).any())
+
+
+@pytest.mark.parametrize('bad', [math.nan, math.inf])
+def test_a_token_that_is_not_finite_spoils_itself_alone(dev, bad):
+    g = gpu_gen(8)
+    E, K, I, N = 4, 96, 64, 80
+    gate_up, down = experts_of(E, 2 * I, K, g, dev), experts_of(E, N, I, g, dev)
+    for dtype in (BF, HF, F32):
+        x = torch.randn(6, K, generator=g, device=dev).to(dtype)
+        x[2, 50] = bad
+        logits = torch.randn(6, E, generator=g, device=dev)
+        y = mxfp4_moe(x, Router(logits, 3), gate_up, down)
+        assert not bool(torch.isfinite(y[2]).any()) and bool(torch.isfinite(y[[0, 1, 3, 4, 5]]).all())
+
+
+@pytest.mark.parametrize('dtype', [BF, F32])
+def test_operands_apart(dev, dtype):
+    g = gpu_gen(9)
+    E, K, I, N, T = 4, 96, 64, 80, 6
+    gate_up, down = experts_of(2 * E, 2 * I + 3, 2 * K, g, dev), experts_of(E + 1, 2 * N, I + 32, g, dev)
+    gu = Mxfp4(gate_up.codes[::2, 2:2 + 2 * I, 32:80], gate_up.scales[::2, 2:2 + 2 * I, 2:5])
+    dn = Mxfp4(down.codes[1:, ::2, 16:48], down.scales[1:, ::2, 1:3])
+    whole = lambda q: Mxfp4(q.codes.contiguous(), q.scales.contiguous())  # noqa: E731
+    x = torch.randn(3, 2, 2 * K, generator=g, device=dev).to(dtype)
+    logits = torch.randn(3, 2, 7, generator=g, device=dev)
+    want = mxfp4_moe(x[..., 5:5 + K].contiguous(), Router(logits[..., 1:5].contiguous(), 2), whole(gu), whole(dn))
+    assert torch.equal(mxfp4_moe(x[..., 5:5 + K], Router(logits[..., 1:5], 2), gu, dn), want) and want.shape == (3, 2, N)
+    x2 = x.view(6, 2 * K)
+    flat = mxfp4_moe(x2[:, 5:5 + K], Router(logits.view(6, 7)[:, 1:5], 2), gu, dn)
+    assert torch.equal(flat, want.view(6, N))
+    x3 = x2[:, 8:8 + K]                            # rows on 16 bytes
+    assert torch.equal(mxfp4_moe(x3, Router(logits.view(6, 7)[:, 1:5], 2), gu, dn), mxfp4_moe(x3.contiguous(), Router(logits.view(6, 7)[:, 1:5].contiguous(), 2), whole(gu), whole(dn)))
+
+
+def test_experts_behind_2_gigabytes(dev):
+    """Codes of the last experts lie behind 2^32 bytes."""
+    E, K, I, N, T = 300, 4096, 2048, 64, 3
+    g = gpu_gen(10)
+    gate_up, down = experts_of(E, 2 * I, K, g, dev), experts_of(E, N, I, g, dev)
+    assert gate_up.codes.numel() > 2 ** 31 and gate_up.codes[-1].data_ptr() - gate_up.codes.data_ptr() > 2 ** 31
+    x = torch.randn(T, K, generator=g, device=dev).to(BF)
+    experts = torch.tensor([[299, 0], [298, 299], [1, 150]], dtype=torch.int32, device=dev)
+    weights = torch.rand(T, 2, generator=g, device=dev)
+    got = mxfp4_moe(x, Routing(experts, weights), gate_up, down)
+    used = [0, 1, 150, 298, 299]
+    part = lambda q: Mxfp4(q.codes[used], q.scales[used], q.cols)  # noqa: E731
+    renamed = torch.tensor([[4, 0], [3, 4], [1, 2]], dtype=torch.int32, device=dev)
+    check_layer(got, BF, x, renamed, weights, part(gate_up), part(down), None, None, 'silu')
+
+
+def test_a_block_of_a_model(dev):
+    """As they are used: norm, router, experts, the next norm and a Linear, on another stream and captured, with eager calls between replays."""
+    g = gpu_gen(11)
+    E, K, I, T = 8, 256, 160, 9
+    gate_up, down = quantize_mxfp4(0.05 * torch.randn(E, 2 * I, K, generator=g, device=dev)), quantize_mxfp4(0.05 * torch.randn(E, K, I, generator=g, device=dev))
+    assert gate_up.codes.shape == (E, 2 * I, K // 2)
+    head = quantize_mxfp4((0.05 * torch.randn(120, K, generator=g, device=dev)).bfloat16())
+    wr = torch.randn(E, K, generator=g, device=dev).bfloat16() / 16
+    weight = torch.ones(K, device=dev, dtype=BF)
+
+    def block(x, stream):
+        n = residual_norm(x, stream, weight)
+        y = mxfp4_moe(n.out, Router((n.out.float() @ wr.float().t()), 2, 'sigmoid', scale=2.5), gate_up, down)
+        n = residual_norm(y, n.residual, weight)
+        return mxfp4_linear(n.out, head), n.residual
+
+    x, res = torch.randn(T, K, generator=g, device=dev).bfloat16(), torch.randn(T, K, generator=g, device=dev).bfloat16()
+    want = block(x, res)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = block(x, res)
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph, other = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = block(x, res)
+    with torch.cuda.graph(other):
+        out2 = block(res, x)
+    for i in range(4):
+        x.copy_(torch.randn(T, K, generator=g, device=dev))
+        want, want2 = block(x, res), block(res, x)
+        graph.replay()
+        other.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)) and all(torch.equal(a, b) for a, b in zip(out2, want2))
+
+
+def test_refusals(dev):
+    g = gpu_gen(12)
+    E, K, I, N, T = 4, 96, 64, 80, 3
+    gate_up, down = experts_of(E, 2 * I, K, g, dev), experts_of(E, N, I, g, dev)
+    x, logits = torch.zeros(T, K, device=dev), torch.zeros(T, E, device=dev)
+    ok = Router(logits, 2)
+    e, w = torch.zeros(T, 2, dtype=torch.int32, device=dev), torch.zeros(T, 2, device=dev)
+    assert mxfp4_moe(x, ok, gate_up, down).shape == (T, N) and mxfp4_moe(x[:0], Router(logits[:0], 2), gate_up, down).shape == (0, N)
+    for bad in (lambda: mxfp4_moe(x[:, :64], ok, gate_up, down), lambda: mxfp4_moe(x, Router(logits[:2], 2), gate_up, down),
+                lambda: mxfp4_moe(x, Router(logits[:, :3], 2), gate_up, down), lambda: mxfp4_moe(x, ok, Mxfp4(gate_up.codes[:3], gate_up.scales[:3], K), down),
+                lambda: mxfp4_moe(x, ok, Mxfp4(gate_up.codes[:, :-2], gate_up.scales[:, :-2], K), down), lambda: mxfp4_moe(x, ok, gate_up, down, activation='relu'),
+                lambda: mxfp4_moe(x, ok, gate_up, down, gate_up_bias=torch.zeros(E, I, device=dev)), lambda: mxfp4_moe(x, ok, gate_up, down, down_bias=torch.zeros(N, device=dev)),
+                lambda: mxfp4_moe(x, Routing(e[:2], w[:2]), gate_up, down), lambda: mxfp4_moe(x, Routing(e, w[:, :1]), gate_up, down),
+                lambda: mxfp4_moe(x, Routing(torch.zeros(T, 5, dtype=torch.int32, device=dev), torch.zeros(T, 5, device=dev)), gate_up, down),
+                lambda: mxfp4_moe(x, Router(logits, 5), gate_up, down)):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: mxfp4_moe(x.to(torch.int8), ok, gate_up, down), lambda: mxfp4_moe(x, Routing(e.long(), w), gate_up, down),
+                lambda: mxfp4_moe(x, Routing(e, w.bfloat16()), gate_up, down), lambda: mxfp4_moe(x, Routing(e.cpu(), w), gate_up, down),
+                lambda: mxfp4_moe(x, ok, gate_up, down, gate_up_bias=torch.zeros(E, 2 * I, device=dev), down_bias=torch.zeros(E, N, device=dev, dtype=BF)),
+                lambda: mxfp4_moe(x, ok, gate_up, down, down_bias=torch.zeros(E, N, device=dev, dtype=torch.int32))):
+        with pytest.raises(LcqError):
+            bad()
