@@ -584,13 +584,14 @@ int lcq_route(const void* logits, int dtype, int64_t T, int64_t E, int64_t ldl, 
  *  experts [T, top] int32, weights [T, top] fp32 (logits NULL): an index outside 0 .. E - 1 is no expert, several of the same of a token count
  *          as one with the sum of their weights
  *  gate_up [E, 2 I, 16 ceil(K / 32)]: the gates' rows, then the ups'; from an expert gate_up_lde, from a row gate_up_ld bytes to the next, all on 16
- *          bytes; gate_up_scales with gate_up_ldse, gate_up_lds.  down [E, N, 16 ceil(I / 32)] the same.  Row distances up to 2^22
+ *          bytes; gate_up_scales with gate_up_ldse, gate_up_lds.  down [E, N, 16 ceil(I / 32)] the same.  Row distances up to 2^22, and
+ *          gate_up_lds (I + 64) up to 2^30
  *  gate_up_bias [E, 2 I], down_bias [E, N] of bias_dtype, or NULL;  y [T, N] of out_dtype;  K, I, N <= 65536
- *  workspace of lcq_mxfp4_moe_workspace_bytes(T, top, K, I), 16-byte aligned.
+ *  workspace of lcq_mxfp4_moe_workspace_bytes(T, top, E, K, I, N, dtype), 16-byte aligned.
  * An expert whose weight is 0 is not asked (its infinities and NaN do not reach y); a token without experts gives 0. */
 #define LCQ_ACT_SILU 0
 #define LCQ_ACT_GELU 1
-int64_t lcq_mxfp4_moe_workspace_bytes(int64_t T, int64_t top, int64_t K, int64_t I);
+int64_t lcq_mxfp4_moe_workspace_bytes(int64_t T, int64_t top, int64_t E, int64_t K, int64_t I, int64_t N, int dtype);
 int lcq_mxfp4_moe(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, const void* logits, int logits_dtype, int64_t ldl, int flags,
                   const float* correction, float scale, const int* experts, const float* weights, int64_t E, int top, const uint8_t* gate_up,
                   int64_t gate_up_lde, int64_t gate_up_ld, const uint8_t* gate_up_scales, int64_t gate_up_ldse, int64_t gate_up_lds,

@@ -17,6 +17,7 @@ typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 template <int I> using Int = std::integral_constant<int, I>;
 
 constexpr int MOST_EXPERTS = 1024, MOST_TOP = 32, MOST_PASS = 128;           // tokens of a pass
+constexpr int MOST_GROUP = 32, COUNTERS = 1024;
 constexpr uint32_t OUTSIDE = 0x80000000u;
 
 __device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
@@ -138,12 +139,17 @@ __global__ __launch_bounds__(256) void route_kernel(RouterArgs r, int64_t T, int
 }
 
 // ---- what the products are told -----------------------------------------------------------------------------------
-// A pass: the slots (token and choice) sorted by expert, in groups of at most 16 of one expert.
+// A pass: the slots (token and choice) sorted by expert, in groups of at most `size` of one expert.
+struct Group {
+  int expert, first, count, pad;                    // first: slot
+  uint8_t token[MOST_GROUP];
+};
 struct Plan {
-  int groups;
-  int expert[MOST_EXPERTS + MOST_PASS * MOST_TOP / 16], first[MOST_EXPERTS + MOST_PASS * MOST_TOP / 16], count[MOST_EXPERTS + MOST_PASS * MOST_TOP / 16];
-  int token[MOST_PASS * MOST_TOP];
+  int groups, pad[15];
+  uint32_t counter[2][COUNTERS];                    // parts that are done: of gate and up, of down
+  int slot[MOST_PASS * MOST_TOP], expert[MOST_PASS * MOST_TOP];              // of a token's choices; slot -1: none
   float weight[MOST_PASS * MOST_TOP];
+  Group group[MOST_PASS * MOST_TOP];
 };
 
 struct Operand { const char* x; int64_t ldx; int dtype, planes, K, Kp; uint16_t* out; };
@@ -163,7 +169,7 @@ __device__ __forceinline__ void planes_of(float v, uint16_t* out) {
 // Workgroup 0 plans the pass; the others lay the tokens out as planes [T, planes, Kp] where they are not that already.
 template <int NL>
 __global__ __launch_bounds__(1024) void plan_kernel(RouterArgs r, const int* __restrict__ given, const float* __restrict__ given_weights, int T,
-                                                    Operand o, Plan* __restrict__ plan) {
+                                                    Operand o, int size, int most_groups, Plan* __restrict__ plan) {
   if (blockIdx.x) {
     const int64_t all = (int64_t)T * o.Kp;
     for (int64_t i = (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x; i < all; i += (int64_t)(gridDim.x - 1) * 1024) {
@@ -203,6 +209,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(RouterArgs r, const int* __r
     if (lane < r.top) { expert[t * r.top + lane] = e; weight[t * r.top + lane] = w; }
   }
   for (int i = tid; i < MOST_EXPERTS * (MOST_PASS / 32); i += 1024) (&chosen[0][0])[i] = 0;
+  for (int i = tid; i < 2 * COUNTERS; i += 1024) (&plan->counter[0][0])[i] = 0;
   __syncthreads();
   for (int i = tid; i < slots; i += 1024) {
     const int t = i / r.top;
@@ -214,7 +221,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(RouterArgs r, const int* __r
   #pragma unroll
   for (int q = 0; q < MOST_PASS / 32; ++q) mine += __builtin_popcount(chosen[tid][q]);
   const int n = (int)mine;
-  mine |= (uint32_t)((n + 15) / 16) << 16;
+  mine |= (uint32_t)((n + size - 1) / size) << 16;
   uint32_t sum = mine;
   #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
@@ -224,23 +231,33 @@ __global__ __launch_bounds__(1024) void plan_kernel(RouterArgs r, const int* __r
   if (lane == 63) sums[wave] = sum;
   __syncthreads();
   for (int w = 0; w < wave; ++w) sum += sums[w];
-  const uint32_t before = sum - mine;
-  place[tid] = before & 0xffff;
-  for (int g = 0; g < (n + 15) / 16; ++g) {
-    const int at = (int)(before >> 16) + g;
-    plan->expert[at] = tid;
-    plan->first[at] = (int)(before & 0xffff) + 16 * g;
-    plan->count[at] = n - 16 * g < 16 ? n - 16 * g : 16;
-  }
-  if (tid == 1023) plan->groups = (int)(sum >> 16);
   __syncthreads();
+  const uint32_t before = sum - mine;
+  place[tid] = before;
+  for (int g = 0; g * size < n; ++g) {
+    Group& to = plan->group[(before >> 16) + g];
+    to.expert = tid;
+    to.first = (int)(before & 0xffff) + size * g;
+    to.count = n - size * g < size ? n - size * g : size;
+  }
+  if (tid == 1023) sums[0] = sum >> 16;
+  __syncthreads();
+  const int groups = (int)sums[0];
+  if (tid == 0) plan->groups = groups;
+  for (int g = groups + tid; g < most_groups; g += 1024) plan->group[g].count = 0;
   for (int i = tid; i < slots; i += 1024) {
     const int e = expert[i], t = i / r.top;
-    if (e < 0) continue;
-    int at = (int)place[e] + __builtin_popcount(chosen[e][t / 32] & ((1u << t % 32) - 1));
-    for (int q = 0; q < t / 32; ++q) at += __builtin_popcount(chosen[e][q]);
-    plan->token[at] = t;
-    plan->weight[at] = weight[i];
+    int slot = -1;
+    if (e >= 0) {
+      int at = __builtin_popcount(chosen[e][t / 32] & ((1u << t % 32) - 1));                 // among the expert's slots
+      for (int q = 0; q < t / 32; ++q) at += __builtin_popcount(chosen[e][q]);
+      const uint32_t b = place[e];
+      slot = (int)(b & 0xffff) + at;
+      plan->group[(b >> 16) + at / size].token[at % size] = (uint8_t)t;
+    }
+    plan->slot[i] = slot;
+    plan->expert[i] = e;
+    plan->weight[i] = weight[i];
   }
 }
 
@@ -253,24 +270,18 @@ struct Weights {
 };
 
 struct MoeArgs {
-  const uint16_t* x;                                // planes of the tokens: [T, P, Kp] or rows ldx apart
-  int64_t ldx, ldp;                                 // elements from a token, a plane to the next
+  const uint16_t* x;                                // planes of the tokens: P of Kp, ldp apart, tokens ldx apart
+  int64_t ldx, ldp;
   Weights gate_up, down;
-  const Plan* plan;
+  Plan* plan;
   uint16_t* h;                                      // [slots, PH, Ip]
+  float *up, *out;                                  // sums of parts of K: of gate and up as the lanes hold them; of down [slots, parts, N]
   void* y;
-  int T, K, N, I, Kp, Ip, activation, dtype;        // Kp, Ip: whole blocks
+  int T, top, N, I, Kp, Ip, activation;             // Kp, Ip: whole blocks
 };
 
-__device__ __forceinline__ i32x4 load16(__amdgpu_buffer_rsrc_t buf, uint32_t of, int at) {
-  return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(buf, of, at, 0));
-}
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, int64_t size) {
-  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)size, 0x00020000);
-}
 // eight codes times their scale, exactly
-__device__ __forceinline__ bf16x8 decoded(int codes, int scale) {
-  const float f = mx_factor((uint32_t)scale);
+__device__ __forceinline__ bf16x8 decoded(int codes, float f) {
   const lcq_bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((uint32_t)codes, f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((uint32_t)codes, f, 1),
                    c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((uint32_t)codes, f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((uint32_t)codes, f, 3);
   return bf16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
@@ -280,186 +291,334 @@ __device__ __forceinline__ float act(float v, int activation) {
   return activation == LCQ_ACT_SILU ? v / (1.0f + expf(-v)) : 0.5f * v * (1.0f + erff(v * 0.70710678118654752440f));
 }
 
-// A lane's 16 bytes of a row are a block; a load of the wave is 16 rows x 64 bytes.  A piece is two of them.
-constexpr int PIECE = 128;
+// The stream of weights that both products are.  A wave has 32 rows (16 gates and their ups, or 32 channels of down), a workgroup's four waves share
+// the tokens' operand.  K goes by in stages of 256 codes through LDS, all by direct loads, DEPTH - 1 stages ahead of the products:
+//   codes   32 rows x 128 bytes per wave, 8 rows a load: whole lines.  (Loaded straight into the matrix pipe's layout, 16 neighbouring
+//           lanes are 16 rows, and every load passes the cache 64 times for 1 KB: 3.4 TB/s.)  Piece p of row r lies at p ^ (r / 2 % 8)
+//   operand rows of 512 bytes, one per slot and plane; piece p of slot s lies at p ^ (s % 16)
+//   scales  the word-aligned 32 bytes of a row that hold those of four stages, or of three where rows are off words: a load per wave and
+//           period.  (One per stage takes as many passes of the L2 as the codes: 5.55 TB/s for 6.17 without scales.)
+// so that 16 lanes of a read touch all banks once.  One barrier per stage, in front of its products: what was read before it is loaded again.
+constexpr int STAGE = 128;                          // bytes of a row's codes
 
-// gate and up: 16 channels of one group per workgroup, whose waves take pieces of K in turn.
-template <int P, int PH, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void up_kernel(MoeArgs g, int tiles) {
-  __shared__ __attribute__((aligned(16))) float red[WAVES][2][64][4];
-  const int group = blockIdx.x / tiles, n0 = (blockIdx.x - group * tiles) * 16;
-  if (group >= g.plan->groups) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), q = lane >> 4, c = lane & 15;
-  const int e = g.plan->expert[group], first = g.plan->first[group], count = g.plan->count[group];
-  const Weights& w = g.gate_up;
-  const int bytes = w.B * 16, rows = g.I - n0 < 16 ? g.I - n0 : 16;          // (0 or less: channels that only fill a block)
-  __amdgpu_buffer_rsrc_t buf[2], sbuf[2];
-  #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int64_t row = n0 + (int64_t)u * g.I;
-    buf[u] = buffer(w.w + e * w.lde + row * w.ldw, rows > 0 ? (rows - 1) * w.ldw + bytes : 0);
-    sbuf[u] = buffer(w.s + e * w.ldse + row * w.lds, rows > 0 ? (rows - 1) * w.lds + w.B : 0);
+template <int P, int GS>
+struct Shape {
+  static constexpr int XOPS = GS * P / 2, X = (XOPS + 3) / 4, FULL = XOPS % 4;               // loads of the operand: of all waves, of the first FULL (0: of all)
+  static constexpr int BYTES = 16384 + GS * P * 512;                         // of a stage, in LDS
+  static constexpr int DEPTH = 3 * (BYTES + 4096) <= 81920 ? 3 : 163840 / (BYTES + 4096) < 5 ? 163840 / (BYTES + 4096) : 5;      // two workgroups per CU, or one
+  static constexpr int LDS = DEPTH * (BYTES + 4096), TB = (GS + 15) / 16;
+  static_assert(DEPTH >= 3, "stages in LDS");
+};
+
+typedef __attribute__((address_space(3))) char* lds_ptr;
+// what no kernel writes while this one reads it: loaded by the scalar unit, apart from the stream of vector loads
+template <class T> __device__ __forceinline__ T fixed(const T& v) { return *(const __attribute__((address_space(4))) T*)(uintptr_t)&v; }
+
+// Workgroups that share a result: the last of `parts` to come here has what all of them stored.
+__device__ __forceinline__ bool last_of(uint32_t* counter, int parts) {
+  __shared__ uint32_t before;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) before = atomicAdd(counter, 1u);
+  __syncthreads();
+  if (before != (uint32_t)parts - 1) return false;
+  __threadfence();
+  return true;
+}
+
+// Gate and up (DOWN false): a workgroup has 64 channels of h of one group, and one of `parts` parts of K.
+// Down: 128 channels, and a run of the units (group, part of K: `parts` of each); the last workgroup of a tile's `runs` sums up a token's choices.
+template <bool DOWN, int P, int GS, int PH>
+__global__ __launch_bounds__(256) void experts_kernel(MoeArgs g, int tiles, int parts, int runs) {
+  typedef Shape<P, GS> S;
+  constexpr int TB = S::TB, DEPTH = S::DEPTH;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];               // DEPTH stages
+  const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Weights& w = DOWN ? g.down : g.gate_up;
+  const int bytes = w.B * 16, stages = (bytes + STAGE - 1) / STAGE;
+  int tile, unit, end;                              // units are numbered group by group
+  if constexpr (DOWN) {
+    const int run = blockIdx.x / tiles, units = fixed(g.plan->groups) * parts;
+    tile = blockIdx.x - run * tiles;
+    unit = (int)((uint32_t)units * (uint32_t)run / (uint32_t)runs);       // (fewer than 2^19 units, 2^10 runs)
+    end = (int)((uint32_t)units * (uint32_t)(run + 1) / (uint32_t)runs);
+  } else {
+    const int all = blockIdx.x / parts, group = all / tiles;
+    tile = all - group * tiles;
+    unit = group * parts + (blockIdx.x - all * parts);
+    end = unit + 1;
+    if (fixed(g.plan->group[group].count) == 0) return;
   }
-  const uint32_t of = c < rows ? (uint32_t)(c * w.ldw) + q * 16 : OUTSIDE, sof = c < rows ? (uint32_t)(c * w.lds) + q : OUTSIDE;
-  const int token = g.plan->token[first + (c < count ? c : 0)];
-  const uint16_t* const x = g.x + token * g.ldx + q * 32;
-  constexpr int DEPTH = P == 1 ? 3 : 2, STEP = WAVES * PIECE;
-  struct Piece { i32x4 w[2][2], x[2][P][4]; int s[2][2]; } ring[DEPTH];
-  const auto load = [&](int k, Piece& p) {
+  constexpr int WIDTH = DOWN ? 128 : 64;
+  const int channels = DOWN ? g.N : g.I, n0 = tile * WIDTH + wave * (WIDTH / 4);
+  // rows of each half of 16: channels n0 .. (their gates, and their ups I rows behind; down: and n0 + 16 ..)
+  int rows[2] = {channels - n0, channels - n0 - (DOWN ? 16 : 0)};
+  #pragma unroll
+  for (int u = 0; u < 2; ++u) rows[u] = rows[u] < 0 ? 0 : rows[u] > 16 ? 16 : rows[u];
+  const int64_t second = DOWN ? 16 : g.I;           // rows from a first half to its second
+
+  const auto one = [](uint32_t v) { return (int)__builtin_amdgcn_readfirstlane((int)v); };
+  const auto buffer = [&](const void* p, int64_t size) {
+    const uint64_t at = (uint64_t)(uintptr_t)p;
+    return i32x4{one((uint32_t)at), one((uint32_t)(at >> 32) & 0xffff), one((uint32_t)size), 0x00020000};
+  };
+  const auto load = [&](uint32_t to, uint32_t of, i32x4 buf, int at) {       // (all but `of` are the wave's)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(one(to)), "v"(of), "s"(buf), "s"(one((uint32_t)at)) : "memory");
+  };
+  const uint32_t lds0 = (uint32_t)(size_t)(lds_ptr)lds;
+
+  // ---- loads: a place in the sequence of stages, and what depends on its group alone ----
+  uint32_t wof[4], xof[S::X], sof;
+  #pragma unroll
+  for (int l = 0; l < 4; ++l) {
+    const int r = l * 8 + (lane >> 3), in = r & 15;
+    wof[l] = in < rows[l >> 1] ? (uint32_t)(in * w.ldw) + (((lane & 7) ^ (r >> 1 & 7)) << 4) : OUTSIDE;
+  }
+  const int piece = (lane & 7) ^ (lane >> 4 & 3);   // of 16 bytes in a row of codes; in odd loads 4 more, as 8 rows turn it
+  const i32x4 bufX = DOWN ? buffer(g.h, 0x7fffffff) : buffer(g.x, 0x7fffffff);
+  i32x4 bufW[2], bufS;
+  const int row_bytes = (DOWN ? g.Ip : g.Kp) * 2;
+  // the first stage of part p of a group
+  const auto first_of = [&](int p) { return (int)((uint32_t)(stages * p) / (uint32_t)parts); };
+  struct Place { int unit, group, part, k, end; } at;
+  const auto go = [&](Place& to, int u) {
+    to.unit = u;
+    to.group = (uint32_t)u / (uint32_t)parts;
+    to.part = u - to.group * parts;
+    to.k = first_of(to.part);
+    to.end = first_of(to.part + 1);
+  };
+  const int period = ((uintptr_t)w.s | (uintptr_t)w.ldse | (uintptr_t)w.lds) & 3 ? 3 : 4;    // stages
+  const auto enter = [&]() {
+    const Group& in = g.plan->group[at.group];
+    const int e = fixed(in.expert), first = fixed(in.first), count = fixed(in.count);
     #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int at = k + i * 64;
-      const bool in = at + q * 16 < bytes;
-      #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        p.w[u][i] = load16(buf[u], in ? of : OUTSIDE, at);
-        p.s[u][i] = __builtin_amdgcn_raw_buffer_load_b8(sbuf[u], in ? sof : OUTSIDE, at >> 4, 0);
+    for (int u = 0; u < 2; ++u)
+      bufW[u] = buffer(w.w + e * w.lde + (n0 + u * second) * w.ldw, rows[u] ? (rows[u] - 1) * w.ldw + bytes : 0);
+    // scales of the wave's rows: from the first half's first row to the second half's last
+    const uint8_t* const s = w.s + e * w.ldse + n0 * w.lds;
+    const int early = (int)((uintptr_t)s & 3);
+    bufS = buffer(s - early, rows[0] ? (early + (rows[1] ? second + rows[1] - 1 : rows[0] - 1) * w.lds + w.B + 3) & ~(int64_t)3 : 0);
+    const int r = lane >> 1;
+    sof = (r & 15) < rows[r >> 4] ? ((uint32_t)(early + ((r & 15) + (r >> 4) * second) * w.lds) & ~3u) + (lane & 1) * 16 : OUTSIDE;
+    #pragma unroll
+    for (int o = 0; o < S::X; ++o) {
+      const int r = (wave + 4 * o) * 2 + (lane >> 5), slot = r / P, plane = r - slot * P;
+      xof[o] = OUTSIDE;
+      if (slot < count) {                           // (of a group that is not full: zeros)
+        if constexpr (DOWN) xof[o] = (uint32_t)((first + slot) * P + plane) * (uint32_t)(g.Ip * 2);
+        else xof[o] = (uint32_t)((in.token[slot] * g.ldx + plane * g.ldp) * 2);
       }
-      #pragma unroll
-      for (int l = 0; l < P; ++l)
-        #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          i32x4 v = {};
-          if (in && c < count && at * 2 + q * 32 + j * 8 < g.Kp) v = *(const i32x4*)(x + l * g.ldp + at * 2 + j * 8);
-          p.x[i][l][j] = v;
-        }
     }
   };
-  int k = wave * PIECE;
-  #pragma unroll
-  for (int d = 0; d < DEPTH; ++d) load(k + d * STEP, ring[d]);
-  f32x4 acc[2] = {};
-  while (k < bytes) {
+  // The next stage, into a place; behind the last one: nothing, from outside.  The scales of a period come in front of its first stage.
+  int lperiod = 0, lplace = DEPTH - 1;
+  const auto fetch = [&](int slot) {
+    const uint32_t over = at.unit < end ? 0u : OUTSIDE, to = lds0 + slot * S::BYTES;
+    if (lperiod == 0) {
+      lplace = lplace == DEPTH - 1 ? 0 : lplace + 1;
+      load(lds0 + DEPTH * S::BYTES + (lplace * 4 + wave) * 1024, sof | over, bufS, at.k * 8);
+      lperiod = period;
+    }
+    --lperiod;
     #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-      Piece& p = ring[d];
+    for (int l = 0; l < 4; ++l) {
+      const uint32_t outside = (piece ^ (l & 1) * 4) * 16 < bytes - at.k * STAGE ? over : OUTSIDE;
+      load(to + (wave * 4 + l) * 1024, wof[l] | outside, bufW[l >> 1], at.k * STAGE);
+    }
+    #pragma unroll
+    for (int o = 0; o < S::X; ++o) {
+      const int x = wave + 4 * o;
+      if (S::FULL && o == S::X - 1 && wave >= S::FULL) break;
+      const int p = (lane & 31) ^ ((x * 2 + (lane >> 5)) / P & 15);          // piece of an operand's row
+      load(to + 16384 + x * 1024, (xof[o] + p * 16) | over | (p * 16 + at.k * 512 < row_bytes ? 0u : OUTSIDE), bufX, at.k * 512);
+    }
+    if (++at.k == at.end && at.unit < end) {
+      go(at, at.unit + 1);
+      lperiod = 0;
+      if (DOWN && at.unit < end) enter();
+    }
+  };
+
+  f32x4 acc[2][TB] = {};
+  if (unit < end) {
+    go(at, unit);
+    enter();
+    #pragma unroll
+    for (int d = 0; d < DEPTH - 1; ++d) fetch(d);
+    // ---- products ----
+    Place now;
+    int slot = 0, first = 0, count = 0, early[2];
+    const auto begin = [&]() {
+      const Group& in = g.plan->group[now.group];
+      const int e = fixed(in.expert);
+      first = fixed(in.first);
+      count = fixed(in.count);
+      #pragma unroll
+      for (int u = 0; u < 2; ++u) early[u] = (int)((uint32_t)(uintptr_t)w.s + (uint32_t)e * (uint32_t)w.ldse + (uint32_t)(n0 + c + u * (int)second) * (uint32_t)w.lds) & 3;
+    };
+    go(now, unit);
+    begin();
+    const char* const codes = lds + wave * 4096 + c * 128;
+    const char* const scales = lds + DEPTH * S::BYTES + wave * 1024 + c * 32 + q;
+    const int turn = c >> 1 & 7;
+    int cperiod = 0, cplace = DEPTH - 1;
+    constexpr int MORE = (DEPTH - 2) * (4 + S::X), LESS = (DEPTH - 2) * (3 + S::X);          // loads that may be on their way
+    while (now.unit < end) {
+      // the next stage has landed, and this wave has read the last one
+      if (S::FULL && wave >= S::FULL) __builtin_amdgcn_s_waitcnt(0x0070 | (LESS & 15) | LESS >> 4 << 14);
+      else __builtin_amdgcn_s_waitcnt(0x0070 | (MORE & 15) | MORE >> 4 << 14);
+      asm volatile("s_barrier" ::: "memory");
+      fetch(slot == 0 ? DEPTH - 1 : slot - 1);
+      if (cperiod == 0) cplace = cplace == DEPTH - 1 ? 0 : cplace + 1;
+      const int here = slot * S::BYTES, scales_here = cplace * 4096 + cperiod * 8;
+      cperiod = cperiod == period - 1 ? 0 : cperiod + 1;
+      i32x4 wv[2][2];
+      float f[2][2];
+      #pragma unroll
+      for (int u = 0; u < 2; ++u)
+        #pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          wv[u][i] = *(const i32x4*)(codes + here + u * 2048 + (((i * 4 + q) ^ turn) << 4));
+          const uint32_t byte = *(const uint8_t*)(scales + scales_here + u * 512 + early[u] + i * 4);
+          f[u][i] = mx_factor(now.k * 8 + i * 4 + q < w.B ? byte : 0u);      // (behind the last block: not a NaN)
+        }
       #pragma unroll
       for (int i = 0; i < 2; ++i)
         #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const bf16x8 v = decoded(p.w[u][i][j], p.s[u][i]);
-            #pragma unroll
-            for (int l = P - 1; l >= 0; --l) acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, p.x[i][l][j]), acc[u], 0, 0, 0);
-          }
-      load(k + DEPTH * STEP, p);
-      k += STEP;
-    }
-  }
-  #pragma unroll
-  for (int u = 0; u < 2; ++u) *(f32x4*)red[wave][u][lane] = acc[u];
-  __syncthreads();
-  // accumulator register r of lane l: channel 4 (l / 16) + r of slot l % 16
-  for (int o = tid; o < 256; o += WAVES * 64) {
-    const int ch = o & 15, slot = o >> 4;
-    if (slot >= count || n0 + ch >= g.Ip) continue;
-    float v[2] = {};
-    #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      #pragma unroll
-      for (int s = 0; s < WAVES; ++s) v[u] += red[s][u][(ch >> 2) * 16 + slot][ch & 3];
-      if (w.bias && ch < rows) v[u] += load_any(w.bias, w.bias_dtype, (int64_t)e * 2 * g.I + u * g.I + n0 + ch);
-    }
-    uint16_t p[PH];
-    planes_of<PH>(ch < rows ? act(v[0], g.activation) * v[1] : 0.0f, p);
-    #pragma unroll
-    for (int l = 0; l < PH; ++l) g.h[((int64_t)(first + slot) * PH + l) * g.Ip + n0 + ch] = p[l];
-  }
-}
-
-// down and the weighted sum: 16 channels of all tokens per workgroup.  The pieces of all groups, one behind the other, are dealt to the waves
-// in equal runs; a wave that leaves a group adds what it has of it to its own sums of the tokens, in LDS.  No atomics: the order is fixed.
-template <int BF, int PH, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void down_kernel(MoeArgs g) {
-  extern __shared__ __attribute__((aligned(16))) float sums[];               // [WAVES, T, 16]
-  const int n0 = blockIdx.x * 16;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), q = lane >> 4, c = lane & 15;
-  const Weights& w = g.down;
-  const int bytes = w.B * 16, rows = g.N - n0 < 16 ? g.N - n0 : 16, pieces = (bytes + PIECE - 1) / PIECE;
-  const int total = g.plan->groups * pieces;
-  const int begin = (int)((int64_t)total * wave / WAVES), end = (int)((int64_t)total * (wave + 1) / WAVES);
-  float* const mine = sums + wave * g.T * 16;
-  for (int i = lane; i < g.T * 16; i += 64) mine[i] = 0;
-  const uint32_t of = c < rows ? (uint32_t)(c * w.ldw) + q * 16 : OUTSIDE, sof = c < rows ? (uint32_t)(c * w.lds) + q : OUTSIDE;
-  constexpr int DEPTH = 2;
-  struct Piece { i32x4 w[2], h[2][PH][4]; int s[2]; } ring[DEPTH];
-  const auto load = [&](int at_, Piece& p) {
-    const int at = at_ < end ? at_ : end - 1;       // (behind the last: once more, unused)
-    const int group = at / pieces, k = (at - group * pieces) * PIECE;
-    const int e = g.plan->expert[group], first = g.plan->first[group], count = g.plan->count[group];
-    const __amdgpu_buffer_rsrc_t buf = buffer(w.w + e * w.lde + n0 * w.ldw, (rows - 1) * w.ldw + bytes), sbuf = buffer(w.s + e * w.ldse + n0 * w.lds, (rows - 1) * w.lds + w.B);
-    const uint16_t* const h = g.h + (int64_t)(first + (c < count ? c : 0)) * PH * g.Ip + q * 32 + k * 2;
-    #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const bool in = k + i * 64 + q * 16 < bytes;
-      p.w[i] = load16(buf, in ? of : OUTSIDE, k + i * 64);
-      p.s[i] = __builtin_amdgcn_raw_buffer_load_b8(sbuf, in ? sof : OUTSIDE, (k >> 4) + i * 4, 0);
-      #pragma unroll
-      for (int l = 0; l < PH; ++l)
-        #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          i32x4 v = {};
-          if (in && c < count) v = *(const i32x4*)(h + l * g.Ip + i * 128 + j * 8);
-          p.h[i][l][j] = v;
-        }
-    }
-  };
-  int at = begin;
-  if (begin < end) {
-    #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) load(at + d, ring[d]);
-    f32x4 acc = {};
-    int group = begin / pieces, left = (group + 1) * pieces - begin;         // pieces of this group from here on
-    bool whole = left == pieces;                    // does this wave have the group's first piece?
-    while (at < end) {
-      #pragma unroll
-      for (int d = 0; d < DEPTH; ++d) {
-        if (at < end) {
-          Piece& p = ring[d];
+          bf16x8 v[2];
           #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int u = 0; u < 2; ++u) v[u] = decoded(wv[u][i][j], f[u][i]);
+          #pragma unroll
+          for (int b = 0; b < TB; ++b)
             #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const bf16x8 v = decoded(p.w[i][j], p.s[i]);
+            for (int l = P - 1; l >= 0; --l) {
+              const int s = (b * 16 + c) & (GS - 1);
+              const bf16x8 x = *(const bf16x8*)(lds + here + 16384 + (s * P + l) * 512 + (((i * 16 + q * 4 + j) ^ (s & 15)) << 4));
               #pragma unroll
-              for (int l = PH - 1; l >= 0; --l) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, p.h[i][l][j]), acc, 0, 0, 0);
+              for (int u = 0; u < 2; ++u) acc[u][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u], x, acc[u][b], 0, 0, 0);
             }
-          load(at + DEPTH, p);
-          ++at;
-          if (--left == 0 || at == end) {
-            const int e = g.plan->expert[group], first = g.plan->first[group], count = g.plan->count[group];
-            if (c < count) {
-              const float weight = g.plan->weight[first + c];
-              f32x4* const to = (f32x4*)(mine + g.plan->token[first + c] * 16 + q * 4);
-              f32x4 v = *to;
-              #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                float b = 0;
-                if (w.bias && whole && q * 4 + r < rows) b = load_any(w.bias, w.bias_dtype, (int64_t)e * g.N + n0 + q * 4 + r);
-                v[r] = __builtin_fmaf(weight, acc[r] + b, v[r]);
-              }
-              *to = v;
+        }
+      slot = slot == DEPTH - 1 ? 0 : slot + 1;
+      if (++now.k == now.end) {
+        if constexpr (DOWN) {
+          #pragma unroll
+          for (int b = 0; b < TB; ++b) {
+            const int s = b * 16 + c;
+            #pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              // (rows of whole fours; what lies behind N is not read)
+              if (s < count && q * 4 < rows[u])
+                *(f32x4*)(g.out + ((int64_t)(first + s) * parts + now.part) * ((g.N + 3) & ~3) + n0 + u * 16 + q * 4) = acc[u][b];
+              acc[u][b] = f32x4{};
             }
-            acc = f32x4{};
-            ++group;
-            left = pieces;
-            whole = true;
           }
         }
+        go(now, now.unit + 1);
+        cperiod = 0;
+        if (DOWN && now.unit < end) begin();
       }
     }
   }
-  __syncthreads();
-  for (int o = tid; o < g.T * 16; o += WAVES * 64) {
-    const int ch = o & 15;
-    const int64_t t = o >> 4;
-    if (ch >= rows) continue;
-    float y = 0;
+  __builtin_amdgcn_s_waitcnt(0x0f70);               // nothing may still be on its way to LDS when the workgroup leaves it
+
+  // ---- results: accumulator register r of lane l is channel 4 (l / 16) + r of slot l % 16 ----
+  if constexpr (!DOWN) {
+    const int group = unit / parts;
+    const Group& in = g.plan->group[group];
+    if (parts > 1) {
+      f32x4* const mine = (f32x4*)g.up + ((int64_t)(blockIdx.x / parts) * parts * 256 + tid) * (2 * TB);
+      #pragma unroll
+      for (int u = 0; u < 2; ++u)
+        #pragma unroll
+        for (int b = 0; b < TB; ++b) mine[(int64_t)(unit - group * parts) * 512 * TB + u * TB + b] = acc[u][b];
+      if (!last_of(&g.plan->counter[0][blockIdx.x / parts], parts)) return;
+      #pragma unroll
+      for (int u = 0; u < 2; ++u)
+        #pragma unroll
+        for (int b = 0; b < TB; ++b) {
+          acc[u][b] = f32x4{};
+          for (int p = 0; p < parts; ++p) acc[u][b] += mine[(int64_t)p * 512 * TB + u * TB + b];
+        }
+    }
+    const int e = in.expert, count = in.count, first = in.first;
+    if (n0 + q * 4 >= g.Ip) return;
     #pragma unroll
-    for (int s = 0; s < WAVES; ++s) y += sums[s * g.T * 16 + o];
-    if constexpr (BF == ROW_F32) ((float*)g.y)[t * g.N + n0 + ch] = y;
-    else store_scalar<BF>(g.y, t * g.N + n0 + ch, rnd<BF>(y));
+    for (int b = 0; b < TB; ++b) {
+      const int s = b * 16 + c;
+      if (s >= count) continue;
+      uint16_t p[4][PH];
+      #pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int ch = q * 4 + r;
+        float v[2] = {acc[0][b][r], acc[1][b][r]};
+        if (w.bias && ch < rows[0]) {
+          #pragma unroll
+          for (int u = 0; u < 2; ++u) v[u] += load_any(w.bias, w.bias_dtype, ((int64_t)e * 2 + u) * g.I + n0 + ch);
+        }
+        planes_of<PH>(ch < rows[0] ? act(v[0], g.activation) * v[1] : 0.0f, p[r]);
+      }
+      #pragma unroll
+      for (int l = 0; l < PH; ++l)
+        *(u32x2*)(g.h + ((int64_t)(first + s) * PH + l) * g.Ip + n0 + q * 4) = u32x2{p[0][l] | (uint32_t)p[1][l] << 16, p[2][l] | (uint32_t)p[3][l] << 16};
+    }
+  }
+}
+
+// y of four channels of a token per lane: the weighted sum of its choices' parts in their order, eight of them on their way at a time in each of
+// four waves.
+template <int BF>
+__global__ __launch_bounds__(256) void sum_kernel(MoeArgs g, int parts) {
+  __shared__ int slot[MOST_TOP];
+  __shared__ float weight[MOST_TOP];
+  __shared__ f32x4 some[4][64];
+  const int t = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = (blockIdx.x * 64 + lane) * 4, Np = (g.N + 3) & ~3;
+  if (threadIdx.x < g.top) {
+    slot[threadIdx.x] = g.plan->slot[t * g.top + threadIdx.x];
+    weight[threadIdx.x] = g.plan->weight[t * g.top + threadIdx.x];
+  }
+  __syncthreads();
+  const int all = g.top * parts, end = all * (wave + 1) / 4;
+  f32x4 y = {};
+  if (n < g.N) {
+    for (int i0 = all * wave / 4; i0 < end; i0 += 8) {
+      f32x4 v[8];
+      float w[8];
+      #pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = i0 + j < end ? i0 + j : end - 1, s = i / parts, at = slot[s];
+        w[j] = i0 + j < end && at >= 0 ? weight[s] : 0.0f;
+        v[j] = f32x4{};
+        if (w[j] != 0.0f) v[j] = *(const f32x4*)(g.out + ((int64_t)at * parts + (i - s * parts)) * Np + n);  // (what has no weight may be anything)
+      }
+      #pragma unroll
+      for (int j = 0; j < 8; ++j)
+        #pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] = __builtin_fmaf(w[j], v[j][r], y[r]);
+    }
+  }
+  some[wave][lane] = y;
+  __syncthreads();
+  if (wave || n >= g.N) return;
+  #pragma unroll
+  for (int s = 1; s < 4; ++s) y += some[s][lane];
+  const int left = g.N - n;
+  if (g.down.bias) {
+    for (int s = 0; s < g.top; ++s) {
+      if (slot[s] < 0) continue;
+      const int64_t at = (int64_t)g.plan->expert[t * g.top + s] * g.N + n;
+      #pragma unroll
+      for (int r = 0; r < 4; ++r) if (r < left) y[r] = __builtin_fmaf(weight[s], load_any(g.down.bias, g.down.bias_dtype, at + r), y[r]);
+    }
+  }
+  const int64_t to = (int64_t)t * g.N + n;
+  #pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    if (r >= left) break;
+    if constexpr (BF == ROW_F32) ((float*)g.y)[to + r] = y[r];
+    else store_scalar<BF>(g.y, to + r, rnd<BF>(y[r]));
   }
 }
 
@@ -474,7 +633,58 @@ int check_router(const RouterArgs& r, int64_t T) {
 }
 
 // are the tokens planes as they are?
-bool direct(int dtype, const void* x, int64_t ldx, int64_t K) { return dtype == LCQ_BF16 && K % 32 == 0 && ldx % 8 == 0 && (uintptr_t)x % 16 == 0; }
+bool direct(int dtype, const void* x, int64_t ldx, int64_t K) {
+  return dtype == LCQ_BF16 && K % 32 == 0 && ldx % 8 == 0 && (uintptr_t)x % 16 == 0 && ldx <= 1 << 22;       // (offsets have 31 bits)
+}
+
+// How a pass of T tokens is cut.
+struct Cut {
+  int P, PH, size, up_tiles, up_parts, down_tiles, down_parts, runs;
+  int64_t groups, h, up, out;                       // bytes
+  Cut(int64_t T, int64_t top, int64_t E, int64_t K, int64_t I, int64_t N, int dtype) {
+    P = dtype == LCQ_BF16 ? 1 : dtype == LCQ_F16 ? 2 : 3;
+    PH = dtype == LCQ_F32 ? 3 : 2;
+    const int64_t slots = T * top;
+    size = T <= 4 || slots <= E ? 4 : P == 3 || T <= 16 || slots <= 14 * E ? 16 : 32;
+    groups = least(slots, least(E, slots) + slots / size);
+    const int64_t up_stages = ((K + 31) / 32 + 7) / 8, down_stages = ((I + 31) / 32 + 7) / 8, Ip = (I + 31) / 32 * 32;
+    up_tiles = (int)((Ip + 63) / 64);
+    up_parts = 1;
+    while (groups * up_tiles * up_parts < 200 && up_stages / (2 * up_parts) >= 3) up_parts *= 2;
+    down_tiles = (int)((N + 127) / 128);
+    int64_t want = 512 / down_tiles;
+    if (want < 1) want = 1;
+    down_parts = 1;
+    while (groups * down_parts < 8 * want && down_stages / (2 * down_parts) >= 2) down_parts *= 2;
+    const int64_t units = groups * down_parts, each = (units + want - 1) / want;
+    runs = (int)((units + each - 1) / each);
+    h = on256(slots * PH * Ip * 2);
+    up = up_parts > 1 ? on256(groups * up_tiles * up_parts * 256 * 32 * (size > 16 ? 2 : 1)) : 0;
+    out = on256(slots * down_parts * ((N + 3) & ~(int64_t)3) * 4);
+  }
+};
+
+template <bool DOWN, int P, int GS, int PH>
+int launch_experts(const MoeArgs& g, const Cut& c, hipStream_t st) {
+  typedef Shape<P, GS> S;
+  const auto kernel = experts_kernel<DOWN, P, GS, PH>;
+  // (more LDS than a launch may have without asking)
+  if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS) != hipSuccess) return LCQ_ELAUNCH;
+  const int64_t blocks = DOWN ? (int64_t)c.down_tiles * c.runs : c.groups * c.up_tiles * c.up_parts;
+  if (blocks > (1 << 24) - 1) return LCQ_ESIZE;
+  kernel<<<dim3((unsigned)blocks), dim3(256), S::LDS, st>>>(g, DOWN ? c.down_tiles : c.up_tiles, DOWN ? c.down_parts : c.up_parts, c.runs);
+  return LCQ_OK;
+}
+template <bool DOWN, int P, int PH>
+int launch_size(const MoeArgs& g, const Cut& c, hipStream_t st) {
+  if (c.size == 4) return launch_experts<DOWN, P, 4, PH>(g, c, st);
+  if constexpr (P < 3) { if (c.size == 32) return launch_experts<DOWN, P, 32, PH>(g, c, st); }
+  return launch_experts<DOWN, P, 16, PH>(g, c, st);
+}
+template <int BF>
+void launch_sum(const MoeArgs& g, const Cut& c, hipStream_t st) {
+  sum_kernel<BF><<<dim3((unsigned)((g.N + 255) / 256), (unsigned)g.T), dim3(256), 0, st>>>(g, c.down_parts);
+}
 
 }  // namespace
 
@@ -496,10 +706,16 @@ int lcq_route(const void* logits, int dtype, int64_t T, int64_t E, int64_t ldl, 
   return LCQ_OK;
 }
 
-int64_t lcq_mxfp4_moe_workspace_bytes(int64_t T, int64_t top, int64_t K, int64_t I) {
-  if (T <= 0 || top <= 0 || K <= 0 || I <= 0 || K > 65536 || I > 65536 || top > MOST_TOP) return 0;
-  const int64_t t = least(T, MOST_PASS), Kp = (K + 31) / 32 * 32, Ip = (I + 31) / 32 * 32;
-  return on256(sizeof(Plan)) + on256(t * top * 3 * Ip * 2) + t * 3 * Kp * 2;
+int64_t lcq_mxfp4_moe_workspace_bytes(int64_t T, int64_t top, int64_t E, int64_t K, int64_t I, int64_t N, int dtype) {
+  if (T <= 0 || top <= 0 || E <= 0 || K <= 0 || I <= 0 || N <= 0 || K > 65536 || I > 65536 || N > 65536 || top > MOST_TOP || E > MOST_EXPERTS || !known(dtype)) return 0;
+  const int64_t t = least(T, MOST_PASS);
+  int64_t most = 0;                                 // (the last pass may have fewer tokens, and be cut into more parts)
+  for (const int64_t n : {t, T % MOST_PASS ? T % MOST_PASS : t}) {
+    const Cut c(n, top, E, K, I, N, dtype);
+    const int64_t size = c.h + c.up + c.out + on256(n * c.P * ((K + 31) / 32 * 32) * 2);
+    most = size > most ? size : most;
+  }
+  return on256(sizeof(Plan)) + most;
 }
 
 int lcq_mxfp4_moe(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, const void* logits, int logits_dtype, int64_t ldl, int flags,
@@ -518,50 +734,44 @@ int lcq_mxfp4_moe(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, c
   if (K > 65536 || I > 65536 || N > 65536) return LCQ_ESIZE;
   const int64_t B = (K + 31) / 32, BI = (I + 31) / 32, Kp = 32 * B, Ip = 32 * BI;
   if (gate_up_ld < 16 * B || gate_up_lds < B || down_ld < 16 * BI || down_lds < BI) return LCQ_EINVAL;
-  if (gate_up_ld > 1 << 22 || gate_up_lds > 1 << 22 || down_ld > 1 << 22 || down_lds > 1 << 22) return LCQ_ESIZE;
+  if (gate_up_ld > 1 << 22 || down_ld > 1 << 22 || gate_up_lds * (I + 64) > 1 << 30 || down_lds > 1 << 22) return LCQ_ESIZE;
   if ((uintptr_t)gate_up % 16 || gate_up_ld % 16 || gate_up_lde % 16 || (uintptr_t)down % 16 || down_ld % 16 || down_lde % 16) return LCQ_EALIGN;
   if (!workspace) return LCQ_EWORKSPACE;
   if ((uintptr_t)workspace % 16) return LCQ_EALIGN;
   hipStream_t st = (hipStream_t)stream;
-  const int64_t most = least(T, MOST_PASS);
   char* const ws = (char*)workspace;
   const bool as_is = direct(dtype, x, ldx, K);
-  const int P = dtype == LCQ_BF16 ? 1 : dtype == LCQ_F16 ? 2 : 3, PH = dtype == LCQ_F32 ? 3 : 2;
   Plan* const plan = (Plan*)ws;
-  uint16_t* const h = (uint16_t*)(ws + on256(sizeof(Plan)));
-  uint16_t* const planes = (uint16_t*)((char*)h + on256(most * top * 3 * Ip * 2));
   const int64_t size = dtype == LCQ_F32 ? 4 : 2, out_size = out_dtype == LCQ_F32 ? 4 : 2, logit_size = logits_dtype == LCQ_F32 ? 4 : 2;
   for (int64_t t0 = 0; t0 < T; t0 += MOST_PASS) {
     const int n = (int)least(T - t0, MOST_PASS);
+    const Cut c(n, top, E, K, I, N, dtype);
+    char* at = ws + on256(sizeof(Plan));
+    uint16_t* const h = (uint16_t*)at;
+    float* const up_sums = (float*)(at += c.h);
+    float* const out_sums = (float*)(at += c.up);
+    uint16_t* const planes = (uint16_t*)(at += c.out);
     const char* const xt = (const char*)x + t0 * ldx * size;
     RouterArgs rt = r;
     if (logits) rt.logits = (const char*)logits + t0 * ldl * logit_size;
-    const Operand o = {xt, ldx, dtype, P, (int)K, (int)Kp, planes};
+    const Operand o = {xt, ldx, dtype, c.P, (int)K, (int)Kp, planes};
     const dim3 grid(as_is ? 1u : 1u + (unsigned)least((n * Kp + 1023) / 1024, 255));
     const int* const ge = experts ? experts + t0 * top : nullptr;
     const float* const gw = experts ? weights + t0 * top : nullptr;
-    if (E <= 64) plan_kernel<1><<<grid, dim3(1024), 0, st>>>(rt, ge, gw, n, o, plan);
-    else if (E <= 256) plan_kernel<4><<<grid, dim3(1024), 0, st>>>(rt, ge, gw, n, o, plan);
-    else plan_kernel<16><<<grid, dim3(1024), 0, st>>>(rt, ge, gw, n, o, plan);
-    MoeArgs g = {as_is ? (const uint16_t*)xt : planes, as_is ? ldx : P * Kp, Kp, {gate_up, gate_up_scales, gate_up_bias, gate_up_lde, gate_up_ld, gate_up_ldse, gate_up_lds, (int)B, bias_dtype},
-                 {down, down_scales, down_bias, down_lde, down_ld, down_ldse, down_lds, (int)BI, bias_dtype}, plan, h, (char*)y + t0 * N * out_size, n, (int)K, (int)N, (int)I,
-                 (int)Kp, (int)Ip, activation, out_dtype};
-    const int64_t slots = (int64_t)n * top, groups = least(slots, least(E, slots) + slots / 16);
-    const int tiles = (int)(Ip / 16);
-    const dim3 up((unsigned)(groups * tiles));
-    if (P == 1) up_kernel<1, 2, 4><<<up, dim3(256), 0, st>>>(g, tiles);
-    else if (P == 2) up_kernel<2, 2, 4><<<up, dim3(256), 0, st>>>(g, tiles);
-    else up_kernel<3, 3, 4><<<up, dim3(256), 0, st>>>(g, tiles);
-    const dim3 dn((unsigned)((N + 15) / 16));
-    const unsigned lds = 8 * n * 64;
-    const auto run = [&](auto bf) {
-      constexpr int BF = decltype(bf)::value;
-      if (PH == 2) down_kernel<BF, 2, 8><<<dn, dim3(512), lds, st>>>(g);
-      else down_kernel<BF, 3, 8><<<dn, dim3(512), lds, st>>>(g);
-    };
-    if (out_dtype == LCQ_BF16) run(Int<ROW_BF16>{});
-    else if (out_dtype == LCQ_F16) run(Int<ROW_F16>{});
-    else run(Int<ROW_F32>{});
+    if (E <= 64) plan_kernel<1><<<grid, dim3(1024), 0, st>>>(rt, ge, gw, n, o, c.size, (int)c.groups, plan);
+    else if (E <= 256) plan_kernel<4><<<grid, dim3(1024), 0, st>>>(rt, ge, gw, n, o, c.size, (int)c.groups, plan);
+    else plan_kernel<16><<<grid, dim3(1024), 0, st>>>(rt, ge, gw, n, o, c.size, (int)c.groups, plan);
+    const MoeArgs g = {as_is ? (const uint16_t*)xt : planes, as_is ? ldx : c.P * Kp, Kp,
+                       {gate_up, gate_up_scales, gate_up_bias, gate_up_lde, gate_up_ld, gate_up_ldse, gate_up_lds, (int)B, bias_dtype},
+                       {down, down_scales, down_bias, down_lde, down_ld, down_ldse, down_lds, (int)BI, bias_dtype}, plan, h, up_sums, out_sums,
+                       (char*)y + t0 * N * out_size, n, top, (int)N, (int)I, (int)Kp, (int)Ip, activation};
+    int rc = c.P == 1 ? launch_size<false, 1, 2>(g, c, st) : c.P == 2 ? launch_size<false, 2, 2>(g, c, st) : launch_size<false, 3, 3>(g, c, st);
+    if (rc) return rc;
+    rc = c.PH == 2 ? launch_size<true, 2, 2>(g, c, st) : launch_size<true, 3, 3>(g, c, st);
+    if (rc) return rc;
+    if (out_dtype == LCQ_BF16) launch_sum<ROW_BF16>(g, c, st);
+    else if (out_dtype == LCQ_F16) launch_sum<ROW_F16>(g, c, st);
+    else launch_sum<ROW_F32>(g, c, st);
   }
   LCQ_CHECK_LAUNCH();
   return LCQ_OK;

@@ -71,7 +71,7 @@ def route_tokens(router):
     return Routing(experts, weights)
 
 
-def _experts(t, width, step):
+def _experts(t, width, step, most=MOST_DISTANCE):
     """[E, rows, width] bytes -> (t or a contiguous copy, distance between experts, between rows), on multiples of `step` bytes."""
     E, rows = t.shape[0], t.shape[1]
     lde, ld = t.stride(0), t.stride(1)
@@ -79,7 +79,7 @@ def _experts(t, width, step):
         ld = width
     if E == 1:
         lde = rows * ld
-    if t.stride(2) != 1 or not width <= ld <= MOST_DISTANCE or ld % step or lde % step:
+    if t.stride(2) != 1 or not width <= ld <= most or ld % step or lde % step:
         t = t.contiguous()
         lde, ld = rows * width, width
     if t.data_ptr() % step:
@@ -154,11 +154,11 @@ def mxfp4_moe(x, router, gate_up, down, *, gate_up_bias=None, down_bias=None, ac
             logits, _, ldl = _rows(on[0], E)
             correction = _whole(on[1])
         gw, g_lde, g_ld = _experts(gw, gw.shape[2], 16)
-        gs, g_ldse, g_lds = _experts(gs, gs.shape[2], 1)
+        gs, g_ldse, g_lds = _experts(gs, gs.shape[2], 1, (1 << 30) // (I + 64))
         dw, d_lde, d_ld = _experts(dw, dw.shape[2], 16)
         ds, d_ldse, d_lds = _experts(ds, ds.shape[2], 1)
         gate_up_bias, down_bias = _whole(gate_up_bias), _whole(down_bias)
-        ws = _workspace(rows, 'lcq_mxfp4_moe_workspace_bytes', T, top, K, I)
+        ws = _workspace(rows, 'lcq_mxfp4_moe_workspace_bytes', T, top, E, K, I, N, code)
         L.check(L.lib().lcq_mxfp4_moe(rows.data_ptr(), code, T, K, ld, _at(logits), logits_code, ldl, flags, _at(correction), scale, _at(experts),
                                       _at(weights), E, top, gw.data_ptr(), g_lde, g_ld, gs.data_ptr(), g_ldse, g_lds, _at(gate_up_bias),
                                       dw.data_ptr(), d_lde, d_ld, ds.data_ptr(), d_ldse, d_lds, _at(down_bias), bias_code, I, N,
