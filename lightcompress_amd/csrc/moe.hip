@@ -4,7 +4,7 @@
 //
 // The activations keep their precision.  A lane takes a block of a weight row, 16 bytes, and the conversion to bf16 applies its scale: that is
 // exact, so the products are those of the stored numbers.  bf16 tokens go into the matrix pipe as they are, others as sums of bf16 planes
-// (fp16: two, exactly; fp32: three, to 2^-24); h, which stays within the layer, as two planes (2^-17), or three for fp32 tokens.
+// (fp16: two, exactly; fp32: four); h, which stays within the layer, as two planes (2^-17), or four for fp32 tokens.
 #include "mxfp4.h"
 #include <type_traits>
 
@@ -38,17 +38,19 @@ __device__ __forceinline__ uint32_t ordered(float v) {
   const uint32_t u = f2u(v + 0.0f);
   return v != v ? 0xffffffffu : (int)u < 0 ? ~u : u | 0x80000000u;
 }
-template <int CTRL>
-__device__ __forceinline__ uint32_t dpp_u(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
+// the largest of a wave's, by lane permutations alone
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-  const auto take = [&](uint32_t o) { v = o > v ? o : v; };
-  take(dpp_u<0xB1>(v));
-  take(dpp_u<0x4E>(v));
-  take(dpp_u<0x141>(v));
-  take(dpp_u<0x140>(v));
-  take((uint32_t)__builtin_amdgcn_ds_swizzle((int)v, 0x401F));
-  const uint32_t lo = __builtin_amdgcn_readlane(v, 0), hi = __builtin_amdgcn_readlane(v, 32);
-  return lo > hi ? lo : hi;
+  const auto take = [&](auto ctrl, auto rows) {
+    const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    v = o > v ? o : v;
+  };
+  take(Int<0xB1>{}, Int<0xf>{});                    // neighbours, pairs, fours, eights: rows of 16
+  take(Int<0x4E>{}, Int<0xf>{});
+  take(Int<0x141>{}, Int<0xf>{});
+  take(Int<0x140>{}, Int<0xf>{});
+  take(Int<0x142>{}, Int<0xa>{});                   // the last of a row into the next
+  take(Int<0x143>{}, Int<0xc>{});
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 __device__ __forceinline__ double wave_sum(double v) {
   #pragma unroll
@@ -63,62 +65,107 @@ __device__ __forceinline__ double wave_sum(double v) {
 template <int NL>
 __device__ __forceinline__ void route_token(const RouterArgs& r, int64_t t, int& expert, float& weight) {
   const int lane = threadIdx.x & 63;
-  float x[NL], score[NL];
-  uint32_t key[NL];
-  float m = -__builtin_inff();
+  float x[NL], score[NL], correction[NL];
+  uint32_t key[NL], raw[NL];
+  const float none = -__builtin_inff();
+  float m = none;
+  #pragma unroll
+  for (int j = 0; j < NL; ++j) {                    // (all loads before the first use)
+    const int e = lane * NL + j < r.E ? lane * NL + j : 0;
+    raw[j] = r.dtype == LCQ_F32 ? ((const uint32_t*)r.logits)[t * r.ldl + e] : (uint32_t)((const uint16_t*)r.logits)[t * r.ldl + e];
+  }
+  #pragma unroll
+  for (int j = 0; j < NL; ++j) correction[j] = r.correction ? r.correction[lane * NL + j < r.E ? lane * NL + j : 0] : 0.0f;
   #pragma unroll
   for (int j = 0; j < NL; ++j) {
-    const int e = lane * NL + j;
-    x[j] = e < r.E ? load_any(r.logits, r.dtype, t * r.ldl + e) : -__builtin_inff();
+    x[j] = r.dtype == LCQ_F32 ? u2f(raw[j]) : r.dtype == LCQ_BF16 ? u2f(raw[j] << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)raw[j]);
+    if (lane * NL + j >= r.E) x[j] = none;
     m = nan_max(m, x[j]);
   }
-  const float none = -__builtin_inff();
-  if (!(r.flags & LCQ_ROUTE_SIGMOID)) m = team_reduce<64, true>(m);
+  m = team_reduce<64, true>(m);
+  const bool sigmoid = r.flags & LCQ_ROUTE_SIGMOID;
   if (r.correction) {
     double s[NL], sum = 0;
     #pragma unroll
     for (int j = 0; j < NL; ++j) {
-      if (r.flags & LCQ_ROUTE_SIGMOID) s[j] = 1.0 / (1.0 + exp(-(double)x[j]));
-      else { s[j] = x[j] == none ? 0.0 : exp((double)x[j] - (double)m); sum += s[j]; }
+      s[j] = exp(sigmoid ? -(double)x[j] : (double)x[j] - (double)m);
+      if (!sigmoid && x[j] == none) s[j] = 0.0;
+      sum += s[j];
     }
-    if (!(r.flags & LCQ_ROUTE_SIGMOID)) sum = wave_sum(sum);
+    sum = wave_sum(sum);
     #pragma unroll
     for (int j = 0; j < NL; ++j) {
-      const int e = lane * NL + j;
-      score[j] = (float)(r.flags & LCQ_ROUTE_SIGMOID ? s[j] : sum == 0.0 ? 0.0 : s[j] / sum);
-      key[j] = e >= r.E ? 0u : ordered(x[j] == none ? none : score[j] + r.correction[e]);
+      const double over = sigmoid ? 1.0 + s[j] : sum;
+      score[j] = (float)(over == 0.0 ? 0.0 : (sigmoid ? 1.0 : s[j]) / over);
+      key[j] = lane * NL + j >= r.E ? 0u : ordered(x[j] == none ? none : score[j] + correction[j]);
     }
   } else {
     float sum = 0;
     #pragma unroll
     for (int j = 0; j < NL; ++j) {
-      if (r.flags & LCQ_ROUTE_SIGMOID) score[j] = 1.0f / (1.0f + expf(-x[j]));
-      else { score[j] = x[j] == none ? 0.0f : expf(x[j] - m); sum += score[j]; }
+      score[j] = expf(sigmoid ? -x[j] : x[j] - m);
+      if (!sigmoid && x[j] == none) score[j] = 0.0f;
+      sum += score[j];
       key[j] = lane * NL + j < r.E ? ordered(x[j]) : 0u;
     }
-    if (!(r.flags & LCQ_ROUTE_SIGMOID)) {
-      sum = team_sum<64>(sum);
-      #pragma unroll
-      for (int j = 0; j < NL; ++j) score[j] = sum == 0.0f ? 0.0f : score[j] / sum;
+    sum = team_sum<64>(sum);
+    #pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const float over = sigmoid ? 1.0f + score[j] : sum;
+      score[j] = over == 0.0f ? 0.0f : (sigmoid ? 1.0f : score[j]) / over;
     }
   }
   expert = 0;
+  if constexpr (NL <= 4) {
+    // a lane's experts in order (neighbours change places only where the later one is larger, so equal ones stay), then the best of all lanes'
+    // first ones again and again
+    uint32_t order = 0;
+    int index[NL];
+    #pragma unroll
+    for (int j = 0; j < NL; ++j) index[j] = j;
+    #pragma unroll
+    for (int round = 0; round < NL; ++round)
+      #pragma unroll
+      for (int j = round & 1; j + 1 < NL; j += 2) {
+        const bool swap = key[j + 1] > key[j];
+        const uint32_t k = key[j], i = index[j];
+        key[j] = swap ? key[j + 1] : k;
+        index[j] = swap ? index[j + 1] : i;
+        key[j + 1] = swap ? k : key[j + 1];
+        index[j + 1] = swap ? i : index[j + 1];
+      }
+    #pragma unroll
+    for (int j = 0; j < NL; ++j) order |= (uint32_t)index[j] << 8 * j;
+    for (int s = 0; s < r.top; ++s) {
+      const int from = __builtin_ctzll(__ballot(key[0] == wave_max(key[0])));                // (the lowest lane has the lowest experts)
+      const int e = from * NL + (__builtin_amdgcn_readlane((int)order, from) & 255);
+      if (lane == s) expert = e;
+      if (lane == from) {
+        #pragma unroll
+        for (int j = 0; j < NL; ++j) key[j] = j + 1 < NL ? key[j + 1] : 0u;
+        order >>= 8;
+      }
+    }
+  } else {
+    for (int s = 0; s < r.top; ++s) {
+      uint32_t best = key[0];
+      int at = 0;
+      #pragma unroll
+      for (int j = 1; j < NL; ++j)
+        if (key[j] > best) { best = key[j]; at = j; }
+      const int from = __builtin_ctzll(__ballot(best == wave_max(best)));
+      const int e = from * NL + __builtin_amdgcn_readlane(at, from);
+      if (lane == s) expert = e;
+      #pragma unroll
+      for (int j = 0; j < NL; ++j)
+        if (lane == from && at == j) key[j] = 0;
+    }
+  }
   weight = 0;
-  for (int s = 0; s < r.top; ++s) {
-    uint32_t best = key[0];
-    int at = 0;
-    float w = score[0];
-    #pragma unroll
-    for (int j = 1; j < NL; ++j)
-      if (key[j] > best) { best = key[j]; at = j; w = score[j]; }
-    const uint32_t most = wave_max(best);
-    const int from = __builtin_ctzll(__ballot(best == most));                // (the lowest lane has the lowest experts)
-    const int e = from * NL + __builtin_amdgcn_readlane(at, from);
-    const float we = u2f(__builtin_amdgcn_readlane(f2u(w), from));
-    if (lane == s) { expert = e; weight = we; }
-    #pragma unroll
-    for (int j = 0; j < NL; ++j)
-      if (lane == from && at == j) key[j] = 0;
+  #pragma unroll
+  for (int j = 0; j < NL; ++j) {
+    const float w = u2f((uint32_t)__builtin_amdgcn_ds_bpermute(expert / NL * 4, (int)f2u(score[j])));
+    if (lane < r.top && expert % NL == j) weight = w;
   }
   if (r.flags & LCQ_ROUTE_RENORMALIZE) {
     const float sum = team_sum<64>(weight);
@@ -142,11 +189,11 @@ __global__ __launch_bounds__(256) void route_kernel(RouterArgs r, int64_t T, int
 // A pass: the slots (token and choice) sorted by expert, in groups of at most `size` of one expert.
 struct Group {
   int expert, first, count, pad;                    // first: slot
-  uint8_t token[MOST_GROUP];
+  uint32_t token[MOST_GROUP / 4];                   // four to a word
 };
 struct Plan {
   int groups, pad[15];
-  uint32_t counter[2][COUNTERS];                    // parts that are done: of gate and up, of down
+  uint32_t counter[COUNTERS];                       // parts of gate and up that are done
   int slot[MOST_PASS * MOST_TOP], expert[MOST_PASS * MOST_TOP];              // of a token's choices; slot -1: none
   float weight[MOST_PASS * MOST_TOP];
   Group group[MOST_PASS * MOST_TOP];
@@ -169,15 +216,15 @@ __device__ __forceinline__ void planes_of(float v, uint16_t* out) {
 // Workgroup 0 plans the pass; the others lay the tokens out as planes [T, planes, Kp] where they are not that already.
 template <int NL>
 __global__ __launch_bounds__(1024) void plan_kernel(RouterArgs r, const int* __restrict__ given, const float* __restrict__ given_weights, int T,
-                                                    Operand o, int size, int most_groups, Plan* __restrict__ plan) {
+                                                    Operand o, int size, Plan* __restrict__ plan) {
   if (blockIdx.x) {
     const int64_t all = (int64_t)T * o.Kp;
     for (int64_t i = (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x; i < all; i += (int64_t)(gridDim.x - 1) * 1024) {
       const int64_t t = i / o.Kp;
       const int k = (int)(i - t * o.Kp);
       const float v = k < o.K ? load_any(o.x, o.dtype, t * o.ldx + k) : 0.0f;
-      uint16_t p[3] = {};
-      planes_of<3>(v, p);
+      uint16_t p[4];
+      planes_of<4>(v, p);
       for (int q = 0; q < o.planes; ++q) o.out[(t * o.planes + q) * o.Kp + k] = p[q];
     }
     return;
@@ -194,8 +241,9 @@ __global__ __launch_bounds__(1024) void plan_kernel(RouterArgs r, const int* __r
       if (lane < r.top) { e = given[(int64_t)t * r.top + lane]; w = given_weights[(int64_t)t * r.top + lane]; }
       // a token's choices of one expert are one, with the sum of their weights
       bool later = false;
-      float sum = 0;
-      for (int s = 0; s < r.top; ++s) {
+      float sum = w;
+      for (int s = 0; s < r.top && !r.logits; ++s) {                         // (a router's are different ones)
+        if (s == 0) sum = 0;
         const int es = __builtin_amdgcn_readlane(e, s);
         const float ws = u2f(__builtin_amdgcn_readlane(f2u(w), s));
         if (es == e) { sum += ws; later = later || s < lane; }
@@ -209,7 +257,6 @@ __global__ __launch_bounds__(1024) void plan_kernel(RouterArgs r, const int* __r
     if (lane < r.top) { expert[t * r.top + lane] = e; weight[t * r.top + lane] = w; }
   }
   for (int i = tid; i < MOST_EXPERTS * (MOST_PASS / 32); i += 1024) (&chosen[0][0])[i] = 0;
-  for (int i = tid; i < 2 * COUNTERS; i += 1024) (&plan->counter[0][0])[i] = 0;
   __syncthreads();
   for (int i = tid; i < slots; i += 1024) {
     const int t = i / r.top;
@@ -230,21 +277,25 @@ __global__ __launch_bounds__(1024) void plan_kernel(RouterArgs r, const int* __r
   }
   if (lane == 63) sums[wave] = sum;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) sum += sums[w];
-  __syncthreads();
-  const uint32_t before = sum - mine;
+  uint32_t in_front = 0, all = 0;
+  #pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    in_front += w < wave ? sums[w] : 0;
+    all += sums[w];
+  }
+  const uint32_t before = in_front + sum - mine;
   place[tid] = before;
+  __syncthreads();
+  // (all stores behind the last barrier, which would wait for them)
+  const int groups = (int)(all >> 16);
+  if (tid == 0) plan->groups = groups;
+  for (int i = tid; i < COUNTERS; i += 1024) plan->counter[i] = 0;
   for (int g = 0; g * size < n; ++g) {
     Group& to = plan->group[(before >> 16) + g];
     to.expert = tid;
     to.first = (int)(before & 0xffff) + size * g;
     to.count = n - size * g < size ? n - size * g : size;
   }
-  if (tid == 1023) sums[0] = sum >> 16;
-  __syncthreads();
-  const int groups = (int)sums[0];
-  if (tid == 0) plan->groups = groups;
-  for (int g = groups + tid; g < most_groups; g += 1024) plan->group[g].count = 0;
   for (int i = tid; i < slots; i += 1024) {
     const int e = expert[i], t = i / r.top;
     int slot = -1;
@@ -253,7 +304,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(RouterArgs r, const int* __r
       for (int q = 0; q < t / 32; ++q) at += __builtin_popcount(chosen[e][q]);
       const uint32_t b = place[e];
       slot = (int)(b & 0xffff) + at;
-      plan->group[(b >> 16) + at / size].token[at % size] = (uint8_t)t;
+      ((uint8_t*)plan->group[(b >> 16) + at / size].token)[at % size] = (uint8_t)t;
     }
     plan->slot[i] = slot;
     plan->expert[i] = e;
@@ -295,24 +346,38 @@ __device__ __forceinline__ float act(float v, int activation) {
 // the tokens' operand.  K goes by in stages of 256 codes through LDS, all by direct loads, DEPTH - 1 stages ahead of the products:
 //   codes   32 rows x 128 bytes per wave, 8 rows a load: whole lines.  (Loaded straight into the matrix pipe's layout, 16 neighbouring
 //           lanes are 16 rows, and every load passes the cache 64 times for 1 KB: 3.4 TB/s.)  Piece p of row r lies at p ^ (r / 2 % 8)
-//   operand rows of 512 bytes, one per slot and plane; piece p of slot s lies at p ^ (s % 16)
+//   operand rows of 512 bytes, one per slot and plane
 //   scales  the word-aligned 32 bytes of a row that hold those of four stages, or of three where rows are off words: a load per wave and
 //           period.  (One per stage takes as many passes of the L2 as the codes: 5.55 TB/s for 6.17 without scales.)
-// so that 16 lanes of a read touch all banks once.  One barrier per stage, in front of its products: what was read before it is loaded again.
+// One barrier per stage, in front of its products: what was read before it is loaded again.
 constexpr int STAGE = 128;                          // bytes of a row's codes
 
+// P planes of a group of GS slots are ROWS rows of the operand, the columns of the matrix pipe's products in blocks of 16; what the planes of
+// a slot give is added up when a unit is done.
 template <int P, int GS>
 struct Shape {
-  static constexpr int XOPS = GS * P / 2, X = (XOPS + 3) / 4, FULL = XOPS % 4;               // loads of the operand: of all waves, of the first FULL (0: of all)
-  static constexpr int BYTES = 16384 + GS * P * 512;                         // of a stage, in LDS
+  static constexpr int ROWS = GS * P, CB = (ROWS + 15) / 16;
+  static constexpr int X = (ROWS + 7) / 8;                                   // a wave's loads of the operand, two rows each (4 rows: of two waves)
+  static constexpr int LOADS = 4 + X, FEWER = ROWS < 8 ? 4 : LOADS;          // of a stage: of the first two waves, of the others
+  static constexpr int BYTES = 16384 + ROWS * 512;                           // of a stage, in LDS
   static constexpr int DEPTH = 3 * (BYTES + 4096) <= 81920 ? 3 : 163840 / (BYTES + 4096) < 5 ? 163840 / (BYTES + 4096) : 5;      // two workgroups per CU, or one
-  static constexpr int LDS = DEPTH * (BYTES + 4096), TB = (GS + 15) / 16;
-  static_assert(DEPTH >= 3, "stages in LDS");
+  static constexpr int LDS = DEPTH * (BYTES + 4096);
+  // 16-byte piece p of an operand's row r lies at p ^ turn(r).  LDS serves 16 lanes of a 16-byte read at once, of lane / 16 = 0: lanes 0 .. 3 and 12 .. 15, of
+  // 1: 4 .. 11 (and the other way round, and so on), and those read pieces 4 apart: with p ^ r two of them met in a bank.
+  __device__ static constexpr int turn(int r) { return ROWS == 4 ? r : ROWS == 8 ? (r & 3) | (r & 4) << 1 : (r & 15) ^ (((r & 15) + 4 & 8) >> 1); }
+  static_assert(DEPTH >= 3 && (P & (P - 1)) == 0 && (GS & (GS - 1)) == 0, "stages in LDS");
 };
 
 typedef __attribute__((address_space(3))) char* lds_ptr;
+template <class T> __device__ __forceinline__ T from_lds(uint32_t at) { return *(const __attribute__((address_space(3))) T*)(lds_ptr)(size_t)at; }
 // what no kernel writes while this one reads it: loaded by the scalar unit, apart from the stream of vector loads
-template <class T> __device__ __forceinline__ T fixed(const T& v) { return *(const __attribute__((address_space(4))) T*)(uintptr_t)&v; }
+template <class T>
+__device__ __forceinline__ T fixed(const T& v) {
+  struct Words { uint32_t of[sizeof(T) / 4]; } w;
+  #pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) / 4); ++i) w.of[i] = ((const __attribute__((address_space(4))) uint32_t*)(uintptr_t)&v)[i];
+  return __builtin_bit_cast(T, w);
+}
 
 // Workgroups that share a result: the last of `parts` to come here has what all of them stored.
 __device__ __forceinline__ bool last_of(uint32_t* counter, int parts) {
@@ -326,37 +391,44 @@ __device__ __forceinline__ bool last_of(uint32_t* counter, int parts) {
   return true;
 }
 
-// Gate and up (DOWN false): a workgroup has 64 channels of h of one group, and one of `parts` parts of K.
-// Down: 128 channels, and a run of the units (group, part of K: `parts` of each); the last workgroup of a tile's `runs` sums up a token's choices.
+// Units of work, one behind the other without a break in the stream of loads:
+//   gate and up (DOWN false): (group, tile of 64 channels of h, one of `parts` parts of K), a workgroup takes every gridDim.x-th;
+//   down: (group, part of K) of one tile of 128 channels, a workgroup takes one of `runs` runs of them.
+// With one wave per SIMD it is bound by the instructions it issues, so what is the same for all stages of a unit, or for all but its last, is
+// not looked at in every stage.
 template <bool DOWN, int P, int GS, int PH>
 __global__ __launch_bounds__(256) void experts_kernel(MoeArgs g, int tiles, int parts, int runs) {
   typedef Shape<P, GS> S;
-  constexpr int TB = S::TB, DEPTH = S::DEPTH;
-  extern __shared__ __attribute__((aligned(1024))) char lds[];               // DEPTH stages
+  constexpr int CB = S::CB, DEPTH = S::DEPTH, WIDTH = DOWN ? 128 : 64;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];               // DEPTH stages, then as many places of scales
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Weights& w = DOWN ? g.down : g.gate_up;
-  const int bytes = w.B * 16, stages = (bytes + STAGE - 1) / STAGE;
-  int tile, unit, end;                              // units are numbered group by group
+  // What a new unit asks of the arguments is loaded again there: kept all the time it would not fit the scalar registers.
+  const auto args = [] {
+    auto p = (const __attribute__((address_space(4))) MoeArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return (const MoeArgs*)p;
+  };
+  const int B = DOWN ? g.down.B : g.gate_up.B, stages = (B + 7) / 8;         // blocks of a row
+  const bool ragged = B % 8 != 0;                   // the last stage is not whole
+  struct Who { int expert, first, count; };
+  const auto who = [&](const Plan* plan, int group) {
+    const Group& in = plan->group[group];
+    return Who{fixed(in.expert), fixed(in.first), fixed(in.count)};
+  };
+  const int groups = fixed(g.plan->groups);
+  int unit, end, step = 1, tile = 0;
   if constexpr (DOWN) {
-    const int run = blockIdx.x / tiles, units = fixed(g.plan->groups) * parts;
+    const int run = blockIdx.x / tiles, units = groups * parts;
     tile = blockIdx.x - run * tiles;
-    unit = (int)((uint32_t)units * (uint32_t)run / (uint32_t)runs);       // (fewer than 2^19 units, 2^10 runs)
+    unit = (int)((uint32_t)units * (uint32_t)run / (uint32_t)runs);          // (fewer than 2^19 units, 2^10 runs)
     end = (int)((uint32_t)units * (uint32_t)(run + 1) / (uint32_t)runs);
   } else {
-    const int all = blockIdx.x / parts, group = all / tiles;
-    tile = all - group * tiles;
-    unit = group * parts + (blockIdx.x - all * parts);
-    end = unit + 1;
-    if (fixed(g.plan->group[group].count) == 0) return;
+    unit = blockIdx.x;
+    end = groups * tiles * parts;
+    step = gridDim.x;
   }
-  constexpr int WIDTH = DOWN ? 128 : 64;
-  const int channels = DOWN ? g.N : g.I, n0 = tile * WIDTH + wave * (WIDTH / 4);
-  // rows of each half of 16: channels n0 .. (their gates, and their ups I rows behind; down: and n0 + 16 ..)
-  int rows[2] = {channels - n0, channels - n0 - (DOWN ? 16 : 0)};
-  #pragma unroll
-  for (int u = 0; u < 2; ++u) rows[u] = rows[u] < 0 ? 0 : rows[u] > 16 ? 16 : rows[u];
-  const int64_t second = DOWN ? 16 : g.I;           // rows from a first half to its second
+  if (unit >= end) return;
 
   const auto one = [](uint32_t v) { return (int)__builtin_amdgcn_readfirstlane((int)v); };
   const auto buffer = [&](const void* p, int64_t size) {
@@ -368,203 +440,249 @@ __global__ __launch_bounds__(256) void experts_kernel(MoeArgs g, int tiles, int 
   };
   const uint32_t lds0 = (uint32_t)(size_t)(lds_ptr)lds;
 
-  // ---- loads: a place in the sequence of stages, and what depends on its group alone ----
-  uint32_t wof[4], xof[S::X], sof;
-  #pragma unroll
-  for (int l = 0; l < 4; ++l) {
-    const int r = l * 8 + (lane >> 3), in = r & 15;
-    wof[l] = in < rows[l >> 1] ? (uint32_t)(in * w.ldw) + (((lane & 7) ^ (r >> 1 & 7)) << 4) : OUTSIDE;
-  }
-  const int piece = (lane & 7) ^ (lane >> 4 & 3);   // of 16 bytes in a row of codes; in odd loads 4 more, as 8 rows turn it
-  const i32x4 bufX = DOWN ? buffer(g.h, 0x7fffffff) : buffer(g.x, 0x7fffffff);
-  i32x4 bufW[2], bufS;
-  const int row_bytes = (DOWN ? g.Ip : g.Kp) * 2;
-  // the first stage of part p of a group
+  // ---- loads: a place in the sequence of stages, and what depends on its unit alone ----
+  // the first stage of part p
   const auto first_of = [&](int p) { return (int)((uint32_t)(stages * p) / (uint32_t)parts); };
-  struct Place { int unit, group, part, k, end; } at;
+  struct Place { int unit, group, tile, part, k, end; } at;
   const auto go = [&](Place& to, int u) {
     to.unit = u;
-    to.group = (uint32_t)u / (uint32_t)parts;
-    to.part = u - to.group * parts;
+    const int all = (uint32_t)u / (uint32_t)parts;
+    to.part = u - all * parts;
+    to.group = DOWN ? all : (uint32_t)all / (uint32_t)tiles;
+    to.tile = DOWN ? tile : all - to.group * tiles;
     to.k = first_of(to.part);
     to.end = first_of(to.part + 1);
   };
-  const int period = ((uintptr_t)w.s | (uintptr_t)w.ldse | (uintptr_t)w.lds) & 3 ? 3 : 4;    // stages
+  // a wave's channels, and rows of their two halves of 16: gates, and their ups I rows behind; down: and the next 16
+  struct Rows { int n0, second, of[2]; };
+  const auto rows_of = [&](const Place& p, int channels) {
+    Rows r;
+    r.n0 = p.tile * WIDTH + wave * (WIDTH / 4);
+    r.second = DOWN ? 16 : channels;
+    #pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int left = channels - r.n0 - (DOWN ? 16 * u : 0);
+      r.of[u] = left < 0 ? 0 : left > 16 ? 16 : left;
+    }
+    return r;
+  };
+  // 16-byte piece of a row in a lane's place: of codes (in odd loads 4 more, as 8 rows turn it), and of the operand
+  const int piece = (lane & 7) ^ (lane >> 4 & 3);
+  const auto operand_piece = [&](int o) { return (lane & 31) ^ S::turn((wave + 4 * o) * 2 + (lane >> 5)); };
+  const i32x4 bufX = buffer(DOWN ? g.h : g.x, 0x7fffffff);
+  const int period = [&](const Weights& w) { return ((uintptr_t)w.s | (uintptr_t)w.ldse | (uintptr_t)w.lds) & 3 ? 3 : 4; }(DOWN ? g.down : g.gate_up);     // stages
+  uint32_t wof[4], xof[S::X], sof;
+  i32x4 bufW[2], bufS;
   const auto enter = [&]() {
-    const Group& in = g.plan->group[at.group];
-    const int e = fixed(in.expert), first = fixed(in.first), count = fixed(in.count);
+    const MoeArgs* const a = args();
+    const Weights w = fixed(DOWN ? a->down : a->gate_up);
+    const Plan* const plan = fixed(a->plan);
+    const auto [e, first, count] = who(plan, at.group);
+    const Rows rows = rows_of(at, DOWN ? fixed(a->N) : fixed(a->I));
+    const int64_t second = rows.second, ldx = DOWN ? 0 : fixed(a->ldx), ldp = DOWN ? fixed(a->Ip) : fixed(a->ldp);
     #pragma unroll
     for (int u = 0; u < 2; ++u)
-      bufW[u] = buffer(w.w + e * w.lde + (n0 + u * second) * w.ldw, rows[u] ? (rows[u] - 1) * w.ldw + bytes : 0);
-    // scales of the wave's rows: from the first half's first row to the second half's last
-    const uint8_t* const s = w.s + e * w.ldse + n0 * w.lds;
-    const int early = (int)((uintptr_t)s & 3);
-    bufS = buffer(s - early, rows[0] ? (early + (rows[1] ? second + rows[1] - 1 : rows[0] - 1) * w.lds + w.B + 3) & ~(int64_t)3 : 0);
-    const int r = lane >> 1;
-    sof = (r & 15) < rows[r >> 4] ? ((uint32_t)(early + ((r & 15) + (r >> 4) * second) * w.lds) & ~3u) + (lane & 1) * 16 : OUTSIDE;
+      bufW[u] = buffer(w.w + e * w.lde + (rows.n0 + u * second) * w.ldw, rows.of[u] ? (rows.of[u] - 1) * w.ldw + B * 16 : 0);
     #pragma unroll
-    for (int o = 0; o < S::X; ++o) {
-      const int r = (wave + 4 * o) * 2 + (lane >> 5), slot = r / P, plane = r - slot * P;
-      xof[o] = OUTSIDE;
-      if (slot < count) {                           // (of a group that is not full: zeros)
-        if constexpr (DOWN) xof[o] = (uint32_t)((first + slot) * P + plane) * (uint32_t)(g.Ip * 2);
-        else xof[o] = (uint32_t)((in.token[slot] * g.ldx + plane * g.ldp) * 2);
+    for (int l = 0; l < 4; ++l) {
+      const int in = (l & 1) * 8 + (lane >> 3);
+      wof[l] = in < rows.of[l >> 1] ? (uint32_t)(in * w.ldw) + ((piece ^ (l & 1) * 4) << 4) : OUTSIDE;
+    }
+    // scales: from the first half's first row to the second half's last
+    const uint8_t* const s = w.s + e * w.ldse + rows.n0 * w.lds;
+    const int early = (int)((uintptr_t)s & 3);
+    bufS = buffer(s - early, rows.of[0] ? (early + (rows.of[1] ? second + rows.of[1] - 1 : rows.of[0] - 1) * w.lds + w.B + 3) & ~(int64_t)3 : 0);
+    const int r = lane >> 1;
+    sof = (r & 15) < (r & 16 ? rows.of[1] : rows.of[0]) ? ((uint32_t)(early + ((r & 15) + (r >> 4) * second) * w.lds) & ~3u) + (lane & 1) * 16 : OUTSIDE;
+    #pragma unroll
+    for (int o = 0; o < S::X; ++o) {                // two rows of the operand; of a group that is not full: zeros
+      uint32_t of[2];
+      #pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = (wave + 4 * o) * 2 + i, slot = r / P, plane = r % P;
+        if constexpr (DOWN) of[i] = (uint32_t)((first + slot) * P + plane) * (uint32_t)(ldp * 2);
+        else {
+          const int token = slot < count ? (int)(fixed(plan->group[at.group].token[slot >> 2]) >> 8 * (slot & 3) & 255) : 0;
+          of[i] = (uint32_t)((token * ldx + plane * ldp) * 2);
+        }
+        if (slot >= count) of[i] = OUTSIDE;
       }
+      xof[o] = (lane & 32 ? of[1] : of[0]) + operand_piece(o) * 16;
     }
   };
   // The next stage, into a place; behind the last one: nothing, from outside.  The scales of a period come in front of its first stage.
   int lperiod = 0, lplace = DEPTH - 1;
   const auto fetch = [&](int slot) {
-    const uint32_t over = at.unit < end ? 0u : OUTSIDE, to = lds0 + slot * S::BYTES;
+    const uint32_t to = lds0 + slot * S::BYTES + wave * 4096, too = lds0 + slot * S::BYTES + 16384 + wave * 1024;
+    const bool over = at.unit >= end;
     if (lperiod == 0) {
       lplace = lplace == DEPTH - 1 ? 0 : lplace + 1;
-      load(lds0 + DEPTH * S::BYTES + (lplace * 4 + wave) * 1024, sof | over, bufS, at.k * 8);
+      load(lds0 + DEPTH * S::BYTES + (lplace * 4 + wave) * 1024, over ? OUTSIDE : sof, bufS, at.k * 8);
       lperiod = period;
     }
     --lperiod;
-    #pragma unroll
-    for (int l = 0; l < 4; ++l) {
-      const uint32_t outside = (piece ^ (l & 1) * 4) * 16 < bytes - at.k * STAGE ? over : OUTSIDE;
-      load(to + (wave * 4 + l) * 1024, wof[l] | outside, bufW[l >> 1], at.k * STAGE);
+    if (over || (ragged && at.k == stages - 1)) {
+      const int left = over ? 0 : B - at.k * 8;   // blocks
+      #pragma unroll
+      for (int l = 0; l < 4; ++l) load(to + l * 1024, (piece ^ (l & 1) * 4) < left ? wof[l] : OUTSIDE, bufW[l >> 1], at.k * STAGE);
+      #pragma unroll
+      for (int o = 0; o < S::X; ++o)
+        if (S::ROWS >= 8 || wave < 2) load(too + o * 4096, operand_piece(o) < left * 4 ? xof[o] : OUTSIDE, bufX, at.k * 512);
+    } else {
+      #pragma unroll
+      for (int l = 0; l < 4; ++l) load(to + l * 1024, wof[l], bufW[l >> 1], at.k * STAGE);
+      #pragma unroll
+      for (int o = 0; o < S::X; ++o)
+        if (S::ROWS >= 8 || wave < 2) load(too + o * 4096, xof[o], bufX, at.k * 512);
     }
-    #pragma unroll
-    for (int o = 0; o < S::X; ++o) {
-      const int x = wave + 4 * o;
-      if (S::FULL && o == S::X - 1 && wave >= S::FULL) break;
-      const int p = (lane & 31) ^ ((x * 2 + (lane >> 5)) / P & 15);          // piece of an operand's row
-      load(to + 16384 + x * 1024, (xof[o] + p * 16) | over | (p * 16 + at.k * 512 < row_bytes ? 0u : OUTSIDE), bufX, at.k * 512);
-    }
-    if (++at.k == at.end && at.unit < end) {
-      go(at, at.unit + 1);
+    if (++at.k == at.end && !over) {
+      go(at, at.unit + step);
       lperiod = 0;
-      if (DOWN && at.unit < end) enter();
+      if (at.unit < end) enter();
     }
   };
 
-  f32x4 acc[2][TB] = {};
-  if (unit < end) {
-    go(at, unit);
-    enter();
-    #pragma unroll
-    for (int d = 0; d < DEPTH - 1; ++d) fetch(d);
-    // ---- products ----
-    Place now;
-    int slot = 0, first = 0, count = 0, early[2];
-    const auto begin = [&]() {
-      const Group& in = g.plan->group[now.group];
-      const int e = fixed(in.expert);
-      first = fixed(in.first);
-      count = fixed(in.count);
-      #pragma unroll
-      for (int u = 0; u < 2; ++u) early[u] = (int)((uint32_t)(uintptr_t)w.s + (uint32_t)e * (uint32_t)w.ldse + (uint32_t)(n0 + c + u * (int)second) * (uint32_t)w.lds) & 3;
-    };
-    go(now, unit);
-    begin();
-    const char* const codes = lds + wave * 4096 + c * 128;
-    const char* const scales = lds + DEPTH * S::BYTES + wave * 1024 + c * 32 + q;
-    const int turn = c >> 1 & 7;
-    int cperiod = 0, cplace = DEPTH - 1;
-    constexpr int MORE = (DEPTH - 2) * (4 + S::X), LESS = (DEPTH - 2) * (3 + S::X);          // loads that may be on their way
-    while (now.unit < end) {
-      // the next stage has landed, and this wave has read the last one
-      if (S::FULL && wave >= S::FULL) __builtin_amdgcn_s_waitcnt(0x0070 | (LESS & 15) | LESS >> 4 << 14);
-      else __builtin_amdgcn_s_waitcnt(0x0070 | (MORE & 15) | MORE >> 4 << 14);
-      asm volatile("s_barrier" ::: "memory");
-      fetch(slot == 0 ? DEPTH - 1 : slot - 1);
-      if (cperiod == 0) cplace = cplace == DEPTH - 1 ? 0 : cplace + 1;
-      const int here = slot * S::BYTES, scales_here = cplace * 4096 + cperiod * 8;
-      cperiod = cperiod == period - 1 ? 0 : cperiod + 1;
-      i32x4 wv[2][2];
-      float f[2][2];
+  // ---- a unit's results: accumulator register r of lane l is channel 4 (l / 16) + r of column l % 16 ----
+  const auto leave = [&](const Place& p, const Who& of, f32x4 (&acc)[2][CB]) {
+    const MoeArgs* const a = args();
+    const Weights w = fixed(DOWN ? a->down : a->gate_up);
+    const int channels = DOWN ? fixed(a->N) : fixed(a->I), Ip = fixed(a->Ip), activation = fixed(a->activation);
+    const Rows rows = rows_of(p, channels);
+    if (!DOWN && parts > 1) {
+      const int shared = p.group * tiles + p.tile;  // by the parts
+      f32x4* const mine = (f32x4*)fixed(a->up) + ((int64_t)shared * parts * 256 + tid) * (2 * CB);
       #pragma unroll
       for (int u = 0; u < 2; ++u)
         #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          wv[u][i] = *(const i32x4*)(codes + here + u * 2048 + (((i * 4 + q) ^ turn) << 4));
-          const uint32_t byte = *(const uint8_t*)(scales + scales_here + u * 512 + early[u] + i * 4);
-          f[u][i] = mx_factor(now.k * 8 + i * 4 + q < w.B ? byte : 0u);      // (behind the last block: not a NaN)
-        }
+        for (int b = 0; b < CB; ++b) mine[(int64_t)p.part * 512 * CB + u * CB + b] = acc[u][b];
+      if (!last_of(&fixed(a->plan)->counter[shared], parts)) return;
       #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int u = 0; u < 2; ++u)
+        #pragma unroll
+        for (int b = 0; b < CB; ++b) {
+          acc[u][b] = f32x4{};
+          for (int s = 0; s < parts; ++s) acc[u][b] += mine[(int64_t)s * 512 * CB + u * CB + b];
+        }
+    }
+    #pragma unroll
+    for (int b = 0; b < CB; ++b) {
+      #pragma unroll
+      for (int u = 0; u < 2; ++u)
+        #pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if constexpr (P >= 2) acc[u][b][r] += lane_xor<1>(acc[u][b][r]);
+          if constexpr (P >= 4) acc[u][b][r] += lane_xor<2>(acc[u][b][r]);
+        }
+      const int s = (b * 16 + c) / P, mine = c % P; // all lanes of a slot have its sums
+      if (s >= of.count || (S::ROWS < 16 && c >= S::ROWS)) continue;
+      if constexpr (DOWN) {
+        #pragma unroll
+        for (int u = 0; u < 2; ++u)                 // (rows of whole fours; what lies behind N is not read)
+          if (mine == 0 && q * 4 < rows.of[u])
+            *(f32x4*)(fixed(a->out) + ((int64_t)(of.first + s) * parts + p.part) * ((channels + 3) & ~3) + rows.n0 + u * 16 + q * 4) = acc[u][b];
+      } else {
+        if (rows.n0 + q * 4 >= Ip) continue;
+        uint16_t h[4][PH];
+        #pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int ch = q * 4 + r;
+          float v[2] = {acc[0][b][r], acc[1][b][r]};
+          if (w.bias && ch < rows.of[0]) {
+            #pragma unroll
+            for (int u = 0; u < 2; ++u) v[u] += load_any(w.bias, w.bias_dtype, ((int64_t)of.expert * 2 + u) * channels + rows.n0 + ch);
+          }
+          planes_of<PH>(ch < rows.of[0] ? act(v[0], activation) * v[1] : 0.0f, h[r]);
+        }
+        #pragma unroll
+        for (int l = 0; l < PH; ++l)
+          if (l % P == mine)
+            *(u32x2*)(fixed(a->h) + ((int64_t)(of.first + s) * PH + l) * Ip + rows.n0 + q * 4) = u32x2{h[0][l] | (uint32_t)h[1][l] << 16, h[2][l] | (uint32_t)h[3][l] << 16};
+      }
+    }
+  };
+
+  // ---- products ----
+  go(at, unit);
+  enter();
+  #pragma unroll
+  for (int d = 0; d < DEPTH - 1; ++d) fetch(d);
+  Place now;
+  Who in;
+  uint32_t scales[2];                               // this lane's: of a row whose bytes start (row's address) % 4 early
+  const auto begin = [&]() {
+    const MoeArgs* const a = args();
+    const Weights w = fixed(DOWN ? a->down : a->gate_up);
+    in = who(fixed(a->plan), now.group);
+    const Rows rows = rows_of(now, DOWN ? fixed(a->N) : fixed(a->I));
+    #pragma unroll
+    for (int u = 0; u < 2; ++u)
+      scales[u] = lds0 + DEPTH * S::BYTES + wave * 1024 + u * 512 + c * 32 + q +
+                  (((uint32_t)(uintptr_t)w.s + (uint32_t)in.expert * (uint32_t)w.ldse + (uint32_t)(rows.n0 + c + u * rows.second) * (uint32_t)w.lds) & 3);
+  };
+  go(now, unit);
+  begin();
+  uint32_t codes[2], operand[4];
+  #pragma unroll
+  for (int i = 0; i < 2; ++i) codes[i] = lds0 + wave * 4096 + c * 128 + (((i * 4 + q) ^ (c >> 1 & 7)) << 4);
+  const int row = S::ROWS < 16 ? c & (S::ROWS - 1) : c;
+  #pragma unroll
+  for (int j = 0; j < 4; ++j) operand[j] = lds0 + 16384 + row * 512 + (((q * 4 + j) ^ S::turn(row)) << 4);
+  int slot = 0, cperiod = 0, cplace = 0;
+  for (;;) {
+    f32x4 acc[2][CB] = {};
+    do {
+      // the next stage has landed, and this wave has read the last one
+      constexpr int MORE = (DEPTH - 2) * S::LOADS, LESS = (DEPTH - 2) * S::FEWER;              // loads that may be on their way
+      if (MORE != LESS && wave >= 2) __builtin_amdgcn_s_waitcnt(0x0070 | (LESS & 15) | LESS >> 4 << 14);
+      else __builtin_amdgcn_s_waitcnt(0x0070 | (MORE & 15) | MORE >> 4 << 14);
+      asm volatile("s_barrier" ::: "memory");
+      fetch(slot == 0 ? DEPTH - 1 : slot - 1);
+      const uint32_t here = slot * S::BYTES, scales_here = cplace * 4096 + cperiod * 8;
+      // all reads of the stage, then the products: left to itself the compiler has two of them on their way, and a wave alone on its SIMD waits
+      // for each
+      i32x4 wv[2][2];
+      uint32_t byte[2][2];
+      bf16x8 x[2][4][CB];
+      #pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        #pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          wv[u][i] = from_lds<i32x4>(codes[i] + here + u * 2048);
+          byte[u][i] = from_lds<uint8_t>(scales[u] + scales_here + i * 4);
+        }
+        #pragma unroll
+        for (int j = 0; j < 4; ++j)
+          #pragma unroll
+          for (int b = 0; b < CB; ++b) x[i][j][b] = from_lds<bf16x8>(operand[j] + here + i * 256 + b * 8192);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      const int left = B - now.k * 8;
+      #pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t there = i * 4 + q < left ? 255u : 0u;                 // (behind the last block: not a NaN)
         #pragma unroll
         for (int j = 0; j < 4; ++j) {
           bf16x8 v[2];
           #pragma unroll
-          for (int u = 0; u < 2; ++u) v[u] = decoded(wv[u][i][j], f[u][i]);
+          for (int u = 0; u < 2; ++u) v[u] = decoded(wv[u][i][j], mx_factor(byte[u][i] & there));
           #pragma unroll
-          for (int b = 0; b < TB; ++b)
+          for (int b = 0; b < CB; ++b)
             #pragma unroll
-            for (int l = P - 1; l >= 0; --l) {
-              const int s = (b * 16 + c) & (GS - 1);
-              const bf16x8 x = *(const bf16x8*)(lds + here + 16384 + (s * P + l) * 512 + (((i * 16 + q * 4 + j) ^ (s & 15)) << 4));
-              #pragma unroll
-              for (int u = 0; u < 2; ++u) acc[u][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u], x, acc[u][b], 0, 0, 0);
-            }
+            for (int u = 0; u < 2; ++u) acc[u][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u], x[i][j][b], acc[u][b], 0, 0, 0);
         }
-      slot = slot == DEPTH - 1 ? 0 : slot + 1;
-      if (++now.k == now.end) {
-        if constexpr (DOWN) {
-          #pragma unroll
-          for (int b = 0; b < TB; ++b) {
-            const int s = b * 16 + c;
-            #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              // (rows of whole fours; what lies behind N is not read)
-              if (s < count && q * 4 < rows[u])
-                *(f32x4*)(g.out + ((int64_t)(first + s) * parts + now.part) * ((g.N + 3) & ~3) + n0 + u * 16 + q * 4) = acc[u][b];
-              acc[u][b] = f32x4{};
-            }
-          }
-        }
-        go(now, now.unit + 1);
-        cperiod = 0;
-        if (DOWN && now.unit < end) begin();
       }
-    }
+      slot = slot == DEPTH - 1 ? 0 : slot + 1;
+      cperiod = cperiod == period - 1 ? 0 : cperiod + 1;
+      if (cperiod == 0) cplace = cplace == DEPTH - 1 ? 0 : cplace + 1;
+    } while (++now.k < now.end);
+    leave(now, in, acc);
+    go(now, now.unit + step);
+    if (now.unit >= end) break;
+    begin();
+    if (cperiod) cplace = cplace == DEPTH - 1 ? 0 : cplace + 1;                // (a unit starts a period)
+    cperiod = 0;
   }
   __builtin_amdgcn_s_waitcnt(0x0f70);               // nothing may still be on its way to LDS when the workgroup leaves it
-
-  // ---- results: accumulator register r of lane l is channel 4 (l / 16) + r of slot l % 16 ----
-  if constexpr (!DOWN) {
-    const int group = unit / parts;
-    const Group& in = g.plan->group[group];
-    if (parts > 1) {
-      f32x4* const mine = (f32x4*)g.up + ((int64_t)(blockIdx.x / parts) * parts * 256 + tid) * (2 * TB);
-      #pragma unroll
-      for (int u = 0; u < 2; ++u)
-        #pragma unroll
-        for (int b = 0; b < TB; ++b) mine[(int64_t)(unit - group * parts) * 512 * TB + u * TB + b] = acc[u][b];
-      if (!last_of(&g.plan->counter[0][blockIdx.x / parts], parts)) return;
-      #pragma unroll
-      for (int u = 0; u < 2; ++u)
-        #pragma unroll
-        for (int b = 0; b < TB; ++b) {
-          acc[u][b] = f32x4{};
-          for (int p = 0; p < parts; ++p) acc[u][b] += mine[(int64_t)p * 512 * TB + u * TB + b];
-        }
-    }
-    const int e = in.expert, count = in.count, first = in.first;
-    if (n0 + q * 4 >= g.Ip) return;
-    #pragma unroll
-    for (int b = 0; b < TB; ++b) {
-      const int s = b * 16 + c;
-      if (s >= count) continue;
-      uint16_t p[4][PH];
-      #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int ch = q * 4 + r;
-        float v[2] = {acc[0][b][r], acc[1][b][r]};
-        if (w.bias && ch < rows[0]) {
-          #pragma unroll
-          for (int u = 0; u < 2; ++u) v[u] += load_any(w.bias, w.bias_dtype, ((int64_t)e * 2 + u) * g.I + n0 + ch);
-        }
-        planes_of<PH>(ch < rows[0] ? act(v[0], g.activation) * v[1] : 0.0f, p[r]);
-      }
-      #pragma unroll
-      for (int l = 0; l < PH; ++l)
-        *(u32x2*)(g.h + ((int64_t)(first + s) * PH + l) * g.Ip + n0 + q * 4) = u32x2{p[0][l] | (uint32_t)p[1][l] << 16, p[2][l] | (uint32_t)p[3][l] << 16};
-    }
-  }
 }
 
 // y of four channels of a token per lane: the weighted sum of its choices' parts in their order, eight of them on their way at a time in each of
@@ -642,10 +760,10 @@ struct Cut {
   int P, PH, size, up_tiles, up_parts, down_tiles, down_parts, runs;
   int64_t groups, h, up, out;                       // bytes
   Cut(int64_t T, int64_t top, int64_t E, int64_t K, int64_t I, int64_t N, int dtype) {
-    P = dtype == LCQ_BF16 ? 1 : dtype == LCQ_F16 ? 2 : 3;
-    PH = dtype == LCQ_F32 ? 3 : 2;
+    P = dtype == LCQ_BF16 ? 1 : dtype == LCQ_F16 ? 2 : 4;
+    PH = dtype == LCQ_F32 ? 4 : 2;
     const int64_t slots = T * top;
-    size = T <= 4 || slots <= E ? 4 : P == 3 || T <= 16 || slots <= 14 * E ? 16 : 32;
+    size = T <= 4 || slots <= E ? 4 : P == 4 || T <= 16 || slots <= 14 * E ? 16 : 32;
     groups = least(slots, least(E, slots) + slots / size);
     const int64_t up_stages = ((K + 31) / 32 + 7) / 8, down_stages = ((I + 31) / 32 + 7) / 8, Ip = (I + 31) / 32 * 32;
     up_tiles = (int)((Ip + 63) / 64);
@@ -655,11 +773,11 @@ struct Cut {
     int64_t want = 512 / down_tiles;
     if (want < 1) want = 1;
     down_parts = 1;
-    while (groups * down_parts < 8 * want && down_stages / (2 * down_parts) >= 2) down_parts *= 2;
+    while (groups * down_parts < 6 * want && down_stages / (2 * down_parts) >= 6) down_parts *= 2;
     const int64_t units = groups * down_parts, each = (units + want - 1) / want;
     runs = (int)((units + each - 1) / each);
     h = on256(slots * PH * Ip * 2);
-    up = up_parts > 1 ? on256(groups * up_tiles * up_parts * 256 * 32 * (size > 16 ? 2 : 1)) : 0;
+    up = up_parts > 1 ? on256(groups * up_tiles * up_parts * 256 * 32 * ((size * P + 15) / 16)) : 0;
     out = on256(slots * down_parts * ((N + 3) & ~(int64_t)3) * 4);
   }
 };
@@ -670,15 +788,15 @@ int launch_experts(const MoeArgs& g, const Cut& c, hipStream_t st) {
   const auto kernel = experts_kernel<DOWN, P, GS, PH>;
   // (more LDS than a launch may have without asking)
   if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS) != hipSuccess) return LCQ_ELAUNCH;
-  const int64_t blocks = DOWN ? (int64_t)c.down_tiles * c.runs : c.groups * c.up_tiles * c.up_parts;
-  if (blocks > (1 << 24) - 1) return LCQ_ESIZE;
+  // as many as run at a time, or fewer
+  const int64_t blocks = DOWN ? (int64_t)c.down_tiles * c.runs : least(c.groups * c.up_tiles * c.up_parts, 256 * (163840 / S::LDS));
   kernel<<<dim3((unsigned)blocks), dim3(256), S::LDS, st>>>(g, DOWN ? c.down_tiles : c.up_tiles, DOWN ? c.down_parts : c.up_parts, c.runs);
   return LCQ_OK;
 }
 template <bool DOWN, int P, int PH>
 int launch_size(const MoeArgs& g, const Cut& c, hipStream_t st) {
   if (c.size == 4) return launch_experts<DOWN, P, 4, PH>(g, c, st);
-  if constexpr (P < 3) { if (c.size == 32) return launch_experts<DOWN, P, 32, PH>(g, c, st); }
+  if constexpr (P < 4) { if (c.size == 32) return launch_experts<DOWN, P, 32, PH>(g, c, st); }
   return launch_experts<DOWN, P, 16, PH>(g, c, st);
 }
 template <int BF>
@@ -712,7 +830,7 @@ int64_t lcq_mxfp4_moe_workspace_bytes(int64_t T, int64_t top, int64_t E, int64_t
   int64_t most = 0;                                 // (the last pass may have fewer tokens, and be cut into more parts)
   for (const int64_t n : {t, T % MOST_PASS ? T % MOST_PASS : t}) {
     const Cut c(n, top, E, K, I, N, dtype);
-    const int64_t size = c.h + c.up + c.out + on256(n * c.P * ((K + 31) / 32 * 32) * 2);
+    const int64_t size = c.h + c.up + c.out + on256(n * c.P * ((K + 31) / 32 * 32) * 2) + on256(n * top * 8);
     most = size > most ? size : most;
   }
   return on256(sizeof(Plan)) + most;
@@ -756,18 +874,26 @@ int lcq_mxfp4_moe(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, c
     if (logits) rt.logits = (const char*)logits + t0 * ldl * logit_size;
     const Operand o = {xt, ldx, dtype, c.P, (int)K, (int)Kp, planes};
     const dim3 grid(as_is ? 1u : 1u + (unsigned)least((n * Kp + 1023) / 1024, 255));
-    const int* const ge = experts ? experts + t0 * top : nullptr;
-    const float* const gw = experts ? weights + t0 * top : nullptr;
-    if (E <= 64) plan_kernel<1><<<grid, dim3(1024), 0, st>>>(rt, ge, gw, n, o, c.size, (int)c.groups, plan);
-    else if (E <= 256) plan_kernel<4><<<grid, dim3(1024), 0, st>>>(rt, ge, gw, n, o, c.size, (int)c.groups, plan);
-    else plan_kernel<16><<<grid, dim3(1024), 0, st>>>(rt, ge, gw, n, o, c.size, (int)c.groups, plan);
+    const int64_t slots = (int64_t)n * top;
+    const int* ge = experts ? experts + t0 * top : nullptr;
+    const float* gw = experts ? weights + t0 * top : nullptr;
+    if (logits && n > 16) {                         // (the waves of one workgroup would take longer)
+      int* const e = (int*)((char*)planes + on256(n * c.P * Kp * 2));
+      const int rc = lcq_route(rt.logits, logits_dtype, n, E, ldl, top, flags, correction, scale, e, (float*)(e + slots), stream);
+      if (rc) return rc;
+      ge = e;
+      gw = (float*)(e + slots);
+    }
     const MoeArgs g = {as_is ? (const uint16_t*)xt : planes, as_is ? ldx : c.P * Kp, Kp,
                        {gate_up, gate_up_scales, gate_up_bias, gate_up_lde, gate_up_ld, gate_up_ldse, gate_up_lds, (int)B, bias_dtype},
                        {down, down_scales, down_bias, down_lde, down_ld, down_ldse, down_lds, (int)BI, bias_dtype}, plan, h, up_sums, out_sums,
                        (char*)y + t0 * N * out_size, n, top, (int)N, (int)I, (int)Kp, (int)Ip, activation};
-    int rc = c.P == 1 ? launch_size<false, 1, 2>(g, c, st) : c.P == 2 ? launch_size<false, 2, 2>(g, c, st) : launch_size<false, 3, 3>(g, c, st);
+    if (E <= 64) plan_kernel<1><<<grid, dim3(1024), 0, st>>>(rt, ge, gw, n, o, c.size, plan);
+    else if (E <= 256) plan_kernel<4><<<grid, dim3(1024), 0, st>>>(rt, ge, gw, n, o, c.size, plan);
+    else plan_kernel<16><<<grid, dim3(1024), 0, st>>>(rt, ge, gw, n, o, c.size, plan);
+    int rc = c.P == 1 ? launch_size<false, 1, 2>(g, c, st) : c.P == 2 ? launch_size<false, 2, 2>(g, c, st) : launch_size<false, 4, 4>(g, c, st);
     if (rc) return rc;
-    rc = c.PH == 2 ? launch_size<true, 2, 2>(g, c, st) : launch_size<true, 3, 3>(g, c, st);
+    rc = c.PH == 2 ? launch_size<true, 2, 2>(g, c, st) : launch_size<true, 4, 4>(g, c, st);
     if (rc) return rc;
     if (out_dtype == LCQ_BF16) launch_sum<ROW_BF16>(g, c, st);
     else if (out_dtype == LCQ_F16) launch_sum<ROW_F16>(g, c, st);
