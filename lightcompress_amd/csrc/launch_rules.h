@@ -91,7 +91,7 @@ inline bool int8_streams(long long M, long long N, long long K) {
 // latter with K (B blocks of 32) cut into parts of at least two periods of 16 blocks.
 struct Mxfp4Cut { bool stream; int tile, parts; };  // tile 0: 256 x 256, 1: 128 x 128
 inline Mxfp4Cut mxfp4_cut(long long M, long long N, long long B) {
-  if (M <= 64) return {true, 0, 1};
+  if (M <= 32) return {true, 0, 1};
   const long long large = (M + 255) / 256 * ((N + 255) / 256), small = (M + 127) / 128 * ((N + 127) / 128), groups = (B + 15) / 16;
   if (large >= 200) return {false, 0, 1};
   int parts = 1;

@@ -34,6 +34,7 @@ __device__ __forceinline__ uint32_t load_raw(const void* p, int dtype, int64_t i
 __device__ __forceinline__ float from_raw(uint32_t u, int dtype) {
   return dtype == LCQ_F32 ? u2f(u) : dtype == LCQ_BF16 ? u2f(u << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)u);
 }
+template <class T> __device__ __forceinline__ T from_lds(uint32_t at) { return *(const __attribute__((address_space(3))) T*)(lds_ptr)(size_t)at; }
 // (the pipe reads four registers of a 4-bit operand)
 __device__ __forceinline__ i32x8 wide(i32x4 v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
 
@@ -356,76 +357,142 @@ __global__ __launch_bounds__(256) void pad_scales_kernel(MxArgs g, int Bp, uint8
 }
 
 // ---- few tokens ---------------------------------------------------------------------------------------------------
-// The weight is read once, straight into the matrix pipe's operands: a lane of v_mfma_scale_f32_16x16x128 takes a block of one of 16
-// channels, so a load of the wave is 16 rows x 64 bytes in a row, and one more brings a scale byte per lane.  A workgroup owns 16 or 32
-// channels, its waves take pieces of 512 codes of K in turn and meet in LDS; the tokens' codes come from the cache, or, where there are
-// few, every workgroup makes them itself, in LDS, while its first weights are on their way.
-constexpr int PIECE = 256;                          // bytes of a row
+// The weight streams past the tokens.  A wave has a block of 16 channels and a KS-th of K; stages of 256 codes go through its own part of LDS by
+// direct loads of whole lines, DEPTH - 1 stages ahead, without a break from one block to the next, and nothing but the joining of a
+// block's KS waves makes waves wait for one another.  (Loaded straight into the matrix pipe's layout, 16 neighbouring lanes are 16 rows and
+// every KB passes the cache 64 times: 16 tokens by 4096 x 14336 took 16.5 us.)
+//   codes of the weight and of the tokens   16 rows x 128 bytes; 16-byte piece p of row r lies at p ^ (r / 2 % 8)
+//   scales   the word-aligned 64 bytes of a row that hold those of eight stages, or of seven where rows are off words
+// Where there are few tokens, every workgroup makes their codes itself, in LDS, while its first weights are on their way.
+constexpr int STAGE_BYTES = 128;                    // of a row
+constexpr int MOST_BIASES = 64;                     // blocks of channels of a workgroup whose biases are read before the stream begins
 
 struct TokenArgs {
   const char* x;
   int64_t ldx, K;
 };
 
-// TB blocks of 16 tokens, NB blocks of 16 channels.  XT: the type of the tokens' values, or -1 for codes.
-template <int TB, int NB, int BF, int XT, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void stream_kernel(MxArgs g, TokenArgs t) {
-  __shared__ __attribute__((aligned(16))) float red[WAVES][NB][TB][64][4];
-  extern __shared__ __attribute__((aligned(16))) uint8_t made[];             // XT >= 0: [M] rows of codes, 16 B + 16 apart (16 lanes' reads touch all banks once); then of scales
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t n0 = (int64_t)blockIdx.x * (16 * NB);
-  const int rows_w = (int)(g.N - n0 < 16 * NB ? g.N - n0 : 16 * NB);
-  const int bytes = g.B * 16, q = lane >> 4;        // this lane's block of four
-  // Loads are told where their matrix ends: blocks past the last and rows past the end read as zero, without a branch.
-  const auto buffer = [](const uint8_t* p, int64_t size) { return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)size, 0x00020000); };
-  const __amdgpu_buffer_rsrc_t bufW = buffer(g.w + n0 * g.ldw, (rows_w - 1) * g.ldw + bytes), bufSW = buffer(g.sw + n0 * g.ldsw, (rows_w - 1) * g.ldsw + g.B);
-  const __amdgpu_buffer_rsrc_t bufA = buffer(g.a, XT < 0 ? (g.M - 1) * g.lda + bytes : 0), bufSA = buffer(g.sa, XT < 0 ? (g.M - 1) * g.ldsa + g.B : 0);
+template <int TB, int XT, int DEPTH_, int PLACES_>
+struct Few {
+  static constexpr int DEPTH = DEPTH_, PLACES = PLACES_, OWN = XT < 0 ? TB : 0;              // blocks of tokens that are loaded
+  static constexpr int BYTES = 2048 * (1 + OWN), SCALES = 1024 * (1 + OWN), LOADS = 2 * (1 + OWN);           // of a stage, a period, a stage's loads
+  static constexpr int WAVE = DEPTH * BYTES + PLACES * SCALES;
+  static constexpr int RED = 4 * WAVE, BIAS = RED + 2 * 4 * TB * 1024, MADE = BIAS + MOST_BIASES * 64;
+};
+
+// TB blocks of 16 tokens.  XT: the type of the tokens' values, or -1 for codes.
+template <int TB, int BF, int XT, int DEPTH, int PLACES>
+__global__ __launch_bounds__(256) void few_kernel(MxArgs g, TokenArgs t, int KS) {
+  typedef Few<TB, XT, DEPTH, PLACES> S;
+  constexpr int OWN = S::OWN;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = wave % KS, of_group = wave / KS, groups = 4 / KS;        // blocks at a time
+  const int stages = (g.B + 7) >> 3, first = stages * part / KS, last = stages * (part + 1) / KS;
+  const int blocks = (int)((g.N + 15) >> 4), rounds = (blocks + groups - 1) / groups;        // a workgroup takes every gridDim.x-th round
+  const bool ragged = g.B % 8 != 0;
+  const auto one = [](uint32_t v) { return (int)__builtin_amdgcn_readfirstlane((int)v); };
+  const auto buffer = [&](const void* p, int64_t size) {
+    const uint64_t at = (uint64_t)(uintptr_t)p;
+    return i32x4{one((uint32_t)at), one((uint32_t)(at >> 32) & 0xffff), one((uint32_t)size), 0x00020000};
+  };
+  const auto load = [&](uint32_t to, uint32_t of, i32x4 buf, int at) {       // (all but `of` are the wave's)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(one(to)), "v"(of), "s"(buf), "s"(one((uint32_t)at)) : "memory");
+  };
   constexpr uint32_t OUTSIDE = 0x80000000u;
-  uint32_t ofW[NB], ofSW[NB], ofA[TB], ofSA[TB];
-  #pragma unroll
-  for (int c = 0; c < NB; ++c) {
-    const int r = c * 16 + (lane & 15);
-    ofW[c] = r < rows_w ? (uint32_t)(r * g.ldw) + q * 16 : OUTSIDE;
-    ofSW[c] = r < rows_w ? (uint32_t)(r * g.ldsw) + q : OUTSIDE;
+  const uint32_t lds0 = (uint32_t)(size_t)(lds_ptr)lds, mine = lds0 + wave * S::WAVE;
+
+  // biases of the first blocks (loads that the compiler knows of would end the stream where they are waited for)
+  float* const biases = (float*)(lds + S::BIAS);
+  if (g.bias) {
+    for (int i = tid; i < MOST_BIASES * 16; i += 256) {
+      const int64_t n = ((int64_t)(blockIdx.x + (i >> 4) / groups * gridDim.x) * groups + (i >> 4) % groups) * 16 + (i & 15);
+      if (n < g.N) biases[i] = load_any(g.bias, g.bias_dtype, n);
+    }
   }
-  #pragma unroll
-  for (int b = 0; b < TB; ++b) {
-    const int r = b * 16 + (lane & 15);
-    ofA[b] = r < g.M ? (uint32_t)(r * g.lda) + q * 16 : OUTSIDE;
-    ofSA[b] = r < g.M ? (uint32_t)(r * g.ldsa) + q : OUTSIDE;
-  }
-  constexpr int DEPTH = TB + NB <= 3 ? 4 : 2, STEP = WAVES * PIECE;
-  struct Piece { i32x4 w[NB][4], a[TB][4]; int sw[NB][4], sa[TB][4]; } ring[DEPTH];
-  const auto load = [&](int k, Piece& p) {          // bytes k .. k + 255 of a row
+
+  // ---- loads ----
+  const int piece = (lane & 7) ^ (lane >> 4 & 3);   // of 16 bytes in a row of codes; in odd loads 4 more, as 8 rows turn it
+  uint32_t wof[2], sof, aof[OWN ? OWN : 1][2], saof[OWN ? OWN : 1];
+  i32x4 bufW, bufS, bufA, bufSA;
+  const int early_a = (int)((uintptr_t)g.sa & 3), period = ((uintptr_t)g.sw | (uintptr_t)g.ldsw | (uintptr_t)g.sa | (uintptr_t)g.ldsa) & 3 ? 7 : 8;
+  if constexpr (OWN > 0) {
+    bufA = buffer(g.a, (g.M - 1) * g.lda + g.B * 16);
+    bufSA = buffer(g.sa - early_a, (early_a + (g.M - 1) * g.ldsa + g.B + 3) & ~(int64_t)3);
     #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t outside = k + i * 64 + q * 16 < bytes ? 0u : OUTSIDE;
+    for (int b = 0; b < OWN; ++b) {
       #pragma unroll
-      for (int c = 0; c < NB; ++c) {
-        p.w[c][i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(bufW, ofW[c] | outside, k + i * 64, 0));
-        p.sw[c][i] = __builtin_amdgcn_raw_buffer_load_b8(bufSW, ofSW[c] | outside, (k >> 4) + i * 4, 0);
+      for (int l = 0; l < 2; ++l) {
+        const int r = b * 16 + l * 8 + (lane >> 3);
+        aof[b][l] = r < g.M ? (uint32_t)(r * g.lda) + ((piece ^ l * 4) << 4) : OUTSIDE;
       }
-      if constexpr (XT < 0) {
+      const int r = b * 16 + (lane >> 2);
+      saof[b] = r < g.M ? ((uint32_t)(early_a + r * g.ldsa) & ~3u) + (lane & 3) * 16 : OUTSIDE;
+    }
+  }
+  int lround = blockIdx.x, lk = first, lperiod = 0, lplace = PLACES - 1;
+  const auto enter = [&]() {
+    const int64_t n0 = ((int64_t)lround * groups + of_group) * 16;
+    const int rows = n0 >= g.N ? 0 : g.N - n0 < 16 ? (int)(g.N - n0) : 16;
+    bufW = buffer(g.w + n0 * g.ldw, rows ? (rows - 1) * g.ldw + g.B * 16 : 0);
+    const uint8_t* const s = g.sw + n0 * g.ldsw;
+    const int early = (int)((uintptr_t)s & 3);
+    bufS = buffer(s - early, rows ? (early + (rows - 1) * g.ldsw + g.B + 3) & ~(int64_t)3 : 0);
+    #pragma unroll
+    for (int l = 0; l < 2; ++l) wof[l] = l * 8 + (lane >> 3) < rows ? (uint32_t)((l * 8 + (lane >> 3)) * g.ldw) + ((piece ^ l * 4) << 4) : OUTSIDE;
+    sof = lane >> 2 < rows ? ((uint32_t)(early + (lane >> 2) * g.ldsw) & ~3u) + (lane & 3) * 16 : OUTSIDE;
+  };
+  // The next stage, into a place; behind the last one: nothing, from outside.  The scales of a period come in front of its first stage.
+  const auto fetch = [&](int slot) {
+    const uint32_t to = mine + slot * S::BYTES;
+    const bool over = lround >= rounds;
+    if (lperiod == 0) {
+      lplace = lplace == PLACES - 1 ? 0 : lplace + 1;
+      const uint32_t too = mine + DEPTH * S::BYTES + lplace * S::SCALES;
+      load(too, over ? OUTSIDE : sof, bufS, lk * 8);
+      #pragma unroll
+      for (int b = 0; b < OWN; ++b) load(too + 1024 * (1 + b), over ? OUTSIDE : saof[b], bufSA, lk * 8);
+      lperiod = period;
+    }
+    --lperiod;
+    if (over || (ragged && lk == stages - 1)) {
+      const int left = over ? 0 : g.B - lk * 8;     // blocks
+      #pragma unroll
+      for (int l = 0; l < 2; ++l) {
+        const bool in = (piece ^ l * 4) < left;
+        load(to + l * 1024, in ? wof[l] : OUTSIDE, bufW, lk * STAGE_BYTES);
         #pragma unroll
-        for (int b = 0; b < TB; ++b) {
-          p.a[b][i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(bufA, ofA[b] | outside, k + i * 64, 0));
-          p.sa[b][i] = __builtin_amdgcn_raw_buffer_load_b8(bufSA, ofSA[b] | outside, (k >> 4) + i * 4, 0);
-        }
+        for (int b = 0; b < OWN; ++b) load(to + 2048 * (1 + b) + l * 1024, in ? aof[b][l] : OUTSIDE, bufA, lk * STAGE_BYTES);
+      }
+    } else {
+      #pragma unroll
+      for (int l = 0; l < 2; ++l) {
+        load(to + l * 1024, wof[l], bufW, lk * STAGE_BYTES);
+        #pragma unroll
+        for (int b = 0; b < OWN; ++b) load(to + 2048 * (1 + b) + l * 1024, aof[b][l], bufA, lk * STAGE_BYTES);
       }
     }
+    if (++lk >= last && !over) {
+      lk = first;
+      lround += gridDim.x;
+      lperiod = 0;
+      if (lround < rounds) enter();
+    }
   };
-  int k = wave * PIECE;
-  #pragma unroll
-  for (int d = 0; d < DEPTH; ++d) {
-    load(k + d * STEP, ring[d]);
-    __builtin_amdgcn_sched_barrier(0);              // (in this order: a wait counts the loads behind it)
+  const bool works = first < last;                  // (K may have fewer stages than waves)
+  if (works) {
+    enter();
+    #pragma unroll
+    for (int d = 0; d < DEPTH - 1; ++d) fetch(d);
   }
+  uint8_t* const made = (uint8_t*)lds + S::MADE;    // XT >= 0: [M] rows of codes, 16 B + 16 apart, then of scales
+  const int bytes = g.B * 16;
   uint8_t* const made_scales = made + g.M * (bytes + 16);
   if constexpr (XT >= 0) {                          // four lanes make a block
     const int pieces = g.B * 4;
     for (int r = 0; r < g.M; ++r) {
       const char* const x = t.x + r * t.ldx * (XT == ROW_F32 ? 4 : 2);
-      for (int p = tid; p < pieces; p += WAVES * 64) {
+      for (int p = tid; p < pieces; p += 256) {
         float v[8];
         mx_load8<XT>(x, p * 8, t.K, v);
         const uint32_t s = mx_scale(mx_quad_max(mx_max_bits(v)));
@@ -433,51 +500,83 @@ __global__ __launch_bounds__(WAVES * 64) void stream_kernel(MxArgs g, TokenArgs 
         if ((p & 3) == 0) made_scales[r * g.B + (p >> 2)] = (uint8_t)s;
       }
     }
-    __syncthreads();
   }
-  const int mine = (lane & 15) < g.M ? lane & 15 : 0;       // (a token past the last one is not stored)
-  f32x4 acc[NB][TB] = {};
-  while (k < bytes) {
-    #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-      Piece& p = ring[d];
+  __syncthreads();
+
+  // ---- products ----
+  uint32_t at[2], sat[OWN ? OWN : 1], mat = 0, msat = 0;
+  #pragma unroll
+  for (int i = 0; i < 2; ++i) at[i] = mine + c * 128 + (((i * 4 + q) ^ (c >> 1 & 7)) << 4);
+  #pragma unroll
+  for (int b = 0; b < OWN; ++b)
+    sat[b] = mine + DEPTH * S::BYTES + 1024 * (1 + b) + c * 64 + q + (((uint32_t)early_a + (uint32_t)(b * 16 + c) * (uint32_t)g.ldsa) & 3);
+  if constexpr (XT >= 0) {
+    const int row = c < g.M ? c : 0;                // (a token past the last one is not stored)
+    mat = lds0 + S::MADE + row * (bytes + 16);
+    msat = lds0 + S::MADE + (uint32_t)g.M * (bytes + 16) + row * g.B;
+  }
+  int slot = 0, cperiod = 0, cplace = 0, turn = 0;
+  for (int round = blockIdx.x, nth = 0; round < rounds; round += gridDim.x, ++nth) {
+    const int64_t n0 = ((int64_t)round * groups + of_group) * 16;
+    const uint32_t sw = mine + DEPTH * S::BYTES + c * 64 + q + (((uint32_t)(uintptr_t)g.sw + (uint32_t)(n0 + c) * (uint32_t)g.ldsw) & 3);
+    f32x4 acc[TB] = {};
+    for (int k = first; k < last; ++k) {
+      // the stage has landed, and what this wave reads of the last one
+      __builtin_amdgcn_s_waitcnt(0x0070 | ((DEPTH - 2) * S::LOADS & 15) | (DEPTH - 2) * S::LOADS >> 4 << 14);
+      asm volatile("" ::: "memory");
+      fetch(slot == 0 ? DEPTH - 1 : slot - 1);
+      const uint32_t here = slot * S::BYTES, scales_here = cplace * S::SCALES + cperiod * 8;
+      const int left = g.B - k * 8;
+      i32x4 w[2], a[TB][2];
+      uint32_t s[2], sa[TB][2];
       #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (XT >= 0) {                    // (behind the last block the weight's codes are 0)
-          const int block = ((k + i * 64) >> 4) + q < g.B ? ((k + i * 64) >> 4) + q : 0;
-          p.a[0][i] = *(const i32x4*)(made + mine * (bytes + 16) + block * 16);
-          p.sa[0][i] = made_scales[mine * g.B + block];
-          // a scale that is NaN must not meet the zeros behind the last block
-          if (((k + i * 64) >> 4) + q >= g.B) p.sa[0][i] = 0;
-        }
-        #pragma unroll
-        for (int c = 0; c < NB; ++c)
+      for (int i = 0; i < 2; ++i) {
+        w[i] = from_lds<i32x4>(at[i] + here);
+        s[i] = from_lds<uint8_t>(sw + scales_here + i * 4);
+        if constexpr (XT >= 0) {                    // (behind the last block the weight's codes are 0, and the scales here made to be)
+          const int block = k * 8 + i * 4 + q < g.B ? k * 8 + i * 4 + q : g.B - 1;
+          a[0][i] = from_lds<i32x4>(mat + block * 16);
+          sa[0][i] = from_lds<uint8_t>(msat + block);
+        } else {
           #pragma unroll
-          for (int b = 0; b < TB; ++b)
-            acc[c][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(p.w[c][i]), wide(p.a[b][i]), acc[c][b], 4, 4, 0, p.sw[c][i], 0, p.sa[b][i]);
+          for (int b = 0; b < TB; ++b) {
+            a[b][i] = from_lds<i32x4>(at[i] + here + 2048 * (1 + b));
+            sa[b][i] = from_lds<uint8_t>(sat[b] + scales_here + i * 4);
+          }
+        }
       }
-      load(k + DEPTH * STEP, p);
-      k += STEP;
       __builtin_amdgcn_sched_barrier(0);
+      #pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t there = i * 4 + q < left ? 255u : 0u;                 // (behind the last block: not a NaN)
+        #pragma unroll
+        for (int b = 0; b < TB; ++b)
+          acc[b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(w[i]), wide(a[b][i]), acc[b], 4, 4, 0, (int)(s[i] & there), 0, (int)(sa[b][i] & there));
+      }
+      slot = slot == DEPTH - 1 ? 0 : slot + 1;
+      cperiod = cperiod == period - 1 ? 0 : cperiod + 1;
+      if (cperiod == 0) cplace = cplace == PLACES - 1 ? 0 : cplace + 1;
+    }
+    if (cperiod) cplace = cplace == PLACES - 1 ? 0 : cplace + 1;             // (a block starts a period)
+    cperiod = 0;
+    // accumulator register r of lane l: channel 4 (l / 16) + r of token l % 16
+    f32x4* const red = (f32x4*)(lds + S::RED) + turn * 4 * TB * 64;
+    turn ^= 1;                                      // (what is read here is written again behind the next barrier but one)
+    #pragma unroll
+    for (int b = 0; b < TB; ++b) red[(wave * TB + b) * 64 + lane] = acc[b];
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    for (int o = tid; o < groups * TB * 256; o += 256) {
+      const int ch = o & 15, tok = o >> 4 & 15, b = (o >> 8) % TB, group = (o >> 8) / TB, token = b * 16 + tok;
+      const int64_t n = ((int64_t)round * groups + group) * 16 + ch;
+      if (token >= g.M || n >= g.N) continue;
+      float y = 0;
+      for (int p = 0; p < KS; ++p) y += ((const float*)&red[((group * KS + p) * TB + b) * 64 + (ch >> 2) * 16 + tok])[ch & 3];
+      if (g.bias) y += nth * groups + group < MOST_BIASES ? biases[(nth * groups + group) * 16 + ch] : load_any(g.bias, g.bias_dtype, n);
+      if constexpr (BF == ROW_F32) ((float*)g.y)[token * g.N + n] = y;
+      else store_scalar<BF>(g.y, token * g.N + n, rnd<BF>(y));
     }
   }
-  #pragma unroll
-  for (int c = 0; c < NB; ++c)
-    #pragma unroll
-    for (int b = 0; b < TB; ++b) *(f32x4*)red[wave][c][b][lane] = acc[c][b];
-  __syncthreads();
-  // accumulator register r of lane l: channel 4 (l / 16) + r of token l % 16
-  for (int o = tid; o < TB * NB * 256; o += WAVES * 64) {
-    const int c = o % (16 * NB), cb = c >> 4, cc = c & 15, token = o / (16 * NB), b = token >> 4, tok = token & 15;
-    const int64_t nn = n0 + c;
-    if (token >= g.M || nn >= g.N) continue;
-    float y = 0;
-    #pragma unroll
-    for (int v = 0; v < WAVES; ++v) y += red[v][cb][b][(cc >> 2) * 16 + tok][cc & 3];
-    if (g.bias) y += load_any(g.bias, g.bias_dtype, nn);
-    if constexpr (BF == ROW_F32) ((float*)g.y)[token * g.N + nn] = y;
-    else store_scalar<BF>(g.y, token * g.N + nn, rnd<BF>(y));
-  }
+  __builtin_amdgcn_s_waitcnt(0x0f70);               // nothing may still be on its way to LDS when the workgroup leaves it
 }
 
 int64_t on256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -499,21 +598,30 @@ void launch_join(const MxArgs& g, const float* sums, int parts, hipStream_t st) 
   else join_kernel<BF, 1><<<dim3((unsigned)((all + 255) / 256)), dim3(256), 0, st>>>(g, sums, parts);
 }
 
-template <int TB, int NB, int BF, int XT, int WAVES>
-void launch_stream(const MxArgs& g, const TokenArgs& t, hipStream_t st) {
-  const unsigned lds = XT < 0 ? 0 : (unsigned)(g.M * (g.B * 16 + 16) + g.M * g.B);
-  stream_kernel<TB, NB, BF, XT, WAVES><<<dim3((unsigned)((g.N + 16 * NB - 1) / (16 * NB))), dim3(WAVES * 64), lds, st>>>(g, t);
+template <int TB, int BF, int XT, int DEPTH, int PLACES>
+int launch_few(const MxArgs& g, const TokenArgs& t, int KS, hipStream_t st) {
+  typedef Few<TB, XT, DEPTH, PLACES> S;
+  const auto kernel = few_kernel<TB, BF, XT, DEPTH, PLACES>;
+  const int lds = S::MADE + (XT < 0 ? 0 : (int)(g.M * (g.B * 16 + 16) + g.M * g.B));
+  if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return LCQ_ELAUNCH;
+  const int64_t rounds = ((g.N + 15) / 16 + 4 / KS - 1) / (4 / KS), most = 256 * (163840 / lds);
+  kernel<<<dim3((unsigned)(rounds < most ? rounds : most)), dim3(256), lds, st>>>(g, t, KS);
+  return LCQ_OK;
+}
+// Waves share K as long as each has four stages of it.  With that, scales of seven stages on their way are those of three periods at most; with
+// fewer, those of five stages of five.
+template <int TB, int BF, int XT>
+int launch_few(const MxArgs& g, const TokenArgs& t, hipStream_t st) {
+  const int stages = (g.B + 7) / 8, KS = stages >= 16 ? 4 : stages >= 8 ? 2 : 1;
+  if constexpr (TB == 2) return stages >= 4 ? launch_few<2, BF, XT, 4, 3>(g, t, KS, st) : launch_few<2, BF, XT, 3, 3>(g, t, KS, st);
+  else return stages >= 4 ? launch_few<1, BF, XT, 7, 3>(g, t, KS, st) : launch_few<1, BF, XT, 5, 5>(g, t, KS, st);
 }
 
 template <int BF>
-void launch(const MxArgs& g, float* sums, hipStream_t st) {
+int launch(const MxArgs& g, float* sums, hipStream_t st) {
   const Mxfp4Cut c = mxfp4_cut(g.M, g.N, g.B);
-  if (c.stream) {
-    if (g.M <= 16) launch_stream<1, 1, BF, -1, 2>(g, TokenArgs{}, st);
-    else if (g.M <= 32) launch_stream<2, 1, BF, -1, 2>(g, TokenArgs{}, st);
-    else launch_stream<4, 1, BF, -1, 2>(g, TokenArgs{}, st);
-  }
-  else if (c.parts > 1) {
+  if (c.stream) return g.M <= 16 ? launch_few<1, BF, -1>(g, TokenArgs{}, st) : launch_few<2, BF, -1>(g, TokenArgs{}, st);
+  if (c.parts > 1) {
     MxArgs p = g;
     p.y = sums;
     launch_tiles<Tile128, ROW_SUM>(p, c.parts, st);
@@ -521,6 +629,7 @@ void launch(const MxArgs& g, float* sums, hipStream_t st) {
   }
   else if (c.tile == 0) launch_tiles<Tile256, BF>(g, 1, st);
   else launch_tiles<Tile128, BF>(g, 1, st);
+  return LCQ_OK;
 }
 
 bool known(int dtype) { return dtype == LCQ_F32 || dtype == LCQ_BF16 || dtype == LCQ_F16; }
@@ -579,9 +688,9 @@ int lcq_mxfp4_matmul(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t l
       g.sa = to; g.sw = to + M * Bp; g.ldsa = g.ldsw = Bp;
     }
   }
-  if (dtype == LCQ_BF16) launch<ROW_BF16>(g, (float*)workspace, st);
-  else if (dtype == LCQ_F16) launch<ROW_F16>(g, (float*)workspace, st);
-  else launch<ROW_F32>(g, (float*)workspace, st);
+  float* const sums = (float*)workspace;
+  const int rc = dtype == LCQ_BF16 ? launch<ROW_BF16>(g, sums, st) : dtype == LCQ_F16 ? launch<ROW_F16>(g, sums, st) : launch<ROW_F32>(g, sums, st);
+  if (rc) return rc;
   LCQ_CHECK_LAUNCH();
   return LCQ_OK;
 }
@@ -605,13 +714,10 @@ int lcq_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w, 
     hipStream_t st = (hipStream_t)stream;
     const auto run = [&](auto xt) {
       constexpr int XT = decltype(xt)::value;
-      if (dtype == LCQ_BF16) launch_stream<1, 1, ROW_BF16, XT, 4>(g, t, st);
-      else if (dtype == LCQ_F16) launch_stream<1, 1, ROW_F16, XT, 4>(g, t, st);
-      else launch_stream<1, 1, ROW_F32, XT, 4>(g, t, st);
+      return dtype == LCQ_BF16 ? launch_few<1, ROW_BF16, XT>(g, t, st) : dtype == LCQ_F16 ? launch_few<1, ROW_F16, XT>(g, t, st) : launch_few<1, ROW_F32, XT>(g, t, st);
     };
-    if (x_dtype == LCQ_BF16) run(Int<ROW_BF16>{});
-    else if (x_dtype == LCQ_F16) run(Int<ROW_F16>{});
-    else run(Int<ROW_F32>{});
+    const int rc = x_dtype == LCQ_BF16 ? run(Int<ROW_BF16>{}) : x_dtype == LCQ_F16 ? run(Int<ROW_F16>{}) : run(Int<ROW_F32>{});
+    if (rc) return rc;
     LCQ_CHECK_LAUNCH();
     return LCQ_OK;
   }
