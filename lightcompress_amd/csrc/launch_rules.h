@@ -87,16 +87,49 @@ inline bool int8_streams(long long M, long long N, long long K) {
   return stream < tiles;
 }
 
-// Product of microscaled 4-bit numbers (mxfp4_matmul.hip): the weight streamed past the tokens, or tiles of 256 x 256 or 128 x 128, the
-// latter with K (B blocks of 32) cut into parts of at least two periods of 16 blocks.
+// Product of microscaled 4-bit numbers (mxfp4_matmul.hip), B blocks of 32 in a row.  Times in us on one MI355X, other weights every time.
+constexpr int MXFP4_CUS = 256;
+inline double mxfp4_rounds(double workgroups) { return (double)(long long)((workgroups + MXFP4_CUS - 1) / MXFP4_CUS); }
+// The weight streamed past groups of 16 or 32 tokens: a unit of work is 4 / KS blocks of 16 channels with such a group, KS waves share the K of a block, and a
+// workgroup per CU takes its share of the units one behind the other.  A unit costs its waves' stages of 8 blocks of K, and 1.2 or 2.5 more where its sums are
+// joined; KS is what makes that least for a workgroup.  N x K with KS 1 / 2 / 4 for 16 and for 32 tokens:
+//   1024 x 1024  5.1 / 4.4 / 4.0   5.9 / 4.9 / 4.3    4096 x 4096   8.6 /  6.4 /  5.7    9.8 /  7.1 /  5.9    7168 x 2048  6.6 / 5.6 / 6.2   7.5 / 6.0 / 7.0
+//   6144 x 4096  8.7 / 6.7 / 7.5   9.7 / 7.2 / 8.3   14336 x 4096   9.6 / 10.4 / 11.7   10.7 / 11.7 / 13.8    2048 x 7168   12 / 7.9 / 6.2    13 / 8.7 / 6.7
+inline long long mxfp4_units(long long M, long long N, int KS) {
+  const long long group = M <= 16 ? 16 : 32, blocks = (N + 15) / 16, at_once = 4 / KS;
+  return (blocks + at_once - 1) / at_once * ((M + group - 1) / group);
+}
+inline double mxfp4_stages(long long M, long long N, long long B, int KS) {            // of a workgroup
+  return mxfp4_rounds((double)mxfp4_units(M, N, KS)) * ((double)(((B + 7) / 8 + KS - 1) / KS) + (M <= 16 ? 1.2 : 2.5));
+}
+inline int mxfp4_waves(long long M, long long N, long long B) {
+  int best = 4;
+  for (int KS = 2; KS >= 1; KS /= 2)
+    if (mxfp4_stages(M, N, B, KS) < mxfp4_stages(M, N, B, best)) best = KS;
+  return best;
+}
+// Or tiles of 256 x 256 or 128 x 128, the latter with K cut into parts of at least two periods of 16 blocks.  What is estimated to be fastest, measured as
+// streamed / 128 / 128 in 2 parts / in 4 / in 8 (and 256):
+//   4096 x 4096   64 tokens  7.7 / 12.4 / 12.3 / 12.6 / 15.2    128  10.6 / 12.5 / 13.0 / 14.9 / 16.2    211  17.6 / 12.9 / 14.4 / 17.8 / 22.6    2048  28.4 (32.3)
+//   4096 x 14336  64 tokens   16 /   35 /   26 /   20 /   18    128    23 /   37 /   29 /   22 /   20    211    45 /   41 /   29 /   22 /   31    1024  44.9 (88)
+//   14336 x 4096  33 tokens   18 / 14.7 / 14.7 /   20 /   30    211    56 /   17 /   31 /   45 /   67   1024    62 with 128 (40)
+//   1001 x 2047  128 tokens  5.4 /  9.4 / 10.0 / 10.8 / 13.2    512   7.9 /  9.5 / 11.1 / 12.9 / 19
 struct Mxfp4Cut { bool stream; int tile, parts; };  // tile 0: 256 x 256, 1: 128 x 128
 inline Mxfp4Cut mxfp4_cut(long long M, long long N, long long B) {
   if (M <= 32) return {true, 0, 1};
-  const long long large = (M + 255) / 256 * ((N + 255) / 256), small = (M + 127) / 128 * ((N + 127) / 128), groups = (B + 15) / 16;
-  if (large >= 200) return {false, 0, 1};
-  int parts = 1;
-  while (parts < 8 && small * parts * 2 <= 256 && groups / (parts * 2) >= 2) parts *= 2;
-  return {false, 1, parts};
+  const double stages = (double)((B + 7) / 8), outputs = (double)M * (double)N;
+  const double large = (double)((M + 255) / 256) * (double)((N + 255) / 256), small = (double)((M + 127) / 128) * (double)((N + 127) / 128);
+  const double scales = B % 16 ? 2.5 : 0;           // put in order in front of the tiles (of 256 x 256 always)
+  double least = 9.5 + mxfp4_rounds(large) * (3 + 1.9 * stages);
+  Mxfp4Cut best = {false, 0, 1};
+  for (int parts = 1; parts <= 8 && (parts == 1 || (B + 15) / 16 >= 2 * parts); parts *= 2) {
+    const double workgroups = small * parts, busy = workgroups < MXFP4_CUS ? workgroups : MXFP4_CUS, stage = busy * 0.0032 > 0.55 ? busy * 0.0032 : 0.55;
+    const double us = 4.4 + scales + mxfp4_rounds(workgroups) * (1 + stage * stages / parts) + (parts > 1 ? 3 + parts * outputs / 5e5 : 0);
+    if (us < least) least = us, best = {false, 1, parts};
+  }
+  const long long teams = (M + 31) / 32;
+  if (teams <= 64 && 3.4 + 0.39 * mxfp4_stages(M, N, B, mxfp4_waves(M, N, B)) < least) best = {true, 0, 1};
+  return best;
 }
 
 }  // namespace lcq

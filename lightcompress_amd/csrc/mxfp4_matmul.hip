@@ -23,6 +23,7 @@ struct MxArgs {
   const void* bias;
   void* y;
   int64_t M, N, lda, ldw, ldsa, ldsw;               // distances in bytes
+  int64_t nextsa, nextsw;                           // tiles: from 16 scales of a row to the next 16
   int B, bias_dtype;                                // blocks of a row
 };
 
@@ -77,19 +78,19 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MxArgs g, int tiles_m, int
   int ti, tj, part;
   {
     const int total = tiles_m * tiles_n * parts, each = (total + 7) >> 3;
-    int v = ((int)blockIdx.x & 7) * each + ((int)blockIdx.x >> 3);
-    if (((int)blockIdx.x >> 3) >= each || v >= total) return;
-    part = v / (tiles_m * tiles_n);
+    uint32_t v = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= each || v >= (uint32_t)total) return;
+    part = parts == 1 ? 0 : v / (uint32_t)(tiles_m * tiles_n);
     v -= part * tiles_m * tiles_n;
-    const int group = v / (4 * tiles_n), first = group * 4, rows = tiles_m - first < 4 ? tiles_m - first : 4;
-    const int in = v - group * 4 * tiles_n;
-    tj = in / rows;
+    const int group = v / (4u * tiles_n), first = group * 4, rows = tiles_m - first < 4 ? tiles_m - first : 4;
+    const uint32_t in = v - group * 4 * tiles_n;
+    tj = rows == 4 ? in / 4 : rows == 2 ? in / 2 : rows == 1 ? in : in / 3;
     ti = first + in - tj * rows;
   }
   const int64_t m0 = (int64_t)ti * T::TM, n0 = (int64_t)tj * T::TN;
   const int rows_a = (int)(g.M - m0 < T::TM ? g.M - m0 : T::TM), rows_w = (int)(g.N - n0 < T::TN ? g.N - n0 : T::TN);
   const int bytes = g.B * 16, groups = (g.B + 15) >> 4;                      // of a row's codes; 16-byte pieces of its scales
-  const int begin = (int)((int64_t)groups * part / parts), periods = (int)((int64_t)groups * (part + 1) / parts) - begin;
+  const int begin = parts == 1 ? 0 : (uint32_t)(groups * part) / (uint32_t)parts, periods = (parts == 1 ? groups : (uint32_t)(groups * (part + 1)) / (uint32_t)parts) - begin;
 
   const auto buffer = [&](const uint8_t* p, int64_t ld, int rows, int row) {
     const uint64_t at = (uint64_t)(uintptr_t)p;
@@ -97,7 +98,7 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MxArgs g, int tiles_m, int
     return i32x4{one((int)(uint32_t)at), one((int)(uint32_t)(at >> 32) & 0xffff), one((int)((rows - 1) * ld + row)), 0x00020000};
   };
   const i32x4 bufA = buffer(g.a + m0 * g.lda, g.lda, rows_a, bytes), bufW = buffer(g.w + n0 * g.ldw, g.ldw, rows_w, bytes);
-  const i32x4 bufSA = buffer(g.sa + m0 * g.ldsa, g.ldsa, rows_a, groups * 16), bufSW = buffer(g.sw + n0 * g.ldsw, g.ldsw, rows_w, groups * 16);
+  const uint8_t *sa = g.sa + m0 * g.ldsa + begin * g.nextsa, *sw = g.sw + n0 * g.ldsw + begin * g.nextsw;       // of the period that is loaded next
   constexpr uint32_t OUTSIDE = 0x80000000u;
   constexpr int ROWS = 1024 / SLAB, LANES = 64 / ROWS;                       // of a load
   constexpr int LA = T::TM / (4 * ROWS), LW = T::TN / (4 * ROWS);            // a wave's loads of tokens and of weights per stage
@@ -110,13 +111,13 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MxArgs g, int tiles_m, int
   #pragma unroll
   for (int p = 0; p < LA + LW; ++p) {
     const int r = (wave * (p < LA ? LA : LW) + (p < LA ? p : p - LA)) * ROWS + lane / LANES;
-    gof[p] = r < (p < LA ? rows_a : rows_w) ? (uint32_t)(r * (p < LA ? g.lda : g.ldw) + piece16[p & 1]) : OUTSIDE;
+    gof[p] = r < (p < LA ? rows_a : rows_w) ? (uint32_t)r * (uint32_t)(p < LA ? g.lda : g.ldw) + piece16[p & 1] : OUTSIDE;
   }
   // scale load i of this wave: rows 64 (wave + 4 i) .. + 63 of tokens, then weights (beyond both: a place that nothing reads)
   #pragma unroll
   for (int i = 0; i < SL; ++i) {
     const int r = (wave + 4 * i) * 64 + lane;
-    sof[i] = r < T::TM ? (r < rows_a ? (uint32_t)(r * g.ldsa) : OUTSIDE) : r - T::TM < rows_w ? (uint32_t)((r - T::TM) * g.ldsw) : OUTSIDE;
+    sof[i] = r < T::TM ? (r < rows_a ? (uint32_t)r * (uint32_t)g.ldsa : OUTSIDE) : r - T::TM < rows_w ? (uint32_t)(r - T::TM) * (uint32_t)g.ldsw : OUTSIDE;
   }
   const uint32_t lds0 = (uint32_t)(size_t)(lds_ptr)lds;
   struct Outside { uint32_t of[2]; };
@@ -130,12 +131,15 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MxArgs g, int tiles_m, int
   // the scales of period p (counted from this part's first), place p % 2
   const auto sload = [&](int p) {
     const uint32_t outside = begin + p < groups ? 0u : OUTSIDE;
+    const i32x4 bufSA = buffer(sa, g.ldsa, rows_a, 16), bufSW = buffer(sw, g.ldsw, rows_w, 16);
+    sa += g.nextsa;
+    sw += g.nextsw;
     #pragma unroll
     for (int i = 0; i < SL; ++i) {
       const uint32_t to = lds0 + STAGES * T::STAGE + ((p & 1) * 4 * SL + wave + 4 * i) * 1024;
       const i32x4 buf = (wave + 4 * i) * 64 < T::TM ? bufSA : bufSW;
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                   ::"s"(to), "v"(sof[i] | outside), "s"(buf), "s"((begin + p) * 16) : "memory");
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                   ::"s"(to), "v"(sof[i] | outside), "s"(buf) : "memory");
     }
   };
 
@@ -149,12 +153,6 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MxArgs g, int tiles_m, int
   #pragma unroll
   for (int ks = 0; ks < STEPS; ++ks) step_at[ks] = ((slot ^ (2 * ks)) - slot) * 16;
   f32x16 acc[FN][FM];
-  #pragma unroll
-  for (int j = 0; j < FN; ++j)
-    #pragma unroll
-    for (int i = 0; i < FM; ++i)
-      #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[j][i][r] = 0;
   i32x4 fr[2][FN + FM];                             // operands of a step: weights, tokens
   i32x4 sc[FN + FM], next[FN + FM];                 // their scales of a period: byte 2 s + lane / 32 is step s's
   const auto rd = [&](int set, int ks, int f, uint32_t stage) {
@@ -196,6 +194,15 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MxArgs g, int tiles_m, int
     if (l == (STAGES - PER) * LOADS) sload(1);
     gload(lds0 + l / LOADS * T::STAGE, k, outside_at(k), l % LOADS);
   }
+  float zero = 0;
+  asm volatile("" : "+v"(zero));                    // (not before the loads are on their way)
+  #pragma unroll
+  for (int j = 0; j < FN; ++j)
+    #pragma unroll
+    for (int i = 0; i < FM; ++i)
+      #pragma unroll
+      for (int r = 0; r < 16; ++r) acc[j][i][r] = zero;
+  __builtin_amdgcn_sched_barrier(0);
   wait(Int<AHEAD - LOADS + (STAGES > PER ? SL : 0)>{});
   #pragma unroll
   for (int f = 0; f < READS; ++f) rds(f, 0);
@@ -289,22 +296,41 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MxArgs g, int tiles_m, int
       }
     }
     asm volatile("" ::: "memory");                  // (LDS serves a wave in order)
-    #pragma unroll
-    for (int o = 0; o < STEP * 32 * CHUNKS / 64; ++o) {
-      const int idx = o * 64 + lane, tt = idx / CHUNKS, ch = idx % CHUNKS;
-      const u32x4 v = *(const u32x4*)(mine + tt * ROW + turned(ch, tt % 32) * 16);
-      const int m = wr * FM * 32 + i0 * 32 + tt, n = wc * FN * 32 + ch * CH;
-      if (m >= rows_a || n >= rows_w) continue;
-      const int64_t cell = (m0 + m) * g.N + n0 + n + (BF == ROW_SUM ? part * g.M * g.N : 0);
-      if (n + CH <= rows_w) {
-        __builtin_memcpy((char*)g.y + cell * E, &v, 16);     // (rows may start anywhere)
-      } else {
+    constexpr int AT_ONCE = 64 / CHUNKS, TIMES = STEP * 32 / AT_ONCE;        // tokens of a store, stores
+    const int t0 = lane / CHUNKS, ch = lane % CHUNKS, n = wc * FN * 32 + ch * CH;
+    char* const to = (char*)g.y + ((m0 + wr * FM * 32 + i0 * 32) * g.N + n0 + (BF == ROW_SUM ? part * g.M * g.N : 0)) * E;
+    if (rows_a == T::TM && rows_w == T::TN) {       // (uniform, as most tiles of a large product are: no comparison, no address but a scalar one)
+      const uint32_t of = (uint32_t)(t0 * g.N + n) * E;                      // (7 N outputs of two bytes or 3 N of four, and a tile's: 32 bits)
+      #pragma unroll
+      for (int o0 = 0; o0 < TIMES; o0 += 8) {
+        u32x4 v[8];
         #pragma unroll
-        for (int e = 0; e < CH; ++e)
-          if (n + e < rows_w) {
-            if constexpr (E == 4) ((uint32_t*)g.y)[cell + e] = v[e];
-            else ((uint16_t*)g.y)[cell + e] = (uint16_t)(v[e / 2] >> 16 * (e % 2));
+        for (int o = 0; o < 8; ++o) v[o] = *(const u32x4*)(mine + ((o0 + o) * AT_ONCE + t0) * ROW + turned(ch, ((o0 + o) * AT_ONCE + t0) % 32) * 16);
+        #pragma unroll
+        for (int o = 0; o < 8; ++o) __builtin_memcpy(to + (int64_t)(o0 + o) * AT_ONCE * g.N * E + of, &v[o], 16);          // (rows may start anywhere)
+      }
+    } else {
+      #pragma unroll 1
+      for (int o0 = 0; o0 < TIMES; o0 += 8) {
+        u32x4 v[8];
+        #pragma unroll
+        for (int o = 0; o < 8; ++o) v[o] = *(const u32x4*)(mine + ((o0 + o) * AT_ONCE + t0) * ROW + turned(ch, ((o0 + o) * AT_ONCE + t0) % 32) * 16);
+        #pragma unroll
+        for (int o = 0; o < 8; ++o) {
+          const int tt = (o0 + o) * AT_ONCE + t0, m = wr * FM * 32 + i0 * 32 + tt;
+          if (m >= rows_a || n >= rows_w) continue;
+          char* const cell = to + ((int64_t)tt * g.N + n) * E;
+          if (n + CH <= rows_w) {
+            __builtin_memcpy(cell, &v[o], 16);
+          } else {
+            #pragma unroll
+            for (int e = 0; e < CH; ++e)
+              if (n + e < rows_w) {
+                if constexpr (E == 4) ((uint32_t*)cell)[e] = v[o][e];
+                else ((uint16_t*)cell)[e] = (uint16_t)(v[o][e / 2] >> 16 * (e % 2));
+              }
           }
+        }
       }
     }
     asm volatile("" ::: "memory");
@@ -341,19 +367,23 @@ __global__ __launch_bounds__(256) void join_kernel(MxArgs g, const float* __rest
   }
 }
 
-// Scales of rows that do not hold whole 16-byte pieces, or do not start on them, to rows that do, with zeros behind them: those of a, then
-// those of w.  (A tile's loads of scales take 16 of a row.)
-__global__ __launch_bounds__(256) void pad_scales_kernel(MxArgs g, int Bp, uint8_t* __restrict__ out, int64_t words) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= words) return;
-  const int per = Bp / 4;
-  const int64_t r = i / per;
-  const int b = (int)(i - r * per) * 4;
-  const uint8_t* const from = r < g.M ? g.sa + r * g.ldsa : g.sw + (r - g.M) * g.ldsw;
-  uint32_t v = 0;
-  #pragma unroll
-  for (int e = 0; e < 4; ++e) v |= (b + e < g.B ? (uint32_t)from[b + e] : 0u) << 8 * e;
-  ((uint32_t*)out)[i] = v;
+// Scales for tiles: [16 scales of a row][row][16], with zeros behind a row's last, those of a and then those of w.  A tile's loads of them are then whole
+// lines; in the rows' own order each of 64 lanes reads 16 bytes of a line of its own, again in every tile of its stripe (8192 x 14336 x 4096: 276 us
+// against 240 without any).
+__global__ __launch_bounds__(256) void order_scales_kernel(MxArgs g, int groups, uint8_t* __restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, of_a = g.M * groups;
+  if (i >= of_a + g.N * groups) return;
+  const bool a = i < of_a;
+  const int64_t rows = a ? g.M : g.N, j = a ? i : i - of_a, group = j / rows, r = j - group * rows, ld = a ? g.ldsa : g.ldsw;
+  const uint8_t* const from = (a ? g.sa : g.sw) + r * ld + group * 16;
+  u32x4 v = {};
+  if ((uintptr_t)from % 16 == 0 && group * 16 + 16 <= g.B) {
+    v = *(const u32x4*)from;
+  } else {
+    #pragma unroll
+    for (int e = 0; e < 16; ++e) v[e / 4] |= (group * 16 + e < g.B ? (uint32_t)from[e] : 0u) << 8 * (e % 4);
+  }
+  *(u32x4*)(out + i * 16) = v;
 }
 
 // ---- few tokens ---------------------------------------------------------------------------------------------------
@@ -380,7 +410,8 @@ struct Few {
   static constexpr int RED = 4 * WAVE, BIAS = RED + 2 * 4 * TB * 1024, MADE = BIAS + MOST_BIASES * 64;
 };
 
-// TB blocks of 16 tokens.  XT: the type of the tokens' values, or -1 for codes.
+// A unit of work: 4 / KS blocks of channels and a group of 16 TB tokens, the groups of the same channels one behind the other.  Workgroup b runs on
+// XCD b % 8: every XCD takes neighbouring units, and the weights that they share from its L2.  XT: the type of the tokens' values, or -1 for codes.
 template <int TB, int BF, int XT, int DEPTH, int PLACES>
 __global__ __launch_bounds__(256) void few_kernel(MxArgs g, TokenArgs t, int KS) {
   typedef Few<TB, XT, DEPTH, PLACES> S;
@@ -389,7 +420,17 @@ __global__ __launch_bounds__(256) void few_kernel(MxArgs g, TokenArgs t, int KS)
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = wave % KS, of_group = wave / KS, groups = 4 / KS;        // blocks at a time
   const int stages = (g.B + 7) >> 3, first = stages * part / KS, last = stages * (part + 1) / KS;
-  const int blocks = (int)((g.N + 15) >> 4), rounds = (blocks + groups - 1) / groups;        // a workgroup takes every gridDim.x-th round
+  const int blocks = (int)((g.N + 15) >> 4), rounds = (blocks + groups - 1) / groups;
+  const int first_unit = gridDim.x % 8 == 0 ? (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3) : blockIdx.x;          // and every gridDim.x-th from there
+  const int teams = XT < 0 ? (int)((g.M + 16 * TB - 1) / (16 * TB)) : 1;     // of tokens
+  struct Unit { int round, team; };
+  const auto next = [&](Unit u) {
+    u.team += gridDim.x % teams;
+    u.round += gridDim.x / teams + (u.team >= teams);
+    u.team -= u.team >= teams ? teams : 0;
+    return u;
+  };
+  const Unit start = {first_unit / teams, first_unit % teams};
   const bool ragged = g.B % 8 != 0;
   const auto one = [](uint32_t v) { return (int)__builtin_amdgcn_readfirstlane((int)v); };
   const auto buffer = [&](const void* p, int64_t size) {
@@ -406,7 +447,7 @@ __global__ __launch_bounds__(256) void few_kernel(MxArgs g, TokenArgs t, int KS)
   float* const biases = (float*)(lds + S::BIAS);
   if (g.bias) {
     for (int i = tid; i < MOST_BIASES * 16; i += 256) {
-      const int64_t n = ((int64_t)(blockIdx.x + (i >> 4) / groups * gridDim.x) * groups + (i >> 4) % groups) * 16 + (i & 15);
+      const int64_t n = ((first_unit + (int64_t)((i >> 4) / groups) * gridDim.x) / teams * groups + (i >> 4) % groups) * 16 + (i & 15);
       if (n < g.N) biases[i] = load_any(g.bias, g.bias_dtype, n);
     }
   }
@@ -415,24 +456,11 @@ __global__ __launch_bounds__(256) void few_kernel(MxArgs g, TokenArgs t, int KS)
   const int piece = (lane & 7) ^ (lane >> 4 & 3);   // of 16 bytes in a row of codes; in odd loads 4 more, as 8 rows turn it
   uint32_t wof[2], sof, aof[OWN ? OWN : 1][2], saof[OWN ? OWN : 1];
   i32x4 bufW, bufS, bufA, bufSA;
-  const int early_a = (int)((uintptr_t)g.sa & 3), period = ((uintptr_t)g.sw | (uintptr_t)g.ldsw | (uintptr_t)g.sa | (uintptr_t)g.ldsa) & 3 ? 7 : 8;
-  if constexpr (OWN > 0) {
-    bufA = buffer(g.a, (g.M - 1) * g.lda + g.B * 16);
-    bufSA = buffer(g.sa - early_a, (early_a + (g.M - 1) * g.ldsa + g.B + 3) & ~(int64_t)3);
-    #pragma unroll
-    for (int b = 0; b < OWN; ++b) {
-      #pragma unroll
-      for (int l = 0; l < 2; ++l) {
-        const int r = b * 16 + l * 8 + (lane >> 3);
-        aof[b][l] = r < g.M ? (uint32_t)(r * g.lda) + ((piece ^ l * 4) << 4) : OUTSIDE;
-      }
-      const int r = b * 16 + (lane >> 2);
-      saof[b] = r < g.M ? ((uint32_t)(early_a + r * g.ldsa) & ~3u) + (lane & 3) * 16 : OUTSIDE;
-    }
-  }
-  int lround = blockIdx.x, lk = first, lperiod = 0, lplace = PLACES - 1;
+  const int period = ((uintptr_t)g.sw | (uintptr_t)g.ldsw | (uintptr_t)g.sa | (uintptr_t)g.ldsa) & 3 ? 7 : 8;
+  Unit lunit = start;
+  int lk = first, lperiod = 0, lplace = PLACES - 1;
   const auto enter = [&]() {
-    const int64_t n0 = ((int64_t)lround * groups + of_group) * 16;
+    const int64_t n0 = ((int64_t)lunit.round * groups + of_group) * 16;
     const int rows = n0 >= g.N ? 0 : g.N - n0 < 16 ? (int)(g.N - n0) : 16;
     bufW = buffer(g.w + n0 * g.ldw, rows ? (rows - 1) * g.ldw + g.B * 16 : 0);
     const uint8_t* const s = g.sw + n0 * g.ldsw;
@@ -441,11 +469,29 @@ __global__ __launch_bounds__(256) void few_kernel(MxArgs g, TokenArgs t, int KS)
     #pragma unroll
     for (int l = 0; l < 2; ++l) wof[l] = l * 8 + (lane >> 3) < rows ? (uint32_t)((l * 8 + (lane >> 3)) * g.ldw) + ((piece ^ l * 4) << 4) : OUTSIDE;
     sof = lane >> 2 < rows ? ((uint32_t)(early + (lane >> 2) * g.ldsw) & ~3u) + (lane & 3) * 16 : OUTSIDE;
+    if constexpr (OWN > 0) {
+      const int64_t m0 = (int64_t)lunit.team * 16 * TB;
+      const int tokens = g.M - m0 < 16 * TB ? (int)(g.M - m0) : 16 * TB;
+      const uint8_t* const sa = g.sa + m0 * g.ldsa;
+      const int early_a = (int)((uintptr_t)sa & 3);
+      bufA = buffer(g.a + m0 * g.lda, (tokens - 1) * g.lda + g.B * 16);
+      bufSA = buffer(sa - early_a, (early_a + (tokens - 1) * g.ldsa + g.B + 3) & ~(int64_t)3);
+      #pragma unroll
+      for (int b = 0; b < OWN; ++b) {
+        #pragma unroll
+        for (int l = 0; l < 2; ++l) {
+          const int r = b * 16 + l * 8 + (lane >> 3);
+          aof[b][l] = r < tokens ? (uint32_t)r * (uint32_t)g.lda + ((piece ^ l * 4) << 4) : OUTSIDE;
+        }
+        const int r = b * 16 + (lane >> 2);
+        saof[b] = r < tokens ? ((uint32_t)early_a + (uint32_t)r * (uint32_t)g.ldsa & ~3u) + (lane & 3) * 16 : OUTSIDE;
+      }
+    }
   };
   // The next stage, into a place; behind the last one: nothing, from outside.  The scales of a period come in front of its first stage.
   const auto fetch = [&](int slot) {
     const uint32_t to = mine + slot * S::BYTES;
-    const bool over = lround >= rounds;
+    const bool over = lunit.round >= rounds;
     if (lperiod == 0) {
       lplace = lplace == PLACES - 1 ? 0 : lplace + 1;
       const uint32_t too = mine + DEPTH * S::BYTES + lplace * S::SCALES;
@@ -474,9 +520,9 @@ __global__ __launch_bounds__(256) void few_kernel(MxArgs g, TokenArgs t, int KS)
     }
     if (++lk >= last && !over) {
       lk = first;
-      lround += gridDim.x;
+      lunit = next(lunit);
       lperiod = 0;
-      if (lround < rounds) enter();
+      if (lunit.round < rounds) enter();
     }
   };
   const bool works = first < last;                  // (K may have fewer stages than waves)
@@ -504,20 +550,22 @@ __global__ __launch_bounds__(256) void few_kernel(MxArgs g, TokenArgs t, int KS)
   __syncthreads();
 
   // ---- products ----
-  uint32_t at[2], sat[OWN ? OWN : 1], mat = 0, msat = 0;
+  uint32_t at[2], mat = 0, msat = 0;
   #pragma unroll
   for (int i = 0; i < 2; ++i) at[i] = mine + c * 128 + (((i * 4 + q) ^ (c >> 1 & 7)) << 4);
-  #pragma unroll
-  for (int b = 0; b < OWN; ++b)
-    sat[b] = mine + DEPTH * S::BYTES + 1024 * (1 + b) + c * 64 + q + (((uint32_t)early_a + (uint32_t)(b * 16 + c) * (uint32_t)g.ldsa) & 3);
   if constexpr (XT >= 0) {
     const int row = c < g.M ? c : 0;                // (a token past the last one is not stored)
     mat = lds0 + S::MADE + row * (bytes + 16);
     msat = lds0 + S::MADE + (uint32_t)g.M * (bytes + 16) + row * g.B;
   }
   int slot = 0, cperiod = 0, cplace = 0, turn = 0;
-  for (int round = blockIdx.x, nth = 0; round < rounds; round += gridDim.x, ++nth) {
-    const int64_t n0 = ((int64_t)round * groups + of_group) * 16;
+  Unit unit = start;
+  for (int nth = 0; unit.round < rounds; unit = next(unit), ++nth) {
+    const int64_t n0 = ((int64_t)unit.round * groups + of_group) * 16, m0 = (int64_t)unit.team * 16 * TB;
+    uint32_t sat[OWN ? OWN : 1];
+    #pragma unroll
+    for (int b = 0; b < OWN; ++b)
+      sat[b] = mine + DEPTH * S::BYTES + 1024 * (1 + b) + c * 64 + q + (((uint32_t)(uintptr_t)g.sa + (uint32_t)(m0 + b * 16 + c) * (uint32_t)g.ldsa) & 3);
     const uint32_t sw = mine + DEPTH * S::BYTES + c * 64 + q + (((uint32_t)(uintptr_t)g.sw + (uint32_t)(n0 + c) * (uint32_t)g.ldsw) & 3);
     f32x4 acc[TB] = {};
     for (int k = first; k < last; ++k) {
@@ -566,8 +614,8 @@ __global__ __launch_bounds__(256) void few_kernel(MxArgs g, TokenArgs t, int KS)
     for (int b = 0; b < TB; ++b) red[(wave * TB + b) * 64 + lane] = acc[b];
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     for (int o = tid; o < groups * TB * 256; o += 256) {
-      const int ch = o & 15, tok = o >> 4 & 15, b = (o >> 8) % TB, group = (o >> 8) / TB, token = b * 16 + tok;
-      const int64_t n = ((int64_t)round * groups + group) * 16 + ch;
+      const int ch = o & 15, tok = o >> 4 & 15, b = (o >> 8) % TB, group = (o >> 8) / TB;
+      const int64_t n = ((int64_t)unit.round * groups + group) * 16 + ch, token = m0 + b * 16 + tok;
       if (token >= g.M || n >= g.N) continue;
       float y = 0;
       for (int p = 0; p < KS; ++p) y += ((const float*)&red[((group * KS + p) * TB + b) * 64 + (ch >> 2) * 16 + tok])[ch & 3];
@@ -604,17 +652,18 @@ int launch_few(const MxArgs& g, const TokenArgs& t, int KS, hipStream_t st) {
   const auto kernel = few_kernel<TB, BF, XT, DEPTH, PLACES>;
   const int lds = S::MADE + (XT < 0 ? 0 : (int)(g.M * (g.B * 16 + 16) + g.M * g.B));
   if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return LCQ_ELAUNCH;
-  const int64_t rounds = ((g.N + 15) / 16 + 4 / KS - 1) / (4 / KS), most = 256 * (163840 / lds);
-  kernel<<<dim3((unsigned)(rounds < most ? rounds : most)), dim3(256), lds, st>>>(g, t, KS);
+  const int64_t units = mxfp4_units(g.M, g.N, KS), most = 256 * (163840 / lds);
+  kernel<<<dim3((unsigned)(units < most ? units : most)), dim3(256), lds, st>>>(g, t, KS);
   return LCQ_OK;
 }
-// Waves share K as long as each has four stages of it.  With that, scales of seven stages on their way are those of three periods at most; with
-// fewer, those of five stages of five.
+// Scales of seven stages on their way are those of three periods at most if every period but a unit's last has seven or eight stages, and a unit four;
+// with fewer, those of five stages are of five.
 template <int TB, int BF, int XT>
 int launch_few(const MxArgs& g, const TokenArgs& t, hipStream_t st) {
-  const int stages = (g.B + 7) / 8, KS = stages >= 16 ? 4 : stages >= 8 ? 2 : 1;
-  if constexpr (TB == 2) return stages >= 4 ? launch_few<2, BF, XT, 4, 3>(g, t, KS, st) : launch_few<2, BF, XT, 3, 3>(g, t, KS, st);
-  else return stages >= 4 ? launch_few<1, BF, XT, 7, 3>(g, t, KS, st) : launch_few<1, BF, XT, 5, 5>(g, t, KS, st);
+  const int KS = mxfp4_waves(g.M, g.N, g.B);
+  const bool four = ((g.B + 7) / 8) / KS >= 4;
+  if constexpr (TB == 2) return four ? launch_few<2, BF, XT, 4, 3>(g, t, KS, st) : launch_few<2, BF, XT, 3, 3>(g, t, KS, st);
+  else return four ? launch_few<1, BF, XT, 7, 3>(g, t, KS, st) : launch_few<1, BF, XT, 5, 5>(g, t, KS, st);
 }
 
 template <int BF>
@@ -672,20 +721,20 @@ int lcq_mxfp4_matmul(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t l
   if (lda > 1 << 22 || ldsa > 1 << 22) return LCQ_ESIZE;
   if ((uintptr_t)a % 16 || lda % 16) return LCQ_EALIGN;
   hipStream_t st = (hipStream_t)stream;
-  MxArgs g = {a, sa, w, sw, bias, y, M, N, lda, ldw, ldsa, ldsw, (int)B, bias_dtype};
+  MxArgs g = {a, sa, w, sw, bias, y, M, N, lda, ldw, ldsa, ldsw, 0, 0, (int)B, bias_dtype};
   const Mxfp4Cut c = mxfp4_cut(M, N, B);
   if (!c.stream) {
-    const bool pads = !on_pieces(sa, ldsa, B) || !on_pieces(sw, ldsw, B);
-    if (pads || c.parts > 1) {
+    const bool orders = c.tile == 0 || !on_pieces(sa, ldsa, B) || !on_pieces(sw, ldsw, B);
+    if (orders || c.parts > 1) {
       if (!workspace) return LCQ_EWORKSPACE;
       if ((uintptr_t)workspace % 16) return LCQ_EALIGN;
     }
-    if (pads) {
-      const int Bp = (int)on16(B);
+    g.nextsa = g.nextsw = 16;
+    if (orders) {
+      const int groups = (int)((B + 15) / 16);
       uint8_t* const to = (uint8_t*)workspace + (c.parts > 1 ? on256(4 * M * N * c.parts) : 0);
-      const int64_t words = (M + N) * (Bp / 4);
-      pad_scales_kernel<<<dim3((unsigned)((words + 255) / 256)), dim3(256), 0, st>>>(g, Bp, to, words);
-      g.sa = to; g.sw = to + M * Bp; g.ldsa = g.ldsw = Bp;
+      order_scales_kernel<<<dim3((unsigned)(((M + N) * groups + 255) / 256)), dim3(256), 0, st>>>(g, groups, to);
+      g.sa = to; g.sw = to + M * groups * 16; g.ldsa = g.ldsw = 16; g.nextsa = M * 16; g.nextsw = N * 16;
     }
   }
   float* const sums = (float*)workspace;
@@ -709,7 +758,7 @@ int lcq_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w, 
   if (!known(x_dtype)) return LCQ_EDTYPE;
   const int64_t B = (K + 31) / 32;
   if (fused(M, K)) {
-    const MxArgs g = {nullptr, nullptr, w, sw, bias, y, M, N, 0, ldw, 0, ldsw, (int)B, bias_dtype};
+    const MxArgs g = {nullptr, nullptr, w, sw, bias, y, M, N, 0, ldw, 0, ldsw, 0, 0, (int)B, bias_dtype};
     const TokenArgs t = {(const char*)x, ldx, K};
     hipStream_t st = (hipStream_t)stream;
     const auto run = [&](auto xt) {
