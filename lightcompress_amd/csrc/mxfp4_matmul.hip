@@ -535,14 +535,21 @@ __global__ __launch_bounds__(256) void few_kernel(MxArgs g, TokenArgs t, int KS)
   const int bytes = g.B * 16;
   uint8_t* const made_scales = made + g.M * (bytes + 16);
   if constexpr (XT >= 0) {                          // four lanes make a block
-    const int pieces = g.B * 4;
-    for (int r = 0; r < g.M; ++r) {
-      const char* const x = t.x + r * t.ldx * (XT == ROW_F32 ? 4 : 2);
-      for (int p = tid; p < pieces; p += 256) {
-        float v[8];
-        mx_load8<XT>(x, p * 8, t.K, v);
-        const uint32_t s = mx_scale(mx_quad_max(mx_max_bits(v)));
-        *(uint32_t*)(made + r * (bytes + 16) + p * 4) = mx_codes(v, s);
+    const uint32_t pieces = g.B * 4, all = (uint32_t)g.M * pieces;
+    constexpr int AT_ONCE = 4;                      // (a loop of single loads waits for memory every time)
+    for (uint32_t i0 = tid; i0 < all; i0 += AT_ONCE * 256) {
+      float v[AT_ONCE][8];
+      #pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        const uint32_t i = i0 + j * 256, r = i / pieces, p = i - r * pieces;
+        if (i < all) mx_load8<XT>(t.x + r * t.ldx * (XT == ROW_F32 ? 4 : 2), p * 8, t.K, v[j]);
+      }
+      #pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        const uint32_t i = i0 + j * 256, r = i / pieces, p = i - r * pieces;
+        if (i >= all) break;                        // (four neighbouring lanes together)
+        const uint32_t s = mx_scale(mx_quad_max(mx_max_bits(v[j])));
+        *(uint32_t*)(made + r * (bytes + 16) + p * 4) = mx_codes(v[j], s);
         if ((p & 3) == 0) made_scales[r * g.B + (p >> 2)] = (uint8_t)s;
       }
     }
@@ -695,8 +702,10 @@ int check(const uint8_t* w, int64_t ldw, const uint8_t* sw, int64_t ldsw, const 
   return LCQ_OK;
 }
 
-// tokens whose codes every workgroup of the product makes itself
-bool fused(int64_t M, int64_t K) { return M <= 2 && K <= 32768; }
+// Tokens whose codes every workgroup of the product makes itself, instead of a kernel of their own in front: its launch is 2.6 us, 4096 values by 256 lanes
+// 0.7 and off 16 bytes 1.0 (fused / not, us, N x K: 4096 x 4096 1 token 6.2 / 8.8, 4 tokens 8.3 / 9.2, 6 tokens 9.7 / 9.1; 1024 x 1024 16 tokens
+// 6.5 / 7.0; 1001 x 2047 4 tokens 7.6 / 7.8, 6 tokens 9.6 / 7.8).
+bool fused(int64_t M, int64_t K) { return M <= 16 && M * K <= (K % 8 ? 8192 : 16384); }
 
 bool on_pieces(const void* p, int64_t ld, int64_t B) { return (uintptr_t)p % 16 == 0 && ld % 16 == 0 && B % 16 == 0; }
 
