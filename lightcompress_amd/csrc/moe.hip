@@ -755,13 +755,17 @@ bool direct(int dtype, const void* x, int64_t ldx, int64_t K) {
   return dtype == LCQ_BF16 && K % 32 == 0 && ldx % 8 == 0 && (uintptr_t)x % 16 == 0 && ldx <= 1 << 22;       // (offsets have 31 bits)
 }
 
+int planes_of_h(int dtype) { return dtype == LCQ_F32 ? 4 : 2; }
+// tokens of a pass: as many as the offsets within h, 31 bits, have room for (64 at least)
+int64_t pass_of(int64_t top, int64_t I, int dtype) { return least(MOST_PASS, (1 << 30) / (top * planes_of_h(dtype) * ((I + 31) / 32 * 32) * 2)); }
+
 // How a pass of T tokens is cut.
 struct Cut {
   int P, PH, size, up_tiles, up_parts, down_tiles, down_parts, runs;
   int64_t groups, h, up, out;                       // bytes
   Cut(int64_t T, int64_t top, int64_t E, int64_t K, int64_t I, int64_t N, int dtype) {
     P = dtype == LCQ_BF16 ? 1 : dtype == LCQ_F16 ? 2 : 4;
-    PH = dtype == LCQ_F32 ? 4 : 2;
+    PH = planes_of_h(dtype);
     const int64_t slots = T * top;
     size = T <= 4 || slots <= E ? 4 : P == 4 || T <= 16 || slots <= 14 * E ? 16 : 32;
     groups = least(slots, least(E, slots) + slots / size);
@@ -826,9 +830,9 @@ int lcq_route(const void* logits, int dtype, int64_t T, int64_t E, int64_t ldl, 
 
 int64_t lcq_mxfp4_moe_workspace_bytes(int64_t T, int64_t top, int64_t E, int64_t K, int64_t I, int64_t N, int dtype) {
   if (T <= 0 || top <= 0 || E <= 0 || K <= 0 || I <= 0 || N <= 0 || K > 65536 || I > 65536 || N > 65536 || top > MOST_TOP || E > MOST_EXPERTS || !known(dtype)) return 0;
-  const int64_t t = least(T, MOST_PASS);
+  const int64_t pass = pass_of(top, I, dtype), t = least(T, pass);
   int64_t most = 0;                                 // (the last pass may have fewer tokens, and be cut into more parts)
-  for (const int64_t n : {t, T % MOST_PASS ? T % MOST_PASS : t}) {
+  for (const int64_t n : {t, T % pass ? T % pass : t}) {
     const Cut c(n, top, E, K, I, N, dtype);
     const int64_t size = c.h + c.up + c.out + on256(n * c.P * ((K + 31) / 32 * 32) * 2) + on256(n * top * 8);
     most = size > most ? size : most;
@@ -861,8 +865,9 @@ int lcq_mxfp4_moe(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, c
   const bool as_is = direct(dtype, x, ldx, K);
   Plan* const plan = (Plan*)ws;
   const int64_t size = dtype == LCQ_F32 ? 4 : 2, out_size = out_dtype == LCQ_F32 ? 4 : 2, logit_size = logits_dtype == LCQ_F32 ? 4 : 2;
-  for (int64_t t0 = 0; t0 < T; t0 += MOST_PASS) {
-    const int n = (int)least(T - t0, MOST_PASS);
+  const int64_t pass = pass_of(top, I, dtype);
+  for (int64_t t0 = 0; t0 < T; t0 += pass) {
+    const int n = (int)least(T - t0, pass);
     const Cut c(n, top, E, K, I, N, dtype);
     char* at = ws + on256(sizeof(Plan));
     uint16_t* const h = (uint16_t*)at;

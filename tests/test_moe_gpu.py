@@ -130,7 +130,7 @@ def check_layer(got, dtype, x, experts, weights, gate_up, down, gb, db, activati
     y, size, moved = layer(x, experts, weights, gate_up, down, gb, db, activation)
     K, I, E = gate_up.cols, down.cols, down.codes.shape[0]
     # sums in fp32: a step per 32 codes and plane, and those of the waves; the activation's few steps; planes of h: 2^-17 (fp32 tokens 2^-24);
-    # fp32 tokens in three planes: 2^-24; the weighted sums of the experts
+    # fp32 tokens in planes: 2^-24 (of a fourth plane even the steps are below that); the weighted sums of the experts
     planes = {BF: 1, HF: 2, F32: 3}[x.dtype]
     first = (planes * K / 32 + 16) * 2.0 ** -23 + (2.0 ** -23 if x.dtype == F32 else 0)
     second = (3 * I / 32 + 64) * 2.0 ** -23 + (2.0 ** -23 if x.dtype == F32 else 2.0 ** -17) + (E + 16) * 2.0 ** -23 + weight_error
@@ -247,6 +247,18 @@ def test_experts_behind_2_gigabytes(dev):
     part = lambda q: Mxfp4(q.codes[used], q.scales[used], q.cols)  # noqa: E731
     renamed = torch.tensor([[4, 0], [3, 4], [1, 2]], dtype=torch.int32, device=dev)
     check_layer(got, BF, x, renamed, weights, part(gate_up), part(down), None, None, 'silu')
+
+
+def test_products_between_behind_2_gigabytes(dev):
+    """128 tokens, 32 choices, 65536 channels in four planes of 16 bits: 2^31 bytes between the two products of one pass."""
+    E, K, I, N, T = 32, 32, 65536, 4, 128
+    g = gpu_gen(13)
+    gate_up, down = experts_of(E, 2 * I, K, g, dev), experts_of(E, N, I, g, dev)
+    x = torch.randn(T, K, generator=g, device=dev)
+    r = Routing(torch.arange(E, dtype=torch.int32, device=dev).repeat(T, 1), torch.rand(T, E, generator=g, device=dev))
+    got = mxfp4_moe(x, r, gate_up, down)
+    some = [0, 63, 64, 127]
+    check_layer(got[some], F32, x[some], r.experts[some], r.weights[some], gate_up, down, None, None, 'silu')
 
 
 def test_a_block_of_a_model(dev):
