@@ -620,15 +620,32 @@ __global__ __launch_bounds__(256) void few_kernel(MxArgs g, TokenArgs t, int KS)
     #pragma unroll
     for (int b = 0; b < TB; ++b) red[(wave * TB + b) * 64 + lane] = acc[b];
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    for (int o = tid; o < groups * TB * 256; o += 256) {
-      const int ch = o & 15, tok = o >> 4 & 15, b = (o >> 8) % TB, group = (o >> 8) / TB;
-      const int64_t n = ((int64_t)unit.round * groups + group) * 16 + ch, token = m0 + b * 16 + tok;
+    for (int o = tid; o < groups * TB * 64; o += 256) {      // four channels of a token
+      const int four = o & 3, tok = o >> 2 & 15, b = (o >> 6) % TB, group = (o >> 6) / TB, block = nth * groups + group;
+      const int64_t n = ((int64_t)unit.round * groups + group) * 16 + four * 4, token = m0 + b * 16 + tok;
       if (token >= g.M || n >= g.N) continue;
-      float y = 0;
-      for (int p = 0; p < KS; ++p) y += ((const float*)&red[((group * KS + p) * TB + b) * 64 + (ch >> 2) * 16 + tok])[ch & 3];
-      if (g.bias) y += nth * groups + group < MOST_BIASES ? biases[(nth * groups + group) * 16 + ch] : load_any(g.bias, g.bias_dtype, n);
-      if constexpr (BF == ROW_F32) ((float*)g.y)[token * g.N + n] = y;
-      else store_scalar<BF>(g.y, token * g.N + n, rnd<BF>(y));
+      const int left = g.N - n < 4 ? (int)(g.N - n) : 4;
+      f32x4 y = {};
+      for (int p = 0; p < KS; ++p) y += red[((group * KS + p) * TB + b) * 64 + four * 16 + tok];
+      if (g.bias) {
+        if (block < MOST_BIASES) y += *(const f32x4*)&biases[block * 16 + four * 4];           // (behind the last channel: anything)
+        else
+          #pragma unroll
+          for (int r = 0; r < 4; ++r) if (r < left) y[r] += load_any(g.bias, g.bias_dtype, n + r);
+      }
+      const int64_t cell = token * g.N + n;         // (rows may start anywhere)
+      if constexpr (BF == ROW_F32) {
+        if (left == 4) __builtin_memcpy((float*)g.y + cell, &y, 16);
+        else
+          #pragma unroll
+          for (int r = 0; r < 3; ++r) if (r < left) ((float*)g.y)[cell + r] = y[r];
+      } else {
+        const u32x2 v = BF == ROW_BF16 ? u32x2{bf16_pack_rne(y[0], y[1]), bf16_pack_rne(y[2], y[3])} : u32x2{f16_pack_rne(y[0], y[1]), f16_pack_rne(y[2], y[3])};
+        if (left == 4) __builtin_memcpy((uint16_t*)g.y + cell, &v, 8);
+        else
+          #pragma unroll
+          for (int r = 0; r < 3; ++r) if (r < left) ((uint16_t*)g.y)[cell + r] = (uint16_t)(v[r / 2] >> 16 * (r % 2));
+      }
     }
   }
   __builtin_amdgcn_s_waitcnt(0x0f70);               // nothing may still be on its way to LDS when the workgroup leaves it
