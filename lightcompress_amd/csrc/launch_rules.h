@@ -93,8 +93,8 @@ inline double mxfp4_rounds(double workgroups) { return (double)(long long)((work
 // The weight streamed past groups of 16 or 32 tokens: a unit of work is 4 / KS blocks of 16 channels with such a group, KS waves share the K of a block, and a
 // workgroup per CU takes its share of the units one behind the other.  A unit costs its waves' stages of 8 blocks of K, and 1.2 or 2.5 more where its sums are
 // joined; KS is what makes that least for a workgroup.  N x K with KS 1 / 2 / 4 for 16 and for 32 tokens:
-//   1024 x 1024  5.1 / 4.4 / 4.0   5.9 / 4.9 / 4.3    4096 x 4096   8.6 /  6.4 /  5.7    9.8 /  7.1 /  5.9    7168 x 2048  6.6 / 5.6 / 6.2   7.5 / 6.0 / 7.0
-//   6144 x 4096  8.7 / 6.7 / 7.5   9.7 / 7.2 / 8.3   14336 x 4096   9.6 / 10.4 / 11.7   10.7 / 11.7 / 13.8    2048 x 7168   12 / 7.9 / 6.2    13 / 8.7 / 6.7
+//   1024 x 1024  5.1 / 4.4 / 4.2   5.5 / 4.7 / 4.4    4096 x 4096   8.6 /  6.6 /  6.0    9.4 /  6.9 /  6.0    7168 x 2048  6.5 / 5.8 / 6.3    7.1 / 5.9 / 7.0
+//   6144 x 4096  8.6 / 6.8 / 7.7   9.5 / 7.1 / 8.5   14336 x 4096   9.7 / 10.5 / 12.1   10.7 / 11.4 / 13.7    2048 x 7168  11.6 / 8.0 / 6.5  12.7 / 8.7 / 6.9
 inline long long mxfp4_units(long long M, long long N, int KS) {
   const long long group = M <= 16 ? 16 : 32, blocks = (N + 15) / 16, at_once = 4 / KS;
   return (blocks + at_once - 1) / at_once * ((M + group - 1) / group);
@@ -110,10 +110,10 @@ inline int mxfp4_waves(long long M, long long N, long long B) {
 }
 // Or tiles of 256 x 256 or 128 x 128, the latter with K cut into parts of at least two periods of 16 blocks.  What is estimated to be fastest, measured as
 // streamed / 128 / 128 in 2 parts / in 4 / in 8 (and 256):
-//   4096 x 4096   64 tokens  7.7 / 12.4 / 12.3 / 12.6 / 15.2    128  10.6 / 12.5 / 13.0 / 14.9 / 16.2    211  17.6 / 12.9 / 14.4 / 17.8 / 22.6    2048  28.4 (32.3)
-//   4096 x 14336  64 tokens   16 /   35 /   26 /   20 /   18    128    23 /   37 /   29 /   22 /   20    211    45 /   41 /   29 /   22 /   31    1024  44.9 (88)
-//   14336 x 4096  33 tokens   18 / 14.7 / 14.7 /   20 /   30    211    56 /   17 /   31 /   45 /   67   1024    62 with 128 (40)
-//   1001 x 2047  128 tokens  5.4 /  9.4 / 10.0 / 10.8 / 13.2    512   7.9 /  9.5 / 11.1 / 12.9 / 19
+//   4096 x 4096    64 tokens  7.1 / 12.3 / 12.3 / 12.6 / 15.2    128   9.8 / 12.7 / 12.5 / 14.6 / 16.4    211  16.1 / 12.8 / 14.0 / 17.3 / 22.4    2048  29.8 (32.7)
+//   4096 x 14336   64 tokens   16 /   39 /   25 /   19 /   18    128    23 /   43 /   28 /   22 /   20    211    43 /   41 /   29 /   23 /   31    1024  45.2 (83)
+//   14336 x 4096   33 tokens   16 / 14.4 / 14.9 /   20 /   30    211    46 /   17 /   31 /   45 /   68   1024  62.5 with 128 (41.9)
+//   1001 x 2047   128 tokens  5.3 /  9.4 / 10.2 / 10.6 / 13.3    512   7.1 /  9.5 / 11.3 / 12.9 / 19
 struct Mxfp4Cut { bool stream; int tile, parts; };  // tile 0: 256 x 256, 1: 128 x 128
 inline Mxfp4Cut mxfp4_cut(long long M, long long N, long long B) {
   if (M <= 32) return {true, 0, 1};

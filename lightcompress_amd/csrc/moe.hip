@@ -1,6 +1,8 @@
 // A mixture-of-experts layer for a few tokens, on experts of microscaled 4-bit numbers:
 //   y[t] = sum_s w[t, s] (down_e h + down_bias_e),   h = act(gate_e x[t] + b) * (up_e x[t] + b),   e = experts[t, s]
-// Tokens that chose the same expert share one pass over its bytes, which is what bounds the layer.
+// Tokens that chose the same expert share one pass over its bytes, which is what bounds the layer: a plan (tokens by expert), gate and up, down, the
+// weighted sum, a kernel each, as each needs all of the one in front.  7168 x 2048, 8 of 256 experts: 1 token 6.4 + 26.9 + 14.4 + 4.0 us (4.5 TB/s of
+// weights while they stream, which is a ramp and a tail too at this length), 16 tokens 10.4 + 271 + 143 + 5.2 (5.7).
 //
 // The activations keep their precision.  A lane takes a block of a weight row, 16 bytes, and the conversion to bf16 applies its scale: that is
 // exact, so the products are those of the stored numbers.  bf16 tokens go into the matrix pipe as they are, others as sums of bf16 planes
@@ -174,6 +176,7 @@ __device__ __forceinline__ void route_token(const RouterArgs& r, int64_t t, int&
   weight *= r.scale;
 }
 
+// A wave per token, as much as fits a CU on its way: 64 tokens of 256 experts with a correction 5.1 us, a launch and the chain of one token; 16384 of 64 experts 8.1 us.
 template <int NL>
 __global__ __launch_bounds__(256) void route_kernel(RouterArgs r, int64_t T, int* __restrict__ experts, float* __restrict__ weights) {
   const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -193,7 +196,7 @@ struct Group {
 };
 struct Plan {
   int groups, pad[15];
-  uint32_t counter[COUNTERS];                       // parts of gate and up that are done
+  uint32_t counter[COUNTERS];                       // parts of gate and up that are done (fewer than 384 units have any)
   int slot[MOST_PASS * MOST_TOP], expert[MOST_PASS * MOST_TOP];              // of a token's choices; slot -1: none
   float weight[MOST_PASS * MOST_TOP];
   Group group[MOST_PASS * MOST_TOP];
@@ -213,7 +216,8 @@ __device__ __forceinline__ void planes_of(float v, uint16_t* out) {
   }
 }
 
-// Workgroup 0 plans the pass; the others lay the tokens out as planes [T, planes, Kp] where they are not that already.
+// Workgroup 0 plans the pass; the others lay the tokens out as planes [T, planes, Kp] where they are not that already.  One workgroup, as every place depends on
+// all choices: 6.4 us with the routing of 1 token of 256 experts, 10.4 of 16 tokens (their choices are a chain in each wave), 5.2 behind the router's kernel.
 template <int NL>
 __global__ __launch_bounds__(1024) void plan_kernel(RouterArgs r, const int* __restrict__ given, const float* __restrict__ given_weights, int T,
                                                     Operand o, int size, Plan* __restrict__ plan) {
@@ -767,13 +771,21 @@ struct Cut {
     P = dtype == LCQ_BF16 ? 1 : dtype == LCQ_F16 ? 2 : 4;
     PH = planes_of_h(dtype);
     const int64_t slots = T * top;
-    size = T <= 4 || slots <= E ? 4 : P == 4 || T <= 16 || slots <= 14 * E ? 16 : 32;
+    // Slots of a group: few columns cost less in every stage, a second group of an expert reads its bytes again.  The whole layer in us with 4 / 16 / 32:
+    //   4 tokens, 6 of 64 experts 39 / 48 / 55    16 tokens, 8 of 256 428 / 471 / 622    64 tokens, 4 of 32 143 / 94 / 123    64 tokens, 2 of 8 - / 97 / 96
+    //   (fp16 - / 106 / 115)    96 tokens, 2 of 8 - / 113 / 98 (fp16 - / 128 / 120)
+    size = T <= 4 || slots <= E ? 4 : P == 4 || T <= 16 || slots <= 18 * E ? 16 : 32;
     groups = least(slots, least(E, slots) + slots / size);
     const int64_t up_stages = ((K + 31) / 32 + 7) / 8, down_stages = ((I + 31) / 32 + 7) / 8, Ip = (I + 31) / 32 * 32;
     up_tiles = (int)((Ip + 63) / 64);
+    // Parts of K of gate and up, where a few narrow experts leave the chip to a few long units: a stage is 0.45 us, making sums visible to the workgroup that adds
+    // them up 0.15 for every workgroup.  1 token, 1 of 4 experts 14336 x 128 in 1 / 2 / 4 / 8 parts 51 / 37 / 29 / 30 us, 2 of 8 7168 x 256 34 / 29 / 28 / 32, but 4 of 16
+    // 1024 x 512 20 / 30 and 8 of 256 7168 x 2048 56 / 176.
     up_parts = 1;
-    while (groups * up_tiles * up_parts < 200 && up_stages / (2 * up_parts) >= 3) up_parts *= 2;
+    while (3 * up_stages > 2 * groups * up_tiles * up_parts * up_parts && up_stages / (2 * up_parts) >= 3) up_parts *= 2;
     down_tiles = (int)((N + 127) / 128);
+    // Runs of down: two workgroups per CU (64 tokens, 4 of 32 experts with 1 / 2 / 4 per CU 92 / 95 / 104, 16 tokens, 8 of 256 463 / 450 / 456); K in parts
+    // where there are too few groups for them (1 token, 2 of 8 experts 4096 x 14336 in 1 / 2 / 4 / 8 parts 77 / 62 / 56 / 54; 8 of 256 56 / 57 / 58).
     int64_t want = 512 / down_tiles;
     if (want < 1) want = 1;
     down_parts = 1;
@@ -882,7 +894,7 @@ int lcq_mxfp4_moe(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, c
     const int64_t slots = (int64_t)n * top;
     const int* ge = experts ? experts + t0 * top : nullptr;
     const float* gw = experts ? weights + t0 * top : nullptr;
-    if (logits && n > 16) {                         // (the waves of one workgroup would take longer)
+    if (logits && n > 16) {                         // (the plan's 16 waves would take turns; up to there a kernel less is 2 us less)
       int* const e = (int*)((char*)planes + on256(n * c.P * Kp * 2));
       const int rc = lcq_route(rt.logits, logits_dtype, n, E, ldl, top, flags, correction, scale, e, (float*)(e + slots), stream);
       if (rc) return rc;

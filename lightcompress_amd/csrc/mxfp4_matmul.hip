@@ -49,6 +49,10 @@ __device__ __forceinline__ i32x8 wide(i32x4 v) { return __builtin_shufflevector(
 //    registers at the end of the period before theirs: a load of four scales per row and stage would fetch a line per row and stage;
 //  * operands are buffered in registers: while the products of one step of 64 codes run, the reads of the next are issued between them;
 //    one barrier per stage, where every wave holds the rest of it in registers: its place is loaded again from there.
+// Tiles of 256 x 256 are bound by the chip's power: 8192 x 14336 x 4096 takes 251 us (3.8 PFLOP/s) with the products at 1.55 GHz, 192 on zeros at 2.35.  A
+// round of tiles is 3.4 us of first loads, 25 of products (38 900 clocks, the pipe alone 32 800), 4.5 of outputs.  With nothing loaded behind the first stages the products
+// run at 1.68 GHz, without reads of LDS either at 1.92; loading the next tile's first stages before the outputs leave, or whole lines in two stages of 128
+// bytes, took as long.  Tiles of 128 x 128 are bound by the loads on their way (a round of 224 with K = 4096: 17 us, 1.9 TB/s of weights).
 constexpr int ROW_SUM = 3;                          // an output type: the sums of a part of K as they are
 constexpr int PERIOD = 256;                         // bytes of a row between scale loads
 
@@ -368,8 +372,8 @@ __global__ __launch_bounds__(256) void join_kernel(MxArgs g, const float* __rest
 }
 
 // Scales for tiles: [16 scales of a row][row][16], with zeros behind a row's last, those of a and then those of w.  A tile's loads of them are then whole
-// lines; in the rows' own order each of 64 lanes reads 16 bytes of a line of its own, again in every tile of its stripe (8192 x 14336 x 4096: 276 us
-// against 240 without any).
+// lines; in the rows' own order each of 64 lanes reads 16 bytes of a line of its own, again in every tile of its stripe (8192 x 14336 x 4096: 285 us, with
+// this kernel's 4 276).  Tiles of 128 x 128 gain nothing by it: 1024 x 4096 x 4096 16.2 us, 18.4 with it.
 __global__ __launch_bounds__(256) void order_scales_kernel(MxArgs g, int groups, uint8_t* __restrict__ out) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, of_a = g.M * groups;
   if (i >= of_a + g.N * groups) return;
@@ -389,8 +393,8 @@ __global__ __launch_bounds__(256) void order_scales_kernel(MxArgs g, int groups,
 // ---- few tokens ---------------------------------------------------------------------------------------------------
 // The weight streams past the tokens.  A wave has a block of 16 channels and a KS-th of K; stages of 256 codes go through its own part of LDS by
 // direct loads of whole lines, DEPTH - 1 stages ahead, without a break from one block to the next, and nothing but the joining of a
-// block's KS waves makes waves wait for one another.  (Loaded straight into the matrix pipe's layout, 16 neighbouring lanes are 16 rows and
-// every KB passes the cache 64 times: 16 tokens by 4096 x 14336 took 16.5 us.)
+// block's KS waves makes waves wait for one another.  16 tokens by 4096 x 14336 take 10.0 us (3.1 TB/s of weights; 3.4 are the launch and the first loads).
+// Loaded straight into the matrix pipe's layout, 16 neighbouring lanes are 16 rows and every KB passes the cache 64 times: 16.5 us.
 //   codes of the weight and of the tokens   16 rows x 128 bytes; 16-byte piece p of row r lies at p ^ (r / 2 % 8)
 //   scales   the word-aligned 64 bytes of a row that hold those of eight stages, or of seven where rows are off words
 // Where there are few tokens, every workgroup makes their codes itself, in LDS, while its first weights are on their way.
