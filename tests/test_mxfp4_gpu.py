@@ -182,6 +182,16 @@ def test_product(dev, M, N, K, bias, dtype):
     assert bool((err <= tol).all()), f'{float((err / tol).max())} of the tolerance'
 
 
+CUTS = [(5, 14336, 520), (9, 6145, 4100), (13, 300017, 96), (20, 14300, 1100), (25, 7170, 2050), (45, 14335, 300), (90, 2500, 16000), (61, 40001, 200),
+        (211, 4000, 14300), (300, 3000, 10000), (1000, 14300, 4100)]
+
+
+@pytest.mark.parametrize('dtype', [F32, BF])
+@pytest.mark.parametrize('M,N,K', CUTS)
+def test_product_of_every_cut(dev, M, N, K, dtype):
+    test_product(dev, M, N, K, True, dtype)
+
+
 @pytest.mark.parametrize('M,N,K', [(1, 300, 2048), (2, 77, 1000), (5, 100, 1999), (16, 515, 2048), (30, 64, 1056), (64, 200, 2048), (65, 130, 2000),
                                    (200, 600, 1537), (3000, 4100, 1030), (257, 255, 1024), (4097, 4097, 544)])
 def test_sums_that_fit_are_exact(dev, M, N, K):
