@@ -579,7 +579,7 @@ int lcq_route(const void* logits, int dtype, int64_t T, int64_t E, int64_t ldl, 
 
 /* A mixture-of-experts layer for a few tokens, the experts in microscaled 4-bit numbers, sums in fp32:
  *    y[t] = sum_s weight[t, s] (down_e (act(gate_e x[t] + b) * (up_e x[t] + b)) + b),  e = expert[t, s]
- *  x       [T, K] of `dtype`, rows ldx elements apart.  Any T; up to 128 tokens share a pass over the experts' bytes
+ *  x       [T, K] of `dtype`, rows ldx elements apart.  T <= 2^25; up to 128 tokens share a pass over the experts' bytes
  *  logits  [T, E] (logits_dtype, ldl) with flags, correction and scale of lcq_route, and experts, weights NULL; or
  *  experts [T, top] int32, weights [T, top] fp32 (logits NULL): an index outside 0 .. E - 1 is no expert, several of the same of a token count
  *          as one with the sum of their weights
