@@ -5,8 +5,10 @@
 // weights while they stream, which is a ramp and a tail too at this length), 16 tokens 10.4 + 271 + 143 + 5.2 (5.7).
 //
 // The activations keep their precision.  A lane takes a block of a weight row, 16 bytes, and the conversion to bf16 applies its scale: that is
-// exact, so the products are those of the stored numbers.  bf16 tokens go into the matrix pipe as they are, others as sums of bf16 planes
-// (fp16: two, exactly; fp32: four); h, which stays within the layer, as two planes (2^-17), or four for fp32 tokens.
+// exact, so the products are those of the stored numbers.  bf16 tokens go into the matrix pipe as they are, fp32 ones as sums of four bf16 planes; h,
+// which stays within the layer, as two planes (2^-17), or four for fp32 tokens.  fp16 tokens go as they are too, with the weights' blocks as fp16, which is
+// exact for scales of 2^-23 .. 2^13; stages with others take the tokens apart into two bf16 numbers (gate and up of 50 tokens, 2 of 8 experts 4090 x 14336: 129 us, as two
+// planes throughout 161; of 96 tokens 4096 x 4096 45 and 66).
 #include "mxfp4.h"
 #include <type_traits>
 
@@ -15,6 +17,8 @@ using namespace lcq;
 
 typedef __attribute__((ext_vector_type(4))) int i32x4;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 
 template <int I> using Int = std::integral_constant<int, I>;
 
@@ -229,6 +233,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(RouterArgs r, const int* __r
       const float v = k < o.K ? load_any(o.x, o.dtype, t * o.ldx + k) : 0.0f;
       uint16_t p[4];
       planes_of<4>(v, p);
+      if (o.dtype == LCQ_F16) p[0] = __builtin_bit_cast(uint16_t, (_Float16)v);              // (one plane)
       for (int q = 0; q < o.planes; ++q) o.out[(t * o.planes + q) * o.Kp + k] = p[q];
     }
     return;
@@ -325,7 +330,7 @@ struct Weights {
 };
 
 struct MoeArgs {
-  const uint16_t* x;                                // planes of the tokens: P of Kp, ldp apart, tokens ldx apart
+  const uint16_t* x;                                // planes of the tokens (bf16, or one of fp16): P of Kp, ldp apart, tokens ldx apart
   int64_t ldx, ldp;
   Weights gate_up, down;
   Plan* plan;
@@ -340,6 +345,24 @@ __device__ __forceinline__ bf16x8 decoded(int codes, float f) {
   const lcq_bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((uint32_t)codes, f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((uint32_t)codes, f, 1),
                    c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((uint32_t)codes, f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((uint32_t)codes, f, 3);
   return bf16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// the same to fp16: exact for scale bytes of LEAST_HALF .. MOST_HALF, as 0.5 * 2^-23 is its least number and 6 * 2^13 below its largest
+constexpr uint32_t LEAST_HALF = 104, MOST_HALF = 140;
+__device__ __forceinline__ f16x8 decoded_half(int codes, float f) {
+  const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4((uint32_t)codes, f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4((uint32_t)codes, f, 1),
+              c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4((uint32_t)codes, f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4((uint32_t)codes, f, 3);
+  return f16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+// eight fp16 numbers as sums of two bf16 ones, exactly (what is infinite or NaN: in the first alone)
+__device__ __forceinline__ void two_of(bf16x8 raw, bf16x8 (&out)[2]) {
+  const f16x8 v = __builtin_bit_cast(f16x8, raw);
+  #pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float f = (float)v[e], high = u2f(bf16_bits(f) << 16);
+    out[0][e] = (__bf16)high;
+    out[1][e] = (__bf16)(__builtin_isfinite(f) ? f - high : 0.0f);
+  }
 }
 
 __device__ __forceinline__ float act(float v, int activation) {
@@ -400,7 +423,7 @@ __device__ __forceinline__ bool last_of(uint32_t* counter, int parts) {
 //   down: (group, part of K) of one tile of 128 channels, a workgroup takes one of `runs` runs of them.
 // With one wave per SIMD it is bound by the instructions it issues, so what is the same for all stages of a unit, or for all but its last, is
 // not looked at in every stage.
-template <bool DOWN, int P, int GS, int PH>
+template <bool DOWN, int P, int GS, int PH, bool HALF>
 __global__ __launch_bounds__(256) void experts_kernel(MoeArgs g, int tiles, int parts, int runs) {
   typedef Shape<P, GS> S;
   constexpr int CB = S::CB, DEPTH = S::DEPTH, WIDTH = DOWN ? 128 : 64;
@@ -661,6 +684,48 @@ __global__ __launch_bounds__(256) void experts_kernel(MoeArgs g, int tiles, int 
       }
       __builtin_amdgcn_sched_barrier(0);
       const int left = B - now.k * 8;
+      if constexpr (HALF) {
+        bool other = false;                         // (a block behind the last has zeros for codes: any scale will do)
+        #pragma unroll
+        for (int i = 0; i < 2; ++i)
+          #pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            byte[u][i] = i * 4 + q < left ? byte[u][i] : 127u;
+            other = other || byte[u][i] < LEAST_HALF || byte[u][i] > MOST_HALF;
+          }
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(other) != 0, 0)) {
+          #pragma unroll
+          for (int i = 0; i < 2; ++i)
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              bf16x8 v[2];
+              #pragma unroll
+              for (int u = 0; u < 2; ++u) v[u] = decoded(wv[u][i][j], mx_factor(byte[u][i]));
+              #pragma unroll
+              for (int b = 0; b < CB; ++b) {
+                bf16x8 two[2];
+                two_of(x[i][j][b], two);
+                #pragma unroll
+                for (int u = 0; u < 2; ++u)
+                  #pragma unroll
+                  for (int l = 0; l < 2; ++l) acc[u][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u], two[l], acc[u][b], 0, 0, 0);
+              }
+            }
+        } else {
+          #pragma unroll
+          for (int i = 0; i < 2; ++i)
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              f16x8 v[2];
+              #pragma unroll
+              for (int u = 0; u < 2; ++u) v[u] = decoded_half(wv[u][i][j], mx_factor(byte[u][i]));
+              #pragma unroll
+              for (int b = 0; b < CB; ++b)
+                #pragma unroll
+                for (int u = 0; u < 2; ++u) acc[u][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[u], __builtin_bit_cast(f16x8, x[i][j][b]), acc[u][b], 0, 0, 0);
+            }
+        }
+      } else
       #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const uint32_t there = i * 4 + q < left ? 255u : 0u;                 // (behind the last block: not a NaN)
@@ -756,7 +821,7 @@ int check_router(const RouterArgs& r, int64_t T) {
 
 // are the tokens planes as they are?
 bool direct(int dtype, const void* x, int64_t ldx, int64_t K) {
-  return dtype == LCQ_BF16 && K % 32 == 0 && ldx % 8 == 0 && (uintptr_t)x % 16 == 0 && ldx <= 1 << 22;       // (offsets have 31 bits)
+  return dtype != LCQ_F32 && K % 32 == 0 && ldx % 8 == 0 && (uintptr_t)x % 16 == 0 && ldx <= 1 << 22;       // (offsets have 31 bits)
 }
 
 int planes_of_h(int dtype) { return dtype == LCQ_F32 ? 4 : 2; }
@@ -768,12 +833,12 @@ struct Cut {
   int P, PH, size, up_tiles, up_parts, down_tiles, down_parts, runs;
   int64_t groups, h, up, out;                       // bytes
   Cut(int64_t T, int64_t top, int64_t E, int64_t K, int64_t I, int64_t N, int dtype) {
-    P = dtype == LCQ_BF16 ? 1 : dtype == LCQ_F16 ? 2 : 4;
+    P = dtype == LCQ_F32 ? 4 : 1;
     PH = planes_of_h(dtype);
     const int64_t slots = T * top;
     // Slots of a group: few columns cost less in every stage, a second group of an expert reads its bytes again.  The whole layer in us with 4 / 16 / 32:
     //   4 tokens, 6 of 64 experts 39 / 48 / 55    16 tokens, 8 of 256 428 / 471 / 622    64 tokens, 4 of 32 143 / 94 / 123    64 tokens, 2 of 8 - / 97 / 96
-    //   (fp16 - / 106 / 115)    96 tokens, 2 of 8 - / 113 / 98 (fp16 - / 128 / 120)
+    //   96 tokens, 2 of 8 - / 113 / 98
     size = T <= 4 || slots <= E ? 4 : P == 4 || T <= 16 || slots <= 18 * E ? 16 : 32;
     groups = least(slots, least(E, slots) + slots / size);
     const int64_t up_stages = ((K + 31) / 32 + 7) / 8, down_stages = ((I + 31) / 32 + 7) / 8, Ip = (I + 31) / 32 * 32;
@@ -798,10 +863,10 @@ struct Cut {
   }
 };
 
-template <bool DOWN, int P, int GS, int PH>
+template <bool DOWN, int P, int GS, int PH, bool HALF>
 int launch_experts(const MoeArgs& g, const Cut& c, hipStream_t st) {
   typedef Shape<P, GS> S;
-  const auto kernel = experts_kernel<DOWN, P, GS, PH>;
+  const auto kernel = experts_kernel<DOWN, P, GS, PH, HALF>;
   // (more LDS than a launch may have without asking)
   if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS) != hipSuccess) return LCQ_ELAUNCH;
   // as many as run at a time, or fewer
@@ -809,11 +874,11 @@ int launch_experts(const MoeArgs& g, const Cut& c, hipStream_t st) {
   kernel<<<dim3((unsigned)blocks), dim3(256), S::LDS, st>>>(g, DOWN ? c.down_tiles : c.up_tiles, DOWN ? c.down_parts : c.up_parts, c.runs);
   return LCQ_OK;
 }
-template <bool DOWN, int P, int PH>
+template <bool DOWN, int P, int PH, bool HALF>
 int launch_size(const MoeArgs& g, const Cut& c, hipStream_t st) {
-  if (c.size == 4) return launch_experts<DOWN, P, 4, PH>(g, c, st);
-  if constexpr (P < 4) { if (c.size == 32) return launch_experts<DOWN, P, 32, PH>(g, c, st); }
-  return launch_experts<DOWN, P, 16, PH>(g, c, st);
+  if (c.size == 4) return launch_experts<DOWN, P, 4, PH, HALF>(g, c, st);
+  if constexpr (P < 4) { if (c.size == 32) return launch_experts<DOWN, P, 32, PH, HALF>(g, c, st); }
+  return launch_experts<DOWN, P, 16, PH, HALF>(g, c, st);
 }
 template <int BF>
 void launch_sum(const MoeArgs& g, const Cut& c, hipStream_t st) {
@@ -908,9 +973,9 @@ int lcq_mxfp4_moe(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, c
     if (E <= 64) plan_kernel<1><<<grid, dim3(1024), 0, st>>>(rt, ge, gw, n, o, c.size, plan);
     else if (E <= 256) plan_kernel<4><<<grid, dim3(1024), 0, st>>>(rt, ge, gw, n, o, c.size, plan);
     else plan_kernel<16><<<grid, dim3(1024), 0, st>>>(rt, ge, gw, n, o, c.size, plan);
-    int rc = c.P == 1 ? launch_size<false, 1, 2>(g, c, st) : c.P == 2 ? launch_size<false, 2, 2>(g, c, st) : launch_size<false, 4, 4>(g, c, st);
+    int rc = dtype == LCQ_BF16 ? launch_size<false, 1, 2, false>(g, c, st) : dtype == LCQ_F16 ? launch_size<false, 1, 2, true>(g, c, st) : launch_size<false, 4, 4, false>(g, c, st);
     if (rc) return rc;
-    rc = c.PH == 2 ? launch_size<true, 2, 2>(g, c, st) : launch_size<true, 4, 4>(g, c, st);
+    rc = c.PH == 2 ? launch_size<true, 2, 2, false>(g, c, st) : launch_size<true, 4, 4, false>(g, c, st);
     if (rc) return rc;
     if (out_dtype == LCQ_BF16) launch_sum<ROW_BF16>(g, c, st);
     else if (out_dtype == LCQ_F16) launch_sum<ROW_F16>(g, c, st);

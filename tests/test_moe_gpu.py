@@ -165,6 +165,22 @@ def test_layer(dev, T, E, top, K, I, N, bias, activation, dtype):
     assert torch.equal(wide.to(dtype), got)
 
 
+@pytest.mark.parametrize('dtype', [BF, HF, F32])
+@pytest.mark.parametrize('low,high', [(95, 146), (90, 100), (103, 105), (139, 142), (150, 160), (104, 141)])
+@pytest.mark.parametrize('T', [3, 20])
+def test_scales_of_any_size(dev, T, low, high, dtype):
+    """Blocks beyond what fp16 holds beside others, and blocks of zeros with the least scale."""
+    g = gpu_gen(low + high)
+    E, top, K, I, N = 4, 2, 1000, 70, 48
+    x = torch.randn(T, K, generator=g, device=dev).to(dtype)
+    gate_up, down = random_mx(E * 2 * I, K, g, dev, low, high), experts_of(E, N, I, g, dev)
+    gate_up = Mxfp4(gate_up.codes.view(E, 2 * I, -1), gate_up.scales.view(E, 2 * I, -1), K)
+    gate_up.codes[1, 3, 32:48], gate_up.scales[1, 3, 2], gate_up.codes[2, 69, :], gate_up.scales[2, 69, :] = 0, 0, 0, 0
+    r = route_tokens(Router(torch.randn(T, E, generator=g, device=dev), top))
+    got = mxfp4_moe(x, r, gate_up, down, out_dtype=F32)
+    check_layer(got, F32, x, r.experts, r.weights, gate_up, down, None, None, 'silu')
+
+
 @pytest.mark.parametrize('T,crowd', [(20, 20), (64, 60), (128, 128), (100, 33)])
 def test_tokens_that_crowd_one_expert(dev, T, crowd):
     """More than 16 tokens of one expert, beside lonely ones."""
