@@ -2,7 +2,7 @@
 //
 // A lane takes eight values (of a bf16 row 16 bytes), four neighbouring lanes a block: its largest magnitude comes from two quad
 // permutations, so nothing waits for the rest of the row.  Four pieces of a lane are on their way at a time.  Bound by memory: 2.53 bytes a value for bf16,
-// either way.  4096 x 14336 to codes 29.4 us (5.0 TB/s, a copy has 5.2), back 22.9 (6.5); 16 x 4096 3.7 and 2.9, which is a launch and a load.
+// either way.  4096 x 14336 to codes 29.4 us (5.0 TB/s, a copy has 5.2), back 22.9 (6.5); 16 x 4096 2.8 and 2.8, which is a launch and a load.
 #include "mxfp4.h"
 #include <type_traits>
 
@@ -10,11 +10,11 @@ namespace {
 using namespace lcq;
 
 template <int I> using Int = std::integral_constant<int, I>;
-constexpr int PIECES = 4;                           // of eight values, per lane
+constexpr int MOST_PIECES = 4;                      // of eight values, per lane
 
 struct Rows {
   int64_t rows, K, pieces, ldx;                     // pieces: of eight values in the whole blocks of a row
-  int lanes;                                        // that share a row (a power of two, 4 .. 256)
+  int lanes, each;                                  // that share a row (a power of two, 4 .. 256); pieces of a lane
   uint32_t chunks;                                  // workgroups along a row
 };
 
@@ -22,12 +22,12 @@ struct Rows {
 __device__ __forceinline__ bool place(const Rows& r, int64_t& row, int64_t& piece, int& step) {
   const uint32_t rows = blockIdx.x / r.chunks, chunk = blockIdx.x - rows * r.chunks;
   row = (int64_t)rows * (256 / r.lanes) + threadIdx.x / r.lanes;
-  piece = (int64_t)chunk * (r.lanes * PIECES) + (threadIdx.x & (r.lanes - 1));
+  piece = (int64_t)chunk * (r.lanes * r.each) + (threadIdx.x & (r.lanes - 1));
   step = r.lanes;
   return row < r.rows;
 }
 
-template <int XT>
+template <int XT, int PIECES>
 __global__ __launch_bounds__(256) void quant_kernel(const char* __restrict__ x, Rows r, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                                                     int64_t lds) {
   int64_t row, piece;
@@ -50,7 +50,7 @@ __global__ __launch_bounds__(256) void quant_kernel(const char* __restrict__ x, 
   }
 }
 
-template <int BF>
+template <int BF, int PIECES>
 __global__ __launch_bounds__(256) void dequant_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const uint8_t* __restrict__ scales, int64_t lds,
                                                       Rows r, char* __restrict__ y) {
   int64_t row, piece;
@@ -98,13 +98,27 @@ int plan(int64_t rows, int64_t K, int64_t ldx, bool joined, Rows& r, dim3& grid)
   if (rows <= 0 || K <= 0 || ldx < 0) return LCQ_EINVAL;
   if (K > (int64_t)1 << 36 || rows > ((int64_t)1 << 36) / ((K + 31) / 32 * 32)) return LCQ_ESIZE;
   if (joined && K % 32 == 0) { K *= rows; rows = 1; }
-  r = Rows{rows, K, (K + 31) / 32 * 4, ldx, 256, 1};
-  while (r.lanes > 4 && r.lanes / 2 * PIECES >= r.pieces) r.lanes /= 2;
-  r.chunks = (uint32_t)((r.pieces + r.lanes * PIECES - 1) / (r.lanes * PIECES));
+  r = Rows{rows, K, (K + 31) / 32 * 4, ldx, 256, MOST_PIECES, 1};
+  // Four loads of a lane run side by side; where there would be fewer workgroups than CUs a lane has one (bf16 rows of 14336 to codes, 1 / 4 pieces: 32 rows
+  // 2.8 / 3.7 us, 128 rows 3.4 / 3.8, 256 rows 4.1 / 4.3; back, 32 rows 2.8 / 3.0, 512 rows 6.0 / 5.6, 1024 rows 8.6 / 7.8).
+  if (rows * r.pieces < 256 * 256 * MOST_PIECES) r.each = 1;
+  while (r.lanes > 4 && r.lanes / 2 * r.each >= r.pieces) r.lanes /= 2;
+  r.chunks = (uint32_t)((r.pieces + r.lanes * r.each - 1) / (r.lanes * r.each));
   const int64_t blocks = (rows + 256 / r.lanes - 1) / (256 / r.lanes) * r.chunks;
   if (blocks > (1 << 24) - 1) return LCQ_ESIZE;
   grid = dim3((unsigned)blocks);
   return LCQ_OK;
+}
+
+template <class Run>
+void by_size(const Rows& r, int dtype, const Run& run) {
+  const auto typed = [&](auto each) {
+    if (dtype == LCQ_BF16) run(Int<ROW_BF16>{}, each);
+    else if (dtype == LCQ_F16) run(Int<ROW_F16>{}, each);
+    else run(Int<ROW_F32>{}, each);
+  };
+  if (r.each == 1) typed(Int<1>{});
+  else typed(Int<MOST_PIECES>{});
 }
 
 }  // namespace
@@ -120,9 +134,8 @@ int lcq_mxfp4_quant(const void* x, int dtype, int64_t rows, int64_t K, int64_t l
   const int bad = plan(rows, K, ldx, ldx == K && lds == K / 32, r, grid);
   if (bad) return bad;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == LCQ_BF16) quant_kernel<ROW_BF16><<<grid, dim3(256), 0, st>>>((const char*)x, r, codes, scales, lds);
-  else if (dtype == LCQ_F16) quant_kernel<ROW_F16><<<grid, dim3(256), 0, st>>>((const char*)x, r, codes, scales, lds);
-  else quant_kernel<ROW_F32><<<grid, dim3(256), 0, st>>>((const char*)x, r, codes, scales, lds);
+  const auto run = [&](auto xt, auto each) { quant_kernel<decltype(xt)::value, decltype(each)::value><<<grid, dim3(256), 0, st>>>((const char*)x, r, codes, scales, lds); };
+  by_size(r, dtype, run);
   LCQ_CHECK_LAUNCH();
   return LCQ_OK;
 }
@@ -136,9 +149,8 @@ int lcq_mxfp4_dequant(const uint8_t* codes, int64_t ldc, const uint8_t* scales, 
   const int bad = plan(rows, K, 0, ldc == K / 2 && lds == K / 32, r, grid);
   if (bad) return bad;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == LCQ_BF16) dequant_kernel<ROW_BF16><<<grid, dim3(256), 0, st>>>(codes, ldc, scales, lds, r, (char*)y);
-  else if (dtype == LCQ_F16) dequant_kernel<ROW_F16><<<grid, dim3(256), 0, st>>>(codes, ldc, scales, lds, r, (char*)y);
-  else dequant_kernel<ROW_F32><<<grid, dim3(256), 0, st>>>(codes, ldc, scales, lds, r, (char*)y);
+  const auto run = [&](auto xt, auto each) { dequant_kernel<decltype(xt)::value, decltype(each)::value><<<grid, dim3(256), 0, st>>>(codes, ldc, scales, lds, r, (char*)y); };
+  by_size(r, dtype, run);
   LCQ_CHECK_LAUNCH();
   return LCQ_OK;
 }

@@ -723,9 +723,9 @@ int check(const uint8_t* w, int64_t ldw, const uint8_t* sw, int64_t ldsw, const 
   return LCQ_OK;
 }
 
-// Tokens whose codes every workgroup of the product makes itself, instead of a kernel of their own in front: its launch is 2.6 us, 4096 values by 256 lanes
-// 0.7 and off 16 bytes 1.0 (fused / not, us, N x K: 4096 x 4096 1 token 6.2 / 8.8, 4 tokens 8.3 / 9.2, 6 tokens 9.7 / 9.1; 1024 x 1024 16 tokens
-// 6.5 / 7.0; 1001 x 2047 4 tokens 7.6 / 7.8, 6 tokens 9.6 / 7.8).
+// Tokens whose codes every workgroup of the product makes itself, instead of a kernel of their own in front: that is 2.2 us, and 4 of the host's; 4096 values by 256 lanes are
+// 0.7 and off 16 bytes 1.0 (fused / not, us, N x K: 4096 x 4096 1 token 6.3 / 8.1, 4 tokens 8.4 / 8.3, 6 tokens 9.9 / 8.4; 1024 x 1024 16 tokens 6.7 / 6.3;
+// 1001 x 2047 3 tokens 6.7 / 6.9, 4 tokens 7.6 / 6.9).
 bool fused(int64_t M, int64_t K) { return M <= 16 && M * K <= (K % 8 ? 8192 : 16384); }
 
 bool on_pieces(const void* p, int64_t ld, int64_t B) { return (uintptr_t)p % 16 == 0 && ld % 16 == 0 && B % 16 == 0; }
