@@ -44,6 +44,14 @@ __device__ __forceinline__ uint32_t mx_quad_max(uint32_t m) {
   return b > m ? b : m;
 }
 
+typedef u32x4 u32x4_anywhere __attribute__((aligned(2)));      // rows may start on any element
+// 16 bytes that go past the caches.  (The asm keeps the store from being made one with the same store on another path, which would lose that.)
+__device__ __forceinline__ void mx_store_past(void* to, u32x4 v) {
+  asm volatile("");
+  __builtin_nontemporal_store(v, (u32x4_anywhere*)to);
+  asm volatile("");
+}
+
 // Eight values of a row of XT, from element k on; what lies behind K is 0.  Rows may start on any element.
 template <int XT>
 __device__ __forceinline__ void mx_load8(const char* row, int64_t k, int64_t K, float* v) {
