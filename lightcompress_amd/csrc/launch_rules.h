@@ -93,8 +93,8 @@ inline double mxfp4_rounds(double workgroups) { return (double)(long long)((work
 // The weight streamed past groups of 16 or 32 tokens: a unit of work is 4 / KS blocks of 16 channels with such a group, KS waves share the K of a block, and a
 // workgroup per CU takes its share of the units one behind the other.  A unit costs its waves' stages of 8 blocks of K, and 1.2 or 2.5 more where its sums are
 // joined; KS is what makes that least for a workgroup.  N x K with KS 1 / 2 / 4 for 16 and for 32 tokens:
-//   1024 x 1024  5.1 / 4.4 / 4.2   5.5 / 4.7 / 4.4    4096 x 4096   8.6 /  6.6 /  6.0    9.4 /  6.9 /  6.0    7168 x 2048  6.5 / 5.8 / 6.3    7.1 / 5.9 / 7.0
-//   6144 x 4096  8.6 / 6.8 / 7.7   9.5 / 7.1 / 8.5   14336 x 4096   9.7 / 10.5 / 12.1   10.7 / 11.4 / 13.7    2048 x 7168  11.6 / 8.0 / 6.5  12.7 / 8.7 / 6.9
+//   1024 x 1024  5.1 / 4.4 / 4.2   5.5 / 4.7 / 4.4    4096 x 4096   8.4 /  6.6 /  5.9    9.5 /  7.0 /  6.1    7168 x 2048  6.6 / 5.7 / 6.2    7.2 / 5.9 / 6.8
+//   6144 x 4096  8.6 / 6.9 / 7.9   9.7 / 7.2 / 8.6   14336 x 4096   9.2 / 10.2 / 11.9   10.4 / 11.6 / 13.8    2048 x 7168  11.4 / 8.1 / 6.6  13.9 / 9.5 / 7.3
 inline long long mxfp4_units(long long M, long long N, int KS) {
   const long long group = M <= 16 ? 16 : 32, blocks = (N + 15) / 16, at_once = 4 / KS;
   return (blocks + at_once - 1) / at_once * ((M + group - 1) / group);

@@ -1,8 +1,8 @@
 // A mixture-of-experts layer for a few tokens, on experts of microscaled 4-bit numbers:
 //   y[t] = sum_s w[t, s] (down_e h + down_bias_e),   h = act(gate_e x[t] + b) * (up_e x[t] + b),   e = experts[t, s]
 // Tokens that chose the same expert share one pass over its bytes, which is what bounds the layer: a plan (tokens by expert), gate and up, down, the
-// weighted sum, a kernel each, as each needs all of the one in front.  7168 x 2048, 8 of 256 experts: 1 token 6.4 + 26.9 + 14.4 + 4.0 us (4.5 TB/s of
-// weights while they stream, which is a ramp and a tail too at this length), 16 tokens 10.4 + 271 + 143 + 5.2 (5.7).
+// weighted sum, a kernel each, as each needs all of the one in front.  7168 x 2048, 8 of 256 experts: 1 token 6.2 + 26.1 + 13.7 + 3.9 us (gate and up
+// 3 of launch, 2.9 to the first stage, 18.2 at the memory's rate, 1.2 of results), 16 tokens 10.5 + 246 + 133 + 5.6 (6.3 TB/s).
 //
 // The activations keep their precision.  A lane takes a block of a weight row, 16 bytes, and the conversion to bf16 applies its scale: that is
 // exact, so the products are those of the stored numbers.  bf16 tokens go into the matrix pipe as they are, fp32 ones as sums of four bf16 planes; h,
@@ -221,7 +221,7 @@ __device__ __forceinline__ void planes_of(float v, uint16_t* out) {
 }
 
 // Workgroup 0 plans the pass; the others lay the tokens out as planes [T, planes, Kp] where they are not that already.  One workgroup, as every place depends on
-// all choices: 6.4 us with the routing of 1 token of 256 experts, 10.4 of 16 tokens (their choices are a chain in each wave), 5.2 behind the router's kernel.
+// all choices: 6.2 us with the routing of 1 token of 256 experts, 10.5 of 16 tokens (their choices are a chain in each wave), 5.2 behind the router's kernel.
 template <int NL>
 __global__ __launch_bounds__(1024) void plan_kernel(RouterArgs r, const int* __restrict__ given, const float* __restrict__ given_weights, int T,
                                                     Operand o, int size, Plan* __restrict__ plan) {
@@ -842,20 +842,20 @@ struct Cut {
     PH = planes_of_h(dtype);
     const int64_t slots = T * top;
     // Slots of a group: few columns cost less in every stage, a second group of an expert reads its bytes again.  The whole layer in us with 4 / 16 / 32:
-    //   4 tokens, 6 of 64 experts 39 / 48 / 55    16 tokens, 8 of 256 428 / 471 / 622    64 tokens, 4 of 32 143 / 94 / 123    64 tokens, 2 of 8 - / 97 / 96
-    //   96 tokens, 2 of 8 - / 113 / 98
+    //   4 tokens, 6 of 64 experts 40 / 48 / 55    16 tokens, 8 of 256 378 / 461 / 617    64 tokens, 4 of 32 159 / 94 / 123    64 tokens, 2 of 8 164 / 95 / 94
+    //   96 tokens, 2 of 8 208 / 112 / 97
     size = T <= 4 || slots <= E ? 4 : P == 4 || T <= 16 || slots <= 18 * E ? 16 : 32;
     groups = least(slots, least(E, slots) + slots / size);
     const int64_t up_stages = ((K + 31) / 32 + 7) / 8, down_stages = ((I + 31) / 32 + 7) / 8, Ip = (I + 31) / 32 * 32;
     up_tiles = (int)((Ip + 63) / 64);
     // Parts of K of gate and up, where a few narrow experts leave the chip to a few long units: a stage is 0.45 us, making sums visible to the workgroup that adds
-    // them up 0.15 for every workgroup.  1 token, 1 of 4 experts 14336 x 128 in 1 / 2 / 4 / 8 parts 51 / 37 / 29 / 30 us, 2 of 8 7168 x 256 34 / 29 / 28 / 32, but 4 of 16
-    // 1024 x 512 20 / 30 and 8 of 256 7168 x 2048 56 / 176.
+    // them up 0.15 for every workgroup.  1 token, 1 of 4 experts 14336 x 128 in 1 / 2 / 4 / 8 parts 52 / 37 / 29 / 27 us, 2 of 8 7168 x 256 34 / 29 / 28 / 32, but 4 of 16
+    // 1024 x 512 20 / 30 and 8 of 256 7168 x 2048 50 / 172.
     up_parts = 1;
     while (3 * up_stages > 2 * groups * up_tiles * up_parts * up_parts && up_stages / (2 * up_parts) >= 3) up_parts *= 2;
     down_tiles = (int)((N + 127) / 128);
-    // Runs of down: two workgroups per CU (64 tokens, 4 of 32 experts with 1 / 2 / 4 per CU 92 / 95 / 104, 16 tokens, 8 of 256 463 / 450 / 456); K in parts
-    // where there are too few groups for them (1 token, 2 of 8 experts 4096 x 14336 in 1 / 2 / 4 / 8 parts 77 / 62 / 56 / 54; 8 of 256 56 / 57 / 58).
+    // Runs of down: two workgroups per CU (64 tokens, 4 of 32 experts with 1 / 2 / 4 per CU 91 / 94 / 101, 16 tokens, 8 of 256 410 / 378 / 385); K in parts
+    // where there are too few groups for them (1 token, 2 of 8 experts 4096 x 14336 in 1 / 2 / 4 / 8 parts 73 / 59 / 53 / 53; 8 of 256 52 / 52 / 54 / 60).
     int64_t want = 512 / down_tiles;
     if (want < 1) want = 1;
     down_parts = 1;

@@ -401,7 +401,7 @@ __global__ __launch_bounds__(256) void order_scales_kernel(MxArgs g, int groups,
 // ---- few tokens ---------------------------------------------------------------------------------------------------
 // The weight streams past the tokens.  A wave has a block of 16 channels and a KS-th of K; stages of 256 codes go through its own part of LDS by
 // direct loads of whole lines, DEPTH - 1 stages ahead, without a break from one block to the next, and nothing but the joining of a
-// block's KS waves makes waves wait for one another.  16 tokens by 4096 x 14336 take 10.0 us (3.1 TB/s of weights; 3.4 are the launch and the first loads).
+// block's KS waves makes waves wait for one another.  16 tokens by 4096 x 14336 take 9.7 us (3.2 TB/s of weights; 3.4 are the launch and the first loads).
 // Loaded straight into the matrix pipe's layout, 16 neighbouring lanes are 16 rows and every KB passes the cache 64 times: 16.5 us.
 //   codes of the weight and of the tokens   16 rows x 128 bytes; 16-byte piece p of row r lies at p ^ (r / 2 % 8)
 //   scales   the word-aligned 64 bytes of a row that hold those of eight stages, or of seven where rows are off words
