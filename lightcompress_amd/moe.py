@@ -71,17 +71,20 @@ def route_tokens(router):
     return Routing(experts, weights)
 
 
-def _experts(t, width, step, most=MOST_DISTANCE):
-    """[E, rows, width] bytes -> (t or a contiguous copy, distance between experts, between rows), on multiples of `step` bytes."""
-    E, rows = t.shape[0], t.shape[1]
-    lde, ld = t.stride(0), t.stride(1)
-    if rows == 1:
-        ld = width
-    if E == 1:
-        lde = rows * ld
-    if t.stride(2) != 1 or not width <= ld <= most or ld % step or lde % step:
-        t = t.contiguous()
-        lde, ld = rows * width, width
+def _experts(t, step, most=MOST_DISTANCE):
+    """Bytes [E, rows, width] -> (t or a contiguous copy, distance between experts, between rows), on multiples of `step` bytes (as widths are)."""
+    E, rows, width = t.shape
+    lde, ld = rows * width, width
+    if not t.is_contiguous():
+        e, r, w = t.stride()
+        if rows == 1:
+            r = width
+        if E == 1:
+            e = rows * r
+        if w != 1 or not width <= r <= most or r % step or e % step:
+            t = t.contiguous()
+        else:
+            lde, ld = e, r
     if t.data_ptr() % step:
         t = t.clone(memory_format=torch.contiguous_format)
         lde, ld = rows * width, width
@@ -153,10 +156,10 @@ def mxfp4_moe(x, router, gate_up, down, *, gate_up_bias=None, down_bias=None, ac
         else:
             logits, _, ldl = _rows(on[0], E)
             correction = _whole(on[1])
-        gw, g_lde, g_ld = _experts(gw, gw.shape[2], 16)
-        gs, g_ldse, g_lds = _experts(gs, gs.shape[2], 1, (1 << 30) // (I + 64))
-        dw, d_lde, d_ld = _experts(dw, dw.shape[2], 16)
-        ds, d_ldse, d_lds = _experts(ds, ds.shape[2], 1)
+        gw, g_lde, g_ld = _experts(gw, 16)
+        gs, g_ldse, g_lds = _experts(gs, 1, (1 << 30) // (I + 64))
+        dw, d_lde, d_ld = _experts(dw, 16)
+        ds, d_ldse, d_lds = _experts(ds, 1)
         gate_up_bias, down_bias = _whole(gate_up_bias), _whole(down_bias)
         ws = _workspace(rows, 'lcq_mxfp4_moe_workspace_bytes', T, top, E, K, I, N, code)
         L.check(L.lib().lcq_mxfp4_moe(rows.data_ptr(), code, T, K, ld, _at(logits), logits_code, ldl, flags, _at(correction), scale, _at(experts),
