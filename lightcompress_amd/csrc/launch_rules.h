@@ -108,24 +108,30 @@ inline int mxfp4_waves(long long M, long long N, long long B) {
     if (mxfp4_stages(M, N, B, KS) < mxfp4_stages(M, N, B, best)) best = KS;
   return best;
 }
-// Or tiles of 256 x 256 or 128 x 128, the latter with K cut into parts of at least two periods of 16 blocks.  What is estimated to be fastest, measured as
-// streamed / 128 / 128 in 2 parts / in 4 / in 8 (and 256):
-//   4096 x 4096    64 tokens  7.1 / 12.3 / 12.3 / 12.6 / 15.2    128   9.8 / 12.7 / 12.5 / 14.6 / 16.4    211  16.1 / 12.8 / 14.0 / 17.3 / 22.4    2048  29.8 (32.7)
-//   4096 x 14336   64 tokens   16 /   39 /   25 /   19 /   18    128    23 /   43 /   28 /   22 /   20    211    43 /   41 /   29 /   23 /   31    1024  45.2 (83)
-//   14336 x 4096   33 tokens   16 / 14.4 / 14.9 /   20 /   30    211    46 /   17 /   31 /   45 /   68   1024  62.5 with 128 (41.9)
-//   1001 x 2047   128 tokens  5.3 /  9.4 / 10.2 / 10.6 / 13.3    512   7.1 /  9.5 / 11.3 / 12.9 / 19
-struct Mxfp4Cut { bool stream; int tile, parts; };  // tile 0: 256 x 256, 1: 128 x 128
+// Or tiles: of 256 x 256, one to a CU, of 128 x 128, one to a CU, or of 64 x 64, two to a CU, the latter two also with K cut into parts of at least two periods of
+// 16 blocks, whose sums are joined.  What is estimated to be fastest, measured as streamed / 64 in 1 part / in 2 / in 4 / 128 in 1 part / in 4 (and 256):
+//   4096 x 4096    64 tokens  7.2 / 8.2 /  9.4 / 10.6 / 12.3 / 12.6    128   9.9 /  8.3 /  9.9 / 13.9 / 12.6 / 14.6    211  16 /  8.7 / 13 / 18 / 12.8 / 17
+//                 512 tokens   29 / 12.7 / 21  /  29  / 13.3 / 26     1024  52 / 22.7 / 36 / 50 / 17.4 / 42            2048 tokens 29.8 with 128 (32.7)
+//   4096 x 14336   64 tokens   16 /  26 /  19  / 14.9 /  39  /  19     128   22 /  26  / 19.3 / 22 / 44 / 22             211  48 /  23 / 25 / 29 / 41 / 22
+//   14336 x 4096   64 tokens   16 / 10.2 / 17  /  21  / 14.8 /  23     128   29 / 15.2 / 26 / 35 / 15.6 / 28             211  47 /  23 / 37 / 52 / 17.8 / 45
+//   7168 x 2048    64 tokens  7.3 /  6.0 / 9.3 / 12.3 /  8.7           211   19 /  8.0 / 18 / 23 /  9.4                   512  31 /  14 / 26 / 38 / 11.2
+//   1001 x 2047   128 tokens  5.4 /  5.6 / 7.1 /  7.8 /  9.4           512  7.0 /  5.9 / 9.7 / 13 /  9.6                  1333  15 / 8.1 / 18 / 24 / 10.4
+struct Mxfp4Cut { bool stream; int tile, parts; };  // tile 0: 256 x 256, 1: 128 x 128, 2: 64 x 64
 inline Mxfp4Cut mxfp4_cut(long long M, long long N, long long B) {
   if (M <= 32) return {true, 0, 1};
-  const double stages = (double)((B + 7) / 8), outputs = (double)M * (double)N;
-  const double large = (double)((M + 255) / 256) * (double)((N + 255) / 256), small = (double)((M + 127) / 128) * (double)((N + 127) / 128);
+  const double stages = (double)((B + 7) / 8), outputs = (double)M * (double)N, weights = (double)N * (double)B * 17 / 5.5e6;
+  const auto tiles = [&](long long side) { return (double)((M + side - 1) / side) * (double)((N + side - 1) / side); };
+  const auto join = [&](int parts) { return parts > 1 ? 3 + parts * outputs / 5e5 : 0.0; };
+  const auto most = [](double a, double b) { return a > b ? a : b; };
   const double scales = B % 16 ? 2.5 : 0;           // put in order in front of the tiles (of 256 x 256 always)
-  double least = 9.5 + mxfp4_rounds(large) * (3 + 1.9 * stages);
+  double least = 9.5 + mxfp4_rounds(tiles(256)) * (3 + 1.9 * stages);
   Mxfp4Cut best = {false, 0, 1};
   for (int parts = 1; parts <= 8 && (parts == 1 || (B + 15) / 16 >= 2 * parts); parts *= 2) {
-    const double workgroups = small * parts, busy = workgroups < MXFP4_CUS ? workgroups : MXFP4_CUS, stage = busy * 0.0032 > 0.55 ? busy * 0.0032 : 0.55;
-    const double us = 4.4 + scales + mxfp4_rounds(workgroups) * (1 + stage * stages / parts) + (parts > 1 ? 3 + parts * outputs / 5e5 : 0);
-    if (us < least) least = us, best = {false, 1, parts};
+    const double w128 = tiles(128) * parts, w64 = tiles(64) * parts;
+    const double us128 = 4.4 + scales + mxfp4_rounds(w128) * (1 + most(0.55, 0.0032 * (w128 < MXFP4_CUS ? w128 : MXFP4_CUS)) * stages / parts) + join(parts);
+    const double us64 = 3.2 + scales + most(weights, mxfp4_rounds(w64 / 2) * most(0.30, 0.0013 * (w64 < 2 * MXFP4_CUS ? w64 : 2 * MXFP4_CUS)) * stages / parts) + join(parts);
+    if (us128 < least) least = us128, best = {false, 1, parts};
+    if (us64 < least) least = us64, best = {false, 2, parts};
   }
   const long long teams = (M + 31) / 32;
   if (teams <= 64 && 3.4 + 0.39 * mxfp4_stages(M, N, B, mxfp4_waves(M, N, B)) < least) best = {true, 0, 1};

@@ -40,7 +40,7 @@ template <class T> __device__ __forceinline__ T from_lds(uint32_t at) { return *
 __device__ __forceinline__ i32x8 wide(i32x4 v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
 
 // ---- tiles --------------------------------------------------------------------------------------------------------
-// A workgroup of four waves (2 x 2) owns 64 FM tokens x 64 FN channels, a wave FM x FN accumulators of 32 x 32.
+// A workgroup of four waves (2 x 2) owns 64 FM tokens x 64 FN channels, a wave FM x FN accumulators of 32 x 32.  (Two of 64 x 64 share a CU.)
 //  * codes stream through LDS stages of SLAB bytes per row by direct loads; rows past the end of a matrix and bytes past a row's blocks
 //    lie outside the buffer that the loads are told and read as zero;
 //  * piece p of 16 bytes (a block) of row r lies at p ^ (r / 4 % 4) or p ^ (r / 2 % 8), so that 16 lanes of an operand read touch all 64
@@ -52,7 +52,8 @@ __device__ __forceinline__ i32x8 wide(i32x4 v) { return __builtin_shufflevector(
 // Tiles of 256 x 256 are bound by the chip's power: 8192 x 14336 x 4096 takes 251 us (3.8 PFLOP/s) with the products at 1.55 GHz, 192 on zeros at 2.35.  A
 // round of tiles is 3.4 us of first loads, 25 of products (38 900 clocks, the pipe alone 32 800), 4.5 of outputs.  With nothing loaded behind the first stages the products
 // run at 1.68 GHz, without reads of LDS either at 1.92; loading the next tile's first stages before the outputs leave, or whole lines in two stages of 128
-// bytes, took as long.  Tiles of 128 x 128 are bound by the loads on their way (a round of 224 with K = 4096: 17 us, 1.9 TB/s of weights).
+// bytes, took as long.  The others are bound by the loads on their way (a round of 224 tiles of 128 x 128 with K = 4096 17 us, 1.9 TB/s of weights, of 64 x 64
+// 10 us, 3 TB/s).
 constexpr int ROW_SUM = 3;                          // an output type: the sums of a part of K as they are
 constexpr int PERIOD = 256;                         // bytes of a row between scale loads
 
@@ -180,7 +181,7 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MxArgs g, int tiles_m, int
   // The reads run a step ahead of the products, so in front of a stage's last step the rest of it is in registers.  There is its
   // barrier: its place is free, and the stage STAGES ahead is loaded there during the next STEPS steps.
   constexpr int SWITCH = STEPS - 1;
-  static_assert(SWITCH >= 1 && STEPS % 2 == 0 && PER <= STAGES && 2 * PER - 1 > STAGES - 2, "stages and periods");
+  static_assert(SWITCH >= 1 && STEPS % 2 == 0 && (PRODUCTS >= LOADS / STEPS) && PER <= STAGES && 2 * PER - 1 > STAGES - 2, "stages and periods");
   const auto wait = [&](auto in_flight_) {          // for all loads but the youngest, and for the operands; then for the other waves
     constexpr int in_flight = decltype(in_flight_)::value;
     static_assert(in_flight < 64, "loads in flight");
@@ -303,32 +304,32 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MxArgs g, int tiles_m, int
       }
     }
     asm volatile("" ::: "memory");                  // (LDS serves a wave in order)
-    constexpr int AT_ONCE = 64 / CHUNKS, TIMES = STEP * 32 / AT_ONCE;        // tokens of a store, stores
+    constexpr int AT_ONCE = 64 / CHUNKS, TIMES = STEP * 32 / AT_ONCE, SOME = TIMES < 8 ? TIMES : 8;          // tokens of a store, stores, those on their way together
     const int t0 = lane / CHUNKS, ch = lane % CHUNKS, n = wc * FN * 32 + ch * CH;
     char* const to = (char*)g.y + ((m0 + wr * FM * 32 + i0 * 32) * g.N + n0 + (BF == ROW_SUM ? part * g.M * g.N : 0)) * E;
     if (rows_a == T::TM && rows_w == T::TN) {       // (uniform, as most tiles of a large product are: no comparison, no address but a scalar one)
       const uint32_t of = (uint32_t)(t0 * g.N + n) * E;                      // (7 N outputs of two bytes or 3 N of four, and a tile's: 32 bits)
       #pragma unroll
-      for (int o0 = 0; o0 < TIMES; o0 += 8) {
-        u32x4 v[8];
+      for (int o0 = 0; o0 < TIMES; o0 += SOME) {
+        u32x4 v[SOME];
         #pragma unroll
-        for (int o = 0; o < 8; ++o) v[o] = *(const u32x4*)(mine + ((o0 + o) * AT_ONCE + t0) * ROW + turned(ch, ((o0 + o) * AT_ONCE + t0) % 32) * 16);
+        for (int o = 0; o < SOME; ++o) v[o] = *(const u32x4*)(mine + ((o0 + o) * AT_ONCE + t0) * ROW + turned(ch, ((o0 + o) * AT_ONCE + t0) % 32) * 16);
         if (past) {
           #pragma unroll
-          for (int o = 0; o < 8; ++o) mx_store_past(to + (int64_t)(o0 + o) * AT_ONCE * g.N * E + of, v[o]);
+          for (int o = 0; o < SOME; ++o) mx_store_past(to + (int64_t)(o0 + o) * AT_ONCE * g.N * E + of, v[o]);
         } else {
           #pragma unroll
-          for (int o = 0; o < 8; ++o) *(u32x4_anywhere*)(to + (int64_t)(o0 + o) * AT_ONCE * g.N * E + of) = v[o];
+          for (int o = 0; o < SOME; ++o) *(u32x4_anywhere*)(to + (int64_t)(o0 + o) * AT_ONCE * g.N * E + of) = v[o];
         }
       }
     } else {
       #pragma unroll 1
-      for (int o0 = 0; o0 < TIMES; o0 += 8) {
-        u32x4 v[8];
+      for (int o0 = 0; o0 < TIMES; o0 += SOME) {
+        u32x4 v[SOME];
         #pragma unroll
-        for (int o = 0; o < 8; ++o) v[o] = *(const u32x4*)(mine + ((o0 + o) * AT_ONCE + t0) * ROW + turned(ch, ((o0 + o) * AT_ONCE + t0) % 32) * 16);
+        for (int o = 0; o < SOME; ++o) v[o] = *(const u32x4*)(mine + ((o0 + o) * AT_ONCE + t0) * ROW + turned(ch, ((o0 + o) * AT_ONCE + t0) % 32) * 16);
         #pragma unroll
-        for (int o = 0; o < 8; ++o) {
+        for (int o = 0; o < SOME; ++o) {
           const int tt = (o0 + o) * AT_ONCE + t0, m = wr * FM * 32 + i0 * 32 + tt;
           if (m >= rows_a || n >= rows_w) continue;
           char* const cell = to + ((int64_t)tt * g.N + n) * E;
@@ -673,6 +674,7 @@ int64_t on16(int64_t blocks) { return (blocks + 15) / 16 * 16; }
 
 typedef Tile<4, 4, 64, 4> Tile256;
 typedef Tile<2, 2, 128, 4> Tile128;
+typedef Tile<1, 1, 128, 4> Tile64;
 
 template <class T, int BF>
 void launch_tiles(const MxArgs& g, int parts, hipStream_t st) {
@@ -714,10 +716,12 @@ int launch(const MxArgs& g, float* sums, hipStream_t st) {
   if (c.parts > 1) {
     MxArgs p = g;
     p.y = sums;
-    launch_tiles<Tile128, ROW_SUM>(p, c.parts, st);
+    if (c.tile == 2) launch_tiles<Tile64, ROW_SUM>(p, c.parts, st);
+    else launch_tiles<Tile128, ROW_SUM>(p, c.parts, st);
     launch_join<BF>(g, sums, c.parts, st);
   }
   else if (c.tile == 0) launch_tiles<Tile256, BF>(g, 1, st);
+  else if (c.tile == 2) launch_tiles<Tile64, BF>(g, 1, st);
   else launch_tiles<Tile128, BF>(g, 1, st);
   return LCQ_OK;
 }

@@ -183,7 +183,8 @@ def test_product(dev, M, N, K, bias, dtype):
 
 
 CUTS = [(5, 14336, 520), (9, 6145, 4100), (13, 300017, 96), (20, 14300, 1100), (25, 7170, 2050), (45, 14335, 300), (90, 2500, 16000), (61, 40001, 200),
-        (211, 4000, 14300), (300, 3000, 10000), (1000, 14300, 4100), (7000, 14501, 70)]          # (the last one's outputs go past the caches)
+        (211, 4000, 14300), (300, 3000, 10000), (1000, 14300, 4100),
+        (4900, 66, 14470), (66, 12450, 11050), (2790, 66, 21800), (6730, 17, 6420), (2070, 16, 3811), (33, 17, 487), (67, 10694, 140), (7000, 14501, 1100)]          # (the last one's outputs go past the caches)
 
 
 @pytest.mark.parametrize('dtype', [F32, BF])
