@@ -552,8 +552,8 @@ int lcq_mxfp4_dequant(const uint8_t* codes, int64_t ldc, const uint8_t* scales, 
 /* y[m, n] = sum_k a[m, k] w[n, k] + bias[n] of such rows: products exact, sums in fp32, rounded once.
  *  a, w    codes [M, 16 B] and [N, 16 B], rows lda / ldw bytes apart, all on 16 bytes;  sa, sw scales, rows ldsa / ldsw apart.  Distances up to 2^22
  *  bias    [N] of bias_dtype or NULL;  y [M, N] of `dtype`;  K <= 65536, M <= 2^28, N <= 2^28 - 16
- *  workspace of lcq_mxfp4_matmul_workspace_bytes(M, N, K) (0: none), 16-byte aligned. */
-int64_t lcq_mxfp4_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
+ *  workspace of lcq_mxfp4_matmul_workspace_bytes(M, N, K, aligned) (0: none), 16-byte aligned.  aligned: are sa, sw, ldsa and ldsw multiples of 16? */
+int64_t lcq_mxfp4_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, int aligned);
 int lcq_mxfp4_matmul(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t ldsa, const uint8_t* w, int64_t ldw, const uint8_t* sw,
                      int64_t ldsw, const void* bias, int bias_dtype, int64_t M, int64_t N, int64_t K, void* y, int dtype, void* workspace,
                      void* stream);

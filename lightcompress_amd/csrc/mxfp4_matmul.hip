@@ -745,17 +745,19 @@ int check(const uint8_t* w, int64_t ldw, const uint8_t* sw, int64_t ldsw, const 
 // 1001 x 2047 3 tokens 6.7 / 6.9, 4 tokens 7.6 / 6.9).
 bool fused(int64_t M, int64_t K) { return M <= 16 && M * K <= (K % 8 ? 8192 : 16384); }
 
-bool on_pieces(const void* p, int64_t ld, int64_t B) { return (uintptr_t)p % 16 == 0 && ld % 16 == 0 && B % 16 == 0; }
+// Are scales put in order in front of the tiles?
+bool orders(const Mxfp4Cut& c, bool aligned, int64_t B) { return c.tile == 0 || !aligned || B % 16; }
 
 }  // namespace
 
 extern "C" {
 
-int64_t lcq_mxfp4_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+int64_t lcq_mxfp4_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, int aligned) {
   if (M <= 0 || N <= 0 || K <= 0 || K > 65536) return 0;
   const int64_t B = (K + 31) / 32;
   const Mxfp4Cut c = mxfp4_cut(M, N, B);
-  return c.stream ? 0 : (c.parts > 1 ? on256(4 * M * N * c.parts) : 0) + (M + N) * on16(B);
+  if (c.stream) return 0;
+  return (c.parts > 1 ? on256(4 * M * N * c.parts) : 0) + (orders(c, aligned, B) ? (M + N) * on16(B) : 0);
 }
 
 int lcq_mxfp4_matmul(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t ldsa, const uint8_t* w, int64_t ldw, const uint8_t* sw, int64_t ldsw,
@@ -771,13 +773,13 @@ int lcq_mxfp4_matmul(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t l
   MxArgs g = {a, sa, w, sw, bias, y, M, N, lda, ldw, ldsa, ldsw, 0, 0, (int)B, bias_dtype};
   const Mxfp4Cut c = mxfp4_cut(M, N, B);
   if (!c.stream) {
-    const bool orders = c.tile == 0 || !on_pieces(sa, ldsa, B) || !on_pieces(sw, ldsw, B);
-    if (orders || c.parts > 1) {
+    const bool ordered = orders(c, ((uintptr_t)sa | (uintptr_t)sw | (uintptr_t)ldsa | (uintptr_t)ldsw) % 16 == 0, B);
+    if (ordered || c.parts > 1) {
       if (!workspace) return LCQ_EWORKSPACE;
       if ((uintptr_t)workspace % 16) return LCQ_EALIGN;
     }
     g.nextsa = g.nextsw = 16;
-    if (orders) {
+    if (ordered) {
       const int groups = (int)((B + 15) / 16);
       uint8_t* const to = (uint8_t*)workspace + (c.parts > 1 ? on256(4 * M * N * c.parts) : 0);
       order_scales_kernel<<<dim3((unsigned)(((M + N) * groups + 255) / 256)), dim3(256), 0, st>>>(g, groups, to);
@@ -794,7 +796,7 @@ int lcq_mxfp4_matmul(const uint8_t* a, int64_t lda, const uint8_t* sa, int64_t l
 int64_t lcq_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0 || K > 65536 || fused(M, K)) return 0;
   const int64_t B = (K + 31) / 32;
-  return on256(M * B * 16) + on256(M * on16(B)) + lcq_mxfp4_matmul_workspace_bytes(M, N, K);
+  return on256(M * B * 16) + on256(M * on16(B)) + lcq_mxfp4_matmul_workspace_bytes(M, N, K, 0);
 }
 
 int lcq_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w, int64_t ldw, const uint8_t* sw, int64_t ldsw, const void* bias,

@@ -27,33 +27,41 @@ class Mxfp4(NamedTuple):
     cols: Optional[int] = None
 
 
-_BYTES = (torch.uint8, getattr(torch, 'float4_e2m1fn_x2', None), getattr(torch, 'float8_e8m0fnu', None))
+_U8 = torch.uint8
+_BYTES = (getattr(torch, 'float4_e2m1fn_x2', None), getattr(torch, 'float8_e8m0fnu', None))
 
 
 def _plain(t, name):
     """t as bytes."""
-    if t.dtype is torch.uint8:
+    if t.dtype is _U8:
         return t
     if t.dtype not in _BYTES:
         raise L.LcqError(f'{name} are bytes (torch.uint8), got {t.dtype}')
-    return t.view(torch.uint8)
+    return t.view(_U8)
 
 
 def _parts(q, name):
     """-> codes and scales as bytes, the number of columns."""
-    codes, scales, cols = _plain(q.codes, f'{name} codes'), _plain(q.scales, f'{name} scales'), q.cols
-    shape = scales.shape
-    if not shape or codes.dim() != len(shape) or codes.shape[:-1] != shape[:-1] or codes.shape[-1] != 16 * shape[-1] or not shape[-1]:
-        raise ValueError(f'{name}: codes {tuple(codes.shape)} and scales {tuple(shape)} are not blocks of 16 bytes and one')
+    codes, scales, cols = q.codes, q.scales, q.cols
+    if codes.dtype is not _U8 or scales.dtype is not _U8:
+        codes, scales = _plain(codes, f'{name} codes'), _plain(scales, f'{name} scales')
+    shape, rows = scales.shape, codes.shape
+    dims = len(shape)
+    B = shape[-1] if dims else 0
+    # (slices of a torch.Size cost half a microsecond each)
+    if not B or len(rows) != dims or rows[-1] != 16 * B or (rows[0] != shape[0] if dims == 2 else rows[:-1] != shape[:-1]):
+        raise ValueError(f'{name}: codes {tuple(rows)} and scales {tuple(shape)} are not blocks of 16 bytes and one')
     if cols is None:
-        cols = BLOCK * shape[-1]
-    elif not BLOCK * (shape[-1] - 1) < cols <= BLOCK * shape[-1]:
-        raise ValueError(f'{name}: {cols} columns in {shape[-1]} blocks of {BLOCK}')
+        cols = BLOCK * B
+    elif not BLOCK * (B - 1) < cols <= BLOCK * B:
+        raise ValueError(f'{name}: {cols} columns in {B} blocks of {BLOCK}')
     return codes, scales, cols
 
 
 def _byte_rows(t, width, step=1):
     """-> (t or a contiguous copy that starts on a multiple of `step` bytes, rows of `width`, distance between rows, such a multiple)."""
+    if t.is_contiguous():
+        return t if t.data_ptr() % step == 0 else t.clone(), t.numel() // width, width
     t, rows, ld = _rows(t, width)
     if rows == 1:
         ld = width
@@ -129,7 +137,8 @@ def mxfp4_matmul(tokens, weight, bias=None, out_dtype=torch.bfloat16):
         w, _, ldw = _byte_rows(w, 16 * B, 16)
         sw, _, ldsw = _byte_rows(sw, B)
         bias = _whole(bias)
-        ws = _workspace(a, 'lcq_mxfp4_matmul_workspace_bytes', M, N, K)
+        aligned = not (sa.data_ptr() | ldsa | sw.data_ptr() | ldsw) % 16
+        ws = _workspace(a, 'lcq_mxfp4_matmul_workspace_bytes', M, N, K, aligned)
         L.check(L.lib().lcq_mxfp4_matmul(a.data_ptr(), lda, sa.data_ptr(), ldsa, w.data_ptr(), ldw, sw.data_ptr(), ldsw, _at(bias),
                                          0 if bias is None else _code(bias.dtype), M, N, K, y.data_ptr(), code, _at(ws), L.stream()),
                 'lcq_mxfp4_matmul')

@@ -65,10 +65,11 @@ def test_the_workspace_follows_the_rules(cut):
         streamed, tile, parts = cut(M, N, K)
         scales = -(-blocks(K) // 16) * 16 * (M + N)
         sums = -(-4 * M * N * parts // 256) * 256 if parts > 1 else 0
-        assert need(M, N, K) == (0 if streamed else sums + scales)
+        assert need(M, N, K, 0) == (0 if streamed else sums + scales)
+        assert need(M, N, K, 1) == (0 if streamed else sums + (scales if tile == 0 or blocks(K) % 16 else 0))
         codes = M <= 16 and M * K <= (8192 if K % 8 else 16384)
-        assert linear(M, N, K) == 0 if codes else linear(M, N, K) >= need(M, N, K) + 16 * M * blocks(K) + M * blocks(K)
-    assert need(0, 1, 1) == need(1, 0, 1) == need(1, 1, 0) == need(1, 1, 65537) == linear(1, 1, 65537) == 0
+        assert linear(M, N, K) == 0 if codes else linear(M, N, K) >= need(M, N, K, 0) + 16 * M * blocks(K) + M * blocks(K)
+    assert need(0, 1, 1, 0) == need(1, 0, 1, 0) == need(1, 1, 0, 0) == need(1, 1, 65537, 0) == linear(1, 1, 65537) == 0
 
 
 def test_measured_choices(rules, cut):
