@@ -230,7 +230,7 @@ def test_a_token_that_is_not_finite_spoils_itself_alone(dev, bad):
         assert not bool(torch.isfinite(y[2]).any()) and bool(torch.isfinite(y[[0, 1, 3, 4, 5]]).all())
 
 
-@pytest.mark.parametrize('dtype', [BF, F32])
+@pytest.mark.parametrize('dtype', [BF, HF, F32])
 def test_operands_apart(dev, dtype):
     g = gpu_gen(9)
     E, K, I, N, T = 4, 96, 64, 80, 6
@@ -247,6 +247,20 @@ def test_operands_apart(dev, dtype):
     assert torch.equal(flat, want.view(6, N))
     x3 = x2[:, 8:8 + K]                            # rows on 16 bytes
     assert torch.equal(mxfp4_moe(x3, Router(logits.view(6, 7)[:, 1:5], 2), gu, dn), mxfp4_moe(x3.contiguous(), Router(logits.view(6, 7)[:, 1:5].contiguous(), 2), whole(gu), whole(dn)))
+
+
+@pytest.mark.parametrize('dtype', [BF, HF, F32])
+def test_one_row_for_all(dev, dtype):
+    """Expanded operands: one token, one row of logits, one expert's weights under every name."""
+    g = gpu_gen(14)
+    E, K, I, N, T = 3, 96, 64, 48, 5
+    gate_up, down = experts_of(1, 2 * I, K, g, dev), experts_of(1, N, I, g, dev)
+    wide = lambda q: Mxfp4(q.codes.expand(E, -1, -1), q.scales.expand(E, -1, -1))  # noqa: E731
+    whole = lambda q: Mxfp4(q.codes.contiguous(), q.scales.contiguous())           # noqa: E731
+    x, logits = torch.randn(1, K, generator=g, device=dev).to(dtype).expand(T, K), torch.randn(1, E, generator=g, device=dev).expand(T, E)
+    got = mxfp4_moe(x, Router(logits, 2), wide(gate_up), wide(down))
+    assert torch.equal(got, mxfp4_moe(x.contiguous(), Router(logits.contiguous(), 2), whole(wide(gate_up)), whole(wide(down))))
+    assert torch.equal(got, got[:1].expand(T, N))
 
 
 def test_experts_behind_2_gigabytes(dev):

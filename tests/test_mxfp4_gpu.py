@@ -293,6 +293,67 @@ def test_another_stream_and_a_graph(dev):
         assert torch.equal(out, want)
 
 
+def test_every_kind_of_cut_in_two_graphs(dev):
+    """Streamed, tiles of each size, parts and their join: two graphs replayed in turn, with eager calls of the same operands between."""
+    g = gpu_gen(4)
+    sizes = [(9, 300, 1000), (40, 520, 2048), (70, 3000, 2000), (300, 264, 9190), (211, 14336, 1056), (1000, 14300, 600)]
+    operands = [(random_mx(M, K, g, dev, 110, 122), random_mx(N, K, g, dev, 110, 122), torch.randn(N, generator=g, device=dev)) for M, N, K in sizes]
+    run = lambda: [mxfp4_matmul(a, w, b) for a, w, b in operands]  # noqa: E731
+    run()
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            outs.append(run())
+    for i in range(3):
+        for a, _, _ in operands:
+            a.codes.copy_(a.codes.roll(1, 0))
+        want = run()
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        for out in outs:
+            assert all(torch.equal(x, y) for x, y in zip(out, want))
+
+
+@pytest.mark.parametrize('M', [1, 40, 100, 300])
+def test_weights_behind_2_gigabytes(dev, M):
+    g = gpu_gen(5)
+    N, K = 66000, 65536
+    a, w = random_mx(M, K, g, dev), random_mx(N, K, g, dev, 110, 122)
+    assert w.codes.numel() > 2 ** 31
+    got = mxfp4_matmul(a, w, out_dtype=F32)
+    for at in (slice(0, 70), slice(N - 70, N)):
+        va, vw = values(a), values(Mxfp4(w.codes[at], w.scales[at], K))
+        err = (got[:, at].to(f64) - va @ vw.t()).abs()
+        assert bool((err <= (K / 64 + 16) * 2.0 ** -23 * (va.abs() @ vw.abs().t()) + TINY[F32]).all())
+
+
+def test_outputs_behind_2_31(dev):
+    g = gpu_gen(6)
+    M, N, K = 300, 8000000, 32
+    a, w = random_mx(M, K, g, dev), random_mx(N, K, g, dev, 110, 122)
+    got = mxfp4_matmul(a, w)
+    assert got.numel() > 2 ** 31
+    for at in (slice(0, 999), slice(N - 999, N)):
+        assert torch.equal(got[:, at], mxfp4_matmul(a, Mxfp4(w.codes[at].contiguous(), w.scales[at].contiguous(), K)))
+
+
+@pytest.mark.parametrize('dtype', [BF, HF, F32])
+def test_one_row_for_all(dev, dtype):
+    """Expanded operands: rows that lie on top of each other."""
+    g = gpu_gen(7)
+    w = random_mx(50, 160, g, dev, 110, 122)
+    for T in (3, 40, 200):
+        x = torch.randn(1, 160, generator=g, device=dev).to(dtype).expand(T, 160)
+        q = quantize_mxfp4(x)
+        assert torch.equal(q.codes, quantize_mxfp4(x[:1]).codes.expand(T, -1)) and torch.equal(mxfp4_linear(x, w), mxfp4_linear(x.contiguous(), w))
+        one = quantize_mxfp4(x[:1])
+        wide = Mxfp4(one.codes.expand(T, -1), one.scales.expand(T, -1), 160)
+        assert torch.equal(mxfp4_matmul(wide, w), mxfp4_matmul(q, w)) and torch.equal(dequantize_mxfp4(wide), dequantize_mxfp4(q))
+        rows = Mxfp4(w.codes[:1].expand(50, -1), w.scales[:1].expand(50, -1), 160)
+        assert torch.equal(mxfp4_matmul(q, rows), mxfp4_matmul(q, Mxfp4(rows.codes.contiguous(), rows.scales.contiguous(), 160)))
+
+
 # -- refusals -------------------------------------------------------------------------------------------------------
 def test_refusals(dev):
     g = gpu_gen(3)
