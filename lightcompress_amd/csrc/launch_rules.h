@@ -130,8 +130,8 @@ inline Mxfp4Cut mxfp4_cut(long long M, long long N, long long B) {
     const double w128 = tiles(128) * parts, w64 = tiles(64) * parts;
     const double us128 = 4.4 + scales + mxfp4_rounds(w128) * (1 + most(0.55, 0.0032 * (w128 < MXFP4_CUS ? w128 : MXFP4_CUS)) * stages / parts) + join(parts);
     const double us64 = 3.2 + scales + most(weights, mxfp4_rounds(w64 / 2) * most(0.30, 0.0013 * (w64 < 2 * MXFP4_CUS ? w64 : 2 * MXFP4_CUS)) * stages / parts) + join(parts);
-    if (us128 < least) least = us128, best = {false, 1, parts};
-    if (us64 < least) least = us64, best = {false, 2, parts};
+    if (us128 < least && w128 <= (1 << 24) - 8) least = us128, best = {false, 1, parts};
+    if (us64 < least && w64 <= (1 << 24) - 8) least = us64, best = {false, 2, parts};        // (a launch has fewer than 2^32 lanes)
   }
   const long long teams = (M + 31) / 32;
   if (teams <= 64 && 3.4 + 0.39 * mxfp4_stages(M, N, B, mxfp4_waves(M, N, B)) < least) best = {true, 0, 1};

@@ -15,7 +15,7 @@ extern "C" int cut(long long M, long long N, long long B) { const lcq::Mxfp4Cut 
 extern "C" int waves(long long M, long long N, long long B) { return lcq::mxfp4_waves(M, N, B); }
 extern "C" long long units(long long M, long long N, long long KS) { return lcq::mxfp4_units(M, N, (int)KS); }
 '''
-WIDTHS = (1, 15, 16, 100, 1000, 4096, 6144, 14336, 140000, 1 << 24)
+WIDTHS = (1, 15, 16, 100, 200, 300, 1000, 4096, 6144, 14336, 140000, 1 << 24)
 DEPTHS = (1, 32, 33, 255, 256, 257, 2047, 4096, 14336, 65536)
 
 
@@ -55,7 +55,10 @@ def test_cuts_are_whole(rules, cut):
             assert KS in (1, 2, 4) and M <= 2048
             group = 16 if M <= 16 else 32
             assert rules.units(M, N, KS) == -(-(-(-N // 16)) // (4 // KS)) * -(-M // group) < 2 ** 31
-        elif parts > 1:                            # parts of 128 x 128 and 64 x 64 tiles only, at least two periods of 16 blocks each
+        if not streamed and -(-M // 128) * -(-N // 128) <= (1 << 24) - 8:    # (what the product takes) fewer than 2^32 lanes
+            side = (256, 128, 64)[tile]
+            assert -(-M // side) * -(-N // side) * parts <= (1 << 24) - 8, (M, N, K)
+        if not streamed and parts > 1:             # parts of 128 x 128 and 64 x 64 tiles only, at least two periods of 16 blocks each
             assert tile in (1, 2) and parts <= 8 and -(-blocks(K) // 16) >= 2 * parts
 
 
