@@ -5,10 +5,10 @@
 // 3 of launch, 2.9 to the first stage, 18.2 at the memory's rate, 1.2 of results), 16 tokens 10.5 + 246 + 133 + 5.6 (6.3 TB/s).
 //
 // The activations keep their precision.  A lane takes a block of a weight row, 16 bytes, and the conversion to bf16 applies its scale: that is
-// exact, so the products are those of the stored numbers.  bf16 tokens go into the matrix pipe as they are, fp32 ones as sums of four bf16 planes; h,
-// which stays within the layer, as two planes (2^-17), or four for fp32 tokens.  fp16 tokens go as they are too, with the weights' blocks as fp16, which is
-// exact for scales of 2^-23 .. 2^13; stages with others take the tokens apart into two bf16 numbers (gate and up of 50 tokens, 2 of 8 experts 4090 x 14336: 129 us, as two
-// planes throughout 161; of 96 tokens 4096 x 4096 45 and 66).
+// exact, so the products are those of the stored numbers.  bf16 tokens go into the matrix pipe as they are, fp32 ones as sums of three bf16 planes, and so
+// does h, which stays within the layer: 24 bits are three times eight, so nothing of an fp32 number is lost (above 2^-110).  fp16 tokens go as they are too, with the
+// weights' blocks as fp16, which is exact for scales of 2^-23 .. 2^13; stages with others take the tokens apart into two bf16 numbers (gate and up of 50 tokens, 2 of 8
+// experts 4090 x 14336: 129 us, as two planes throughout 161; of 96 tokens 4096 x 4096 45 and 66).
 #include "mxfp4.h"
 #include <type_traits>
 
@@ -24,6 +24,8 @@ template <int I> using Int = std::integral_constant<int, I>;
 
 constexpr int MOST_EXPERTS = 1024, MOST_TOP = 32, MOST_PASS = 128;           // tokens of a pass
 constexpr int MOST_GROUP = 32, COUNTERS = 1024;
+constexpr int MOST_DOWN = 16;                       // slots of a group of down
+constexpr int PLANES = 3;                           // bf16 numbers that an fp32 number is the sum of
 constexpr uint32_t OUTSIDE = 0x80000000u;
 
 __device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
@@ -193,13 +195,14 @@ __global__ __launch_bounds__(256) void route_kernel(RouterArgs r, int64_t T, int
 }
 
 // ---- what the products are told -----------------------------------------------------------------------------------
-// A pass: the slots (token and choice) sorted by expert, in groups of at most `size` of one expert.
+// A pass: the slots (token and choice) sorted by expert, in groups of at most `size` of one expert for gate and up.  Down takes the same groups, or, as three planes
+// of 32 slots do not fit LDS, groups of at most 16, which stand behind them.
 struct Group {
   int expert, first, count, pad;                    // first: slot
   uint32_t token[MOST_GROUP / 4];                   // four to a word
 };
 struct Plan {
-  int groups, pad[15];
+  int groups, down_first, down_groups, pad[13];
   uint32_t counter[COUNTERS];                       // parts of gate and up that are done (fewer than 384 units have any)
   int slot[MOST_PASS * MOST_TOP], expert[MOST_PASS * MOST_TOP];              // of a token's choices; slot -1: none
   float weight[MOST_PASS * MOST_TOP];
@@ -209,10 +212,9 @@ struct Plan {
 struct Operand { const char* x; int64_t ldx; int dtype, planes, K, Kp; uint16_t* out; };
 
 // Values as sums of bf16 numbers (what is infinite or NaN: in the first alone).
-template <int P>
 __device__ __forceinline__ void planes_of(float v, uint16_t* out) {
   #pragma unroll
-  for (int p = 0; p < P; ++p) {
+  for (int p = 0; p < PLANES; ++p) {
     const uint32_t u = bf16_bits(v);
     out[p] = (uint16_t)u;
     const float taken = u2f(u << 16);
@@ -231,8 +233,8 @@ __global__ __launch_bounds__(1024) void plan_kernel(RouterArgs r, const int* __r
       const int64_t t = i / o.Kp;
       const int k = (int)(i - t * o.Kp);
       const float v = k < o.K ? load_any(o.x, o.dtype, t * o.ldx + k) : 0.0f;
-      uint16_t p[4];
-      planes_of<4>(v, p);
+      uint16_t p[PLANES];
+      planes_of(v, p);
       if (o.dtype == LCQ_F16) p[0] = __builtin_bit_cast(uint16_t, (_Float16)v);              // (one plane)
       for (int q = 0; q < o.planes; ++q) o.out[(t * o.planes + q) * o.Kp + k] = p[q];
     }
@@ -272,39 +274,51 @@ __global__ __launch_bounds__(1024) void plan_kernel(RouterArgs r, const int* __r
     if (expert[i] >= 0) atomicOr(&chosen[expert[i]][t / 32], 1u << t % 32);
   }
   __syncthreads();
-  // slots of the experts in front of each in the low half, their groups in the high half
-  uint32_t mine = 0;
+  int n = 0;
   #pragma unroll
-  for (int q = 0; q < MOST_PASS / 32; ++q) mine += __builtin_popcount(chosen[tid][q]);
-  const int n = (int)mine;
-  mine |= (uint32_t)((n + size - 1) / size) << 16;
-  uint32_t sum = mine;
-  #pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint32_t o_ = __shfl_up(sum, d);
-    if (lane >= d) sum += o_;
-  }
-  if (lane == 63) sums[wave] = sum;
-  __syncthreads();
-  uint32_t in_front = 0, all = 0;
-  #pragma unroll
-  for (int w = 0; w < 16; ++w) {
-    in_front += w < wave ? sums[w] : 0;
-    all += sums[w];
-  }
-  const uint32_t before = in_front + sum - mine;
+  for (int q = 0; q < MOST_PASS / 32; ++q) n += __builtin_popcount(chosen[tid][q]);
+  // the sum of what the experts in front of each have, and of all
+  const auto in_front = [&](uint32_t mine, uint32_t& all) {
+    uint32_t sum = mine, before = 0;
+    #pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const uint32_t o_ = __shfl_up(sum, d);
+      if (lane >= d) sum += o_;
+    }
+    if (lane == 63) sums[wave] = sum;
+    __syncthreads();
+    all = 0;
+    #pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      before += w < wave ? sums[w] : 0;
+      all += sums[w];
+    }
+    return before + sum - mine;
+  };
+  const bool split = size > MOST_DOWN;
+  uint32_t all, all_down = 0, before_down = 0;
+  const uint32_t before = in_front((uint32_t)n | (uint32_t)((n + size - 1) / size) << 16, all);          // slots in the low half, groups in the high half
   place[tid] = before;
   __syncthreads();
+  if (split) before_down = in_front((uint32_t)((n + MOST_DOWN - 1) / MOST_DOWN), all_down);
   // (all stores behind the last barrier, which would wait for them)
   const int groups = (int)(all >> 16);
-  if (tid == 0) plan->groups = groups;
-  for (int i = tid; i < COUNTERS; i += 1024) plan->counter[i] = 0;
-  for (int g = 0; g * size < n; ++g) {
-    Group& to = plan->group[(before >> 16) + g];
-    to.expert = tid;
-    to.first = (int)(before & 0xffff) + size * g;
-    to.count = n - size * g < size ? n - size * g : size;
+  if (tid == 0) {
+    plan->groups = groups;
+    plan->down_first = split ? groups : 0;
+    plan->down_groups = split ? (int)all_down : groups;
   }
+  for (int i = tid; i < COUNTERS; i += 1024) plan->counter[i] = 0;
+  const auto list = [&](uint32_t first, int size) {
+    for (int g = 0; g * size < n; ++g) {
+      Group& to = plan->group[first + g];
+      to.expert = tid;
+      to.first = (int)(before & 0xffff) + size * g;
+      to.count = n - size * g < size ? n - size * g : size;
+    }
+  };
+  list(before >> 16, size);
+  if (split) list((uint32_t)groups + before_down, MOST_DOWN);
   for (int i = tid; i < slots; i += 1024) {
     const int e = expert[i], t = i / r.top;
     int slot = -1;
@@ -334,7 +348,7 @@ struct MoeArgs {
   int64_t ldx, ldp;
   Weights gate_up, down;
   Plan* plan;
-  uint16_t* h;                                      // [slots, PH, Ip]
+  uint16_t* h;                                      // [slots, PLANES, Ip]
   float *up, *out;                                  // sums of parts of K: of gate and up as the lanes hold them; of down [slots, parts, N]
   void* y;
   int T, top, N, I, Kp, Ip, activation;             // Kp, Ip: whole blocks
@@ -379,20 +393,29 @@ __device__ __forceinline__ float act(float v, int activation) {
 // One barrier per stage, in front of its products: what was read before it is loaded again.
 constexpr int STAGE = 128;                          // bytes of a row's codes
 
-// P planes of a group of GS slots are ROWS rows of the operand, the columns of the matrix pipe's products in blocks of 16; what the planes of
-// a slot give is added up when a unit is done.
+// P planes of a group of GS slots are ROWS rows of the operand.  Of four slots the planes are columns of one product, four of a slot (the last one is not looked
+// at), added up when a unit is done; of 16 they are blocks of 16 columns, each with a product of its own into the same sums.
 template <int P, int GS>
 struct Shape {
-  static constexpr int ROWS = GS * P, CB = (ROWS + 15) / 16;
-  static constexpr int X = (ROWS + 7) / 8;                                   // a wave's loads of the operand, two rows each (4 rows: of two waves)
-  static constexpr int LOADS = 4 + X, FEWER = ROWS < 8 ? 4 : LOADS;          // of a stage: of the first two waves, of the others
+  static constexpr bool JOINED = P > 1 && GS == 4;
+  static constexpr int ROWS = GS * P, CB = GS == 32 ? 2 : 1;                 // blocks of columns of the sums
+  static constexpr int OB = JOINED || ROWS < 16 ? 1 : ROWS / 16;             // and of the operand
+  static constexpr int X = (ROWS + 7) / 8;                                   // a wave's loads of the operand, two rows each (of the last four rows: of two waves)
+  static constexpr int LOADS = 4 + X, FEWER = 4 + ROWS / 8;                  // of a stage: of the first two waves, of the others
   static constexpr int BYTES = 16384 + ROWS * 512;                           // of a stage, in LDS
   static constexpr int DEPTH = 3 * (BYTES + 4096) <= 81920 ? 3 : 163840 / (BYTES + 4096) < 5 ? 163840 / (BYTES + 4096) : 5;      // two workgroups per CU, or one
   static constexpr int LDS = DEPTH * (BYTES + 4096);
-  // 16-byte piece p of an operand's row r lies at p ^ turn(r).  LDS serves 16 lanes of a 16-byte read at once, of lane / 16 = 0: lanes 0 .. 3 and 12 .. 15, of
-  // 1: 4 .. 11 (and the other way round, and so on), and those read pieces 4 apart: with p ^ r two of them met in a bank.
-  __device__ static constexpr int turn(int r) { return ROWS == 4 ? r : ROWS == 8 ? (r & 3) | (r & 4) << 1 : (r & 15) ^ (((r & 15) + 4 & 8) >> 1); }
-  static_assert(DEPTH >= 3 && (P & (P - 1)) == 0 && (GS & (GS - 1)) == 0, "stages in LDS");
+  // The row that column c of block b reads, and the slot and plane of a row.
+  __device__ static constexpr int row(int b, int c) { return JOINED ? c / 4 * P + (c % 4 < P ? c % 4 : P - 1) : ROWS < 16 ? c % ROWS : b * 16 + c; }
+  __device__ static constexpr int slot(int r) { return JOINED ? r / P : r % GS; }
+  __device__ static constexpr int plane(int r) { return JOINED ? r % P : r / GS; }
+  // 16-byte piece p of an operand's row lies at p ^ turn(c) if column c reads it.  LDS serves 16 lanes of a 16-byte read at once, of lane / 16 = 0: lanes 0 .. 3 and
+  // 12 .. 15, of 1: 4 .. 11 (and the other way round, and so on), and those read pieces 4 apart: with p ^ c two of them met in a bank.
+  __device__ static constexpr int turn(int r) {
+    const int c = JOINED ? r / P * 4 + r % P : r & 15;
+    return ROWS == 4 ? r : c ^ ((c + 4 & 8) >> 1);
+  }
+  static_assert(DEPTH >= 3 && (P == 1 || P == PLANES) && (GS == 4 || GS == 16 || GS == 32), "stages in LDS");
 };
 
 typedef __attribute__((address_space(3))) char* lds_ptr;
@@ -423,10 +446,10 @@ __device__ __forceinline__ bool last_of(uint32_t* counter, int parts) {
 //   down: (group, part of K) of one tile of 128 channels, a workgroup takes one of `runs` runs of them.
 // With one wave per SIMD it is bound by the instructions it issues, so what is the same for all stages of a unit, or for all but its last, is
 // not looked at in every stage.
-template <bool DOWN, int P, int GS, int PH, bool HALF>
+template <bool DOWN, int P, int GS, bool HALF>
 __global__ __launch_bounds__(256) void experts_kernel(MoeArgs g, int tiles, int parts, int runs) {
   typedef Shape<P, GS> S;
-  constexpr int CB = S::CB, DEPTH = S::DEPTH, WIDTH = DOWN ? 128 : 64;
+  constexpr int CB = S::CB, OB = S::OB, DEPTH = S::DEPTH, WIDTH = DOWN ? 128 : 64;
   extern __shared__ __attribute__((aligned(1024))) char lds[];               // DEPTH stages, then as many places of scales
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -440,10 +463,10 @@ __global__ __launch_bounds__(256) void experts_kernel(MoeArgs g, int tiles, int 
   const bool ragged = B % 8 != 0;                   // the last stage is not whole
   struct Who { int expert, first, count; };
   const auto who = [&](const Plan* plan, int group) {
-    const Group& in = plan->group[group];
+    const Group& in = plan->group[DOWN ? fixed(plan->down_first) + group : group];
     return Who{fixed(in.expert), fixed(in.first), fixed(in.count)};
   };
-  const int groups = fixed(g.plan->groups);
+  const int groups = fixed(DOWN ? g.plan->down_groups : g.plan->groups);
   int unit, end, step = 1, tile = 0;
   if constexpr (DOWN) {
     const int run = blockIdx.x / tiles, units = groups * parts;
@@ -531,8 +554,8 @@ __global__ __launch_bounds__(256) void experts_kernel(MoeArgs g, int tiles, int 
       uint32_t of[2];
       #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int r = (wave + 4 * o) * 2 + i, slot = r / P, plane = r % P;
-        if constexpr (DOWN) of[i] = (uint32_t)((first + slot) * P + plane) * (uint32_t)(ldp * 2);
+        const int r = (wave + 4 * o) * 2 + i, slot = S::slot(r), plane = S::plane(r);
+        if constexpr (DOWN) of[i] = (uint32_t)((first + slot) * PLANES + plane) * (uint32_t)(ldp * 2);
         else {
           const int token = slot < count ? (int)(fixed(plan->group[at.group].token[slot >> 2]) >> 8 * (slot & 3) & 255) : 0;
           of[i] = (uint32_t)((token * ldx + plane * ldp) * 2);
@@ -559,13 +582,13 @@ __global__ __launch_bounds__(256) void experts_kernel(MoeArgs g, int tiles, int 
       for (int l = 0; l < 4; ++l) weights(to + l * 1024, (piece ^ (l & 1) * 4) < left ? wof[l] : OUTSIDE, bufW[l >> 1], at.k * STAGE);
       #pragma unroll
       for (int o = 0; o < S::X; ++o)
-        if (S::ROWS >= 8 || wave < 2) load(too + o * 4096, operand_piece(o) < left * 4 ? xof[o] : OUTSIDE, bufX, at.k * 512);
+        if (o < S::ROWS / 8 || wave < 2) load(too + o * 4096, operand_piece(o) < left * 4 ? xof[o] : OUTSIDE, bufX, at.k * 512);
     } else {
       #pragma unroll
       for (int l = 0; l < 4; ++l) weights(to + l * 1024, wof[l], bufW[l >> 1], at.k * STAGE);
       #pragma unroll
       for (int o = 0; o < S::X; ++o)
-        if (S::ROWS >= 8 || wave < 2) load(too + o * 4096, xof[o], bufX, at.k * 512);
+        if (o < S::ROWS / 8 || wave < 2) load(too + o * 4096, xof[o], bufX, at.k * 512);
     }
     if (++at.k == at.end && !over) {
       go(at, at.unit + step);
@@ -598,15 +621,18 @@ __global__ __launch_bounds__(256) void experts_kernel(MoeArgs g, int tiles, int 
     }
     #pragma unroll
     for (int b = 0; b < CB; ++b) {
-      #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      if constexpr (S::JOINED) {                    // then all lanes of a slot have its sums
         #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if constexpr (P >= 2) acc[u][b][r] += lane_xor<1>(acc[u][b][r]);
-          if constexpr (P >= 4) acc[u][b][r] += lane_xor<2>(acc[u][b][r]);
-        }
-      const int s = (b * 16 + c) / P, mine = c % P; // all lanes of a slot have its sums
-      if (s >= of.count || (S::ROWS < 16 && c >= S::ROWS)) continue;
+        for (int u = 0; u < 2; ++u)
+          #pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float v = c % 4 < P ? acc[u][b][r] : 0.0f;
+            v += lane_xor<1>(v);
+            acc[u][b][r] = v + lane_xor<2>(v);
+          }
+      }
+      const int s = S::JOINED ? c / 4 : b * 16 + c, mine = S::JOINED ? c % 4 : 0;
+      if (s >= of.count || s >= GS) continue;
       if constexpr (DOWN) {
         #pragma unroll
         for (int u = 0; u < 2; ++u)                 // (rows of whole fours; what lies behind N is not read)
@@ -614,7 +640,7 @@ __global__ __launch_bounds__(256) void experts_kernel(MoeArgs g, int tiles, int 
             *(f32x4*)(fixed(a->out) + ((int64_t)(of.first + s) * parts + p.part) * ((channels + 3) & ~3) + rows.n0 + u * 16 + q * 4) = acc[u][b];
       } else {
         if (rows.n0 + q * 4 >= Ip) continue;
-        uint16_t h[4][PH];
+        uint16_t h[4][PLANES];
         #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int ch = q * 4 + r;
@@ -623,12 +649,12 @@ __global__ __launch_bounds__(256) void experts_kernel(MoeArgs g, int tiles, int 
             #pragma unroll
             for (int u = 0; u < 2; ++u) v[u] += load_any(w.bias, w.bias_dtype, ((int64_t)of.expert * 2 + u) * channels + rows.n0 + ch);
           }
-          planes_of<PH>(ch < rows.of[0] ? act(v[0], activation) * v[1] : 0.0f, h[r]);
+          planes_of(ch < rows.of[0] ? act(v[0], activation) * v[1] : 0.0f, h[r]);
         }
         #pragma unroll
-        for (int l = 0; l < PH; ++l)
-          if (l % P == mine)
-            *(u32x2*)(fixed(a->h) + ((int64_t)(of.first + s) * PH + l) * Ip + rows.n0 + q * 4) = u32x2{h[0][l] | (uint32_t)h[1][l] << 16, h[2][l] | (uint32_t)h[3][l] << 16};
+        for (int l = 0; l < PLANES; ++l)
+          if (!S::JOINED || l == mine)
+            *(u32x2*)(fixed(a->h) + ((int64_t)(of.first + s) * PLANES + l) * Ip + rows.n0 + q * 4) = u32x2{h[0][l] | (uint32_t)h[1][l] << 16, h[2][l] | (uint32_t)h[3][l] << 16};
       }
     }
   };
@@ -656,7 +682,7 @@ __global__ __launch_bounds__(256) void experts_kernel(MoeArgs g, int tiles, int 
   uint32_t codes[2], operand[4];
   #pragma unroll
   for (int i = 0; i < 2; ++i) codes[i] = lds0 + wave * 4096 + c * 128 + (((i * 4 + q) ^ (c >> 1 & 7)) << 4);
-  const int row = S::ROWS < 16 ? c & (S::ROWS - 1) : c;
+  const int row = S::row(0, c);                     // (of block b 16 b behind it)
   #pragma unroll
   for (int j = 0; j < 4; ++j) operand[j] = lds0 + 16384 + row * 512 + (((q * 4 + j) ^ S::turn(row)) << 4);
   int slot = 0, cperiod = 0, cplace = 0;
@@ -674,7 +700,7 @@ __global__ __launch_bounds__(256) void experts_kernel(MoeArgs g, int tiles, int 
       // for each
       i32x4 wv[2][2];
       uint32_t byte[2][2];
-      bf16x8 x[2][4][CB];
+      bf16x8 x[2][4][OB];
       #pragma unroll
       for (int i = 0; i < 2; ++i) {
         #pragma unroll
@@ -685,7 +711,7 @@ __global__ __launch_bounds__(256) void experts_kernel(MoeArgs g, int tiles, int 
         #pragma unroll
         for (int j = 0; j < 4; ++j)
           #pragma unroll
-          for (int b = 0; b < CB; ++b) x[i][j][b] = from_lds<bf16x8>(operand[j] + here + i * 256 + b * 8192);
+          for (int b = 0; b < OB; ++b) x[i][j][b] = from_lds<bf16x8>(operand[j] + here + i * 256 + b * 8192);
       }
       __builtin_amdgcn_sched_barrier(0);
       const int left = B - now.k * 8;
@@ -740,9 +766,9 @@ __global__ __launch_bounds__(256) void experts_kernel(MoeArgs g, int tiles, int 
           #pragma unroll
           for (int u = 0; u < 2; ++u) v[u] = decoded(wv[u][i][j], mx_factor(byte[u][i] & there));
           #pragma unroll
-          for (int b = 0; b < CB; ++b)
+          for (int b = OB - 1; b >= 0; --b)         // (the smallest planes first)
             #pragma unroll
-            for (int u = 0; u < 2; ++u) acc[u][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u], x[i][j][b], acc[u][b], 0, 0, 0);
+            for (int u = 0; u < 2; ++u) acc[u][b % CB] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u], x[i][j][b], acc[u][b % CB], 0, 0, 0);
         }
       }
       slot = slot == DEPTH - 1 ? 0 : slot + 1;
@@ -829,23 +855,22 @@ bool direct(int dtype, const void* x, int64_t ldx, int64_t K) {
   return dtype != LCQ_F32 && K % 32 == 0 && ldx % 8 == 0 && (uintptr_t)x % 16 == 0 && ldx <= 1 << 22;       // (offsets have 31 bits)
 }
 
-int planes_of_h(int dtype) { return dtype == LCQ_F32 ? 4 : 2; }
-// tokens of a pass: as many as the offsets within h, 31 bits, have room for (64 at least)
-int64_t pass_of(int64_t top, int64_t I, int dtype) { return least(MOST_PASS, (1 << 30) / (top * planes_of_h(dtype) * ((I + 31) / 32 * 32) * 2)); }
+// tokens of a pass: as many as the offsets within h, 31 bits, have room for (85 at least)
+int64_t pass_of(int64_t top, int64_t I) { return least(MOST_PASS, (1 << 30) / (top * PLANES * ((I + 31) / 32 * 32) * 2)); }
 
 // How a pass of T tokens is cut.
 struct Cut {
-  int P, PH, size, up_tiles, up_parts, down_tiles, down_parts, runs;
+  int P, size, up_tiles, up_parts, down_tiles, down_parts, runs;
   int64_t groups, h, up, out;                       // bytes
   Cut(int64_t T, int64_t top, int64_t E, int64_t K, int64_t I, int64_t N, int dtype) {
-    P = dtype == LCQ_F32 ? 4 : 1;
-    PH = planes_of_h(dtype);
+    P = dtype == LCQ_F32 ? PLANES : 1;
     const int64_t slots = T * top;
     // Slots of a group: few columns cost less in every stage, a second group of an expert reads its bytes again.  The whole layer in us with 4 / 16 / 32:
     //   4 tokens, 6 of 64 experts 40 / 48 / 55    16 tokens, 8 of 256 378 / 461 / 617    64 tokens, 4 of 32 159 / 94 / 123    64 tokens, 2 of 8 164 / 95 / 94
     //   96 tokens, 2 of 8 208 / 112 / 97
-    size = T <= 4 || slots <= E ? 4 : P == 4 || T <= 16 || slots <= 18 * E ? 16 : 32;
-    groups = least(slots, least(E, slots) + slots / size);
+    size = T <= 4 || slots <= E ? 4 : P > 1 || T <= 16 || slots <= 18 * E ? 16 : 32;
+    const auto groups_of = [&](int size) { return least(slots, least(E, slots) + slots / size); };
+    groups = groups_of(size);
     const int64_t up_stages = ((K + 31) / 32 + 7) / 8, down_stages = ((I + 31) / 32 + 7) / 8, Ip = (I + 31) / 32 * 32;
     up_tiles = (int)((Ip + 63) / 64);
     // Parts of K of gate and up, where a few narrow experts leave the chip to a few long units: a stage is 0.45 us, making sums visible to the workgroup that adds
@@ -859,19 +884,20 @@ struct Cut {
     int64_t want = 512 / down_tiles;
     if (want < 1) want = 1;
     down_parts = 1;
-    while (groups * down_parts < 6 * want && down_stages / (2 * down_parts) >= 6) down_parts *= 2;
-    const int64_t units = groups * down_parts, each = (units + want - 1) / want;
+    const int64_t down_groups = groups_of(size < MOST_DOWN ? size : MOST_DOWN);
+    while (down_groups * down_parts < 6 * want && down_stages / (2 * down_parts) >= 6) down_parts *= 2;
+    const int64_t units = down_groups * down_parts, each = (units + want - 1) / want;
     runs = (int)((units + each - 1) / each);
-    h = on256(slots * PH * Ip * 2);
-    up = up_parts > 1 ? on256(groups * up_tiles * up_parts * 256 * 32 * ((size * P + 15) / 16)) : 0;
+    h = on256(slots * PLANES * Ip * 2);
+    up = up_parts > 1 ? on256(groups * up_tiles * up_parts * 256 * 32 * (size == 32 ? 2 : 1)) : 0;
     out = on256(slots * down_parts * ((N + 3) & ~(int64_t)3) * 4);
   }
 };
 
-template <bool DOWN, int P, int GS, int PH, bool HALF>
+template <bool DOWN, int P, int GS, bool HALF>
 int launch_experts(const MoeArgs& g, const Cut& c, hipStream_t st) {
   typedef Shape<P, GS> S;
-  const auto kernel = experts_kernel<DOWN, P, GS, PH, HALF>;
+  const auto kernel = experts_kernel<DOWN, P, GS, HALF>;
   // (more LDS than a launch may have without asking)
   if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS) != hipSuccess) return LCQ_ELAUNCH;
   // as many as run at a time, or fewer
@@ -879,11 +905,11 @@ int launch_experts(const MoeArgs& g, const Cut& c, hipStream_t st) {
   kernel<<<dim3((unsigned)blocks), dim3(256), S::LDS, st>>>(g, DOWN ? c.down_tiles : c.up_tiles, DOWN ? c.down_parts : c.up_parts, c.runs);
   return LCQ_OK;
 }
-template <bool DOWN, int P, int PH, bool HALF>
+template <bool DOWN, int P, bool HALF>
 int launch_size(const MoeArgs& g, const Cut& c, hipStream_t st) {
-  if (c.size == 4) return launch_experts<DOWN, P, 4, PH, HALF>(g, c, st);
-  if constexpr (P < 4) { if (c.size == 32) return launch_experts<DOWN, P, 32, PH, HALF>(g, c, st); }
-  return launch_experts<DOWN, P, 16, PH, HALF>(g, c, st);
+  if (c.size == 4) return launch_experts<DOWN, P, 4, HALF>(g, c, st);
+  if constexpr (P == 1) { if (c.size == 32) return launch_experts<DOWN, P, 32, HALF>(g, c, st); }
+  return launch_experts<DOWN, P, MOST_DOWN, HALF>(g, c, st);
 }
 template <int BF>
 void launch_sum(const MoeArgs& g, const Cut& c, hipStream_t st) {
@@ -912,7 +938,7 @@ int lcq_route(const void* logits, int dtype, int64_t T, int64_t E, int64_t ldl, 
 
 int64_t lcq_mxfp4_moe_workspace_bytes(int64_t T, int64_t top, int64_t E, int64_t K, int64_t I, int64_t N, int dtype) {
   if (T <= 0 || top <= 0 || E <= 0 || K <= 0 || I <= 0 || N <= 0 || K > 65536 || I > 65536 || N > 65536 || top > MOST_TOP || E > MOST_EXPERTS || !known(dtype)) return 0;
-  const int64_t pass = pass_of(top, I, dtype), t = least(T, pass);
+  const int64_t pass = pass_of(top, I), t = least(T, pass);
   int64_t most = 0;                                 // (the last pass may have fewer tokens, and be cut into more parts)
   for (const int64_t n : {t, T % pass ? T % pass : t}) {
     const Cut c(n, top, E, K, I, N, dtype);
@@ -947,7 +973,7 @@ int lcq_mxfp4_moe(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, c
   const bool as_is = direct(dtype, x, ldx, K);
   Plan* const plan = (Plan*)ws;
   const int64_t size = dtype == LCQ_F32 ? 4 : 2, out_size = out_dtype == LCQ_F32 ? 4 : 2, logit_size = logits_dtype == LCQ_F32 ? 4 : 2;
-  const int64_t pass = pass_of(top, I, dtype);
+  const int64_t pass = pass_of(top, I);
   for (int64_t t0 = 0; t0 < T; t0 += pass) {
     const int n = (int)least(T - t0, pass);
     const Cut c(n, top, E, K, I, N, dtype);
@@ -978,9 +1004,9 @@ int lcq_mxfp4_moe(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, c
     if (E <= 64) plan_kernel<1><<<grid, dim3(1024), 0, st>>>(rt, ge, gw, n, o, c.size, plan);
     else if (E <= 256) plan_kernel<4><<<grid, dim3(1024), 0, st>>>(rt, ge, gw, n, o, c.size, plan);
     else plan_kernel<16><<<grid, dim3(1024), 0, st>>>(rt, ge, gw, n, o, c.size, plan);
-    int rc = dtype == LCQ_BF16 ? launch_size<false, 1, 2, false>(g, c, st) : dtype == LCQ_F16 ? launch_size<false, 1, 2, true>(g, c, st) : launch_size<false, 4, 4, false>(g, c, st);
+    int rc = dtype == LCQ_BF16 ? launch_size<false, 1, false>(g, c, st) : dtype == LCQ_F16 ? launch_size<false, 1, true>(g, c, st) : launch_size<false, PLANES, false>(g, c, st);
     if (rc) return rc;
-    rc = c.PH == 2 ? launch_size<true, 2, 2, false>(g, c, st) : launch_size<true, 4, 4, false>(g, c, st);
+    rc = launch_size<true, PLANES, false>(g, c, st);
     if (rc) return rc;
     if (out_dtype == LCQ_BF16) launch_sum<ROW_BF16>(g, c, st);
     else if (out_dtype == LCQ_F16) launch_sum<ROW_F16>(g, c, st);

@@ -100,7 +100,7 @@ def mxfp4_moe(x, router, gate_up, down, *, gate_up_bias=None, down_bias=None, ac
     times counts once, with the sum of the weights).  gate_up: Mxfp4 of [E, 2 I, K], the gates' rows and then the ups';  down: Mxfp4 of [E, N, I].
     gate_up_bias [E, 2 I], down_bias [E, N]: of one type.  activation 'silu' or 'gelu' (by erf).  -> [..., N] of x's type or `out_dtype`.
 
-    Activations are not quantized; sums are fp32.  An expert whose weight is 0 is not asked; a token without experts gives 0.  This is for
+    Activations are not quantized, sums and act(...) * (...) are fp32.  An expert whose weight is 0 is not asked; a token without experts gives 0.  This is for
     few tokens: up to 128 at a time share a pass over the experts' bytes.  Operands with strides are copied (experts and their rows may lie apart)."""
     shape = x.shape
     K = _cols(shape)

@@ -352,3 +352,32 @@ def test_refusals(dev):
                 lambda: mxfp4_moe(x, ok, gate_up, down, down_bias=torch.zeros(E, N, device=dev, dtype=torch.int32))):
         with pytest.raises(LcqError):
             bad()
+
+
+def picks(E, rows, cols, columns, dev):
+    """Experts whose row r is a 1.0 in column columns[r] and zeros."""
+    codes = torch.zeros(E, rows, 16 * ((cols + 31) // 32), dtype=torch.uint8, device=dev)
+    r = torch.arange(rows, device=dev)
+    codes[:, r, columns // 2] = (2 << 4 * (columns % 2)).to(torch.uint8)
+    return Mxfp4(codes, torch.full((E, rows, (cols + 31) // 32), 127, dtype=torch.uint8, device=dev), cols)
+
+
+@pytest.mark.parametrize('dtype', [BF, HF, F32])
+@pytest.mark.parametrize('T,E,top', [(1, 4, 1), (3, 4, 2), (20, 4, 2), (100, 4, 1), (128, 3, 2)])
+def test_what_lies_between_the_products_keeps_32_bits(dev, T, E, top, dtype):
+    """Weights that pick one column: gate, up and y are single numbers, exact in fp32, so that y is silu(gate) * up as fp32 has it.  An exponential of at most
+    two units (4 U), a sum, a quotient and a product of half a unit each: 7 U, and U^2 terms."""
+    g = gpu_gen(T)
+    K, I, N = 100, 70, 90
+    x = (3 * torch.randn(T, K, generator=g, device=dev)).to(dtype)
+    gate, up, out = (torch.randint(0, n, (m,), generator=g, device=dev) for n, m in ((K, I), (K, I), (I, N)))
+    gate_up, down = picks(E, 2 * I, K, torch.cat([gate, up]), dev), picks(E, N, I, out, dev)
+    experts = torch.stack([torch.randperm(E, generator=g, device=dev)[:top] for _ in range(T)]).int()
+    weights = torch.zeros(T, top, device=dev)
+    weights[:, -1] = 1.0
+    if T > 4:
+        experts[:, -1] = torch.where(torch.arange(T, device=dev) < T // 2, 1, experts[:, -1])     # (a crowd; an expert twice counts once)
+    got = mxfp4_moe(x, Routing(experts, weights), gate_up, down, out_dtype=F32)
+    xs = x.to(f64)
+    want = (torch.nn.functional.silu(xs[:, gate]) * xs[:, up])[:, out]
+    assert bool(((got.to(f64) - want).abs() <= 8 * U * want.abs() + 2.0 ** -133).all())
