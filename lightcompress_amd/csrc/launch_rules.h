@@ -1,6 +1,7 @@
 // Rules by which an entry point takes one of several kernels, as functions of sizes, types and alignment alone.  Plain C++: they can
 // be checked without a GPU and without a HIP compiler.
 #pragma once
+#include <type_traits>
 
 namespace lcq {
 
@@ -137,5 +138,15 @@ inline Mxfp4Cut mxfp4_cut(long long M, long long N, long long B) {
   if (teams <= 64 && 3.4 + 0.39 * mxfp4_stages(M, N, B, mxfp4_waves(M, N, B)) < least) best = {true, 0, 1};
   return best;
 }
+
+// A wave's outputs of a tile leave 64 pieces of 16 bytes at a time, rows of 32 FN outputs of E bytes: TOKENS rows together.  A lane's place among them, N outputs to a
+// row, is told apart from the store's in 32 bits where those hold it for every N that the product takes (tiles of 256 and 128), and in 64 bits elsewhere.
+constexpr long long MXFP4_MOST_N = (1 << 28) - 16;
+template <int FN, int E>
+struct Mxfp4Store {
+  static constexpr int TOKENS = 64 * 16 / (32 * FN * E);
+  static constexpr long long MOST = (TOKENS - 1) * MXFP4_MOST_N * E + 64 * FN * E;       // (a tile has twice the wave's channels)
+  typedef std::conditional_t<MOST <= 0xffffffffLL, unsigned, unsigned long long> Offset;
+};
 
 }  // namespace lcq

@@ -304,11 +304,11 @@ __global__ __launch_bounds__(256, 1) void tile_kernel(MxArgs g, int tiles_m, int
       }
     }
     asm volatile("" ::: "memory");                  // (LDS serves a wave in order)
-    constexpr int AT_ONCE = 64 / CHUNKS, TIMES = STEP * 32 / AT_ONCE, SOME = TIMES < 8 ? TIMES : 8;          // tokens of a store, stores, those on their way together
+    constexpr int AT_ONCE = Mxfp4Store<FN, E>::TOKENS, TIMES = STEP * 32 / AT_ONCE, SOME = TIMES < 8 ? TIMES : 8;          // tokens of a store, stores, those on their way together
     const int t0 = lane / CHUNKS, ch = lane % CHUNKS, n = wc * FN * 32 + ch * CH;
     char* const to = (char*)g.y + ((m0 + wr * FM * 32 + i0 * 32) * g.N + n0 + (BF == ROW_SUM ? part * g.M * g.N : 0)) * E;
     if (rows_a == T::TM && rows_w == T::TN) {       // (uniform, as most tiles of a large product are: no comparison, no address but a scalar one)
-      const uint32_t of = (uint32_t)(t0 * g.N + n) * E;                      // (7 N outputs of two bytes or 3 N of four, and a tile's: 32 bits)
+      const auto of = (typename Mxfp4Store<FN, E>::Offset)((t0 * g.N + n) * E);
       #pragma unroll
       for (int o0 = 0; o0 < TIMES; o0 += SOME) {
         u32x4 v[SOME];
@@ -732,7 +732,7 @@ int check(const uint8_t* w, int64_t ldw, const uint8_t* sw, int64_t ldsw, const 
   if (!w || !sw || !y || M <= 0 || N <= 0 || K <= 0) return LCQ_EINVAL;
   if (!known(dtype) || (bias && !known(bias_dtype))) return LCQ_EDTYPE;
   // A launch has fewer than 2^32 lanes: tiles of 128 x 128, rounded up to eight; 16 channels of 256 lanes.  Offsets within a tile have 31 bits.
-  if (K > 65536 || M > 1 << 28 || N > (1 << 28) - 16 || (M + 127) / 128 * ((N + 127) / 128) > (1 << 24) - 8) return LCQ_ESIZE;
+  if (K > 65536 || M > 1 << 28 || N > MXFP4_MOST_N || (M + 127) / 128 * ((N + 127) / 128) > (1 << 24) - 8) return LCQ_ESIZE;
   const int64_t B = (K + 31) / 32;
   if (ldw < 16 * B || ldsw < B) return LCQ_EINVAL;
   if (ldw > 1 << 22 || ldsw > 1 << 22) return LCQ_ESIZE;

@@ -13,6 +13,14 @@ WRAPPERS = '''
 #include "launch_rules.h"
 extern "C" int cut(long long M, long long N, long long B) { const lcq::Mxfp4Cut c = lcq::mxfp4_cut(M, N, B); return c.stream * 1024 + c.tile * 256 + c.parts; }
 extern "C" int waves(long long M, long long N, long long B) { return lcq::mxfp4_waves(M, N, B); }
+template <int FN, int E> long long lost(long long N) {         // of the largest offset of a store, in the type that the kernel has for it
+  typedef lcq::Mxfp4Store<FN, E> S;
+  const long long of = ((S::TOKENS - 1) * N + 64 * FN - 16 / E) * E;
+  return of - (long long)(typename S::Offset)of;
+}
+extern "C" long long lost_of(long long FN, long long E, long long N) {
+  return FN == 4 ? (E == 2 ? lost<4, 2>(N) : lost<4, 4>(N)) : FN == 2 ? (E == 2 ? lost<2, 2>(N) : lost<2, 4>(N)) : E == 2 ? lost<1, 2>(N) : lost<1, 4>(N);
+}
 extern "C" long long units(long long M, long long N, long long KS) { return lcq::mxfp4_units(M, N, (int)KS); }
 '''
 WIDTHS = (1, 15, 16, 100, 200, 300, 1000, 4096, 6144, 14336, 140000, 1 << 24)
@@ -31,9 +39,9 @@ def rules(tmp_path_factory):
     (d / 'w.cpp').write_text(WRAPPERS)
     subprocess.run(['g++', '-std=c++17', '-shared', '-fPIC', f'-I{CSRC}', str(d / 'w.cpp'), '-o', str(d / 'w.so')], check=True)
     so = ctypes.CDLL(str(d / 'w.so'))
-    for f in (so.cut, so.waves, so.units):
+    for f in (so.cut, so.waves, so.units, so.lost_of):
         f.argtypes = [ctypes.c_longlong] * 3
-    so.units.restype = ctypes.c_longlong
+    so.units.restype = so.lost_of.restype = ctypes.c_longlong
     return so
 
 
@@ -96,3 +104,13 @@ def test_sizes_of_the_gpu_tests_reach_every_cut(rules, cut):
     ragged = [(M, N, K) for (M, N, K), c in got if c[0] and M > 32 and M % 32 and N % 16 and K % 256]
     many = [(M, N, K) for (M, N, K), c in got if c[0] and rules.units(M, N, rules.waves(M, N, blocks(K))) > 256]
     assert len(ragged) >= 3 and {M > 32 for M, _, _ in many} == {True, False}
+
+
+def test_offsets_of_stores_keep_their_bits(rules, cut):
+    """Tiles of 64 x 64 are what more channels than 32 bits have bytes for get: 15 rows of two bytes or 7 of four to a store, 2^32 bytes from 143 165 577 channels on."""
+    most = (1 << 28) - 16
+    for N in (143165577, 150000000, 153391690, 160000000, 200000000, most):
+        for E, FN in itertools.product((2, 4), (1, 2, 4)):
+            assert rules.lost_of(FN, E, N) == 0, (N, E, FN)
+    assert {cut(64, N, K)[:2] for N in (150000000, 155000000, most) for K in (32, 512)} == {(0, 2)}
+    assert 15 * 2 * 150000000 > 1 << 32 and 7 * 4 * 155000000 > 1 << 32

@@ -338,6 +338,18 @@ def test_outputs_behind_2_31(dev):
         assert torch.equal(got[:, at], mxfp4_matmul(a, Mxfp4(w.codes[at].contiguous(), w.scales[at].contiguous(), K)))
 
 
+@pytest.mark.parametrize('M,N,dtype', [(64, 150000000, BF), (130, 143165600, HF), (64, 155000000, F32)])
+def test_rows_of_a_store_behind_2_32_bytes(dev, M, N, dtype):
+    """64 x 64 tiles whose stores reach over 15 rows of two bytes, or 7 of four: 2^32 bytes and more."""
+    g = gpu_gen(8)
+    K = 32
+    a, w = random_mx(M, K, g, dev), random_mx(N, K, g, dev, 110, 122)
+    got = mxfp4_matmul(a, w, out_dtype=dtype)
+    for at in (0, 1 << 20, N // 2 // 64 * 64, N - 64 - 1000):
+        rows = slice(at, at + 1000)
+        assert torch.equal(got[:, rows], mxfp4_matmul(a, Mxfp4(w.codes[rows].contiguous(), w.scales[rows].contiguous(), K), out_dtype=dtype))
+
+
 @pytest.mark.parametrize('dtype', [BF, HF, F32])
 def test_one_row_for_all(dev, dtype):
     """Expanded operands: rows that lie on top of each other."""
