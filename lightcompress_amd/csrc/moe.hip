@@ -211,11 +211,11 @@ struct Plan {
 
 struct Operand { const char* x; int64_t ldx; int dtype, planes, K, Kp; uint16_t* out; };
 
-// Values as sums of bf16 numbers (what is infinite or NaN: in the first alone).
+// Values as sums of bf16 numbers (what is infinite or NaN: in the first alone).  What the first would round to an infinity is cut off instead: 16 bits are left.
 __device__ __forceinline__ void planes_of(float v, uint16_t* out) {
   #pragma unroll
   for (int p = 0; p < PLANES; ++p) {
-    const uint32_t u = bf16_bits(v);
+    const uint32_t raw = f2u(v), u = p == 0 && (raw & 0x7fffffff) < 0x7f800000 && (raw & 0x7fffffff) >= 0x7f7f8000 ? raw >> 16 : bf16_bits(v);
     out[p] = (uint16_t)u;
     const float taken = u2f(u << 16);
     v = (u & 0x7f80) == 0x7f80 ? 0.0f : v - taken;

@@ -381,3 +381,27 @@ def test_what_lies_between_the_products_keeps_32_bits(dev, T, E, top, dtype):
     xs = x.to(f64)
     want = (torch.nn.functional.silu(xs[:, gate]) * xs[:, up])[:, out]
     assert bool(((got.to(f64) - want).abs() <= 8 * U * want.abs() + 2.0 ** -133).all())
+
+
+@pytest.mark.parametrize('T', [1, 20])
+def test_the_largest_numbers_stay_finite(dev, T):
+    """Above 2^128 (1 - 2^-9) the nearest bf16 number is an infinity: tokens, and what lies between the products.  Weights that pick one column, y scaled by
+    2^-10: the numbers themselves, but for silu of 16 (7 U, as above)."""
+    most = torch.finfo(F32).max
+    E, K, I, N = 2, 64, 32, 40
+    down = picks(E, N, I, torch.arange(N, device=dev) % I, dev)
+    down = down._replace(scales=down.scales - 10)
+    experts, weights = torch.arange(T, dtype=torch.int32, device=dev)[:, None] % E, torch.ones(T, 1, device=dev)
+    gate_up = picks(E, 2 * I, K, torch.cat([torch.arange(I), 32 + torch.arange(I)]).to(dev), dev)
+    small = gate_up._replace(scales=torch.where(torch.arange(2 * I, device=dev)[:, None] < I, 127, 117).to(torch.uint8).expand(E, -1, 2).contiguous())
+    x = torch.full((T, K), 16.0, device=dev)
+    x[:, 32:] = torch.tensor([most, -most, 3.396e38, -3.395e38], device=dev).repeat(8)
+    for t, q, dtype in ((x, small, F32), (torch.cat([torch.full((T, 32), 2.0 ** 60), torch.full((T, 32), most * 2.0 ** -60)], 1).to(dev), gate_up, F32),
+                        (torch.cat([torch.full((T, 32), 1.0078125 * 2.0 ** 60), torch.full((T, 32), -1.984375 * 2.0 ** 67)], 1).to(dev), gate_up, BF)):
+        t = t.to(dtype)
+        got = mxfp4_moe(t, Routing(experts, weights), q, down, out_dtype=F32)
+        xs = t.to(f64)
+        h = torch.nn.functional.silu(xs[:, :32]) * xs[:, 32:] * (2.0 ** -10 if q is small else 1)
+        want = h[:, torch.arange(N, device=dev) % I] * 2.0 ** -10
+        assert float(h.abs().max()) <= most
+        assert bool(((got.to(f64) - want).abs() <= 8 * U * want.abs()).all())
