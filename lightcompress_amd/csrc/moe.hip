@@ -69,7 +69,7 @@ __device__ __forceinline__ double wave_sum(double v) {
 // One token by one wave: lane s < top gets the s-th choice.  A lane looks at NL consecutive experts.
 //  softmax: e^(l - max) / sum;  sigmoid: 1 / (1 + e^-l).  Chosen by the logits (both grow with them), or, with a correction, by
 //  fp32(score) + correction, the scores from 64 bits, so that they are the numbers they should be to the last bit.
-// -inf is chosen last and weighs 0.
+// -inf is chosen last and weighs 0.  Scores that are divided by their sum and are too small for 32 bits are taken times e^-(their largest logit).
 template <int NL>
 __device__ __forceinline__ void route_token(const RouterArgs& r, int64_t t, int& expert, float& weight) {
   const int lane = threadIdx.x & 63;
@@ -91,7 +91,7 @@ __device__ __forceinline__ void route_token(const RouterArgs& r, int64_t t, int&
     m = nan_max(m, x[j]);
   }
   m = team_reduce<64, true>(m);
-  const bool sigmoid = r.flags & LCQ_ROUTE_SIGMOID;
+  const bool sigmoid = r.flags & LCQ_ROUTE_SIGMOID, renormalize = r.flags & LCQ_ROUTE_RENORMALIZE;
   if (r.correction) {
     double s[NL], sum = 0;
     #pragma unroll
@@ -109,18 +109,26 @@ __device__ __forceinline__ void route_token(const RouterArgs& r, int64_t t, int&
     }
   } else {
     float sum = 0;
+    bool small = false;
     #pragma unroll
     for (int j = 0; j < NL; ++j) {
       score[j] = expf(sigmoid ? -x[j] : x[j] - m);
       if (!sigmoid && x[j] == none) score[j] = 0.0f;
       sum += score[j];
       key[j] = lane * NL + j < r.E ? ordered(x[j]) : 0u;
+      small = small || (x[j] < -60.0f && x[j] != none);
     }
     sum = team_sum<64>(sum);
     #pragma unroll
     for (int j = 0; j < NL; ++j) {
       const float over = sigmoid ? 1.0f + score[j] : sum;
       score[j] = over == 0.0f ? 0.0f : (sigmoid ? 1.0f : score[j]) / over;
+    }
+    if (sigmoid && __builtin_expect(__builtin_amdgcn_ballot_w64(small) != 0, 0)) {           // e^-l may overflow, and 1 + e^l is 1
+      const float from = renormalize && m < -60.0f ? m : 0.0f;               // (the largest logit is chosen)
+      #pragma unroll
+      for (int j = 0; j < NL; ++j)
+        if (x[j] < -60.0f && x[j] != none) score[j] = expf(x[j] - from);
     }
   }
   expert = 0;
@@ -169,14 +177,25 @@ __device__ __forceinline__ void route_token(const RouterArgs& r, int64_t t, int&
         if (lane == from && at == j) key[j] = 0;
     }
   }
-  weight = 0;
-  #pragma unroll
-  for (int j = 0; j < NL; ++j) {
-    const float w = u2f((uint32_t)__builtin_amdgcn_ds_bpermute(expert / NL * 4, (int)f2u(score[j])));
-    if (lane < r.top && expert % NL == j) weight = w;
-  }
-  if (r.flags & LCQ_ROUTE_RENORMALIZE) {
-    const float sum = team_sum<64>(weight);
+  // what the lane's expert has of `of`
+  const auto gathered = [&](const float (&of)[NL], float other) {
+    float v = other;
+    #pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const float w = u2f((uint32_t)__builtin_amdgcn_ds_bpermute(expert / NL * 4, (int)f2u(of[j])));
+      if (lane < r.top && expert % NL == j) v = w;
+    }
+    return v;
+  };
+  weight = gathered(score, 0.0f);
+  if (renormalize) {
+    float sum = team_sum<64>(weight);
+    // With a correction the chosen logits may all lie far below those that the scores are relative to (NaN: stays one).
+    if (r.correction && __builtin_expect(sum < 0x1p-100f, 0)) {
+      const float l = gathered(x, none), best = team_reduce<64, true>(l);
+      weight = l == none ? 0.0f : expf(l - best);   // (of sigmoid too: 1 + e^l is 1)
+      sum = team_sum<64>(weight);
+    }
     weight = sum == 0.0f ? 0.0f : weight / sum;
   }
   weight *= r.scale;

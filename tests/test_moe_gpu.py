@@ -405,3 +405,31 @@ def test_the_largest_numbers_stay_finite(dev, T):
         want = h[:, torch.arange(N, device=dev) % I] * 2.0 ** -10
         assert float(h.abs().max()) <= most
         assert bool(((got.to(f64) - want).abs() <= 8 * U * want.abs()).all())
+
+
+@pytest.mark.parametrize('scoring,corrected', [('softmax', False), ('softmax', True), ('sigmoid', False), ('sigmoid', True)])
+@pytest.mark.parametrize('dtype', [F32, BF, HF])
+@pytest.mark.parametrize('E,top', [(8, 2), (100, 8), (600, 5)])
+def test_route_of_scores_too_small_for_32_bits(dev, E, top, dtype, scoring, corrected):
+    """Chosen logits of -95, -200 and -600: their scores are subnormal or 0 in 32 bits, their shares are not.  One expert stands out in half of the tokens; with a correction it
+    is not chosen all the same.  Bounds as in test_route, differences of logits up to 12 units in the exponent."""
+    g = gpu_gen(E)
+    x = torch.randn(8, E, generator=g, device=dev) + torch.tensor([-95.0, -200.0, -600.0, -90.0], device=dev).repeat(2)[:, None]
+    x[4:, E // 3] = 2.0
+    x[:, E - 1] = -math.inf
+    x = x.to(dtype)
+    c = torch.zeros(E, device=dev) if corrected else None
+    if corrected:
+        c[E // 3] = -3.0
+    for renormalize in (True, False):
+        got = route_tokens(Router(x, top, scoring, renormalize, c, 2.5))
+        experts, weights = routed(x, top, scoring, renormalize, c, 2.5)
+        assert torch.equal(got.experts.long(), experts)
+        assert bool(((got.weights.to(f64) - weights).abs() <= 64 * U * weights + 1e-37).all())
+        if renormalize:
+            assert bool(((got.weights.sum(-1) - 2.5).abs() <= 64 * U * 2.5).all())
+    if dtype == F32:                               # and the layer asks them
+        gate_up, down = experts_of(E, 64, 32, g, dev), experts_of(E, 48, 32, g, dev)
+        t = torch.randn(8, 32, generator=g, device=dev)
+        y = mxfp4_moe(t, Router(x, top, scoring, True, c), gate_up, down)
+        assert torch.equal(y, mxfp4_moe(t, route_tokens(Router(x, top, scoring, True, c)), gate_up, down)) and bool((y != 0).any(1).all())
