@@ -546,7 +546,8 @@ int lcq_token_logprobs_of(const void* logits, int dtype, int64_t B, int64_t S, i
  *  codes   [rows, 16 B], 4-byte aligned;  scales [rows, B], rows `lds` bytes apart: output */
 int lcq_mxfp4_quant(const void* x, int dtype, int64_t rows, int64_t K, int64_t ldx, uint8_t* codes, uint8_t* scales, int64_t lds, void* stream);
 
-/* What codes (rows ldc bytes apart, a multiple of 4) and scales (rows lds apart) stand for: y [rows, K] of `dtype`, rounded once (fp32 and bf16 hold every value). */
+/* What codes (rows ldc bytes apart, a multiple of 4) and scales (rows lds apart) stand for: y [rows, K] of `dtype`, rounded once. fp32 and bf16 hold every value but
+ * those of 2^128 and more (4 and 6 with scale byte 253, 2 to 6 with 254; lcq_mxfp4_quant makes none above 252), which become infinities. */
 int lcq_mxfp4_dequant(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, int64_t rows, int64_t K, void* y, int dtype, void* stream);
 
 /* y[m, n] = sum_k a[m, k] w[n, k] + bias[n] of such rows: products exact, sums in fp32, rounded once.
@@ -588,6 +589,7 @@ int lcq_route(const void* logits, int dtype, int64_t T, int64_t E, int64_t ldl, 
  *          gate_up_lds (I + 64) up to 2^30
  *  gate_up_bias [E, 2 I], down_bias [E, N] of bias_dtype, or NULL;  y [T, N] of out_dtype;  K, I, N <= 65536
  *  workspace of lcq_mxfp4_moe_workspace_bytes(T, top, E, K, I, N, dtype), 16-byte aligned.
+ * Weights of 2^128 and more (4 and 6 with scale byte 253, 2 to 6 with 254) count as infinite.
  * An expert whose weight is 0 is not asked (its infinities and NaN do not reach y); a token without experts gives 0. */
 #define LCQ_ACT_SILU 0
 #define LCQ_ACT_GELU 1

@@ -373,7 +373,7 @@ struct MoeArgs {
   int T, top, N, I, Kp, Ip, activation;             // Kp, Ip: whole blocks
 };
 
-// eight codes times their scale, exactly
+// eight codes times their scale, exactly (what is 2^128 or more: an infinity)
 __device__ __forceinline__ bf16x8 decoded(int codes, float f) {
   const lcq_bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((uint32_t)codes, f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((uint32_t)codes, f, 1),
                    c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((uint32_t)codes, f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((uint32_t)codes, f, 3);

@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256) void dequant_kernel(const uint8_t* __restrict_
         for (int e = 0; e < 8; ++e) if (k + e < r.K) to[e] = v[e / 2][e % 2];
     } else {
       uint16_t* const to = (uint16_t*)y + row * r.K + k;
-      u32x4 w;                                      // (bf16 holds every one of these values)
+      u32x4 w;                                      // (bf16 holds every one of these values that fp32 holds)
       #pragma unroll
       for (int e = 0; e < 4; ++e) w[e] = BF == ROW_BF16 ? bf16_pack_rne(v[e].x, v[e].y) : f16_pack_rne(v[e].x, v[e].y);
       if (k + 8 <= r.K) put(to, w, r.past);

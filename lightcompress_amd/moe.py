@@ -100,8 +100,9 @@ def mxfp4_moe(x, router, gate_up, down, *, gate_up_bias=None, down_bias=None, ac
     times counts once, with the sum of the weights).  gate_up: Mxfp4 of [E, 2 I, K], the gates' rows and then the ups';  down: Mxfp4 of [E, N, I].
     gate_up_bias [E, 2 I], down_bias [E, N]: of one type.  activation 'silu' or 'gelu' (by erf).  -> [..., N] of x's type or `out_dtype`.
 
-    Activations are not quantized, sums and act(...) * (...) are fp32.  An expert whose weight is 0 is not asked; a token without experts gives 0.  This is for
-    few tokens: up to 128 at a time share a pass over the experts' bytes.  Operands with strides are copied (experts and their rows may lie apart)."""
+    Activations are not quantized, sums and act(...) * (...) are fp32.  An expert whose weight is 0 is not asked; a token without experts gives 0.
+    Weights of 2^128 and more (4 and 6 with scale byte 253, 2 to 6 with 254) count as infinite.  This is for few tokens: up to 128 at a time share a
+    pass over the experts' bytes.  Operands with strides are copied (experts and their rows may lie apart)."""
     shape = x.shape
     K = _cols(shape)
     code = _code(x.dtype)

@@ -93,7 +93,8 @@ def quantize_mxfp4(x):
 
 
 def dequantize_mxfp4(q, dtype=torch.bfloat16):
-    """What q stands for, [..., cols] of `dtype` (fp32 and bf16 hold every value, fp16 rounds or overflows)."""
+    """What q stands for, [..., cols] of `dtype` (fp32 and bf16 hold every value below 2^128, which quantize_mxfp4 does not pass; larger ones - 4 and
+    6 with scale byte 253, 2 to 6 with 254 - are infinite.  fp16 rounds or overflows)."""
     codes, scales, K = _parts(q, 'q')
     code = _code(dtype)
     if not _here(codes, scales):

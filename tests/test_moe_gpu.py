@@ -433,3 +433,23 @@ def test_route_of_scores_too_small_for_32_bits(dev, E, top, dtype, scoring, corr
         t = torch.randn(8, 32, generator=g, device=dev)
         y = mxfp4_moe(t, Router(x, top, scoring, True, c), gate_up, down)
         assert torch.equal(y, mxfp4_moe(t, route_tokens(Router(x, top, scoring, True, c)), gate_up, down)) and bool((y != 0).any(1).all())
+
+
+@pytest.mark.parametrize('dtype', [BF, HF, F32])
+def test_scales_at_the_top(dev, dtype):
+    """A weight of 2^128 and more counts as infinite, one just below it does not."""
+    E, K, I, N, T = 1, 64, 32, 32, 3
+    gate_up, down = picks(E, 2 * I, K, torch.cat([torch.arange(I), 32 + torch.arange(I)]).to(dev), dev), picks(E, N, I, torch.arange(N, device=dev), dev)
+    gate_up.scales[:, I:, 1] = 254                 # 1.0 there: 2^127
+    gate_up.codes[0, I + 5, 16 + 2] = 4 << 4       # 2.0: 2^128
+    gate_up.scales[0, I + 7, 1] = 253
+    gate_up.codes[0, I + 7, 16 + 3] = 6 << 4       # 4.0: 2^128
+    x = torch.full((T, K), 16.0, device=dev)
+    x[:, 32:] = 2.0 ** -20
+    one = Routing(torch.zeros(T, 1, dtype=torch.int32, device=dev), torch.ones(T, 1, device=dev))
+    y = mxfp4_moe(x.to(dtype), one, gate_up, down, out_dtype=F32)
+    assert not bool(torch.isfinite(y).any())       # (down has zeros for the two infinities, so that all channels are NaN)
+    gate_up.codes[0, I + 5, 16 + 2], gate_up.codes[0, I + 7, 16 + 3] = 2 << 4, 5 << 4         # 1.0: 2^127, and 3.0: 1.5 2^127
+    y = mxfp4_moe(x.to(dtype), one, gate_up, down, out_dtype=F32)
+    h = 16 / (1 + math.exp(-16)) * 2.0 ** 107 * torch.where(torch.arange(N, device=dev) == 7, 1.5, 1.0)
+    assert bool(((y.to(f64) - h).abs() <= 8 * U * h).all())

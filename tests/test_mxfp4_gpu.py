@@ -151,6 +151,33 @@ def test_more_values_than_31_bits(dev):
     assert torch.equal(y[8, -64:], dequantize_mxfp4(quantize_mxfp4(x[8, -64:]))) and int(torch.count_nonzero(y)) == int(torch.count_nonzero(y[8, -64:]))
 
 
+def test_scales_at_both_ends(dev):
+    """Every code with the least and the largest scales.  Above the largest fp32 number: 4 and 6 with byte 253, 2 to 6 with 254; those are infinite."""
+    low = torch.arange(16, dtype=torch.uint8, device=dev)
+    codes = (low | low.flip(0) << 4).expand(12, 16).contiguous()
+    scales = torch.tensor([0, 1, 2, 3, 7, 127, 250, 251, 252, 253, 254, 255], dtype=torch.uint8, device=dev)[:, None]
+    q = Mxfp4(codes, scales)
+    want = values(q)
+    for out in (F32, BF, HF):
+        y = dequantize_mxfp4(q, out)
+        torch.testing.assert_close(y, want.float().to(out), rtol=0, atol=0, equal_nan=True)
+    y = dequantize_mxfp4(q, F32)
+    assert [int(torch.isinf(r).sum()) for r in y] == [0] * 9 + [8, 16, 0] and bool(torch.isnan(y[11]).all())
+    assert torch.equal(y[:9].to(f64), want[:9])
+
+
+@pytest.mark.parametrize('M', [1, 20, 100, 300])
+def test_products_of_the_largest_scales(dev, M):
+    """The product takes all scales as they are: sums of tokens of 2^-110 or so with weights that fp32 does not hold are ordinary numbers."""
+    g = gpu_gen(M)
+    N, K = 130, 544
+    a, w = random_mx(M, K, g, dev, 15, 18), random_mx(N, K, g, dev, 252, 255)
+    va, vw = values(a), values(w)
+    assert bool((vw.abs() > torch.finfo(F32).max).any())
+    size = va.abs() @ vw.abs().t()
+    assert bool(((mxfp4_matmul(a, w, out_dtype=F32).to(f64) - va @ vw.t()).abs() <= (K / 64 + 16) * 2.0 ** -23 * size).all())
+
+
 # -- the product ----------------------------------------------------------------------------------------------------
 SIZES = [(1, 1, 1), (1, 64, 64), (1, 1000, 4096), (2, 17, 63), (3, 4096, 128), (7, 100, 2050), (8, 256, 1024), (15, 33, 80), (16, 4096, 4096),
          (17, 130, 272), (31, 64, 4112), (32, 512, 512), (33, 257, 1040), (48, 1024, 2048), (64, 64, 64), (65, 1001, 2047), (100, 300, 4096),
