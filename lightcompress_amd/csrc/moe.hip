@@ -7,7 +7,7 @@
 // The activations keep their precision.  A lane takes a block of a weight row, 16 bytes, and the conversion to bf16 applies its scale: that is
 // exact, so the products are those of the stored numbers.  bf16 tokens go into the matrix pipe as they are, fp32 ones as sums of three bf16 planes, and so
 // does h, which stays within the layer: 24 bits are three times eight, so nothing of an fp32 number is lost (above 2^-110).  fp16 tokens go as they are too, with the
-// weights' blocks as fp16, which is exact for scales of 2^-23 .. 2^13; stages with others take the tokens apart into two bf16 numbers (gate and up of 50 tokens, 2 of 8
+// weights' blocks as fp16, which is exact for scales of 2^-23 .. 2^13; stages with others, beside blocks of zeros, take the tokens apart into two bf16 numbers (gate and up of 50 tokens, 2 of 8
 // experts 4090 x 14336: 129 us, as two planes throughout 161; of 96 tokens 4096 x 4096 45 and 66).
 #include "mxfp4.h"
 #include <type_traits>
@@ -743,7 +743,19 @@ __global__ __launch_bounds__(256) void experts_kernel(MoeArgs g, int tiles, int 
             byte[u][i] = i * 4 + q < left ? byte[u][i] : 127u;
             other = other || byte[u][i] < LEAST_HALF || byte[u][i] > MOST_HALF;
           }
-        if (__builtin_expect(__builtin_amdgcn_ballot_w64(other) != 0, 0)) {
+        bool apart = false;
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(other) != 0, 0)) {  // (nor does it matter to blocks of zeros, as all are behind the last channel)
+          other = false;
+          #pragma unroll
+          for (int i = 0; i < 2; ++i)
+            #pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              if (byte[u][i] != 255 && (wv[u][i][0] | wv[u][i][1] | wv[u][i][2] | wv[u][i][3]) == 0) byte[u][i] = 127u;
+              other = other || byte[u][i] < LEAST_HALF || byte[u][i] > MOST_HALF;
+            }
+          apart = __builtin_amdgcn_ballot_w64(other) != 0;
+        }
+        if (__builtin_expect(apart, 0)) {
           #pragma unroll
           for (int i = 0; i < 2; ++i)
             #pragma unroll

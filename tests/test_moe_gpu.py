@@ -453,3 +453,22 @@ def test_scales_at_the_top(dev, dtype):
     y = mxfp4_moe(x.to(dtype), one, gate_up, down, out_dtype=F32)
     h = 16 / (1 + math.exp(-16)) * 2.0 ** 107 * torch.where(torch.arange(N, device=dev) == 7, 1.5, 1.0)
     assert bool(((y.to(f64) - h).abs() <= 8 * U * h).all())
+
+
+@pytest.mark.parametrize('T', [3, 20, 100])
+def test_zeros_change_no_rounding_of_fp16_tokens(dev, T):
+    """Channels behind the last one, and blocks of zeros with the least scale, as the quantizer makes them: the same sums, bit for bit, as with the rows there as zeros and
+    with a scale beside the others'."""
+    g = gpu_gen(T)
+    E, top, K, I, N = 4, 2, 1000, 70, 48
+    x = torch.randn(T, K, generator=g, device=dev).to(HF)
+    r = route_tokens(Router(torch.randn(T, E, generator=g, device=dev), top))
+    gate_up, down = experts_of(E, 2 * 128, K, g, dev), experts_of(E, N, 128, g, dev)
+    for q in (gate_up.codes[:, 70:128], gate_up.codes[:, 198:], down.codes[:, :, 35:], gate_up.codes[1, 3, 32:48], gate_up.codes[2, 60, :]):
+        q.zero_()
+    want = mxfp4_moe(x, r, gate_up, down, out_dtype=F32)
+    fewer = Mxfp4(torch.cat([gate_up.codes[:, :70], gate_up.codes[:, 128:198]], 1), torch.cat([gate_up.scales[:, :70], gate_up.scales[:, 128:198]], 1), K)
+    fewer.scales[1, 3, 2], fewer.scales[2, 60, :] = 0, 0
+    part = Mxfp4(down.codes[:, :, :48].contiguous(), down.scales[:, :, :3].contiguous(), I)
+    assert torch.equal(mxfp4_moe(x, r, fewer, part, out_dtype=F32), want)
+    check_layer(want, F32, x, r.experts, r.weights, gate_up, down, None, None, 'silu')
