@@ -472,3 +472,21 @@ def test_zeros_change_no_rounding_of_fp16_tokens(dev, T):
     part = Mxfp4(down.codes[:, :, :48].contiguous(), down.scales[:, :, :3].contiguous(), I)
     assert torch.equal(mxfp4_moe(x, r, fewer, part, out_dtype=F32), want)
     check_layer(want, F32, x, r.experts, r.weights, gate_up, down, None, None, 'silu')
+
+
+def test_experts_behind_4_gigabytes(dev):
+    """Codes of the last experts lie behind 2^32 bytes, of gate and up and of down."""
+    E, K, I, N, T = 600, 4096, 2048, 8192, 3
+    g = gpu_gen(15)
+    gate_up, down = experts_of(E, 2 * I, K, g, dev), experts_of(E, N, I, g, dev)
+    for q in (gate_up, down):
+        assert q.codes[-1].data_ptr() - q.codes.data_ptr() > 2 ** 32
+    x = torch.randn(T, K, generator=g, device=dev).to(BF)
+    experts = torch.tensor([[599, 0], [598, 599], [1, 300]], dtype=torch.int32, device=dev)
+    weights = torch.rand(T, 2, generator=g, device=dev)
+    got = mxfp4_moe(x, Routing(experts, weights), gate_up, down)
+    used = [0, 1, 300, 598, 599]
+    part = lambda q: Mxfp4(q.codes[used], q.scales[used], q.cols)  # noqa: E731
+    renamed = torch.tensor([[4, 0], [3, 4], [1, 2]], dtype=torch.int32, device=dev)
+    check_layer(got, BF, x, renamed, weights, part(gate_up), part(down), None, None, 'silu')
+    assert torch.equal(mxfp4_moe(x, Routing(renamed, weights), part(gate_up), part(down)), got)
