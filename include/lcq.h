@@ -542,11 +542,11 @@ int lcq_token_logprobs_of(const void* logits, int dtype, int64_t B, int64_t S, i
 
 /* The codes of rows of values.  A block's scale is 2^(floor(log2 max|x|) - 2), at least 2^-127; codes are the nearest, ties to the even one,
  * saturated at 6.  A block with an infinity or a NaN gets scale 255 and codes 0.
- *  x       [rows, K] of `dtype`, rows `ldx` elements apart
+ *  x       [rows, K] of `dtype`, rows `ldx` elements apart;  rows * 32 B <= 2^36, rows <= 2^30 - 64 unless they are whole blocks without gaps
  *  codes   [rows, 16 B], 4-byte aligned;  scales [rows, B], rows `lds` bytes apart: output */
 int lcq_mxfp4_quant(const void* x, int dtype, int64_t rows, int64_t K, int64_t ldx, uint8_t* codes, uint8_t* scales, int64_t lds, void* stream);
 
-/* What codes (rows ldc bytes apart, a multiple of 4) and scales (rows lds apart) stand for: y [rows, K] of `dtype`, rounded once. fp32 and bf16 hold every value but
+/* What codes (rows ldc bytes apart, a multiple of 4) and scales (rows lds apart) stand for: y [rows, K] of `dtype`, as many rows, rounded once. fp32 and bf16 hold every value but
  * those of 2^128 and more (4 and 6 with scale byte 253, 2 to 6 with 254; lcq_mxfp4_quant makes none above 252), which become infinities. */
 int lcq_mxfp4_dequant(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, int64_t rows, int64_t K, void* y, int dtype, void* stream);
 

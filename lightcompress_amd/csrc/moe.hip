@@ -995,7 +995,7 @@ int lcq_mxfp4_moe(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, c
   if (K > 65536 || I > 65536 || N > 65536) return LCQ_ESIZE;
   const int64_t B = (K + 31) / 32, BI = (I + 31) / 32, Kp = 32 * B, Ip = 32 * BI;
   if (gate_up_ld < 16 * B || gate_up_lds < B || down_ld < 16 * BI || down_lds < BI) return LCQ_EINVAL;
-  if (gate_up_ld > 1 << 22 || down_ld > 1 << 22 || gate_up_lds * (I + 64) > 1 << 30 || down_lds > 1 << 22) return LCQ_ESIZE;
+  if (gate_up_ld > 1 << 22 || down_ld > 1 << 22 || gate_up_lds > (1 << 30) / (I + 64) || down_lds > 1 << 22) return LCQ_ESIZE;
   if ((uintptr_t)gate_up % 16 || gate_up_ld % 16 || gate_up_lde % 16 || (uintptr_t)down % 16 || down_ld % 16 || down_lde % 16) return LCQ_EALIGN;
   if (!workspace) return LCQ_EWORKSPACE;
   if ((uintptr_t)workspace % 16) return LCQ_EALIGN;

@@ -127,3 +127,13 @@ def test_the_entries_of_experts_refuse_before_a_launch():
     need = L.lib().lcq_mxfp4_moe_workspace_bytes
     assert need(0, 2, 4, 64, 40, 48, 1) == need(2, 33, 64, 64, 40, 48, 1) == need(2, 2, 4, 65537, 40, 48, 1) == need(2, 2, 4, 64, 40, 48, 3) == 0
     assert need(2, 2, 4, 64, 40, 48, 1) > 0 and need(128, 32, 32, 32, 65536, 4, 0) < 2 ** 31 + 2 ** 28 and need(1 << 25, 2, 4, 64, 40, 48, 1) == need(128, 2, 4, 64, 40, 48, 1)
+
+
+def test_sizes_whose_products_pass_64_bits_are_refused():
+    """Distances that a multiplication would wrap, and the rows that a quantization takes at most."""
+    layer = lambda gsd: L.lib().lcq_mxfp4_moe(P, 1, 2, 64, 64, P, 0, 4, 0, None, 1.0, None, None, 4, 2, P, 2560, 32, P, 160, gsd, None, P, 1536, 32, P, 96, 2, None, 0,  # noqa: E731
+                                              40, 48, 0, P, 1, P, None)
+    assert {layer(gsd) for gsd in ((1 << 30) // 104 + 1, 1 << 60, 1 << 61, 1 << 62, (1 << 63) - 1)} == {ESIZE}
+    for rows, K in ((1 << 30, 1), (1 << 30, 33), (1 << 32, 32), ((1 << 36) // 64 + 1, 64)):
+        assert L.lib().lcq_mxfp4_quant(P, 0, rows, K, K, P, P, -(-K // 32) + 1, None) == ESIZE
+        assert L.lib().lcq_mxfp4_dequant(P, 1 << 20, P, 1 << 20, rows, K, P, 0, None) == ESIZE
