@@ -490,3 +490,16 @@ def test_experts_behind_4_gigabytes(dev):
     renamed = torch.tensor([[4, 0], [3, 4], [1, 2]], dtype=torch.int32, device=dev)
     check_layer(got, BF, x, renamed, weights, part(gate_up), part(down), None, None, 'silu')
     assert torch.equal(mxfp4_moe(x, Routing(renamed, weights), part(gate_up), part(down)), got)
+
+
+@pytest.mark.parametrize('dtype', [BF, F32])
+def test_tokens_at_the_seam_of_two_passes(dev, dtype):
+    """32 choices, 65536 channels in three planes of 16 bits: 85 tokens have 2^30 bytes between the two products, so 128 take two passes."""
+    E, K, I, N, T = 32, 32, 65536, 4, 128
+    g = gpu_gen(16)
+    gate_up, down = experts_of(E, 2 * I, K, g, dev), experts_of(E, N, I, g, dev)
+    x = torch.randn(T, K, generator=g, device=dev).to(dtype)
+    r = Routing(torch.arange(E, dtype=torch.int32, device=dev).repeat(T, 1), torch.rand(T, E, generator=g, device=dev))
+    got = mxfp4_moe(x, r, gate_up, down)
+    some = [83, 84, 85, 86, 127]
+    check_layer(got[some], dtype, x[some], r.experts[some], r.weights[some], gate_up, down, None, None, 'silu')
