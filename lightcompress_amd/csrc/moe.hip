@@ -1,8 +1,8 @@
 // A mixture-of-experts layer for a few tokens, on experts of microscaled 4-bit numbers:
 //   y[t] = sum_s w[t, s] (down_e h + down_bias_e),   h = act(gate_e x[t] + b) * (up_e x[t] + b),   e = experts[t, s]
 // Tokens that chose the same expert share one pass over its bytes, which is what bounds the layer: a plan (tokens by expert), gate and up, down, the
-// weighted sum, a kernel each, as each needs all of the one in front.  7168 x 2048, 8 of 256 experts: 1 token 6.2 + 26.1 + 13.7 + 3.9 us (gate and up
-// 3 of launch, 2.9 to the first stage, 18.2 at the memory's rate, 1.2 of results), 16 tokens 10.5 + 246 + 133 + 5.6 (6.3 TB/s).
+// weighted sum, a kernel each, as each needs all of the one in front.  7168 x 2048, 8 of 256 experts: 1 token 6.5 + 27.6 + 14.4 + 3.8 us (gate and up
+// 3 of launch, 2.9 to the first stage, 18.2 at the memory's rate, 1.2 of results), 16 tokens 10.9 + 250 + 140 + 5.2 (6.2 TB/s in a row).
 //
 // The activations keep their precision.  A lane takes a block of a weight row, 16 bytes, and the conversion to bf16 applies its scale: that is
 // exact, so the products are those of the stored numbers.  bf16 tokens go into the matrix pipe as they are, fp32 ones as sums of three bf16 planes, and so
@@ -201,7 +201,7 @@ __device__ __forceinline__ void route_token(const RouterArgs& r, int64_t t, int&
   weight *= r.scale;
 }
 
-// A wave per token, as much as fits a CU on its way: 64 tokens of 256 experts with a correction 5.1 us, a launch and the chain of one token; 16384 of 64 experts 8.1 us.
+// A wave per token, as much as fits a CU on its way: 64 tokens of 256 experts with a correction 5.2 us, a launch and the chain of one token; 16384 of 64 experts 8.4 us.
 template <int NL>
 __global__ __launch_bounds__(256) void route_kernel(RouterArgs r, int64_t T, int* __restrict__ experts, float* __restrict__ weights) {
   const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -242,7 +242,7 @@ __device__ __forceinline__ void planes_of(float v, uint16_t* out) {
 }
 
 // Workgroup 0 plans the pass; the others lay the tokens out as planes [T, planes, Kp] where they are not that already.  One workgroup, as every place depends on
-// all choices: 6.2 us with the routing of 1 token of 256 experts, 10.5 of 16 tokens (their choices are a chain in each wave), 5.2 behind the router's kernel.
+// all choices: 6.5 us with the routing of 1 token of 256 experts, 10.9 of 16 tokens (their choices are a chain in each wave), 5.2 behind the router's kernel.
 template <int NL>
 __global__ __launch_bounds__(1024) void plan_kernel(RouterArgs r, const int* __restrict__ given, const float* __restrict__ given_weights, int T,
                                                     Operand o, int size, Plan* __restrict__ plan) {
@@ -897,8 +897,8 @@ struct Cut {
     P = dtype == LCQ_F32 ? PLANES : 1;
     const int64_t slots = T * top;
     // Slots of a group: few columns cost less in every stage, a second group of an expert reads its bytes again.  The whole layer in us with 4 / 16 / 32:
-    //   4 tokens, 6 of 64 experts 40 / 48 / 55    16 tokens, 8 of 256 378 / 461 / 617    64 tokens, 4 of 32 159 / 94 / 123    64 tokens, 2 of 8 164 / 95 / 94
-    //   96 tokens, 2 of 8 208 / 112 / 97
+    //   4 tokens, 6 of 64 experts 2048 x 1408 41 / 51 / 54    16 tokens, 8 of 256 7168 x 2048 379 / 516 / 580    64 tokens, 4 of 32 4096 x 1408 152 / 100 / 107
+    //   64 tokens, 2 of 8 4096 x 4096 161 / 104 / 100    96 tokens 208 / 124 / 111
     size = T <= 4 || slots <= E ? 4 : P > 1 || T <= 16 || slots <= 18 * E ? 16 : 32;
     const auto groups_of = [&](int size) { return least(slots, least(E, slots) + slots / size); };
     groups = groups_of(size);
@@ -910,8 +910,8 @@ struct Cut {
     up_parts = 1;
     while (3 * up_stages > 2 * groups * up_tiles * up_parts * up_parts && up_stages / (2 * up_parts) >= 3) up_parts *= 2;
     down_tiles = (int)((N + 127) / 128);
-    // Runs of down: two workgroups per CU (64 tokens, 4 of 32 experts with 1 / 2 / 4 per CU 91 / 94 / 101, 16 tokens, 8 of 256 410 / 378 / 385); K in parts
-    // where there are too few groups for them (1 token, 2 of 8 experts 4096 x 14336 in 1 / 2 / 4 / 8 parts 73 / 59 / 53 / 53; 8 of 256 52 / 52 / 54 / 60).
+    // Runs of down: two workgroups per CU (64 tokens, 4 of 32 experts with 1 / 2 / 4 per CU 99 / 100 / 109, 16 tokens, 8 of 256 417 / 379 / 386); K in parts
+    // where there are too few groups for them (1 token, 2 of 8 experts 4096 x 14336 in 1 / 2 / 4 / 8 parts 77 / 60 / 54 / 54; 8 of 256 53 / 53 / 55 / 61).
     int64_t want = 512 / down_tiles;
     if (want < 1) want = 1;
     down_parts = 1;

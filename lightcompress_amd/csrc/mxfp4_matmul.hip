@@ -52,7 +52,7 @@ __device__ __forceinline__ i32x8 wide(i32x4 v) { return __builtin_shufflevector(
 // Tiles of 256 x 256 are bound by the chip's power: 8192 x 14336 x 4096 takes 251 us (3.8 PFLOP/s) with the products at 1.55 GHz, 192 on zeros at 2.35.  A
 // round of tiles is 3.4 us of first loads, 25 of products (38 900 clocks, the pipe alone 32 800), 4.5 of outputs.  With nothing loaded behind the first stages the products
 // run at 1.68 GHz, without reads of LDS either at 1.92; loading the next tile's first stages before the outputs leave, or whole lines in two stages of 128
-// bytes, took as long.  The others are bound by the loads on their way (a round of 224 tiles of 128 x 128 with K = 4096 17 us, 1.9 TB/s of weights, of 64 x 64
+// bytes, took as long.  The others are bound by the loads on their way (a round of 224 tiles of 128 x 128 with K = 4096 18 us, 1.7 TB/s of weights from memory, 14.7 from the caches, of 64 x 64
 // 10 us, 3 TB/s).
 constexpr int ROW_SUM = 3;                          // an output type: the sums of a part of K as they are
 constexpr int PERIOD = 256;                         // bytes of a row between scale loads
